@@ -167,6 +167,38 @@ CAST_MAX_JOBS = 32
 _SIGS["fb_cast_bf16"] = (_I, [ctypes.POINTER(CastJob), _I, _P])
 _SIGS["fb_fill_normal_bf16"] = (_I, [_P, _I64, _I, _I64, _U64, _P])
 
+_SIGS["fb_layer_norm_fwd"] = (_I, [_I, _P, _I64, _P, _I64, _P, _P, _I, _F, _P, _I64, _P, _I64, _P, _P, _I64, _I, _P])
+_SIGS["fb_layer_norm_bwd_ws_bytes"] = (_SZ, [_I64, _I])
+_SIGS["fb_layer_norm_bwd"] = (_I, [_I, _P, _I64, _P, _I64, _P, _I, _P, _P, _P, _I64, _P, _I64, _P, _P, _I, _I64, _I,
+                                   _P, _SZ, _P])
+
+F32, BF16 = 0, 1
+ACTS = {"silu": 0, "gelu": 1, "relu": 2}
+
+
+def _fields(*specs):
+    """Structure fields from "name name:type ..." groups; pointers by default."""
+    kinds = {"i": ctypes.c_int, "q": ctypes.c_int64, "p": ctypes.c_void_p}
+    return [(n.partition(":")[0], kinds[n.partition(":")[2] or "p"]) for s in specs for n in s.split()]
+
+
+class GatedFfn(ctypes.Structure):
+    """fb_gated_ffn (include/fast_b200.h)."""
+    _fields_ = _fields("type:i act:i grad_type:i accumulate:i n:q D:i F:i", "x ldx:q w_gate ld_gate:q",
+                       "w_up ld_up:q w_down ld_down:q y ldy:q", "dy lddy:q dx lddx:q dw_gate ldd_gate:q",
+                       "dw_up ldd_up:q dw_down ldd_down:q")
+
+
+class SoftmaxXent(ctypes.Structure):
+    """fb_softmax_xent (include/fast_b200.h)."""
+    _fields_ = _fields("type:i grad_type:i accumulate:i D:i n:q V:q", "h ldh:q w ldw:q target loss lse",
+                       "dloss dh lddh:q dw lddw:q")
+
+
+for _n, _s in (("gated_ffn", GatedFfn), ("softmax_xent", SoftmaxXent)):
+    _SIGS["fb_%s_ws_bytes" % _n] = (_SZ, [ctypes.POINTER(_s), _I])
+    _SIGS["fb_%s_fwd" % _n] = _SIGS["fb_%s_bwd" % _n] = (_I, [ctypes.POINTER(_s), _P, _SZ, _P])
+
 for _name, (_res, _args) in _SIGS.items():
     _fn = getattr(lib, _name)
     _fn.restype = _res

@@ -585,6 +585,82 @@ int fb_mailbox_update_neighbors(const int32_t *nodes, const int32_t *row, const 
                                 float *mailbox_ts, int32_t *next_pos, int mailbox_size, unsigned long long *last,
                                 uint32_t *gen, uint32_t *done, cudaStream_t stream);
 
+/* ------------------------------------------------------------------------- */
+/* Node-ranking head: layer norm, gated feed-forward block and softmax cross  */
+/* entropy over every candidate node.  No counterpart in the reference, whose */
+/* EdgePredictor (layers.py:31-50) scores one negative per edge.              */
+/* ------------------------------------------------------------------------- */
+/* Element types of the rows an operator takes. */
+enum { FB_F32 = 0, FB_BF16 = 1 };
+/* Layer norm over rows [n, D] (leading dimensions in elements, any alignment):
+ *   s = x + res, kept in `sum` in the rows' type (res NULL: s = x, no sum)
+ *   y = (s - mean) rstd gamma + beta,  rstd = 1 / sqrt(var + eps)
+ * mean, rstd [n] (fp32, each may be NULL) are what the backward takes.  gamma,
+ * beta (may be NULL) are fp32 or of the rows' type (param_type).  Statistics
+ * are fp32.  D <= 16384. */
+int fb_layer_norm_fwd(int type, const void *x, int64_t ldx, const void *res, int64_t ldr, const void *gamma,
+                      const void *beta, int param_type, float eps, void *sum, int64_t lds, void *y, int64_t ldy,
+                      float *mean, float *rstd, int64_t n, int D, cudaStream_t stream);
+/* Backward from dy and the normalised rows x (`sum` when there was a residual):
+ * dx (+ ds, the gradient that reaches the sum on its own; may be NULL), the
+ * gradient of x and of res alike; dgamma = sum dy xhat, dbeta = sum dy (each
+ * may be NULL; += when accumulate, fp32 only).  Deterministic.
+ * ws: fb_layer_norm_bwd_ws_bytes(n, D) bytes. */
+size_t fb_layer_norm_bwd_ws_bytes(int64_t n, int D);
+int fb_layer_norm_bwd(int type, const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *gamma,
+                      int param_type, const float *mean, const float *rstd, const void *ds, int64_t ldds, void *dx,
+                      int64_t lddx, void *dgamma, void *dbeta, int accumulate, int64_t n, int D, void *ws,
+                      size_t ws_bytes, cudaStream_t stream);
+/* Gated feed-forward block  y = (act(x Wg^T) * (x Wu^T)) Wd^T  over rows x
+ * [n, D]; w_gate, w_up [F, D], w_down [D, F] (torch.nn.Linear layout), all of
+ * one type; products accumulate in fp32.  The backward takes dy and x alone (it
+ * recomputes what the activation saw) and writes dx (rows' type) and the weight
+ * gradients (grad_type: fp32 or the rows' type; += when accumulate, fp32 only);
+ * any of the four may be NULL.  GELU is the erf form.  Deterministic.
+ * ws: fb_gated_ffn_ws_bytes(args, backward) bytes. */
+enum { FB_ACT_SILU = 0, FB_ACT_GELU = 1, FB_ACT_RELU = 2 };
+typedef struct fb_gated_ffn {
+  int type, act, grad_type, accumulate;
+  int64_t n;
+  int D, F;
+  const void *x; int64_t ldx;
+  const void *w_gate; int64_t ld_gate;
+  const void *w_up; int64_t ld_up;
+  const void *w_down; int64_t ld_down;
+  void *y; int64_t ldy;                    /* forward */
+  const void *dy; int64_t lddy;            /* backward */
+  void *dx; int64_t lddx;
+  void *dw_gate; int64_t ldd_gate;
+  void *dw_up; int64_t ldd_up;
+  void *dw_down; int64_t ldd_down;
+} fb_gated_ffn;
+size_t fb_gated_ffn_ws_bytes(const fb_gated_ffn *args, int backward);
+int fb_gated_ffn_fwd(const fb_gated_ffn *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+int fb_gated_ffn_bwd(const fb_gated_ffn *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+/* Softmax cross entropy of rows h [n, D] over the V rows of a table w [V, D]
+ * (logits h w^T, never kept), one type, fp32 accumulation:
+ *   lse[i] = log sum_v exp(l_iv),  loss[i] = lse[i] - l_i,target[i]
+ * A negative target holds its row out: loss 0 and no gradient.  A target >= V
+ * gives a NaN loss and no gradient.  Backward, from lse and dloss [n] (fp32):
+ *   G_iv = dloss[i] (exp(l_iv - lse[i]) - [v == target[i]])
+ *   dh = G w (rows' type),  dw = G^T h (grad_type; += when accumulate, fp32 only)
+ * dh or dw may be NULL.  Deterministic.
+ * ws: fb_softmax_xent_ws_bytes(args, backward) bytes. */
+typedef struct fb_softmax_xent {
+  int type, grad_type, accumulate, D;
+  int64_t n, V;
+  const void *h; int64_t ldh;
+  const void *w; int64_t ldw;
+  const int64_t *target;
+  float *loss, *lse;                       /* forward: written; backward: lse read */
+  const float *dloss;                      /* backward */
+  void *dh; int64_t lddh;
+  void *dw; int64_t lddw;
+} fb_softmax_xent;
+size_t fb_softmax_xent_ws_bytes(const fb_softmax_xent *args, int backward);
+int fb_softmax_xent_fwd(const fb_softmax_xent *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+int fb_softmax_xent_bwd(const fb_softmax_xent *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
