@@ -3,18 +3,24 @@
 //   dh = dy Wd, dg = dh u act'(g), du = dh act(g)
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 // Only x is kept between the two: the backward recomputes g and u.
-#include <cuda_bf16.h>
-#include <algorithm>
-#include "head.cuh"
+//
+// bf16: two launches forward, four backward (plus the sums of split
+// reductions), each a product on SM pairs (pair_gemm.cuh).  The first of each
+// direction computes g and u side by side in one tile -- one CTA of the pair
+// stages Wg, the other Wu -- and for the backward dh beside them, and applies
+// the activation to the fp32 accumulators: h, dg, du are rounded once, and g,
+// u, dh never reach memory.  fp32: the grouped 3xTF32 products with the
+// activation between them.
+#include "pair_gemm.cuh"
 
 namespace {
 
 using namespace fbh;
 
-enum : int { kSilu = FB_ACT_SILU, kGelu = FB_ACT_GELU, kRelu = FB_ACT_RELU };
+constexpr int kSilu = FB_ACT_SILU, kGelu = FB_ACT_GELU;
 
 // act(g) and act'(g)
-template <int ACT> __device__ __forceinline__ float2 act2(float g) {
+template <int ACT> __device__ __forceinline__ float2 act_exact(float g) {
   if (ACT == kSilu) {
     const float s = 1.f / (1.f + expf(-g));
     return make_float2(g * s, s * (1.f + g * (1.f - s)));
@@ -26,47 +32,26 @@ template <int ACT> __device__ __forceinline__ float2 act2(float g) {
   return make_float2(fmaxf(g, 0.f), g > 0.f ? 1.f : 0.f);
 }
 
-__device__ __forceinline__ void put(float *p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
-
-// h = act(g) u over n elements (pitches alike, padding included).
-template <int ACT, typename T> __global__ void k_glu_fwd(const float *g, const float *u, T *h, int64_t n) {
+// h = act(g) u over n elements (pitches alike, padding included), in g's place.
+template <int ACT> __global__ void k_glu_fwd(float *g, const float *u, int64_t n) {
   fb::pdl_enter();
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    put(h + i, act2<ACT>(g[i]).x * u[i]);
+    g[i] = act_exact<ACT>(g[i]).x * u[i];
 }
 
-// (dg, du, h) from (g, u, dh); the outputs may be the inputs.
-template <int ACT, typename T>
-__global__ void k_glu_bwd(const float *g, const float *u, const float *dh, T *dg, T *du, T *h, int64_t n) {
+// (dg, du, h) in the places of (g, u, dh).
+template <int ACT> __global__ void k_glu_bwd(float *g, float *u, float *dh, int64_t n) {
   fb::pdl_enter();
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const float gv = g[i], uv = u[i], d = dh[i];
-    const float2 a = act2<ACT>(gv);
-    put(dg + i, d * uv * a.y);
-    put(du + i, d * a.x);
-    put(h + i, a.x * uv);
+    const float uv = u[i], d = dh[i];
+    const float2 a = act_exact<ACT>(g[i]);
+    g[i] = d * uv * a.y;
+    u[i] = d * a.x;
+    dh[i] = a.x * uv;
   }
 }
 
 unsigned blocks_for(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, 148 * 16)); }
-
-template <typename T> int glu_fwd(Call &c, int act, const float *g, const float *u, T *h, int64_t n) {
-  if (c.dry) return FB_OK;
-  auto k = act == kSilu ? k_glu_fwd<kSilu, T> : (act == kGelu ? k_glu_fwd<kGelu, T> : k_glu_fwd<kRelu, T>);
-  FB_TRY_CUDA(fb::launch(k, blocks_for(n), 256, 0, c.stream, g, u, h, n));
-  FB_LAUNCHED("k_glu_fwd");
-  return FB_OK;
-}
-
-template <typename T>
-int glu_bwd(Call &c, int act, const float *g, const float *u, const float *dh, T *dg, T *du, T *h, int64_t n) {
-  if (c.dry) return FB_OK;
-  auto k = act == kSilu ? k_glu_bwd<kSilu, T> : (act == kGelu ? k_glu_bwd<kGelu, T> : k_glu_bwd<kRelu, T>);
-  FB_TRY_CUDA(fb::launch(k, blocks_for(n), 256, 0, c.stream, g, u, dh, dg, du, h, n));
-  FB_LAUNCHED("k_glu_bwd");
-  return FB_OK;
-}
 
 int check(const fb_gated_ffn *a, bool bwd) {
   if (!a) return fb::set_error(FB_ERR_ARG, "gated_ffn: null arguments");
@@ -92,78 +77,110 @@ int check(const fb_gated_ffn *a, bool bwd) {
   return FB_OK;
 }
 
-template <typename T> int forward(Call &c, const fb_gated_ffn &a) {
-  const int64_t N = a.n, Fp = round_up(a.F, 8);
-  Mat x, wg, wu, wd;
-  FBH_TRY(aligned(c, a.type, Mat{a.x, a.ldx}, N, a.D, &x));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_gate, a.ld_gate}, a.F, a.D, &wg));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_up, a.ld_up}, a.F, a.D, &wu));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_down, a.ld_down}, a.D, a.F, &wd));
+int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
+  const int64_t N = a.n, Fp = round_up(a.F, 4);
   FBH_TAKE(g, c, float, N * Fp);
   FBH_TAKE(u, c, float, N * Fp);
-  T *h = reinterpret_cast<T *>(g);
-  if (a.type != FB_F32) {
-    FBH_TAKE(hb, c, T, N * Fp);
-    h = hb;
+  FBH_TRY(product(c, FB_GEMM_NT, x, wg, g, Fp, N, a.F, a.D, 0));
+  FBH_TRY(product(c, FB_GEMM_NT, x, wu, u, Fp, N, a.F, a.D, 0));
+  if (!c.dry) {
+    auto k = a.act == kSilu ? k_glu_fwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_fwd<FB_ACT_GELU> : k_glu_fwd<FB_ACT_RELU>);
+    FB_TRY_CUDA(fb::launch(k, blocks_for(N * Fp), 256, 0, c.stream, g, (const float *)u, N * Fp));
+    FB_LAUNCHED("k_glu_fwd");
   }
-  FBH_TRY(product(c, a.type, FB_GEMM_NT, x, wg, g, Fp, N, a.F, a.D, 0));
-  FBH_TRY(product(c, a.type, FB_GEMM_NT, x, wu, u, Fp, N, a.F, a.D, 0));
-  FBH_TRY(glu_fwd<T>(c, a.act, g, u, h, N * Fp));
-  if (a.type == FB_F32)
-    return product(c, a.type, FB_GEMM_NT, Mat{h, Fp}, wd, static_cast<float *>(a.y), a.ldy, N, a.D, a.F, 0);
-  FBH_TAKE(y, c, float, N * a.D);
-  FBH_TRY(product(c, a.type, FB_GEMM_NT, Mat{h, Fp}, wd, y, a.D, N, a.D, a.F, 0));
-  return store_rows(c, y, a.D, a.y, a.ldy, a.type, N, a.D, 0);
+  return product(c, FB_GEMM_NT, Mat{g, Fp}, wd, static_cast<float *>(a.y), a.ldy, N, a.D, a.F, 0);
 }
 
-// A weight gradient G^T X ([rows_out, cols]) in grad_type.
-int weight_grad(Call &c, const fb_gated_ffn &a, const Mat &G, const Mat &X, void *out, int64_t ldo, int rows_out,
-                int cols) {
-  if (!out) return FB_OK;
-  if (a.grad_type == FB_F32)
-    return product(c, a.type, FB_GEMM_TN, G, X, static_cast<float *>(out), ldo, a.n, rows_out, cols, a.accumulate);
-  const size_t mark = c.off;
-  FBH_TAKE(t, c, float, (int64_t)rows_out * cols);
-  FBH_TRY(product(c, a.type, FB_GEMM_TN, G, X, t, cols, a.n, rows_out, cols, 0));
-  FBH_TRY(store_rows(c, t, cols, out, ldo, a.grad_type, rows_out, cols, 0));
-  c.off = mark;
-  return FB_OK;
-}
-
-template <typename T> int backward(Call &c, const fb_gated_ffn &a) {
-  const int64_t N = a.n, Fp = round_up(a.F, 8);
-  Mat x, wg, wu, wd, dy;
-  FBH_TRY(aligned(c, a.type, Mat{a.x, a.ldx}, N, a.D, &x));
-  FBH_TRY(aligned(c, a.type, Mat{a.dy, a.lddy}, N, a.D, &dy));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_gate, a.ld_gate}, a.F, a.D, &wg));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_up, a.ld_up}, a.F, a.D, &wu));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_down, a.ld_down}, a.D, a.F, &wd));
-  FBH_TAKE(g, c, float, N * Fp);
-  FBH_TAKE(u, c, float, N * Fp);
-  FBH_TAKE(dh, c, float, N * Fp);
-  T *dg = reinterpret_cast<T *>(g), *du = reinterpret_cast<T *>(u), *h = reinterpret_cast<T *>(dh);
-  if (a.type != FB_F32) {
-    FBH_TAKE(b, c, T, 3 * N * Fp);
-    dg = b, du = b + N * Fp, h = b + 2 * N * Fp;
+int backward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu,
+                 const Mat &wd) {
+  const int64_t N = a.n, Fp = round_up(a.F, 4);
+  FBH_TAKE(g, c, float, N * Fp);             // then dg
+  FBH_TAKE(u, c, float, N * Fp);             // then du
+  FBH_TAKE(d, c, float, N * Fp);             // dh, then h
+  FBH_TRY(product(c, FB_GEMM_NT, x, wg, g, Fp, N, a.F, a.D, 0));
+  FBH_TRY(product(c, FB_GEMM_NT, x, wu, u, Fp, N, a.F, a.D, 0));
+  FBH_TRY(product(c, FB_GEMM_NN, dy, wd, d, Fp, N, a.F, a.D, 0));
+  if (!c.dry) {
+    auto k = a.act == kSilu ? k_glu_bwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_bwd<FB_ACT_GELU> : k_glu_bwd<FB_ACT_RELU>);
+    FB_TRY_CUDA(fb::launch(k, blocks_for(N * Fp), 256, 0, c.stream, g, u, d, N * Fp));
+    FB_LAUNCHED("k_glu_bwd");
   }
-  FBH_TRY(product(c, a.type, FB_GEMM_NT, x, wg, g, Fp, N, a.F, a.D, 0));
-  FBH_TRY(product(c, a.type, FB_GEMM_NT, x, wu, u, Fp, N, a.F, a.D, 0));
-  FBH_TRY(product(c, a.type, FB_GEMM_NN, dy, wd, dh, Fp, N, a.F, a.D, 0));
-  FBH_TRY(glu_bwd<T>(c, a.act, g, u, dh, dg, du, h, N * Fp));
   if (a.dx) {
     float *dx = static_cast<float *>(a.dx);
-    int64_t ld = a.lddx;
-    if (a.type != FB_F32) {
-      FBH_TAKE(t, c, float, N * a.D);
-      dx = t, ld = a.D;
-    }
-    FBH_TRY(product(c, a.type, FB_GEMM_NN, Mat{dg, Fp}, wg, dx, ld, N, a.D, a.F, 0));
-    FBH_TRY(product(c, a.type, FB_GEMM_NN, Mat{du, Fp}, wu, dx, ld, N, a.D, a.F, 1));
-    if (a.type != FB_F32) FBH_TRY(store_rows(c, dx, ld, a.dx, a.lddx, a.type, N, a.D, 0));
+    FBH_TRY(product(c, FB_GEMM_NN, Mat{g, Fp}, wg, dx, a.lddx, N, a.D, a.F, 0));
+    FBH_TRY(product(c, FB_GEMM_NN, Mat{u, Fp}, wu, dx, a.lddx, N, a.D, a.F, 1));
   }
-  FBH_TRY(weight_grad(c, a, Mat{dg, Fp}, x, a.dw_gate, a.ldd_gate, a.F, a.D));
-  FBH_TRY(weight_grad(c, a, Mat{du, Fp}, x, a.dw_up, a.ldd_up, a.F, a.D));
-  return weight_grad(c, a, dy, Mat{h, Fp}, a.dw_down, a.ldd_down, a.D, a.F);
+  auto grad = [&](const Mat &G, const Mat &X, void *o, int64_t ld, int rows, int cols) {
+    return o ? product(c, FB_GEMM_TN, G, X, static_cast<float *>(o), ld, N, rows, cols, a.accumulate) : FB_OK;
+  };
+  FBH_TRY(grad(Mat{g, Fp}, x, a.dw_gate, a.ldd_gate, a.F, a.D));
+  FBH_TRY(grad(Mat{u, Fp}, x, a.dw_up, a.ldd_up, a.F, a.D));
+  return grad(dy, Mat{d, Fp}, a.dw_down, a.ldd_down, a.D, a.F);
+}
+
+// g and u (and dh) of every tile, the activation in the epilogue: h [N, Fp],
+// and for the backward dgu [N, 2 Fp] = [dg | du].  Fp = F rounded up to 64;
+// the padding columns are zeros (weight rows past F read as zeros).
+template <int EPI>
+int glu(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu, const Mat &wd,
+        __nv_bfloat16 *h, __nv_bfloat16 *dgu, int64_t Fp) {
+  using namespace fbpair;
+  if (c.dry) return FB_OK;
+  PairArgs p;
+  std::memset(&p, 0, sizeof(p));
+  p.phases = EPI == kGluBwd ? 2 : 1;
+  p.probs = p.splits = 1;
+  p.kb[0] = p.kb[1] = p.kper = tiles_of(a.D, BK);
+  p.mt = tiles_of(a.n, 256);
+  p.nt = tiles_of(Fp, 128);
+  p.M = (int)a.n;
+  p.N = (int)Fp;
+  p.act = a.act;
+  p.has_tc = 1;
+  p.err = err_word();
+  FBH_TRY(make_map(&p.ta[0], x.p, a.n, a.D, x.ld, kHalfM));
+  FBH_TRY(make_map(&p.tb[0], wg.p, a.F, a.D, wg.ld, 128));
+  FBH_TRY(make_map(&p.tb[1], wu.p, a.F, a.D, wu.ld, 128));
+  FBH_TRY(make_map(&p.tc[0], h, a.n, Fp, Fp, 32, false, true));
+  if (EPI == kGluBwd) {
+    FBH_TRY(make_map(&p.ta[1], dy.p, a.n, a.D, dy.ld, kHalfM));
+    FBH_TRY(make_map(&p.tw, wd.p, a.D, a.F, wd.ld, BK));
+    FBH_TRY(make_map(&p.tc[1], dgu, a.n, Fp, 2 * Fp, 32, false, true));
+    FBH_TRY(make_map(&p.tc[2], dgu + Fp, a.n, Fp, 2 * Fp, 32, false, true));
+  }
+  return launch_pair<EPI, false, false, 256>(p, c.stream);
+}
+
+int forward_bf16(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
+  const int64_t Fp = round_up(a.F, 64);
+  FBH_TAKE(h, c, __nv_bfloat16, a.n * Fp);
+  FBH_TRY(glu<fbpair::kGluFwd>(c, a, x, Mat{}, wg, wu, wd, h, nullptr, Fp));
+  const Term t{wd, 0, a.F};
+  return pair_rows(c, Mat{h, Fp}, a.n, a.F, &t, 1, false, a.D, Out{a.y, a.ldy, FB_BF16, 0});
+}
+
+int backward_bf16(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu,
+                  const Mat &wd) {
+  const int64_t Fp = round_up(a.F, 64);
+  FBH_TAKE(h, c, __nv_bfloat16, a.n * Fp);
+  FBH_TAKE(dgu, c, __nv_bfloat16, a.n * 2 * Fp);
+  FBH_TRY(glu<fbpair::kGluBwd>(c, a, x, dy, wg, wu, wd, h, dgu, Fp));
+  if (a.dx) {
+    const Term t[2] = {{wg, 0, a.F}, {wu, (int)Fp, a.F}};
+    FBH_TRY(pair_rows(c, Mat{dgu, 2 * Fp}, a.n, (int)(2 * Fp), t, 2, true, a.D, Out{a.dx, a.lddx, FB_BF16, 0}));
+  }
+  const Out og{a.dw_gate, a.ldd_gate, a.grad_type, a.accumulate}, ou{a.dw_up, a.ldd_up, a.grad_type, a.accumulate};
+  const Out both[2] = {og, ou};
+  if (a.dw_gate && a.dw_up) {
+    FBH_TRY(pair_columns(c, Mat{dgu, 2 * Fp}, a.n, (int)(2 * Fp), (int)Fp, 2, a.F, x, a.D, both));
+  } else if (a.dw_gate) {
+    FBH_TRY(pair_columns(c, Mat{dgu, 2 * Fp}, a.n, a.F, 0, 1, a.F, x, a.D, &og));
+  } else if (a.dw_up) {
+    FBH_TRY(pair_columns(c, Mat{dgu + Fp, 2 * Fp}, a.n, a.F, 0, 1, a.F, x, a.D, &ou));
+  }
+  const Out od{a.dw_down, a.ldd_down, a.grad_type, a.accumulate};
+  if (a.dw_down) FBH_TRY(pair_columns(c, dy, a.n, a.D, 0, 1, a.D, Mat{h, Fp}, a.F, &od));
+  return FB_OK;
 }
 
 // Weight gradients of a call without rows: zeros.
@@ -177,8 +194,14 @@ int empty_grads(const fb_gated_ffn &a, cudaStream_t st) {
 }
 
 int run(Call &c, const fb_gated_ffn &a, bool bwd) {
-  if (a.type == FB_F32) return bwd ? backward<float>(c, a) : forward<float>(c, a);
-  return bwd ? backward<__nv_bfloat16>(c, a) : forward<__nv_bfloat16>(c, a);
+  Mat x, wg, wu, wd, dy{};
+  FBH_TRY(aligned(c, a.type, Mat{a.x, a.ldx}, a.n, a.D, &x));
+  FBH_TRY(aligned(c, a.type, Mat{a.w_gate, a.ld_gate}, a.F, a.D, &wg));
+  FBH_TRY(aligned(c, a.type, Mat{a.w_up, a.ld_up}, a.F, a.D, &wu));
+  FBH_TRY(aligned(c, a.type, Mat{a.w_down, a.ld_down}, a.D, a.F, &wd));
+  if (!bwd) return a.type == FB_F32 ? forward_f32(c, a, x, wg, wu, wd) : forward_bf16(c, a, x, wg, wu, wd);
+  FBH_TRY(aligned(c, a.type, Mat{a.dy, a.lddy}, a.n, a.D, &dy));
+  return a.type == FB_F32 ? backward_f32(c, a, x, dy, wg, wu, wd) : backward_bf16(c, a, x, dy, wg, wu, wd);
 }
 
 }  // namespace

@@ -1,6 +1,5 @@
 // See head.cuh.
 #include "head.cuh"
-#include <cuda_bf16.h>
 #include <algorithm>
 
 namespace {
@@ -14,24 +13,6 @@ __global__ void k_copy_rows(const U *src, int64_t lds, U *dst, int64_t ldd, int6
     const int64_t r = i / ldd;
     const int c = (int)(i - r * ldd);
     dst[i] = c < cols ? src[r * lds + c] : (U)0;
-  }
-}
-
-template <bool kBf16>
-__global__ void k_store_rows(const float *src, int64_t lds, void *dst, int64_t ldd, int64_t rows, int cols,
-                             int accumulate) {
-  fb::pdl_enter();
-  const int64_t total = rows * cols;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / cols;
-    const int c = (int)(i - r * cols);
-    const float v = src[r * lds + c];
-    if (kBf16) {
-      static_cast<__nv_bfloat16 *>(dst)[r * ldd + c] = __float2bfloat16_rn(v);
-    } else {
-      float *o = static_cast<float *>(dst) + r * ldd + c;
-      *o = accumulate ? *o + v : v;
-    }
   }
 }
 
@@ -60,46 +41,18 @@ int aligned(Call &c, int type, const Mat &m, int64_t rows, int cols, Mat *out) {
   return FB_OK;
 }
 
-int product(Call &c, int type, int kind, const Mat &A, const Mat &B, float *C, int64_t ldc, int64_t M, int N, int K,
+int product(Call &c, int kind, const Mat &A, const Mat &B, float *C, int64_t ldc, int64_t M, int N, int K,
             int accumulate) {
-  size_t bytes;
   fb_gemm_problem p{};
-  fb_gemm_bf16_problem q{};
-  if (type == FB_F32) {
-    p.kind = kind;
-    p.A = static_cast<const float *>(A.p); p.lda = A.ld; p.k1 = K;
-    p.B = static_cast<const float *>(B.p); p.ldb = B.ld;
-    p.C = C; p.ldc = ldc; p.M = M; p.N = N; p.K = K; p.accumulate = accumulate;
-    bytes = fb_gemm_group_ws_bytes(&p, 1);
-  } else {
-    q.kind = kind;
-    q.A = static_cast<const uint16_t *>(A.p); q.lda = A.ld; q.k1 = K;
-    q.B = static_cast<const uint16_t *>(B.p); q.ldb = B.ld;
-    q.C = C; q.ldc = ldc; q.M = M; q.N = N; q.K = K; q.accumulate = accumulate;
-    bytes = fb_gemm_bf16_group_ws_bytes(&q, 1);
-  }
-  const size_t mark = c.off;
+  p.kind = kind;
+  p.A = static_cast<const float *>(A.p); p.lda = A.ld; p.k1 = K;
+  p.B = static_cast<const float *>(B.p); p.ldb = B.ld;
+  p.C = C; p.ldc = ldc; p.M = M; p.N = N; p.K = K; p.accumulate = accumulate;
+  const size_t bytes = fb_gemm_group_ws_bytes(&p, 1), mark = c.off;
   void *ws = c.take(bytes);
   if (!ws) return fb::set_error(FB_ERR_ARG, "workspace too small");
-  if (!c.dry) {
-    const int rc = type == FB_F32 ? fb_gemm_group(&p, 1, ws, bytes, c.stream)
-                                  : fb_gemm_bf16_group(&q, 1, ws, bytes, c.stream);
-    if (rc) return rc;
-  }
+  if (!c.dry) FBH_TRY(fb_gemm_group(&p, 1, ws, bytes, c.stream));
   c.off = mark;
-  return FB_OK;
-}
-
-int store_rows(Call &c, const float *src, int64_t lds, void *dst, int64_t ldd, int dst_type, int64_t rows, int cols,
-               int accumulate) {
-  if (c.dry || rows == 0) return FB_OK;
-  if (dst_type == FB_BF16)
-    FB_TRY_CUDA(fb::launch(k_store_rows<true>, blocks_for(rows * cols), 256, 0, c.stream, src, lds, dst, ldd, rows,
-                           cols, 0));
-  else
-    FB_TRY_CUDA(fb::launch(k_store_rows<false>, blocks_for(rows * cols), 256, 0, c.stream, src, lds, dst, ldd, rows,
-                           cols, accumulate));
-  FB_LAUNCHED("k_store_rows");
   return FB_OK;
 }
 

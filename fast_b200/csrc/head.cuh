@@ -39,14 +39,32 @@ struct Mat {
 // workspace when m is not.
 int aligned(Call &c, int type, const Mat &m, int64_t rows, int cols, Mat *out);
 
-// C (+)= A B^T (NT), A B (NN) or A^T B (TN: C [N, K] over M rows), as
-// fb_gemm_group / fb_gemm_bf16_group define them; C is fp32.
-int product(Call &c, int type, int kind, const Mat &A, const Mat &B, float *C, int64_t ldc, int64_t M, int N, int K,
+// fp32: C (+)= A B^T (NT), A B (NN) or A^T B (TN: C [N, K] over M rows), as
+// fb_gemm_group defines them.
+int product(Call &c, int kind, const Mat &A, const Mat &B, float *C, int64_t ldc, int64_t M, int N, int K,
             int accumulate);
 
-// dst (fp32 or bf16) = src (fp32), or += when accumulate (fp32 dst).
-int store_rows(Call &c, const float *src, int64_t lds, void *dst, int64_t ldd, int dst_type, int64_t rows, int cols,
-               int accumulate);
+// Where a product goes: rows of fp32 or bf16, written, or (fp32) added to.
+struct Out {
+  void *p;
+  int64_t ld;
+  int type, accumulate;
+};
+
+// bf16 products on pairs of SMs (pair_gemm.cuh); operands as `aligned` leaves
+// them, fp32 accumulation, one rounding at the end.
+//   rows: C[m, n] = sum over 1 or 2 terms of A[m, ax_t + k] B_t(n, k), A [M, acols], k < K_t; B_t is [N, K_t], or
+//         [K_t, N] when b_mn.  ax_t is a multiple of 64.
+struct Term {
+  Mat B;
+  int ax, K;
+};
+int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, int n_terms, bool b_mn, int N,
+              const Out &out);
+//   columns: C_p[m, n] = sum over the `rows` rows r of A[r, p * aprob + m] B[r, n], m < M, n < N, for p < probs
+//         (1 or 2) outputs; A has acols columns.
+int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int probs, int M, const Mat &B, int N,
+                 const Out *out);
 
 }  // namespace fbh
 

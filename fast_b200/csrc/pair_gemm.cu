@@ -1,0 +1,162 @@
+// Plain products of the node-ranking head on pairs of SMs (pair_gemm.cuh), and
+// the sum of their partial results when the reduction is split.
+#include "pair_gemm.cuh"
+
+namespace {
+
+using namespace fbpair;
+using namespace fbh;
+
+// out (+)= sum over splits of P[s], in split order; P rows have pitch ldp.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) k_sum_splits(const float *P, int64_t split_stride, int64_t ldp, int splits,
+                                                    void *out, int64_t ldo, int64_t rows, int cols, int accumulate) {
+  fb::pdl_enter();
+  const int64_t total = rows * cols;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / cols;
+    const int c = (int)(i - r * cols);
+    const float *p = P + r * ldp + c;
+    float s = 0.f;
+    int z = 0;
+    for (; z + 8 <= splits; z += 8) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = p[(z + u) * split_stride];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+    for (; z < splits; ++z) s += p[z * split_stride];
+    if (kBf16) {
+      static_cast<__nv_bfloat16 *>(out)[r * ldo + c] = __float2bfloat16_rn(s);
+    } else {
+      float *o = static_cast<float *>(out) + r * ldo + c;
+      *o = accumulate ? *o + s : s;
+    }
+  }
+}
+
+int sum_splits(Call &c, const float *P, int64_t split_stride, int64_t ldp, int splits, const Out &o, int64_t rows,
+               int cols) {
+  const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows * cols + 255) / 256, 148 * 16));
+  if (o.type == FB_BF16)
+    FB_TRY_CUDA(fb::launch(k_sum_splits<true>, blocks, 256, 0, c.stream, P, split_stride, ldp, splits, o.p, o.ld, rows,
+                           cols, 0));
+  else
+    FB_TRY_CUDA(fb::launch(k_sum_splits<false>, blocks, 256, 0, c.stream, P, split_stride, ldp, splits, o.p, o.ld, rows,
+                           cols, o.accumulate));
+  FB_LAUNCHED("k_sum_splits");
+  return FB_OK;
+}
+
+// Tile width and splits for results of M x N over kb stages.  256 columns keep
+// the tensor cores fed; a grid that would leave half the SM pairs idle takes
+// 128-column tiles, then splits the reduction, at least kMinStages a split.
+constexpr int kMinStages = 4;
+struct Plan {
+  int bn, splits, kper;
+};
+Plan plan_of(int64_t M, int N, int probs, int kb, bool may_split) {
+  const int slots = num_sms() / 2;
+  Plan p{N > 128 ? 256 : 128, 1, kb};
+  const int64_t mt = tiles_of(M, 256);
+  if (p.bn == 256 && mt * tiles_of(N, 256) * probs * 2 <= slots) p.bn = 128;
+  const int64_t tiles = mt * tiles_of(N, p.bn) * probs;
+  if (may_split && tiles * 2 <= slots) {
+    const int s = (int)std::min<int64_t>(slots / tiles, kb / kMinStages);
+    if (s > 1) {
+      p.kper = (kb + s - 1) / s;
+      p.splits = tiles_of(kb, p.kper);
+    }
+  }
+  return p;
+}
+
+template <bool A_MN, bool B_MN> int dispatch(const PairArgs &a, int bn, bool f32, cudaStream_t st) {
+  if (f32)
+    return bn == 256 ? launch_pair<kStoreF32, A_MN, B_MN, 256>(a, st) : launch_pair<kStoreF32, A_MN, B_MN, 128>(a, st);
+  return bn == 256 ? launch_pair<kStoreBf16, A_MN, B_MN, 256>(a, st) : launch_pair<kStoreBf16, A_MN, B_MN, 128>(a, st);
+}
+
+// Fills the tiling and the outputs (or the partial results') of `a`, launches, sums the splits.
+template <bool A_MN, bool B_MN> int finish(Call &c, PairArgs &a, const Plan &p, int64_t M, int N, const Out *out) {
+  a.mt = tiles_of(M, 256);
+  a.nt = tiles_of(N, p.bn);
+  a.splits = p.splits;
+  a.kper = p.kper;
+  a.M = (int)M;
+  a.N = N;
+  a.err = c.dry ? nullptr : err_word();
+  const int64_t prow = (int64_t)a.mt * 256, pld = round_up(N, 4);
+  float *P[2] = {nullptr, nullptr};
+  const size_t mark = c.off;
+  if (p.splits > 1)
+    for (int i = 0; i < a.probs; ++i) {
+      P[i] = static_cast<float *>(c.take((size_t)(p.splits * prow * pld) * 4));
+      if (!P[i]) return fb::set_error(FB_ERR_ARG, "workspace too small");
+    }
+  c.off = mark;
+  if (c.dry) return FB_OK;
+  const bool f32 = p.splits > 1 || out[0].type == FB_F32;
+  a.has_tc = 1;
+  a.accumulate = p.splits > 1 ? 0 : out[0].accumulate;
+  a.split_rows = prow;
+  for (int i = 0; i < a.probs; ++i) {
+    if (p.splits > 1) {
+      FBH_TRY(make_map(&a.tc[i], P[i], p.splits * prow, N, pld, 32, true));
+    } else {
+      a.C[i] = out[i].p;
+      a.ldc = out[i].ld;
+      if (out[i].ld != out[0].ld || !map_ok(out[i].p, out[i].ld, f32 ? 4 : 2)) a.has_tc = 0;
+    }
+  }
+  if (p.splits == 1 && a.has_tc)
+    for (int i = 0; i < a.probs; ++i) FBH_TRY(make_map(&a.tc[i], out[i].p, M, N, out[i].ld, 32, f32));
+  FBH_TRY((dispatch<A_MN, B_MN>(a, p.bn, f32, c.stream)));
+  if (p.splits > 1)
+    for (int i = 0; i < a.probs; ++i) FBH_TRY(sum_splits(c, P[i], prow * pld, pld, p.splits, out[i], M, N));
+  return FB_OK;
+}
+
+}  // namespace
+
+namespace fbh {
+
+int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, int n_terms, bool b_mn, int N,
+              const Out &out) {
+  if (M == 0) return FB_OK;
+  PairArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.phases = n_terms;
+  a.probs = 1;
+  for (int t = 0; t < n_terms; ++t) {
+    a.kb[t] = tiles_of(terms[t].K, BK);
+    a.ax[t] = terms[t].ax;
+  }
+  const Plan p = plan_of(M, N, 1, a.kb[0], n_terms == 1);
+  if (!c.dry)
+    for (int t = 0; t < n_terms; ++t) {
+      FBH_TRY(make_map(&a.ta[t], A.p, M, acols, A.ld, kHalfM));
+      if (b_mn) FBH_TRY(make_map(&a.tb[t], terms[t].B.p, terms[t].K, N, terms[t].B.ld, BK));
+      else FBH_TRY(make_map(&a.tb[t], terms[t].B.p, N, terms[t].K, terms[t].B.ld, p.bn / 2));
+    }
+  return b_mn ? finish<false, true>(c, a, p, M, N, &out) : finish<false, false>(c, a, p, M, N, &out);
+}
+
+int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int probs, int M, const Mat &B, int N,
+                 const Out *out) {
+  PairArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.phases = 1;
+  a.probs = probs;
+  a.aprob = aprob;
+  a.kb[0] = tiles_of(rows, BK);
+  const Plan p = plan_of(M, N, probs, a.kb[0], true);
+  if (!c.dry) {
+    FBH_TRY(make_map(&a.ta[0], A.p, rows, acols, A.ld, BK));
+    FBH_TRY(make_map(&a.tb[0], B.p, rows, N, B.ld, BK));
+  }
+  return finish<true, true>(c, a, p, M, N, out);
+}
+
+}  // namespace fbh

@@ -1,0 +1,698 @@
+// bf16 products on pairs of SMs for the node-ranking head: tcgen05.mma with
+// cta_group::2, operands by TMA, fp32 accumulators in tensor memory, and the
+// operators' own arithmetic in the epilogue.
+//
+//   kernel k_pair<EPI, A_MN, B_MN, BN>: C[m, n] = sum_k A(m, k) B(n, k)
+//   A_MN / B_MN: the operand lies with its m (n) index contiguous (the matrix
+//   is stored [k][m]); else with k contiguous.
+//
+// A cluster of two CTAs works on a 256 x BN tile: each CTA stages 128 rows of
+// A and BN / 2 rows of B, the MMA of the even CTA reads both halves from both
+// SMs, and each CTA's tensor memory holds its own 128 rows of the tile.  So
+// every operand byte is staged once per pair: a BN = 256 tile moves 64 bytes
+// of shared memory a cycle and SM in each direction (TMA writes, MMA reads),
+// half of what one SM alone would need.
+//
+// CTA = 12 warps: 0 TMA producer (one lane), 1 TMEM allocator and, in the
+// even CTA, MMA issuer (one lane), 4..11 epilogue (two per TMEM lane
+// quadrant, each half of the columns).  Stages of 64 k travel through a ring
+// of kStages; the loads of both CTAs count on the even CTA's barrier, MMA
+// completion frees the stage in both.  Accumulators: two of up to 256 columns
+// (the epilogue drains one while the other fills), one of 384 for kGluBwd.
+//
+// No load uses cluster multicast.  Every wait is bounded: past the limit a
+// CTA records an error, stops, gives its copies time to land and leaves.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <algorithm>
+#include <cstring>
+#include "head.cuh"
+#include "tc_common.cuh"
+
+namespace fbpair {
+
+using namespace fbtc;
+
+enum : int { kStoreBf16 = 0, kStoreF32 = 1, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5 };
+enum : int { kSilu = FB_ACT_SILU, kGelu = FB_ACT_GELU, kRelu = FB_ACT_RELU };
+
+constexpr int BK = 64;                        // k per stage: one 128-byte swizzle row of bf16
+constexpr int kHalfM = 128;                   // rows of a tile per CTA
+constexpr int kABytes = kHalfM * BK * 2;      // 16 KB
+constexpr int kBBytes = 128 * BK * 2;         // 16 KB: BN / 2 <= 128 rows
+constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kBox = BK * 128;                // MN-major box: 64 k rows of 64 elements
+constexpr int kEpiWarps = 8, kWarpEpi0 = 4;
+constexpr int kThreads = (kWarpEpi0 + kEpiWarps) * 32;
+constexpr int kTmemCols = 512;
+constexpr int kStageOut = 4096;               // one staged output block: 32 rows of 128 bytes
+constexpr int kGluOut = 2048;                 // of the gated block's outputs: 32 rows of 64 bytes
+template <int EPI> __host__ __device__ constexpr int out_bytes() {
+  return EPI == kGluBwd ? 3 * kGluOut : (EPI == kGluFwd ? kGluOut : kStageOut);
+}
+template <int EPI> __host__ __device__ constexpr int stages() { return EPI == kGluBwd ? 5 : 6; }
+template <int EPI> __host__ __device__ constexpr int smem_bytes() {
+  return 1024 + stages<EPI>() * kStageBytes + kEpiWarps * out_bytes<EPI>() + 256;
+}
+static_assert(smem_bytes<kGluBwd>() <= 232448 && smem_bytes<kLse>() <= 232448, "shared memory exceeds 227 KB");
+
+// Fields of one launch.  Two phases may feed a tile: kGluBwd's second one
+// fills the dh columns; elsewhere it continues the same sum (dx = dg Wg + du Wu).
+struct PairArgs {
+  CUtensorMap ta[2], tb[2];                   // by phase; kGluFwd / kGluBwd: tb[0] = Wg, tb[1] = Wu, tw = Wd
+  CUtensorMap tw;
+  CUtensorMap tc[3];                          // outputs (has_tc)
+  int32_t *err;
+  int mt, nt, probs, splits;                  // tiles along m and n, problems of one shape, splits of k
+  int phases, kb[2], kper;                    // stages per phase; stages per split (phase 0, splits > 1)
+  int ax[2];                                  // A's first column per phase (k contiguous) ...
+  int aprob;                                  // ... and per problem (m contiguous: columns of A between problems)
+  int M, N;                                   // rows and columns of one problem's result
+  int has_tc;
+  int accumulate;                             // kStoreF32: add to what is there
+  void *C[2];                                 // no has_tc: the results, row pitch ldc
+  int64_t ldc;
+  int64_t split_rows;                         // splits > 1: rows of C between two splits
+  int act;
+  float2 *part;                               // kLse: [M][2 nt] (max, sum of exp2) partials
+  const int64_t *target;                      // kProb
+  const float *lse, *dloss;
+  int64_t V, v0;
+};
+static_assert(sizeof(PairArgs) <= 4096, "kernel parameters exceed 4 KB");
+
+// ---- PTX -----------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-memory address of `p` in the even CTA of the pair.
+__device__ __forceinline__ uint32_t leader_addr(const void *p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Wait for a phase whose arrivals come from both CTAs.
+__device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
+  if (try_wait_cluster(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!try_wait_cluster(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      *abort_flag = 1;
+      atomicOr(err, kErrTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+// A tile of this CTA's shared memory, counted on a barrier of the even CTA.
+__device__ __forceinline__ void load2(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void alloc2(uint32_t *holder, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void dealloc2(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void mma2(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The barrier at this offset in both CTAs, once every MMA issued so far is complete.
+__device__ __forceinline__ void commit2(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void store_tile(const CUtensorMap *map, const void *src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void add_tile(const CUtensorMap *map, const void *src, int x, int y) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void store_wait() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+// 32 accumulator columns without the wait (tmem_wait before the values are used).
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptor (128-byte swizzle, 1024-byte aligned tile).
+// K-major: rows of 128 B, 8-row groups 1024 B apart; 16 k = 32 B further on.
+// MN-major: [64 k][64 mn] boxes side by side along mn, 8-row groups 1024 B
+// apart; 16 k = 2 KB further on.
+__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, bool mn) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(mn ? (kBox >> 4) : 1) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;                     // descriptor version (sm_100)
+  d |= (uint64_t)2 << 61;                     // SWIZZLE_128B
+  return d;
+}
+// D fp32, A and B bf16, dense, M = 256 over the pair
+__host__ __device__ constexpr uint32_t idesc2(int bn, bool a_mn, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+}
+
+// 2^x by the hardware's approximation (2 ulp, denormal results are zeros)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- epilogue pieces -----------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// act(g) and act'(g)
+template <int ACT> __device__ __forceinline__ float2 act2(float g) {
+  if (ACT == kSilu) {
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    return make_float2(g * s, s * (1.f + g * (1.f - s)));
+  }
+  if (ACT == kGelu) {
+    const float phi = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    return make_float2(g * phi, phi + g * __expf(-0.5f * g * g) * 0.39894228040143268f);
+  }
+  return make_float2(fmaxf(g, 0.f), g > 0.f ? 1.f : 0.f);
+}
+
+// One lane's row (128 bytes in eight 16-byte pieces) of a staged block: the
+// layout a 128-byte-swizzled tensor map stores from.
+__device__ __forceinline__ void stage_row(uint8_t *buf, int lane, const uint32_t (&w)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4 *>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+}
+
+// Sends a staged block (32 rows from `row`, 64 bf16 or 32 fp32 columns from
+// `col`) to output `o`.  Rows at or past `rows` and columns past a.N stay out.
+template <bool F32OUT>
+__device__ __forceinline__ void send(const PairArgs &a, int o, const uint8_t *buf, int64_t ybase, int row, int col,
+                                     int lane) {
+  fence_async_smem();
+  __syncwarp();
+  const bool in = row < a.M && col < a.N;
+  if (lane == 0) {                            // one bulk group per block, empty or not
+    if (in && a.has_tc) {
+      if (F32OUT && a.accumulate) add_tile(&a.tc[o], buf, col, (int)(ybase + row));
+      else store_tile(&a.tc[o], buf, col, (int)(ybase + row));
+    }
+    store_commit();
+  }
+  if (!in || a.has_tc) return;
+  const int nr = min(32, a.M - row);
+  if (F32OUT) {
+    float *p = static_cast<float *>(a.C[o]) + (ybase + row) * a.ldc + col + lane;
+    if (col + lane < a.N)
+      for (int r = 0; r < nr; ++r) {
+        const float v = *reinterpret_cast<const float *>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+        p[r * a.ldc] = a.accumulate ? p[r * a.ldc] + v : v;
+      }
+  } else {
+    uint16_t *p = static_cast<uint16_t *>(a.C[o]) + (ybase + row) * a.ldc + col;
+    for (int r = 0; r < nr; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = lane + 32 * h;
+        if (col + c < a.N)
+          p[r * a.ldc + c] =
+              *reinterpret_cast<const uint16_t *>(buf + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+      }
+  }
+}
+
+struct Tile {
+  int m, n, prob, k0, k1;
+  int64_t ybase;                              // first row of this split's results
+};
+
+// Tiles run along m inside groups of 8 m-tiles, so that a wave's tiles share
+// few distinct operand rows; problems outermost, then splits.
+__device__ __forceinline__ Tile tile_at(const PairArgs &a, int t) {
+  Tile q;
+  const int per = a.mt * a.nt;
+  const int z = t / per;
+  int r = t - z * per;
+  const int s = z % a.splits;
+  q.prob = z / a.splits;
+  const int grp = 8 * a.nt, g = r / grp;
+  r -= g * grp;
+  const int gm = min(8, a.mt - 8 * g);
+  q.m = 8 * g + r % gm;
+  q.n = r / gm;
+  q.k0 = a.splits > 1 ? s * a.kper : 0;
+  q.k1 = a.splits > 1 ? min(a.kb[0], q.k0 + a.kper) : a.kb[0];
+  q.ybase = a.splits > 1 ? s * a.split_rows : 0;
+  return q;
+}
+
+// Columns c .. c + 31 of g (and + 128: u, + 256: dh) of this warp's 32 rows:
+// h (and dg, du) staged as blocks of 32 rows x 64 bytes in the 64-byte
+// swizzle and sent off.
+template <int ACT, bool BWD>
+__device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, uint8_t *buf, int row, int col,
+                                          int lane) {
+  uint32_t w[BWD ? 3 : 1][16];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    uint32_t g[16], u[16], d[BWD ? 16 : 1];
+    tmem_ld16_nowait(t + c + 16 * q, g);
+    tmem_ld16_nowait(t + 128 + c + 16 * q, u);
+    if constexpr (BWD) tmem_ld16_nowait(t + 256 + c + 16 * q, d);
+    tmem_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float h[2], dg[2], du[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 f = act2<ACT>(__uint_as_float(g[2 * i + e]));
+        const float uv = __uint_as_float(u[2 * i + e]);
+        h[e] = f.x * uv;
+        if constexpr (BWD) {
+          const float dv = __uint_as_float(d[2 * i + e]);
+          dg[e] = dv * uv * f.y;
+          du[e] = dv * f.x;
+        }
+      }
+      w[0][8 * q + i] = pack(h[0], h[1]);
+      if constexpr (BWD) {
+        w[1][8 * q + i] = pack(dg[0], dg[1]);
+        w[2][8 * q + i] = pack(du[0], du[1]);
+      }
+    }
+  }
+  if (lane == 0) store_wait<0>();             // the block before has left the buffers
+  __syncwarp();
+#pragma unroll
+  for (int o = 0; o < (BWD ? 3 : 1); ++o)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      *reinterpret_cast<uint4 *>(buf + o * kGluOut + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(w[o][4 * k], w[o][4 * k + 1], w[o][4 * k + 2], w[o][4 * k + 3]);
+  fence_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (row < a.M && col < a.N)
+#pragma unroll
+      for (int o = 0; o < (BWD ? 3 : 1); ++o) store_tile(&a.tc[o], buf + o * kGluOut, col, row);
+    store_commit();
+  }
+}
+
+template <int EPI, bool A_MN, bool B_MN, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(const __grid_constant__ PairArgs a) {
+  constexpr int kStages = stages<EPI>(), kBufs = EPI == kGluBwd ? 1 : 2;
+  constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd;      // B: 128 rows of Wg in one CTA, of Wu in the other
+  static_assert(!kDual || BN == 256, "the gate and up columns fill a 256-column tile");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = align1024(smem_raw);
+  auto sA = [&](int s) { return smem + s * kStageBytes; };
+  auto sB = [&](int s) { return smem + s * kStageBytes + kABytes; };
+  uint8_t *outs = smem + kStages * kStageBytes;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(outs + kEpiWarps * out_bytes<EPI>());
+  uint64_t *full = bars, *empty = bars + kStages, *accf = bars + 2 * kStages, *acce = accf + 2;
+  uint32_t *holder = reinterpret_cast<uint32_t *>(acce + 2);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full + s, 1);                 // the even CTA's: its own expect, both CTAs' bytes
+      mbar_init(empty + s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(accf + b, 1);
+      mbar_init(acce + b, 2 * kEpiWarps);     // the even CTA's: both CTAs' epilogue warps
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) alloc2(holder, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                             // both CTAs' barriers exist before either signals one
+  tc_fence_after();
+  const uint32_t tmem = *holder;
+  fb::pdl_enter();
+
+  const int total = a.mt * a.nt * a.probs * a.splits;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  int32_t *err = a.err;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t g = 0;
+      bool stop = false;
+      for (int t = first; t < total && !stop; t += step) {
+        const Tile q = tile_at(a, t);
+        const int m0 = q.m * 256 + (int)rank * kHalfM;
+        for (int p = 0; p < a.phases && !stop; ++p) {
+          const bool dh = EPI == kGluBwd && p == 1;
+          const int bn = dh ? 128 : BN;
+          const int j1 = p == 0 ? q.k1 : a.kb[1];
+          const uint32_t bytes = (uint32_t)(kABytes + bn / 2 * BK * 2);
+          const bool bmn = dh || B_MN;
+          for (int j = p == 0 ? q.k0 : 0; j < j1; ++j) {
+            const int s = g % kStages;
+            if (g >= (uint32_t)kStages && !wait(empty + s, ((g / kStages) - 1) & 1, abort_flag, err)) {
+              stop = true;
+              break;
+            }
+            if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
+            const uint32_t bar = leader_addr(full + s);
+            if (A_MN) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                load2(sA(s) + i * kBox, &a.ta[p], bar, q.prob * a.aprob + m0 + 64 * i, BK * j);
+            } else {
+              load2(sA(s), &a.ta[p], bar, a.ax[p] + BK * j, m0);
+            }
+            if (kDual && !dh) {
+              load2(sB(s), &a.tb[rank], bar, BK * j, q.n * 128);
+            } else {
+              const CUtensorMap *mb = dh ? &a.tw : &a.tb[p];
+              const int n0 = q.n * bn + (int)rank * (bn / 2);
+              if (bmn) {
+                for (int i = 0; i < bn / 128; ++i) load2(sB(s) + i * kBox, mb, bar, n0 + 64 * i, BK * j);
+              } else {
+                load2(sB(s), mb, bar, BK * j, n0);
+              }
+            }
+            ++g;
+          }
+        }
+      }
+      // the MMAs have read every stage (and their arrivals reached this CTA) before it leaves
+      for (uint32_t h = g > (uint32_t)kStages ? g - kStages : 0; h < g && !stop; ++h)
+        if (!wait(empty + h % kStages, (h / kStages) & 1, abort_flag, err)) stop = true;
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      uint32_t g = 0, it = 0;
+      bool stop = false;
+      for (int t = first; t < total && !stop; t += step, ++it) {
+        const Tile q = tile_at(a, t);
+        const int buf = it % kBufs;
+        const uint32_t use = it / kBufs;
+        if (use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) break;
+        tc_fence_after();
+        for (int p = 0; p < a.phases && !stop; ++p) {
+          const bool dh = EPI == kGluBwd && p == 1;
+          const bool bmn = dh || B_MN;
+          const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(BN, A_MN, B_MN);
+          const uint32_t d = tmem + (dh ? 256u : (uint32_t)(buf * 256));
+          const uint64_t adv_a = A_MN ? (2048 >> 4) : 2, adv_b = bmn ? (2048 >> 4) : 2;
+          const bool fresh = p == 0 || dh;    // the sum starts here
+          const int j0 = p == 0 ? q.k0 : 0, j1 = p == 0 ? q.k1 : a.kb[1];
+          for (int j = j0; j < j1; ++j) {
+            const int s = g % kStages;
+            if (!wait(full + s, (g / kStages) & 1, abort_flag, err)) {
+              stop = true;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t ad = sdesc(smem_u32(sA(s)), A_MN), bd = sdesc(smem_u32(sB(s)), bmn);
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk)
+              mma2(d, ad + kk * adv_a, bd + kk * adv_b, idesc, (fresh && j == j0 && kk == 0) ? 0u : 1u);
+            commit2(empty + s);
+            ++g;
+          }
+        }
+        if (!stop) commit2(accf + buf);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kWarpEpi0) {
+    const int e = warp - kWarpEpi0, qd = warp & 3, half = e >> 2;
+    const uint32_t tlane = (uint32_t)(qd * 32) << 16;
+    uint8_t *obuf = outs + e * out_bytes<EPI>();
+    uint32_t it = 0;
+    for (int t = first; t < total; t += step, ++it) {
+      const Tile q = tile_at(a, t);
+      const int buf = it % kBufs;
+      if (!__all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0)) break;
+      tc_fence_after();
+      const uint32_t tb = tmem + tlane + (uint32_t)(buf * 256);
+      const int row = q.m * 256 + (int)rank * kHalfM + qd * 32;   // this warp's first row
+      if constexpr (EPI == kGluFwd || EPI == kGluBwd) {
+        constexpr bool bwd = EPI == kGluBwd;
+#pragma unroll 1
+        for (int c = half * 64; c < half * 64 + 64; c += 32) {
+          const int col = q.n * 128 + c;
+          if (a.act == kSilu) glu_block<kSilu, bwd>(a, tb, c, obuf, row, col, lane);
+          else if (a.act == kGelu) glu_block<kGelu, bwd>(a, tb, c, obuf, row, col, lane);
+          else glu_block<kRelu, bwd>(a, tb, c, obuf, row, col, lane);
+        }
+      } else if constexpr (EPI == kStoreBf16) {
+#pragma unroll 1
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 64) {
+          uint32_t r0[32], r1[32], w[32];
+          tmem_ld32_nowait(tb + c, r0);
+          tmem_ld32_nowait(tb + c + 32, r1);
+          tmem_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            w[i] = pack(__uint_as_float(r0[2 * i]), __uint_as_float(r0[2 * i + 1]));
+            w[16 + i] = pack(__uint_as_float(r1[2 * i]), __uint_as_float(r1[2 * i + 1]));
+          }
+          if (lane == 0) store_wait<0>();
+          __syncwarp();
+          stage_row(obuf, lane, w);
+          send<false>(a, q.prob, obuf, q.ybase, row, q.n * BN + c, lane);
+          __syncwarp();
+        }
+      } else if constexpr (EPI == kStoreF32) {
+#pragma unroll 1
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+          uint32_t r[32];
+          tmem_ld32_nowait(tb + c, r);
+          tmem_wait();
+          if (lane == 0) store_wait<0>();
+          __syncwarp();
+          stage_row(obuf, lane, r);
+          send<true>(a, q.prob, obuf, q.ybase, row, q.n * BN + c, lane);
+          __syncwarp();
+        }
+      } else if constexpr (EPI == kLse) {
+        // running maximum and sum of exp2 of this lane's row over its half of the tile's columns
+        constexpr float kLog2e = 1.44269504088896340736f;
+        float m = -INFINITY, s = 0.f;
+        const int cbase = q.n * BN;
+#pragma unroll 1
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+          if (cbase + c >= a.N) break;
+          uint32_t r[32];
+          tmem_ld32_nowait(tb + c, r);
+          tmem_wait();
+          const int left = a.N - (cbase + c);
+          if (left < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i >= left) r[i] = 0xFF800000u;                  // -inf: past the table
+          }
+          float cm = __uint_as_float(r[0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) cm = fmaxf(cm, __uint_as_float(r[i]));
+          const float nm = fmaxf(m, cm * kLog2e);
+          // nothing but -inf so far: subtract 0 so that exp2 gives zeros (and NaN stays NaN)
+          const float base = nm == -INFINITY ? 0.f : nm;
+          s *= ex2(m - base);
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            s0 += ex2(fmaf(__uint_as_float(r[i]), kLog2e, -base));
+            s1 += ex2(fmaf(__uint_as_float(r[i + 1]), kLog2e, -base));
+          }
+          s += s0 + s1;
+          m = nm;
+        }
+        if (row + lane < a.M) a.part[(int64_t)(row + lane) * (2 * a.nt) + 2 * q.n + half] = make_float2(m, s);
+      } else if constexpr (EPI == kProb) {
+        constexpr float kLog2e = 1.44269504088896340736f;
+        const int i0 = row + lane;
+        const int64_t tg = i0 < a.M ? a.target[i0] : -1;
+        const bool live = tg >= 0 && tg < a.V;
+        const float z = live ? a.lse[i0] * kLog2e : 0.f, d = live ? a.dloss[i0] : 0.f;
+        const uint32_t mask = live ? 0xFFFFFFFFu : 0u;            // a held-out row is zeros whatever its logits are
+        const int64_t tc = live ? tg - a.v0 : -1;                 // the target's column of this piece
+#pragma unroll 1
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 64) {
+          const int col = q.n * BN + c;
+          uint32_t r0[32], r1[32], w[32];
+          tmem_ld32_nowait(tb + c, r0);
+          tmem_ld32_nowait(tb + c + 32, r1);
+          tmem_wait();
+          const int hit = (tc >= col && tc < col + 64) ? (int)(tc - col) : -1;
+          const bool any = __any_sync(0xffffffffu, hit >= 0);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float l0 = __uint_as_float(i < 16 ? r0[2 * i] : r1[2 * (i - 16)]);
+            const float l1 = __uint_as_float(i < 16 ? r0[2 * i + 1] : r1[2 * (i - 16) + 1]);
+            float p0 = ex2(fmaf(l0, kLog2e, -z)), p1 = ex2(fmaf(l1, kLog2e, -z));
+            if (any) {
+              if (hit == 2 * i) p0 -= 1.f;
+              if (hit == 2 * i + 1) p1 -= 1.f;
+            }
+            w[i] = pack(p0 * d, p1 * d) & mask;
+          }
+          if (lane == 0) store_wait<0>();
+          __syncwarp();
+          stage_row(obuf, lane, w);
+          send<false>(a, 0, obuf, 0, row, col, lane);
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(leader_addr(acce + buf));
+    }
+    if (lane == 0) store_wait<0>();
+    __syncwarp();
+  }
+  __syncwarp();
+  if (*abort_flag) {                          // copies in flight land before the shared memory goes away
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                             // neither CTA leaves while the other may still reach into it
+  if (warp == 1) dealloc2(tmem, kTmemCols);
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+// A bf16 (or fp32: f32) matrix in boxes of 128-byte rows x box_rows, 128-byte swizzle.
+// half: 64-byte rows and swizzle.
+inline int make_map(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows,
+                    bool f32 = false, bool half = false) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fb::set_error(FB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int es = f32 ? 4 : 2;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * es)};
+  cuuint32_t box[2] = {(cuuint32_t)((half ? 64 : 128) / es), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                         const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         half ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fb::set_error(FB_ERR_ARG, "tensor map rejected (alignment or stride)");
+  return FB_OK;
+}
+
+inline bool map_ok(const void *p, int64_t ld, int es) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * es)) & 15u) == 0;
+}
+
+// Clusters of two that fit on the device at once.
+template <auto kernel> int pair_slots(int smem) {
+  static int slots[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int &s = slots[dev & 63];
+  if (!s) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(num_sms() / 2 * 2);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    s = n > 0 ? n : num_sms() / 2;
+  }
+  return s;
+}
+
+template <int EPI, bool A_MN, bool B_MN, int BN> int launch_pair(const PairArgs &a, cudaStream_t stream) {
+  constexpr auto k = k_pair<EPI, A_MN, B_MN, BN>;
+  constexpr int smem = smem_bytes<EPI>();
+  const int slots = pair_slots<k>(smem);
+  if (!slots) return fb::cuda_error(cudaGetLastError(), "k_pair shared memory");
+  const int64_t tiles = (int64_t)a.mt * a.nt * a.probs * a.splits;
+  if (tiles == 0) return FB_OK;
+  const unsigned grid = 2 * (unsigned)std::min<int64_t>(tiles, slots);
+  FB_TRY_CUDA(fb::launch(k, grid, kThreads, smem, stream, a));
+  FB_LAUNCHED("k_pair");
+  return FB_OK;
+}
+
+inline int tiles_of(int64_t n, int t) { return (int)((n + t - 1) / t); }
+
+}  // namespace fbpair

@@ -1,13 +1,17 @@
 // Softmax cross entropy of rows h [n, D] against every row of a table w [V, D]:
 //   l = h w^T,  lse_i = log sum_v exp(l_iv),  loss_i = lse_i - l_i,target
 //   G = dloss_i (exp(l_iv - lse_i) - [v == target]),  dh = G w,  dw = G^T h
-// The logits are never kept: both directions take the table in pieces of as
-// many rows as make a logits piece of kPieceBytes (it stays in the L2), the
-// forward carrying each row's running maximum and sum over the pieces.
-#include <cuda_bf16.h>
-#include <algorithm>
+// The logits are never kept.  bf16 (products on SM pairs, pair_gemm.cuh): the
+// forward reduces every 256-column tile of logits to a maximum and a sum per
+// row in its epilogue, one launch over the whole table, and a second kernel
+// joins them; the backward takes the table in pieces of as many rows as make a
+// G piece of kPieceBytes (so that it stays in the L2 between its three
+// products), computes G from the logits in the epilogue that would have stored
+// them, then adds G w to dh and writes G^T h.  fp32: the grouped 3xTF32
+// products over pieces of logits, the forward carrying each row's running
+// maximum and sum from piece to piece.
 #include <cmath>
-#include "head.cuh"
+#include "pair_gemm.cuh"
 
 namespace {
 
@@ -22,6 +26,35 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
   const float m = fmaxf(a.m, b.m);
   if (m == -INFINITY) return MaxSum{m, a.s + b.s};     // a NaN sum stays one
   return MaxSum{m, a.s * expf(a.m - m) + b.s * expf(b.m - m)};
+}
+
+// bf16 rows: one warp joins a row's partial (max, sum of exp2) pairs, takes the
+// target's logit as an fp32 dot product of its own, and writes lse and loss.
+__global__ void __launch_bounds__(128) k_xent_finish(const float2 *part, int np, const uint16_t *h, int64_t ldh,
+                                                     const uint16_t *w, int64_t ldw, int D, int64_t V,
+                                                     const int64_t *target, float *loss, float *lse, int64_t n) {
+  fb::pdl_enter();
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= n) return;
+  const float2 *p = part + r * np;
+  float m = -INFINITY;
+  for (int i = lane; i < np; i += 32) m = fmaxf(m, p[i].x);
+  m = fb::warp_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  for (int i = lane; i < np; i += 32) s += p[i].y * exp2f(p[i].x - base);
+  s = fb::warp_sum(s);
+  const int64_t t = target[r];
+  float l = 0.f;
+  if (t >= 0 && t < V)
+    for (int i = lane; i < D; i += 32)
+      l = fmaf(__uint_as_float((uint32_t)h[r * ldh + i] << 16), __uint_as_float((uint32_t)w[t * ldw + i] << 16), l);
+  l = fb::warp_sum(l);
+  if (lane) return;
+  const float z = (m + log2f(s)) * 0.69314718055994530942f;
+  lse[r] = z;
+  loss[r] = t < 0 ? 0.f : (t >= V ? NAN : z - l);
 }
 
 // One CTA per row: the piece's maximum and sum join the row's state; the
@@ -67,14 +100,10 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float *l, int64_t ldl, 
   loss[r] = t < 0 ? 0.f : (t >= V ? NAN : z - lt);
 }
 
-__device__ __forceinline__ void put(float *p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
-
-// G of one piece (G may be the logits themselves).  Rows held out of the loss
+// fp32 rows: G of one piece, in the logits' place.  Rows held out of the loss
 // are zeros whatever their logits are.
-template <typename T>
-__global__ void k_xent_grad(const float *l, int64_t ldl, int v0, int cols, int64_t V, const int64_t *target,
-                            const float *lse, const float *dloss, T *G, int64_t ldg) {
+__global__ void k_xent_grad(float *l, int64_t ldl, int v0, int cols, int64_t V, const int64_t *target, const float *lse,
+                            const float *dloss) {
   fb::pdl_enter();
   const int64_t r = blockIdx.x;
   const int64_t t = target[r];
@@ -83,13 +112,24 @@ __global__ void k_xent_grad(const float *l, int64_t ldl, int v0, int cols, int64
   for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < cols; c += gridDim.y * blockDim.x) {
     float v = 0.f;
     if (live) v = d * (expf(l[r * ldl + c] - z) - (t == v0 + c ? 1.f : 0.f));
-    put(G + r * ldg + c, v);
+    l[r * ldl + c] = v;
+  }
+}
+
+// bf16 rows: dst = src rounded.
+__global__ void k_round_rows(const float *src, int64_t lds, __nv_bfloat16 *dst, int64_t ldd, int64_t rows, int cols) {
+  fb::pdl_enter();
+  const int64_t total = rows * cols;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / cols;
+    const int c = (int)(i - r * cols);
+    dst[r * ldd + c] = __float2bfloat16_rn(src[r * lds + c]);
   }
 }
 
 // Table rows per piece: a multiple of 64, so that pieces start 16-byte aligned.
-int64_t piece_rows(int64_t n, int64_t V) {
-  const int64_t r = std::max<int64_t>(256, kPieceBytes / 4 / std::max<int64_t>(n, 1) / 64 * 64);
+int64_t piece_rows(int64_t n, int64_t V, int es) {
+  const int64_t r = std::max<int64_t>(256, kPieceBytes / es / std::max<int64_t>(n, 1) / 64 * 64);
   return std::min<int64_t>(r, round_up(V, 64));
 }
 
@@ -118,17 +158,14 @@ Mat rows_from(const Mat &m, int type, int64_t r) {
   return Mat{static_cast<const uint8_t *>(m.p) + r * m.ld * elem(type), m.ld};
 }
 
-int forward(Call &c, const fb_softmax_xent &a) {
-  Mat h, w;
-  FBH_TRY(aligned(c, a.type, Mat{a.h, a.ldh}, a.n, a.D, &h));
-  FBH_TRY(aligned(c, a.type, Mat{a.w, a.ldw}, a.V, a.D, &w));
-  const int64_t pr = piece_rows(a.n, a.V);
+int forward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
+  const int64_t pr = piece_rows(a.n, a.V, 4);
   FBH_TAKE(l, c, float, a.n * pr);
   FBH_TAKE(state, c, float, 2 * a.n);
   FBH_TAKE(tl, c, float, a.n);
   for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
     const int cols = (int)std::min<int64_t>(pr, a.V - v0);
-    FBH_TRY(product(c, a.type, FB_GEMM_NT, h, rows_from(w, a.type, v0), l, pr, a.n, cols, a.D, 0));
+    FBH_TRY(product(c, FB_GEMM_NT, h, rows_from(w, a.type, v0), l, pr, a.n, cols, a.D, 0));
     if (c.dry) break;                        // every piece takes the same workspace
     FB_TRY_CUDA(fb::launch(k_xent_rows, (unsigned)a.n, 256, 0, c.stream, (const float *)l, pr, (int)v0, cols, a.V,
                            a.target, state, tl, a.loss, a.lse, (int)(v0 == 0), (int)(v0 + pr >= a.V)));
@@ -137,57 +174,118 @@ int forward(Call &c, const fb_softmax_xent &a) {
   return FB_OK;
 }
 
-template <typename T> int backward(Call &c, const fb_softmax_xent &a) {
-  Mat h, w;
-  FBH_TRY(aligned(c, a.type, Mat{a.h, a.ldh}, a.n, a.D, &h));
-  FBH_TRY(aligned(c, a.type, Mat{a.w, a.ldw}, a.V, a.D, &w));
-  const int64_t pr = piece_rows(a.n, a.V);
+int backward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
+  const int64_t pr = piece_rows(a.n, a.V, 4);
   FBH_TAKE(l, c, float, a.n * pr);
-  T *G = reinterpret_cast<T *>(l);
-  float *dh = static_cast<float *>(a.dh), *dwt = nullptr;
-  int64_t lddh = a.lddh;
-  if (a.type != FB_F32) {
-    FBH_TAKE(gb, c, T, a.n * pr);
-    G = gb;
-    if (a.dh) {
-      FBH_TAKE(t, c, float, a.n * a.D);
-      dh = t, lddh = a.D;
+  for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
+    const int cols = (int)std::min<int64_t>(pr, a.V - v0);
+    const Mat wp = rows_from(w, a.type, v0), G{l, pr};
+    FBH_TRY(product(c, FB_GEMM_NT, h, wp, l, pr, a.n, cols, a.D, 0));
+    if (!c.dry) {
+      FB_TRY_CUDA(fb::launch(k_xent_grad, dim3((unsigned)a.n, (unsigned)std::min(64, (cols + 255) / 256)), 256, 0,
+                             c.stream, l, pr, (int)v0, cols, a.V, a.target, (const float *)a.lse, a.dloss));
+      FB_LAUNCHED("k_xent_grad");
     }
+    if (a.dh) FBH_TRY(product(c, FB_GEMM_NN, G, wp, static_cast<float *>(a.dh), a.lddh, a.n, a.D, cols, v0 > 0));
+    if (a.dw)
+      FBH_TRY(product(c, FB_GEMM_TN, G, h, static_cast<float *>(a.dw) + v0 * a.lddw, a.lddw, a.n, cols, a.D,
+                      a.accumulate));
+    // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
+    if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
-  if (a.dw && a.grad_type != FB_F32) {
-    FBH_TAKE(t, c, float, pr * a.D);
-    dwt = t;
+  return FB_OK;
+}
+
+// The common fields of a launch over the logits of rows h against table rows w.
+int logits_args(fbpair::PairArgs &p, const fb_softmax_xent &a, const Mat &h, int64_t n, const Mat &w, int cols) {
+  using namespace fbpair;
+  std::memset(&p, 0, sizeof(p));
+  p.phases = p.probs = p.splits = 1;
+  p.kb[0] = p.kper = tiles_of(a.D, BK);
+  p.mt = tiles_of(n, 256);
+  p.nt = tiles_of(cols, 256);
+  p.M = (int)n;
+  p.N = cols;
+  p.err = err_word();
+  FBH_TRY(make_map(&p.ta[0], h.p, n, a.D, h.ld, kHalfM));
+  return make_map(&p.tb[0], w.p, cols, a.D, w.ld, 128);
+}
+
+int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
+  using namespace fbpair;
+  const int nt = tiles_of(a.V, 256);
+  // rows per launch: the partials of one stay within kPieceBytes
+  const int64_t rows = std::min<int64_t>(a.n, std::max<int64_t>(256, kPieceBytes / (16ll * nt) / 256 * 256));
+  FBH_TAKE(part, c, float2, rows * 2 * nt);
+  if (c.dry) return FB_OK;
+  for (int64_t r0 = 0; r0 < a.n; r0 += rows) {
+    const int64_t n = std::min(rows, a.n - r0);
+    const Mat hp = rows_from(h, a.type, r0);
+    PairArgs p;
+    FBH_TRY(logits_args(p, a, hp, n, w, (int)a.V));
+    p.part = part;
+    FBH_TRY((launch_pair<kLse, false, false, 256>(p, c.stream)));
+    FB_TRY_CUDA(fb::launch(k_xent_finish, (unsigned)((n + 3) / 4), 128, 0, c.stream, (const float2 *)part, 2 * nt,
+                           static_cast<const uint16_t *>(hp.p), hp.ld, static_cast<const uint16_t *>(w.p), w.ld, a.D,
+                           a.V, a.target + r0, a.loss + r0, a.lse + r0, n));
+    FB_LAUNCHED("k_xent_finish");
+  }
+  return FB_OK;
+}
+
+int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
+  using namespace fbpair;
+  const int64_t pr = piece_rows(a.n, a.V, 2);
+  const bool sum = a.dh && pr < a.V;         // dh adds up over the pieces in fp32
+  FBH_TAKE(G, c, __nv_bfloat16, a.n * pr);
+  const int64_t lds = round_up(a.D, 4);
+  float *acc = nullptr;
+  if (sum) {
+    FBH_TAKE(t, c, float, a.n * lds);
+    acc = t;
   }
   for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
     const int cols = (int)std::min<int64_t>(pr, a.V - v0);
     const Mat wp = rows_from(w, a.type, v0), Gm{G, pr};
-    FBH_TRY(product(c, a.type, FB_GEMM_NT, h, wp, l, pr, a.n, cols, a.D, 0));
     if (!c.dry) {
-      FB_TRY_CUDA(fb::launch(k_xent_grad<T>, dim3((unsigned)a.n, (unsigned)std::min(64, (cols + 255) / 256)), 256, 0,
-                             c.stream, (const float *)l, pr, (int)v0, cols, a.V, a.target, (const float *)a.lse,
-                             a.dloss, G, pr));
-      FB_LAUNCHED("k_xent_grad");
+      PairArgs p;
+      FBH_TRY(logits_args(p, a, h, a.n, wp, cols));
+      p.target = a.target;
+      p.lse = a.lse;
+      p.dloss = a.dloss;
+      p.V = a.V;
+      p.v0 = v0;
+      p.has_tc = 1;
+      FBH_TRY(make_map(&p.tc[0], G, a.n, cols, pr, 32));
+      FBH_TRY((launch_pair<kProb, false, false, 256>(p, c.stream)));
     }
-    if (a.dh) FBH_TRY(product(c, a.type, FB_GEMM_NN, Gm, wp, dh, lddh, a.n, a.D, cols, v0 > 0));
+    if (a.dh) {
+      const Term t{wp, 0, cols};
+      FBH_TRY(pair_rows(c, Gm, a.n, cols, &t, 1, true, a.D,
+                        sum ? Out{acc, lds, FB_F32, v0 > 0} : Out{a.dh, a.lddh, FB_BF16, 0}));
+    }
     if (a.dw) {
-      if (dwt) {
-        FBH_TRY(product(c, a.type, FB_GEMM_TN, Gm, h, dwt, a.D, a.n, cols, a.D, 0));
-        FBH_TRY(store_rows(c, dwt, a.D, static_cast<uint8_t *>(a.dw) + v0 * a.lddw * elem(a.grad_type), a.lddw,
-                           a.grad_type, cols, a.D, 0));
-      } else {
-        FBH_TRY(product(c, a.type, FB_GEMM_TN, Gm, h, static_cast<float *>(a.dw) + v0 * a.lddw, a.lddw, a.n, cols,
-                        a.D, a.accumulate));
-      }
+      const Out o{static_cast<uint8_t *>(a.dw) + v0 * a.lddw * elem(a.grad_type), a.lddw, a.grad_type, a.accumulate};
+      FBH_TRY(pair_columns(c, Gm, a.n, cols, 0, 1, cols, h, a.D, &o));
     }
-    if (c.dry) break;
+    // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
+    if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
-  if (a.dh && a.type != FB_F32) FBH_TRY(store_rows(c, dh, lddh, a.dh, a.lddh, a.type, a.n, a.D, 0));
+  if (sum && !c.dry) {
+    const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>((a.n * a.D + 255) / 256, 148 * 16));
+    FB_TRY_CUDA(fb::launch(k_round_rows, blocks, 256, 0, c.stream, (const float *)acc, lds,
+                           static_cast<__nv_bfloat16 *>(a.dh), a.lddh, a.n, a.D));
+    FB_LAUNCHED("k_round_rows");
+  }
   return FB_OK;
 }
 
 int run(Call &c, const fb_softmax_xent &a, bool bwd) {
-  if (!bwd) return forward(c, a);
-  return a.type == FB_F32 ? backward<float>(c, a) : backward<__nv_bfloat16>(c, a);
+  Mat h, w;
+  FBH_TRY(aligned(c, a.type, Mat{a.h, a.ldh}, a.n, a.D, &h));
+  FBH_TRY(aligned(c, a.type, Mat{a.w, a.ldw}, a.V, a.D, &w));
+  if (a.type == FB_F32) return bwd ? backward_f32(c, a, h, w) : forward_f32(c, a, h, w);
+  return bwd ? backward_bf16(c, a, h, w) : forward_bf16(c, a, h, w);
 }
 
 }  // namespace
