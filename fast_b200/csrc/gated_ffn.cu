@@ -9,8 +9,8 @@
 // direction computes g and u side by side in one tile -- one CTA of the pair
 // stages Wg, the other Wu -- and for the backward dh beside them, and applies
 // the activation to the fp32 accumulators: h, dg, du are rounded once, and g,
-// u, dh never reach memory.  fp32: the grouped 3xTF32 products with the
-// activation between them.
+// u, dh never reach memory.  fp32: the same products over planes, with the
+// activation between them in a kernel of its own.
 #include "pair_gemm.cuh"
 
 namespace {
@@ -32,22 +32,39 @@ template <int ACT> __device__ __forceinline__ float2 act_exact(float g) {
   return make_float2(fmaxf(g, 0.f), g > 0.f ? 1.f : 0.f);
 }
 
-// h = act(g) u over n elements (pitches alike, padding included), in g's place.
-template <int ACT> __global__ void k_glu_fwd(float *g, const float *u, int64_t n) {
-  fb::pdl_enter();
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    g[i] = act_exact<ACT>(g[i]).x * u[i];
+// v as three bf16 planes `plane` elements apart (see k_operands).
+__device__ __forceinline__ void put3(uint16_t *p, int64_t plane, float v) {
+  const uint32_t b0 = __float_as_uint(v) & 0xFFFF0000u;
+  const bool fin = (b0 & 0x7F800000u) != 0x7F800000u;
+  const float r1 = fin ? v - __uint_as_float(b0) : 0.f;
+  const uint32_t b1 = __float_as_uint(r1) & 0xFFFF0000u;
+  p[0] = (uint16_t)(b0 >> 16);
+  p[plane] = (uint16_t)(b1 >> 16);
+  p[2 * plane] = (uint16_t)(__float_as_uint(r1 - __uint_as_float(b1)) >> 16);
 }
 
-// (dg, du, h) in the places of (g, u, dh).
-template <int ACT> __global__ void k_glu_bwd(float *g, float *u, float *dh, int64_t n) {
+// fp32: h = act(g) u over rows x Fp elements, as planes; gu rows are [g | u].
+template <int ACT> __global__ void k_glu_fwd(const float *gu, uint16_t *h, int64_t rows, int Fp) {
   fb::pdl_enter();
+  const int64_t n = rows * Fp;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const float uv = u[i], d = dh[i];
-    const float2 a = act_exact<ACT>(g[i]);
-    g[i] = d * uv * a.y;
-    u[i] = d * a.x;
-    dh[i] = a.x * uv;
+    const float *p = gu + i / Fp * 2 * Fp + i % Fp;
+    put3(h + i, n, act_exact<ACT>(p[0]).x * p[Fp]);
+  }
+}
+
+// fp32: h, and dgu rows [dg | du], as planes, from gu rows [g | u] and dh.
+template <int ACT>
+__global__ void k_glu_bwd(const float *gu, const float *dh, uint16_t *h, uint16_t *dgu, int64_t rows, int Fp) {
+  fb::pdl_enter();
+  const int64_t n = rows * Fp;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t at = i / Fp * 2 * Fp + i % Fp;
+    const float uv = gu[at + Fp], d = dh[i];
+    const float2 a = act_exact<ACT>(gu[at]);
+    put3(dgu + at, 2 * n, d * uv * a.y);
+    put3(dgu + at + Fp, 2 * n, d * a.x);
+    put3(h + i, n, a.x * uv);
   }
 }
 
@@ -77,45 +94,26 @@ int check(const fb_gated_ffn *a, bool bwd) {
   return FB_OK;
 }
 
-int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
-  const int64_t N = a.n, Fp = round_up(a.F, 4);
-  FBH_TAKE(g, c, float, N * Fp);
-  FBH_TAKE(u, c, float, N * Fp);
-  FBH_TRY(product(c, FB_GEMM_NT, x, wg, g, Fp, N, a.F, a.D, 0));
-  FBH_TRY(product(c, FB_GEMM_NT, x, wu, u, Fp, N, a.F, a.D, 0));
-  if (!c.dry) {
-    auto k = a.act == kSilu ? k_glu_fwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_fwd<FB_ACT_GELU> : k_glu_fwd<FB_ACT_RELU>);
-    FB_TRY_CUDA(fb::launch(k, blocks_for(N * Fp), 256, 0, c.stream, g, (const float *)u, N * Fp));
-    FB_LAUNCHED("k_glu_fwd");
-  }
-  return product(c, FB_GEMM_NT, Mat{g, Fp}, wd, static_cast<float *>(a.y), a.ldy, N, a.D, a.F, 0);
+// fp32: g | u [N, 2 Fp] (and dh), then the activation; the padding columns up
+// to Fp are zeros (weight rows past F read as zeros).
+int gate_up_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, float *gu, int64_t Fp) {
+  const Term g{wg, 0, a.D}, u{wu, 0, a.D};
+  FBH_TRY(pair_rows(c, x, a.n, a.D, &g, 1, false, (int)Fp, Out{gu, 2 * Fp, FB_F32, 0}, a.F));
+  return pair_rows(c, x, a.n, a.D, &u, 1, false, (int)Fp, Out{gu + Fp, 2 * Fp, FB_F32, 0}, a.F);
 }
 
-int backward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu,
-                 const Mat &wd) {
-  const int64_t N = a.n, Fp = round_up(a.F, 4);
-  FBH_TAKE(g, c, float, N * Fp);             // then dg
-  FBH_TAKE(u, c, float, N * Fp);             // then du
-  FBH_TAKE(d, c, float, N * Fp);             // dh, then h
-  FBH_TRY(product(c, FB_GEMM_NT, x, wg, g, Fp, N, a.F, a.D, 0));
-  FBH_TRY(product(c, FB_GEMM_NT, x, wu, u, Fp, N, a.F, a.D, 0));
-  FBH_TRY(product(c, FB_GEMM_NN, dy, wd, d, Fp, N, a.F, a.D, 0));
+int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
+  const int64_t Fp = round_up(a.F, 64);
+  FBH_TAKE(gu, c, float, a.n * 2 * Fp);
+  FBH_TAKE(h, c, uint16_t, 3 * a.n * Fp);
+  FBH_TRY(gate_up_f32(c, a, x, wg, wu, gu, Fp));
   if (!c.dry) {
-    auto k = a.act == kSilu ? k_glu_bwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_bwd<FB_ACT_GELU> : k_glu_bwd<FB_ACT_RELU>);
-    FB_TRY_CUDA(fb::launch(k, blocks_for(N * Fp), 256, 0, c.stream, g, u, d, N * Fp));
-    FB_LAUNCHED("k_glu_bwd");
+    auto k = a.act == kSilu ? k_glu_fwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_fwd<FB_ACT_GELU> : k_glu_fwd<FB_ACT_RELU>);
+    FB_TRY_CUDA(fb::launch(k, blocks_for(a.n * Fp), 256, 0, c.stream, (const float *)gu, h, a.n, (int)Fp));
+    FB_LAUNCHED("k_glu_fwd");
   }
-  if (a.dx) {
-    float *dx = static_cast<float *>(a.dx);
-    FBH_TRY(product(c, FB_GEMM_NN, Mat{g, Fp}, wg, dx, a.lddx, N, a.D, a.F, 0));
-    FBH_TRY(product(c, FB_GEMM_NN, Mat{u, Fp}, wu, dx, a.lddx, N, a.D, a.F, 1));
-  }
-  auto grad = [&](const Mat &G, const Mat &X, void *o, int64_t ld, int rows, int cols) {
-    return o ? product(c, FB_GEMM_TN, G, X, static_cast<float *>(o), ld, N, rows, cols, a.accumulate) : FB_OK;
-  };
-  FBH_TRY(grad(Mat{g, Fp}, x, a.dw_gate, a.ldd_gate, a.F, a.D));
-  FBH_TRY(grad(Mat{u, Fp}, x, a.dw_up, a.ldd_up, a.F, a.D));
-  return grad(dy, Mat{d, Fp}, a.dw_down, a.ldd_down, a.D, a.F);
+  const Term t{wd, 0, a.F};
+  return pair_rows(c, Mat{h, Fp, a.n * Fp}, a.n, a.F, &t, 1, false, a.D, Out{a.y, a.ldy, FB_F32, 0});
 }
 
 // g and u (and dh) of every tile, the activation in the epilogue: h [N, Fp],
@@ -159,28 +157,54 @@ int forward_bf16(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, co
   return pair_rows(c, Mat{h, Fp}, a.n, a.F, &t, 1, false, a.D, Out{a.y, a.ldy, FB_BF16, 0});
 }
 
+// dx and the weight gradients from h [n, Fp] and dgu [n, 2 Fp].
+int gradients(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu, const Mat &h,
+              const Mat &dgu, int64_t Fp) {
+  if (a.dx) {
+    const Term t[2] = {{wg, 0, a.F}, {wu, (int)Fp, a.F}};
+    FBH_TRY(pair_rows(c, dgu, a.n, (int)(2 * Fp), t, 2, true, a.D, Out{a.dx, a.lddx, a.type, 0}));
+  }
+  const Out og{a.dw_gate, a.ldd_gate, a.grad_type, a.accumulate}, ou{a.dw_up, a.ldd_up, a.grad_type, a.accumulate};
+  const Out both[2] = {og, ou};
+  if (a.dw_gate && a.dw_up) {
+    FBH_TRY(pair_columns(c, dgu, a.n, (int)(2 * Fp), (int)Fp, 2, a.F, x, a.D, both));
+  } else if (a.dw_gate) {
+    FBH_TRY(pair_columns(c, dgu, a.n, a.F, 0, 1, a.F, x, a.D, &og));
+  } else if (a.dw_up) {
+    const Mat du{static_cast<const uint16_t *>(dgu.p) + Fp, dgu.ld, dgu.plane};
+    FBH_TRY(pair_columns(c, du, a.n, a.F, 0, 1, a.F, x, a.D, &ou));
+  }
+  const Out od{a.dw_down, a.ldd_down, a.grad_type, a.accumulate};
+  if (a.dw_down) FBH_TRY(pair_columns(c, dy, a.n, a.D, 0, 1, a.D, h, a.F, &od));
+  return FB_OK;
+}
+
+int backward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu,
+                 const Mat &wd) {
+  const int64_t Fp = round_up(a.F, 64), n = a.n * Fp;
+  FBH_TAKE(gu, c, float, 2 * n);
+  FBH_TAKE(dh, c, float, n);
+  FBH_TAKE(h, c, uint16_t, 3 * n);
+  FBH_TAKE(dgu, c, uint16_t, 6 * n);
+  FBH_TRY(gate_up_f32(c, a, x, wg, wu, gu, Fp));
+  const Term t{wd, 0, a.D};
+  FBH_TRY(pair_rows(c, dy, a.n, a.D, &t, 1, true, (int)Fp, Out{dh, Fp, FB_F32, 0}, a.F));
+  if (!c.dry) {
+    auto k = a.act == kSilu ? k_glu_bwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_bwd<FB_ACT_GELU> : k_glu_bwd<FB_ACT_RELU>);
+    FB_TRY_CUDA(fb::launch(k, blocks_for(n), 256, 0, c.stream, (const float *)gu, (const float *)dh, h, dgu, a.n,
+                           (int)Fp));
+    FB_LAUNCHED("k_glu_bwd");
+  }
+  return gradients(c, a, x, dy, wg, wu, Mat{h, Fp, n}, Mat{dgu, 2 * Fp, 2 * n}, Fp);
+}
+
 int backward_bf16(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu,
                   const Mat &wd) {
   const int64_t Fp = round_up(a.F, 64);
   FBH_TAKE(h, c, __nv_bfloat16, a.n * Fp);
   FBH_TAKE(dgu, c, __nv_bfloat16, a.n * 2 * Fp);
   FBH_TRY(glu<fbpair::kGluBwd>(c, a, x, dy, wg, wu, wd, h, dgu, Fp));
-  if (a.dx) {
-    const Term t[2] = {{wg, 0, a.F}, {wu, (int)Fp, a.F}};
-    FBH_TRY(pair_rows(c, Mat{dgu, 2 * Fp}, a.n, (int)(2 * Fp), t, 2, true, a.D, Out{a.dx, a.lddx, FB_BF16, 0}));
-  }
-  const Out og{a.dw_gate, a.ldd_gate, a.grad_type, a.accumulate}, ou{a.dw_up, a.ldd_up, a.grad_type, a.accumulate};
-  const Out both[2] = {og, ou};
-  if (a.dw_gate && a.dw_up) {
-    FBH_TRY(pair_columns(c, Mat{dgu, 2 * Fp}, a.n, (int)(2 * Fp), (int)Fp, 2, a.F, x, a.D, both));
-  } else if (a.dw_gate) {
-    FBH_TRY(pair_columns(c, Mat{dgu, 2 * Fp}, a.n, a.F, 0, 1, a.F, x, a.D, &og));
-  } else if (a.dw_up) {
-    FBH_TRY(pair_columns(c, Mat{dgu + Fp, 2 * Fp}, a.n, a.F, 0, 1, a.F, x, a.D, &ou));
-  }
-  const Out od{a.dw_down, a.ldd_down, a.grad_type, a.accumulate};
-  if (a.dw_down) FBH_TRY(pair_columns(c, dy, a.n, a.D, 0, 1, a.D, Mat{h, Fp}, a.F, &od));
-  return FB_OK;
+  return gradients(c, a, x, dy, wg, wu, Mat{h, Fp}, Mat{dgu, 2 * Fp}, Fp);
 }
 
 // Weight gradients of a call without rows: zeros.
@@ -195,12 +219,11 @@ int empty_grads(const fb_gated_ffn &a, cudaStream_t st) {
 
 int run(Call &c, const fb_gated_ffn &a, bool bwd) {
   Mat x, wg, wu, wd, dy{};
-  FBH_TRY(aligned(c, a.type, Mat{a.x, a.ldx}, a.n, a.D, &x));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_gate, a.ld_gate}, a.F, a.D, &wg));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_up, a.ld_up}, a.F, a.D, &wu));
-  FBH_TRY(aligned(c, a.type, Mat{a.w_down, a.ld_down}, a.D, a.F, &wd));
+  const Operand ops[5] = {{Mat{a.x, a.ldx}, a.n, a.D, &x}, {Mat{a.w_gate, a.ld_gate}, a.F, a.D, &wg},
+                          {Mat{a.w_up, a.ld_up}, a.F, a.D, &wu}, {Mat{a.w_down, a.ld_down}, a.D, a.F, &wd},
+                          {Mat{a.dy, a.lddy}, a.n, a.D, &dy}};
+  FBH_TRY(operands(c, a.type, ops, bwd ? 5 : 4));
   if (!bwd) return a.type == FB_F32 ? forward_f32(c, a, x, wg, wu, wd) : forward_bf16(c, a, x, wg, wu, wd);
-  FBH_TRY(aligned(c, a.type, Mat{a.dy, a.lddy}, a.n, a.D, &dy));
   return a.type == FB_F32 ? backward_f32(c, a, x, dy, wg, wu, wd) : backward_bf16(c, a, x, dy, wg, wu, wd);
 }
 

@@ -29,20 +29,26 @@ struct Call {
   }
 };
 
-// A row-major matrix [rows, cols] of the operator's type.
+// A row-major matrix [rows, cols] of the operator's type; as an operand of the
+// products a bf16 matrix, or (plane > 0) the three bf16 planes of an fp32 one,
+// `plane` elements apart.
 struct Mat {
   const void *p;
   int64_t ld;
+  int64_t plane = 0;
 };
 
-// m as the products read it: 16-byte aligned base and pitch.  Copies into the
-// workspace when m is not.
-int aligned(Call &c, int type, const Mat &m, int64_t rows, int cols, Mat *out);
-
-// fp32: C (+)= A B^T (NT), A B (NN) or A^T B (TN: C [N, K] over M rows), as
-// fb_gemm_group defines them.
-int product(Call &c, int kind, const Mat &A, const Mat &B, float *C, int64_t ldc, int64_t M, int N, int K,
-            int accumulate);
+// The matrices of a call as the products read them: bf16 with a 16-byte
+// aligned base and pitch (copied into the workspace when they are not), fp32
+// split into planes; one launch for all of them.
+constexpr int kMaxOperands = 6;
+struct Operand {
+  Mat src;
+  int64_t rows;
+  int cols;
+  Mat *out;
+};
+int operands(Call &c, int type, const Operand *ops, int n);
 
 // Where a product goes: rows of fp32 or bf16, written, or (fp32) added to.
 struct Out {
@@ -51,16 +57,17 @@ struct Out {
   int type, accumulate;
 };
 
-// bf16 products on pairs of SMs (pair_gemm.cuh); operands as `aligned` leaves
-// them, fp32 accumulation, one rounding at the end.
+// Products on pairs of SMs (pair_gemm.cuh); operands as `operands` leaves
+// them, fp32 accumulation, one rounding at the end (planes: fp32 results).
 //   rows: C[m, n] = sum over 1 or 2 terms of A[m, ax_t + k] B_t(n, k), A [M, acols], k < K_t; B_t is [N, K_t], or
 //         [K_t, N] when b_mn.  ax_t is a multiple of 64.
 struct Term {
   Mat B;
   int ax, K;
 };
+//   b_n < N: B has only b_n of the N rows (columns); the rest of C is zeros.
 int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, int n_terms, bool b_mn, int N,
-              const Out &out);
+              const Out &out, int b_n = 0);
 //   columns: C_p[m, n] = sum over the `rows` rows r of A[r, p * aprob + m] B[r, n], m < M, n < N, for p < probs
 //         (1 or 2) outputs; A has acols columns.
 int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int probs, int M, const Mat &B, int N,

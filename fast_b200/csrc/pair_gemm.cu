@@ -56,9 +56,9 @@ constexpr int kMinStages = 4;
 struct Plan {
   int bn, splits, kper;
 };
-Plan plan_of(int64_t M, int N, int probs, int kb, bool may_split) {
+Plan plan_of(int64_t M, int N, int probs, int kb, bool may_split, bool planes) {
   const int slots = num_sms() / 2;
-  Plan p{N > 128 ? 256 : 128, 1, kb};
+  Plan p{N > 128 && !planes ? 256 : 128, 1, kb};
   const int64_t mt = tiles_of(M, 256);
   if (p.bn == 256 && mt * tiles_of(N, 256) * probs * 2 <= slots) p.bn = 128;
   const int64_t tiles = mt * tiles_of(N, p.bn) * probs;
@@ -72,14 +72,15 @@ Plan plan_of(int64_t M, int N, int probs, int kb, bool may_split) {
   return p;
 }
 
-template <bool A_MN, bool B_MN> int dispatch(const PairArgs &a, int bn, bool f32, cudaStream_t st) {
+template <bool A_MN, bool B_MN> int dispatch(const PairArgs &a, int bn, bool f32, bool planes, cudaStream_t st) {
+  if (planes) return launch_pair<kStoreF32, A_MN, B_MN, 128, 3>(a, st);
   if (f32)
     return bn == 256 ? launch_pair<kStoreF32, A_MN, B_MN, 256>(a, st) : launch_pair<kStoreF32, A_MN, B_MN, 128>(a, st);
   return bn == 256 ? launch_pair<kStoreBf16, A_MN, B_MN, 256>(a, st) : launch_pair<kStoreBf16, A_MN, B_MN, 128>(a, st);
 }
 
 // Fills the tiling and the outputs (or the partial results') of `a`, launches, sums the splits.
-template <bool A_MN, bool B_MN> int finish(Call &c, PairArgs &a, const Plan &p, int64_t M, int N, const Out *out) {
+template <bool A_MN, bool B_MN> int finish(Call &c, PairArgs &a, const Plan &p, bool planes, int64_t M, int N, const Out *out) {
   a.mt = tiles_of(M, 256);
   a.nt = tiles_of(N, p.bn);
   a.splits = p.splits;
@@ -112,10 +113,14 @@ template <bool A_MN, bool B_MN> int finish(Call &c, PairArgs &a, const Plan &p, 
   }
   if (p.splits == 1 && a.has_tc)
     for (int i = 0; i < a.probs; ++i) FBH_TRY(make_map(&a.tc[i], out[i].p, M, N, out[i].ld, 32, f32));
-  FBH_TRY((dispatch<A_MN, B_MN>(a, p.bn, f32, c.stream)));
+  FBH_TRY((dispatch<A_MN, B_MN>(a, p.bn, f32, planes, c.stream)));
   if (p.splits > 1)
     for (int i = 0; i < a.probs; ++i) FBH_TRY(sum_splits(c, P[i], prow * pld, pld, p.splits, out[i], M, N));
   return FB_OK;
+}
+
+int operand_map(CUtensorMap *m, const Mat &x, int64_t rows, int64_t cols, int box_rows) {
+  return x.plane ? make_map3(m, x.p, rows, cols, x.ld, x.plane, box_rows) : make_map(m, x.p, rows, cols, x.ld, box_rows);
 }
 
 }  // namespace
@@ -123,8 +128,9 @@ template <bool A_MN, bool B_MN> int finish(Call &c, PairArgs &a, const Plan &p, 
 namespace fbh {
 
 int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, int n_terms, bool b_mn, int N,
-              const Out &out) {
+              const Out &out, int b_n) {
   if (M == 0) return FB_OK;
+  if (!b_n) b_n = N;
   PairArgs a;
   std::memset(&a, 0, sizeof(a));
   a.phases = n_terms;
@@ -133,14 +139,14 @@ int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, in
     a.kb[t] = tiles_of(terms[t].K, BK);
     a.ax[t] = terms[t].ax;
   }
-  const Plan p = plan_of(M, N, 1, a.kb[0], n_terms == 1);
+  const Plan p = plan_of(M, N, 1, a.kb[0], n_terms == 1, A.plane > 0);
   if (!c.dry)
     for (int t = 0; t < n_terms; ++t) {
-      FBH_TRY(make_map(&a.ta[t], A.p, M, acols, A.ld, kHalfM));
-      if (b_mn) FBH_TRY(make_map(&a.tb[t], terms[t].B.p, terms[t].K, N, terms[t].B.ld, BK));
-      else FBH_TRY(make_map(&a.tb[t], terms[t].B.p, N, terms[t].K, terms[t].B.ld, p.bn / 2));
+      FBH_TRY(operand_map(&a.ta[t], A, M, acols, kHalfM));
+      if (b_mn) FBH_TRY(operand_map(&a.tb[t], terms[t].B, terms[t].K, b_n, BK));
+      else FBH_TRY(operand_map(&a.tb[t], terms[t].B, b_n, terms[t].K, p.bn / 2));
     }
-  return b_mn ? finish<false, true>(c, a, p, M, N, &out) : finish<false, false>(c, a, p, M, N, &out);
+  return b_mn ? finish<false, true>(c, a, p, A.plane > 0, M, N, &out) : finish<false, false>(c, a, p, A.plane > 0, M, N, &out);
 }
 
 int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int probs, int M, const Mat &B, int N,
@@ -151,12 +157,12 @@ int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int 
   a.probs = probs;
   a.aprob = aprob;
   a.kb[0] = tiles_of(rows, BK);
-  const Plan p = plan_of(M, N, probs, a.kb[0], true);
+  const Plan p = plan_of(M, N, probs, a.kb[0], true, A.plane > 0);
   if (!c.dry) {
-    FBH_TRY(make_map(&a.ta[0], A.p, rows, acols, A.ld, BK));
-    FBH_TRY(make_map(&a.tb[0], B.p, rows, N, B.ld, BK));
+    FBH_TRY(operand_map(&a.ta[0], A, rows, acols, BK));
+    FBH_TRY(operand_map(&a.tb[0], B, rows, N, BK));
   }
-  return finish<true, true>(c, a, p, M, N, out);
+  return finish<true, true>(c, a, p, A.plane > 0, M, N, out);
 }
 
 }  // namespace fbh

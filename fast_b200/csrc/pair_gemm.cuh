@@ -2,9 +2,15 @@
 // cta_group::2, operands by TMA, fp32 accumulators in tensor memory, and the
 // operators' own arithmetic in the epilogue.
 //
-//   kernel k_pair<EPI, A_MN, B_MN, BN>: C[m, n] = sum_k A(m, k) B(n, k)
+//   kernel k_pair<EPI, A_MN, B_MN, BN, P>: C[m, n] = sum_k A(m, k) B(n, k)
 //   A_MN / B_MN: the operand lies with its m (n) index contiguous (the matrix
 //   is stored [k][m]); else with k contiguous.
+//   P = 3: fp32 operands, each as three bf16 planes x = x0 + x1 + x2 of 8
+//   significant bits (exact: 24 bits in all).  Six of the nine plane products
+//   are summed, smallest first; the three left out are below 2^-24 of the
+//   product.  The tensor cores' accumulation truncates, so it runs over 64 k
+//   only: the epilogue warps add each such slab to an fp32 sum in registers
+//   while the next one is computed.
 //
 // A cluster of two CTAs works on a 256 x BN tile: each CTA stages 128 rows of
 // A and BN / 2 rows of B, the MMA of the even CTA reads both halves from both
@@ -124,6 +130,14 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
     }
   }
   return true;
+}
+// The same from plane z of a matrix kept as planes.
+__device__ __forceinline__ void load3(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
 // A tile of this CTA's shared memory, counted on a barrier of the even CTA.
 __device__ __forceinline__ void load2(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
@@ -364,8 +378,13 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
   }
 }
 
-template <int EPI, bool A_MN, bool B_MN, int BN>
+// Planes of the six products of P = 3, smallest first (one hex digit each, from the right).
+constexpr uint32_t kPlaneA = 0x001102u, kPlaneB = 0x010120u;
+
+template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(const __grid_constant__ PairArgs a) {
+  static_assert(P == 1 || (P == 3 && EPI == kStoreF32), "planes feed fp32 results");
+  constexpr int kPairs = P == 3 ? 6 : 1;
   constexpr int kStages = stages<EPI>(), kBufs = EPI == kGluBwd ? 1 : 2;
   constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd;      // B: 128 rows of Wg in one CTA, of Wu in the other
   static_assert(!kDual || BN == 256, "the gate and up columns fill a 256-column tile");
@@ -418,7 +437,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
           const int j1 = p == 0 ? q.k1 : a.kb[1];
           const uint32_t bytes = (uint32_t)(kABytes + bn / 2 * BK * 2);
           const bool bmn = dh || B_MN;
-          for (int j = p == 0 ? q.k0 : 0; j < j1; ++j) {
+          const int jb = p == 0 ? q.k0 : 0;
+          for (int i = jb * kPairs; i < j1 * kPairs; ++i) {
+            const int j = i / kPairs, za = (kPlaneA >> (4 * (i % kPairs))) & 15, zb = (kPlaneB >> (4 * (i % kPairs))) & 15;
             const int s = g % kStages;
             if (g >= (uint32_t)kStages && !wait(empty + s, ((g / kStages) - 1) & 1, abort_flag, err)) {
               stop = true;
@@ -426,22 +447,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
             }
             if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
             const uint32_t bar = leader_addr(full + s);
+            auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int z) {
+              if (P == 1) load2(dst, map, bar, x, y);
+              else load3(dst, map, bar, x, y, z);
+            };
             if (A_MN) {
 #pragma unroll
-              for (int i = 0; i < 2; ++i)
-                load2(sA(s) + i * kBox, &a.ta[p], bar, q.prob * a.aprob + m0 + 64 * i, BK * j);
+              for (int h = 0; h < 2; ++h)
+                load(sA(s) + h * kBox, &a.ta[p], q.prob * a.aprob + m0 + 64 * h, BK * j, za);
             } else {
-              load2(sA(s), &a.ta[p], bar, a.ax[p] + BK * j, m0);
+              load(sA(s), &a.ta[p], a.ax[p] + BK * j, m0, za);
             }
             if (kDual && !dh) {
-              load2(sB(s), &a.tb[rank], bar, BK * j, q.n * 128);
+              load(sB(s), &a.tb[rank], BK * j, q.n * 128, zb);
             } else {
               const CUtensorMap *mb = dh ? &a.tw : &a.tb[p];
               const int n0 = q.n * bn + (int)rank * (bn / 2);
               if (bmn) {
-                for (int i = 0; i < bn / 128; ++i) load2(sB(s) + i * kBox, mb, bar, n0 + 64 * i, BK * j);
+                for (int h = 0; h < bn / 128; ++h) load(sB(s) + h * kBox, mb, n0 + 64 * h, BK * j, zb);
               } else {
-                load2(sB(s), mb, bar, BK * j, n0);
+                load(sB(s), mb, BK * j, n0, zb);
               }
             }
             ++g;
@@ -454,38 +479,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
     }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
-      uint32_t g = 0, it = 0;
+      uint32_t g = 0, it = 0;                 // stages and accumulators used so far
       bool stop = false;
-      for (int t = first; t < total && !stop; t += step, ++it) {
+      for (int t = first; t < total && !stop; t += step) {
         const Tile q = tile_at(a, t);
-        const int buf = it % kBufs;
-        const uint32_t use = it / kBufs;
-        if (use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) break;
-        tc_fence_after();
         for (int p = 0; p < a.phases && !stop; ++p) {
           const bool dh = EPI == kGluBwd && p == 1;
           const bool bmn = dh || B_MN;
           const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(BN, A_MN, B_MN);
-          const uint32_t d = tmem + (dh ? 256u : (uint32_t)(buf * 256));
           const uint64_t adv_a = A_MN ? (2048 >> 4) : 2, adv_b = bmn ? (2048 >> 4) : 2;
-          const bool fresh = p == 0 || dh;    // the sum starts here
           const int j0 = p == 0 ? q.k0 : 0, j1 = p == 0 ? q.k1 : a.kb[1];
-          for (int j = j0; j < j1; ++j) {
+          for (int i = j0 * kPairs; i < j1 * kPairs; ++i) {
+            // a new accumulator: at the tile's start, or (planes) at every slab's
+            const bool fresh = P == 3 ? i % kPairs == 0 : (i == j0 && (p == 0 || dh));
+            const int buf = it % kBufs;
+            if (fresh && !dh) {
+              const uint32_t use = it / kBufs;
+              if (use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
+                stop = true;
+                break;
+              }
+              tc_fence_after();
+            }
             const int s = g % kStages;
             if (!wait(full + s, (g / kStages) & 1, abort_flag, err)) {
               stop = true;
               break;
             }
             tc_fence_after();
+            const uint32_t d = tmem + (dh ? 256u : (uint32_t)(buf * 256));
             const uint64_t ad = sdesc(smem_u32(sA(s)), A_MN), bd = sdesc(smem_u32(sB(s)), bmn);
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk)
-              mma2(d, ad + kk * adv_a, bd + kk * adv_b, idesc, (fresh && j == j0 && kk == 0) ? 0u : 1u);
+              mma2(d, ad + kk * adv_a, bd + kk * adv_b, idesc, (fresh && kk == 0) ? 0u : 1u);
             commit2(empty + s);
             ++g;
+            if (P == 3 ? (i + 1) % kPairs == 0 : (i + 1 == j1 && p + 1 == a.phases)) {
+              commit2(accf + buf);
+              ++it;
+            }
           }
         }
-        if (!stop) commit2(accf + buf);
       }
     }
     __syncwarp();
@@ -496,6 +530,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
     uint32_t it = 0;
     for (int t = first; t < total; t += step, ++it) {
       const Tile q = tile_at(a, t);
+      if constexpr (P == 3) {
+        const int row = q.m * 256 + (int)rank * kHalfM + qd * 32;
+        float acc[BN / 2];
+#pragma unroll
+        for (int i = 0; i < BN / 2; ++i) acc[i] = 0.f;
+        bool ok = true;
+        const int slabs = (q.k1 - q.k0) + (a.phases > 1 ? a.kb[1] : 0);
+        for (int k = 0; k < slabs && ok; ++k, ++it) {
+          const int buf = it % kBufs;
+          ok = __all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tb = tmem + tlane + (uint32_t)(buf * 256 + half * (BN / 2));
+#pragma unroll
+          for (int c = 0; c < BN / 2; c += 32) {
+            uint32_t r[32];
+            tmem_ld32_nowait(tb + c, r);
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[c + i] += __uint_as_float(r[i]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(leader_addr(acce + buf));
+        }
+        --it;                                 // the loop header counts one
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < BN / 2; c += 32) {
+          uint32_t r[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(acc[c + i]);
+          if (lane == 0) store_wait<0>();
+          __syncwarp();
+          stage_row(obuf, lane, r);
+          send<true>(a, q.prob, obuf, q.ybase, row, q.n * BN + half * (BN / 2) + c, lane);
+          __syncwarp();
+        }
+        continue;
+      }
       const int buf = it % kBufs;
       if (!__all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0)) break;
       tc_fence_after();
@@ -648,6 +722,22 @@ inline int make_map(CUtensorMap *m, const void *base, int64_t rows, int64_t cols
   return FB_OK;
 }
 
+// The same for the three planes of a matrix, `rows` rows each.
+inline int make_map3(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t ld, int64_t plane,
+                     int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fb::set_error(FB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 3};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(plane * 2)};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fb::set_error(FB_ERR_ARG, "tensor map rejected (alignment or stride)");
+  return FB_OK;
+}
+
 inline bool map_ok(const void *p, int64_t ld, int es) {
   return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * es)) & 15u) == 0;
 }
@@ -680,8 +770,8 @@ template <auto kernel> int pair_slots(int smem) {
   return s;
 }
 
-template <int EPI, bool A_MN, bool B_MN, int BN> int launch_pair(const PairArgs &a, cudaStream_t stream) {
-  constexpr auto k = k_pair<EPI, A_MN, B_MN, BN>;
+template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1> int launch_pair(const PairArgs &a, cudaStream_t stream) {
+  constexpr auto k = k_pair<EPI, A_MN, B_MN, BN, P>;
   constexpr int smem = smem_bytes<EPI>();
   const int slots = pair_slots<k>(smem);
   if (!slots) return fb::cuda_error(cudaGetLastError(), "k_pair shared memory");

@@ -7,9 +7,9 @@
 // joins them; the backward takes the table in pieces of as many rows as make a
 // G piece of kPieceBytes (so that it stays in the L2 between its three
 // products), computes G from the logits in the epilogue that would have stored
-// them, then adds G w to dh and writes G^T h.  fp32: the grouped 3xTF32
-// products over pieces of logits, the forward carrying each row's running
-// maximum and sum from piece to piece.
+// them, then adds G w to dh and writes G^T h.  fp32: the same products over
+// planes, pieces of logits in both directions, the forward carrying each
+// row's running maximum and sum from piece to piece.
 #include <cmath>
 #include "pair_gemm.cuh"
 
@@ -100,10 +100,10 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float *l, int64_t ldl, 
   loss[r] = t < 0 ? 0.f : (t >= V ? NAN : z - lt);
 }
 
-// fp32 rows: G of one piece, in the logits' place.  Rows held out of the loss
-// are zeros whatever their logits are.
-__global__ void k_xent_grad(float *l, int64_t ldl, int v0, int cols, int64_t V, const int64_t *target, const float *lse,
-                            const float *dloss) {
+// fp32 rows: G of one piece as three bf16 planes (see k_operands).  Rows held
+// out of the loss are zeros whatever their logits are.
+__global__ void k_xent_grad(const float *l, int64_t ldl, int v0, int cols, int64_t V, const int64_t *target,
+                            const float *lse, const float *dloss, uint16_t *G, int64_t plane) {
   fb::pdl_enter();
   const int64_t r = blockIdx.x;
   const int64_t t = target[r];
@@ -112,7 +112,13 @@ __global__ void k_xent_grad(float *l, int64_t ldl, int v0, int cols, int64_t V, 
   for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < cols; c += gridDim.y * blockDim.x) {
     float v = 0.f;
     if (live) v = d * (expf(l[r * ldl + c] - z) - (t == v0 + c ? 1.f : 0.f));
-    l[r * ldl + c] = v;
+    uint16_t *p = G + r * ldl + c;
+    const uint32_t b0 = __float_as_uint(v) & 0xFFFF0000u;
+    const float r1 = v - __uint_as_float(b0);
+    const uint32_t b1 = __float_as_uint(r1) & 0xFFFF0000u;
+    p[0] = (uint16_t)(b0 >> 16);
+    p[plane] = (uint16_t)(b1 >> 16);
+    p[2 * plane] = (uint16_t)(__float_as_uint(r1 - __uint_as_float(b1)) >> 16);
   }
 }
 
@@ -154,8 +160,11 @@ int check(const fb_softmax_xent *a, bool bwd) {
   return FB_OK;
 }
 
-Mat rows_from(const Mat &m, int type, int64_t r) {
-  return Mat{static_cast<const uint8_t *>(m.p) + r * m.ld * elem(type), m.ld};
+Mat rows_from(const Mat &m, int64_t r) { return Mat{static_cast<const uint16_t *>(m.p) + r * m.ld, m.ld, m.plane}; }
+
+int logits_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &wp, int cols, float *l, int64_t pr) {
+  const Term t{wp, 0, a.D};
+  return pair_rows(c, h, a.n, a.D, &t, 1, false, cols, Out{l, pr, FB_F32, 0});
 }
 
 int forward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
@@ -165,11 +174,14 @@ int forward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   FBH_TAKE(tl, c, float, a.n);
   for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
     const int cols = (int)std::min<int64_t>(pr, a.V - v0);
-    FBH_TRY(product(c, FB_GEMM_NT, h, rows_from(w, a.type, v0), l, pr, a.n, cols, a.D, 0));
-    if (c.dry) break;                        // every piece takes the same workspace
-    FB_TRY_CUDA(fb::launch(k_xent_rows, (unsigned)a.n, 256, 0, c.stream, (const float *)l, pr, (int)v0, cols, a.V,
-                           a.target, state, tl, a.loss, a.lse, (int)(v0 == 0), (int)(v0 + pr >= a.V)));
-    FB_LAUNCHED("k_xent_rows");
+    FBH_TRY(logits_f32(c, a, h, rows_from(w, v0), cols, l, pr));
+    if (!c.dry) {
+      FB_TRY_CUDA(fb::launch(k_xent_rows, (unsigned)a.n, 256, 0, c.stream, (const float *)l, pr, (int)v0, cols, a.V,
+                             a.target, state, tl, a.loss, a.lse, (int)(v0 == 0), (int)(v0 + pr >= a.V)));
+      FB_LAUNCHED("k_xent_rows");
+    }
+    // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
+    if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
   return FB_OK;
 }
@@ -177,20 +189,25 @@ int forward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
 int backward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   const int64_t pr = piece_rows(a.n, a.V, 4);
   FBH_TAKE(l, c, float, a.n * pr);
+  FBH_TAKE(G, c, uint16_t, 3 * a.n * pr);
   for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
     const int cols = (int)std::min<int64_t>(pr, a.V - v0);
-    const Mat wp = rows_from(w, a.type, v0), G{l, pr};
-    FBH_TRY(product(c, FB_GEMM_NT, h, wp, l, pr, a.n, cols, a.D, 0));
+    const Mat wp = rows_from(w, v0), Gm{G, pr, a.n * pr};
+    FBH_TRY(logits_f32(c, a, h, wp, cols, l, pr));
     if (!c.dry) {
       FB_TRY_CUDA(fb::launch(k_xent_grad, dim3((unsigned)a.n, (unsigned)std::min(64, (cols + 255) / 256)), 256, 0,
-                             c.stream, l, pr, (int)v0, cols, a.V, a.target, (const float *)a.lse, a.dloss));
+                             c.stream, (const float *)l, pr, (int)v0, cols, a.V, a.target, (const float *)a.lse, a.dloss,
+                             G, a.n * pr));
       FB_LAUNCHED("k_xent_grad");
     }
-    if (a.dh) FBH_TRY(product(c, FB_GEMM_NN, G, wp, static_cast<float *>(a.dh), a.lddh, a.n, a.D, cols, v0 > 0));
-    if (a.dw)
-      FBH_TRY(product(c, FB_GEMM_TN, G, h, static_cast<float *>(a.dw) + v0 * a.lddw, a.lddw, a.n, cols, a.D,
-                      a.accumulate));
-    // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
+    if (a.dh) {
+      const Term t{wp, 0, cols};
+      FBH_TRY(pair_rows(c, Gm, a.n, cols, &t, 1, true, a.D, Out{a.dh, a.lddh, FB_F32, v0 > 0}));
+    }
+    if (a.dw) {
+      const Out o{static_cast<float *>(a.dw) + v0 * a.lddw, a.lddw, FB_F32, a.accumulate};
+      FBH_TRY(pair_columns(c, Gm, a.n, cols, 0, 1, cols, h, a.D, &o));
+    }
     if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
   return FB_OK;
@@ -220,7 +237,7 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
   if (c.dry) return FB_OK;
   for (int64_t r0 = 0; r0 < a.n; r0 += rows) {
     const int64_t n = std::min(rows, a.n - r0);
-    const Mat hp = rows_from(h, a.type, r0);
+    const Mat hp = rows_from(h, r0);
     PairArgs p;
     FBH_TRY(logits_args(p, a, hp, n, w, (int)a.V));
     p.part = part;
@@ -246,7 +263,7 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
   }
   for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
     const int cols = (int)std::min<int64_t>(pr, a.V - v0);
-    const Mat wp = rows_from(w, a.type, v0), Gm{G, pr};
+    const Mat wp = rows_from(w, v0), Gm{G, pr};
     if (!c.dry) {
       PairArgs p;
       FBH_TRY(logits_args(p, a, h, a.n, wp, cols));
@@ -268,7 +285,6 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
       const Out o{static_cast<uint8_t *>(a.dw) + v0 * a.lddw * elem(a.grad_type), a.lddw, a.grad_type, a.accumulate};
       FBH_TRY(pair_columns(c, Gm, a.n, cols, 0, 1, cols, h, a.D, &o));
     }
-    // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
     if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
   if (sum && !c.dry) {
@@ -282,8 +298,8 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
 
 int run(Call &c, const fb_softmax_xent &a, bool bwd) {
   Mat h, w;
-  FBH_TRY(aligned(c, a.type, Mat{a.h, a.ldh}, a.n, a.D, &h));
-  FBH_TRY(aligned(c, a.type, Mat{a.w, a.ldw}, a.V, a.D, &w));
+  const Operand ops[2] = {{Mat{a.h, a.ldh}, a.n, a.D, &h}, {Mat{a.w, a.ldw}, a.V, a.D, &w}};
+  FBH_TRY(operands(c, a.type, ops, 2));
   if (a.type == FB_F32) return bwd ? backward_f32(c, a, h, w) : forward_f32(c, a, h, w);
   return bwd ? backward_bf16(c, a, h, w) : forward_bf16(c, a, h, w);
 }
