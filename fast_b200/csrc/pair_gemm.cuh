@@ -94,6 +94,15 @@ __device__ __forceinline__ uint32_t cta_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// One lane of the (converged) warp.  The loops around the single-lane work run
+// on all lanes: their values then are warp-uniform to the compiler, which an
+// MMA's descriptors have to be (in a one-lane branch every MMA cost 173 cycles
+// whatever its width).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -103,25 +112,18 @@ __device__ __forceinline__ uint32_t leader_addr(const void *p) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
   return a;
 }
+// Arrival from either CTA.  What it orders are tensor-memory reads, fenced by
+// tcgen05.fence before it, so the default CTA scope is enough; a cluster-scope
+// release or acquire here also waits for every global store in flight (2x the
+// time of the short products).
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// Wait for a phase whose arrivals come from both CTAs.
-__device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
+// mbar_wait whose first try, which mostly succeeds, reads no clock.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
-  if (try_wait_cluster(bar, parity)) return true;
+  if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!try_wait_cluster(bar, parity)) {
+  while (!mbar_try_wait(bar, parity)) {
     if (*abort_flag) return false;
     if (clock64() - t0 > kWaitCycles) {
       *abort_flag = 1;
@@ -398,7 +400,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
   uint32_t *holder = reinterpret_cast<uint32_t *>(acce + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -425,61 +427,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
   int32_t *err = a.err;
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t g = 0;
-      bool stop = false;
-      for (int t = first; t < total && !stop; t += step) {
-        const Tile q = tile_at(a, t);
-        const int m0 = q.m * 256 + (int)rank * kHalfM;
-        for (int p = 0; p < a.phases && !stop; ++p) {
-          const bool dh = EPI == kGluBwd && p == 1;
-          const int bn = dh ? 128 : BN;
-          const int j1 = p == 0 ? q.k1 : a.kb[1];
-          const uint32_t bytes = (uint32_t)(kABytes + bn / 2 * BK * 2);
-          const bool bmn = dh || B_MN;
-          const int jb = p == 0 ? q.k0 : 0;
-          for (int i = jb * kPairs; i < j1 * kPairs; ++i) {
-            const int j = i / kPairs, za = (kPlaneA >> (4 * (i % kPairs))) & 15, zb = (kPlaneB >> (4 * (i % kPairs))) & 15;
-            const int s = g % kStages;
-            if (g >= (uint32_t)kStages && !wait(empty + s, ((g / kStages) - 1) & 1, abort_flag, err)) {
+    const bool one = elect_one();
+    int s = 0;
+    uint32_t turn = 0;                        // turns of the ring so far
+    bool stop = false;
+    for (int t = first; t < total && !stop; t += step) {
+      const Tile q = tile_at(a, t);
+      const int m0 = q.m * 256 + (int)rank * kHalfM;
+      for (int p = 0; p < a.phases && !stop; ++p) {
+        const bool dh = EPI == kGluBwd && p == 1;
+        const int bn = dh ? 128 : BN;
+        const int j1 = p == 0 ? q.k1 : a.kb[1];
+        const uint32_t bytes = (uint32_t)(kABytes + bn / 2 * BK * 2);
+        const bool bmn = dh || B_MN;
+        const CUtensorMap *ma = &a.ta[p], *mb = dh ? &a.tw : (kDual ? &a.tb[rank] : &a.tb[p]);
+        const int ax = A_MN ? q.prob * a.aprob + m0 : a.ax[p];
+        const int n0 = kDual && !dh ? q.n * 128 : q.n * bn + (int)rank * (bn / 2);
+        for (int j = p == 0 ? q.k0 : 0; j < j1 && !stop; ++j)
+#pragma unroll 1
+          for (int pr = 0; pr < kPairs; ++pr) {
+            if (turn > 0 && !wait(empty + s, (turn - 1) & 1, abort_flag, err)) {
               stop = true;
               break;
             }
-            if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
-            const uint32_t bar = leader_addr(full + s);
-            auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int z) {
-              if (P == 1) load2(dst, map, bar, x, y);
-              else load3(dst, map, bar, x, y, z);
-            };
-            if (A_MN) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                load(sA(s) + h * kBox, &a.ta[p], q.prob * a.aprob + m0 + 64 * h, BK * j, za);
-            } else {
-              load(sA(s), &a.ta[p], a.ax[p] + BK * j, m0, za);
-            }
-            if (kDual && !dh) {
-              load(sB(s), &a.tb[rank], BK * j, q.n * 128, zb);
-            } else {
-              const CUtensorMap *mb = dh ? &a.tw : &a.tb[p];
-              const int n0 = q.n * bn + (int)rank * (bn / 2);
-              if (bmn) {
-                for (int h = 0; h < bn / 128; ++h) load(sB(s) + h * kBox, mb, n0 + 64 * h, BK * j, zb);
+            if (one) {
+              const int za = (kPlaneA >> (4 * pr)) & 15, zb = (kPlaneB >> (4 * pr)) & 15;
+              uint8_t *sa = sA(s), *sb = sB(s);
+              const uint32_t full_at = leader_addr(full + s);
+              if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
+              auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int z) {
+                if (P == 1) load2(dst, map, full_at, x, y);
+                else load3(dst, map, full_at, x, y, z);
+              };
+              if (A_MN) {
+                load(sa, ma, ax, BK * j, za);
+                load(sa + kBox, ma, ax + 64, BK * j, za);
               } else {
-                load(sB(s), mb, BK * j, n0, zb);
+                load(sa, ma, ax + BK * j, m0, za);
+              }
+              if (bmn) {
+                load(sb, mb, n0, BK * j, zb);
+                if (bn == 256) load(sb + kBox, mb, n0 + 64, BK * j, zb);
+              } else {
+                load(sb, mb, BK * j, n0, zb);
               }
             }
-            ++g;
+            __syncwarp();
+            if (++s == kStages) s = 0, ++turn;
           }
-        }
       }
-      // the MMAs have read every stage (and their arrivals reached this CTA) before it leaves
-      for (uint32_t h = g > (uint32_t)kStages ? g - kStages : 0; h < g && !stop; ++h)
-        if (!wait(empty + h % kStages, (h / kStages) & 1, abort_flag, err)) stop = true;
+    }
+    // the MMAs have read every stage (and their arrivals reached this CTA) before it leaves
+    for (int k = 0; k < kStages && !stop; ++k) {
+      if (turn > 0 && !wait(empty + s, (turn - 1) & 1, abort_flag, err)) stop = true;
+      if (++s == kStages) s = 0, ++turn;
     }
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
-      uint32_t g = 0, it = 0;                 // stages and accumulators used so far
+    if (rank == 0) {
+      const bool one = elect_one();
+      const uint64_t ad0 = sdesc(smem_u32(smem), A_MN), bd_k = sdesc(smem_u32(smem + kABytes), false),
+                     bd_mn = sdesc(smem_u32(smem + kABytes), true);
+      int s = 0;
+      uint32_t turn = 0, it = 0;              // turns of the ring, accumulators used so far
       bool stop = false;
       for (int t = first; t < total && !stop; t += step) {
         const Tile q = tile_at(a, t);
@@ -487,38 +496,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
           const bool dh = EPI == kGluBwd && p == 1;
           const bool bmn = dh || B_MN;
           const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(BN, A_MN, B_MN);
-          const uint64_t adv_a = A_MN ? (2048 >> 4) : 2, adv_b = bmn ? (2048 >> 4) : 2;
+          const uint64_t adv_a = A_MN ? (2048 >> 4) : 2, adv_b = bmn ? (2048 >> 4) : 2, bd0 = bmn ? bd_mn : bd_k;
           const int j0 = p == 0 ? q.k0 : 0, j1 = p == 0 ? q.k1 : a.kb[1];
-          for (int i = j0 * kPairs; i < j1 * kPairs; ++i) {
-            // a new accumulator: at the tile's start, or (planes) at every slab's
-            const bool fresh = P == 3 ? i % kPairs == 0 : (i == j0 && (p == 0 || dh));
-            const int buf = it % kBufs;
-            if (fresh && !dh) {
-              const uint32_t use = it / kBufs;
-              if (use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
+          for (int j = j0; j < j1 && !stop; ++j)
+#pragma unroll 1
+            for (int pr = 0; pr < kPairs; ++pr) {
+              // a new accumulator: at the tile's start, or (planes) at every slab's
+              const bool fresh = P == 3 ? pr == 0 : (j == j0 && (p == 0 || dh));
+              const uint32_t buf = it % kBufs, use = it / kBufs;
+              if (fresh && !dh && use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
+                stop = true;
+                break;
+              }
+              if (!wait(full + s, turn & 1, abort_flag, err)) {
                 stop = true;
                 break;
               }
               tc_fence_after();
-            }
-            const int s = g % kStages;
-            if (!wait(full + s, (g / kStages) & 1, abort_flag, err)) {
-              stop = true;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t d = tmem + (dh ? 256u : (uint32_t)(buf * 256));
-            const uint64_t ad = sdesc(smem_u32(sA(s)), A_MN), bd = sdesc(smem_u32(sB(s)), bmn);
+              const bool last = P == 3 ? pr + 1 == kPairs : (j + 1 == j1 && p + 1 == a.phases);
+              if (one) {
+                const uint32_t d = tmem + (dh ? 256u : buf * 256u);
+                const uint64_t at = (uint64_t)(s * (kStageBytes >> 4));
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk)
-              mma2(d, ad + kk * adv_a, bd + kk * adv_b, idesc, (fresh && kk == 0) ? 0u : 1u);
-            commit2(empty + s);
-            ++g;
-            if (P == 3 ? (i + 1) % kPairs == 0 : (i + 1 == j1 && p + 1 == a.phases)) {
-              commit2(accf + buf);
-              ++it;
+                for (int kk = 0; kk < BK / 16; ++kk)
+                  mma2(d, ad0 + at + kk * adv_a, bd0 + at + kk * adv_b, idesc, (fresh && kk == 0) ? 0u : 1u);
+                commit2(empty + s);
+                if (last) commit2(accf + buf);
+              }
+              __syncwarp();
+              if (last) ++it;
+              if (++s == kStages) s = 0, ++turn;
             }
-          }
         }
       }
     }
