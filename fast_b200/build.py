@@ -3,6 +3,7 @@
   fast_b200/libfast_b200.so       C ABI + sm_100a kernels   (nvcc)
   fast_b200/_ext/fastAgg.so       drop-in fastAgg module     (g++ + libtorch)
   fast_b200/_ext/sampler_core.so  drop-in sampler_core       (g++ + libtorch)
+  fast_b200/_ext/head_ops.so      node-ranking head wrappers (g++ + libtorch)
 
 Every target is rebuilt only when one of its sources is newer.  nvcc
 cross-compiles for sm_100a, so this runs on machines without a GPU.
@@ -100,6 +101,7 @@ def build_all(verbose=False):
     build_lib(verbose)
     build_shim("fastAgg", os.path.join(SHIM, "fastagg.cpp"), verbose)
     build_shim("sampler_core", os.path.join(SHIM, "sampler_core.cpp"), verbose)
+    build_shim("head_ops", os.path.join(SHIM, "head_ops.cpp"), verbose)
 
 
 if __name__ == "__main__":

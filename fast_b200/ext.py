@@ -1,4 +1,5 @@
-"""Imports the in-tree drop-in modules ``fastAgg`` and ``sampler_core``.
+"""Imports the in-tree drop-in modules ``fastAgg`` and ``sampler_core``, and
+``head_ops``, the torch-level calls of the node-ranking head (``ops`` wraps it).
 
 They are built into ``fast_b200/_ext`` (``python -m fast_b200.build``).
 ``install_dropin()`` puts that directory on ``sys.path`` so unmodified
@@ -34,3 +35,4 @@ def _load(name):
 
 fastAgg = _load("fastAgg")
 sampler_core = _load("sampler_core")
+head_ops = _load("head_ops")

@@ -11,7 +11,8 @@ import os
 
 import torch
 
-from .capi import ACTS, BF16, F32, GatedFfn, SoftmaxXent, call, ptr, stream_ptr, lib
+from .capi import ACTS, call, ptr, stream_ptr, lib
+from .ext import head_ops
 
 
 class KernelTimer:
@@ -678,62 +679,27 @@ def attn_bwd(q, k, v, rptr, att, dagg, heads, slope, drop_p=0.0, seed=0, offset=
 
 
 # ---- node-ranking head: layer norm, gated feed-forward block, softmax cross entropy over all nodes ----
-_HEAD_TYPES = {torch.float32: F32, torch.bfloat16: BF16}
-
-
-def _head_rows(t, name, dtype, shape=None):
-    """Checks a matrix of the head's operators: CUDA, of `dtype`, rows of unit
-    column stride that do not overlap, of `shape` when given."""
-    if t.dtype != dtype or t.dim() != 2 or not t.is_cuda:
-        raise ValueError("%s must be a CUDA %s matrix" % (name, dtype))
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError("%s must have shape %s, not %s" % (name, shape, tuple(t.shape)))
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError("%s must have unit column stride" % name)
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError("%s must have rows that do not overlap" % name)
-
-
-def _ld(t):
-    """Leading dimension of a matrix (a single row's stride says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
-
-
-def _head_type(t, name):
-    try:
-        return _HEAD_TYPES[t.dtype]
-    except KeyError:
-        raise ValueError("%s must be fp32 or bf16" % name) from None
-
-
-def _norm_params(x, gamma, beta, name):
-    for t in (gamma, beta):
-        if t is not None and (t.dtype not in (torch.float32, x.dtype) or t.dtype != gamma.dtype or not t.is_cuda
-                              or t.dim() != 1 or t.shape[0] != x.shape[1] or not t.is_contiguous()):
-            raise ValueError("%s: gamma and beta must be contiguous CUDA vectors of the row width, fp32 or of the "
-                             "rows' type" % name)
-    return F32 if gamma.dtype == torch.float32 else BF16
+# The calls go through the head_ops module (argument checks, outputs and
+# workspaces in C++): operands of the wrong type, shape, layout or device raise
+# ValueError.
+def _head_call(name, kernels, nbytes, flops, *args):
+    fn = getattr(head_ops, name)
+    if TIMER is None and not NVTX:
+        LAUNCHES[0] += kernels
+        return fn(*args)
+    out = []
+    _launch(name, nbytes, flops, kernels, lambda: out.append(fn(*args)))
+    return out[-1]
 
 
 def layer_norm_fwd(x, gamma, beta=None, eps=1e-5, res=None):
     """Layer norm of rows x [n, D] (fp32 or bf16, any row pitch), statistics
     in fp32.  Returns (y, mean, rstd); with a residual `res` it normalises
-    s = x + res, kept in the rows' type, and returns (y, s, mean, rstd)."""
-    ty = _head_type(x, "layer_norm_fwd x")
-    _head_rows(x, "layer_norm_fwd x", x.dtype)
-    pt = _norm_params(x, gamma, beta, "layer_norm_fwd")
-    n, D = x.shape
-    y = torch.empty(n, D, device=x.device, dtype=x.dtype)
-    stats = torch.empty(2, n, device=x.device, dtype=torch.float32)
-    s, ldr = None, 0
-    if res is not None:
-        _head_rows(res, "layer_norm_fwd res", x.dtype, (n, D))
-        s, ldr = torch.empty_like(y), _ld(res)
-    mean = stats.data_ptr()
-    _launch("layer_norm_fwd", x.element_size() * n * D * (2 if res is None else 4), 8 * n * D, 1,
-            lambda: call("fb_layer_norm_fwd", ty, x.data_ptr(), _ld(x), ptr(res), ldr, gamma.data_ptr(), ptr(beta), pt,
-                         eps, ptr(s), D, y.data_ptr(), D, mean, mean + 4 * n, n, D, stream_ptr()))
-    return (y, stats[0], stats[1]) if res is None else (y, s, stats[0], stats[1])
+    s = x + res, kept in the rows' type, and returns (y, s, mean, rstd).
+    gamma and beta are fp32 or of the rows' type."""
+    m = x.numel()
+    return _head_call("layer_norm_fwd", 1, x.element_size() * m * (2 if res is None else 4), 8 * m, x, gamma, beta, eps,
+                      res)
 
 
 def layer_norm_bwd(dy, x, gamma, mean, rstd, ds=None, dgamma=None, dbeta=None):
@@ -741,53 +707,16 @@ def layer_norm_bwd(dy, x, gamma, mean, rstd, ds=None, dgamma=None, dbeta=None):
     when there was a residual): returns (dx, dgamma, dbeta).  dx, the gradient
     of x and of res alike, includes ds, the gradient that reaches s on its own.
     dgamma / dbeta have gamma's type; fp32 vectors given are accumulated into."""
-    ty = _head_type(x, "layer_norm_bwd x")
-    _head_rows(x, "layer_norm_bwd x", x.dtype)
-    n, D = x.shape
-    _head_rows(dy, "layer_norm_bwd dy", x.dtype, (n, D))
-    pt = _norm_params(x, gamma, None, "layer_norm_bwd")
-    for t in (mean, rstd):
-        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
-            raise ValueError("layer_norm_bwd: mean and rstd must be contiguous CUDA fp32 vectors, one value a row")
-    if ds is not None:
-        _head_rows(ds, "layer_norm_bwd ds", x.dtype, (n, D))
-    acc = dgamma is not None or dbeta is not None
-    if acc:
-        for t in (dgamma, dbeta):
-            if t is None or t.dtype != torch.float32 or pt != F32 or t.numel() != D or not t.is_contiguous():
-                raise ValueError("layer_norm_bwd: dgamma and dbeta to accumulate into must be given together, as "
-                                 "contiguous fp32 vectors beside an fp32 gamma")
-    else:
-        dgamma, dbeta = torch.empty(2, D, device=x.device, dtype=gamma.dtype)
-    dx = torch.empty(n, D, device=x.device, dtype=x.dtype)
-    nb = int(lib.fb_layer_norm_bwd_ws_bytes(n, D))
-    ws = torch.empty(nb, device=x.device, dtype=torch.uint8)
-    _launch("layer_norm_bwd", x.element_size() * n * D * (3 if ds is None else 4), 10 * n * D, 2,
-            lambda: call("fb_layer_norm_bwd", ty, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), gamma.data_ptr(), pt,
-                         mean.data_ptr(), rstd.data_ptr(), ptr(ds), 0 if ds is None else _ld(ds), dx.data_ptr(), D,
-                         dgamma.data_ptr(), dbeta.data_ptr(), int(acc), n, D, ws.data_ptr(), nb, stream_ptr()))
-    return dx, dgamma, dbeta
+    m = x.numel()
+    return _head_call("layer_norm_bwd", 2, x.element_size() * m * (3 if ds is None else 4), 10 * m, dy, x, gamma, mean,
+                      rstd, ds, dgamma, dbeta)
 
 
-def _ffn_args(x, w_gate, w_up, w_down, act, name):
-    ty = _head_type(x, name + " x")
-    if act not in ACTS:
-        raise ValueError("%s: act must be one of %s" % (name, ", ".join(sorted(ACTS))))
-    _head_rows(x, name + " x", x.dtype)
-    n, D = x.shape
-    Fw = w_gate.shape[0]
-    _head_rows(w_gate, name + " w_gate", x.dtype, (Fw, D))
-    _head_rows(w_up, name + " w_up", x.dtype, (Fw, D))
-    _head_rows(w_down, name + " w_down", x.dtype, (D, Fw))
-    return GatedFfn(ty, ACTS[act], ty, 0, n, D, Fw, x.data_ptr(), _ld(x), w_gate.data_ptr(), _ld(w_gate),
-                    w_up.data_ptr(), _ld(w_up), w_down.data_ptr(), _ld(w_down))
-
-
-def _head_call(name, a, backward, dev, nbytes, flops, kernels):
-    nb = int(getattr(lib, "fb_%s_ws_bytes" % name)(a, backward))
-    ws = torch.empty(nb, device=dev, dtype=torch.uint8)
-    fn = "fb_%s_%s" % (name, "bwd" if backward else "fwd")
-    _launch(fn[3:], nbytes, flops, kernels, lambda: call(fn, a, ws.data_ptr(), nb, stream_ptr()))
+def _act(act):
+    try:
+        return ACTS[act]
+    except (KeyError, TypeError):
+        raise ValueError("gated_ffn: act must be one of %s" % ", ".join(sorted(ACTS))) from None
 
 
 def gated_ffn_fwd(x, w_gate, w_up, w_down, act="silu"):
@@ -795,52 +724,18 @@ def gated_ffn_fwd(x, w_gate, w_up, w_down, act="silu"):
     weights w_gate, w_up [F, D], w_down [D, F], all fp32 or all bf16 (any row
     pitch).  act: "silu", "gelu" (erf form) or "relu".  Products accumulate
     in fp32; the backward needs nothing but the inputs."""
-    a = _ffn_args(x, w_gate, w_up, w_down, act, "gated_ffn_fwd")
-    y = torch.empty(a.n, a.D, device=x.device, dtype=x.dtype)
-    a.y, a.ldy = y.data_ptr(), a.D
-    es = x.element_size()
-    _head_call("gated_ffn", a, 0, x.device, es * a.D * (2 * a.n + 3 * a.F), 6 * a.n * a.D * a.F, 2)
-    return y
-
-
-def _grad_buffers(given, shapes, like, name):
-    """Weight gradients: fresh ones of the weights' type, or the fp32 buffers
-    given (accumulated into).  Returns (tensors, type, accumulate)."""
-    if given is None:
-        return [torch.empty(s, device=like.device, dtype=like.dtype) for s in shapes], _HEAD_TYPES[like.dtype], 0
-    if len(given) != len(shapes):
-        raise ValueError("%s: %d gradient buffers expected" % (name, len(shapes)))
-    for t, s in zip(given, shapes):
-        _head_rows(t, name + " gradient buffer", torch.float32, s)
-    return list(given), F32, 1
+    m, w = x.numel(), w_gate.numel()
+    return _head_call("gated_ffn_fwd", 2, x.element_size() * (2 * m + 3 * w), 6 * m * w_gate.shape[0], x, w_gate, w_up,
+                      w_down, _act(act))
 
 
 def gated_ffn_bwd(dy, x, w_gate, w_up, w_down, act="silu", grads=None):
     """Gradients of gated_ffn_fwd: (dx, dw_gate, dw_up, dw_down).  The weight
     gradients have the weights' type; `grads`, three fp32 buffers, are
     accumulated into instead (a flat gradient buffer's views)."""
-    a = _ffn_args(x, w_gate, w_up, w_down, act, "gated_ffn_bwd")
-    n, D, Fw = a.n, a.D, a.F
-    _head_rows(dy, "gated_ffn_bwd dy", x.dtype, (n, D))
-    dx = torch.empty(n, D, device=x.device, dtype=x.dtype)
-    dw, a.grad_type, a.accumulate = _grad_buffers(grads, [(Fw, D), (Fw, D), (D, Fw)], x, "gated_ffn_bwd")
-    a.dy, a.lddy, a.dx, a.lddx = dy.data_ptr(), _ld(dy), dx.data_ptr(), D
-    a.dw_gate, a.ldd_gate, a.dw_up, a.ldd_up = dw[0].data_ptr(), _ld(dw[0]), dw[1].data_ptr(), _ld(dw[1])
-    a.dw_down, a.ldd_down = dw[2].data_ptr(), _ld(dw[2])
-    _head_call("gated_ffn", a, 1, x.device, x.element_size() * D * (3 * n + 6 * Fw), 16 * n * D * Fw, 4)
-    return dx, dw[0], dw[1], dw[2]
-
-
-def _xent_args(h, w, target, name):
-    ty = _head_type(h, name + " h")
-    _head_rows(h, name + " h", h.dtype)
-    n, D = h.shape
-    V = w.shape[0]
-    _head_rows(w, name + " w", h.dtype, (V, D))
-    if target.dtype != torch.int64 or target.dim() != 1 or target.shape[0] != n or not target.is_cuda \
-            or not target.is_contiguous():
-        raise ValueError("%s: target must be a contiguous CUDA int64 vector, one entry a row" % name)
-    return SoftmaxXent(ty, ty, 0, D, n, V, h.data_ptr(), _ld(h), w.data_ptr(), _ld(w), target.data_ptr())
+    m, w = x.numel(), w_gate.numel()
+    return _head_call("gated_ffn_bwd", 4, x.element_size() * (3 * m + 6 * w), 16 * m * w_gate.shape[0], dy, x, w_gate,
+                      w_up, w_down, _act(act), grads)
 
 
 def softmax_xent_fwd(h, w, target):
@@ -848,28 +743,17 @@ def softmax_xent_fwd(h, w, target):
     w [V, D] (both fp32 or both bf16), without keeping the logits: returns
     (loss, lse), fp32 [n].  A negative target holds its row out of the loss
     (loss 0); one >= V gives a NaN loss."""
-    a = _xent_args(h, w, target, "softmax_xent_fwd")
-    n = a.n
-    out = torch.empty(2, n, device=h.device, dtype=torch.float32)
-    a.loss, a.lse = out.data_ptr(), out.data_ptr() + 4 * n
-    _head_call("softmax_xent", a, 0, h.device, h.element_size() * a.D * (n + a.V) + 16 * n, 2 * n * a.D * a.V, 2)
-    return out[0], out[1]
+    m, k = h.numel(), w.numel()
+    return _head_call("softmax_xent_fwd", 2, h.element_size() * (m + k) + 16 * h.shape[0], 2 * m * w.shape[0], h, w,
+                      target)
 
 
 def softmax_xent_bwd(h, w, target, lse, dloss, dw=None):
     """Gradients of softmax_xent_fwd for dloss [n] (fp32): (dh, dw), of the
     inputs' type; an fp32 buffer given as dw is accumulated into instead."""
-    a = _xent_args(h, w, target, "softmax_xent_bwd")
-    n, D, V = a.n, a.D, a.V
-    for t in (lse, dloss):
-        if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or not t.is_cuda:
-            raise ValueError("softmax_xent_bwd: lse and dloss must be contiguous CUDA fp32 vectors, one entry a row")
-    dh = torch.empty(n, D, device=h.device, dtype=h.dtype)
-    (dw,), a.grad_type, a.accumulate = _grad_buffers(None if dw is None else [dw], [(V, D)], h, "softmax_xent_bwd")
-    a.lse, a.dloss = lse.data_ptr(), dloss.data_ptr()
-    a.dh, a.lddh, a.dw, a.lddw = dh.data_ptr(), D, dw.data_ptr(), _ld(dw)
-    _head_call("softmax_xent", a, 1, h.device, h.element_size() * D * 2 * (n + V) + 16 * n, 6 * n * D * V, 3)
-    return dh, dw
+    m, k = h.numel(), w.numel()
+    return _head_call("softmax_xent_bwd", 3, 2 * h.element_size() * (m + k) + 16 * h.shape[0], 6 * m * w.shape[0], h, w,
+                      target, lse, dloss, dw)
 
 
 class AttentionCore(torch.autograd.Function):
