@@ -97,9 +97,9 @@ int check(const fb_gated_ffn *a, bool bwd) {
 // fp32: g | u [N, 2 Fp] (and dh), then the activation; the padding columns up
 // to Fp are zeros (weight rows past F read as zeros).
 int gate_up_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, float *gu, int64_t Fp) {
-  const Term g{wg, 0, a.D}, u{wu, 0, a.D};
-  FBH_TRY(pair_rows(c, x, a.n, a.D, &g, 1, false, (int)Fp, Out{gu, 2 * Fp, FB_F32, 0}, a.F));
-  return pair_rows(c, x, a.n, a.D, &u, 1, false, (int)Fp, Out{gu + Fp, 2 * Fp, FB_F32, 0}, a.F);
+  const Mat w[2] = {wg, wu};
+  const Out o[2] = {{gu, 2 * Fp, FB_F32, 0}, {gu + Fp, 2 * Fp, FB_F32, 0}};
+  return pair_rows2(c, x, a.n, w, a.D, (int)Fp, o, a.F);
 }
 
 int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
@@ -128,7 +128,8 @@ int glu(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &
   std::memset(&p, 0, sizeof(p));
   p.phases = EPI == kGluBwd ? 2 : 1;
   p.probs = p.splits = 1;
-  p.kb[0] = p.kb[1] = p.kper = tiles_of(a.D, BK);
+  p.kb[0] = p.kb[1] = tiles_of(a.D, BK);
+  p.kper = p.phases * p.kb[0];
   p.mt = tiles_of(a.n, 256);
   p.nt = tiles_of(Fp, 128);
   p.M = (int)a.n;

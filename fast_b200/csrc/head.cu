@@ -62,7 +62,8 @@ int operands(Call &c, int type, const Operand *ops, int n) {
     const Operand &o = ops[i];
     *o.out = Mat{o.src.p, o.src.ld};
     if (!planes && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * 2)) & 15u) == 0) continue;
-    const int64_t ld = round_up(o.cols, 8), plane = o.rows * ld;
+    // rows on 128-byte boundaries: a 128-byte box row that crosses one costs the copy engine two requests
+    const int64_t ld = round_up(o.cols, 64), plane = o.rows * ld;
     void *p = c.take((size_t)(plane * (planes ? 6 : 2)));
     if (!p) return fb::set_error(FB_ERR_ARG, "workspace too small");
     *o.out = Mat{p, ld, planes ? plane : 0};

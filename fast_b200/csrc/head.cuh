@@ -68,6 +68,8 @@ struct Term {
 //   b_n < N: B has only b_n of the N rows (columns); the rest of C is zeros.
 int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, int n_terms, bool b_mn, int N,
               const Out &out, int b_n = 0);
+//   rows2: C_p = A B_p^T for two B [b_n, K] (C's columns past b_n are zeros)
+int pair_rows2(Call &c, const Mat &A, int64_t M, const Mat *B, int K, int N, const Out *out, int b_n);
 //   columns: C_p[m, n] = sum over the `rows` rows r of A[r, p * aprob + m] B[r, n], m < M, n < N, for p < probs
 //         (1 or 2) outputs; A has acols columns.
 int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int probs, int M, const Mat &B, int N,

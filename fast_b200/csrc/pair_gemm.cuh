@@ -46,8 +46,9 @@ enum : int { kSilu = FB_ACT_SILU, kGelu = FB_ACT_GELU, kRelu = FB_ACT_RELU };
 constexpr int BK = 64;                        // k per stage: one 128-byte swizzle row of bf16
 constexpr int kHalfM = 128;                   // rows of a tile per CTA
 constexpr int kABytes = kHalfM * BK * 2;      // 16 KB
-constexpr int kBBytes = 128 * BK * 2;         // 16 KB: BN / 2 <= 128 rows
-constexpr int kStageBytes = kABytes + kBBytes;
+// B of a stage: BN / 2 <= 128 rows; planes: 64 rows of each
+template <int P> __host__ __device__ constexpr int b_bytes() { return (P == 3 ? 64 : 128) * BK * 2; }
+template <int P> __host__ __device__ constexpr int stage_bytes() { return P * (kABytes + b_bytes<P>()); }
 constexpr int kBox = BK * 128;                // MN-major box: 64 k rows of 64 elements
 constexpr int kEpiWarps = 8, kWarpEpi0 = 4;
 constexpr int kThreads = (kWarpEpi0 + kEpiWarps) * 32;
@@ -57,21 +58,24 @@ constexpr int kGluOut = 2048;                 // of the gated block's outputs: 3
 template <int EPI> __host__ __device__ constexpr int out_bytes() {
   return EPI == kGluBwd ? 3 * kGluOut : (EPI == kGluFwd ? kGluOut : kStageOut);
 }
-template <int EPI> __host__ __device__ constexpr int stages() { return EPI == kGluBwd ? 5 : 6; }
-template <int EPI> __host__ __device__ constexpr int smem_bytes() {
-  return 1024 + stages<EPI>() * kStageBytes + kEpiWarps * out_bytes<EPI>() + 256;
+template <int EPI, int P> __host__ __device__ constexpr int stages() { return P == 3 ? 2 : (EPI == kGluBwd ? 5 : 6); }
+template <int EPI, int P> __host__ __device__ constexpr int smem_bytes() {
+  return 1024 + stages<EPI, P>() * stage_bytes<P>() + kEpiWarps * out_bytes<EPI>() + 256;
 }
-static_assert(smem_bytes<kGluBwd>() <= 232448 && smem_bytes<kLse>() <= 232448, "shared memory exceeds 227 KB");
+static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kLse, 1>() <= 232448 &&
+                  smem_bytes<kStoreF32, 3>() <= 232448, "shared memory exceeds 227 KB");
 
 // Fields of one launch.  Two phases may feed a tile: kGluBwd's second one
-// fills the dh columns; elsewhere it continues the same sum (dx = dg Wg + du Wu).
+// fills the dh columns; elsewhere it continues the same sum (dx = dg Wg + du
+// Wu) and its stages follow the first's.
 struct PairArgs {
-  CUtensorMap ta[2], tb[2];                   // by phase; kGluFwd / kGluBwd: tb[0] = Wg, tb[1] = Wu, tw = Wd
+  CUtensorMap ta[2], tb[2];                   // by phase (bprob: B by problem); kGlu*: tb[0] = Wg, tb[1] = Wu, tw = Wd
   CUtensorMap tw;
   CUtensorMap tc[3];                          // outputs (has_tc)
   int32_t *err;
   int mt, nt, probs, splits;                  // tiles along m and n, problems of one shape, splits of k
-  int phases, kb[2], kper;                    // stages per phase; stages per split (phase 0, splits > 1)
+  int phases, kb[2], kper;                    // stages per phase; stages per split
+  int bprob;                                  // each problem has a B of its own
   int ax[2];                                  // A's first column per phase (k contiguous) ...
   int aprob;                                  // ... and per problem (m contiguous: columns of A between problems)
   int M, N;                                   // rows and columns of one problem's result
@@ -303,7 +307,7 @@ __device__ __forceinline__ void send(const PairArgs &a, int o, const uint8_t *bu
 }
 
 struct Tile {
-  int m, n, prob, k0, k1;
+  int m, n, prob, k0, k1;                     // k0 .. k1 - 1: stages, the phases' one after the other
   int64_t ybase;                              // first row of this split's results
 };
 
@@ -321,8 +325,9 @@ __device__ __forceinline__ Tile tile_at(const PairArgs &a, int t) {
   const int gm = min(8, a.mt - 8 * g);
   q.m = 8 * g + r % gm;
   q.n = r / gm;
-  q.k0 = a.splits > 1 ? s * a.kper : 0;
-  q.k1 = a.splits > 1 ? min(a.kb[0], q.k0 + a.kper) : a.kb[0];
+  const int kb = a.kb[0] + (a.phases > 1 ? a.kb[1] : 0);
+  q.k0 = s * a.kper;
+  q.k1 = min(kb, q.k0 + a.kper);
   q.ybase = a.splits > 1 ? s * a.split_rows : 0;
   return q;
 }
@@ -386,14 +391,13 @@ constexpr uint32_t kPlaneA = 0x001102u, kPlaneB = 0x010120u;
 template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(const __grid_constant__ PairArgs a) {
   static_assert(P == 1 || (P == 3 && EPI == kStoreF32), "planes feed fp32 results");
-  constexpr int kPairs = P == 3 ? 6 : 1;
-  constexpr int kStages = stages<EPI>(), kBufs = EPI == kGluBwd ? 1 : 2;
+  constexpr int kStages = stages<EPI, P>(), kStageBytes = stage_bytes<P>(), kBBytes = b_bytes<P>(), kBufs = EPI == kGluBwd ? 1 : 2;
   constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd;      // B: 128 rows of Wg in one CTA, of Wu in the other
   static_assert(!kDual || BN == 256, "the gate and up columns fill a 256-column tile");
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
   auto sA = [&](int s) { return smem + s * kStageBytes; };
-  auto sB = [&](int s) { return smem + s * kStageBytes + kABytes; };
+  auto sB = [&](int s) { return smem + s * kStageBytes + P * kABytes; };
   uint8_t *outs = smem + kStages * kStageBytes;
   uint64_t *bars = reinterpret_cast<uint64_t *>(outs + kEpiWarps * out_bytes<EPI>());
   uint64_t *full = bars, *empty = bars + kStages, *accf = bars + 2 * kStages, *acce = accf + 2;
@@ -415,6 +419,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
     fence_barrier_init();
   }
   if (warp == 1) alloc2(holder, kTmemCols);
+  if (warp == 2 && lane < 2 && (a.phases > lane || lane == 0)) prefetch_map(&a.ta[lane]);
+  if (warp == 2 && lane >= 2 && lane < 4 && (lane == 2 || kDual || a.phases > 1 || a.bprob)) prefetch_map(&a.tb[lane - 2]);
+  if (warp == 2 && lane == 4 && EPI == kGluBwd) prefetch_map(&a.tw);
   tc_fence_before();
   __syncthreads();
   cluster_sync();                             // both CTAs' barriers exist before either signals one
@@ -434,47 +441,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
     for (int t = first; t < total && !stop; t += step) {
       const Tile q = tile_at(a, t);
       const int m0 = q.m * 256 + (int)rank * kHalfM;
-      for (int p = 0; p < a.phases && !stop; ++p) {
+      for (int j = q.k0; j < q.k1; ++j) {
+        const int p = j >= a.kb[0] ? 1 : 0, jj = j - (p ? a.kb[0] : 0);
         const bool dh = EPI == kGluBwd && p == 1;
         const int bn = dh ? 128 : BN;
-        const int j1 = p == 0 ? q.k1 : a.kb[1];
-        const uint32_t bytes = (uint32_t)(kABytes + bn / 2 * BK * 2);
         const bool bmn = dh || B_MN;
-        const CUtensorMap *ma = &a.ta[p], *mb = dh ? &a.tw : (kDual ? &a.tb[rank] : &a.tb[p]);
-        const int ax = A_MN ? q.prob * a.aprob + m0 : a.ax[p];
-        const int n0 = kDual && !dh ? q.n * 128 : q.n * bn + (int)rank * (bn / 2);
-        for (int j = p == 0 ? q.k0 : 0; j < j1 && !stop; ++j)
-#pragma unroll 1
-          for (int pr = 0; pr < kPairs; ++pr) {
-            if (turn > 0 && !wait(empty + s, (turn - 1) & 1, abort_flag, err)) {
-              stop = true;
-              break;
+        if (turn > 0 && !wait(empty + s, (turn - 1) & 1, abort_flag, err)) {
+          stop = true;
+          break;
+        }
+        if (one) {
+          const CUtensorMap *ma = &a.ta[p], *mb = dh ? &a.tw : (kDual ? &a.tb[rank] : &a.tb[a.bprob ? q.prob : p]);
+          const int n0 = kDual && !dh ? q.n * 128 : q.n * bn + (int)rank * (bn / 2);
+          const uint32_t full_at = leader_addr(full + s);
+          if (rank == 0) mbar_expect_tx(full + s, 2u * P * (uint32_t)(kABytes + bn / 2 * BK * 2));
+#pragma unroll
+          for (int z = 0; z < P; ++z) {
+            uint8_t *sa = sA(s) + z * kABytes, *sb = sB(s) + z * kBBytes;
+            auto load = [&](void *dst, const CUtensorMap *map, int x, int y) {
+              if (P == 1) load2(dst, map, full_at, x, y);
+              else load3(dst, map, full_at, x, y, z);
+            };
+            if (A_MN) {
+              load(sa, ma, q.prob * a.aprob + m0, BK * jj);
+              load(sa + kBox, ma, q.prob * a.aprob + m0 + 64, BK * jj);
+            } else {
+              load(sa, ma, a.ax[p] + BK * jj, m0);
             }
-            if (one) {
-              const int za = (kPlaneA >> (4 * pr)) & 15, zb = (kPlaneB >> (4 * pr)) & 15;
-              uint8_t *sa = sA(s), *sb = sB(s);
-              const uint32_t full_at = leader_addr(full + s);
-              if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
-              auto load = [&](void *dst, const CUtensorMap *map, int x, int y, int z) {
-                if (P == 1) load2(dst, map, full_at, x, y);
-                else load3(dst, map, full_at, x, y, z);
-              };
-              if (A_MN) {
-                load(sa, ma, ax, BK * j, za);
-                load(sa + kBox, ma, ax + 64, BK * j, za);
-              } else {
-                load(sa, ma, ax + BK * j, m0, za);
-              }
-              if (bmn) {
-                load(sb, mb, n0, BK * j, zb);
-                if (bn == 256) load(sb + kBox, mb, n0 + 64, BK * j, zb);
-              } else {
-                load(sb, mb, BK * j, n0, zb);
-              }
+            if (bmn) {
+              load(sb, mb, n0, BK * jj);
+              if (bn == 256) load(sb + kBox, mb, n0 + 64, BK * jj);
+            } else {
+              load(sb, mb, BK * jj, n0);
             }
-            __syncwarp();
-            if (++s == kStages) s = 0, ++turn;
           }
+        }
+        __syncwarp();
+        if (++s == kStages) s = 0, ++turn;
       }
     }
     // the MMAs have read every stage (and their arrivals reached this CTA) before it leaves
@@ -485,48 +488,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
   } else if (warp == 1) {
     if (rank == 0) {
       const bool one = elect_one();
-      const uint64_t ad0 = sdesc(smem_u32(smem), A_MN), bd_k = sdesc(smem_u32(smem + kABytes), false),
-                     bd_mn = sdesc(smem_u32(smem + kABytes), true);
+      const uint64_t ad0 = sdesc(smem_u32(smem), A_MN), bd_k = sdesc(smem_u32(smem + P * kABytes), false),
+                     bd_mn = sdesc(smem_u32(smem + P * kABytes), true);
       int s = 0;
       uint32_t turn = 0, it = 0;              // turns of the ring, accumulators used so far
       bool stop = false;
       for (int t = first; t < total && !stop; t += step) {
         const Tile q = tile_at(a, t);
-        for (int p = 0; p < a.phases && !stop; ++p) {
-          const bool dh = EPI == kGluBwd && p == 1;
+        for (int j = q.k0; j < q.k1; ++j) {
+          const bool dh = EPI == kGluBwd && j >= a.kb[0];
           const bool bmn = dh || B_MN;
           const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(BN, A_MN, B_MN);
           const uint64_t adv_a = A_MN ? (2048 >> 4) : 2, adv_b = bmn ? (2048 >> 4) : 2, bd0 = bmn ? bd_mn : bd_k;
-          const int j0 = p == 0 ? q.k0 : 0, j1 = p == 0 ? q.k1 : a.kb[1];
-          for (int j = j0; j < j1 && !stop; ++j)
-#pragma unroll 1
-            for (int pr = 0; pr < kPairs; ++pr) {
-              // a new accumulator: at the tile's start, or (planes) at every slab's
-              const bool fresh = P == 3 ? pr == 0 : (j == j0 && (p == 0 || dh));
-              const uint32_t buf = it % kBufs, use = it / kBufs;
-              if (fresh && !dh && use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
-                stop = true;
-                break;
-              }
-              if (!wait(full + s, turn & 1, abort_flag, err)) {
-                stop = true;
-                break;
-              }
-              tc_fence_after();
-              const bool last = P == 3 ? pr + 1 == kPairs : (j + 1 == j1 && p + 1 == a.phases);
-              if (one) {
-                const uint32_t d = tmem + (dh ? 256u : buf * 256u);
-                const uint64_t at = (uint64_t)(s * (kStageBytes >> 4));
+          // a new accumulator at the tile's start, or (planes) for every slab; dh's columns start at its first stage
+          const bool next = P == 3 || j == q.k0;
+          const bool fresh = next || (dh && j == a.kb[0]);
+          const uint32_t buf = it % kBufs, use = it / kBufs;
+          if (next && use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
+            stop = true;
+            break;
+          }
+          if (!wait(full + s, turn & 1, abort_flag, err)) {
+            stop = true;
+            break;
+          }
+          tc_fence_after();
+          const bool last = P == 3 || j + 1 == q.k1;
+          if (one) {
+            const uint32_t d = tmem + (dh ? 256u : buf * 256u);
+            const uint64_t at = (uint64_t)(s * (kStageBytes >> 4));
 #pragma unroll
-                for (int kk = 0; kk < BK / 16; ++kk)
-                  mma2(d, ad0 + at + kk * adv_a, bd0 + at + kk * adv_b, idesc, (fresh && kk == 0) ? 0u : 1u);
-                commit2(empty + s);
-                if (last) commit2(accf + buf);
-              }
-              __syncwarp();
-              if (last) ++it;
-              if (++s == kStages) s = 0, ++turn;
+            for (int pr = 0; pr < (P == 3 ? 6 : 1); ++pr) {
+              const uint64_t za = (kPlaneA >> (4 * pr) & 15) * (uint64_t)(kABytes >> 4),
+                             zb = (kPlaneB >> (4 * pr) & 15) * (uint64_t)(kBBytes >> 4);
+#pragma unroll
+              for (int kk = 0; kk < BK / 16; ++kk)
+                mma2(d, ad0 + at + (P == 3 ? za : 0) + kk * adv_a, bd0 + at + (P == 3 ? zb : 0) + kk * adv_b, idesc,
+                     (fresh && kk == 0 && pr == 0) ? 0u : 1u);
             }
+            commit2(empty + s);
+            if (last) commit2(accf + buf);
+          }
+          __syncwarp();
+          if (last) ++it;
+          if (++s == kStages) s = 0, ++turn;
         }
       }
     }
@@ -544,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
 #pragma unroll
         for (int i = 0; i < BN / 2; ++i) acc[i] = 0.f;
         bool ok = true;
-        const int slabs = (q.k1 - q.k0) + (a.phases > 1 ? a.kb[1] : 0);
+        const int slabs = q.k1 - q.k0;
         for (int k = 0; k < slabs && ok; ++k, ++it) {
           const int buf = it % kBufs;
           ok = __all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0);
@@ -780,7 +785,7 @@ template <auto kernel> int pair_slots(int smem) {
 
 template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1> int launch_pair(const PairArgs &a, cudaStream_t stream) {
   constexpr auto k = k_pair<EPI, A_MN, B_MN, BN, P>;
-  constexpr int smem = smem_bytes<EPI>();
+  constexpr int smem = smem_bytes<EPI, P>();
   const int slots = pair_slots<k>(smem);
   if (!slots) return fb::cuda_error(cudaGetLastError(), "k_pair shared memory");
   const int64_t tiles = (int64_t)a.mt * a.nt * a.probs * a.splits;
