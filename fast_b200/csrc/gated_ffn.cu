@@ -11,6 +11,7 @@
 // the activation to the fp32 accumulators: h, dg, du are rounded once, and g,
 // u, dh never reach memory.  fp32: the same products over planes, with the
 // activation between them in a kernel of its own.
+#include "few_rows.cuh"
 #include "pair_gemm.cuh"
 
 namespace {
@@ -18,19 +19,6 @@ namespace {
 using namespace fbh;
 
 constexpr int kSilu = FB_ACT_SILU, kGelu = FB_ACT_GELU;
-
-// act(g) and act'(g)
-template <int ACT> __device__ __forceinline__ float2 act_exact(float g) {
-  if (ACT == kSilu) {
-    const float s = 1.f / (1.f + expf(-g));
-    return make_float2(g * s, s * (1.f + g * (1.f - s)));
-  }
-  if (ACT == kGelu) {
-    const float phi = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-    return make_float2(g * phi, phi + g * expf(-0.5f * g * g) * 0.39894228040143268f);
-  }
-  return make_float2(fmaxf(g, 0.f), g > 0.f ? 1.f : 0.f);
-}
 
 // v as three bf16 planes `plane` elements apart (see k_operands).
 __device__ __forceinline__ void put3(uint16_t *p, int64_t plane, float v) {
@@ -49,7 +37,7 @@ template <int ACT> __global__ void k_glu_fwd(const float *gu, uint16_t *h, int64
   const int64_t n = rows * Fp;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const float *p = gu + i / Fp * 2 * Fp + i % Fp;
-    put3(h + i, n, act_exact<ACT>(p[0]).x * p[Fp]);
+    put3(h + i, n, fbact::act_exact<ACT>(p[0]).x * p[Fp]);
   }
 }
 
@@ -61,7 +49,7 @@ __global__ void k_glu_bwd(const float *gu, const float *dh, uint16_t *h, uint16_
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t at = i / Fp * 2 * Fp + i % Fp;
     const float uv = gu[at + Fp], d = dh[i];
-    const float2 a = act_exact<ACT>(gu[at]);
+    const float2 a = fbact::act_exact<ACT>(gu[at]);
     put3(dgu + at, 2 * n, d * uv * a.y);
     put3(dgu + at + Fp, 2 * n, d * a.x);
     put3(h + i, n, a.x * uv);
@@ -219,6 +207,12 @@ int empty_grads(const fb_gated_ffn &a, cudaStream_t st) {
 }
 
 int run(Call &c, const fb_gated_ffn &a, bool bwd) {
+  if (!bwd && few_rows_ok(a.n, std::max(a.D, a.F))) {
+    FBH_TAKE(h, c, float, a.n * a.F);
+    FBH_TRY(few_rows_glu(c, a.type, a.act, Mat{a.x, a.ldx}, a.n, a.D, Mat{a.w_gate, a.ld_gate}, Mat{a.w_up, a.ld_up}, a.F,
+                         h));
+    return few_rows_product(c, a.type, h, a.n, a.F, Mat{a.w_down, a.ld_down}, a.D, a.y, a.ldy);
+  }
   Mat x, wg, wu, wd, dy{};
   const Operand ops[5] = {{Mat{a.x, a.ldx}, a.n, a.D, &x}, {Mat{a.w_gate, a.ld_gate}, a.F, a.D, &wg},
                           {Mat{a.w_up, a.ld_up}, a.F, a.D, &wu}, {Mat{a.w_down, a.ld_down}, a.D, a.F, &wd},

@@ -33,6 +33,7 @@
 #include <cuda_bf16.h>
 #include <algorithm>
 #include <cstring>
+#include "act.cuh"
 #include "head.cuh"
 #include "tc_common.cuh"
 
@@ -41,7 +42,9 @@ namespace fbpair {
 using namespace fbtc;
 
 enum : int { kStoreBf16 = 0, kStoreF32 = 1, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5 };
-enum : int { kSilu = FB_ACT_SILU, kGelu = FB_ACT_GELU, kRelu = FB_ACT_RELU };
+using fbact::kGelu;
+using fbact::kRelu;
+using fbact::kSilu;
 
 constexpr int BK = 64;                        // k per stage: one 128-byte swizzle row of bf16
 constexpr int kHalfM = 128;                   // rows of a tile per CTA
@@ -247,19 +250,6 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// act(g) and act'(g)
-template <int ACT> __device__ __forceinline__ float2 act2(float g) {
-  if (ACT == kSilu) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
-    return make_float2(g * s, s * (1.f + g * (1.f - s)));
-  }
-  if (ACT == kGelu) {
-    const float phi = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-    return make_float2(g * phi, phi + g * __expf(-0.5f * g * g) * 0.39894228040143268f);
-  }
-  return make_float2(fmaxf(g, 0.f), g > 0.f ? 1.f : 0.f);
-}
-
 // One lane's row (128 bytes in eight 16-byte pieces) of a staged block: the
 // layout a 128-byte-swizzled tensor map stores from.
 __device__ __forceinline__ void stage_row(uint8_t *buf, int lane, const uint32_t (&w)[32]) {
@@ -351,7 +341,7 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
       float h[2], dg[2], du[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float2 f = act2<ACT>(__uint_as_float(g[2 * i + e]));
+        const float2 f = fbact::act_fast<ACT>(__uint_as_float(g[2 * i + e]));
         const float uv = __uint_as_float(u[2 * i + e]);
         h[e] = f.x * uv;
         if constexpr (BWD) {

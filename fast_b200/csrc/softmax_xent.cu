@@ -11,6 +11,7 @@
 // planes, pieces of logits in both directions, the forward carrying each
 // row's running maximum and sum from piece to piece.
 #include <cmath>
+#include "few_rows.cuh"
 #include "pair_gemm.cuh"
 
 namespace {
@@ -28,33 +29,60 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
   return MaxSum{m, a.s * expf(a.m - m) + b.s * expf(b.m - m)};
 }
 
-// bf16 rows: one warp joins a row's partial (max, sum of exp2) pairs, takes the
-// target's logit as an fp32 dot product of its own, and writes lse and loss.
-__global__ void __launch_bounds__(128) k_xent_finish(const float2 *part, int np, const uint16_t *h, int64_t ldh,
-                                                     const uint16_t *w, int64_t ldw, int D, int64_t V,
-                                                     const int64_t *target, float *loss, float *lse, int64_t n) {
+__device__ __forceinline__ float value(const float *p) { return *p; }
+__device__ __forceinline__ float value(const uint16_t *p) { return __uint_as_float((uint32_t)*p << 16); }   // bf16
+
+// TH threads (a warp, or a CTA of 256 where rows are few and latency counts)
+// join a row's partial (max, sum of exp2) pairs, take the target's logit as an
+// fp32 dot product of its own, and write lse and loss.
+template <typename U, int TH>
+__global__ void __launch_bounds__(TH == 32 ? 128 : TH) k_xent_finish(const float2 *part, int np, const U *h, int64_t ldh,
+                                                                     const U *w, int64_t ldw, int D, int64_t V,
+                                                                     const int64_t *target, float *loss, float *lse,
+                                                                     int64_t n) {
+  __shared__ float3 sm[TH / 32];
   fb::pdl_enter();
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const int64_t r = TH == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  const int t = threadIdx.x % TH;
   if (r >= n) return;
+  const int64_t tg = target[r];
   const float2 *p = part + r * np;
-  float m = -INFINITY;
-  for (int i = lane; i < np; i += 32) m = fmaxf(m, p[i].x);
-  m = fb::warp_max(m);
-  const float base = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
-  for (int i = lane; i < np; i += 32) s += p[i].y * exp2f(p[i].x - base);
-  s = fb::warp_sum(s);
-  const int64_t t = target[r];
-  float l = 0.f;
-  if (t >= 0 && t < V)
-    for (int i = lane; i < D; i += 32)
-      l = fmaf(__uint_as_float((uint32_t)h[r * ldh + i] << 16), __uint_as_float((uint32_t)w[t * ldw + i] << 16), l);
+  float m = -INFINITY, s = 0.f, l = 0.f;
+#pragma unroll 2
+  for (int i = t; i < np; i += TH) {
+    const float2 q = p[i];
+    const float nm = fmaxf(m, q.x), base = nm == -INFINITY ? 0.f : nm;
+    s = s * exp2f(m - base) + q.y * exp2f(q.x - base);
+    m = nm;
+  }
+  if (tg >= 0 && tg < V)
+#pragma unroll 4
+    for (int i = t; i < D; i += TH) l = fmaf(value(h + r * ldh + i), value(w + tg * ldw + i), l);
+  auto fold = [&](float m2, float s2) {
+    const float nm = fmaxf(m, m2), base = nm == -INFINITY ? 0.f : nm;
+    s = s * exp2f(m - base) + s2 * exp2f(m2 - base);
+    m = nm;
+  };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    fold(m2, s2);
+  }
   l = fb::warp_sum(l);
-  if (lane) return;
+  if (TH > 32) {
+    if ((t & 31) == 0) sm[t / 32] = make_float3(m, s, l);
+    __syncthreads();
+    if (t) return;
+#pragma unroll
+    for (int q = 1; q < TH / 32; ++q) {
+      fold(sm[q].x, sm[q].y);
+      l += sm[q].z;
+    }
+  }
+  if (t) return;
   const float z = (m + log2f(s)) * 0.69314718055994530942f;
   lse[r] = z;
-  loss[r] = t < 0 ? 0.f : (t >= V ? NAN : z - l);
+  loss[r] = tg < 0 ? 0.f : (tg >= V ? NAN : z - l);
 }
 
 // One CTA per row: the piece's maximum and sum join the row's state; the
@@ -228,6 +256,27 @@ int logits_args(fbpair::PairArgs &p, const fb_softmax_xent &a, const Mat &h, int
   return make_map(&p.tb[0], w.p, cols, a.D, w.ld, 128);
 }
 
+// lse and loss of rows r0 .. r0 + n - 1 (h: those rows) from their partials.
+template <typename U>
+int finish(Call &c, const fb_softmax_xent &a, const float2 *part, int np, const Mat &h, const Mat &w, int64_t r0,
+           int64_t n) {
+  const bool wide = n <= 1024;
+  FB_TRY_CUDA(fb::launch(wide ? k_xent_finish<U, 256> : k_xent_finish<U, 32>, (unsigned)(wide ? n : (n + 3) / 4),
+                         wide ? 256 : 128, 0, c.stream, part, np, static_cast<const U *>(h.p), h.ld,
+                         static_cast<const U *>(w.p), w.ld, a.D, a.V, a.target + r0, a.loss + r0, a.lse + r0, n));
+  FB_LAUNCHED("k_xent_finish");
+  return FB_OK;
+}
+
+int forward_few(Call &c, const fb_softmax_xent &a) {
+  const Mat h{a.h, a.ldh}, w{a.w, a.ldw};
+  const int np = few_rows_parts();
+  FBH_TAKE(part, c, float2, a.n * np);
+  FBH_TRY(few_rows_lse(c, a.type, h, a.n, a.D, w, a.V, part));
+  if (c.dry) return FB_OK;
+  return a.type == FB_F32 ? finish<float>(c, a, part, np, h, w, 0, a.n) : finish<uint16_t>(c, a, part, np, h, w, 0, a.n);
+}
+
 int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   using namespace fbpair;
   const int nt = tiles_of(a.V, 256);
@@ -242,10 +291,7 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
     FBH_TRY(logits_args(p, a, hp, n, w, (int)a.V));
     p.part = part;
     FBH_TRY((launch_pair<kLse, false, false, 256>(p, c.stream)));
-    FB_TRY_CUDA(fb::launch(k_xent_finish, (unsigned)((n + 3) / 4), 128, 0, c.stream, (const float2 *)part, 2 * nt,
-                           static_cast<const uint16_t *>(hp.p), hp.ld, static_cast<const uint16_t *>(w.p), w.ld, a.D,
-                           a.V, a.target + r0, a.loss + r0, a.lse + r0, n));
-    FB_LAUNCHED("k_xent_finish");
+    FBH_TRY(finish<uint16_t>(c, a, part, 2 * nt, hp, w, r0, n));
   }
   return FB_OK;
 }
@@ -297,6 +343,7 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
 }
 
 int run(Call &c, const fb_softmax_xent &a, bool bwd) {
+  if (!bwd && few_rows_ok(a.n, a.D)) return forward_few(c, a);
   Mat h, w;
   const Operand ops[2] = {{Mat{a.h, a.ldh}, a.n, a.D, &h}, {Mat{a.w, a.ldw}, a.V, a.D, &w}};
   FBH_TRY(operands(c, a.type, ops, 2));
