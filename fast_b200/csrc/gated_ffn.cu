@@ -128,12 +128,12 @@ int glu(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &
   FBH_TRY(make_map(&p.ta[0], x.p, a.n, a.D, x.ld, kHalfM));
   FBH_TRY(make_map(&p.tb[0], wg.p, a.F, a.D, wg.ld, 128));
   FBH_TRY(make_map(&p.tb[1], wu.p, a.F, a.D, wu.ld, 128));
-  FBH_TRY(make_map(&p.tc[0], h, a.n, Fp, Fp, 32, false, true));
+  FBH_TRY(make_map(&p.tc[0], h, a.n, Fp, Fp, 32));
   if (EPI == kGluBwd) {
     FBH_TRY(make_map(&p.ta[1], dy.p, a.n, a.D, dy.ld, kHalfM));
     FBH_TRY(make_map(&p.tw, wd.p, a.D, a.F, wd.ld, BK));
-    FBH_TRY(make_map(&p.tc[1], dgu, a.n, Fp, 2 * Fp, 32, false, true));
-    FBH_TRY(make_map(&p.tc[2], dgu + Fp, a.n, Fp, 2 * Fp, 32, false, true));
+    FBH_TRY(make_map(&p.tc[1], dgu, a.n, Fp, 2 * Fp, 32));
+    FBH_TRY(make_map(&p.tc[2], dgu + Fp, a.n, Fp, 2 * Fp, 32));
   }
   return launch_pair<EPI, false, false, 256>(p, c.stream);
 }

@@ -19,9 +19,11 @@
 // of shared memory a cycle and SM in each direction (TMA writes, MMA reads),
 // half of what one SM alone would need.
 //
-// CTA = 12 warps: 0 TMA producer (one lane), 1 TMEM allocator and, in the
-// even CTA, MMA issuer (one lane), 4..11 epilogue (two per TMEM lane
-// quadrant, each half of the columns).  Stages of 64 k travel through a ring
+// CTA = 12 or 20 warps: 0 TMA producer (one lane), 1 TMEM allocator and, in the
+// even CTA, MMA issuer (one lane), the rest from 4 on epilogue: two per TMEM
+// lane quadrant, each half of the columns, or four, each a quarter, where the
+// epilogue takes an exponential of every element (with two its latencies were
+// in the open: 3.3 us a tile where the exponentials alone take 1.1).  Stages of 64 k travel through a ring
 // of kStages; the loads of both CTAs count on the even CTA's barrier, MMA
 // completion frees the stage in both.  Accumulators: two of up to 256 columns
 // (the epilogue drains one while the other fills), one of 384 for kGluBwd.
@@ -41,7 +43,7 @@ namespace fbpair {
 
 using namespace fbtc;
 
-enum : int { kStoreBf16 = 0, kStoreF32 = 1, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5 };
+enum : int { kStoreBf16 = 0, kStoreF32 = 1, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6 };
 using fbact::kGelu;
 using fbact::kRelu;
 using fbact::kSilu;
@@ -53,19 +55,25 @@ constexpr int kABytes = kHalfM * BK * 2;      // 16 KB
 template <int P> __host__ __device__ constexpr int b_bytes() { return (P == 3 ? 64 : 128) * BK * 2; }
 template <int P> __host__ __device__ constexpr int stage_bytes() { return P * (kABytes + b_bytes<P>()); }
 constexpr int kBox = BK * 128;                // MN-major box: 64 k rows of 64 elements
-constexpr int kEpiWarps = 8, kWarpEpi0 = 4;
-constexpr int kThreads = (kWarpEpi0 + kEpiWarps) * 32;
+constexpr int kWarpEpi0 = 4;
+template <int EPI> __host__ __device__ constexpr int epi_warps() {
+  return EPI == kLse || EPI == kLseLong || EPI == kProb ? 16 : 8;
+}
+template <int EPI> __host__ __device__ constexpr int threads_of() { return (kWarpEpi0 + epi_warps<EPI>()) * 32; }
 constexpr int kTmemCols = 512;
 constexpr int kStageOut = 4096;               // one staged output block: 32 rows of 128 bytes
-constexpr int kGluOut = 2048;                 // of the gated block's outputs: 32 rows of 64 bytes
+constexpr int kLseSlab = 16;                  // kLseLong: stages summed in tensor memory at a time
 template <int EPI> __host__ __device__ constexpr int out_bytes() {
-  return EPI == kGluBwd ? 3 * kGluOut : (EPI == kGluFwd ? kGluOut : kStageOut);
+  return EPI == kGluBwd ? 3 * kStageOut : (EPI == kLse || EPI == kLseLong ? 0 : kStageOut);
 }
-template <int EPI, int P> __host__ __device__ constexpr int stages() { return P == 3 ? 2 : (EPI == kGluBwd ? 5 : 6); }
+template <int EPI, int P> __host__ __device__ constexpr int stages() {
+  return P == 3 ? 2 : (EPI == kGluBwd ? 4 : (EPI == kProb ? 5 : 6));
+}
 template <int EPI, int P> __host__ __device__ constexpr int smem_bytes() {
-  return 1024 + stages<EPI, P>() * stage_bytes<P>() + kEpiWarps * out_bytes<EPI>() + 256;
+  return 1024 + stages<EPI, P>() * stage_bytes<P>() + epi_warps<EPI>() * out_bytes<EPI>() + 256;
 }
-static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kLse, 1>() <= 232448 &&
+static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 232448 &&
+                  smem_bytes<kStoreBf16, 1>() <= 232448 &&
                   smem_bytes<kStoreF32, 3>() <= 232448, "shared memory exceeds 227 KB");
 
 // Fields of one launch.  Two phases may feed a tile: kGluBwd's second one
@@ -88,7 +96,7 @@ struct PairArgs {
   int64_t ldc;
   int64_t split_rows;                         // splits > 1: rows of C between two splits
   int act;
-  float2 *part;                               // kLse: [M][2 nt] (max, sum of exp2) partials
+  float2 *part;                               // kLse: [M][4 nt] (max, sum of exp2) partials
   const int64_t *target;                      // kProb
   const float *lse, *dloss;
   int64_t V, v0;
@@ -259,6 +267,14 @@ __device__ __forceinline__ void stage_row(uint8_t *buf, int lane, const uint32_t
         make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
 }
 
+// Its first or second 64 bytes.
+__device__ __forceinline__ void stage_half(uint8_t *buf, int lane, int which, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint4 *>(buf + lane * 128 + (((4 * which + k) ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+}
+
 // Sends a staged block (32 rows from `row`, 64 bf16 or 32 fp32 columns from
 // `col`) to output `o`.  Rows at or past `rows` and columns past a.N stay out.
 template <bool F32OUT>
@@ -323,11 +339,11 @@ __device__ __forceinline__ Tile tile_at(const PairArgs &a, int t) {
 }
 
 // Columns c .. c + 31 of g (and + 128: u, + 256: dh) of this warp's 32 rows:
-// h (and dg, du) staged as blocks of 32 rows x 64 bytes in the 64-byte
-// swizzle and sent off.
+// h (and dg, du) staged as half of the warp's 128-byte rows, sent off with the
+// second half: the copy engine takes a 64-byte row no faster than a 128-byte one.
 template <int ACT, bool BWD>
-__device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, uint8_t *buf, int row, int col,
-                                          int lane) {
+__device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, int which, uint8_t *buf, int row,
+                                          int col, int lane) {
   uint32_t w[BWD ? 3 : 1][16];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
@@ -357,20 +373,19 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
       }
     }
   }
-  if (lane == 0) store_wait<0>();             // the block before has left the buffers
-  __syncwarp();
+  if (which == 0) {
+    if (lane == 0) store_wait<0>();           // the tile before has left the buffers
+    __syncwarp();
+  }
 #pragma unroll
-  for (int o = 0; o < (BWD ? 3 : 1); ++o)
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      *reinterpret_cast<uint4 *>(buf + o * kGluOut + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
-          make_uint4(w[o][4 * k], w[o][4 * k + 1], w[o][4 * k + 2], w[o][4 * k + 3]);
+  for (int o = 0; o < (BWD ? 3 : 1); ++o) stage_half(buf + o * kStageOut, lane, which, w[o]);
+  if (which == 0) return;
   fence_async_smem();
   __syncwarp();
   if (lane == 0) {
     if (row < a.M && col < a.N)
 #pragma unroll
-      for (int o = 0; o < (BWD ? 3 : 1); ++o) store_tile(&a.tc[o], buf + o * kGluOut, col, row);
+      for (int o = 0; o < (BWD ? 3 : 1); ++o) store_tile(&a.tc[o], buf + o * kStageOut, col, row);
     store_commit();
   }
 }
@@ -379,9 +394,10 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
 constexpr uint32_t kPlaneA = 0x001102u, kPlaneB = 0x010120u;
 
 template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(const __grid_constant__ PairArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1) k_pair(const __grid_constant__ PairArgs a) {
   static_assert(P == 1 || (P == 3 && EPI == kStoreF32), "planes feed fp32 results");
   constexpr int kStages = stages<EPI, P>(), kStageBytes = stage_bytes<P>(), kBBytes = b_bytes<P>(), kBufs = EPI == kGluBwd ? 1 : 2;
+  constexpr int kEpiWarps = epi_warps<EPI>();
   constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd;      // B: 128 rows of Wg in one CTA, of Wu in the other
   static_assert(!kDual || BN == 256, "the gate and up columns fill a 256-column tile");
   extern __shared__ uint8_t smem_raw[];
@@ -490,8 +506,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
           const bool bmn = dh || B_MN;
           const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(BN, A_MN, B_MN);
           const uint64_t adv_a = A_MN ? (2048 >> 4) : 2, adv_b = bmn ? (2048 >> 4) : 2, bd0 = bmn ? bd_mn : bd_k;
-          // a new accumulator at the tile's start, or (planes) for every slab; dh's columns start at its first stage
-          const bool next = P == 3 || j == q.k0;
+          // a new accumulator at the tile's start, or for every slab; dh's columns start at its first stage
+          const bool next = P == 3 || j == q.k0 || (EPI == kLseLong && (j & (kLseSlab - 1)) == 0);
           const bool fresh = next || (dh && j == a.kb[0]);
           const uint32_t buf = it % kBufs, use = it / kBufs;
           if (next && use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
@@ -503,7 +519,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
             break;
           }
           tc_fence_after();
-          const bool last = P == 3 || j + 1 == q.k1;
+          const bool last = P == 3 || j + 1 == q.k1 || (EPI == kLseLong && ((j + 1) & (kLseSlab - 1)) == 0);
           if (one) {
             const uint32_t d = tmem + (dh ? 256u : buf * 256u);
             const uint64_t at = (uint64_t)(s * (kStageBytes >> 4));
@@ -527,7 +543,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
     }
     __syncwarp();
   } else if (warp >= kWarpEpi0) {
-    const int e = warp - kWarpEpi0, qd = warp & 3, half = e >> 2;
+    const int e = warp - kWarpEpi0, qd = warp & 3, half = e >> 2;   // (16 warps: the quarter)
     const uint32_t tlane = (uint32_t)(qd * 32) << 16;
     uint8_t *obuf = outs + e * out_bytes<EPI>();
     uint32_t it = 0;
@@ -573,6 +589,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
         }
         continue;
       }
+      if constexpr (EPI == kLseLong) {
+        // kLse for more than kLseSlab stages: the tensor cores' accumulation truncates (6e-8 of the logit a stage,
+        // all one way) and a loss is fp32, so tensor memory sums kLseSlab stages at a time and registers the rest.
+        constexpr float kLog2e = 1.44269504088896340736f;
+        float v[64];
+        const int row = q.m * 256 + (int)rank * kHalfM + qd * 32, c0 = half * 64, left = a.N - (q.n * BN + c0);
+        bool ok = true;
+        for (int j = q.k0; j < q.k1; j += kLseSlab, ++it) {
+          const int buf = it % kBufs;
+          ok = __all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tb = tmem + tlane + (uint32_t)(buf * 256 + c0);
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t r[32];
+            tmem_ld32_nowait(tb + c, r);
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[c + i] = j == q.k0 ? __uint_as_float(r[i]) : v[c + i] + __uint_as_float(r[i]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(leader_addr(acce + buf));
+        }
+        --it;                                 // the loop header counts one
+        if (!ok) break;
+        if (left < 64) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= left) v[i] = -INFINITY;  // past the table
+        }
+        float m = v[0];
+#pragma unroll
+        for (int i = 1; i < 64; ++i) m = fmaxf(m, v[i]);
+        m *= kLog2e;
+        // nothing but -inf: subtract 0, so that exp2 gives zeros (and NaN stays NaN)
+        const float base = m == -INFINITY ? 0.f : m;
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          s0 += ex2(fmaf(v[i], kLog2e, -base));
+          s1 += ex2(fmaf(v[i + 1], kLog2e, -base));
+        }
+        if (row + lane < a.M) a.part[(int64_t)(row + lane) * (4 * a.nt) + 4 * q.n + half] = make_float2(m, s0 + s1);
+        continue;
+      }
       const int buf = it % kBufs;
       if (!__all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0)) break;
       tc_fence_after();
@@ -581,11 +644,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
       if constexpr (EPI == kGluFwd || EPI == kGluBwd) {
         constexpr bool bwd = EPI == kGluBwd;
 #pragma unroll 1
-        for (int c = half * 64; c < half * 64 + 64; c += 32) {
-          const int col = q.n * 128 + c;
-          if (a.act == kSilu) glu_block<kSilu, bwd>(a, tb, c, obuf, row, col, lane);
-          else if (a.act == kGelu) glu_block<kGelu, bwd>(a, tb, c, obuf, row, col, lane);
-          else glu_block<kRelu, bwd>(a, tb, c, obuf, row, col, lane);
+        for (int which = 0; which < 2; ++which) {
+          const int c = half * 64 + 32 * which, col = q.n * 128 + half * 64;
+          if (a.act == kSilu) glu_block<kSilu, bwd>(a, tb, c, which, obuf, row, col, lane);
+          else if (a.act == kGelu) glu_block<kGelu, bwd>(a, tb, c, which, obuf, row, col, lane);
+          else glu_block<kRelu, bwd>(a, tb, c, which, obuf, row, col, lane);
         }
       } else if constexpr (EPI == kStoreBf16) {
 #pragma unroll 1
@@ -618,17 +681,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
           __syncwarp();
         }
       } else if constexpr (EPI == kLse) {
-        // running maximum and sum of exp2 of this lane's row over its half of the tile's columns
+        // maximum and sum of exp2 of this lane's row over its quarter of the tile's columns
         constexpr float kLog2e = 1.44269504088896340736f;
         float m = -INFINITY, s = 0.f;
-        const int cbase = q.n * BN;
-#pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-          if (cbase + c >= a.N) break;
+#pragma unroll
+        for (int c = half * 64; c < half * 64 + 64; c += 32) {
+          const int left = a.N - (q.n * BN + c);
           uint32_t r[32];
           tmem_ld32_nowait(tb + c, r);
           tmem_wait();
-          const int left = a.N - (cbase + c);
           if (left < 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -638,7 +699,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
 #pragma unroll
           for (int i = 1; i < 32; ++i) cm = fmaxf(cm, __uint_as_float(r[i]));
           const float nm = fmaxf(m, cm * kLog2e);
-          // nothing but -inf so far: subtract 0 so that exp2 gives zeros (and NaN stays NaN)
+          // nothing but -inf so far: subtract 0, so that exp2 gives zeros (and NaN stays NaN)
           const float base = nm == -INFINITY ? 0.f : nm;
           s *= ex2(m - base);
           float s0 = 0.f, s1 = 0.f;
@@ -650,7 +711,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
           s += s0 + s1;
           m = nm;
         }
-        if (row + lane < a.M) a.part[(int64_t)(row + lane) * (2 * a.nt) + 2 * q.n + half] = make_float2(m, s);
+        if (row + lane < a.M) a.part[(int64_t)(row + lane) * (4 * a.nt) + 4 * q.n + half] = make_float2(m, s);
       } else if constexpr (EPI == kProb) {
         constexpr float kLog2e = 1.44269504088896340736f;
         const int i0 = row + lane;
@@ -659,32 +720,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
         const float z = live ? a.lse[i0] * kLog2e : 0.f, d = live ? a.dloss[i0] : 0.f;
         const uint32_t mask = live ? 0xFFFFFFFFu : 0u;            // a held-out row is zeros whatever its logits are
         const int64_t tc = live ? tg - a.v0 : -1;                 // the target's column of this piece
-#pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 64) {
-          const int col = q.n * BN + c;
-          uint32_t r0[32], r1[32], w[32];
-          tmem_ld32_nowait(tb + c, r0);
-          tmem_ld32_nowait(tb + c + 32, r1);
-          tmem_wait();
-          const int hit = (tc >= col && tc < col + 64) ? (int)(tc - col) : -1;
-          const bool any = __any_sync(0xffffffffu, hit >= 0);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float l0 = __uint_as_float(i < 16 ? r0[2 * i] : r1[2 * (i - 16)]);
-            const float l1 = __uint_as_float(i < 16 ? r0[2 * i + 1] : r1[2 * (i - 16) + 1]);
-            float p0 = ex2(fmaf(l0, kLog2e, -z)), p1 = ex2(fmaf(l1, kLog2e, -z));
-            if (any) {
-              if (hit == 2 * i) p0 -= 1.f;
-              if (hit == 2 * i + 1) p1 -= 1.f;
-            }
-            w[i] = pack(p0 * d, p1 * d) & mask;
+        for (int c = 0; c < 64; c += 32) {
+          const int col = q.n * BN + half * 64 + c;
+          uint32_t r[32], w[16];
+          tmem_ld32_nowait(tb + half * 64 + c, r);
+          tmem_wait();
+          const int hit = (tc >= col && tc < col + 32) ? (int)(tc - col) : -1;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(ex2(fmaf(__uint_as_float(r[i]), kLog2e, -z)));
+          if (__any_sync(0xffffffffu, hit >= 0)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (hit == i) r[i] = __float_as_uint(__uint_as_float(r[i]) - 1.f);
           }
-          if (lane == 0) store_wait<0>();
-          __syncwarp();
-          stage_row(obuf, lane, w);
-          send<false>(a, 0, obuf, 0, row, col, lane);
-          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            w[i] = pack(__uint_as_float(r[2 * i]) * d, __uint_as_float(r[2 * i + 1]) * d) & mask;
+          if (c == 0) {
+            if (lane == 0) store_wait<0>();   // the tile before has left the buffer
+            __syncwarp();
+          }
+          stage_half(obuf, lane, c / 32, w);
         }
+        send<false>(a, 0, obuf, 0, row, q.n * BN + half * 64, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -707,19 +766,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_pair(
 
 // ---- host ----------------------------------------------------------------------------------------
 // A bf16 (or fp32: f32) matrix in boxes of 128-byte rows x box_rows, 128-byte swizzle.
-// half: 64-byte rows and swizzle.
 inline int make_map(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows,
-                    bool f32 = false, bool half = false) {
+                    bool f32 = false) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return fb::set_error(FB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const int es = f32 ? 4 : 2;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)(ld * es)};
-  cuuint32_t box[2] = {(cuuint32_t)((half ? 64 : 128) / es), (cuuint32_t)box_rows};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r = enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                          const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         half ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fb::set_error(FB_ERR_ARG, "tensor map rejected (alignment or stride)");
   return FB_OK;
@@ -746,7 +804,7 @@ inline bool map_ok(const void *p, int64_t ld, int es) {
 }
 
 // Clusters of two that fit on the device at once.
-template <auto kernel> int pair_slots(int smem) {
+template <auto kernel> int pair_slots(int smem, int threads) {
   static int slots[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -755,7 +813,7 @@ template <auto kernel> int pair_slots(int smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(num_sms() / 2 * 2);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -776,12 +834,12 @@ template <auto kernel> int pair_slots(int smem) {
 template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1> int launch_pair(const PairArgs &a, cudaStream_t stream) {
   constexpr auto k = k_pair<EPI, A_MN, B_MN, BN, P>;
   constexpr int smem = smem_bytes<EPI, P>();
-  const int slots = pair_slots<k>(smem);
+  const int slots = pair_slots<k>(smem, threads_of<EPI>());
   if (!slots) return fb::cuda_error(cudaGetLastError(), "k_pair shared memory");
   const int64_t tiles = (int64_t)a.mt * a.nt * a.probs * a.splits;
   if (tiles == 0) return FB_OK;
   const unsigned grid = 2 * (unsigned)std::min<int64_t>(tiles, slots);
-  FB_TRY_CUDA(fb::launch(k, grid, kThreads, smem, stream, a));
+  FB_TRY_CUDA(fb::launch(k, grid, threads_of<EPI>(), smem, stream, a));
   FB_LAUNCHED("k_pair");
   return FB_OK;
 }

@@ -281,8 +281,8 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
   using namespace fbpair;
   const int nt = tiles_of(a.V, 256);
   // rows per launch: the partials of one stay within kPieceBytes
-  const int64_t rows = std::min<int64_t>(a.n, std::max<int64_t>(256, kPieceBytes / (16ll * nt) / 256 * 256));
-  FBH_TAKE(part, c, float2, rows * 2 * nt);
+  const int64_t rows = std::min<int64_t>(a.n, std::max<int64_t>(256, kPieceBytes / (32ll * nt) / 256 * 256));
+  FBH_TAKE(part, c, float2, rows * 4 * nt);
   if (c.dry) return FB_OK;
   for (int64_t r0 = 0; r0 < a.n; r0 += rows) {
     const int64_t n = std::min(rows, a.n - r0);
@@ -290,8 +290,9 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
     PairArgs p;
     FBH_TRY(logits_args(p, a, hp, n, w, (int)a.V));
     p.part = part;
-    FBH_TRY((launch_pair<kLse, false, false, 256>(p, c.stream)));
-    FBH_TRY(finish<uint16_t>(c, a, part, 2 * nt, hp, w, r0, n));
+    FBH_TRY((p.kb[0] > kLseSlab ? launch_pair<kLseLong, false, false, 256>(p, c.stream)
+                                : launch_pair<kLse, false, false, 256>(p, c.stream)));
+    FBH_TRY(finish<uint16_t>(c, a, part, 4 * nt, hp, w, r0, n));
   }
   return FB_OK;
 }
