@@ -5,8 +5,7 @@
 // forward reduces every 256-column tile of logits to a maximum and a sum per
 // row in its epilogue, one launch over the whole table, and a second kernel
 // joins them; the backward takes the table in pieces of as many rows as make a
-// G piece of kPieceBytes (so that it stays in the L2 between its three
-// products), computes G from the logits in the epilogue that would have stored
+// G piece of kPieceBytes, computes G from the logits in the epilogue that would have stored
 // them, then adds G w to dh and writes G^T h.  fp32: the same products over
 // planes, pieces of logits in both directions, the forward carrying each
 // row's running maximum and sum from piece to piece.
@@ -18,7 +17,13 @@ namespace {
 
 using namespace fbh;
 
-constexpr int64_t kPieceBytes = 48ll << 20;
+// Memory of a piece (bf16: of G; fp32: of the logits, G's planes take 1.5 times
+// that beside them).  A piece that stays in the 126 MB L2 was expected to pay,
+// but its products are short: 48 / 160 / 512 MB a piece took 160 / 110 / 110 us
+// for 4,000 rows x 16,700 nodes x 104 and 2.45 / 2.22 / 2.13 ms for 8,192 x
+// 50,000 x 1,024; beyond that little changes and memory is not given back.
+constexpr int64_t kPieceBytes = 512ll << 20, kPieceBytesF32 = 256ll << 20;
+constexpr int64_t kPartBytes = 256ll << 20;   // of the forward's partials
 
 struct MaxSum {
   float m, s;                                // sum of exp(l - m); m = -inf, s = 0: nothing yet
@@ -163,7 +168,8 @@ __global__ void k_round_rows(const float *src, int64_t lds, __nv_bfloat16 *dst, 
 
 // Table rows per piece: a multiple of 64, so that pieces start 16-byte aligned.
 int64_t piece_rows(int64_t n, int64_t V, int es) {
-  const int64_t r = std::max<int64_t>(256, kPieceBytes / es / std::max<int64_t>(n, 1) / 64 * 64);
+  const int64_t bytes = es == 4 ? kPieceBytesF32 : kPieceBytes;
+  const int64_t r = std::max<int64_t>(256, bytes / es / std::max<int64_t>(n, 1) / 64 * 64);
   return std::min<int64_t>(r, round_up(V, 64));
 }
 
@@ -281,7 +287,7 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
   using namespace fbpair;
   const int nt = tiles_of(a.V, 256);
   // rows per launch: the partials of one stay within kPieceBytes
-  const int64_t rows = std::min<int64_t>(a.n, std::max<int64_t>(256, kPieceBytes / (32ll * nt) / 256 * 256));
+  const int64_t rows = std::min<int64_t>(a.n, std::max<int64_t>(256, kPartBytes / (32ll * nt) / 256 * 256));
   FBH_TAKE(part, c, float2, rows * 4 * nt);
   if (c.dry) return FB_OK;
   for (int64_t r0 = 0; r0 < a.n; r0 += rows) {
