@@ -4,8 +4,8 @@
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 // Only x is kept between the two: the backward recomputes g and u.
 //
-// bf16: two launches forward, four backward (plus the sums of split
-// reductions), each a product on SM pairs (pair_gemm.cuh).  The first of each
+// bf16: two launches forward, two backward (plus the sums of split
+// reductions), each of products on SM pairs (pair_gemm.cuh).  The first of each
 // direction computes g and u side by side in one tile -- one CTA of the pair
 // stages Wg, the other Wu -- and for the backward dh beside them, and applies
 // the activation to the fp32 accumulators: h, dg, du are rounded once, and g,
@@ -85,9 +85,10 @@ int check(const fb_gated_ffn *a, bool bwd) {
 // fp32: g | u [N, 2 Fp] (and dh), then the activation; the padding columns up
 // to Fp are zeros (weight rows past F read as zeros).
 int gate_up_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, float *gu, int64_t Fp) {
-  const Mat w[2] = {wg, wu};
-  const Out o[2] = {{gu, 2 * Fp, FB_F32, 0}, {gu + Fp, 2 * Fp, FB_F32, 0}};
-  return pair_rows2(c, x, a.n, w, a.D, (int)Fp, o, a.F);
+  Product p[2] = {rows_product(x, a.n, a.D, wg, false, (int)Fp, Out{gu, 2 * Fp, FB_F32, 0}),
+                  rows_product(x, a.n, a.D, wu, false, (int)Fp, Out{gu + Fp, 2 * Fp, FB_F32, 0})};
+  p[0].b_n = p[1].b_n = a.F;
+  return products(c, p, 2);
 }
 
 int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
@@ -100,8 +101,8 @@ int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, con
     FB_TRY_CUDA(fb::launch(k, blocks_for(a.n * Fp), 256, 0, c.stream, (const float *)gu, h, a.n, (int)Fp));
     FB_LAUNCHED("k_glu_fwd");
   }
-  const Term t{wd, 0, a.F};
-  return pair_rows(c, Mat{h, Fp, a.n * Fp}, a.n, a.F, &t, 1, false, a.D, Out{a.y, a.ldy, FB_F32, 0});
+  const Product p = rows_product(Mat{h, Fp, a.n * Fp}, a.n, a.F, wd, false, a.D, Out{a.y, a.ldy, FB_F32, 0});
+  return products(c, &p, 1);
 }
 
 // g and u (and dh) of every tile, the activation in the epilogue: h [N, Fp],
@@ -113,59 +114,43 @@ int glu(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &
   using namespace fbpair;
   if (c.dry) return FB_OK;
   PairArgs p;
-  std::memset(&p, 0, sizeof(p));
-  p.phases = EPI == kGluBwd ? 2 : 1;
-  p.probs = p.splits = 1;
-  p.kb[0] = p.kb[1] = tiles_of(a.D, BK);
-  p.kper = p.phases * p.kb[0];
-  p.mt = tiles_of(a.n, 256);
-  p.nt = tiles_of(Fp, 128);
-  p.M = (int)a.n;
-  p.N = (int)Fp;
+  one_product(p, a.n, Fp, 128, tiles_of(a.D, BK), EPI == kGluBwd ? 2 : 1);
   p.act = a.act;
-  p.has_tc = 1;
-  p.err = err_word();
-  FBH_TRY(make_map(&p.ta[0], x.p, a.n, a.D, x.ld, kHalfM));
-  FBH_TRY(make_map(&p.tb[0], wg.p, a.F, a.D, wg.ld, 128));
-  FBH_TRY(make_map(&p.tb[1], wu.p, a.F, a.D, wu.ld, 128));
-  FBH_TRY(make_map(&p.tc[0], h, a.n, Fp, Fp, 32));
+  PairProb &b = p.p[0];
+  FBH_TRY(make_map(&b.ta[0], x.p, a.n, a.D, x.ld, kHalfM));
+  FBH_TRY(make_map(&b.tb[0], wg.p, a.F, a.D, wg.ld, 128));
+  FBH_TRY(make_map(&b.tb[1], wu.p, a.F, a.D, wu.ld, 128));
+  FBH_TRY(make_map(&b.tc, h, a.n, Fp, Fp, 32));
   if (EPI == kGluBwd) {
-    FBH_TRY(make_map(&p.ta[1], dy.p, a.n, a.D, dy.ld, kHalfM));
+    FBH_TRY(make_map(&b.ta[1], dy.p, a.n, a.D, dy.ld, kHalfM));
     FBH_TRY(make_map(&p.tw, wd.p, a.D, a.F, wd.ld, BK));
-    FBH_TRY(make_map(&p.tc[1], dgu, a.n, Fp, 2 * Fp, 32));
-    FBH_TRY(make_map(&p.tc[2], dgu + Fp, a.n, Fp, 2 * Fp, 32));
+    FBH_TRY(make_map(&p.tc2[0], dgu, a.n, Fp, 2 * Fp, 32));
+    FBH_TRY(make_map(&p.tc2[1], dgu + Fp, a.n, Fp, 2 * Fp, 32));
   }
-  return launch_pair<EPI, false, false, 256>(p, c.stream);
+  return launch_pair<EPI>(p, c.stream);
 }
 
 int forward_bf16(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
   const int64_t Fp = round_up(a.F, 64);
   FBH_TAKE(h, c, __nv_bfloat16, a.n * Fp);
   FBH_TRY(glu<fbpair::kGluFwd>(c, a, x, Mat{}, wg, wu, wd, h, nullptr, Fp));
-  const Term t{wd, 0, a.F};
-  return pair_rows(c, Mat{h, Fp}, a.n, a.F, &t, 1, false, a.D, Out{a.y, a.ldy, FB_BF16, 0});
+  const Product p = rows_product(Mat{h, Fp}, a.n, a.F, wd, false, a.D, Out{a.y, a.ldy, FB_BF16, 0});
+  return products(c, &p, 1);
 }
 
 // dx and the weight gradients from h [n, Fp] and dgu [n, 2 Fp].
 int gradients(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu, const Mat &h,
               const Mat &dgu, int64_t Fp) {
-  if (a.dx) {
-    const Term t[2] = {{wg, 0, a.F}, {wu, (int)Fp, a.F}};
-    FBH_TRY(pair_rows(c, dgu, a.n, (int)(2 * Fp), t, 2, true, a.D, Out{a.dx, a.lddx, a.type, 0}));
-  }
-  const Out og{a.dw_gate, a.ldd_gate, a.grad_type, a.accumulate}, ou{a.dw_up, a.ldd_up, a.grad_type, a.accumulate};
-  const Out both[2] = {og, ou};
-  if (a.dw_gate && a.dw_up) {
-    FBH_TRY(pair_columns(c, dgu, a.n, (int)(2 * Fp), (int)Fp, 2, a.F, x, a.D, both));
-  } else if (a.dw_gate) {
-    FBH_TRY(pair_columns(c, dgu, a.n, a.F, 0, 1, a.F, x, a.D, &og));
-  } else if (a.dw_up) {
-    const Mat du{static_cast<const uint16_t *>(dgu.p) + Fp, dgu.ld, dgu.plane};
-    FBH_TRY(pair_columns(c, du, a.n, a.F, 0, 1, a.F, x, a.D, &ou));
-  }
-  const Out od{a.dw_down, a.ldd_down, a.grad_type, a.accumulate};
-  if (a.dw_down) FBH_TRY(pair_columns(c, dy, a.n, a.D, 0, 1, a.D, h, a.F, &od));
-  return FB_OK;
+  const Mat du{static_cast<const uint16_t *>(dgu.p) + Fp, dgu.ld, dgu.plane};
+  auto grad = [&](void *p, int64_t ld) { return Out{p, ld, a.grad_type, a.accumulate}; };
+  Product dx = rows_product(dgu, a.n, a.F, wg, true, a.D, Out{a.dx, a.lddx, a.type, 0});
+  dx.acols = (int)(2 * Fp);
+  dx.term[1] = Term{wu, (int)Fp, a.F};
+  dx.terms = 2;
+  const Product p[4] = {dx, columns_product(dgu, a.n, a.F, x, a.D, grad(a.dw_gate, a.ldd_gate)),
+                        columns_product(du, a.n, a.F, x, a.D, grad(a.dw_up, a.ldd_up)),
+                        columns_product(dy, a.n, a.D, h, a.F, grad(a.dw_down, a.ldd_down))};
+  return products(c, p, 4);
 }
 
 int backward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu,
@@ -176,8 +161,9 @@ int backward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, co
   FBH_TAKE(h, c, uint16_t, 3 * n);
   FBH_TAKE(dgu, c, uint16_t, 6 * n);
   FBH_TRY(gate_up_f32(c, a, x, wg, wu, gu, Fp));
-  const Term t{wd, 0, a.D};
-  FBH_TRY(pair_rows(c, dy, a.n, a.D, &t, 1, true, (int)Fp, Out{dh, Fp, FB_F32, 0}, a.F));
+  Product ph = rows_product(dy, a.n, a.D, wd, true, (int)Fp, Out{dh, Fp, FB_F32, 0});
+  ph.b_n = a.F;
+  FBH_TRY(products(c, &ph, 1));
   if (!c.dry) {
     auto k = a.act == kSilu ? k_glu_bwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_bwd<FB_ACT_GELU> : k_glu_bwd<FB_ACT_RELU>);
     FB_TRY_CUDA(fb::launch(k, blocks_for(n), 256, 0, c.stream, (const float *)gu, (const float *)dh, h, dgu, a.n,

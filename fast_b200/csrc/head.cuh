@@ -57,23 +57,35 @@ struct Out {
   int type, accumulate;
 };
 
-// Products on pairs of SMs (pair_gemm.cuh); operands as `operands` leaves
+// Products on pairs of SMs (pair_gemm.cuh), operands as `operands` leaves
 // them, fp32 accumulation, one rounding at the end (planes: fp32 results).
-//   rows: C[m, n] = sum over 1 or 2 terms of A[m, ax_t + k] B_t(n, k), A [M, acols], k < K_t; B_t is [N, K_t], or
-//         [K_t, N] when b_mn.  ax_t is a multiple of 64.
+//   rows:    C[m, n] = sum over 1 or 2 terms of A[m, ax_t + k] B_t(n, k), A [M, acols], k < K_t; B_t is [b_n, K_t], or
+//            [K_t, b_n] when b_mn; C's columns from b_n to N are zeros.  ax_t is a multiple of 64.
+//   columns: C[m, n] = sum over the `rows` rows r of A[r, m] B_0[r, n]
 struct Term {
   Mat B;
   int ax, K;
 };
-//   b_n < N: B has only b_n of the N rows (columns); the rest of C is zeros.
-int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, int n_terms, bool b_mn, int N,
-              const Out &out, int b_n = 0);
-//   rows2: C_p = A B_p^T for two B [b_n, K] (C's columns past b_n are zeros)
-int pair_rows2(Call &c, const Mat &A, int64_t M, const Mat *B, int K, int N, const Out *out, int b_n);
-//   columns: C_p[m, n] = sum over the `rows` rows r of A[r, p * aprob + m] B[r, n], m < M, n < N, for p < probs
-//         (1 or 2) outputs; A has acols columns.
-int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int probs, int M, const Mat &B, int N,
-                 const Out *out);
+struct Product {
+  bool columns, b_mn;
+  Mat A;
+  int acols;
+  int64_t rows;
+  Term term[2];
+  int terms;
+  int64_t M;
+  int N, b_n;
+  Out out;
+};
+inline Product rows_product(const Mat &A, int64_t M, int K, const Mat &B, bool b_mn, int N, const Out &out) {
+  return Product{false, b_mn, A, K, M, {{B, 0, K}, {}}, 1, M, N, N, out};
+}
+inline Product columns_product(const Mat &A, int64_t rows, int M, const Mat &B, int N, const Out &out) {
+  return Product{true, true, A, M, rows, {{B, 0, 0}, {}}, 1, M, N, N, out};
+}
+// Up to 4 independent products, all over bf16 or all over planes, in one
+// launch (and one for the sums of those whose reduction is split).
+int products(Call &c, const Product *p, int n);
 
 }  // namespace fbh
 

@@ -1,5 +1,5 @@
 // Plain products of the node-ranking head on pairs of SMs (pair_gemm.cuh), and
-// the sum of their partial results when the reduction is split.
+// the sum of their partial results where the reduction is split.
 #include "pair_gemm.cuh"
 
 namespace {
@@ -8,122 +8,117 @@ using namespace fbpair;
 using namespace fbh;
 
 // out (+)= sum over splits of P[s], in split order; P rows have pitch ldp.
-// blockIdx.y: the problem.
-struct SumArgs {
-  const float *P[2];
-  void *out[2];
-  int64_t ldo[2];
-  int64_t split_stride, ldp, rows;
-  int splits, cols, accumulate;
+struct SumJob {
+  const float *P;
+  void *out;
+  int64_t ldo, ldp, split_stride, rows;
+  int splits, cols, accumulate, bf16;
+  unsigned first;                              // first CTA of the job
 };
-template <bool kBf16> __global__ void __launch_bounds__(256) k_sum_splits(const __grid_constant__ SumArgs a) {
+struct SumArgs {
+  SumJob j[kMaxProbs];
+  int n;
+};
+constexpr int kSumPerCta = 256 * 4;
+
+__global__ void __launch_bounds__(256) k_sum_splits(const __grid_constant__ SumArgs a) {
   fb::pdl_enter();
-  const float *const P = a.P[blockIdx.y];
-  void *const out = a.out[blockIdx.y];
-  const int64_t ldo = a.ldo[blockIdx.y], ldp = a.ldp, split_stride = a.split_stride, rows = a.rows;
-  const int splits = a.splits, cols = a.cols, accumulate = a.accumulate;
-  const int64_t total = rows * cols;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / cols;
-    const int c = (int)(i - r * cols);
-    const float *p = P + r * ldp + c;
+  int q = 0;
+  while (q + 1 < a.n && blockIdx.x >= a.j[q + 1].first) ++q;
+  const SumJob &j = a.j[q];
+  const int64_t total = j.rows * j.cols, at = (int64_t)(blockIdx.x - j.first) * kSumPerCta, stride = j.split_stride;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t i = at + e * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int64_t r = i / j.cols;
+    const int c = (int)(i - r * j.cols);
+    const float *p = j.P + r * j.ldp + c;
     float s = 0.f;
     int z = 0;
-    for (; z + 8 <= splits; z += 8) {
+    for (; z + 8 <= j.splits; z += 8) {
       float v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = p[(z + u) * split_stride];
+      for (int u = 0; u < 8; ++u) v[u] = p[(z + u) * stride];
 #pragma unroll
       for (int u = 0; u < 8; ++u) s += v[u];
     }
-    for (; z < splits; ++z) s += p[z * split_stride];
-    if (kBf16) {
-      static_cast<__nv_bfloat16 *>(out)[r * ldo + c] = __float2bfloat16_rn(s);
+    for (; z < j.splits; ++z) s += p[z * stride];
+    if (j.bf16) {
+      static_cast<__nv_bfloat16 *>(j.out)[r * j.ldo + c] = __float2bfloat16_rn(s);
     } else {
-      float *o = static_cast<float *>(out) + r * ldo + c;
-      *o = accumulate ? *o + s : s;
+      float *o = static_cast<float *>(j.out) + r * j.ldo + c;
+      *o = j.accumulate ? *o + s : s;
     }
   }
 }
 
-int sum_splits(Call &c, SumArgs a, int probs, int type) {
-  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((a.rows * a.cols + 255) / 256, 148 * 16)), probs);
-  if (type == FB_BF16) FB_TRY_CUDA(fb::launch(k_sum_splits<true>, grid, 256, 0, c.stream, a));
-  else FB_TRY_CUDA(fb::launch(k_sum_splits<false>, grid, 256, 0, c.stream, a));
-  FB_LAUNCHED("k_sum_splits");
-  return FB_OK;
-}
-
-// Tile width and splits for results of M x N over kb stages.  256 columns keep
-// the tensor cores fed; a grid that would leave half the SM pairs idle takes
-// 128-column tiles, then splits the reduction, at least min_stages a split (a
-// stage of planes is six products).
+// Tile widths and splits of a launch's products.  256 columns keep the tensor
+// cores fed; where that leaves half the SM pairs idle, 128.  Reductions are
+// split into parts of about `part` stages, at least min_stages (a stage of
+// planes is six products); of a few part sizes around the launch's mean work
+// per pair the one whose busiest pair is done first is taken, by a model in SM
+// cycles: a stage and a tile as measured, the partial results written and read
+// at 2.6 KB a cycle, and a second launch for their sum.
 constexpr int min_stages(bool planes) { return planes ? 2 : 4; }
-struct Plan {
-  int bn, splits, kper;
-};
-Plan plan_of(int64_t M, int N, int probs, int kb, bool planes) {
+constexpr int kStage256 = 515, kStage128 = 390, kStagePlanes = 1600, kTileCycles = 1500, kSumCycles = 6000;
+
+int split_of(int kb, int part, bool planes) {
+  const int s = std::max(1, std::min(kb / min_stages(planes), (kb + part / 2) / part));
+  const int per = (kb + s - 1) / s;
+  return (kb + per - 1) / per;
+}
+
+void plan(PairArgs &a, bool planes) {
   const int slots = num_sms() / 2;
-  Plan p{N > 128 && !planes ? 256 : 128, 1, kb};
-  const int64_t mt = tiles_of(M, 256);
-  if (p.bn == 256 && mt * tiles_of(N, 256) * probs * 2 <= slots) p.bn = 128;
-  const int64_t tiles = mt * tiles_of(N, p.bn) * probs;
-  if (tiles * 2 <= slots) {
-    const int s = (int)std::min<int64_t>(slots / tiles, kb / min_stages(planes));
-    if (s > 1) {
-      p.kper = (kb + s - 1) / s;
-      p.splits = tiles_of(kb, p.kper);
+  int64_t tiles = 0, work = 0;
+  int longest = 1;
+  for (int i = 0; i < a.n; ++i) {
+    PairProb &b = a.p[i];
+    b.bn = b.N > 128 && !planes ? 256 : 128;
+    b.mt = tiles_of(b.M, 256);
+    tiles += (int64_t)b.mt * tiles_of(b.N, b.bn);
+  }
+  for (int i = 0; i < a.n; ++i) {
+    PairProb &b = a.p[i];
+    if (tiles * 2 <= slots) b.bn = 128;
+    b.nt = tiles_of(b.N, b.bn);
+    work += (int64_t)b.mt * b.nt * (b.kb[0] + b.kb[1]);
+    longest = std::max(longest, b.kb[0] + b.kb[1]);
+  }
+  const int mean = (int)std::max<int64_t>(1, (work + slots - 1) / slots);
+  int best = longest;
+  if (tiles < 8ll * slots && longest >= 2 * min_stages(planes)) {
+    double least = 0;
+    for (int part : {longest, 2 * mean, mean, (mean + 1) / 2, (mean + 2) / 3}) {
+      if (part > longest || part < 1) continue;
+      int64_t at = 0;
+      double load[256] = {0}, sum = 0;
+      const int n = std::min(slots, 256);
+      for (int i = 0; i < a.n; ++i) {
+        const PairProb &b = a.p[i];
+        const int kb = b.kb[0] + b.kb[1], s = split_of(kb, part, planes);
+        const int64_t t = (int64_t)b.mt * b.nt * s;
+        const double cost = (double)((kb + s - 1) / s) * (planes ? kStagePlanes : (b.bn == 256 ? kStage256 : kStage128)) +
+                            kTileCycles;
+        for (int c = 0; c < n; ++c) load[c] += cost * (double)((at + t - 1 - c + n) / n - (at - 1 - c + n) / n);
+        at += t;
+        if (s > 1) sum += 8.0 * s * b.M * b.N / 2600;
+      }
+      double busiest = 0;
+      for (int c = 0; c < n; ++c) busiest = std::max(busiest, load[c]);
+      const double cycles = busiest + (sum > 0 ? sum + kSumCycles : 0);
+      if (least == 0 || cycles < least) least = cycles, best = part;
     }
   }
-  return p;
-}
-
-template <bool A_MN, bool B_MN> int dispatch(const PairArgs &a, int bn, bool f32, bool planes, cudaStream_t st) {
-  if (planes) return launch_pair<kStoreF32, A_MN, B_MN, 128, 3>(a, st);
-  if (f32)
-    return bn == 256 ? launch_pair<kStoreF32, A_MN, B_MN, 256>(a, st) : launch_pair<kStoreF32, A_MN, B_MN, 128>(a, st);
-  return bn == 256 ? launch_pair<kStoreBf16, A_MN, B_MN, 256>(a, st) : launch_pair<kStoreBf16, A_MN, B_MN, 128>(a, st);
-}
-
-// Fills the tiling and the outputs (or the partial results') of `a`, launches, sums the splits.
-template <bool A_MN, bool B_MN> int finish(Call &c, PairArgs &a, const Plan &p, bool planes, int64_t M, int N, const Out *out) {
-  a.mt = tiles_of(M, 256);
-  a.nt = tiles_of(N, p.bn);
-  a.splits = p.splits;
-  a.kper = p.kper;
-  a.M = (int)M;
-  a.N = N;
-  a.err = c.dry ? nullptr : err_word();
-  const int64_t prow = (int64_t)a.mt * 256, pld = round_up(N, 4);
-  float *P[2] = {nullptr, nullptr};
-  const size_t mark = c.off;
-  if (p.splits > 1)
-    for (int i = 0; i < a.probs; ++i) {
-      P[i] = static_cast<float *>(c.take((size_t)(p.splits * prow * pld) * 4));
-      if (!P[i]) return fb::set_error(FB_ERR_ARG, "workspace too small");
-    }
-  c.off = mark;
-  if (c.dry) return FB_OK;
-  const bool f32 = p.splits > 1 || out[0].type == FB_F32;
-  a.has_tc = 1;
-  a.accumulate = p.splits > 1 ? 0 : out[0].accumulate;
-  a.split_rows = prow;
-  for (int i = 0; i < a.probs; ++i) {
-    if (p.splits > 1) {
-      FBH_TRY(make_map(&a.tc[i], P[i], p.splits * prow, N, pld, 32, true));
-    } else {
-      a.C[i] = out[i].p;
-      a.ldc = out[i].ld;
-      if (out[i].ld != out[0].ld || !map_ok(out[i].p, out[i].ld, f32 ? 4 : 2)) a.has_tc = 0;
-    }
+  a.tile0[0] = 0;
+  for (int i = 0; i < a.n; ++i) {
+    PairProb &b = a.p[i];
+    const int kb = b.kb[0] + b.kb[1];
+    b.splits = split_of(kb, best, planes);
+    b.kper = (kb + b.splits - 1) / b.splits;
+    a.tile0[i + 1] = a.tile0[i] + b.mt * b.nt * b.splits;
   }
-  if (p.splits == 1 && a.has_tc)
-    for (int i = 0; i < a.probs; ++i) FBH_TRY(make_map(&a.tc[i], out[i].p, M, N, out[i].ld, 32, f32));
-  FBH_TRY((dispatch<A_MN, B_MN>(a, p.bn, f32, planes, c.stream)));
-  if (p.splits == 1) return FB_OK;
-  SumArgs sa{{P[0], P[1]}, {out[0].p, nullptr}, {out[0].ld, 0}, prow * pld, pld, M, p.splits, N, out[0].accumulate};
-  if (a.probs > 1) sa.out[1] = out[1].p, sa.ldo[1] = out[1].ld;
-  return sum_splits(c, sa, a.probs, out[0].type);
 }
 
 int operand_map(CUtensorMap *m, const Mat &x, int64_t rows, int64_t cols, int box_rows) {
@@ -134,58 +129,79 @@ int operand_map(CUtensorMap *m, const Mat &x, int64_t rows, int64_t cols, int bo
 
 namespace fbh {
 
-int pair_rows(Call &c, const Mat &A, int64_t M, int acols, const Term *terms, int n_terms, bool b_mn, int N,
-              const Out &out, int b_n) {
-  if (M == 0) return FB_OK;
-  if (!b_n) b_n = N;
+int products(Call &c, const Product *all, int n_all) {
+  const Product *ps[kMaxProbs];
   PairArgs a;
   std::memset(&a, 0, sizeof(a));
-  a.phases = n_terms;
-  a.probs = 1;
-  for (int t = 0; t < n_terms; ++t) {
-    a.kb[t] = tiles_of(terms[t].K, BK);
-    a.ax[t] = terms[t].ax;
+  // longest reductions first: tiles go to the SM pairs in turn
+  for (int i = 0; i < n_all; ++i) {
+    const Product &p = all[i];
+    if (p.M == 0 || !p.out.p) continue;
+    int at = a.n++;
+    auto len = [](const Product &q) { return q.columns ? q.rows : (int64_t)q.term[0].K + (q.terms > 1 ? q.term[1].K : 0); };
+    for (; at > 0 && len(*ps[at - 1]) < len(p); --at) ps[at] = ps[at - 1];
+    ps[at] = &p;
   }
-  const Plan p = plan_of(M, N, 1, a.kb[0] + a.kb[1], A.plane > 0);
-  if (!c.dry)
-    for (int t = 0; t < n_terms; ++t) {
-      FBH_TRY(operand_map(&a.ta[t], A, M, acols, kHalfM));
-      if (b_mn) FBH_TRY(operand_map(&a.tb[t], terms[t].B, terms[t].K, b_n, BK));
-      else FBH_TRY(operand_map(&a.tb[t], terms[t].B, b_n, terms[t].K, p.bn / 2));
+  if (a.n == 0) return FB_OK;
+  const bool planes = ps[0]->A.plane > 0;
+  for (int i = 0; i < a.n; ++i) {
+    const Product &p = *ps[i];
+    PairProb &b = a.p[i];
+    b.M = (int)p.M;
+    b.N = p.N;
+    b.a_mn = p.columns;
+    b.b_mn = p.b_mn;
+    for (int t = 0; t < p.terms; ++t) {
+      b.kb[t] = tiles_of(p.columns ? p.rows : p.term[t].K, BK);
+      b.ax[t] = p.term[t].ax;
     }
-  return b_mn ? finish<false, true>(c, a, p, A.plane > 0, M, N, &out) : finish<false, false>(c, a, p, A.plane > 0, M, N, &out);
-}
-
-int pair_rows2(Call &c, const Mat &A, int64_t M, const Mat *B, int K, int N, const Out *out, int b_n) {
-  if (M == 0) return FB_OK;
-  PairArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.phases = 1;
-  a.probs = 2;
-  a.bprob = 1;
-  a.kb[0] = tiles_of(K, BK);
-  const Plan p = plan_of(M, N, 2, a.kb[0], A.plane > 0);
-  if (!c.dry) {
-    FBH_TRY(operand_map(&a.ta[0], A, M, K, kHalfM));
-    for (int i = 0; i < 2; ++i) FBH_TRY(operand_map(&a.tb[i], B[i], b_n, K, p.bn / 2));
   }
-  return finish<false, false>(c, a, p, A.plane > 0, M, N, out);
-}
-
-int pair_columns(Call &c, const Mat &A, int64_t rows, int acols, int aprob, int probs, int M, const Mat &B, int N,
-                 const Out *out) {
-  PairArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.phases = 1;
-  a.probs = probs;
-  a.aprob = aprob;
-  a.kb[0] = tiles_of(rows, BK);
-  const Plan p = plan_of(M, N, probs, a.kb[0], A.plane > 0);
-  if (!c.dry) {
-    FBH_TRY(operand_map(&a.ta[0], A, rows, acols, BK));
-    FBH_TRY(operand_map(&a.tb[0], B, rows, N, BK));
+  plan(a, planes);
+  const size_t mark = c.off;
+  SumArgs sums;
+  sums.n = 0;
+  unsigned ctas = 0;
+  for (int i = 0; i < a.n; ++i) {
+    const Product &p = *ps[i];
+    PairProb &b = a.p[i];
+    const int64_t prow = (int64_t)b.mt * 256, pld = round_up(p.N, 4);
+    b.split_rows = (int)prow;
+    b.f32 = b.splits > 1 || p.out.type == FB_F32;
+    if (b.splits > 1) {
+      float *P = static_cast<float *>(c.take((size_t)(b.splits * prow * pld) * 4));
+      if (!P) return fb::set_error(FB_ERR_ARG, "workspace too small");
+      sums.j[sums.n++] = SumJob{P, p.out.p, p.out.ld, pld, prow * pld, p.M, b.splits, p.N, p.out.accumulate,
+                                p.out.type == FB_BF16, ctas};
+      ctas += (unsigned)((p.M * p.N + kSumPerCta - 1) / kSumPerCta);
+      b.has_tc = 1;
+      if (!c.dry) FBH_TRY(make_map(&b.tc, P, b.splits * prow, p.N, pld, 32, true));
+    } else if (!c.dry) {
+      b.C = p.out.p;
+      b.ldc = p.out.ld;
+      b.accumulate = p.out.accumulate;
+      b.has_tc = map_ok(p.out.p, p.out.ld, b.f32 ? 4 : 2);
+      if (b.has_tc) FBH_TRY(make_map(&b.tc, p.out.p, p.M, p.N, p.out.ld, 32, b.f32));
+    }
+    if (c.dry) continue;
+    for (int t = 0; t < p.terms; ++t) {
+      const Term &tm = p.term[t];
+      if (p.columns) {
+        FBH_TRY(operand_map(&b.ta[t], p.A, p.rows, p.acols, BK));
+        FBH_TRY(operand_map(&b.tb[t], tm.B, p.rows, p.N, BK));
+      } else {
+        FBH_TRY(operand_map(&b.ta[t], p.A, p.M, p.acols, kHalfM));
+        FBH_TRY(p.b_mn ? operand_map(&b.tb[t], tm.B, tm.K, p.b_n, BK) : operand_map(&b.tb[t], tm.B, p.b_n, tm.K, b.bn / 2));
+      }
+    }
   }
-  return finish<true, true>(c, a, p, A.plane > 0, M, N, out);
+  c.off = mark;
+  if (c.dry) return FB_OK;
+  a.err = err_word();
+  FBH_TRY((planes ? launch_pair<kStore, 3>(a, c.stream) : launch_pair<kStore, 1>(a, c.stream)));
+  if (sums.n == 0) return FB_OK;
+  FB_TRY_CUDA(fb::launch(k_sum_splits, ctas, 256, 0, c.stream, sums));
+  FB_LAUNCHED("k_sum_splits");
+  return FB_OK;
 }
 
 }  // namespace fbh

@@ -2,9 +2,12 @@
 // cta_group::2, operands by TMA, fp32 accumulators in tensor memory, and the
 // operators' own arithmetic in the epilogue.
 //
-//   kernel k_pair<EPI, A_MN, B_MN, BN, P>: C[m, n] = sum_k A(m, k) B(n, k)
-//   A_MN / B_MN: the operand lies with its m (n) index contiguous (the matrix
+//   kernel k_pair<EPI, P>: C[m, n] = sum_k A(m, k) B(n, k)
+//   a_mn / b_mn: the operand lies with its m (n) index contiguous (the matrix
 //   is stored [k][m]); else with k contiguous.
+//   EPI = kStore takes up to kMaxProbs independent products in one launch
+//   (their layouts, tile widths and output types are fields): a backward pass's
+//   products are short, and a launch of its own costs one 3 to 4 us of ramp.
 //   P = 3: fp32 operands, each as three bf16 planes x = x0 + x1 + x2 of 8
 //   significant bits (exact: 24 bits in all).  Six of the nine plane products
 //   are summed, smallest first; the three left out are below 2^-24 of the
@@ -43,7 +46,7 @@ namespace fbpair {
 
 using namespace fbtc;
 
-enum : int { kStoreBf16 = 0, kStoreF32 = 1, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6 };
+enum : int { kStore = 0, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6 };
 using fbact::kGelu;
 using fbact::kRelu;
 using fbact::kSilu;
@@ -73,28 +76,32 @@ template <int EPI, int P> __host__ __device__ constexpr int smem_bytes() {
   return 1024 + stages<EPI, P>() * stage_bytes<P>() + epi_warps<EPI>() * out_bytes<EPI>() + 256;
 }
 static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 232448 &&
-                  smem_bytes<kStoreBf16, 1>() <= 232448 &&
-                  smem_bytes<kStoreF32, 3>() <= 232448, "shared memory exceeds 227 KB");
+                  smem_bytes<kStore, 1>() <= 232448 &&
+                  smem_bytes<kStore, 3>() <= 232448, "shared memory exceeds 227 KB");
 
-// Fields of one launch.  Two phases may feed a tile: kGluBwd's second one
-// fills the dh columns; elsewhere it continues the same sum (dx = dg Wg + du
-// Wu) and its stages follow the first's.
-struct PairArgs {
-  CUtensorMap ta[2], tb[2];                   // by phase (bprob: B by problem); kGlu*: tb[0] = Wg, tb[1] = Wu, tw = Wd
-  CUtensorMap tw;
-  CUtensorMap tc[3];                          // outputs (has_tc)
-  int32_t *err;
-  int mt, nt, probs, splits;                  // tiles along m and n, problems of one shape, splits of k
-  int phases, kb[2], kper;                    // stages per phase; stages per split
-  int bprob;                                  // each problem has a B of its own
-  int ax[2];                                  // A's first column per phase (k contiguous) ...
-  int aprob;                                  // ... and per problem (m contiguous: columns of A between problems)
-  int M, N;                                   // rows and columns of one problem's result
-  int has_tc;
-  int accumulate;                             // kStoreF32: add to what is there
-  void *C[2];                                 // no has_tc: the results, row pitch ldc
+constexpr int kMaxProbs = 4;
+
+// One product.  Two terms may feed a tile: kGluBwd's second one fills the dh
+// columns; elsewhere it continues the same sum (dx = dg Wg + du Wu) and its
+// stages follow the first's.
+struct PairProb {
+  CUtensorMap ta[2], tb[2];                   // by term; kGlu*: tb[0] = Wg, tb[1] = Wu
+  CUtensorMap tc;                             // output (has_tc); the splits' partial results, one above the other
+  int a_mn, b_mn, bn, f32;                    // layouts, tile width, output type
+  int mt, nt, splits, kb[2], kper;            // tiles along m and n, splits of k; stages per term and per split
+  int ax[2];                                  // A's first column per term (k contiguous)
+  int M, N;                                   // rows and columns of the result
+  int has_tc, accumulate;                     // accumulate (fp32): add to what is there
+  int split_rows;                             // rows of tc between two splits
+  void *C;                                    // no has_tc: the result, row pitch ldc
   int64_t ldc;
-  int64_t split_rows;                         // splits > 1: rows of C between two splits
+};
+// Fields of one launch; all but kStore have one product.
+struct PairArgs {
+  PairProb p[kMaxProbs];
+  int n, tile0[kMaxProbs + 1];                // products; tiles before each
+  int32_t *err;
+  CUtensorMap tw, tc2[2];                     // kGluBwd: Wd; outputs dg, du
   int act;
   float2 *part;                               // kLse: [M][4 nt] (max, sum of exp2) partials
   const int64_t *target;                      // kProb
@@ -276,31 +283,31 @@ __device__ __forceinline__ void stage_half(uint8_t *buf, int lane, int which, co
 }
 
 // Sends a staged block (32 rows from `row`, 64 bf16 or 32 fp32 columns from
-// `col`) to output `o`.  Rows at or past `rows` and columns past a.N stay out.
+// `col`) to the product's output.  Rows past M and columns past N stay out.
 template <bool F32OUT>
-__device__ __forceinline__ void send(const PairArgs &a, int o, const uint8_t *buf, int64_t ybase, int row, int col,
-                                     int lane) {
+__device__ __forceinline__ void send(const PairProb &a, const CUtensorMap *tc, const uint8_t *buf, int ybase, int row,
+                                     int col, int lane) {
   fence_async_smem();
   __syncwarp();
   const bool in = row < a.M && col < a.N;
   if (lane == 0) {                            // one bulk group per block, empty or not
     if (in && a.has_tc) {
-      if (F32OUT && a.accumulate) add_tile(&a.tc[o], buf, col, (int)(ybase + row));
-      else store_tile(&a.tc[o], buf, col, (int)(ybase + row));
+      if (F32OUT && a.accumulate) add_tile(tc, buf, col, ybase + row);
+      else store_tile(tc, buf, col, ybase + row);
     }
     store_commit();
   }
   if (!in || a.has_tc) return;
   const int nr = min(32, a.M - row);
   if (F32OUT) {
-    float *p = static_cast<float *>(a.C[o]) + (ybase + row) * a.ldc + col + lane;
+    float *p = static_cast<float *>(a.C) + row * a.ldc + col + lane;
     if (col + lane < a.N)
       for (int r = 0; r < nr; ++r) {
         const float v = *reinterpret_cast<const float *>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
         p[r * a.ldc] = a.accumulate ? p[r * a.ldc] + v : v;
       }
   } else {
-    uint16_t *p = static_cast<uint16_t *>(a.C[o]) + (ybase + row) * a.ldc + col;
+    uint16_t *p = static_cast<uint16_t *>(a.C) + row * a.ldc + col;
     for (int r = 0; r < nr; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -313,28 +320,30 @@ __device__ __forceinline__ void send(const PairArgs &a, int o, const uint8_t *bu
 }
 
 struct Tile {
-  int m, n, prob, k0, k1;                     // k0 .. k1 - 1: stages, the phases' one after the other
-  int64_t ybase;                              // first row of this split's results
+  int p, m, n, k0, k1;                        // k0 .. k1 - 1: stages, the terms' one after the other
+  int ybase;                                  // first row of this split's results
 };
 
-// Tiles run along m inside groups of 8 m-tiles, so that a wave's tiles share
-// few distinct operand rows; problems outermost, then splits.
-__device__ __forceinline__ Tile tile_at(const PairArgs &a, int t) {
+// Products one after the other, then splits; tiles run along m inside groups
+// of 8 m-tiles, so that a wave's tiles share few distinct operand rows.
+template <int EPI> __device__ __forceinline__ Tile tile_at(const PairArgs &a, int t) {
   Tile q;
-  const int per = a.mt * a.nt;
-  const int z = t / per;
-  int r = t - z * per;
-  const int s = z % a.splits;
-  q.prob = z / a.splits;
-  const int grp = 8 * a.nt, g = r / grp;
+  q.p = 0;
+  if (EPI == kStore)
+    while (q.p + 1 < a.n && t >= a.tile0[q.p + 1]) ++q.p;
+  const PairProb &b = a.p[q.p];
+  t -= EPI == kStore ? a.tile0[q.p] : 0;
+  const int mt = b.mt, nt = b.nt, per = mt * nt;
+  const int s = EPI == kStore ? t / per : 0;
+  int r = t - s * per;
+  const int grp = 8 * nt, g = r / grp;
   r -= g * grp;
-  const int gm = min(8, a.mt - 8 * g);
+  const int gm = min(8, mt - 8 * g);
   q.m = 8 * g + r % gm;
   q.n = r / gm;
-  const int kb = a.kb[0] + (a.phases > 1 ? a.kb[1] : 0);
-  q.k0 = s * a.kper;
-  q.k1 = min(kb, q.k0 + a.kper);
-  q.ybase = a.splits > 1 ? s * a.split_rows : 0;
+  q.k0 = s * b.kper;
+  q.k1 = min(b.kb[0] + b.kb[1], q.k0 + b.kper);
+  q.ybase = s * b.split_rows;
   return q;
 }
 
@@ -383,9 +392,9 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
   fence_async_smem();
   __syncwarp();
   if (lane == 0) {
-    if (row < a.M && col < a.N)
+    if (row < a.p[0].M && col < a.p[0].N)
 #pragma unroll
-      for (int o = 0; o < (BWD ? 3 : 1); ++o) store_tile(&a.tc[o], buf + o * kStageOut, col, row);
+      for (int o = 0; o < (BWD ? 3 : 1); ++o) store_tile(o ? &a.tc2[o - 1] : &a.p[0].tc, buf + o * kStageOut, col, row);
     store_commit();
   }
 }
@@ -393,13 +402,12 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
 // Planes of the six products of P = 3, smallest first (one hex digit each, from the right).
 constexpr uint32_t kPlaneA = 0x001102u, kPlaneB = 0x010120u;
 
-template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1>
+template <int EPI, int P = 1>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1) k_pair(const __grid_constant__ PairArgs a) {
-  static_assert(P == 1 || (P == 3 && EPI == kStoreF32), "planes feed fp32 results");
-  constexpr int kStages = stages<EPI, P>(), kStageBytes = stage_bytes<P>(), kBBytes = b_bytes<P>(), kBufs = EPI == kGluBwd ? 1 : 2;
-  constexpr int kEpiWarps = epi_warps<EPI>();
+  static_assert(P == 1 || (P == 3 && EPI == kStore), "planes feed plain products");
+  constexpr int kStages = stages<EPI, P>(), kStageBytes = stage_bytes<P>(), kBBytes = b_bytes<P>();
+  constexpr int kBufs = EPI == kGluBwd ? 1 : 2, kEpiWarps = epi_warps<EPI>();
   constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd;      // B: 128 rows of Wg in one CTA, of Wu in the other
-  static_assert(!kDual || BN == 256, "the gate and up columns fill a 256-column tile");
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
   auto sA = [&](int s) { return smem + s * kStageBytes; };
@@ -425,9 +433,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
     fence_barrier_init();
   }
   if (warp == 1) alloc2(holder, kTmemCols);
-  if (warp == 2 && lane < 2 && (a.phases > lane || lane == 0)) prefetch_map(&a.ta[lane]);
-  if (warp == 2 && lane >= 2 && lane < 4 && (lane == 2 || kDual || a.phases > 1 || a.bprob)) prefetch_map(&a.tb[lane - 2]);
-  if (warp == 2 && lane == 4 && EPI == kGluBwd) prefetch_map(&a.tw);
+  if (warp == 2 && lane < a.n) {
+    const PairProb &b = a.p[lane];
+    prefetch_map(&b.ta[0]);
+    prefetch_map(&b.tb[0]);
+    if (b.kb[1]) prefetch_map(&b.ta[1]);
+    if (b.kb[1] || kDual) prefetch_map(&b.tb[1]);
+    if (EPI == kGluBwd) prefetch_map(&a.tw);
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();                             // both CTAs' barriers exist before either signals one
@@ -435,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
   const uint32_t tmem = *holder;
   fb::pdl_enter();
 
-  const int total = a.mt * a.nt * a.probs * a.splits;
+  const int total = a.tile0[a.n];
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
   int32_t *err = a.err;
 
@@ -445,19 +458,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
     uint32_t turn = 0;                        // turns of the ring so far
     bool stop = false;
     for (int t = first; t < total && !stop; t += step) {
-      const Tile q = tile_at(a, t);
-      const int m0 = q.m * 256 + (int)rank * kHalfM;
+      const Tile q = tile_at<EPI>(a, t);
+      const PairProb &b = a.p[EPI == kStore ? q.p : 0];
+      const int m0 = q.m * 256 + (int)rank * kHalfM, kb0 = b.kb[0];
+      const bool amn = EPI == kStore && b.a_mn, bmn_ = EPI == kStore && b.b_mn;
+      const int bn_ = P == 3 ? 128 : (EPI == kStore ? b.bn : 256);
       for (int j = q.k0; j < q.k1; ++j) {
-        const int p = j >= a.kb[0] ? 1 : 0, jj = j - (p ? a.kb[0] : 0);
+        const int p = j >= kb0 ? 1 : 0, jj = j - (p ? kb0 : 0);
         const bool dh = EPI == kGluBwd && p == 1;
-        const int bn = dh ? 128 : BN;
-        const bool bmn = dh || B_MN;
+        const int bn = dh ? 128 : bn_;
+        const bool bmn = dh || bmn_;
         if (turn > 0 && !wait(empty + s, (turn - 1) & 1, abort_flag, err)) {
           stop = true;
           break;
         }
         if (one) {
-          const CUtensorMap *ma = &a.ta[p], *mb = dh ? &a.tw : (kDual ? &a.tb[rank] : &a.tb[a.bprob ? q.prob : p]);
+          const CUtensorMap *ma = &b.ta[p], *mb = dh ? &a.tw : &b.tb[kDual ? rank : p];
           const int n0 = kDual && !dh ? q.n * 128 : q.n * bn + (int)rank * (bn / 2);
           const uint32_t full_at = leader_addr(full + s);
           if (rank == 0) mbar_expect_tx(full + s, 2u * P * (uint32_t)(kABytes + bn / 2 * BK * 2));
@@ -468,11 +484,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
               if (P == 1) load2(dst, map, full_at, x, y);
               else load3(dst, map, full_at, x, y, z);
             };
-            if (A_MN) {
-              load(sa, ma, q.prob * a.aprob + m0, BK * jj);
-              load(sa + kBox, ma, q.prob * a.aprob + m0 + 64, BK * jj);
+            if (amn) {
+              load(sa, ma, m0, BK * jj);
+              load(sa + kBox, ma, m0 + 64, BK * jj);
             } else {
-              load(sa, ma, a.ax[p] + BK * jj, m0);
+              load(sa, ma, b.ax[p] + BK * jj, m0);
             }
             if (bmn) {
               load(sb, mb, n0, BK * jj);
@@ -494,21 +510,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
   } else if (warp == 1) {
     if (rank == 0) {
       const bool one = elect_one();
-      const uint64_t ad0 = sdesc(smem_u32(smem), A_MN), bd_k = sdesc(smem_u32(smem + P * kABytes), false),
-                     bd_mn = sdesc(smem_u32(smem + P * kABytes), true);
       int s = 0;
       uint32_t turn = 0, it = 0;              // turns of the ring, accumulators used so far
       bool stop = false;
       for (int t = first; t < total && !stop; t += step) {
-        const Tile q = tile_at(a, t);
+        const Tile q = tile_at<EPI>(a, t);
+      const PairProb &b = a.p[EPI == kStore ? q.p : 0];
+        const bool amn = EPI == kStore && b.a_mn, bmn_ = EPI == kStore && b.b_mn;
+        const int bn = P == 3 ? 128 : (EPI == kStore ? b.bn : 256), kb0 = b.kb[0];
+        const uint64_t ad0 = sdesc(smem_u32(smem), amn), adv_a = amn ? (2048 >> 4) : 2;
         for (int j = q.k0; j < q.k1; ++j) {
-          const bool dh = EPI == kGluBwd && j >= a.kb[0];
-          const bool bmn = dh || B_MN;
-          const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(BN, A_MN, B_MN);
-          const uint64_t adv_a = A_MN ? (2048 >> 4) : 2, adv_b = bmn ? (2048 >> 4) : 2, bd0 = bmn ? bd_mn : bd_k;
+          const bool dh = EPI == kGluBwd && j >= kb0, bmn = dh || bmn_;
+          const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(bn, amn, bmn);
+          const uint64_t bd0 = sdesc(smem_u32(smem + P * kABytes), bmn), adv_b = bmn ? (2048 >> 4) : 2;
           // a new accumulator at the tile's start, or for every slab; dh's columns start at its first stage
           const bool next = P == 3 || j == q.k0 || (EPI == kLseLong && (j & (kLseSlab - 1)) == 0);
-          const bool fresh = next || (dh && j == a.kb[0]);
+          const bool fresh = next || (dh && j == kb0);
           const uint32_t buf = it % kBufs, use = it / kBufs;
           if (next && use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
             stop = true;
@@ -548,12 +565,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
     uint8_t *obuf = outs + e * out_bytes<EPI>();
     uint32_t it = 0;
     for (int t = first; t < total; t += step, ++it) {
-      const Tile q = tile_at(a, t);
+      const Tile q = tile_at<EPI>(a, t);
+      const PairProb &b = a.p[EPI == kStore ? q.p : 0];
       if constexpr (P == 3) {
         const int row = q.m * 256 + (int)rank * kHalfM + qd * 32;
-        float acc[BN / 2];
+        float acc[64];
 #pragma unroll
-        for (int i = 0; i < BN / 2; ++i) acc[i] = 0.f;
+        for (int i = 0; i < 64; ++i) acc[i] = 0.f;
         bool ok = true;
         const int slabs = q.k1 - q.k0;
         for (int k = 0; k < slabs && ok; ++k, ++it) {
@@ -561,9 +579,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           ok = __all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t tb = tmem + tlane + (uint32_t)(buf * 256 + half * (BN / 2));
+          const uint32_t tb = tmem + tlane + (uint32_t)(buf * 256 + half * 64);
 #pragma unroll
-          for (int c = 0; c < BN / 2; c += 32) {
+          for (int c = 0; c < 64; c += 32) {
             uint32_t r[32];
             tmem_ld32_nowait(tb + c, r);
             tmem_wait();
@@ -577,14 +595,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         --it;                                 // the loop header counts one
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < BN / 2; c += 32) {
+        for (int c = 0; c < 64; c += 32) {
           uint32_t r[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(acc[c + i]);
           if (lane == 0) store_wait<0>();
           __syncwarp();
           stage_row(obuf, lane, r);
-          send<true>(a, q.prob, obuf, q.ybase, row, q.n * BN + half * (BN / 2) + c, lane);
+          send<true>(b, &b.tc, obuf, q.ybase, row, q.n * 128 + half * 64 + c, lane);
           __syncwarp();
         }
         continue;
@@ -594,7 +612,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         // all one way) and a loss is fp32, so tensor memory sums kLseSlab stages at a time and registers the rest.
         constexpr float kLog2e = 1.44269504088896340736f;
         float v[64];
-        const int row = q.m * 256 + (int)rank * kHalfM + qd * 32, c0 = half * 64, left = a.N - (q.n * BN + c0);
+        const int row = q.m * 256 + (int)rank * kHalfM + qd * 32, c0 = half * 64, left = b.N - (q.n * 256 + c0);
         bool ok = true;
         for (int j = q.k0; j < q.k1; j += kLseSlab, ++it) {
           const int buf = it % kBufs;
@@ -633,7 +651,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           s0 += ex2(fmaf(v[i], kLog2e, -base));
           s1 += ex2(fmaf(v[i + 1], kLog2e, -base));
         }
-        if (row + lane < a.M) a.part[(int64_t)(row + lane) * (4 * a.nt) + 4 * q.n + half] = make_float2(m, s0 + s1);
+        if (row + lane < b.M) a.part[(int64_t)(row + lane) * (4 * b.nt) + 4 * q.n + half] = make_float2(m, s0 + s1);
         continue;
       }
       const int buf = it % kBufs;
@@ -650,35 +668,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           else if (a.act == kGelu) glu_block<kGelu, bwd>(a, tb, c, which, obuf, row, col, lane);
           else glu_block<kRelu, bwd>(a, tb, c, which, obuf, row, col, lane);
         }
-      } else if constexpr (EPI == kStoreBf16) {
+      } else if constexpr (EPI == kStore) {
+        const int w0 = half * (b.bn / 2), w1 = w0 + b.bn / 2, n0 = q.n * b.bn;
+        if (b.f32) {
 #pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 64) {
-          uint32_t r0[32], r1[32], w[32];
-          tmem_ld32_nowait(tb + c, r0);
-          tmem_ld32_nowait(tb + c + 32, r1);
-          tmem_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            w[i] = pack(__uint_as_float(r0[2 * i]), __uint_as_float(r0[2 * i + 1]));
-            w[16 + i] = pack(__uint_as_float(r1[2 * i]), __uint_as_float(r1[2 * i + 1]));
+          for (int c = w0; c < w1; c += 32) {
+            uint32_t r[32];
+            tmem_ld32_nowait(tb + c, r);
+            tmem_wait();
+            if (lane == 0) store_wait<0>();
+            __syncwarp();
+            stage_row(obuf, lane, r);
+            send<true>(b, &b.tc, obuf, q.ybase, row, n0 + c, lane);
+            __syncwarp();
           }
-          if (lane == 0) store_wait<0>();
-          __syncwarp();
-          stage_row(obuf, lane, w);
-          send<false>(a, q.prob, obuf, q.ybase, row, q.n * BN + c, lane);
-          __syncwarp();
-        }
-      } else if constexpr (EPI == kStoreF32) {
+        } else {
 #pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-          uint32_t r[32];
-          tmem_ld32_nowait(tb + c, r);
-          tmem_wait();
-          if (lane == 0) store_wait<0>();
-          __syncwarp();
-          stage_row(obuf, lane, r);
-          send<true>(a, q.prob, obuf, q.ybase, row, q.n * BN + c, lane);
-          __syncwarp();
+          for (int c = w0; c < w1; c += 64) {
+            uint32_t r0[32], r1[32], w[32];
+            tmem_ld32_nowait(tb + c, r0);
+            tmem_ld32_nowait(tb + c + 32, r1);
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              w[i] = pack(__uint_as_float(r0[2 * i]), __uint_as_float(r0[2 * i + 1]));
+              w[16 + i] = pack(__uint_as_float(r1[2 * i]), __uint_as_float(r1[2 * i + 1]));
+            }
+            if (lane == 0) store_wait<0>();
+            __syncwarp();
+            stage_row(obuf, lane, w);
+            send<false>(b, &b.tc, obuf, q.ybase, row, n0 + c, lane);
+            __syncwarp();
+          }
         }
       } else if constexpr (EPI == kLse) {
         // maximum and sum of exp2 of this lane's row over its quarter of the tile's columns
@@ -686,7 +707,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         float m = -INFINITY, s = 0.f;
 #pragma unroll
         for (int c = half * 64; c < half * 64 + 64; c += 32) {
-          const int left = a.N - (q.n * BN + c);
+          const int left = b.N - (q.n * 256 + c);
           uint32_t r[32];
           tmem_ld32_nowait(tb + c, r);
           tmem_wait();
@@ -711,18 +732,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           s += s0 + s1;
           m = nm;
         }
-        if (row + lane < a.M) a.part[(int64_t)(row + lane) * (4 * a.nt) + 4 * q.n + half] = make_float2(m, s);
+        if (row + lane < b.M) a.part[(int64_t)(row + lane) * (4 * b.nt) + 4 * q.n + half] = make_float2(m, s);
       } else if constexpr (EPI == kProb) {
         constexpr float kLog2e = 1.44269504088896340736f;
         const int i0 = row + lane;
-        const int64_t tg = i0 < a.M ? a.target[i0] : -1;
+        const int64_t tg = i0 < b.M ? a.target[i0] : -1;
         const bool live = tg >= 0 && tg < a.V;
         const float z = live ? a.lse[i0] * kLog2e : 0.f, d = live ? a.dloss[i0] : 0.f;
         const uint32_t mask = live ? 0xFFFFFFFFu : 0u;            // a held-out row is zeros whatever its logits are
         const int64_t tc = live ? tg - a.v0 : -1;                 // the target's column of this piece
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
-          const int col = q.n * BN + half * 64 + c;
+          const int col = q.n * 256 + half * 64 + c;
           uint32_t r[32], w[16];
           tmem_ld32_nowait(tb + half * 64 + c, r);
           tmem_wait();
@@ -743,7 +764,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           }
           stage_half(obuf, lane, c / 32, w);
         }
-        send<false>(a, 0, obuf, 0, row, q.n * BN + half * 64, lane);
+        send<false>(b, &b.tc, obuf, 0, row, q.n * 256 + half * 64, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -831,19 +852,37 @@ template <auto kernel> int pair_slots(int smem, int threads) {
   return s;
 }
 
-template <int EPI, bool A_MN, bool B_MN, int BN, int P = 1> int launch_pair(const PairArgs &a, cudaStream_t stream) {
-  constexpr auto k = k_pair<EPI, A_MN, B_MN, BN, P>;
+template <int EPI, int P = 1> int launch_pair(const PairArgs &a, cudaStream_t stream) {
+  constexpr auto k = k_pair<EPI, P>;
   constexpr int smem = smem_bytes<EPI, P>();
   const int slots = pair_slots<k>(smem, threads_of<EPI>());
   if (!slots) return fb::cuda_error(cudaGetLastError(), "k_pair shared memory");
-  const int64_t tiles = (int64_t)a.mt * a.nt * a.probs * a.splits;
+  const int tiles = a.tile0[a.n];
   if (tiles == 0) return FB_OK;
-  const unsigned grid = 2 * (unsigned)std::min<int64_t>(tiles, slots);
-  FB_TRY_CUDA(fb::launch(k, grid, threads_of<EPI>(), smem, stream, a));
+  FB_TRY_CUDA(fb::launch(k, 2 * (unsigned)std::min(tiles, slots), threads_of<EPI>(), smem, stream, a));
   FB_LAUNCHED("k_pair");
   return FB_OK;
 }
 
 inline int tiles_of(int64_t n, int t) { return (int)((n + t - 1) / t); }
+
+// A launch of one product of M x N over kb stages, 256-column tiles of `tile` result columns, unsplit.
+inline void one_product(PairArgs &a, int64_t M, int64_t N, int tile, int kb, int terms) {
+  std::memset(&a, 0, sizeof(a));
+  PairProb &b = a.p[0];
+  a.n = 1;
+  b.bn = 256;
+  b.mt = tiles_of(M, 256);
+  b.nt = tiles_of(N, tile);
+  b.splits = 1;
+  b.kb[0] = kb;
+  b.kb[1] = terms > 1 ? kb : 0;
+  b.kper = terms * kb;
+  b.M = (int)M;
+  b.N = (int)N;
+  b.has_tc = 1;
+  a.tile0[1] = b.mt * b.nt;
+  a.err = err_word();
+}
 
 }  // namespace fbpair

@@ -197,8 +197,8 @@ int check(const fb_softmax_xent *a, bool bwd) {
 Mat rows_from(const Mat &m, int64_t r) { return Mat{static_cast<const uint16_t *>(m.p) + r * m.ld, m.ld, m.plane}; }
 
 int logits_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &wp, int cols, float *l, int64_t pr) {
-  const Term t{wp, 0, a.D};
-  return pair_rows(c, h, a.n, a.D, &t, 1, false, cols, Out{l, pr, FB_F32, 0});
+  const Product p = rows_product(h, a.n, a.D, wp, false, cols, Out{l, pr, FB_F32, 0});
+  return products(c, &p, 1);
 }
 
 int forward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
@@ -234,14 +234,10 @@ int backward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
                              G, a.n * pr));
       FB_LAUNCHED("k_xent_grad");
     }
-    if (a.dh) {
-      const Term t{wp, 0, cols};
-      FBH_TRY(pair_rows(c, Gm, a.n, cols, &t, 1, true, a.D, Out{a.dh, a.lddh, FB_F32, v0 > 0}));
-    }
-    if (a.dw) {
-      const Out o{static_cast<float *>(a.dw) + v0 * a.lddw, a.lddw, FB_F32, a.accumulate};
-      FBH_TRY(pair_columns(c, Gm, a.n, cols, 0, 1, cols, h, a.D, &o));
-    }
+    void *dw = a.dw ? static_cast<float *>(a.dw) + v0 * a.lddw : nullptr;
+    const Product p[2] = {rows_product(Gm, a.n, cols, wp, true, a.D, Out{a.dh, a.lddh, FB_F32, v0 > 0}),
+                          columns_product(Gm, a.n, cols, h, a.D, Out{dw, a.lddw, FB_F32, a.accumulate})};
+    FBH_TRY(products(c, p, 2));
     if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
   return FB_OK;
@@ -250,16 +246,9 @@ int backward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
 // The common fields of a launch over the logits of rows h against table rows w.
 int logits_args(fbpair::PairArgs &p, const fb_softmax_xent &a, const Mat &h, int64_t n, const Mat &w, int cols) {
   using namespace fbpair;
-  std::memset(&p, 0, sizeof(p));
-  p.phases = p.probs = p.splits = 1;
-  p.kb[0] = p.kper = tiles_of(a.D, BK);
-  p.mt = tiles_of(n, 256);
-  p.nt = tiles_of(cols, 256);
-  p.M = (int)n;
-  p.N = cols;
-  p.err = err_word();
-  FBH_TRY(make_map(&p.ta[0], h.p, n, a.D, h.ld, kHalfM));
-  return make_map(&p.tb[0], w.p, cols, a.D, w.ld, 128);
+  one_product(p, n, cols, 256, tiles_of(a.D, BK), 1);
+  FBH_TRY(make_map(&p.p[0].ta[0], h.p, n, a.D, h.ld, kHalfM));
+  return make_map(&p.p[0].tb[0], w.p, cols, a.D, w.ld, 128);
 }
 
 // lse and loss of rows r0 .. r0 + n - 1 (h: those rows) from their partials.
@@ -296,8 +285,7 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
     PairArgs p;
     FBH_TRY(logits_args(p, a, hp, n, w, (int)a.V));
     p.part = part;
-    FBH_TRY((p.kb[0] > kLseSlab ? launch_pair<kLseLong, false, false, 256>(p, c.stream)
-                                : launch_pair<kLse, false, false, 256>(p, c.stream)));
+    FBH_TRY(p.p[0].kb[0] > kLseSlab ? launch_pair<kLseLong>(p, c.stream) : launch_pair<kLse>(p, c.stream));
     FBH_TRY(finish<uint16_t>(c, a, part, 4 * nt, hp, w, r0, n));
   }
   return FB_OK;
@@ -325,19 +313,14 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
       p.dloss = a.dloss;
       p.V = a.V;
       p.v0 = v0;
-      p.has_tc = 1;
-      FBH_TRY(make_map(&p.tc[0], G, a.n, cols, pr, 32));
-      FBH_TRY((launch_pair<kProb, false, false, 256>(p, c.stream)));
+      FBH_TRY(make_map(&p.p[0].tc, G, a.n, cols, pr, 32));
+      FBH_TRY(launch_pair<kProb>(p, c.stream));
     }
-    if (a.dh) {
-      const Term t{wp, 0, cols};
-      FBH_TRY(pair_rows(c, Gm, a.n, cols, &t, 1, true, a.D,
-                        sum ? Out{acc, lds, FB_F32, v0 > 0} : Out{a.dh, a.lddh, FB_BF16, 0}));
-    }
-    if (a.dw) {
-      const Out o{static_cast<uint8_t *>(a.dw) + v0 * a.lddw * elem(a.grad_type), a.lddw, a.grad_type, a.accumulate};
-      FBH_TRY(pair_columns(c, Gm, a.n, cols, 0, 1, cols, h, a.D, &o));
-    }
+    void *dw = a.dw ? static_cast<uint8_t *>(a.dw) + v0 * a.lddw * elem(a.grad_type) : nullptr;
+    const Product p[2] = {rows_product(Gm, a.n, cols, wp, true, a.D,
+                                       sum ? Out{acc, lds, FB_F32, v0 > 0} : Out{a.dh, a.lddh, FB_BF16, 0}),
+                          columns_product(Gm, a.n, cols, h, a.D, Out{dw, a.lddw, a.grad_type, a.accumulate})};
+    FBH_TRY(products(c, p, 2));
     if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
   if (sum && !c.dry) {
