@@ -13,6 +13,7 @@
 // activation between them in a kernel of its own.
 #include "few_rows.cuh"
 #include "pair_gemm.cuh"
+#include "planes.cuh"
 
 namespace {
 
@@ -20,43 +21,44 @@ using namespace fbh;
 
 constexpr int kSilu = FB_ACT_SILU, kGelu = FB_ACT_GELU;
 
-// v as three bf16 planes `plane` elements apart (see k_operands).
-__device__ __forceinline__ void put3(uint16_t *p, int64_t plane, float v) {
-  const uint32_t b0 = __float_as_uint(v) & 0xFFFF0000u;
-  const bool fin = (b0 & 0x7F800000u) != 0x7F800000u;
-  const float r1 = fin ? v - __uint_as_float(b0) : 0.f;
-  const uint32_t b1 = __float_as_uint(r1) & 0xFFFF0000u;
-  p[0] = (uint16_t)(b0 >> 16);
-  p[plane] = (uint16_t)(b1 >> 16);
-  p[2 * plane] = (uint16_t)(__float_as_uint(r1 - __uint_as_float(b1)) >> 16);
-}
-
 // fp32: h = act(g) u over rows x Fp elements, as planes; gu rows are [g | u].
-template <int ACT> __global__ void k_glu_fwd(const float *gu, uint16_t *h, int64_t rows, int Fp) {
+template <int ACT> __global__ void __launch_bounds__(256) k_glu_fwd(const float *gu, uint16_t *h, int64_t rows, int Fp) {
   fb::pdl_enter();
   const int64_t n = rows * Fp;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     const float *p = gu + i / Fp * 2 * Fp + i % Fp;
-    put3(h + i, n, fbact::act_exact<ACT>(p[0]).x * p[Fp]);
+    const float4 g = *reinterpret_cast<const float4 *>(p), u = *reinterpret_cast<const float4 *>(p + Fp);
+    fbplanes::put4(h + i, n, fbact::act_exact<ACT>(g.x).x * u.x, fbact::act_exact<ACT>(g.y).x * u.y,
+                   fbact::act_exact<ACT>(g.z).x * u.z, fbact::act_exact<ACT>(g.w).x * u.w);
   }
 }
 
 // fp32: h, and dgu rows [dg | du], as planes, from gu rows [g | u] and dh.
 template <int ACT>
-__global__ void k_glu_bwd(const float *gu, const float *dh, uint16_t *h, uint16_t *dgu, int64_t rows, int Fp) {
+__global__ void __launch_bounds__(256) k_glu_bwd(const float *gu, const float *dh, uint16_t *h, uint16_t *dgu, int64_t rows,
+                                                 int Fp) {
   fb::pdl_enter();
   const int64_t n = rows * Fp;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     const int64_t at = i / Fp * 2 * Fp + i % Fp;
-    const float uv = gu[at + Fp], d = dh[i];
-    const float2 a = fbact::act_exact<ACT>(gu[at]);
-    put3(dgu + at, 2 * n, d * uv * a.y);
-    put3(dgu + at + Fp, 2 * n, d * a.x);
-    put3(h + i, n, a.x * uv);
+    float g[4], u[4], d[4];
+    *reinterpret_cast<float4 *>(g) = *reinterpret_cast<const float4 *>(gu + at);
+    *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(gu + at + Fp);
+    *reinterpret_cast<float4 *>(d) = *reinterpret_cast<const float4 *>(dh + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 a = fbact::act_exact<ACT>(g[k]);
+      g[k] = d[k] * u[k] * a.y;
+      d[k] *= a.x;
+      u[k] *= a.x;
+    }
+    fbplanes::put4(dgu + at, 2 * n, g[0], g[1], g[2], g[3]);
+    fbplanes::put4(dgu + at + Fp, 2 * n, d[0], d[1], d[2], d[3]);
+    fbplanes::put4(h + i, n, u[0], u[1], u[2], u[3]);
   }
 }
 
-unsigned blocks_for(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, 148 * 16)); }
+unsigned blocks_for(int64_t n) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 1023) / 1024, 148 * 8)); }
 
 int check(const fb_gated_ffn *a, bool bwd) {
   if (!a) return fb::set_error(FB_ERR_ARG, "gated_ffn: null arguments");

@@ -1,50 +1,58 @@
 // See head.cuh.
 #include "head.cuh"
 #include <algorithm>
+#include "planes.cuh"
 
 namespace {
 
 struct Job {
   const void *src;
-  int64_t lds, rows, ldd, plane;
+  int64_t lds, plane;
   void *dst;
-  int cols;
+  int ldd, cols, wide;                       // wide: 16-byte (8-byte) loads of the source's groups of 4
+  uint32_t groups, per_row;                  // groups of 4 columns, in all and a row
   unsigned first;                            // first CTA of the job
 };
 struct Jobs {
   Job j[fbh::kMaxOperands];
   int n;
 };
-constexpr int kPerCta = 256 * 8;             // elements a CTA lays out
+constexpr int kGroups = 2;                   // groups of 4 a thread lays out
 
-// bf16 rows into a pitch, or (planes) fp32 x as x0 + x1 + x2: the leading 8
-// significant bits, the next 8, the last 8.  Cutting bits off is exact and
-// cannot overflow; x0 of an infinity or NaN carries it alone.
+// bf16 rows into a pitch of whole 128-byte lines, or (planes) fp32 rows split.
 template <bool PLANES> __global__ void __launch_bounds__(256) k_operands(const __grid_constant__ Jobs a) {
   fb::pdl_enter();
   int q = 0;
   while (q + 1 < a.n && blockIdx.x >= a.j[q + 1].first) ++q;
   const Job &j = a.j[q];
-  const int64_t total = j.rows * j.cols, at = (int64_t)(blockIdx.x - j.first) * kPerCta;
+  const uint32_t at = (blockIdx.x - j.first) * (256 * kGroups) + threadIdx.x;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int64_t i = at + e * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int64_t r = i / j.cols;
-    const int c = (int)(i - r * j.cols);
-    uint16_t *d = static_cast<uint16_t *>(j.dst) + r * j.ldd + c;
-    if (!PLANES) {
-      *d = static_cast<const uint16_t *>(j.src)[r * j.lds + c];
+  for (int e = 0; e < kGroups; ++e) {
+    const uint32_t i = at + e * 256;
+    if (i >= j.groups) return;
+    const uint32_t r = i / j.per_row;
+    const int c = (int)(i - r * j.per_row) * 4;
+    uint16_t *d = static_cast<uint16_t *>(j.dst) + (int64_t)r * j.ldd + c;
+    if constexpr (PLANES) {
+      const float *s = static_cast<const float *>(j.src) + r * j.lds + c;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (j.wide) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(s);
+      else
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c + k < j.cols) v[k] = s[k];
+      fbplanes::put4(d, j.plane, v[0], v[1], v[2], v[3]);
     } else {
-      const float x = static_cast<const float *>(j.src)[r * j.lds + c];
-      const uint32_t b0 = __float_as_uint(x) & 0xFFFF0000u;
-      const bool fin = (b0 & 0x7F800000u) != 0x7F800000u;
-      const float r1 = fin ? x - __uint_as_float(b0) : 0.f;
-      const uint32_t b1 = __float_as_uint(r1) & 0xFFFF0000u;
-      const uint32_t b2 = __float_as_uint(r1 - __uint_as_float(b1));
-      d[0] = (uint16_t)(b0 >> 16);
-      d[j.plane] = (uint16_t)(b1 >> 16);
-      d[2 * j.plane] = (uint16_t)(b2 >> 16);
+      const uint16_t *s = static_cast<const uint16_t *>(j.src) + r * j.lds + c;
+      ushort4 v = make_ushort4(0, 0, 0, 0);
+      if (j.wide) v = *reinterpret_cast<const ushort4 *>(s);
+      else {
+        v.x = s[0];
+        if (c + 1 < j.cols) v.y = s[1];
+        if (c + 2 < j.cols) v.z = s[2];
+        if (c + 3 < j.cols) v.w = s[3];
+      }
+      *reinterpret_cast<ushort4 *>(d) = v;
     }
   }
 }
@@ -68,8 +76,13 @@ int operands(Call &c, int type, const Operand *ops, int n) {
     if (!p) return fb::set_error(FB_ERR_ARG, "workspace too small");
     *o.out = Mat{p, ld, planes ? plane : 0};
     if (o.rows == 0) continue;
-    jobs.j[jobs.n++] = Job{o.src.p, o.src.ld, o.rows, ld, plane, p, o.cols, ctas};
-    ctas += (unsigned)((o.rows * o.cols + kPerCta - 1) / kPerCta);
+    const uint32_t per_row = (uint32_t)(o.cols + 3) / 4;
+    const int64_t groups = o.rows * per_row;
+    if (groups > UINT32_MAX / 2) return fb::set_error(FB_ERR_UNSUPPORTED, "operand of more than 2^33 elements");
+    const int es = elem(type);
+    const bool wide = o.cols % 4 == 0 && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * es)) & (4 * es - 1)) == 0;
+    jobs.j[jobs.n++] = Job{o.src.p, o.src.ld, plane, p, (int)ld, o.cols, wide, (uint32_t)groups, per_row, ctas};
+    ctas += (unsigned)((groups + 256 * kGroups - 1) / (256 * kGroups));
   }
   if (c.dry || jobs.n == 0) return FB_OK;
   FB_TRY_CUDA(fb::launch(planes ? k_operands<true> : k_operands<false>, ctas, 256, 0, c.stream, jobs));

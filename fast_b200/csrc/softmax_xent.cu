@@ -12,6 +12,7 @@
 #include <cmath>
 #include "few_rows.cuh"
 #include "pair_gemm.cuh"
+#include "planes.cuh"
 
 namespace {
 
@@ -90,8 +91,9 @@ __global__ void __launch_bounds__(TH == 32 ? 128 : TH) k_xent_finish(const float
   loss[r] = tg < 0 ? 0.f : (tg >= V ? NAN : z - l);
 }
 
-// One CTA per row: the piece's maximum and sum join the row's state; the
-// target's logit is picked up when the piece holds it.  last: lse and loss.
+// One CTA per row (pitch ldl, a multiple of 4): the piece's maximum and sum
+// join the row's state; the target's logit is picked up when the piece holds
+// it.  last: lse and loss.
 __global__ void __launch_bounds__(256) k_xent_rows(const float *l, int64_t ldl, int v0, int cols, int64_t V,
                                                    const int64_t *target, float *state, float *tl, float *loss,
                                                    float *lse, int first, int last) {
@@ -99,17 +101,18 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float *l, int64_t ldl, 
   fb::pdl_enter();
   const int64_t r = blockIdx.x;
   const float *p = l + r * ldl;
-  float m = -INFINITY;
-  bool nan = false;
-  for (int c = threadIdx.x; c < cols; c += 256) {
-    const float v = p[c];
-    nan |= isnan(v);
-    m = fmaxf(m, v);
+  MaxSum a{-INFINITY, 0.f};
+  for (int c = threadIdx.x * 4; c < cols; c += 1024) {
+    float v[4];
+    *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k >= cols) v[k] = -INFINITY;   // past the piece
+    const float m = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), a.m);
+    const float base = m == -INFINITY ? 0.f : m;           // nothing but -inf: zeros, and NaN stays NaN
+    a.s = a.s * expf(a.m - base) + expf(v[0] - base) + expf(v[1] - base) + expf(v[2] - base) + expf(v[3] - base);
+    a.m = m;
   }
-  MaxSum a{m, 0.f};
-  if (m != -INFINITY)
-    for (int c = threadIdx.x; c < cols; c += 256) a.s += expf(p[c] - m);
-  if (nan) a.s = NAN;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     a = join(a, MaxSum{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
@@ -133,25 +136,25 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float *l, int64_t ldl, 
   loss[r] = t < 0 ? 0.f : (t >= V ? NAN : z - lt);
 }
 
-// fp32 rows: G of one piece as three bf16 planes (see k_operands).  Rows held
-// out of the loss are zeros whatever their logits are.
-__global__ void k_xent_grad(const float *l, int64_t ldl, int v0, int cols, int64_t V, const int64_t *target,
-                            const float *lse, const float *dloss, uint16_t *G, int64_t plane) {
+// fp32 rows: G of one piece as planes (pitch ldl, a multiple of 4; the columns
+// past cols are never read).  Rows held out of the loss are zeros whatever
+// their logits are.
+__global__ void __launch_bounds__(256) k_xent_grad(const float *l, int64_t ldl, int v0, int cols, int64_t V,
+                                                   const int64_t *target, const float *lse, const float *dloss,
+                                                   uint16_t *G, int64_t plane) {
   fb::pdl_enter();
   const int64_t r = blockIdx.x;
   const int64_t t = target[r];
   const bool live = t >= 0 && t < V;
   const float z = lse[r], d = dloss[r];
-  for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < cols; c += gridDim.y * blockDim.x) {
-    float v = 0.f;
-    if (live) v = d * (expf(l[r * ldl + c] - z) - (t == v0 + c ? 1.f : 0.f));
-    uint16_t *p = G + r * ldl + c;
-    const uint32_t b0 = __float_as_uint(v) & 0xFFFF0000u;
-    const float r1 = v - __uint_as_float(b0);
-    const uint32_t b1 = __float_as_uint(r1) & 0xFFFF0000u;
-    p[0] = (uint16_t)(b0 >> 16);
-    p[plane] = (uint16_t)(b1 >> 16);
-    p[2 * plane] = (uint16_t)(__float_as_uint(r1 - __uint_as_float(b1)) >> 16);
+  for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(l + r * ldl + c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = d * (expf(v[k] - z) - (t == v0 + c + k ? 1.f : 0.f));
+    }
+    fbplanes::put4(G + r * ldl + c, plane, v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -229,7 +232,7 @@ int backward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
     const Mat wp = rows_from(w, v0), Gm{G, pr, a.n * pr};
     FBH_TRY(logits_f32(c, a, h, wp, cols, l, pr));
     if (!c.dry) {
-      FB_TRY_CUDA(fb::launch(k_xent_grad, dim3((unsigned)a.n, (unsigned)std::min(64, (cols + 255) / 256)), 256, 0,
+      FB_TRY_CUDA(fb::launch(k_xent_grad, dim3((unsigned)a.n, (unsigned)std::min(64, (cols + 1023) / 1024)), 256, 0,
                              c.stream, (const float *)l, pr, (int)v0, cols, a.V, a.target, (const float *)a.lse, a.dloss,
                              G, a.n * pr));
       FB_LAUNCHED("k_xent_grad");
