@@ -54,9 +54,9 @@ using fbact::kSilu;
 constexpr int BK = 64;                        // k per stage: one 128-byte swizzle row of bf16
 constexpr int kHalfM = 128;                   // rows of a tile per CTA
 constexpr int kABytes = kHalfM * BK * 2;      // 16 KB
-// B of a stage: BN / 2 <= 128 rows; planes: 64 rows of each
+// B of a stage: BN / 2 <= 128 rows; planes (a stage holds one plane of a slab): 64 rows
 template <int P> __host__ __device__ constexpr int b_bytes() { return (P == 3 ? 64 : 128) * BK * 2; }
-template <int P> __host__ __device__ constexpr int stage_bytes() { return P * (kABytes + b_bytes<P>()); }
+template <int P> __host__ __device__ constexpr int stage_bytes() { return kABytes + b_bytes<P>(); }
 constexpr int kBox = BK * 128;                // MN-major box: 64 k rows of 64 elements
 constexpr int kWarpEpi0 = 4;
 template <int EPI> __host__ __device__ constexpr int epi_warps() {
@@ -70,7 +70,7 @@ template <int EPI> __host__ __device__ constexpr int out_bytes() {
   return EPI == kGluBwd ? 3 * kStageOut : (EPI == kLse || EPI == kLseLong ? 0 : kStageOut);
 }
 template <int EPI, int P> __host__ __device__ constexpr int stages() {
-  return P == 3 ? 2 : (EPI == kGluBwd ? 4 : (EPI == kProb ? 5 : 6));
+  return P == 3 ? 8 : (EPI == kGluBwd ? 4 : (EPI == kProb ? 5 : 6));
 }
 template <int EPI, int P> __host__ __device__ constexpr int smem_bytes() {
   return 1024 + stages<EPI, P>() * stage_bytes<P>() + epi_warps<EPI>() * out_bytes<EPI>() + 256;
@@ -399,9 +399,6 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
   }
 }
 
-// Planes of the six products of P = 3, smallest first (one hex digit each, from the right).
-constexpr uint32_t kPlaneA = 0x001102u, kPlaneB = 0x010120u;
-
 template <int EPI, int P = 1>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1) k_pair(const __grid_constant__ PairArgs a) {
   static_assert(P == 1 || (P == 3 && EPI == kStore), "planes feed plain products");
@@ -411,7 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
   auto sA = [&](int s) { return smem + s * kStageBytes; };
-  auto sB = [&](int s) { return smem + s * kStageBytes + P * kABytes; };
+  auto sB = [&](int s) { return smem + s * kStageBytes + kABytes; };
   uint8_t *outs = smem + kStages * kStageBytes;
   uint64_t *bars = reinterpret_cast<uint64_t *>(outs + kEpiWarps * out_bytes<EPI>());
   uint64_t *full = bars, *empty = bars + kStages, *accf = bars + 2 * kStages, *acce = accf + 2;
@@ -468,18 +465,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         const bool dh = EPI == kGluBwd && p == 1;
         const int bn = dh ? 128 : bn_;
         const bool bmn = dh || bmn_;
-        if (turn > 0 && !wait(empty + s, (turn - 1) & 1, abort_flag, err)) {
-          stop = true;
-          break;
-        }
-        if (one) {
-          const CUtensorMap *ma = &b.ta[p], *mb = dh ? &a.tw : &b.tb[kDual ? rank : p];
-          const int n0 = kDual && !dh ? q.n * 128 : q.n * bn + (int)rank * (bn / 2);
-          const uint32_t full_at = leader_addr(full + s);
-          if (rank == 0) mbar_expect_tx(full + s, 2u * P * (uint32_t)(kABytes + bn / 2 * BK * 2));
-#pragma unroll
-          for (int z = 0; z < P; ++z) {
-            uint8_t *sa = sA(s) + z * kABytes, *sb = sB(s) + z * kBBytes;
+        const CUtensorMap *ma = &b.ta[p], *mb = dh ? &a.tw : &b.tb[kDual ? rank : p];
+        const int n0 = kDual && !dh ? q.n * 128 : q.n * bn + (int)rank * (bn / 2);
+#pragma unroll 1
+        for (int k = 0; k < P; ++k) {
+          if (turn > 0 && !wait(empty + s, (turn - 1) & 1, abort_flag, err)) {
+            stop = true;
+            break;
+          }
+          if (one) {
+            const int z = (3 - k) % 3;        // planes 0, 2, 1: the order the products need them in
+            const uint32_t full_at = leader_addr(full + s);
+            uint8_t *sa = sA(s), *sb = sB(s);
+            if (rank == 0) mbar_expect_tx(full + s, 2u * (uint32_t)(kABytes + bn / 2 * BK * 2));
             auto load = [&](void *dst, const CUtensorMap *map, int x, int y) {
               if (P == 1) load2(dst, map, full_at, x, y);
               else load3(dst, map, full_at, x, y, z);
@@ -497,9 +495,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
               load(sb, mb, BK * jj, n0);
             }
           }
+          __syncwarp();
+          if (++s == kStages) s = 0, ++turn;
         }
-        __syncwarp();
-        if (++s == kStages) s = 0, ++turn;
+        if (stop) break;
       }
     }
     // the MMAs have read every stage (and their arrivals reached this CTA) before it leaves
@@ -522,7 +521,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         for (int j = q.k0; j < q.k1; ++j) {
           const bool dh = EPI == kGluBwd && j >= kb0, bmn = dh || bmn_;
           const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(bn, amn, bmn);
-          const uint64_t bd0 = sdesc(smem_u32(smem + P * kABytes), bmn), adv_b = bmn ? (2048 >> 4) : 2;
+          const uint64_t bd0 = sdesc(smem_u32(smem + kABytes), bmn), adv_b = bmn ? (2048 >> 4) : 2;
           // a new accumulator at the tile's start, or for every slab; dh's columns start at its first stage
           const bool next = P == 3 || j == q.k0 || (EPI == kLseLong && (j & (kLseSlab - 1)) == 0);
           const bool fresh = next || (dh && j == kb0);
@@ -535,26 +534,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
             stop = true;
             break;
           }
-          tc_fence_after();
           const bool last = P == 3 || j + 1 == q.k1 || (EPI == kLseLong && ((j + 1) & (kLseSlab - 1)) == 0);
-          if (one) {
-            const uint32_t d = tmem + (dh ? 256u : buf * 256u);
-            const uint64_t at = (uint64_t)(s * (kStageBytes >> 4));
+          const uint32_t d = tmem + (dh ? 256u : buf * 256u);
+          // one product of 64 k: A of stage sa, B of stage sb
+          auto issue = [&](int sa, int sb, bool first) {
+            const uint64_t ad = ad0 + (uint64_t)(sa * (kStageBytes >> 4)), bd = bd0 + (uint64_t)(sb * (kStageBytes >> 4));
 #pragma unroll
-            for (int pr = 0; pr < (P == 3 ? 6 : 1); ++pr) {
-              const uint64_t za = (kPlaneA >> (4 * pr) & 15) * (uint64_t)(kABytes >> 4),
-                             zb = (kPlaneB >> (4 * pr) & 15) * (uint64_t)(kBBytes >> 4);
-#pragma unroll
-              for (int kk = 0; kk < BK / 16; ++kk)
-                mma2(d, ad0 + at + (P == 3 ? za : 0) + kk * adv_a, bd0 + at + (P == 3 ? zb : 0) + kk * adv_b, idesc,
-                     (fresh && kk == 0 && pr == 0) ? 0u : 1u);
+            for (int kk = 0; kk < BK / 16; ++kk)
+              mma2(d, ad + kk * adv_a, bd + kk * adv_b, idesc, (first && kk == 0) ? 0u : 1u);
+          };
+          if constexpr (P == 1) {
+            tc_fence_after();
+            if (one) {
+              issue(s, s, fresh);
+              commit2(empty + s);
+              if (last) commit2(accf + buf);
             }
-            commit2(empty + s);
-            if (last) commit2(accf + buf);
+            __syncwarp();
+            if (++s == kStages) s = 0, ++turn;
+          } else {
+            // the slab's planes 0, 2, 1 in stages s, s1, s2: products 20, 02, 11, 10, 01, 00, smallest first, each
+            // stage freed after its last one
+            const int s1 = s + 1 == kStages ? 0 : s + 1, s2 = s1 + 1 == kStages ? 0 : s1 + 1;
+            const uint32_t t1 = turn + (s1 == 0 ? 1 : 0), t2 = t1 + (s2 == 0 ? 1 : 0);
+            if (!wait(full + s1, t1 & 1, abort_flag, err)) {
+              stop = true;
+              break;
+            }
+            tc_fence_after();
+            if (one) {
+              issue(s1, s, true);
+              issue(s, s1, false);
+              commit2(empty + s1);
+            }
+            __syncwarp();
+            if (!wait(full + s2, t2 & 1, abort_flag, err)) {
+              stop = true;
+              break;
+            }
+            tc_fence_after();
+            if (one) {
+              issue(s2, s2, false);
+              issue(s2, s, false);
+              issue(s, s2, false);
+              commit2(empty + s2);
+              issue(s, s, false);
+              commit2(empty + s);
+              commit2(accf + buf);
+            }
+            __syncwarp();
+            s = s2 + 1 == kStages ? 0 : s2 + 1;
+            turn = t2 + (s == 0 ? 1 : 0);
           }
-          __syncwarp();
           if (last) ++it;
-          if (++s == kStages) s = 0, ++turn;
         }
       }
     }
