@@ -92,21 +92,30 @@ void plan(PairArgs &a, bool planes) {
     double least = 0;
     for (int part : {longest, 2 * mean, mean, (mean + 1) / 2, (mean + 2) / 3}) {
       if (part > longest || part < 1) continue;
-      int64_t at = 0;
-      double load[256] = {0}, sum = 0;
-      const int n = std::min(slots, 256);
+      // the busiest pair is among those that get a product's first tile
+      int64_t at = 0, starts[kMaxProbs];
+      for (int i = 0; i < a.n; ++i) {
+        const PairProb &b = a.p[i];
+        starts[i] = at % slots;
+        at += (int64_t)b.mt * b.nt * split_of(b.kb[0] + b.kb[1], part, planes);
+      }
+      at = 0;
+      double load[kMaxProbs] = {0}, sum = 0;
       for (int i = 0; i < a.n; ++i) {
         const PairProb &b = a.p[i];
         const int kb = b.kb[0] + b.kb[1], s = split_of(kb, part, planes);
         const int64_t t = (int64_t)b.mt * b.nt * s;
         const double cost = (double)((kb + s - 1) / s) * (planes ? kStagePlanes : (b.bn == 256 ? kStage256 : kStage128)) +
                             kTileCycles;
-        for (int c = 0; c < n; ++c) load[c] += cost * (double)((at + t - 1 - c + n) / n - (at - 1 - c + n) / n);
+        for (int k = 0; k < a.n; ++k) {
+          const int64_t c = slots - 1 - starts[k];
+          load[k] += cost * (double)((at + t + c) / slots - (at + c) / slots);
+        }
         at += t;
         if (s > 1) sum += 8.0 * s * b.M * b.N / 2600;
       }
       double busiest = 0;
-      for (int c = 0; c < n; ++c) busiest = std::max(busiest, load[c]);
+      for (int k = 0; k < a.n; ++k) busiest = std::max(busiest, load[k]);
       const double cycles = busiest + (sum > 0 ? sum + kSumCycles : 0);
       if (least == 0 || cycles < least) least = cycles, best = part;
     }

@@ -125,9 +125,8 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
   return p != 0;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Shared-memory address of `p` in the even CTA of the pair.
 __device__ __forceinline__ uint32_t leader_addr(const void *p) {
   uint32_t a;
@@ -417,18 +416,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(full + s, 1);                 // the even CTA's: its own expect, both CTAs' bytes
-      mbar_init(empty + s, 1);
+  if (warp == 0) {
+    if (lane < kStages) {
+      mbar_init(full + lane, 1);              // the even CTA's: its own expect, both CTAs' bytes
+      mbar_init(empty + lane, 1);
+    } else if (lane >= 16 && lane < 18) {
+      mbar_init(accf + lane - 16, 1);
+      mbar_init(acce + lane - 16, 2 * kEpiWarps);   // the even CTA's: both CTAs' epilogue warps
+    } else if (lane == 18) {
+      *abort_flag = 0;
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(accf + b, 1);
-      mbar_init(acce + b, 2 * kEpiWarps);     // the even CTA's: both CTAs' epilogue warps
-    }
-    *abort_flag = 0;
     fence_barrier_init();
+    __syncwarp();
   }
+  cluster_arrive();                           // the wait comes before a CTA first signals its peer
   if (warp == 1) alloc2(holder, kTmemCols);
   if (warp == 2 && lane < a.n) {
     const PairProb &b = a.p[lane];
@@ -440,10 +441,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();                             // both CTAs' barriers exist before either signals one
   tc_fence_after();
   const uint32_t tmem = *holder;
   fb::pdl_enter();
+  cluster_wait();                             // both CTAs' barriers exist
 
   const int total = a.tile0[a.n];
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
@@ -813,7 +814,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();                             // neither CTA leaves while the other may still reach into it
+  cluster_arrive();
+  cluster_wait();                             // neither CTA leaves while the other may still reach into it
   if (warp == 1) dealloc2(tmem, kTmemCols);
 }
 
