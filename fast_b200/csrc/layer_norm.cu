@@ -17,7 +17,11 @@
 // issued before the row ahead of it is reduced, which keeps memory busy
 // through the reductions.  Rows of 2 KB and more with 16-byte aligned operands
 // (BULK) come by bulk copies into a ring of rows in shared memory instead, up
-// to kRing bytes ahead of the row in work: BULKFIG  Elements move in the widest power-of-two groups (up
+// to kRing bytes ahead of the row in work (backward of 16,384 x 4,096 bf16 rows
+// with a residual: 185 us by register prefetch, 112 by the ring).  The forward's
+// ring and registers are small enough for four CTAs an SM: what is left is the
+// latency of a row's two reductions, and more rows in work cover it (88 us for
+// the same rows, 6.1 TB/s; 99 us with a ring of 64 KB and two CTAs).  Elements move in the widest power-of-two groups (up
 // to 16 bytes) that every operand's base, pitch and width allow.  All sums are
 // fp32.
 //
@@ -79,7 +83,7 @@ template <typename T, int V> __device__ __forceinline__ void pack(Vec<T, V> &v, 
 // `ops` operands, filled by bulk copies that thread 0 issues.  A stage is
 // consumed into registers before a CTA barrier, after which it is refilled, so
 // it needs no second barrier.
-constexpr int kRing = 64 * 1024;
+constexpr int kRing = 32 * 1024;
 constexpr int kMaxStages = 8;
 struct Ring {
   uint8_t *base;
@@ -201,7 +205,7 @@ struct FwdArgs {
 };
 
 template <typename T, int V, int G, int E, bool BULK>
-__global__ void __launch_bounds__(threads_of<G>(), G < 512 ? 3 : 1024 / G) k_layer_norm_fwd(const FwdArgs a) {
+__global__ void __launch_bounds__(threads_of<G>(), G < 512 ? 4 : 1024 / G) k_layer_norm_fwd(const FwdArgs a) {
   constexpr int kRows = threads_of<G>() / G, C = E / V;
   extern __shared__ __align__(16) float dyn[];   // gamma, beta
   __shared__ float2 sm[64];
@@ -526,7 +530,7 @@ struct Align {
   int vec(int D) const {
     int v = 16 / es;
     while (v > 1 && (D % v || (m & (v * es - 1)))) v >>= 1;
-    return v * es < 8 ? 1 : (es == 4 && v == 2 ? 1 : v);   // built for 16-byte groups, 8-byte ones of bf16, single ones
+    return es == 4 && v == 2 ? 1 : v;        // built for 16-byte groups, 8- and 4-byte ones of bf16, single ones
   }
 };
 
@@ -585,6 +589,7 @@ template <template <typename, int, int, int, bool> class K, typename... A> int b
   }
   if (V == 8) return by_group<K, bf16, 8, 16>(G, a...);
   if (V == 4) return by_group<K, bf16, 4, 16>(G, a...);
+  if (V == 2) return by_group<K, bf16, 2, 16>(G, a...);
   return wide ? K<bf16, 1, 1024, 16, false>::go(a...) : by_group<K, bf16, 1, 8>(G, a...);
 }
 
@@ -614,7 +619,7 @@ int bwd_ctas(int type, int V, int64_t n, int D) {
 template <auto kernel> int want_smem(size_t smem) {
   static bool set[64] = {false};
   int dev = 0;
-  if (smem <= 48 * 1024) return FB_OK;
+  if (smem <= 40 * 1024) return FB_OK;       // the 48 KB that need no asking include the static arrays
   cudaGetDevice(&dev);
   if (!set[dev & 63]) {
     FB_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -635,7 +640,7 @@ template <typename T, int V, int G, int E, bool BULK> struct Fwd {
   static int go(FwdArgs a, cudaStream_t st) {
     constexpr auto k = k_layer_norm_fwd<T, V, G, E, BULK>;
     size_t smem = 2 * sizeof(float) * pitch_of(a.D);
-    int per_sm = G < 512 ? 3 : 1024 / G;
+    int per_sm = G < 512 ? 4 : 1024 / G;
     if (BULK) {
       const int unit = (a.res ? 2 : 1) * (threads_of<G>() / G) * a.D * (int)sizeof(T);
       a.stages = stages_of(unit, smem);

@@ -46,7 +46,7 @@ def _c(k):
 # ---- layer norm --------------------------------------------------------------------------------------------------
 NORM = [(1, 1, 0, 0), (3, 7, 0, 0), (5, 100, 4, 0), (33, 413, 6, 1), (130, 64, 0, 0), (300, 128, 8, 0), (17, 500, 0, 2),
         (7, 1024, 0, 0), (9, 1027, 0, 0), (2, 2050, 0, 0), (5, 4096, 0, 0), (3, 5000, 0, 0), (3, 8200, 0, 0),
-        (2, 16384, 0, 0), (40000, 16, 0, 0)]
+        (2, 16384, 0, 0), (40000, 16, 0, 0), (2, 6144, 0, 0), (2, 6144, 1, 0), (3, 5890, 1, 0), (33, 414, 0, 0)]
 
 
 @pytest.mark.parametrize("n,d,pad,off", NORM)
@@ -127,7 +127,8 @@ def test_layer_norm_keeps_nonfinite_rows_to_themselves(cuda):
 
 # ---- gated feed-forward block ------------------------------------------------------------------------------------
 FFN = [(1, 16, 16, 0), (1, 100, 37, 0), (2, 1024, 520, 0), (3, 413, 50, 3), (7, 64, 129, 0), (130, 100, 400, 4),
-       (257, 72, 300, 0), (300, 264, 520, 8), (64, 33, 65, 1), (515, 130, 260, 0), (1000, 172, 688, 4)]
+       (257, 72, 300, 0), (300, 264, 520, 8), (64, 33, 65, 1), (515, 130, 260, 0), (1000, 172, 688, 4), (1, 11900, 24, 0),
+       (1, 12288, 16, 0), (8, 1500, 24, 1), (9, 100, 64, 0)]
 
 
 def _act(name, g):
