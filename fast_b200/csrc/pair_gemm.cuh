@@ -24,9 +24,10 @@
 //
 // CTA = 12 or 20 warps: 0 TMA producer (one lane), 1 TMEM allocator and, in the
 // even CTA, MMA issuer (one lane), the rest from 4 on epilogue: two per TMEM
-// lane quadrant, each half of the columns, or four, each a quarter, where the
-// epilogue takes an exponential of every element (with two its latencies were
-// in the open: 3.3 us a tile where the exponentials alone take 1.1).  Stages of 64 k travel through a ring
+// lane quadrant, each half of the columns.  Where the epilogue takes an
+// exponential of every element there are two such sets, one for each
+// accumulator: they work on alternate tiles, so that one's exponentials (the
+// XU pipe) fall into the other's loads, maxima and stores.  Stages of 64 k travel through a ring
 // of kStages; the loads of both CTAs count on the even CTA's barrier, MMA
 // completion frees the stage in both.  Accumulators: two of up to 256 columns
 // (the epilogue drains one while the other fills), one of 384 for kGluBwd.
@@ -103,7 +104,7 @@ struct PairArgs {
   int32_t *err;
   CUtensorMap tw, tc2[2];                     // kGluBwd: Wd; outputs dg, du
   int act;
-  float2 *part;                               // kLse: [M][4 nt] (max, sum of exp2) partials
+  float2 *part;                               // kLse: [M][2 nt] (kLseLong: [M][4 nt]) (max, sum of exp2) partials
   const int64_t *target;                      // kProb
   const float *lse, *dloss;
   int64_t V, v0;
@@ -403,6 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
   static_assert(P == 1 || (P == 3 && EPI == kStore), "planes feed plain products");
   constexpr int kStages = stages<EPI, P>(), kStageBytes = stage_bytes<P>(), kBBytes = b_bytes<P>();
   constexpr int kBufs = EPI == kGluBwd ? 1 : 2, kEpiWarps = epi_warps<EPI>();
+  constexpr bool kAlt = EPI == kLse || EPI == kProb;            // two sets of epilogue warps, alternate tiles
   constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd;      // B: 128 rows of Wg in one CTA, of Wu in the other
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
@@ -422,7 +424,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
       mbar_init(empty + lane, 1);
     } else if (lane >= 16 && lane < 18) {
       mbar_init(accf + lane - 16, 1);
-      mbar_init(acce + lane - 16, 2 * kEpiWarps);   // the even CTA's: both CTAs' epilogue warps
+      mbar_init(acce + lane - 16, kAlt ? kEpiWarps : 2 * kEpiWarps);   // the even CTA's: both CTAs' epilogue warps
     } else if (lane == 18) {
       *abort_flag = 0;
     }
@@ -593,7 +595,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
     }
     __syncwarp();
   } else if (warp >= kWarpEpi0) {
-    const int e = warp - kWarpEpi0, qd = warp & 3, half = e >> 2;   // (16 warps: the quarter)
+    const int e = warp - kWarpEpi0, qd = warp & 3, half = kAlt ? e >> 2 & 1 : e >> 2;   // (kLseLong: the quarter)
     const uint32_t tlane = (uint32_t)(qd * 32) << 16;
     uint8_t *obuf = outs + e * out_bytes<EPI>();
     uint32_t it = 0;
@@ -688,6 +690,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         continue;
       }
       const int buf = it % kBufs;
+      if (kAlt && buf != e >> 3) continue;
       if (!__all_sync(0xffffffffu, wait(accf + buf, (it / kBufs) & 1, abort_flag, err) ? 1 : 0)) break;
       tc_fence_after();
       const uint32_t tb = tmem + tlane + (uint32_t)(buf * 256);
@@ -735,11 +738,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           }
         }
       } else if constexpr (EPI == kLse) {
-        // maximum and sum of exp2 of this lane's row over its quarter of the tile's columns
+        // maximum and sum of exp2 of this lane's row over its half of the tile's columns
         constexpr float kLog2e = 1.44269504088896340736f;
         float m = -INFINITY, s = 0.f;
-#pragma unroll
-        for (int c = half * 64; c < half * 64 + 64; c += 32) {
+#pragma unroll 1
+        for (int c = half * 128; c < half * 128 + 128; c += 32) {
           const int left = b.N - (q.n * 256 + c);
           uint32_t r[32];
           tmem_ld32_nowait(tb + c, r);
@@ -765,7 +768,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           s += s0 + s1;
           m = nm;
         }
-        if (row + lane < b.M) a.part[(int64_t)(row + lane) * (4 * b.nt) + 4 * q.n + half] = make_float2(m, s);
+        if (row + lane < b.M) a.part[(int64_t)(row + lane) * (2 * b.nt) + 2 * q.n + half] = make_float2(m, s);
       } else if constexpr (EPI == kProb) {
         constexpr float kLog2e = 1.44269504088896340736f;
         const int i0 = row + lane;
@@ -774,30 +777,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         const float z = live ? a.lse[i0] * kLog2e : 0.f, d = live ? a.dloss[i0] : 0.f;
         const uint32_t mask = live ? 0xFFFFFFFFu : 0u;            // a held-out row is zeros whatever its logits are
         const int64_t tc = live ? tg - a.v0 : -1;                 // the target's column of this piece
+#pragma unroll 1
+        for (int c64 = half * 128; c64 < half * 128 + 128; c64 += 64) {
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          const int col = q.n * 256 + half * 64 + c;
-          uint32_t r[32], w[16];
-          tmem_ld32_nowait(tb + half * 64 + c, r);
-          tmem_wait();
-          const int hit = (tc >= col && tc < col + 32) ? (int)(tc - col) : -1;
+          for (int c = 0; c < 64; c += 32) {
+            const int col = q.n * 256 + c64 + c;
+            uint32_t r[32], w[16];
+            tmem_ld32_nowait(tb + c64 + c, r);
+            tmem_wait();
+            const int hit = (tc >= col && tc < col + 32) ? (int)(tc - col) : -1;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(ex2(fmaf(__uint_as_float(r[i]), kLog2e, -z)));
-          if (__any_sync(0xffffffffu, hit >= 0)) {
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(ex2(fmaf(__uint_as_float(r[i]), kLog2e, -z)));
+            if (__any_sync(0xffffffffu, hit >= 0)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (hit == i) r[i] = __float_as_uint(__uint_as_float(r[i]) - 1.f);
+              for (int i = 0; i < 32; ++i)
+                if (hit == i) r[i] = __float_as_uint(__uint_as_float(r[i]) - 1.f);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              w[i] = pack(__uint_as_float(r[2 * i]) * d, __uint_as_float(r[2 * i + 1]) * d) & mask;
+            if (c == 0) {
+              if (lane == 0) store_wait<0>(); // the block before has left the buffer
+              __syncwarp();
+            }
+            stage_half(obuf, lane, c / 32, w);
           }
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[i] = pack(__uint_as_float(r[2 * i]) * d, __uint_as_float(r[2 * i + 1]) * d) & mask;
-          if (c == 0) {
-            if (lane == 0) store_wait<0>();   // the tile before has left the buffer
-            __syncwarp();
-          }
-          stage_half(obuf, lane, c / 32, w);
+          send<false>(b, &b.tc, obuf, 0, row, q.n * 256 + c64, lane);
         }
-        send<false>(b, &b.tc, obuf, 0, row, q.n * 256 + half * 64, lane);
       }
       tc_fence_before();
       __syncwarp();

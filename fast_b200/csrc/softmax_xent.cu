@@ -289,7 +289,7 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
     FBH_TRY(logits_args(p, a, hp, n, w, (int)a.V));
     p.part = part;
     FBH_TRY(p.p[0].kb[0] > kLseSlab ? launch_pair<kLseLong>(p, c.stream) : launch_pair<kLse>(p, c.stream));
-    FBH_TRY(finish<uint16_t>(c, a, part, 4 * nt, hp, w, r0, n));
+    FBH_TRY(finish<uint16_t>(c, a, part, (p.p[0].kb[0] > kLseSlab ? 4 : 2) * nt, hp, w, r0, n));
   }
   return FB_OK;
 }
