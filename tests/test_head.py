@@ -86,3 +86,13 @@ def test_softmax_xent_entry_refuses():
     assert lib.fb_softmax_xent_fwd(args(n=0), None, 0, None) == 0
     for rc, bad in ((1, dict(dloss=None)), (1, dict(lddh=4)), (1, dict(grad_type=3)), (3, dict(accumulate=1))):
         assert lib.fb_softmax_xent_bwd(args(**bad), p, 1 << 40, None) == rc, bad
+
+
+def test_module_refuses_an_unknown_activation():
+    from fast_b200.ranking import GatedFeedForward, NodeRankingHead
+    with pytest.raises(ValueError):
+        GatedFeedForward(8, 16, act="tanh")
+    head = NodeRankingHead(8, 20, hidden=12)
+    assert {n: tuple(p.shape) for n, p in head.named_parameters()} == {
+        "node_table": (20, 8), "norm1.weight": (8,), "norm1.bias": (8,), "norm2.weight": (8,), "norm2.bias": (8,),
+        "ffn.w_gate": (12, 8), "ffn.w_up": (12, 8), "ffn.w_down": (8, 12)}
