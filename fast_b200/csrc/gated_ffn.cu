@@ -119,12 +119,12 @@ int glu(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &
   one_product(p, a.n, Fp, 128, tiles_of(a.D, BK), EPI == kGluBwd ? 2 : 1);
   p.act = a.act;
   PairProb &b = p.p[0];
-  FBH_TRY(make_map(&b.ta[0], x.p, a.n, a.D, x.ld, kHalfM));
+  FBH_TRY(make_map(&b.ta[EPI == kGluBwd ? 1 : 0], x.p, a.n, a.D, x.ld, kHalfM));
   FBH_TRY(make_map(&b.tb[0], wg.p, a.F, a.D, wg.ld, 128));
   FBH_TRY(make_map(&b.tb[1], wu.p, a.F, a.D, wu.ld, 128));
   FBH_TRY(make_map(&b.tc, h, a.n, Fp, Fp, 32));
   if (EPI == kGluBwd) {
-    FBH_TRY(make_map(&b.ta[1], dy.p, a.n, a.D, dy.ld, kHalfM));
+    FBH_TRY(make_map(&b.ta[0], dy.p, a.n, a.D, dy.ld, kHalfM));   // dh comes first
     FBH_TRY(make_map(&p.tw, wd.p, a.D, a.F, wd.ld, BK));
     FBH_TRY(make_map(&p.tc2[0], dgu, a.n, Fp, 2 * Fp, 32));
     FBH_TRY(make_map(&p.tc2[1], dgu + Fp, a.n, Fp, 2 * Fp, 32));

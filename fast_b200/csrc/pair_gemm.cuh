@@ -30,7 +30,9 @@
 // XU pipe) fall into the other's loads, maxima and stores.  Stages of 64 k travel through a ring
 // of kStages; the loads of both CTAs count on the even CTA's barrier, MMA
 // completion frees the stage in both.  Accumulators: two of up to 256 columns
-// (the epilogue drains one while the other fills), one of 384 for kGluBwd.
+// (the epilogue drains one while the other fills).  kGluBwd's tile takes 384:
+// g | u has one place and dh two, dh comes first, and the g | u stages wait for
+// the epilogue of the tile before, which has had dh's time to drain them.
 //
 // No load uses cluster multicast.  Every wait is bounded: past the limit a
 // CTA records an error, stops, gives its copies time to land and leaves.
@@ -82,8 +84,8 @@ static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 23
 
 constexpr int kMaxProbs = 4;
 
-// One product.  Two terms may feed a tile: kGluBwd's second one fills the dh
-// columns; elsewhere it continues the same sum (dx = dg Wg + du Wu) and its
+// One product.  Two terms may feed a tile: kGluBwd's first one fills the dh
+// columns, its second g | u; elsewhere the second continues the same sum (dx = dg Wg + du Wu) and its
 // stages follow the first's.
 struct PairProb {
   CUtensorMap ta[2], tb[2];                   // by term; kGlu*: tb[0] = Wg, tb[1] = Wu
@@ -347,11 +349,11 @@ template <int EPI> __device__ __forceinline__ Tile tile_at(const PairArgs &a, in
   return q;
 }
 
-// Columns c .. c + 31 of g (and + 128: u, + 256: dh) of this warp's 32 rows:
+// Columns c .. c + 31 of g (and + 128: u, and of dh at td) of this warp's 32 rows:
 // h (and dg, du) staged as half of the warp's 128-byte rows, sent off with the
 // second half: the copy engine takes a 64-byte row no faster than a 128-byte one.
 template <int ACT, bool BWD>
-__device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, int which, uint8_t *buf, int row,
+__device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, uint32_t td, int c, int which, uint8_t *buf, int row,
                                           int col, int lane) {
   uint32_t w[BWD ? 3 : 1][16];
 #pragma unroll
@@ -359,7 +361,7 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, int c, 
     uint32_t g[16], u[16], d[BWD ? 16 : 1];
     tmem_ld16_nowait(t + c + 16 * q, g);
     tmem_ld16_nowait(t + 128 + c + 16 * q, u);
-    if constexpr (BWD) tmem_ld16_nowait(t + 256 + c + 16 * q, d);
+    if constexpr (BWD) tmem_ld16_nowait(td + c + 16 * q, d);
     tmem_wait();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -465,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
       const int bn_ = P == 3 ? 128 : (EPI == kStore ? b.bn : 256);
       for (int j = q.k0; j < q.k1; ++j) {
         const int p = j >= kb0 ? 1 : 0, jj = j - (p ? kb0 : 0);
-        const bool dh = EPI == kGluBwd && p == 1;
+        const bool dh = EPI == kGluBwd && p == 0;
         const int bn = dh ? 128 : bn_;
         const bool bmn = dh || bmn_;
         const CUtensorMap *ma = &b.ta[p], *mb = dh ? &a.tw : &b.tb[kDual ? rank : p];
@@ -522,12 +524,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         const int bn = P == 3 ? 128 : (EPI == kStore ? b.bn : 256), kb0 = b.kb[0];
         const uint64_t ad0 = sdesc(smem_u32(smem), amn), adv_a = amn ? (2048 >> 4) : 2;
         for (int j = q.k0; j < q.k1; ++j) {
-          const bool dh = EPI == kGluBwd && j >= kb0, bmn = dh || bmn_;
+          const bool dh = EPI == kGluBwd && j < kb0, bmn = dh || bmn_;
           const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(bn, amn, bmn);
           const uint64_t bd0 = sdesc(smem_u32(smem + kABytes), bmn), adv_b = bmn ? (2048 >> 4) : 2;
-          // a new accumulator at the tile's start, or for every slab; dh's columns start at its first stage
-          const bool next = P == 3 || j == q.k0 || (EPI == kLseLong && (j & (kLseSlab - 1)) == 0);
-          const bool fresh = next || (dh && j == kb0);
+          // a new accumulator at the tile's start (kGluBwd: where g | u start), or for every slab
+          const bool next = P == 3 || (EPI == kGluBwd ? j == kb0 : j == q.k0) ||
+                            (EPI == kLseLong && (j & (kLseSlab - 1)) == 0);
+          const bool fresh = next || (dh && j == q.k0);
           const uint32_t buf = it % kBufs, use = it / kBufs;
           if (next && use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
             stop = true;
@@ -538,7 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
             break;
           }
           const bool last = P == 3 || j + 1 == q.k1 || (EPI == kLseLong && ((j + 1) & (kLseSlab - 1)) == 0);
-          const uint32_t d = tmem + (dh ? 256u : buf * 256u);
+          const uint32_t d = tmem + (dh ? 256u + (it & 1) * 128u : buf * 256u);
           // one product of 64 k: A of stage sa, B of stage sb
           auto issue = [&](int sa, int sb, bool first) {
             const uint64_t ad = ad0 + (uint64_t)(sa * (kStageBytes >> 4)), bd = bd0 + (uint64_t)(sb * (kStageBytes >> 4));
@@ -697,12 +700,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
       const int row = q.m * 256 + (int)rank * kHalfM + qd * 32;   // this warp's first row
       if constexpr (EPI == kGluFwd || EPI == kGluBwd) {
         constexpr bool bwd = EPI == kGluBwd;
+        const uint32_t td = tb + 256 + (it & 1) * 128;
 #pragma unroll 1
         for (int which = 0; which < 2; ++which) {
           const int c = half * 64 + 32 * which, col = q.n * 128 + half * 64;
-          if (a.act == kSilu) glu_block<kSilu, bwd>(a, tb, c, which, obuf, row, col, lane);
-          else if (a.act == kGelu) glu_block<kGelu, bwd>(a, tb, c, which, obuf, row, col, lane);
-          else glu_block<kRelu, bwd>(a, tb, c, which, obuf, row, col, lane);
+          if (a.act == kSilu) glu_block<kSilu, bwd>(a, tb, td, c, which, obuf, row, col, lane);
+          else if (a.act == kGelu) glu_block<kGelu, bwd>(a, tb, td, c, which, obuf, row, col, lane);
+          else glu_block<kRelu, bwd>(a, tb, td, c, which, obuf, row, col, lane);
         }
       } else if constexpr (EPI == kStore) {
         const int w0 = half * (b.bn / 2), w1 = w0 + b.bn / 2, n0 = q.n * b.bn;
