@@ -84,13 +84,15 @@ int check(const fb_gated_ffn *a, bool bwd) {
   return FB_OK;
 }
 
-// fp32: g | u [N, 2 Fp] (and dh), then the activation; the padding columns up
-// to Fp are zeros (weight rows past F read as zeros).
-int gate_up_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, float *gu, int64_t Fp) {
-  Product p[2] = {rows_product(x, a.n, a.D, wg, false, (int)Fp, Out{gu, 2 * Fp, FB_F32, 0}),
+// fp32: g | u [N, 2 Fp] (and dh [N, Fp], from dy), then the activation; the
+// padding columns up to Fp are zeros (weight rows past F read as zeros).
+int gate_up_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, float *gu, int64_t Fp,
+                const Mat *dy = nullptr, const Mat *wd = nullptr, float *dh = nullptr) {
+  Product p[3] = {rows_product(x, a.n, a.D, wg, false, (int)Fp, Out{gu, 2 * Fp, FB_F32, 0}),
                   rows_product(x, a.n, a.D, wu, false, (int)Fp, Out{gu + Fp, 2 * Fp, FB_F32, 0})};
-  p[0].b_n = p[1].b_n = a.F;
-  return products(c, p, 2);
+  if (dh) p[2] = rows_product(*dy, a.n, a.D, *wd, true, (int)Fp, Out{dh, Fp, FB_F32, 0});
+  p[0].b_n = p[1].b_n = p[2].b_n = a.F;
+  return products(c, p, dh ? 3 : 2);
 }
 
 int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, const Mat &wu, const Mat &wd) {
@@ -162,10 +164,7 @@ int backward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, co
   FBH_TAKE(dh, c, float, n);
   FBH_TAKE(h, c, uint16_t, 3 * n);
   FBH_TAKE(dgu, c, uint16_t, 6 * n);
-  FBH_TRY(gate_up_f32(c, a, x, wg, wu, gu, Fp));
-  Product ph = rows_product(dy, a.n, a.D, wd, true, (int)Fp, Out{dh, Fp, FB_F32, 0});
-  ph.b_n = a.F;
-  FBH_TRY(products(c, &ph, 1));
+  FBH_TRY(gate_up_f32(c, a, x, wg, wu, gu, Fp, &dy, &wd, dh));
   if (!c.dry) {
     auto k = a.act == kSilu ? k_glu_bwd<FB_ACT_SILU> : (a.act == kGelu ? k_glu_bwd<FB_ACT_GELU> : k_glu_bwd<FB_ACT_RELU>);
     FB_TRY_CUDA(fb::launch(k, blocks_for(n), 256, 0, c.stream, (const float *)gu, (const float *)dh, h, dgu, a.n,

@@ -19,37 +19,39 @@ struct SumArgs {
   SumJob j[kMaxProbs];
   int n;
 };
-constexpr int kSumPerCta = 256 * 4;
+constexpr int kSumPerCta = 256;
 
-__global__ void __launch_bounds__(256) k_sum_splits(const __grid_constant__ SumArgs a) {
+__global__ void __launch_bounds__(kSumPerCta) k_sum_splits(const __grid_constant__ SumArgs a) {
   fb::pdl_enter();
   int q = 0;
   while (q + 1 < a.n && blockIdx.x >= a.j[q + 1].first) ++q;
   const SumJob &j = a.j[q];
-  const int64_t total = j.rows * j.cols, at = (int64_t)(blockIdx.x - j.first) * kSumPerCta, stride = j.split_stride;
+  const int64_t i = (int64_t)(blockIdx.x - j.first) * kSumPerCta + threadIdx.x, stride = j.split_stride;
+  if (i >= j.rows * j.cols) return;
+  const int64_t r = i < ((int64_t)1 << 31) ? (int64_t)((uint32_t)i / (uint32_t)j.cols) : i / j.cols;
+  const int c = (int)(i - r * j.cols);
+  const float *p = j.P + r * j.ldp + c;
+  float s = 0.f;
+  int z = 0;
+  for (; z + 8 <= j.splits; z += 8) {
+    float v[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t i = at + e * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int64_t r = i / j.cols;
-    const int c = (int)(i - r * j.cols);
-    const float *p = j.P + r * j.ldp + c;
-    float s = 0.f;
-    int z = 0;
-    for (; z + 8 <= j.splits; z += 8) {
-      float v[8];
+    for (int u = 0; u < 8; ++u) v[u] = p[(z + u) * stride];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = p[(z + u) * stride];
+    for (int u = 0; u < 8; ++u) s += v[u];
+  }
+  if (z < j.splits) {                          // the last few at once too
+    float v[7];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s += v[u];
-    }
-    for (; z < j.splits; ++z) s += p[z * stride];
-    if (j.bf16) {
-      static_cast<__nv_bfloat16 *>(j.out)[r * j.ldo + c] = __float2bfloat16_rn(s);
-    } else {
-      float *o = static_cast<float *>(j.out) + r * j.ldo + c;
-      *o = j.accumulate ? *o + s : s;
-    }
+    for (int u = 0; u < 7; ++u) v[u] = z + u < j.splits ? p[(z + u) * stride] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 7; ++u) s += v[u];
+  }
+  if (j.bf16) {
+    static_cast<__nv_bfloat16 *>(j.out)[r * j.ldo + c] = __float2bfloat16_rn(s);
+  } else {
+    float *o = static_cast<float *>(j.out) + r * j.ldo + c;
+    *o = j.accumulate ? *o + s : s;
   }
 }
 
