@@ -682,13 +682,14 @@ def attn_bwd(q, k, v, rptr, att, dagg, heads, slope, drop_p=0.0, seed=0, offset=
 # The calls go through the head_ops module (argument checks, outputs and
 # workspaces in C++): operands of the wrong type, shape, layout or device raise
 # ValueError.
-def _head_call(name, kernels, nbytes, flops, *args):
-    fn = getattr(head_ops, name)
+def _head_call(fn, kernels, work, *args):
+    """Calls a head_ops function; work() gives its algorithmic bytes and flops
+    and is asked for only when a timer runs (a small call is bound by the host)."""
     if TIMER is None and not NVTX:
         LAUNCHES[0] += kernels
         return fn(*args)
     out = []
-    _launch(name, nbytes, flops, kernels, lambda: out.append(fn(*args)))
+    _launch(fn.__name__, *work(), kernels, lambda: out.append(fn(*args)))
     return out[-1]
 
 
@@ -697,11 +698,8 @@ def layer_norm_fwd(x, gamma, beta=None, eps=1e-5, res=None):
     in fp32.  Returns (y, mean, rstd); with a residual `res` it normalises
     s = x + res, kept in the rows' type, and returns (y, s, mean, rstd).
     gamma and beta are fp32 or of the rows' type."""
-    if TIMER is None and not NVTX:           # the least a small call can cost
-        LAUNCHES[0] += 1
-        return head_ops.layer_norm_fwd(x, gamma, beta, eps, res)
-    m = x.numel()
-    return _head_call("layer_norm_fwd", 1, x.element_size() * m * (2 if res is None else 4), 8 * m, x, gamma, beta, eps,
+    return _head_call(head_ops.layer_norm_fwd, 1,
+                      lambda: (x.element_size() * x.numel() * (2 if res is None else 4), 8 * x.numel()), x, gamma, beta, eps,
                       res)
 
 
@@ -710,11 +708,8 @@ def layer_norm_bwd(dy, x, gamma, mean, rstd, ds=None, dgamma=None, dbeta=None):
     when there was a residual): returns (dx, dgamma, dbeta).  dx, the gradient
     of x and of res alike, includes ds, the gradient that reaches s on its own.
     dgamma / dbeta have gamma's type; fp32 vectors given are accumulated into."""
-    if TIMER is None and not NVTX:
-        LAUNCHES[0] += 2
-        return head_ops.layer_norm_bwd(dy, x, gamma, mean, rstd, ds, dgamma, dbeta)
-    m = x.numel()
-    return _head_call("layer_norm_bwd", 2, x.element_size() * m * (3 if ds is None else 4), 10 * m, dy, x, gamma, mean,
+    return _head_call(head_ops.layer_norm_bwd, 2,
+                      lambda: (x.element_size() * x.numel() * (3 if ds is None else 4), 10 * x.numel()), dy, x, gamma, mean,
                       rstd, ds, dgamma, dbeta)
 
 
@@ -730,18 +725,18 @@ def gated_ffn_fwd(x, w_gate, w_up, w_down, act="silu"):
     weights w_gate, w_up [F, D], w_down [D, F], all fp32 or all bf16 (any row
     pitch).  act: "silu", "gelu" (erf form) or "relu".  Products accumulate
     in fp32; the backward needs nothing but the inputs."""
-    m, w = x.numel(), w_gate.numel()
-    return _head_call("gated_ffn_fwd", 2, x.element_size() * (2 * m + 3 * w), 6 * m * w_gate.shape[0], x, w_gate, w_up,
-                      w_down, _act(act))
+    return _head_call(head_ops.gated_ffn_fwd, 2,
+                      lambda: (x.element_size() * (2 * x.numel() + 3 * w_gate.numel()), 6 * x.numel() * w_gate.shape[0]), x,
+                      w_gate, w_up, w_down, _act(act))
 
 
 def gated_ffn_bwd(dy, x, w_gate, w_up, w_down, act="silu", grads=None):
     """Gradients of gated_ffn_fwd: (dx, dw_gate, dw_up, dw_down).  The weight
     gradients have the weights' type; `grads`, three fp32 buffers, are
     accumulated into instead (a flat gradient buffer's views)."""
-    m, w = x.numel(), w_gate.numel()
-    return _head_call("gated_ffn_bwd", 4, x.element_size() * (3 * m + 6 * w), 16 * m * w_gate.shape[0], dy, x, w_gate,
-                      w_up, w_down, _act(act), grads)
+    return _head_call(head_ops.gated_ffn_bwd, 2,
+                      lambda: (x.element_size() * (3 * x.numel() + 6 * w_gate.numel()), 16 * x.numel() * w_gate.shape[0]), dy,
+                      x, w_gate, w_up, w_down, _act(act), grads)
 
 
 def softmax_xent_fwd(h, w, target):
@@ -749,17 +744,17 @@ def softmax_xent_fwd(h, w, target):
     w [V, D] (both fp32 or both bf16), without keeping the logits: returns
     (loss, lse), fp32 [n].  A negative target holds its row out of the loss
     (loss 0); one >= V gives a NaN loss."""
-    m, k = h.numel(), w.numel()
-    return _head_call("softmax_xent_fwd", 2, h.element_size() * (m + k) + 16 * h.shape[0], 2 * m * w.shape[0], h, w,
+    return _head_call(head_ops.softmax_xent_fwd, 2,
+                      lambda: (h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 2 * h.numel() * w.shape[0]), h, w,
                       target)
 
 
 def softmax_xent_bwd(h, w, target, lse, dloss, dw=None):
     """Gradients of softmax_xent_fwd for dloss [n] (fp32): (dh, dw), of the
     inputs' type; an fp32 buffer given as dw is accumulated into instead."""
-    m, k = h.numel(), w.numel()
-    return _head_call("softmax_xent_bwd", 3, 2 * h.element_size() * (m + k) + 16 * h.shape[0], 6 * m * w.shape[0], h, w,
-                      target, lse, dloss, dw)
+    return _head_call(head_ops.softmax_xent_bwd, 2,
+                      lambda: (2 * h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 6 * h.numel() * w.shape[0]),
+                      h, w, target, lse, dloss, dw)
 
 
 class AttentionCore(torch.autograd.Function):

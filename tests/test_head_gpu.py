@@ -46,7 +46,8 @@ def _c(k):
 # ---- layer norm --------------------------------------------------------------------------------------------------
 NORM = [(1, 1, 0, 0), (3, 7, 0, 0), (5, 100, 4, 0), (33, 413, 6, 1), (130, 64, 0, 0), (300, 128, 8, 0), (17, 500, 0, 2),
         (7, 1024, 0, 0), (9, 1027, 0, 0), (2, 2050, 0, 0), (5, 4096, 0, 0), (3, 5000, 0, 0), (3, 8200, 0, 0),
-        (2, 16384, 0, 0), (40000, 16, 0, 0), (2, 6144, 0, 0), (2, 6144, 1, 0), (3, 5890, 1, 0), (33, 414, 0, 0)]
+        (2, 16384, 0, 0), (40000, 16, 0, 0), (2, 6144, 0, 0), (2, 6144, 1, 0), (3, 5890, 1, 0), (33, 414, 0, 0), (700, 413, 0, 1),
+        (5, 3, 0, 1), (301, 2047, 0, 0), (300, 4095, 2, 1), (3, 9001, 0, 1), (2, 16383, 0, 1)]
 
 
 @pytest.mark.parametrize("n,d,pad,off", NORM)
