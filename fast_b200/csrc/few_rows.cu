@@ -8,6 +8,8 @@
 // keeps half of the values, so 32 sums take 31 shuffles, and lane i ends with
 // sum i / (32 / (R MT)).  Where the weight has too few rows to fill the GPU,
 // KS warps share a row's elements and their sums meet in shared memory.
+// Gate and up weights are taken in pairs of rows (kGlu: the block's hidden row;
+// kGateUp: both sums, for the backward).
 //
 // The gated block's second product asks the L2 for its first rows before it
 // waits for the first product, which they do not come from.  (Asking for every
@@ -26,7 +28,8 @@ constexpr int R = 4;
 constexpr int kWarps = 16;
 constexpr int kMaxSmem = 200 * 1024;
 
-enum : int { kGlu = 0, kPlain = 1, kLogits = 2 };
+enum : int { kGlu = 0, kPlain = 1, kLogits = 2, kGateUp = 3 };
+template <int MODE> __host__ __device__ constexpr bool two() { return MODE == kGlu || MODE == kGateUp; }   // two weights
 
 struct Args {
   const void *x;
@@ -41,6 +44,7 @@ struct Args {
   void *out;
   int64_t ldo;
   float2 *part;
+  int out_f32;                                // kPlain: out is fp32 (else of the weights' type)
 };
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
@@ -116,6 +120,11 @@ __device__ __forceinline__ float act1(int act, float g) {
   return fbact::act_exact<fbact::kRelu>(g).x;
 }
 
+template <typename T> __device__ __forceinline__ void put(const Args &a, int64_t at, float v) {
+  if (sizeof(T) == 2 && !a.out_f32) static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(v);
+  else static_cast<float *>(a.out)[at] = v;
+}
+
 // x's pitch in shared memory: whole 32-lane steps, zeros past K.
 template <int V> __host__ __device__ constexpr int x_pitch(int K) { return (K + 32 * V - 1) / (32 * V) * (32 * V); }
 
@@ -130,15 +139,15 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 8 ? 1 : 2) k_few_rows(const
   const int part = warp % a.ks, slot = warp / a.ks, slots = kWarps / a.ks;
   const int steps = Kp / (32 * V), per = (steps + a.ks - 1) / a.ks;
   const int s0 = part * per, s1 = min(steps, s0 + per);
-  constexpr int kRowsPer = MODE == kGlu ? R / 2 : R;       // weight rows (of each matrix) a warp takes at a time
+  constexpr int kRowsPer = two<MODE>() ? R / 2 : R;       // weight rows (of each matrix) a warp takes at a time
   const int64_t groups = (a.rows + kRowsPer - 1) / kRowsPer;
   // asks the L2 for this warp's part of the rows of group g
   auto ahead = [&](int64_t g) {
     if (V == 1 || lane >= R) return;
-    const int64_t row = (g + slot) * kRowsPer + (MODE == kGlu ? lane / 2 : lane);
+    const int64_t row = (g + slot) * kRowsPer + (two<MODE>() ? lane / 2 : lane);
     const int k0 = s0 * 32 * V, k1 = min(a.K, s1 * 32 * V);
     if (row >= a.rows || k1 <= k0) return;
-    const T *p = (MODE == kGlu && (lane & 1)) ? static_cast<const T *>(a.w2) + row * a.ldw2
+    const T *p = (two<MODE>() && (lane & 1)) ? static_cast<const T *>(a.w2) + row * a.ldw2
                                               : static_cast<const T *>(a.w) + row * a.ldw;
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p + k0), "r"((uint32_t)((k1 - k0) * sizeof(T)))
                  : "memory");
@@ -161,10 +170,10 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 8 ? 1 : 2) k_few_rows(const
     bool in[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = MODE == kGlu ? row0 + r / 2 : row0 + r;
+      const int64_t row = two<MODE>() ? row0 + r / 2 : row0 + r;
       in[r] = row < a.rows;
       const int64_t q = in[r] ? row : 0;
-      p[r] = (MODE == kGlu && (r & 1)) ? static_cast<const T *>(a.w2) + q * a.ldw2
+      p[r] = (two<MODE>() && (r & 1)) ? static_cast<const T *>(a.w2) + q * a.ldw2
                                        : static_cast<const T *>(a.w) + q * a.ldw;
     }
     float acc[NV];
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 8 ? 1 : 2) k_few_rows(const
       }
       continue;
     }
-    if (a.ks > 1 || MODE == kGlu) {
+    if (a.ks > 1 || two<MODE>()) {
       __syncthreads();                        // the turn before has been read
       if (lane % (32 / NV) == 0) red[warp][idx] = v;
       __syncthreads();
@@ -205,31 +214,29 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 8 ? 1 : 2) k_few_rows(const
     if (MODE == kPlain && a.ks == 1) {
       const int64_t row = row0 + idx / MT;
       if (lane % (32 / NV) == 0 && row < a.rows && m < a.n) {
-        T *o = static_cast<T *>(a.out) + m * a.ldo + row;
-        if constexpr (sizeof(T) == 2) *o = __float2bfloat16_rn(v);
-        else *o = v;
+        put<T>(a, m * a.ldo + row, v);
       }
       continue;
     }
     // one thread per result: sums of the KS warps, in order
-    constexpr int kOut = MODE == kGlu ? NV / 2 : NV;
+    constexpr int kOut = two<MODE>() ? NV / 2 : NV;
     for (int t = threadIdx.x; t < slots * kOut; t += blockDim.x) {
       const int sl = t / kOut, i = t - sl * kOut, r = i / MT, mm = i - r * MT;
       const int64_t row = (g0 + sl) * kRowsPer + r;
       if (row >= a.rows || mm >= a.n) continue;
-      if (MODE == kGlu) {
+      if (two<MODE>()) {
         float g = 0.f, u = 0.f;
         for (int q = 0; q < a.ks; ++q) {
           g += red[sl * a.ks + q][(2 * r) * MT + mm];
           u += red[sl * a.ks + q][(2 * r + 1) * MT + mm];
         }
-        static_cast<float *>(a.out)[mm * a.ldo + row] = act1(a.act, g) * u;
+        float *o = static_cast<float *>(a.out) + mm * a.ldo + row;
+        if (MODE == kGateUp) o[0] = g, o[a.rows] = u;
+        else *o = act1(a.act, g) * u;
       } else {
         float s = 0.f;
         for (int q = 0; q < a.ks; ++q) s += red[sl * a.ks + q][i];
-        T *o = static_cast<T *>(a.out) + mm * a.ldo + row;
-        if constexpr (sizeof(T) == 2) *o = __float2bfloat16_rn(s);
-        else *o = s;
+        put<T>(a, mm * a.ldo + row, s);
       }
     }
   }
@@ -282,16 +289,19 @@ template <typename T, int V, int MT, int MODE> int go(const Args &a, unsigned gr
 template <typename T, int V, int MODE> int by_rows(const Args &a, unsigned grid, cudaStream_t st) {
   if (a.n == 1) return go<T, V, 1, MODE>(a, grid, st);
   if (a.n == 2) return go<T, V, 2, MODE>(a, grid, st);
-  if (a.n <= 4) return go<T, V, 4, MODE>(a, grid, st);
-  return go<T, V, 8, MODE>(a, grid, st);
+  if constexpr (MODE != kGateUp || sizeof(T) == 4) {   // bf16 backward: at most 2 rows
+    if (a.n <= 4) return go<T, V, 4, MODE>(a, grid, st);
+    return go<T, V, 8, MODE>(a, grid, st);
+  }
+  return fb::set_error(FB_ERR_ARG, "few rows: more rows than this path takes");
 }
 template <int MODE> int run(int type, Args a, cudaStream_t st) {
   const int es = elem(type), v = 16 / es;
   uintptr_t m = reinterpret_cast<uintptr_t>(a.w) | (uintptr_t)(a.ldw * es);
-  if (MODE == kGlu) m |= reinterpret_cast<uintptr_t>(a.w2) | (uintptr_t)(a.ldw2 * es);
+  if (two<MODE>()) m |= reinterpret_cast<uintptr_t>(a.w2) | (uintptr_t)(a.ldw2 * es);
   const bool wide = (m & 15) == 0 && a.K % v == 0;
   // warps sharing a row until every SM has two CTAs, while each keeps two steps of the row
-  const int64_t per = MODE == kGlu ? R / 2 : R, groups = (a.rows + per - 1) / per;
+  const int64_t per = two<MODE>() ? R / 2 : R, groups = (a.rows + per - 1) / per;
   const int steps = (a.K + 32 * (wide ? v : 1) - 1) / (32 * (wide ? v : 1));
   a.ks = 1;
   if (MODE != kLogits)
@@ -306,27 +316,38 @@ template <int MODE> int run(int type, Args a, cudaStream_t st) {
 
 namespace fbh {
 
-bool few_rows_ok(int64_t n, int64_t K) {
+bool few_rows_ok(int type, bool bwd, int64_t n, int64_t K, int64_t weight_elements) {
+  const int64_t most = type == FB_F32 ? 8 : (weight_elements > (1 << 20) ? 2 : (bwd ? 0 : 8));
   const int64_t mt = n == 1 ? 1 : (n == 2 ? 2 : (n <= 4 ? 4 : 8));
-  return n >= 1 && n <= kFewRows && mt * round_up(K, 256) * (int64_t)sizeof(float) <= kMaxSmem;
+  return n >= 1 && n <= most && mt * round_up(K, 256) * (int64_t)sizeof(float) <= kMaxSmem;
 }
 
 int few_rows_glu(Call &c, int type, int act, const Mat &x, int64_t n, int D, const Mat &wg, const Mat &wu, int F,
                  float *h) {
-  Args a{x.p, x.ld, type == FB_F32, wg.p, wu.p, wg.ld, wu.ld, (int)n, D, F, 1, act, h, F, nullptr};
+  Args a{x.p, x.ld, type == FB_F32, wg.p, wu.p, wg.ld, wu.ld, (int)n, D, F, 1, act, h, F, nullptr, 1};
   return c.dry ? FB_OK : run<kGlu>(type, a, c.stream);
 }
 
 int few_rows_product(Call &c, int type, const float *x, int64_t n, int K, const Mat &w, int N, void *out, int64_t ldo) {
-  Args a{x, K, 1, w.p, nullptr, w.ld, 0, (int)n, K, N, 1, 0, out, ldo, nullptr};
+  Args a{x, K, 1, w.p, nullptr, w.ld, 0, (int)n, K, N, 1, 0, out, ldo, nullptr, type == FB_F32};
   return c.dry ? FB_OK : run<kPlain>(type, a, c.stream);
 }
 
 int few_rows_parts() { return 2 * sms(); }
 
 int few_rows_lse(Call &c, int type, const Mat &h, int64_t n, int D, const Mat &w, int64_t V, float2 *part) {
-  Args a{h.p, h.ld, type == FB_F32, w.p, nullptr, w.ld, 0, (int)n, D, V, 1, 0, nullptr, 0, part};
+  Args a{h.p, h.ld, type == FB_F32, w.p, nullptr, w.ld, 0, (int)n, D, V, 1, 0, nullptr, 0, part, 0};
   return c.dry ? FB_OK : run<kLogits>(type, a, c.stream);
+}
+
+int few_rows_gate_up(Call &c, int type, const Mat &x, int64_t n, int D, const Mat &wg, const Mat &wu, int F, float *gu) {
+  Args a{x.p, x.ld, type == FB_F32, wg.p, wu.p, wg.ld, wu.ld, (int)n, D, F, 1, 0, gu, 2 * F, nullptr, 1};
+  return c.dry ? FB_OK : run<kGateUp>(type, a, c.stream);
+}
+
+int few_rows_logits(Call &c, int type, const Mat &h, int64_t n, int D, const Mat &w, int64_t V, float *l) {
+  Args a{h.p, h.ld, type == FB_F32, w.p, nullptr, w.ld, 0, (int)n, D, V, 1, 0, l, V, nullptr, 1};
+  return c.dry ? FB_OK : run<kPlain>(type, a, c.stream);
 }
 
 }  // namespace fbh

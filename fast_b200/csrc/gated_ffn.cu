@@ -194,7 +194,9 @@ int empty_grads(const fb_gated_ffn &a, cudaStream_t st) {
 }
 
 int run(Call &c, const fb_gated_ffn &a, bool bwd) {
-  if (!bwd && few_rows_ok(a.n, std::max(a.D, a.F))) {
+  if (bwd && few_rows_ok(a.type, bwd, a.n, a.D, (int64_t)a.D * a.F) && a.F <= kFewRowsTable)
+    return few_rows_ffn_bwd(c, a);
+  if (!bwd && few_rows_ok(a.type, bwd, a.n, std::max(a.D, a.F), (int64_t)a.D * a.F)) {
     FBH_TAKE(h, c, float, a.n * a.F);
     FBH_TRY(few_rows_glu(c, a.type, a.act, Mat{a.x, a.ldx}, a.n, a.D, Mat{a.w_gate, a.ld_gate}, Mat{a.w_up, a.ld_up}, a.F,
                          h));

@@ -336,7 +336,7 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
 }
 
 int run(Call &c, const fb_softmax_xent &a, bool bwd) {
-  if (!bwd && few_rows_ok(a.n, a.D)) return forward_few(c, a);
+  if (few_rows_ok(a.type, bwd, a.n, a.D, a.D * a.V) && (!bwd || a.V <= kFewRowsTable)) return bwd ? few_rows_xent_bwd(c, a) : forward_few(c, a);
   Mat h, w;
   const Operand ops[2] = {{Mat{a.h, a.ldh}, a.n, a.D, &h}, {Mat{a.w, a.ldw}, a.V, a.D, &w}};
   FBH_TRY(operands(c, a.type, ops, 2));

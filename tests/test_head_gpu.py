@@ -195,6 +195,14 @@ def test_gated_ffn(cuda, n, d, f, pad, dtype, act):
         _check("accumulated " + name, b, want + 0.5, e, F32)
 
 
+# few rows against weights of more than 2^20 elements: the path that reads them without tensor cores, both layouts
+@pytest.mark.parametrize("n,d,f,pad", [(1, 520, 2056, 0), (2, 520, 2056, 8), (2, 519, 2051, 0), (1, 1100, 1000, 3),
+                                       (3, 520, 2056, 0), (8, 519, 2051, 0), (8, 2056, 520, 4)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_ffn_few_rows_of_large_weights(cuda, n, d, f, pad, dtype):
+    test_gated_ffn(cuda, n, d, f, pad, dtype, "silu")
+
+
 def test_gated_ffn_gradient_against_differences(cuda):
     """fp32: <dy, y(p + e v) - y(p - e v)> / 2e against <grad, v> for every input."""
     from fast_b200 import ops
@@ -265,6 +273,13 @@ def test_softmax_xent(cuda, n, d, v, pad, dtype):
     dh2, _ = ops.softmax_xent_bwd(h, w, t, lse, dl, dw=buf)
     assert torch.equal(dh, dh2)
     _check("accumulated dw", buf, G.t() @ Hd + 0.25, eG.t() @ Hd.abs() + _c(n) * ((G.abs() + eG).t() @ Hd.abs()), F32)
+
+
+@pytest.mark.parametrize("n,d,v,pad", [(1, 130, 9001, 0), (2, 128, 9000, 0), (2, 127, 9003, 1), (2, 1030, 2000, 0),
+                                       (3, 128, 9000, 8), (7, 1030, 2001, 0), (8, 127, 9003, 0)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_softmax_xent_few_rows_of_large_tables(cuda, n, d, v, pad, dtype):
+    test_softmax_xent(cuda, n, d, v, pad, dtype)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
