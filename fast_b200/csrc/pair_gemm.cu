@@ -132,10 +132,6 @@ void plan(PairArgs &a, bool planes) {
   }
 }
 
-int operand_map(CUtensorMap *m, const Mat &x, int64_t rows, int64_t cols, int box_rows) {
-  return x.plane ? make_map3(m, x.p, rows, cols, x.ld, x.plane, box_rows) : make_map(m, x.p, rows, cols, x.ld, box_rows);
-}
-
 }  // namespace
 
 namespace fbh {

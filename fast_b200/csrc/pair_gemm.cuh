@@ -13,7 +13,9 @@
 //   are summed, smallest first; the three left out are below 2^-24 of the
 //   product.  The tensor cores' accumulation truncates, so it runs over 64 k
 //   only: the epilogue warps add each such slab to an fp32 sum in registers
-//   while the next one is computed.
+//   while the next one is computed.  kLsePlanes and kProbPlanes are kLse and
+//   kProb on that sum, in registers: the logits of fp32 rows are not stored
+//   either, and G leaves as its three planes.
 //
 // A cluster of two CTAs works on a 256 x BN tile: each CTA stages 128 rows of
 // A and BN / 2 rows of B, the MMA of the even CTA reads both halves from both
@@ -43,13 +45,14 @@
 #include <cstring>
 #include "act.cuh"
 #include "head.cuh"
+#include "planes.cuh"
 #include "tc_common.cuh"
 
 namespace fbpair {
 
 using namespace fbtc;
 
-enum : int { kStore = 0, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6 };
+enum : int { kStore = 0, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6, kLsePlanes = 7, kProbPlanes = 8 };
 using fbact::kGelu;
 using fbact::kRelu;
 using fbact::kSilu;
@@ -80,7 +83,7 @@ template <int EPI, int P> __host__ __device__ constexpr int smem_bytes() {
 }
 static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 232448 &&
                   smem_bytes<kStore, 1>() <= 232448 &&
-                  smem_bytes<kStore, 3>() <= 232448, "shared memory exceeds 227 KB");
+                  smem_bytes<kStore, 3>() <= 232448 && smem_bytes<kProbPlanes, 3>() <= 232448, "shared memory exceeds 227 KB");
 
 constexpr int kMaxProbs = 4;
 
@@ -104,10 +107,10 @@ struct PairArgs {
   PairProb p[kMaxProbs];
   int n, tile0[kMaxProbs + 1];                // products; tiles before each
   int32_t *err;
-  CUtensorMap tw, tc2[2];                     // kGluBwd: Wd; outputs dg, du
+  CUtensorMap tw, tc2[2];                     // kGluBwd: Wd; outputs dg, du (kProbPlanes: G's planes 1, 2)
   int act;
-  float2 *part;                               // kLse: [M][2 nt] (kLseLong: [M][4 nt]) (max, sum of exp2) partials
-  const int64_t *target;                      // kProb
+  float2 *part;                               // kLse*: [M][2 nt] (kLseLong: [M][4 nt]) (max, sum of exp2) partials
+  const int64_t *target;                      // kProb*
   const float *lse, *dloss;
   int64_t V, v0;
 };
@@ -321,6 +324,29 @@ __device__ __forceinline__ void send(const PairProb &a, const CUtensorMap *tc, c
   }
 }
 
+// Maximum and sum of exp2 of a row's 64 logits, of which `left` are inside the table, in units of log2.
+__device__ __forceinline__ float2 max_sum(float (&v)[64], int left) {
+  constexpr float kLog2e = 1.44269504088896340736f;
+  if (left < 64) {
+#pragma unroll
+    for (int i = 0; i < 64; ++i)
+      if (i >= left) v[i] = -INFINITY;        // past the table
+  }
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < 64; ++i) m = fmaxf(m, v[i]);
+  m *= kLog2e;
+  // nothing but -inf: subtract 0, so that exp2 gives zeros (and NaN stays NaN)
+  const float base = m == -INFINITY ? 0.f : m;
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < 64; i += 2) {
+    s0 += ex2(fmaf(v[i], kLog2e, -base));
+    s1 += ex2(fmaf(v[i + 1], kLog2e, -base));
+  }
+  return make_float2(m, s0 + s1);
+}
+
 struct Tile {
   int p, m, n, k0, k1;                        // k0 .. k1 - 1: stages, the terms' one after the other
   int ybase;                                  // first row of this split's results
@@ -403,7 +429,7 @@ __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, uint32_
 
 template <int EPI, int P = 1>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1) k_pair(const __grid_constant__ PairArgs a) {
-  static_assert(P == 1 || (P == 3 && EPI == kStore), "planes feed plain products");
+  static_assert((P == 3) == (EPI == kLsePlanes || EPI == kProbPlanes) || EPI == kStore, "the epilogue fits its operands");
   constexpr int kStages = stages<EPI, P>(), kStageBytes = stage_bytes<P>(), kBBytes = b_bytes<P>();
   constexpr int kBufs = EPI == kGluBwd ? 1 : 2, kEpiWarps = epi_warps<EPI>();
   constexpr bool kAlt = EPI == kLse || EPI == kProb;            // two sets of epilogue warps, alternate tiles
@@ -632,23 +658,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         }
         --it;                                 // the loop header counts one
         if (!ok) break;
+        const int col = q.n * 128 + half * 64;
+        if constexpr (EPI == kLsePlanes) {
+          if (row + lane < b.M)
+            a.part[(int64_t)(row + lane) * (2 * b.nt) + 2 * q.n + half] = max_sum(acc, b.N - col);
+        } else if constexpr (EPI == kProbPlanes) {
+          const int i0 = row + lane;
+          const int64_t tg = i0 < b.M ? a.target[i0] : -1;
+          const bool live = tg >= 0 && tg < a.V;
+          const float z = live ? a.lse[i0] : 0.f, d = live ? a.dloss[i0] : 0.f;
+          const int64_t tc = live ? tg - a.v0 - col : -1;         // the target's column among these
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t r[32];
+          for (int i = 0; i < 64; ++i) {      // a held-out row is zeros whatever its logits are
+            const float e = expf(acc[i] - z) - (tc == i ? 1.f : 0.f);
+            acc[i] = live ? d * e : 0.f;
+          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(acc[c + i]);
-          if (lane == 0) store_wait<0>();
-          __syncwarp();
-          stage_row(obuf, lane, r);
-          send<true>(b, &b.tc, obuf, q.ybase, row, q.n * 128 + half * 64 + c, lane);
-          __syncwarp();
+          for (int k = 0; k < 3; ++k) {       // planes.cuh's split, one plane after the other
+            uint32_t r[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              r[i] = fbplanes::pair(__float_as_uint(acc[2 * i]), __float_as_uint(acc[2 * i + 1]));
+              acc[2 * i] = fbplanes::rest(acc[2 * i], k == 0);
+              acc[2 * i + 1] = fbplanes::rest(acc[2 * i + 1], k == 0);
+            }
+            if (lane == 0) store_wait<0>();
+            __syncwarp();
+            stage_row(obuf, lane, r);
+            send<false>(b, k == 0 ? &b.tc : &a.tc2[k - 1], obuf, 0, row, col, lane);
+            __syncwarp();
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t r[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(acc[c + i]);
+            if (lane == 0) store_wait<0>();
+            __syncwarp();
+            stage_row(obuf, lane, r);
+            send<true>(b, &b.tc, obuf, q.ybase, row, col + c, lane);
+            __syncwarp();
+          }
         }
         continue;
       }
       if constexpr (EPI == kLseLong) {
         // kLse for more than kLseSlab stages: the tensor cores' accumulation truncates (6e-8 of the logit a stage,
         // all one way) and a loss is fp32, so tensor memory sums kLseSlab stages at a time and registers the rest.
-        constexpr float kLog2e = 1.44269504088896340736f;
         float v[64];
         const int row = q.m * 256 + (int)rank * kHalfM + qd * 32, c0 = half * 64, left = b.N - (q.n * 256 + c0);
         bool ok = true;
@@ -672,24 +729,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         }
         --it;                                 // the loop header counts one
         if (!ok) break;
-        if (left < 64) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= left) v[i] = -INFINITY;  // past the table
-        }
-        float m = v[0];
-#pragma unroll
-        for (int i = 1; i < 64; ++i) m = fmaxf(m, v[i]);
-        m *= kLog2e;
-        // nothing but -inf: subtract 0, so that exp2 gives zeros (and NaN stays NaN)
-        const float base = m == -INFINITY ? 0.f : m;
-        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          s0 += ex2(fmaf(v[i], kLog2e, -base));
-          s1 += ex2(fmaf(v[i + 1], kLog2e, -base));
-        }
-        if (row + lane < b.M) a.part[(int64_t)(row + lane) * (4 * b.nt) + 4 * q.n + half] = make_float2(m, s0 + s1);
+        if (row + lane < b.M) a.part[(int64_t)(row + lane) * (4 * b.nt) + 4 * q.n + half] = max_sum(v, left);
         continue;
       }
       const int buf = it % kBufs;
@@ -862,6 +902,11 @@ inline int make_map3(CUtensorMap *m, const void *base, int64_t rows, int64_t col
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fb::set_error(FB_ERR_ARG, "tensor map rejected (alignment or stride)");
   return FB_OK;
+}
+
+// A product's operand in boxes of box_rows rows: bf16, or fp32 as planes.
+inline int operand_map(CUtensorMap *m, const fbh::Mat &x, int64_t rows, int64_t cols, int box_rows) {
+  return x.plane ? make_map3(m, x.p, rows, cols, x.ld, x.plane, box_rows) : make_map(m, x.p, rows, cols, x.ld, box_rows);
 }
 
 inline bool map_ok(const void *p, int64_t ld, int es) {

@@ -9,14 +9,14 @@ namespace fbplanes {
 struct Split {
   uint32_t b0, b1, b2;                        // fp32 bits of the planes (low halves zero; b2's are cut on packing)
 };
+// What a plane leaves of x; `first`: x may be an infinity or NaN, which leaves nothing.
+__device__ __forceinline__ float rest(float x, bool first) {
+  const uint32_t b = __float_as_uint(x) & 0xFFFF0000u;
+  return first && (b & 0x7F800000u) == 0x7F800000u ? 0.f : x - __uint_as_float(b);
+}
 __device__ __forceinline__ Split split(float x) {
-  Split s;
-  s.b0 = __float_as_uint(x) & 0xFFFF0000u;
-  const bool fin = (s.b0 & 0x7F800000u) != 0x7F800000u;
-  const float r1 = fin ? x - __uint_as_float(s.b0) : 0.f;
-  s.b1 = __float_as_uint(r1) & 0xFFFF0000u;
-  s.b2 = __float_as_uint(r1 - __uint_as_float(s.b1));
-  return s;
+  const float r1 = rest(x, true);
+  return Split{__float_as_uint(x) & 0xFFFF0000u, __float_as_uint(r1) & 0xFFFF0000u, __float_as_uint(rest(r1, false))};
 }
 __device__ __forceinline__ uint32_t pair(uint32_t lo, uint32_t hi) { return __byte_perm(lo, hi, 0x7632); }
 

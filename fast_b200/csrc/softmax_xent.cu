@@ -1,39 +1,27 @@
 // Softmax cross entropy of rows h [n, D] against every row of a table w [V, D]:
 //   l = h w^T,  lse_i = log sum_v exp(l_iv),  loss_i = lse_i - l_i,target
 //   G = dloss_i (exp(l_iv - lse_i) - [v == target]),  dh = G w,  dw = G^T h
-// The logits are never kept.  bf16 (products on SM pairs, pair_gemm.cuh): the
-// forward reduces every 256-column tile of logits to a maximum and a sum per
-// row in its epilogue, one launch over the whole table, and a second kernel
-// joins them; the backward takes the table in pieces of as many rows as make a
-// G piece of kPieceBytes, computes G from the logits in the epilogue that would have stored
-// them, then adds G w to dh and writes G^T h.  fp32: the same products over
-// planes, pieces of logits in both directions, the forward carrying each
-// row's running maximum and sum from piece to piece.
+// The logits are never kept.  The products run on SM pairs (pair_gemm.cuh), fp32
+// rows as three bf16 planes: the forward reduces every tile of logits to a
+// maximum and a sum per row in its epilogue, one launch over the whole table,
+// and a second kernel joins them; the backward takes the table in pieces of as
+// many rows as make a G piece of kPieceBytes, computes G from the logits in the
+// epilogue that would have stored them, then adds G w to dh and writes G^T h.
 #include <cmath>
 #include "few_rows.cuh"
 #include "pair_gemm.cuh"
-#include "planes.cuh"
 
 namespace {
 
 using namespace fbh;
 
-// Memory of a piece (bf16: of G; fp32: of the logits, G's planes take 1.5 times
-// that beside them).  A piece that stays in the 126 MB L2 was expected to pay,
-// but its products are short: 48 / 160 / 512 MB a piece took 160 / 110 / 110 us
-// for 4,000 rows x 16,700 nodes x 104 and 2.45 / 2.22 / 2.13 ms for 8,192 x
-// 50,000 x 1,024; beyond that little changes and memory is not given back.
-constexpr int64_t kPieceBytes = 512ll << 20, kPieceBytesF32 = 256ll << 20;
+// Memory of a piece of G (bf16: 2 bytes an element, fp32: its planes' 6).  A
+// piece that stays in the 126 MB L2 was expected to pay, but its products are
+// short: 48 / 160 / 512 MB a piece took 160 / 110 / 110 us for 4,000 rows x
+// 16,700 nodes x 104 and 2.45 / 2.22 / 2.13 ms for 8,192 x 50,000 x 1,024 (bf16);
+// beyond that little changes and memory is not given back.
+constexpr int64_t kPieceBytes = 512ll << 20;
 constexpr int64_t kPartBytes = 256ll << 20;   // of the forward's partials
-
-struct MaxSum {
-  float m, s;                                // sum of exp(l - m); m = -inf, s = 0: nothing yet
-};
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return MaxSum{m, a.s + b.s};     // a NaN sum stays one
-  return MaxSum{m, a.s * expf(a.m - m) + b.s * expf(b.m - m)};
-}
 
 __device__ __forceinline__ float value(const float *p) { return *p; }
 __device__ __forceinline__ float value(const uint16_t *p) { return __uint_as_float((uint32_t)*p << 16); }   // bf16
@@ -91,73 +79,6 @@ __global__ void __launch_bounds__(TH == 32 ? 128 : TH) k_xent_finish(const float
   loss[r] = tg < 0 ? 0.f : (tg >= V ? NAN : z - l);
 }
 
-// One CTA per row (pitch ldl, a multiple of 4): the piece's maximum and sum
-// join the row's state; the target's logit is picked up when the piece holds
-// it.  last: lse and loss.
-__global__ void __launch_bounds__(256) k_xent_rows(const float *l, int64_t ldl, int v0, int cols, int64_t V,
-                                                   const int64_t *target, float *state, float *tl, float *loss,
-                                                   float *lse, int first, int last) {
-  __shared__ MaxSum sm[8];
-  fb::pdl_enter();
-  const int64_t r = blockIdx.x;
-  const float *p = l + r * ldl;
-  MaxSum a{-INFINITY, 0.f};
-  for (int c = threadIdx.x * 4; c < cols; c += 1024) {
-    float v[4];
-    *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p + c);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (c + k >= cols) v[k] = -INFINITY;   // past the piece
-    const float m = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), a.m);
-    const float base = m == -INFINITY ? 0.f : m;           // nothing but -inf: zeros, and NaN stays NaN
-    a.s = a.s * expf(a.m - base) + expf(v[0] - base) + expf(v[1] - base) + expf(v[2] - base) + expf(v[3] - base);
-    a.m = m;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = join(a, MaxSum{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = a;
-  __syncthreads();
-  if (threadIdx.x) return;
-#pragma unroll
-  for (int w = 1; w < 8; ++w) a = join(a, sm[w]);
-  if (!first) a = join(a, MaxSum{state[2 * r], state[2 * r + 1]});
-  const int64_t t = target[r];
-  float lt = first ? 0.f : tl[r];
-  if (t >= v0 && t < v0 + cols) lt = p[t - v0];
-  if (!last) {
-    state[2 * r] = a.m;
-    state[2 * r + 1] = a.s;
-    tl[r] = lt;
-    return;
-  }
-  const float z = a.m + logf(a.s);
-  lse[r] = z;
-  loss[r] = t < 0 ? 0.f : (t >= V ? NAN : z - lt);
-}
-
-// fp32 rows: G of one piece as planes (pitch ldl, a multiple of 4; the columns
-// past cols are never read).  Rows held out of the loss are zeros whatever
-// their logits are.
-__global__ void __launch_bounds__(256) k_xent_grad(const float *l, int64_t ldl, int v0, int cols, int64_t V,
-                                                   const int64_t *target, const float *lse, const float *dloss,
-                                                   uint16_t *G, int64_t plane) {
-  fb::pdl_enter();
-  const int64_t r = blockIdx.x;
-  const int64_t t = target[r];
-  const bool live = t >= 0 && t < V;
-  const float z = lse[r], d = dloss[r];
-  for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(l + r * ldl + c);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = d * (expf(v[k] - z) - (t == v0 + c + k ? 1.f : 0.f));
-    }
-    fbplanes::put4(G + r * ldl + c, plane, v[0], v[1], v[2], v[3]);
-  }
-}
-
 // bf16 rows: dst = src rounded.
 __global__ void k_round_rows(const float *src, int64_t lds, __nv_bfloat16 *dst, int64_t ldd, int64_t rows, int cols) {
   fb::pdl_enter();
@@ -170,9 +91,8 @@ __global__ void k_round_rows(const float *src, int64_t lds, __nv_bfloat16 *dst, 
 }
 
 // Table rows per piece: a multiple of 64, so that pieces start 16-byte aligned.
-int64_t piece_rows(int64_t n, int64_t V, int es) {
-  const int64_t bytes = es == 4 ? kPieceBytesF32 : kPieceBytes;
-  const int64_t r = std::max<int64_t>(256, bytes / es / std::max<int64_t>(n, 1) / 64 * 64);
+int64_t piece_rows(int64_t n, int64_t V, int bytes) {
+  const int64_t r = std::max<int64_t>(256, kPieceBytes / bytes / std::max<int64_t>(n, 1) / 64 * 64);
   return std::min<int64_t>(r, round_up(V, 64));
 }
 
@@ -199,59 +119,13 @@ int check(const fb_softmax_xent *a, bool bwd) {
 
 Mat rows_from(const Mat &m, int64_t r) { return Mat{static_cast<const uint16_t *>(m.p) + r * m.ld, m.ld, m.plane}; }
 
-int logits_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &wp, int cols, float *l, int64_t pr) {
-  const Product p = rows_product(h, a.n, a.D, wp, false, cols, Out{l, pr, FB_F32, 0});
-  return products(c, &p, 1);
-}
-
-int forward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
-  const int64_t pr = piece_rows(a.n, a.V, 4);
-  FBH_TAKE(l, c, float, a.n * pr);
-  FBH_TAKE(state, c, float, 2 * a.n);
-  FBH_TAKE(tl, c, float, a.n);
-  for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
-    const int cols = (int)std::min<int64_t>(pr, a.V - v0);
-    FBH_TRY(logits_f32(c, a, h, rows_from(w, v0), cols, l, pr));
-    if (!c.dry) {
-      FB_TRY_CUDA(fb::launch(k_xent_rows, (unsigned)a.n, 256, 0, c.stream, (const float *)l, pr, (int)v0, cols, a.V,
-                             a.target, state, tl, a.loss, a.lse, (int)(v0 == 0), (int)(v0 + pr >= a.V)));
-      FB_LAUNCHED("k_xent_rows");
-    }
-    // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
-    if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
-  }
-  return FB_OK;
-}
-
-int backward_f32(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
-  const int64_t pr = piece_rows(a.n, a.V, 4);
-  FBH_TAKE(l, c, float, a.n * pr);
-  FBH_TAKE(G, c, uint16_t, 3 * a.n * pr);
-  for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
-    const int cols = (int)std::min<int64_t>(pr, a.V - v0);
-    const Mat wp = rows_from(w, v0), Gm{G, pr, a.n * pr};
-    FBH_TRY(logits_f32(c, a, h, wp, cols, l, pr));
-    if (!c.dry) {
-      FB_TRY_CUDA(fb::launch(k_xent_grad, dim3((unsigned)a.n, (unsigned)std::min(64, (cols + 1023) / 1024)), 256, 0,
-                             c.stream, (const float *)l, pr, (int)v0, cols, a.V, a.target, (const float *)a.lse, a.dloss,
-                             G, a.n * pr));
-      FB_LAUNCHED("k_xent_grad");
-    }
-    void *dw = a.dw ? static_cast<float *>(a.dw) + v0 * a.lddw : nullptr;
-    const Product p[2] = {rows_product(Gm, a.n, cols, wp, true, a.D, Out{a.dh, a.lddh, FB_F32, v0 > 0}),
-                          columns_product(Gm, a.n, cols, h, a.D, Out{dw, a.lddw, FB_F32, a.accumulate})};
-    FBH_TRY(products(c, p, 2));
-    if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
-  }
-  return FB_OK;
-}
-
 // The common fields of a launch over the logits of rows h against table rows w.
 int logits_args(fbpair::PairArgs &p, const fb_softmax_xent &a, const Mat &h, int64_t n, const Mat &w, int cols) {
   using namespace fbpair;
-  one_product(p, n, cols, 256, tiles_of(a.D, BK), 1);
-  FBH_TRY(make_map(&p.p[0].ta[0], h.p, n, a.D, h.ld, kHalfM));
-  return make_map(&p.p[0].tb[0], w.p, cols, a.D, w.ld, 128);
+  const bool planes = h.plane > 0;
+  one_product(p, n, cols, planes ? 128 : 256, tiles_of(a.D, BK), 1);
+  FBH_TRY(operand_map(&p.p[0].ta[0], h, n, a.D, kHalfM));
+  return operand_map(&p.p[0].tb[0], w, cols, a.D, planes ? 64 : 128);
 }
 
 // lse and loss of rows r0 .. r0 + n - 1 (h: those rows) from their partials.
@@ -275,12 +149,13 @@ int forward_few(Call &c, const fb_softmax_xent &a) {
   return a.type == FB_F32 ? finish<float>(c, a, part, np, h, w, 0, a.n) : finish<uint16_t>(c, a, part, np, h, w, 0, a.n);
 }
 
-int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
+int forward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   using namespace fbpair;
-  const int nt = tiles_of(a.V, 256);
-  // rows per launch: the partials of one stay within kPieceBytes
-  const int64_t rows = std::min<int64_t>(a.n, std::max<int64_t>(256, kPartBytes / (32ll * nt) / 256 * 256));
-  FBH_TAKE(part, c, float2, rows * 4 * nt);
+  const bool f32 = a.type == FB_F32, longer = !f32 && tiles_of(a.D, BK) > kLseSlab;
+  const int64_t np = (int64_t)tiles_of(a.V, f32 ? 128 : 256) * (longer ? 4 : 2);   // partials of a row
+  // rows per launch: the partials of one stay within kPartBytes
+  const int64_t rows = std::min<int64_t>(a.n, std::max<int64_t>(256, kPartBytes / (8 * np) / 256 * 256));
+  FBH_TAKE(part, c, float2, rows * np);
   if (c.dry) return FB_OK;
   for (int64_t r0 = 0; r0 < a.n; r0 += rows) {
     const int64_t n = std::min(rows, a.n - r0);
@@ -288,17 +163,25 @@ int forward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) 
     PairArgs p;
     FBH_TRY(logits_args(p, a, hp, n, w, (int)a.V));
     p.part = part;
-    FBH_TRY(p.p[0].kb[0] > kLseSlab ? launch_pair<kLseLong>(p, c.stream) : launch_pair<kLse>(p, c.stream));
-    FBH_TRY(finish<uint16_t>(c, a, part, (p.p[0].kb[0] > kLseSlab ? 4 : 2) * nt, hp, w, r0, n));
+    if (f32) {
+      FBH_TRY((launch_pair<kLsePlanes, 3>(p, c.stream)));
+      FBH_TRY(finish<float>(c, a, part, (int)np, Mat{static_cast<const float *>(a.h) + r0 * a.ldh, a.ldh}, Mat{a.w, a.ldw},
+                            r0, n));
+    } else {
+      FBH_TRY(longer ? launch_pair<kLseLong>(p, c.stream) : launch_pair<kLse>(p, c.stream));
+      FBH_TRY(finish<uint16_t>(c, a, part, (int)np, hp, w, r0, n));
+    }
   }
   return FB_OK;
 }
 
-int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
+int backward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   using namespace fbpair;
-  const int64_t pr = piece_rows(a.n, a.V, 2);
-  const bool sum = a.dh && pr < a.V;         // dh adds up over the pieces in fp32
-  FBH_TAKE(G, c, __nv_bfloat16, a.n * pr);
+  const bool f32 = a.type == FB_F32;
+  const int np = f32 ? 3 : 1;                 // planes of G
+  const int64_t pr = piece_rows(a.n, a.V, 2 * np);
+  const bool sum = !f32 && a.dh && pr < a.V;  // bf16 dh adds up over the pieces in fp32
+  FBH_TAKE(G, c, uint16_t, np * a.n * pr);
   const int64_t lds = round_up(a.D, 4);
   float *acc = nullptr;
   if (sum) {
@@ -307,7 +190,7 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
   }
   for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
     const int cols = (int)std::min<int64_t>(pr, a.V - v0);
-    const Mat wp = rows_from(w, v0), Gm{G, pr};
+    const Mat wp = rows_from(w, v0), Gm{G, pr, f32 ? a.n * pr : 0};
     if (!c.dry) {
       PairArgs p;
       FBH_TRY(logits_args(p, a, h, a.n, wp, cols));
@@ -316,14 +199,16 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
       p.dloss = a.dloss;
       p.V = a.V;
       p.v0 = v0;
-      FBH_TRY(make_map(&p.p[0].tc, G, a.n, cols, pr, 32));
-      FBH_TRY(launch_pair<kProb>(p, c.stream));
+      for (int k = 0; k < np; ++k)
+        FBH_TRY(make_map(k == 0 ? &p.p[0].tc : &p.tc2[k - 1], G + k * Gm.plane, a.n, cols, pr, 32));
+      FBH_TRY(f32 ? (launch_pair<kProbPlanes, 3>(p, c.stream)) : (launch_pair<kProb>(p, c.stream)));
     }
     void *dw = a.dw ? static_cast<uint8_t *>(a.dw) + v0 * a.lddw * elem(a.grad_type) : nullptr;
-    const Product p[2] = {rows_product(Gm, a.n, cols, wp, true, a.D,
-                                       sum ? Out{acc, lds, FB_F32, v0 > 0} : Out{a.dh, a.lddh, FB_BF16, 0}),
+    const Out dh = sum ? Out{acc, lds, FB_F32, v0 > 0} : Out{a.dh, a.lddh, a.type, f32 && v0 > 0};
+    const Product p[2] = {rows_product(Gm, a.n, cols, wp, true, a.D, dh),
                           columns_product(Gm, a.n, cols, h, a.D, Out{dw, a.lddw, a.grad_type, a.accumulate})};
     FBH_TRY(products(c, p, 2));
+    // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
     if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
   }
   if (sum && !c.dry) {
@@ -336,12 +221,12 @@ int backward_bf16(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w)
 }
 
 int run(Call &c, const fb_softmax_xent &a, bool bwd) {
-  if (few_rows_ok(a.type, bwd, a.n, a.D, a.D * a.V) && (!bwd || a.V <= kFewRowsTable)) return bwd ? few_rows_xent_bwd(c, a) : forward_few(c, a);
+  if (few_rows_ok(a.type, bwd, a.n, a.D, a.D * a.V) && (!bwd || a.V <= kFewRowsTable))
+    return bwd ? few_rows_xent_bwd(c, a) : forward_few(c, a);
   Mat h, w;
   const Operand ops[2] = {{Mat{a.h, a.ldh}, a.n, a.D, &h}, {Mat{a.w, a.ldw}, a.V, a.D, &w}};
   FBH_TRY(operands(c, a.type, ops, 2));
-  if (a.type == FB_F32) return bwd ? backward_f32(c, a, h, w) : forward_f32(c, a, h, w);
-  return bwd ? backward_bf16(c, a, h, w) : forward_bf16(c, a, h, w);
+  return bwd ? backward(c, a, h, w) : forward(c, a, h, w);
 }
 
 }  // namespace
