@@ -185,7 +185,8 @@ template <typename T, int MT> __global__ void __launch_bounds__(256) k_few_outer
     return;
   }
   __shared__ __align__(16) float as[128][MT];  // the CTA's rows of a
-  const int c0 = (int)(blk % j.col_tiles) * 128 + lane * 4;
+  // this lane's columns: c0 + e step, four side by side where they are written at once, else a warp's side by side
+  const int c0 = (int)(blk % j.col_tiles) * 128 + (j.wide ? lane * 4 : lane), step = j.wide ? 1 : 32;
   const int64_t R0 = (int64_t)(blk / j.col_tiles) * 128;
   const int rows = (int)min((int64_t)128, j.rows - R0);
 #pragma unroll
@@ -197,7 +198,8 @@ template <typename T, int MT> __global__ void __launch_bounds__(256) k_few_outer
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) b[m][e] = m < a.n && c0 + e < j.cols ? read_f<T>(j.b, m * j.ldb + c0 + e, j.b_f32) : 0.f;
+    for (int e = 0; e < 4; ++e)
+      b[m][e] = m < a.n && c0 + e * step < j.cols ? read_f<T>(j.b, m * j.ldb + c0 + e * step, j.b_f32) : 0.f;
   __syncthreads();
   for (int q = warp * 16; q < min(warp * 16 + 16, rows); ++q) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -211,7 +213,7 @@ template <typename T, int MT> __global__ void __launch_bounds__(256) k_few_outer
     if (!j.wide) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c0 + e < j.cols) write_f(j, at + e, v[e]);
+        if (c0 + e * 32 < j.cols) write_f(j, at + e * 32, v[e]);
     } else if (c0 < j.cols) {
       if (j.o_f32) {
         *reinterpret_cast<float4 *>(static_cast<float *>(j.out) + at) = make_float4(v[0], v[1], v[2], v[3]);

@@ -90,7 +90,7 @@ void plan(PairArgs &a, bool planes) {
   }
   const int mean = (int)std::max<int64_t>(1, (work + slots - 1) / slots);
   int best = longest;
-  if (tiles < 8ll * slots && longest >= 2 * min_stages(planes)) {
+  if (longest >= 2 * min_stages(planes)) {
     double least = 0;
     for (int part : {longest, 2 * mean, mean, (mean + 1) / 2, (mean + 2) / 3}) {
       if (part > longest || part < 1) continue;
