@@ -1,7 +1,7 @@
 // Softmax cross entropy of rows h [n, D] against every row of a table w [V, D]:
 //   l = h w^T,  lse_i = log sum_v exp(l_iv),  loss_i = lse_i - l_i,target
 //   G = dloss_i (exp(l_iv - lse_i) - [v == target]),  dh = G w,  dw = G^T h
-// The logits are never kept.  The products run on SM pairs (pair_gemm.cuh), fp32
+// The logits are not kept (but see few_tiles()).  The products run on SM pairs (pair_gemm.cuh), fp32
 // rows as three bf16 planes: the forward reduces every tile of logits to a
 // maximum and a sum per row in its epilogue, one launch over the whole table,
 // and a second kernel joins them; the backward takes the table in pieces of as
@@ -79,6 +79,51 @@ __global__ void __launch_bounds__(TH == 32 ? 128 : TH) k_xent_finish(const float
   loss[r] = tg < 0 ? 0.f : (tg >= V ? NAN : z - l);
 }
 
+// fp32 rows of few tiles (few_tiles()): from stored logits [n, ldl], ldl a multiple of 4.  A warp reduces an eighth of
+// a row to its partial (max, sum of exp2), as the products' epilogue would have.
+__global__ void __launch_bounds__(256) k_logit_parts(const float *l, int64_t ldl, int V, float2 *part) {
+  constexpr float kLog2e = 1.44269504088896340736f;
+  fb::pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float *p = l + blockIdx.x * ldl;
+  float m = -INFINITY, s = 0.f;
+  auto fold = [&](float m2, float s2) {
+    const float nm = fmaxf(m, m2), base = nm == -INFINITY ? 0.f : nm;    // nothing but -inf: zeros, and NaN stays NaN
+    s = s * exp2f(m - base) + s2 * exp2f(m2 - base);
+    m = nm;
+  };
+  for (int c = warp * 32 + lane; c < V; c += 256) {
+    const float v = p[c];
+    const float nm = fmaxf(m, v * kLog2e), base = nm == -INFINITY ? 0.f : nm;
+    s = s * exp2f(m - base) + exp2f(fmaf(v, kLog2e, -base));
+    m = nm;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    fold(m2, s2);
+  }
+  if (lane == 0) part[(int64_t)blockIdx.x * 8 + warp] = make_float2(m, s);
+}
+
+// The planes of G, pitch ldl as the logits'; columns past V are never read.
+__global__ void __launch_bounds__(256) k_logit_grad(const float *l, int64_t ldl, int V, const int64_t *target,
+                                                    const float *lse, const float *dloss, uint16_t *G, int64_t plane) {
+  fb::pdl_enter();
+  const int64_t r = blockIdx.x, t = target[r];
+  const bool live = t >= 0 && t < V;          // a held-out row is zeros whatever its logits are
+  const float z = lse[r], d = dloss[r];
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (c >= V) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(l + r * ldl + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = d * (expf(v[k] - z) - (t == c + k ? 1.f : 0.f));
+  }
+  fbplanes::put4(G + r * ldl + c, plane, v[0], v[1], v[2], v[3]);
+}
+
 // bf16 rows: dst = src rounded.
 __global__ void k_round_rows(const float *src, int64_t lds, __nv_bfloat16 *dst, int64_t ldd, int64_t rows, int cols) {
   fb::pdl_enter();
@@ -128,6 +173,20 @@ int logits_args(fbpair::PairArgs &p, const fb_softmax_xent &a, const Mat &h, int
   return operand_map(&p.p[0].tb[0], w, cols, a.D, planes ? 64 : 128);
 }
 
+// fp32 rows whose logits make too few tiles for the SM pairs, of sums long enough to be split: the launches that keep
+// no logits do not split them, so here the logits are stored (a few MB) and read again.
+// us, stored / not, forward and backward together, rows x width, nodes: 548 x 3,942, 657 (18 tiles) 118 / 180;
+// 100 x 2,048, 1,000 (8) 52 / 89; 200 x 600, 1,000 (8) 45 / 48; with 36 tiles, at 200 rows and 4,600 nodes, 255 / 274 for
+// 4,096 columns but 162 / 159 for 2,048 and 92 / 87 for 1,024.
+bool few_tiles(const fb_softmax_xent &a) {
+  return a.type == FB_F32 && a.D > 8 * fbpair::BK &&
+         ((a.n + 255) / 256) * ((a.V + 127) / 128) * 4 <= fbtc::num_sms() / 2;
+}
+int stored_logits(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w, float *l, int64_t ldl) {
+  const Product p = rows_product(h, a.n, a.D, w, false, (int)a.V, Out{l, ldl, FB_F32, 0});
+  return products(c, &p, 1);
+}
+
 // lse and loss of rows r0 .. r0 + n - 1 (h: those rows) from their partials.
 template <typename U>
 int finish(Call &c, const fb_softmax_xent &a, const float2 *part, int np, const Mat &h, const Mat &w, int64_t r0,
@@ -151,6 +210,16 @@ int forward_few(Call &c, const fb_softmax_xent &a) {
 
 int forward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   using namespace fbpair;
+  if (few_tiles(a)) {
+    const int64_t ldl = round_up(a.V, 64);
+    FBH_TAKE(l, c, float, a.n * ldl);
+    FBH_TAKE(part, c, float2, a.n * 8);
+    FBH_TRY(stored_logits(c, a, h, w, l, ldl));
+    if (c.dry) return FB_OK;
+    FB_TRY_CUDA(fb::launch(k_logit_parts, (unsigned)a.n, 256, 0, c.stream, (const float *)l, ldl, (int)a.V, part));
+    FB_LAUNCHED("k_logit_parts");
+    return finish<float>(c, a, part, 8, Mat{a.h, a.ldh}, Mat{a.w, a.ldw}, 0, a.n);
+  }
   const bool f32 = a.type == FB_F32, longer = !f32 && tiles_of(a.D, BK) > kLseSlab;
   const int64_t np = (int64_t)tiles_of(a.V, f32 ? 128 : 256) * (longer ? 4 : 2);   // partials of a row
   // rows per launch: the partials of one stay within kPartBytes
@@ -182,6 +251,12 @@ int backward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   const int64_t pr = piece_rows(a.n, a.V, 2 * np);
   const bool sum = !f32 && a.dh && pr < a.V;  // bf16 dh adds up over the pieces in fp32
   FBH_TAKE(G, c, uint16_t, np * a.n * pr);
+  const bool few = few_tiles(a);
+  float *l = nullptr;                         // few: the logits
+  if (few) {
+    FBH_TAKE(t, c, float, a.n * pr);
+    l = t;
+  }
   const int64_t lds = round_up(a.D, 4);
   float *acc = nullptr;
   if (sum) {
@@ -191,7 +266,14 @@ int backward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   for (int64_t v0 = 0; v0 < a.V; v0 += pr) {
     const int cols = (int)std::min<int64_t>(pr, a.V - v0);
     const Mat wp = rows_from(w, v0), Gm{G, pr, f32 ? a.n * pr : 0};
-    if (!c.dry) {
+    if (few) {                                // one piece
+      FBH_TRY(stored_logits(c, a, h, w, l, pr));
+      if (!c.dry) {
+        FB_TRY_CUDA(fb::launch(k_logit_grad, dim3((unsigned)a.n, (unsigned)((a.V + 1023) / 1024)), 256, 0, c.stream,
+                               (const float *)l, pr, (int)a.V, a.target, (const float *)a.lse, a.dloss, G, a.n * pr));
+        FB_LAUNCHED("k_logit_grad");
+      }
+    } else if (!c.dry) {
       PairArgs p;
       FBH_TRY(logits_args(p, a, h, a.n, wp, cols));
       p.target = a.target;

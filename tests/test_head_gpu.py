@@ -275,6 +275,13 @@ def test_softmax_xent(cuda, n, d, v, pad, dtype):
     _check("accumulated dw", buf, G.t() @ Hd + 0.25, eG.t() @ Hd.abs() + _c(n) * ((G.abs() + eG).t() @ Hd.abs()), F32)
 
 
+# few tiles of long sums: fp32 stores these logits, in parts of the sums
+@pytest.mark.parametrize("n,d,v,pad", [(9, 513, 2048, 0), (300, 1030, 657, 3), (60, 2050, 1, 0), (256, 640, 130, 4)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_softmax_xent_few_tiles_of_long_sums(cuda, n, d, v, pad, dtype):
+    test_softmax_xent(cuda, n, d, v, pad, dtype)
+
+
 @pytest.mark.parametrize("n,d,v,pad", [(1, 130, 9001, 0), (2, 128, 9000, 0), (2, 127, 9003, 1), (2, 1030, 2000, 0),
                                        (3, 128, 9000, 8), (7, 1030, 2001, 0), (8, 127, 9003, 0)])
 @pytest.mark.parametrize("dtype", TYPES)
