@@ -60,6 +60,16 @@ EncodeTiledFn encode_fn() {
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<EncodeTiledFn>(p);
   }
+  // The encoder is a driver call and needs a current context, which the
+  // runtime makes current only with a thread's first call of its own that
+  // touches the device; autograd's threads may come here before any.
+  static thread_local uint64_t bound = 0;      // devices whose context this thread has had
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(bound >> (dev & 63) & 1)) {
+    cudaSetDevice(dev);
+    bound |= (uint64_t)1 << (dev & 63);
+  }
   return fn;
 }
 
