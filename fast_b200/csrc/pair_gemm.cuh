@@ -9,9 +9,10 @@
 //   (their layouts, tile widths and output types are fields): a backward pass's
 //   products are short, and a launch of its own costs one 3 to 4 us of ramp.
 //   P = 3: fp32 operands, each as three bf16 planes x = x0 + x1 + x2 of 8
-//   significant bits (exact: 24 bits in all).  Six of the nine plane products
-//   are summed, smallest first; the three left out are below 2^-24 of the
-//   product.  The tensor cores' accumulation truncates, so it runs over 64 k
+//   significant bits (exact: 24 bits in all; planes.cuh).  Six of the nine plane
+//   products are summed, smallest first.  The three left out are below 2^-21 of
+//   the product (x1 < 2^-7 x, x2 < 2^-15 x), 2^-24.5 on average, all of its sign.
+//   The tensor cores' accumulation truncates, so it runs over 64 k
 //   only: the epilogue warps add each such slab to an fp32 sum in registers
 //   while the next one is computed.  kLsePlanes and kProbPlanes are kLse and
 //   kProb on that sum, in registers: the logits of fp32 rows are not stored
@@ -321,6 +322,31 @@ __device__ __forceinline__ void send(const PairProb &a, const CUtensorMap *tc, c
           p[r * a.ldc + c] =
               *reinterpret_cast<const uint16_t *>(buf + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
       }
+  }
+}
+
+// 64 values of a lane's row as their planes (planes.cuh), one plane after the other, to the launch's three outputs.
+template <bool FINITE>
+__device__ __forceinline__ void send_planes(const PairArgs &a, float (&v)[64], uint8_t *buf, int row, int col, int lane) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    uint32_t r[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      if (k == 2) {
+        r[i] = fbplanes::pair(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]));
+        continue;
+      }
+      const fbplanes::Cut lo = fbplanes::cut<FINITE>(v[2 * i]), hi = fbplanes::cut<FINITE>(v[2 * i + 1]);
+      r[i] = fbplanes::pair(lo.lead, hi.lead);
+      v[2 * i] = lo.rest;
+      v[2 * i + 1] = hi.rest;
+    }
+    if (lane == 0) store_wait<0>();
+    __syncwarp();
+    stage_row(buf, lane, r);
+    send<false>(a.p[0], k == 0 ? &a.p[0].tc : &a.tc2[k - 1], buf, 0, row, col, lane);
+    __syncwarp();
   }
 }
 
@@ -673,21 +699,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
             const float e = expf(acc[i] - z) - (tc == i ? 1.f : 0.f);
             acc[i] = live ? d * e : 0.f;
           }
+          float fin = 0.f;
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {       // planes.cuh's split, one plane after the other
-            uint32_t r[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              r[i] = fbplanes::pair(__float_as_uint(acc[2 * i]), __float_as_uint(acc[2 * i + 1]));
-              acc[2 * i] = fbplanes::rest(acc[2 * i], k == 0);
-              acc[2 * i + 1] = fbplanes::rest(acc[2 * i + 1], k == 0);
-            }
-            if (lane == 0) store_wait<0>();
-            __syncwarp();
-            stage_row(obuf, lane, r);
-            send<false>(b, k == 0 ? &b.tc : &a.tc2[k - 1], obuf, 0, row, col, lane);
-            __syncwarp();
-          }
+          for (int i = 0; i < 64; ++i) fin = fbplanes::probe(acc[i], fin);
+          if (__all_sync(0xffffffffu, fin == 0.f)) send_planes<true>(a, acc, obuf, row, col, lane);
+          else send_planes<false>(a, acc, obuf, row, col, lane);
         } else {
 #pragma unroll
           for (int c = 0; c < 64; c += 32) {

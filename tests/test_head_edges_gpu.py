@@ -54,3 +54,100 @@ def test_block_alone_trains(cuda):
     x = torch.randn(150, 64, device=cuda).bfloat16()
     ffn(x).backward(torch.ones(150, 64, device=cuda, dtype=BF))
     assert all(bool(p.grad.isfinite().all()) for p in ffn.parameters())
+
+
+# ---- infinities ------------------------------------------------------------------------------------------------------
+# rows on both sides of every rule that picks a path: few rows, tiles, fp32 logits stored in split sums
+@pytest.mark.parametrize("n,d,v", [(1, 40, 700), (8, 33, 700), (9, 33, 700), (300, 40, 3000), (60, 600, 500)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_softmax_xent_nodes_masked_by_an_infinite_bias(cuda, n, d, v, dtype):
+    """h has a column of ones, the table -inf there for some nodes: they have probability 0."""
+    from fast_b200 import ops
+    g = _gen(cuda, n, d, v)
+    h, w = _mat(cuda, g, n, d, dtype), _mat(cuda, g, v, d, dtype, 2 * d ** -0.5)
+    h[:, 0] = 1
+    masked = torch.arange(v, device=cuda) % 3 == 1
+    w[masked, 0] = -math.inf
+    t = torch.randint(0, v // 3, (n,), device=cuda, generator=g) * 3
+    dl = torch.rand(n, device=cuda, generator=g) + 0.5
+    loss, lse = ops.softmax_xent_fwd(h, w, t)
+    H, W = h.double(), w.double()[~masked]
+    L = H @ W.t()
+    Z = torch.logsumexp(L, 1)
+    el = (_c(d) * (H.abs() @ W.abs().t())).max(1).values
+    fn = 2.0 ** -20 * (1 + Z.abs() + L.abs().max(1).values)
+    at = (t - (t + 1) // 3).unsqueeze(1)                       # t's place among the nodes left
+    _check("lse", lse, Z, el + fn, F32)
+    _check("loss", loss, Z - L.gather(1, at)[:, 0], 2 * el + fn, F32)
+    dh, dw = ops.softmax_xent_bwd(h, w, t, lse, dl)
+    P = torch.softmax(L, 1)
+    G = P.clone()
+    G.scatter_add_(1, at, torch.full_like(at, -1, dtype=torch.float64))
+    scale = dl.double().unsqueeze(1)
+    eG = scale * (P * (2 * el + 2 * fn).unsqueeze(1) + 2.0 ** -22 * G.abs())
+    G = G * scale
+    eG = eG + (2.0 ** -8 if dtype == BF else 0.0) * (G.abs() + eG)
+    assert bool((dw[masked] == 0).all())
+    _check("dw", dw[~masked], G.t() @ H, eG.t() @ H.abs() + _c(n) * ((G.abs() + eG).t() @ H.abs()), dtype)
+    # the bias column of dh is 0 times -inf; the others are sums over the nodes left
+    _check("dh", dh[:, 1:], (G @ W)[:, 1:], (eG @ W.abs() + _c(v) * ((G.abs() + eG) @ W.abs()))[:, 1:], dtype)
+
+
+@pytest.mark.parametrize("n", [1, 8, 9, 200])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_ffn_with_infinite_values(cuda, n, dtype):
+    """An infinite weight makes infinities of its own column, an infinite row reaches no other row."""
+    from fast_b200 import ops
+    d, f = 40, 72
+    g = _gen(cuda, n, d, f)
+    x = _mat(cuda, g, n, d, dtype)
+    wg, wu, wd = _mat(cuda, g, f, d, dtype, 0.2), _mat(cuda, g, f, d, dtype, 0.2), _mat(cuda, g, d, f, dtype, 0.2)
+    plain = ops.gated_ffn_fwd(x, wg, wu, wd)
+    G, U = x.double() @ wg.double().t(), x.double() @ wu.double().t()
+    H = G * torch.sigmoid(G) * U
+    big = wd.clone()
+    big[5, 7], big[6, 7] = math.inf, -math.inf
+    y = ops.gated_ffn_fwd(x, wg, wu, big)
+    sure = H[:, 7].abs() > 1e-2                                 # rows whose sign no rounding turns
+    want = torch.where(H[:, 7] > 0, math.inf, -math.inf)
+    assert bool((y[sure, 5].double() == want[sure]).all()) and bool((y[sure, 6].double() == -want[sure]).all())
+    rest = [k for k in range(d) if k not in (5, 6)]
+    assert torch.equal(y[:, rest], plain[:, rest])
+    if n > 1:
+        x2 = x.clone()
+        x2[1, 3] = math.inf
+        y = ops.gated_ffn_fwd(x2, wg, wu, wd)
+        keep = torch.arange(n, device=cuda) != 1
+        assert torch.equal(y[keep], plain[keep]) and not bool(torch.isfinite(y[1]).any())
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_fp32_products_of_infinities(cuda, value):
+    """Logits of one node (lse is the logit itself) from one infinite element against ones, halves, short and long
+    significands, zero and infinities."""
+    from fast_b200 import ops
+    n, d = 12, 40
+    h = torch.full((n, d), 0.375, device=cuda)
+    h[:, 5] = torch.tensor([1, -1, 0.5, 1 + 2.0 ** -10, 1 / 3, -1 / 3, 1e-20, 3e38, 0, math.inf, -math.inf, math.nan], device=cuda)
+    w = torch.full((1, d), 0.25, device=cuda)
+    w[0, 5] = value
+    want = (h.double() @ w.double().t())[:, 0]
+    # one logit: lse = max + log(1), but an infinite maximum has no finite distance to itself
+    lse = ops.softmax_xent_fwd(h, w, torch.zeros(n, dtype=torch.int64, device=cuda))[1].double()
+    low = want == -math.inf
+    assert bool((lse[low] == -math.inf).all()) and not bool(torch.isfinite(lse).any())
+    # the same through the gated block's last product: relu(1) * 1 in column 5, weights of the table's row
+    x = torch.zeros(n, 16, device=cuda)
+    x[:, 0] = 1
+    x[:, 1:9] = torch.randn(n, 8, device=cuda)
+    wg, wu, wd = torch.zeros(24, 16, device=cuda), torch.zeros(24, 16, device=cuda), torch.ones(16, 24, device=cuda)
+    wg[:, 0] = 1
+    wu[:, 0] = h[3, 5]
+    wd[4, 5] = value
+    y = ops.gated_ffn_fwd(x, wg, wu, wd, act="relu")
+    ref = (x.double() @ wg.double().t()).relu() * (x.double() @ wu.double().t()) @ wd.double().t()
+    assert torch.equal(y[:, 4].double().isnan(), ref[:, 4].isnan())
+    if not math.isnan(value):
+        assert bool((y[:, 4].double() == ref[:, 4]).all())
+    other = [k for k in range(16) if k != 4]
+    assert bool(torch.isfinite(y[:, other]).all())
