@@ -150,6 +150,8 @@ struct OutJob {
   void *out;
   int cols, a_f32, b_f32, o_f32, accumulate, kind, splits, wide;   // wide: aligned groups of 4, written
   unsigned first, col_tiles;
+  const int64_t *target;                     // given: rows m whose target is not one of V are left out
+  int64_t V;
 };
 struct OutArgs {
   OutJob j[4];
@@ -196,10 +198,12 @@ template <typename T, int MT> __global__ void __launch_bounds__(256) k_few_outer
   }
   float b[MT][4];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m) {
+    const bool live = m < a.n && (!j.target || (j.target[m] >= 0 && j.target[m] < j.V));   // zeros against a's zeros
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      b[m][e] = m < a.n && c0 + e * step < j.cols ? read_f<T>(j.b, m * j.ldb + c0 + e * step, j.b_f32) : 0.f;
+      b[m][e] = live && c0 + e * step < j.cols ? read_f<T>(j.b, m * j.ldb + c0 + e * step, j.b_f32) : 0.f;
+  }
   __syncthreads();
   for (int q = warp * 16; q < min(warp * 16 + 16, rows); ++q) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -291,17 +295,18 @@ struct Outers {
   }
   // out [rows, cols] (+)= a^T b
   void outer(const void *pa, int64_t lda, int a_f32, int64_t rows, const void *pb, int64_t ldb, int b_f32, int cols, void *out,
-             int64_t ldo, int o_type, int accumulate) {
+             int64_t ldo, int o_type, int accumulate, const int64_t *target = nullptr, int64_t V = 0) {
     if (!out) return;
     const int es = elem(o_type);
     const bool wide = !accumulate && cols % 4 == 0 &&
                       ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * es)) & (uintptr_t)(4 * es - 1)) == 0;
     const unsigned ct = (unsigned)((cols + 127) / 128);
-    add(OutJob{pa, pb, lda, ldb, ldo, rows, out, cols, a_f32, b_f32, o_type == FB_F32, accumulate, 0, 0, wide, 0, ct},
+    add(OutJob{pa, pb, lda, ldb, ldo, rows, out, cols, a_f32, b_f32, o_type == FB_F32, accumulate, 0, 0, wide, 0, ct, target,
+               V},
         ct * (unsigned)((rows + 127) / 128));
   }
   void sum(const Columns &p, int64_t n, int cols, void *out, int64_t ldo, int o_type) {
-    add(OutJob{p.P, nullptr, 0, 0, ldo, n, out, cols, 1, 1, o_type == FB_F32, 0, 1, p.splits, 0, 0, 1},
+    add(OutJob{p.P, nullptr, 0, 0, ldo, n, out, cols, 1, 1, o_type == FB_F32, 0, 1, p.splits, 0, 0, 1, nullptr, 0},
         (unsigned)((n * cols + 255) / 256));
   }
   template <typename T> int go(cudaStream_t st) {
@@ -373,7 +378,8 @@ int few_rows_xent_bwd(Call &c, const fb_softmax_xent &a) {
   if (a.dh) FBH_TRY(columns(c, a.type, xl, a.V, &w, 1, n, a.V, a.D, &dh));
   if (c.dry) return FB_OK;
   Outers out(n);
-  out.outer(l, a.V, 1, a.V, a.h, a.ldh, f32, a.D, a.dw, a.lddw, a.grad_type, a.accumulate);
+  out.outer(l, a.V, 1, a.V, a.h, a.ldh, f32, a.D, a.dw, a.lddw, a.grad_type, a.accumulate,
+            a.target, a.V);
   if (a.dh) out.sum(dh, n, a.D, a.dh, a.lddh, a.type);
   return f32 ? out.go<float>(c.stream) : out.go<bf16>(c.stream);
 }

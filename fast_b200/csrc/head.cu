@@ -10,6 +10,8 @@ struct Job {
   int64_t lds, plane;
   void *dst;
   int ldd, cols, wide;                       // wide: 16-byte (8-byte) loads of the source's groups of 4
+  const int64_t *target;                     // Operand's
+  int64_t V;
   uint32_t groups, per_row;                  // groups of 4 columns, in all and a row
   unsigned first;                            // first CTA of the job
 };
@@ -33,11 +35,12 @@ template <bool PLANES> __global__ void __launch_bounds__(256) k_operands(const _
     const uint32_t r = i / j.per_row;
     const int c = (int)(i - r * j.per_row) * 4;
     uint16_t *d = static_cast<uint16_t *>(j.dst) + (int64_t)r * j.ldd + c;
+    const bool live = !j.target || (j.target[r] >= 0 && j.target[r] < j.V);
     if constexpr (PLANES) {
       const float *s = static_cast<const float *>(j.src) + r * j.lds + c;
       float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (j.wide) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(s);
-      else
+      if (j.wide && live) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(s);
+      else if (live)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (c + k < j.cols) v[k] = s[k];
@@ -45,8 +48,8 @@ template <bool PLANES> __global__ void __launch_bounds__(256) k_operands(const _
     } else {
       const uint16_t *s = static_cast<const uint16_t *>(j.src) + r * j.lds + c;
       ushort4 v = make_ushort4(0, 0, 0, 0);
-      if (j.wide) v = *reinterpret_cast<const ushort4 *>(s);
-      else {
+      if (j.wide && live) v = *reinterpret_cast<const ushort4 *>(s);
+      else if (live) {
         v.x = s[0];
         if (c + 1 < j.cols) v.y = s[1];
         if (c + 2 < j.cols) v.z = s[2];
@@ -69,7 +72,7 @@ int operands(Call &c, int type, const Operand *ops, int n) {
   for (int i = 0; i < n; ++i) {
     const Operand &o = ops[i];
     *o.out = Mat{o.src.p, o.src.ld};
-    if (!planes && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * 2)) & 15u) == 0) continue;
+    if (!planes && !o.target && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * 2)) & 15u) == 0) continue;
     // rows on 128-byte boundaries: a 128-byte box row that crosses one costs the copy engine two requests
     const int64_t ld = round_up(o.cols, 64), plane = o.rows * ld;
     void *p = c.take((size_t)(plane * (planes ? 6 : 2)));
@@ -81,7 +84,7 @@ int operands(Call &c, int type, const Operand *ops, int n) {
     if (groups > UINT32_MAX / 2) return fb::set_error(FB_ERR_UNSUPPORTED, "operand of more than 2^33 elements");
     const int es = elem(type);
     const bool wide = o.cols % 4 == 0 && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * es)) & (4 * es - 1)) == 0;
-    jobs.j[jobs.n++] = Job{o.src.p, o.src.ld, plane, p, (int)ld, o.cols, wide, (uint32_t)groups, per_row, ctas};
+    jobs.j[jobs.n++] = Job{o.src.p, o.src.ld, plane, p, (int)ld, o.cols, wide, o.target, o.V, (uint32_t)groups, per_row, ctas};
     ctas += (unsigned)((groups + 256 * kGroups - 1) / (256 * kGroups));
   }
   if (c.dry || jobs.n == 0) return FB_OK;

@@ -40,13 +40,17 @@ struct Mat {
 
 // The matrices of a call as the products read them: bf16 with a 16-byte
 // aligned base and pitch (copied into the workspace when they are not), fp32
-// split into planes; one launch for all of them.
+// split into planes; one launch for all of them.  Rows held out of a loss are
+// laid out as zeros: their gradient's zeros alone would not keep an infinity
+// or a NaN out of a sum over the rows.
 constexpr int kMaxOperands = 6;
 struct Operand {
   Mat src;
   int64_t rows;
   int cols;
   Mat *out;
+  const int64_t *target = nullptr;           // given: rows whose target is not one of V are laid out as zeros
+  int64_t V = 0;
 };
 int operands(Call &c, int type, const Operand *ops, int n);
 

@@ -306,7 +306,11 @@ int run(Call &c, const fb_softmax_xent &a, bool bwd) {
   if (few_rows_ok(a.type, bwd, a.n, a.D, a.D * a.V) && (!bwd || a.V <= kFewRowsTable))
     return bwd ? few_rows_xent_bwd(c, a) : forward_few(c, a);
   Mat h, w;
-  const Operand ops[2] = {{Mat{a.h, a.ldh}, a.n, a.D, &h}, {Mat{a.w, a.ldw}, a.V, a.D, &w}};
+  // dw sums over the rows, so rows held out are zeros to it (bf16 rows that could be read where they lie are copied for
+  // that: 4,000 x 100 against 16,700 nodes, training, 141 us before that copy and 139 with it; 8,192 x 1,024 against
+  // 50,000, 2.73 and 2.71 ms)
+  Operand ops[2] = {{Mat{a.h, a.ldh}, a.n, a.D, &h}, {Mat{a.w, a.ldw}, a.V, a.D, &w}};
+  if (bwd && a.dw) ops[0].target = a.target, ops[0].V = a.V;
   FBH_TRY(operands(c, a.type, ops, 2));
   return bwd ? backward(c, a, h, w) : forward(c, a, h, w);
 }

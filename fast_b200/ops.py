@@ -743,7 +743,8 @@ def softmax_xent_fwd(h, w, target):
     """Cross entropy of softmax(h w^T) for rows h [n, D] over every row of
     w [V, D] (both fp32 or both bf16), without keeping the logits: returns
     (loss, lse), fp32 [n].  A negative target holds its row out of the loss
-    (loss 0); one >= V gives a NaN loss."""
+    (loss 0, and no gradient whatever the row holds); one >= V gives a NaN loss
+    and no gradient."""
     return _head_call(head_ops.softmax_xent_fwd, 2,
                       lambda: (h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 2 * h.numel() * w.shape[0]), h, w,
                       target)

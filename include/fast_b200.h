@@ -640,8 +640,8 @@ int fb_gated_ffn_bwd(const fb_gated_ffn *args, void *ws, size_t ws_bytes, cudaSt
 /* Softmax cross entropy of rows h [n, D] over the V rows of a table w [V, D]
  * (logits h w^T, never kept), one type, fp32 accumulation:
  *   lse[i] = log sum_v exp(l_iv),  loss[i] = lse[i] - l_i,target[i]
- * A negative target holds its row out: loss 0 and no gradient.  A target >= V
- * gives a NaN loss and no gradient.  Backward, from lse and dloss [n] (fp32):
+ * A negative target holds its row out: loss 0 and no gradient, whatever the
+ * row holds.  A target >= V gives a NaN loss and no gradient.  Backward, from lse and dloss [n] (fp32):
  *   G_iv = dloss[i] (exp(l_iv - lse[i]) - [v == target[i]])
  *   dh = G w (rows' type),  dw = G^T h (grad_type; += when accumulate, fp32 only)
  * dh or dw may be NULL.  Deterministic.

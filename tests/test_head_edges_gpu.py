@@ -151,3 +151,40 @@ def test_fp32_products_of_infinities(cuda, value):
         assert bool((y[:, 4].double() == ref[:, 4]).all())
     other = [k for k in range(16) if k != 4]
     assert bool(torch.isfinite(y[:, other]).all())
+
+
+# ---- rows held out of the loss ---------------------------------------------------------------------------------------
+# few rows; tiles over aligned rows, read where they lie, and over copied ones; stored logits
+@pytest.mark.parametrize("n,d,v,pad", [(2, 64, 17000, 0), (8, 33, 900, 0), (40, 64, 900, 0), (300, 64, 700, 8),
+                                       (300, 33, 700, 1), (60, 600, 500, 0)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_softmax_xent_held_out_rows_reach_no_gradient(cuda, n, d, v, pad, dtype):
+    """Whatever a row without a target holds, the gradients are those of a call in which it holds zeros."""
+    from fast_b200 import ops
+    g = _gen(cuda, n, d, v)
+    h, w = _mat(cuda, g, n, d, dtype, 1.0, pad), _mat(cuda, g, v, d, dtype, d ** -0.5, pad)
+    t = torch.randint(0, v, (n,), device=cuda, generator=g)
+    dl = torch.rand(n, device=cuda, generator=g) + 0.5
+    out = [1] if n < 5 else [1, 3, n - 1]
+    t[out] = -1
+    if n >= 5:
+        t[3] = v + 5                                            # no target in the table: no gradient either
+    clean = h.clone()
+    clean[out] = 0
+    _, lse = ops.softmax_xent_fwd(clean, w, t)
+    want = ops.softmax_xent_bwd(clean, w, t, lse, dl)
+    h[1] = math.nan
+    if n >= 5:
+        h[3, ::2], h[n - 1, -1] = math.inf, -math.inf
+    kept = h.clone()
+    loss, lse = ops.softmax_xent_fwd(h, w, t)
+    assert bool((loss[t < 0] == 0).all()) and bool(loss[(t >= 0) & (t < v)].isfinite().all())
+    dl[out] = math.nan                                          # nor does their gradient of the loss
+    dh, dw = ops.softmax_xent_bwd(h, w, t, lse, dl)
+    assert bool(dh.isfinite().all()) and bool(dw.isfinite().all())
+    assert torch.equal(dh, want[0]) and torch.equal(dw, want[1])
+    buf = torch.zeros(v, d, device=cuda)
+    ops.softmax_xent_bwd(h, w, t, lse, dl, dw=buf)
+    assert bool(buf.isfinite().all())
+    same = torch.equal(h.view(torch.int16 if dtype == BF else torch.int32), kept.view(torch.int16 if dtype == BF else torch.int32))
+    assert same                                                 # the caller's rows stay as they are
