@@ -188,3 +188,30 @@ def test_softmax_xent_held_out_rows_reach_no_gradient(cuda, n, d, v, pad, dtype)
     assert bool(buf.isfinite().all())
     same = torch.equal(h.view(torch.int16 if dtype == BF else torch.int32), kept.view(torch.int16 if dtype == BF else torch.int32))
     assert same                                                 # the caller's rows stay as they are
+
+
+# ---- the tail of GELU ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 2, 8, 89])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gelu_of_negative_values_keeps_its_relative_accuracy(cuda, rows, dtype):
+    """h = gelu(g) * 1 and dg = gelu'(g) for g in [-8, -3], where erf is nearly -1: an error that is small beside 1 is
+    not small beside the result.  fp32: the normal distribution function to 5 ulp, the exponential to 2, both times a
+    few products, whose sum in gelu' cancels by a factor of at most 1.3: below 2^-19.  bf16: 2^-8 for the rounding and
+    2^-10 for what the fast exponential and the tail's polynomial leave."""
+    from fast_b200 import ops
+    g = torch.linspace(-8, -3, 89, device=cuda).bfloat16().to(dtype)[:, None]
+    wg, wu, wd = (torch.zeros(16, 16, device=cuda, dtype=dtype) for _ in range(3))
+    wg[0, 0], wu[0, 1], wd[0, 0] = 1, 1, 1
+    x = torch.zeros(89, 16, device=cuda, dtype=dtype)
+    x[:, :1], x[:, 1] = g, 1
+    dy = torch.zeros_like(x)
+    dy[:, 0] = 1
+    y = torch.cat([ops.gated_ffn_fwd(p, wg, wu, wd, act="gelu") for p in x.split(rows)])[:, :1].double()
+    dx = torch.cat([ops.gated_ffn_bwd(q, p, wg, wu, wd, act="gelu")[0] for p, q in zip(x.split(rows), dy.split(rows))])
+    G = g.double()
+    phi = 0.5 * torch.special.erfc(-G * 0.5 ** 0.5)
+    tol = 2.0 ** -19 if dtype == F32 else 2.0 ** -8 + 2.0 ** -10
+    want = G * phi
+    assert float(((y - want) / want).abs().max()) <= tol
+    want = phi + G * torch.exp(-G * G / 2) / math.sqrt(2 * math.pi)
+    assert float(((dx[:, :1].double() - want) / want).abs().max()) <= tol
