@@ -21,6 +21,7 @@ offset, edge, head), not from torch's generator.
 import torch
 
 from .ext import fastAgg
+from .first_order import first_order
 
 
 class FusedSoftmaxAggTGAT(torch.autograd.Function):
@@ -39,6 +40,7 @@ class FusedSoftmaxAggTGAT(torch.autograd.Function):
         return agg
 
     @staticmethod
+    @first_order
     def backward(ctx, d_agg):
         q, k, v, rptr, att = ctx.saved_tensors
         dq, dk, dv = fastAgg.backward_fused_softmax_agg(q, k, v, rptr, att, d_agg.contiguous(), *ctx.args)

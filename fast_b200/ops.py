@@ -13,6 +13,7 @@ import torch
 
 from .capi import ACTS, call, ptr, stream_ptr, lib
 from .ext import head_ops
+from .first_order import first_order
 
 
 class KernelTimer:
@@ -813,6 +814,7 @@ class AttentionCore(torch.autograd.Function):
         return agg
 
     @staticmethod
+    @first_order
     def backward(ctx, dagg):
         A, KV, Qin, Q, att, W_q, W_kv, wv, b_t, offset_dev = ctx.saved_tensors
         dn, de, dtime, D, heads, slope, drop_p, seed, has_h = ctx.cfg

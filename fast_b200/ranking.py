@@ -20,6 +20,7 @@ import math
 import torch
 
 from . import ops
+from .first_order import first_order
 
 
 def _rows(t):
@@ -48,6 +49,7 @@ class LayerNormFunction(torch.autograd.Function):
         return y, s
 
     @staticmethod
+    @first_order
     def backward(ctx, dy, ds=None):
         s, gamma, mean, rstd = ctx.saved_tensors
         has_res, has_beta = ctx.flags
@@ -68,6 +70,7 @@ class GatedFfnFunction(torch.autograd.Function):
         return ops.gated_ffn_fwd(x, w_gate, w_up, w_down, act)
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         x, w_gate, w_up, w_down = ctx.saved_tensors
         return (*ops.gated_ffn_bwd(_rows(dy), x, w_gate, w_up, w_down, ctx.act), None)
@@ -84,6 +87,7 @@ class SoftmaxXentFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @first_order
     def backward(ctx, dloss):
         h, w, target, lse = ctx.saved_tensors
         dh, dw = ops.softmax_xent_bwd(h, w, target, lse, dloss.contiguous())
