@@ -731,13 +731,20 @@ def gated_ffn_fwd(x, w_gate, w_up, w_down, act="silu"):
                       w_gate, w_up, w_down, _act(act))
 
 
-def gated_ffn_bwd(dy, x, w_gate, w_up, w_down, act="silu", grads=None):
+def _grad_f32(name, grad_dtype, rows):
+    if grad_dtype not in (None, rows.dtype, torch.float32):
+        raise ValueError("%s: grad_dtype must be the weights' type or torch.float32" % name)
+    return grad_dtype == torch.float32
+
+
+def gated_ffn_bwd(dy, x, w_gate, w_up, w_down, act="silu", grads=None, grad_dtype=None):
     """Gradients of gated_ffn_fwd: (dx, dw_gate, dw_up, dw_down).  The weight
-    gradients have the weights' type; `grads`, three fp32 buffers, are
-    accumulated into instead (a flat gradient buffer's views)."""
+    gradients are sums in fp32, rounded to the weights' type or, with
+    grad_dtype=torch.float32, returned as they are; `grads`, three fp32
+    buffers, are accumulated into instead (a flat gradient buffer's views)."""
     return _head_call(head_ops.gated_ffn_bwd, 2,
                       lambda: (x.element_size() * (3 * x.numel() + 6 * w_gate.numel()), 16 * x.numel() * w_gate.shape[0]), dy,
-                      x, w_gate, w_up, w_down, _act(act), grads)
+                      x, w_gate, w_up, w_down, _act(act), grads, _grad_f32("gated_ffn_bwd", grad_dtype, x))
 
 
 def softmax_xent_fwd(h, w, target):
@@ -751,12 +758,13 @@ def softmax_xent_fwd(h, w, target):
                       target)
 
 
-def softmax_xent_bwd(h, w, target, lse, dloss, dw=None):
+def softmax_xent_bwd(h, w, target, lse, dloss, dw=None, grad_dtype=None):
     """Gradients of softmax_xent_fwd for dloss [n] (fp32): (dh, dw), of the
-    inputs' type; an fp32 buffer given as dw is accumulated into instead."""
+    inputs' type (dw, a sum in fp32, as it is with grad_dtype=torch.float32);
+    an fp32 buffer given as dw is accumulated into instead."""
     return _head_call(head_ops.softmax_xent_bwd, 2,
                       lambda: (2 * h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 6 * h.numel() * w.shape[0]),
-                      h, w, target, lse, dloss, dw)
+                      h, w, target, lse, dloss, dw, _grad_f32("softmax_xent_bwd", grad_dtype, h))
 
 
 class AttentionCore(torch.autograd.Function):

@@ -9,8 +9,11 @@ the whole node table, and answers it for single queries:
     loss_i = log sum_v exp(h_i . w_v) - h_i . w_target(i)
 
 The logits [rows, nodes] are never kept.  The modules carry fp32 parameters
-(as the framework's models do); `dtype` is what the kernels compute in:
-torch.float32, or torch.bfloat16 with fp32 accumulation and statistics.
+(as the framework's models do) and give them fp32 gradients; `dtype` is what
+the kernels compute in: torch.float32, or torch.bfloat16 with fp32 accumulation
+and statistics.  bf16 from fp32 parameters converts them at every call; a head
+that only answers queries saves that as a bf16 module throughout
+(NodeRankingHead(..., dtype=torch.bfloat16).to(torch.bfloat16)).
 
     python -m fast_b200.ranking          # trains it on a synthetic temporal graph (one GPU)
 """
@@ -28,6 +31,11 @@ def _rows(t):
     if t.dim() == 2 and t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]):
         return t
     return t.contiguous()
+
+
+def _f32_or_none(w):
+    """The type a weight's gradient is asked for: fp32 for fp32, else the rows'."""
+    return torch.float32 if w.dtype == torch.float32 else None
 
 
 class LayerNormFunction(torch.autograd.Function):
@@ -60,28 +68,31 @@ class LayerNormFunction(torch.autograd.Function):
 
 
 class GatedFfnFunction(torch.autograd.Function):
-    """y = (act(x Wg^T) * (x Wu^T)) Wd^T; only x is kept for the backward."""
+    """y = (act(x Wg^T) * (x Wu^T)) Wd^T; x and the weights in x's type are kept
+    for the backward.  Weights of fp32 receive fp32 gradients whatever x's type."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act):
-        x = _rows(x)
-        ctx.save_for_backward(x, w_gate, w_up, w_down)
-        ctx.act = act
-        return ops.gated_ffn_fwd(x, w_gate, w_up, w_down, act)
+        x, *w = (_rows(t.to(x.dtype)) for t in (x, w_gate, w_up, w_down))
+        ctx.save_for_backward(x, *w)
+        ctx.act, ctx.grad_dtype = act, _f32_or_none(w_gate)
+        return ops.gated_ffn_fwd(x, *w, act)
 
     @staticmethod
     @first_order
     def backward(ctx, dy):
-        x, w_gate, w_up, w_down = ctx.saved_tensors
-        return (*ops.gated_ffn_bwd(_rows(dy), x, w_gate, w_up, w_down, ctx.act), None)
+        x, *w = ctx.saved_tensors
+        return (*ops.gated_ffn_bwd(_rows(dy), x, *w, ctx.act, grad_dtype=ctx.grad_dtype), None)
 
 
 class SoftmaxXentFunction(torch.autograd.Function):
-    """Per-row cross entropy (fp32 [n]) of softmax(h w^T)."""
+    """Per-row cross entropy (fp32 [n]) of softmax(h w^T), w in h's type.  A
+    table of fp32 receives an fp32 gradient."""
 
     @staticmethod
     def forward(ctx, h, w, target):
-        h, w = _rows(h), _rows(w)
+        ctx.grad_dtype = _f32_or_none(w)
+        h, w = _rows(h), _rows(w.to(h.dtype))
         loss, lse = ops.softmax_xent_fwd(h, w, target)
         ctx.save_for_backward(h, w, target, lse)
         return loss
@@ -90,7 +101,7 @@ class SoftmaxXentFunction(torch.autograd.Function):
     @first_order
     def backward(ctx, dloss):
         h, w, target, lse = ctx.saved_tensors
-        dh, dw = ops.softmax_xent_bwd(h, w, target, lse, dloss.contiguous())
+        dh, dw = ops.softmax_xent_bwd(h, w, target, lse, dloss.contiguous(), grad_dtype=ctx.grad_dtype)
         return dh, dw, None
 
 
@@ -107,8 +118,7 @@ class GatedFeedForward(torch.nn.Module):
         self.w_down = torch.nn.Parameter(torch.randn(dim, hidden) * hidden ** -0.5)
 
     def forward(self, x):
-        c = [t.to(self.dtype) for t in (x, self.w_gate, self.w_up, self.w_down)]
-        return GatedFfnFunction.apply(*c, self.act)
+        return GatedFfnFunction.apply(x.to(self.dtype), self.w_gate, self.w_up, self.w_down, self.act)
 
 
 class NodeRankingHead(torch.nn.Module):
@@ -137,7 +147,7 @@ class NodeRankingHead(torch.nn.Module):
         return h
 
     def forward(self, x, target, res=None):
-        rows = SoftmaxXentFunction.apply(self.embed(x, res), self.node_table.to(self.dtype), target)
+        rows = SoftmaxXentFunction.apply(self.embed(x, res), self.node_table, target)
         return rows.sum() / (target >= 0).sum().clamp(min=1), rows
 
 

@@ -128,9 +128,9 @@ py::tuple layer_norm_bwd(const Tensor &dy, const Tensor &x, const Tensor &gamma,
   return py::make_tuple(dx, dg, db);
 }
 
-// A weight gradient: fresh, of the weights' type, or the fp32 buffer given.
-Tensor grad(const OptTensor &given, const char *name, const Tensor &like, int64_t r, int64_t c) {
-  if (!given) return empty({r, c}, like, like.scalar_type());
+// A weight gradient: fresh, of the weights' type or (f32) fp32, or the fp32 buffer given.
+Tensor grad(const OptTensor &given, const char *name, const Tensor &like, int64_t r, int64_t c, bool f32) {
+  if (!given) return empty({r, c}, like, f32 ? at::kFloat : like.scalar_type());
   rows(*given, name, at::kFloat, like, r, c);
   return *given;
 }
@@ -168,17 +168,18 @@ Tensor gated_ffn_fwd(const Tensor &x, const Tensor &wg, const Tensor &wu, const 
 }
 
 py::tuple gated_ffn_bwd(const Tensor &dy, const Tensor &x, const Tensor &wg, const Tensor &wu, const Tensor &wd, int act,
-                        const std::optional<std::vector<Tensor>> &grads) {
+                        const std::optional<std::vector<Tensor>> &grads, bool f32) {
   fb_gated_ffn a = ffn_args(x, wg, wu, wd, act);
   rows(dy, "gated_ffn_bwd dy", x.scalar_type(), x, a.n, a.D);
   if (grads && grads->size() != 3) refuse("gated_ffn_bwd: 3 gradient buffers expected");
   const c10::cuda::CUDAGuard guard(x.device());
   const auto given = [&](int i) { return grads ? OptTensor((*grads)[i]) : std::nullopt; };
-  const Tensor dg = grad(given(0), "gated_ffn_bwd gradient buffer", x, a.F, a.D);
-  const Tensor du = grad(given(1), "gated_ffn_bwd gradient buffer", x, a.F, a.D);
-  const Tensor dd = grad(given(2), "gated_ffn_bwd gradient buffer", x, a.D, a.F);
+  const Tensor dg = grad(given(0), "gated_ffn_bwd gradient buffer", x, a.F, a.D, f32);
+  const Tensor du = grad(given(1), "gated_ffn_bwd gradient buffer", x, a.F, a.D, f32);
+  const Tensor dd = grad(given(2), "gated_ffn_bwd gradient buffer", x, a.D, a.F, f32);
   const Tensor dx = empty({a.n, a.D}, x, x.scalar_type());
-  if (grads) a.grad_type = FB_F32, a.accumulate = 1;
+  if (grads || f32) a.grad_type = FB_F32;
+  a.accumulate = grads.has_value();
   a.dy = ptr(dy), a.lddy = ld(dy);
   a.dx = ptr(dx), a.lddx = a.D;
   a.dw_gate = ptr(dg), a.ldd_gate = ld(dg);
@@ -217,14 +218,15 @@ py::tuple softmax_xent_fwd(const Tensor &h, const Tensor &w, const Tensor &targe
 }
 
 py::tuple softmax_xent_bwd(const Tensor &h, const Tensor &w, const Tensor &target, const Tensor &lse,
-                           const Tensor &dloss, const OptTensor &dw_in) {
+                           const Tensor &dloss, const OptTensor &dw_in, bool f32) {
   fb_softmax_xent a = xent_args(h, w, target);
   vec(lse, "softmax_xent_bwd lse", at::kFloat, h, a.n);
   vec(dloss, "softmax_xent_bwd dloss", at::kFloat, h, a.n);
   const c10::cuda::CUDAGuard guard(h.device());
   const Tensor dh = empty({a.n, a.D}, h, h.scalar_type());
-  const Tensor dw = grad(dw_in, "softmax_xent_bwd dw", h, a.V, a.D);
-  if (dw_in) a.grad_type = FB_F32, a.accumulate = 1;
+  const Tensor dw = grad(dw_in, "softmax_xent_bwd dw", h, a.V, a.D, f32);
+  if (dw_in || f32) a.grad_type = FB_F32;
+  a.accumulate = dw_in.has_value();
   a.lse = (float *)ptr(lse), a.dloss = (const float *)ptr(dloss);
   a.dh = ptr(dh), a.lddh = a.D;
   a.dw = ptr(dw), a.lddw = ld(dw);

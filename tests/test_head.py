@@ -96,3 +96,13 @@ def test_module_refuses_an_unknown_activation():
     assert {n: tuple(p.shape) for n, p in head.named_parameters()} == {
         "node_table": (20, 8), "norm1.weight": (8,), "norm1.bias": (8,), "norm2.weight": (8,), "norm2.bias": (8,),
         "ffn.w_gate": (12, 8), "ffn.w_up": (12, 8), "ffn.w_down": (8, 12)}
+
+
+def test_backward_wrappers_refuse_a_gradient_type():
+    from fast_b200 import ops
+    x, v, t = torch.zeros(4, 8), torch.zeros(4), torch.zeros(4, dtype=torch.int64)
+    for bad in (torch.float16, torch.bfloat16, torch.float64):
+        with pytest.raises(ValueError, match="grad_dtype"):
+            ops.gated_ffn_bwd(x, x, x, x, x, grad_dtype=bad)
+        with pytest.raises(ValueError, match="grad_dtype"):
+            ops.softmax_xent_bwd(x, x, t, v, v, grad_dtype=bad)

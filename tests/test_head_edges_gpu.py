@@ -215,3 +215,32 @@ def test_gelu_of_negative_values_keeps_its_relative_accuracy(cuda, rows, dtype):
     assert float(((y - want) / want).abs().max()) <= tol
     want = phi + G * torch.exp(-G * G / 2) / math.sqrt(2 * math.pi)
     assert float(((dx[:, :1].double() - want) / want).abs().max()) <= tol
+
+
+# ---- the module's gradients ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [1, 150])
+def test_bf16_head_gives_its_fp32_parameters_unrounded_gradients(cuda, n):
+    """Weight gradients are fp32 sums; fp32 parameters receive them as they are, not rounded to bf16 on the way."""
+    from fast_b200 import ops
+    from fast_b200.ranking import GatedFeedForward, NodeRankingHead, SoftmaxXentFunction
+    torch.manual_seed(2)
+    ffn = GatedFeedForward(64, 136, dtype=BF).to(cuda)
+    x, dy = torch.randn(n, 64, device=cuda).bfloat16(), torch.randn(n, 64, device=cuda).bfloat16()
+    ffn(x).backward(dy)
+    bufs = [torch.zeros(p.shape, device=cuda) for p in (ffn.w_gate, ffn.w_up, ffn.w_down)]
+    ops.gated_ffn_bwd(dy, x, *(p.detach().bfloat16() for p in (ffn.w_gate, ffn.w_up, ffn.w_down)), grads=bufs)
+    for p, b in zip((ffn.w_gate, ffn.w_up, ffn.w_down), bufs):
+        assert p.grad.dtype == F32 and torch.equal(p.grad, b)
+    table = torch.randn(300, 64, device=cuda, requires_grad=True)
+    t = torch.randint(0, 300, (n,), device=cuda)
+    SoftmaxXentFunction.apply(x, table, t).sum().backward()
+    buf, w = torch.zeros(300, 64, device=cuda), table.detach().bfloat16()
+    _, lse = ops.softmax_xent_fwd(x, w, t)
+    ops.softmax_xent_bwd(x, w, t, lse, torch.ones(n, device=cuda), dw=buf)
+    assert table.grad.dtype == F32 and torch.equal(table.grad, buf)
+    # a module that is bf16 throughout: no fp32 parameters, no conversions of them, gradients of their type
+    head = NodeRankingHead(64, 300, hidden=136, dtype=BF).to(cuda).to(BF)
+    loss, _ = head(x, t)
+    loss.backward()
+    assert all(p.grad.dtype == BF and bool(p.grad.isfinite().all()) for p in head.parameters())
+    assert torch.isfinite(loss)
