@@ -222,7 +222,7 @@ extern "C" size_t fb_gated_ffn_ws_bytes(const fb_gated_ffn *a, int backward) {
 extern "C" int fb_gated_ffn_fwd(const fb_gated_ffn *a, void *ws, size_t ws_bytes, cudaStream_t stream) {
   FBH_TRY(check(a, false));
   if (a->n == 0) return FB_OK;
-  if (!ws) return fb::set_error(FB_ERR_ARG, "gated_ffn_fwd: no workspace");
+  FBH_TRY(check_ws(ws, "gated_ffn_fwd"));
   Call c(ws, ws_bytes, stream);
   return run(c, *a, false);
 }
@@ -230,7 +230,7 @@ extern "C" int fb_gated_ffn_fwd(const fb_gated_ffn *a, void *ws, size_t ws_bytes
 extern "C" int fb_gated_ffn_bwd(const fb_gated_ffn *a, void *ws, size_t ws_bytes, cudaStream_t stream) {
   FBH_TRY(check(a, true));
   if (a->n == 0) return empty_grads(*a, stream);
-  if (!ws) return fb::set_error(FB_ERR_ARG, "gated_ffn_bwd: no workspace");
+  FBH_TRY(check_ws(ws, "gated_ffn_bwd"));
   Call c(ws, ws_bytes, stream);
   return run(c, *a, true);
 }

@@ -29,6 +29,14 @@ struct Call {
   }
 };
 
+// Pieces of a workspace are accessed 16 bytes at a time and mapped for bulk copies.
+inline int check_ws(const void *ws, const char *name) {
+  if (!ws) return fb::set_error(FB_ERR_ARG, std::string(name) + ": no workspace");
+  if (reinterpret_cast<uintptr_t>(ws) & 15u)
+    return fb::set_error(FB_ERR_ARG, std::string(name) + ": the workspace must be 16-byte aligned");
+  return FB_OK;
+}
+
 // A row-major matrix [rows, cols] of the operator's type; as an operand of the
 // products a bf16 matrix, or (plane > 0) the three bf16 planes of an fp32 one,
 // `plane` elements apart.

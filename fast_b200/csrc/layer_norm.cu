@@ -764,6 +764,8 @@ extern "C" int fb_layer_norm_bwd(int type, const void *dy, int64_t lddy, const v
   const bool weights = dgamma || dbeta;
   if (weights && n > 0 && (!ws || ws_bytes < fb_layer_norm_bwd_ws_bytes(n, D)))
     return fb::set_error(FB_ERR_ARG, "layer_norm_bwd: workspace too small");
+  if (weights && n > 0 && (reinterpret_cast<uintptr_t>(ws) & 15u))
+    return fb::set_error(FB_ERR_ARG, "layer_norm_bwd: the workspace must be 16-byte aligned");
   if (n == 0) {                              // an empty sum is zero
     const size_t pb = (size_t)D * elem(param_type);
     if (dgamma && !accumulate) FB_TRY_CUDA(cudaMemsetAsync(dgamma, 0, pb, stream));

@@ -326,7 +326,7 @@ extern "C" size_t fb_softmax_xent_ws_bytes(const fb_softmax_xent *a, int backwar
 extern "C" int fb_softmax_xent_fwd(const fb_softmax_xent *a, void *ws, size_t ws_bytes, cudaStream_t stream) {
   FBH_TRY(check(a, false));
   if (a->n == 0) return FB_OK;
-  if (!ws) return fb::set_error(FB_ERR_ARG, "softmax_xent_fwd: no workspace");
+  FBH_TRY(check_ws(ws, "softmax_xent_fwd"));
   Call c(ws, ws_bytes, stream);
   return run(c, *a, false);
 }
@@ -339,7 +339,7 @@ extern "C" int fb_softmax_xent_bwd(const fb_softmax_xent *a, void *ws, size_t ws
                                     stream));
     return FB_OK;
   }
-  if (!ws) return fb::set_error(FB_ERR_ARG, "softmax_xent_bwd: no workspace");
+  FBH_TRY(check_ws(ws, "softmax_xent_bwd"));
   Call c(ws, ws_bytes, stream);
   return run(c, *a, true);
 }

@@ -605,7 +605,7 @@ int fb_layer_norm_fwd(int type, const void *x, int64_t ldx, const void *res, int
  * dx (+ ds, the gradient that reaches the sum on its own; may be NULL), the
  * gradient of x and of res alike; dgamma = sum dy xhat, dbeta = sum dy (each
  * may be NULL; += when accumulate, fp32 only).  Deterministic.
- * ws: fb_layer_norm_bwd_ws_bytes(n, D) bytes. */
+ * ws: fb_layer_norm_bwd_ws_bytes(n, D) bytes, 16-byte aligned. */
 size_t fb_layer_norm_bwd_ws_bytes(int64_t n, int D);
 int fb_layer_norm_bwd(int type, const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *gamma,
                       int param_type, const float *mean, const float *rstd, const void *ds, int64_t ldds, void *dx,
@@ -617,7 +617,7 @@ int fb_layer_norm_bwd(int type, const void *dy, int64_t lddy, const void *x, int
  * recomputes what the activation saw) and writes dx (rows' type) and the weight
  * gradients (grad_type: fp32 or the rows' type; += when accumulate, fp32 only);
  * any of the four may be NULL.  GELU is the erf form.  Deterministic.
- * ws: fb_gated_ffn_ws_bytes(args, backward) bytes. */
+ * ws: fb_gated_ffn_ws_bytes(args, backward) bytes, 16-byte aligned. */
 enum { FB_ACT_SILU = 0, FB_ACT_GELU = 1, FB_ACT_RELU = 2 };
 typedef struct fb_gated_ffn {
   int type, act, grad_type, accumulate;
@@ -645,7 +645,7 @@ int fb_gated_ffn_bwd(const fb_gated_ffn *args, void *ws, size_t ws_bytes, cudaSt
  *   G_iv = dloss[i] (exp(l_iv - lse[i]) - [v == target[i]])
  *   dh = G w (rows' type),  dw = G^T h (grad_type; += when accumulate, fp32 only)
  * dh or dw may be NULL.  Deterministic.
- * ws: fb_softmax_xent_ws_bytes(args, backward) bytes. */
+ * ws: fb_softmax_xent_ws_bytes(args, backward) bytes, 16-byte aligned. */
 typedef struct fb_softmax_xent {
   int type, grad_type, accumulate, D;
   int64_t n, V;

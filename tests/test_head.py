@@ -106,3 +106,18 @@ def test_backward_wrappers_refuse_a_gradient_type():
             ops.gated_ffn_bwd(x, x, x, x, x, grad_dtype=bad)
         with pytest.raises(ValueError, match="grad_dtype"):
             ops.softmax_xent_bwd(x, x, t, v, v, grad_dtype=bad)
+
+
+def test_entries_refuse_a_workspace_that_is_not_aligned():
+    """The workspace's pieces are accessed 16 bytes at a time and mapped for bulk copies: refused before any launch."""
+    from fast_b200.capi import GatedFfn, SoftmaxXent, lib
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    f = GatedFfn(0, 0, 0, 0, 2, 8, 16, p, 8, p, 8, p, 8, p, 16, p, 8, p, 8, p, 8, p, 8, p, 8, p, 16)
+    x = SoftmaxXent(1, 1, 0, 8, 2, 30, p, 8, p, 8, p, p, p, p, p, 8, p, 8)
+    for off in (1, 4, 8):
+        assert lib.fb_gated_ffn_fwd(f, p + off, 1 << 40, None) == 1
+        assert lib.fb_gated_ffn_bwd(f, p + off, 1 << 40, None) == 1
+        assert lib.fb_softmax_xent_fwd(x, p + off, 1 << 40, None) == 1
+        assert lib.fb_softmax_xent_bwd(x, p + off, 1 << 40, None) == 1
+        assert lib.fb_layer_norm_bwd(0, p, 8, p, 8, p, 0, p, p, None, 0, p, 8, p, p, 0, 2, 8, p + off, 1 << 20, None) == 1
