@@ -37,6 +37,7 @@ _SZ = ctypes.c_size_t
 _SIGS = {
     "fb_last_error": (ctypes.c_char_p, []),
     "fb_version": (ctypes.c_char_p, []),
+    "fb_launches": (ctypes.c_int64, []),
     "fb_sampler_create": (_I, [_P, _P, _P, _P, _I64, _I64, _I, _I, _P, _I, _I, _I, _F, _U64, _P]),
     "fb_sampler_destroy": (_I, [_P]),
     "fb_sampler_reset": (_I, [_P, _P]),

@@ -15,7 +15,14 @@ int cuda_error(cudaError_t e, const char *where) {
   g_last_error = std::string(where) + ": " + cudaGetErrorString(e);
   return FB_ERR_CUDA;
 }
+
+int64_t &launches() {
+  static thread_local int64_t n = 0;
+  return n;
+}
 }  // namespace fb
+
+extern "C" int64_t fb_launches(void) { return fb::launches(); }
 
 extern "C" const char *fb_last_error(void) { return fb::g_last_error.c_str(); }
 

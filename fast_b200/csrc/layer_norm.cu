@@ -694,6 +694,7 @@ cudaError_t launch_cluster(K kernel, unsigned grid, unsigned block, size_t smem,
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = fb::pdl_enabled() ? 2 : 1;
+  ++fb::launches();
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 

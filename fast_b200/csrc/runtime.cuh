@@ -27,6 +27,9 @@ bool tc_problem_ok(const fb_gemm_problem &p);
 int64_t tc_ws_floats(const fb_gemm_problem &p);   // TN partial sums, floats
 int tc_group(const fb_gemm_problem *const *probs, float *const *ws, int n, cudaStream_t stream);
 
+// Kernels the calling thread has launched by launch() (and launch_cluster of layer_norm.cu).
+int64_t &launches();
+
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                    Args &&...args) {
@@ -40,6 +43,7 @@ cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  ++launches();
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 }  // namespace fb

@@ -51,6 +51,7 @@ class KernelTimer:
 TIMER = None            # set to a KernelTimer to time every kernel wrapper
 USE_TC = False          # route eligible gemm_nt calls to the tcgen05 kernel
 LAUNCHES = [0]          # kernels launched through these wrappers
+head_ops.count_into(LAUNCHES)
 # FB_NVTX=1: each wrapper's launches inside an NVTX range named like its timer
 # entry (eager steps), so a profiler can select one group by name
 NVTX = os.environ.get("FB_NVTX", "0") == "1"
@@ -683,15 +684,16 @@ def attn_bwd(q, k, v, rptr, att, dagg, heads, slope, drop_p=0.0, seed=0, offset=
 # The calls go through the head_ops module (argument checks, outputs and
 # workspaces in C++): operands of the wrong type, shape, layout or device raise
 # ValueError.
-def _head_call(fn, kernels, work, *args):
-    """Calls a head_ops function; work() gives its algorithmic bytes and flops
-    and is asked for only when a timer runs (a small call is bound by the host)."""
+def _head_call(fn, work, *args):
+    """Calls a head_ops function, which counts its launches itself; work() gives
+    its algorithmic bytes and flops and is asked for only when a timer runs (a
+    small call is bound by the host)."""
     if TIMER is None and not NVTX:
-        LAUNCHES[0] += kernels
         return fn(*args)
-    out = []
-    _launch(fn.__name__, *work(), kernels, lambda: out.append(fn(*args)))
-    return out[-1]
+    before, runs = LAUNCHES[0], []
+    _launch(fn.__name__, *work(), 0, lambda: runs.append(fn(*args)))
+    LAUNCHES[0] = before + (LAUNCHES[0] - before) // len(runs)    # a timer may call it more than once
+    return runs[-1]
 
 
 def layer_norm_fwd(x, gamma, beta=None, eps=1e-5, res=None):
@@ -699,7 +701,7 @@ def layer_norm_fwd(x, gamma, beta=None, eps=1e-5, res=None):
     in fp32.  Returns (y, mean, rstd); with a residual `res` it normalises
     s = x + res, kept in the rows' type, and returns (y, s, mean, rstd).
     gamma and beta are fp32 or of the rows' type."""
-    return _head_call(head_ops.layer_norm_fwd, 1,
+    return _head_call(head_ops.layer_norm_fwd,
                       lambda: (x.element_size() * x.numel() * (2 if res is None else 4), 8 * x.numel()), x, gamma, beta, eps,
                       res)
 
@@ -709,7 +711,7 @@ def layer_norm_bwd(dy, x, gamma, mean, rstd, ds=None, dgamma=None, dbeta=None):
     when there was a residual): returns (dx, dgamma, dbeta).  dx, the gradient
     of x and of res alike, includes ds, the gradient that reaches s on its own.
     dgamma / dbeta have gamma's type; fp32 vectors given are accumulated into."""
-    return _head_call(head_ops.layer_norm_bwd, 2,
+    return _head_call(head_ops.layer_norm_bwd,
                       lambda: (x.element_size() * x.numel() * (3 if ds is None else 4), 10 * x.numel()), dy, x, gamma, mean,
                       rstd, ds, dgamma, dbeta)
 
@@ -726,7 +728,7 @@ def gated_ffn_fwd(x, w_gate, w_up, w_down, act="silu"):
     weights w_gate, w_up [F, D], w_down [D, F], all fp32 or all bf16 (any row
     pitch).  act: "silu", "gelu" (erf form) or "relu".  Products accumulate
     in fp32; the backward needs nothing but the inputs."""
-    return _head_call(head_ops.gated_ffn_fwd, 2,
+    return _head_call(head_ops.gated_ffn_fwd,
                       lambda: (x.element_size() * (2 * x.numel() + 3 * w_gate.numel()), 6 * x.numel() * w_gate.shape[0]), x,
                       w_gate, w_up, w_down, _act(act))
 
@@ -742,7 +744,7 @@ def gated_ffn_bwd(dy, x, w_gate, w_up, w_down, act="silu", grads=None, grad_dtyp
     gradients are sums in fp32, rounded to the weights' type or, with
     grad_dtype=torch.float32, returned as they are; `grads`, three fp32
     buffers, are accumulated into instead (a flat gradient buffer's views)."""
-    return _head_call(head_ops.gated_ffn_bwd, 2,
+    return _head_call(head_ops.gated_ffn_bwd,
                       lambda: (x.element_size() * (3 * x.numel() + 6 * w_gate.numel()), 16 * x.numel() * w_gate.shape[0]), dy,
                       x, w_gate, w_up, w_down, _act(act), grads, _grad_f32("gated_ffn_bwd", grad_dtype, x))
 
@@ -753,7 +755,7 @@ def softmax_xent_fwd(h, w, target):
     (loss, lse), fp32 [n].  A negative target holds its row out of the loss
     (loss 0, and no gradient whatever the row holds); one >= V gives a NaN loss
     and no gradient."""
-    return _head_call(head_ops.softmax_xent_fwd, 2,
+    return _head_call(head_ops.softmax_xent_fwd,
                       lambda: (h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 2 * h.numel() * w.shape[0]), h, w,
                       target)
 
@@ -762,7 +764,7 @@ def softmax_xent_bwd(h, w, target, lse, dloss, dw=None, grad_dtype=None):
     """Gradients of softmax_xent_fwd for dloss [n] (fp32): (dh, dw), of the
     inputs' type (dw, a sum in fp32, as it is with grad_dtype=torch.float32);
     an fp32 buffer given as dw is accumulated into instead."""
-    return _head_call(head_ops.softmax_xent_bwd, 2,
+    return _head_call(head_ops.softmax_xent_bwd,
                       lambda: (2 * h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 6 * h.numel() * w.shape[0]),
                       h, w, target, lse, dloss, dw, _grad_f32("softmax_xent_bwd", grad_dtype, h))
 

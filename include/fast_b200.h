@@ -38,6 +38,9 @@ typedef enum {
 const char *fb_last_error(void);
 /* Library version string. */
 const char *fb_version(void);
+/* Kernels the calling thread has launched through the entry points that count
+ * theirs (the node-ranking head's: how many a call takes depends on its sizes). */
+int64_t fb_launches(void);
 
 /* ------------------------------------------------------------------------- */
 /* Temporal neighbour sampler (runtime object).                               */

@@ -244,3 +244,31 @@ def test_bf16_head_gives_its_fp32_parameters_unrounded_gradients(cuda, n):
     loss.backward()
     assert all(p.grad.dtype == BF and bool(p.grad.isfinite().all()) for p in head.parameters())
     assert torch.isfinite(loss)
+
+
+# ---- counts ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,d,f", [(0, 64, 128), (1, 64, 128), (40, 64, 128), (300, 413, 700), (5000, 64, 128)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_launches_are_counted(cuda, n, d, f, dtype):
+    """ops.LAUNCHES rises by the kernel nodes that the same call leaves in a captured graph."""
+    from cuda.bindings import runtime
+    from fast_b200 import ops
+    g = _gen(cuda, n, d, f)
+    x, dy, ln = _mat(cuda, g, n, d, dtype), _mat(cuda, g, n, d, dtype), torch.ones(d, device=cuda)
+    wg, wu, wd = _mat(cuda, g, f, d, dtype), _mat(cuda, g, f, d, dtype), _mat(cuda, g, d, f, dtype)
+    t, one = torch.zeros(n, dtype=torch.int64, device=cuda), torch.ones(n, device=cuda)
+    for run in (lambda: ops.layer_norm_fwd(x, ln), lambda: ops.layer_norm_bwd(dy, x, ln, one, one),
+                lambda: ops.gated_ffn_fwd(x, wg, wu, wd), lambda: ops.gated_ffn_bwd(dy, x, wg, wu, wd),
+                lambda: ops.softmax_xent_fwd(x, wg, t), lambda: ops.softmax_xent_bwd(x, wg, t, one, one)):
+        before = ops.LAUNCHES[0]
+        run()
+        counted = ops.LAUNCHES[0] - before
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph):
+            run()
+        raw = runtime.cudaGraph_t(init_value=graph.raw_cuda_graph())
+        err, _, count = runtime.cudaGraphGetNodes(raw)
+        assert err == runtime.cudaError_t.cudaSuccess
+        err, nodes, _ = runtime.cudaGraphGetNodes(raw, count)
+        kinds = [runtime.cudaGraphNodeGetType(nd)[1] for nd in nodes[:count]]
+        assert counted == kinds.count(runtime.cudaGraphNodeType.cudaGraphNodeTypeKernel), (counted, kinds)
