@@ -87,10 +87,13 @@ class GatedFfnFunction(torch.autograd.Function):
 
 class SoftmaxXentFunction(torch.autograd.Function):
     """Per-row cross entropy (fp32 [n]) of softmax(h w^T), w in h's type.  A
-    table of fp32 receives an fp32 gradient."""
+    table of fp32 receives an fp32 gradient.  target: whole numbers of any type."""
 
     @staticmethod
     def forward(ctx, h, w, target):
+        if target.is_floating_point() or target.is_complex() or target.dtype == torch.bool:
+            raise ValueError("softmax cross entropy: the targets must be node numbers")
+        target = target.to(torch.int64).contiguous()
         ctx.grad_dtype = _f32_or_none(w)
         h, w = _rows(h), _rows(w.to(h.dtype))
         loss, lse = ops.softmax_xent_fwd(h, w, target)
@@ -118,14 +121,15 @@ class GatedFeedForward(torch.nn.Module):
         self.w_down = torch.nn.Parameter(torch.randn(dim, hidden) * hidden ** -0.5)
 
     def forward(self, x):
-        return GatedFfnFunction.apply(x.to(self.dtype), self.w_gate, self.w_up, self.w_down, self.act)
+        rows = x.to(self.dtype).reshape(-1, x.shape[-1])
+        return GatedFfnFunction.apply(rows, self.w_gate, self.w_up, self.w_down, self.act).view(x.shape)
 
 
 class NodeRankingHead(torch.nn.Module):
     """Residual, norm, gated block, norm, and the softmax over `nodes` nodes.
     forward(x, target, res) -> (mean loss over the rows whose target is not
     negative, per-row losses); embed(x, res) -> the rows that are compared with
-    the node table."""
+    the node table.  x and res are [..., dim], target [...]."""
 
     def __init__(self, dim, nodes, hidden=None, act="silu", dtype=torch.float32, eps=1e-5):
         super().__init__()
@@ -138,16 +142,19 @@ class NodeRankingHead(torch.nn.Module):
         self.node_table = torch.nn.Parameter(torch.randn(nodes, dim) * dim ** -0.5)
 
     def embed(self, x, res=None):
-        x = x.to(self.dtype)
+        shape = x.shape
+        x = x.to(self.dtype).reshape(-1, shape[-1])
         if res is None:
             s, y = x, LayerNormFunction.apply(x, self.norm1["weight"], self.norm1["bias"], self.eps, None)
         else:
-            y, s = LayerNormFunction.apply(x, self.norm1["weight"], self.norm1["bias"], self.eps, res.to(self.dtype))
+            res = res.to(self.dtype).reshape(-1, shape[-1])
+            y, s = LayerNormFunction.apply(x, self.norm1["weight"], self.norm1["bias"], self.eps, res)
         h, _ = LayerNormFunction.apply(self.ffn(y), self.norm2["weight"], self.norm2["bias"], self.eps, s)
-        return h
+        return h.view(shape)
 
     def forward(self, x, target, res=None):
-        rows = SoftmaxXentFunction.apply(self.embed(x, res), self.node_table, target)
+        h = self.embed(x, res)
+        rows = SoftmaxXentFunction.apply(h.view(-1, h.shape[-1]), self.node_table, target.reshape(-1)).view(target.shape)
         return rows.sum() / (target >= 0).sum().clamp(min=1), rows
 
 

@@ -110,3 +110,42 @@ def test_operators_in_a_captured_graph(cuda):
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(out, new))
     assert not torch.equal(out[0], want[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_head_takes_the_layouts_that_torch_takes(cuda, dtype):
+    """Strided and int32 targets, weights and tables that are transposes, rows under several leading dimensions: the
+    results are those of contiguous int64 ones."""
+    from fast_b200.ranking import GatedFeedForward, GatedFfnFunction, NodeRankingHead, SoftmaxXentFunction
+    torch.manual_seed(5)
+    x, w = torch.randn(24, 40, device=cuda).to(dtype), torch.randn(90, 40, device=cuda).to(dtype)
+    t = torch.randint(0, 90, (24,), device=cuda)
+    t[3] = -1
+    wide = torch.stack([t, t + 1], 1)
+    want = SoftmaxXentFunction.apply(x, w, t)
+    for other in (wide[:, 0], t.int(), t.short(), wide.int()[:, 0]):
+        assert torch.equal(SoftmaxXentFunction.apply(x, w, other), want)
+    table = w.t().contiguous().requires_grad_(True)             # [D, V]; its transpose has no unit column stride
+    got = SoftmaxXentFunction.apply(x, table.t(), t)
+    assert torch.equal(got, want)
+    got.sum().backward()
+    assert table.grad.shape == table.shape and bool(table.grad.isfinite().all())
+    ws = [torch.randn(s, device=cuda).to(dtype) for s in ((64, 40), (64, 40), (40, 64))]
+    y = GatedFfnFunction.apply(x, *ws, "silu")
+    turned = [p.t().contiguous().requires_grad_(True) for p in ws]
+    y2 = GatedFfnFunction.apply(x, *(p.t() for p in turned), "silu")
+    assert torch.equal(y, y2)
+    y2.sum().backward()
+    assert all(p.grad.shape == p.shape for p in turned)
+    with pytest.raises(ValueError):
+        SoftmaxXentFunction.apply(x, w, t.float())
+    ffn = GatedFeedForward(40, 64, dtype=dtype).to(cuda)
+    assert torch.equal(ffn(x.view(2, 3, 4, 40)), ffn(x).view(2, 3, 4, 40))
+    head = NodeRankingHead(40, 90, dtype=dtype).to(cuda)
+    xs = x.float().view(4, 6, 40).requires_grad_(True)
+    loss, rows = head(xs, t.view(4, 6), x.view(4, 6, 40))
+    flat, flat_rows = head(x, t, x)
+    assert torch.equal(loss, flat) and torch.equal(rows, flat_rows.view(4, 6))
+    assert head.embed(xs).shape == xs.shape
+    loss.backward()
+    assert xs.grad.shape == xs.shape
