@@ -51,14 +51,16 @@ template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// V elements of a weight row as floats; zeros when !in.
+// V elements of a weight row as floats; zeros when !in.  Volatile: a load must
+// not be moved ahead of the wait for the kernel before, which may have written
+// the weights.
 template <typename T, int V> struct Raw;
 template <> struct Raw<__nv_bfloat16, 8> {
   uint4 v;
   __device__ __forceinline__ void load(const __nv_bfloat16 *p, bool in) {
     v = make_uint4(0, 0, 0, 0);
     if (in)                                   // read once: past the L1
-      asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+      asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
           : "l"(p));
   }
@@ -72,7 +74,7 @@ template <> struct Raw<float, 4> {
   __device__ __forceinline__ void load(const float *p, bool in) {
     v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (in)
-      asm("ld.global.nc.L1::no_allocate.L2::256B.v4.f32 {%0, %1, %2, %3}, [%4];"
+      asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.f32 {%0, %1, %2, %3}, [%4];"
           : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
           : "l"(p));
   }

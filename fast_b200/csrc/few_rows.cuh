@@ -20,7 +20,8 @@ namespace fbh {
 //   logits 2,048 x 50,000       fp32 fwd 1: 69 / 381, 8: 109 / 381;  bwd 1: 219 / 1221, 8: 327 / 1221
 //                               bf16 fwd 1: 39 / 59, 2: 42 / 59, 4: 77 / 59;  bwd 1: 136 / 312, 2: 151 / 312, 4: 213 / 312
 //   gated block 100 x 400       bf16 fwd 1: 8.2 / 12.4, 8: 9.9 / 12.4;  bwd 1: 19.7 / 16.9, 8: 24.5 / 16.9
-//   logits 1,590 x 20,011       bf16 bwd 1: 125 / 126, 2: 130 / 126, 4: 155 / 126 (rows that no wide load lines up with)
+//   logits 1,590 x 20,011       bf16 bwd 1: 125 / 126, 2: 130 / 126, 4: 155 / 126 (rows that no wide load lines up with:
+//                               2 of them lose 3% here, 4 us of a call that no rule of its own is made for)
 bool few_rows_ok(int type, bool bwd, int64_t n, int64_t K, int64_t weight_elements);
 // h [n, F] (fp32, pitch F) = act(x Wg^T) (x Wu^T)
 int few_rows_glu(Call &c, int type, int act, const Mat &x, int64_t n, int D, const Mat &wg, const Mat &wu, int F,
