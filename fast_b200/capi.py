@@ -173,7 +173,6 @@ _SIGS["fb_layer_norm_bwd_ws_bytes"] = (_SZ, [_I64, _I])
 _SIGS["fb_layer_norm_bwd"] = (_I, [_I, _P, _I64, _P, _I64, _P, _I, _P, _P, _P, _I64, _P, _I64, _P, _P, _I, _I64, _I,
                                    _P, _SZ, _P])
 
-F32, BF16 = 0, 1
 ACTS = {"silu": 0, "gelu": 1, "relu": 2}
 
 
