@@ -404,6 +404,11 @@ template <int EPI> __device__ __forceinline__ Tile tile_at(const PairArgs &a, in
 // Columns c .. c + 31 of g (and + 128: u, and of dh at td) of this warp's 32 rows:
 // h (and dg, du) staged as half of the warp's 128-byte rows, sent off with the
 // second half: the copy engine takes a 64-byte row no faster than a 128-byte one.
+// h, dg and du are rounded to bf16 here, once each: they are the next products'
+// operands, and the tensor cores' bf16 products are what a bf16 call is for (fp32
+// operands take six of them).  The results then carry two roundings, their own
+// and this one: 0.0024 off in the 2-norm, 0.0017 with h, dg, du in fp32 (12,000 x
+// 172 x 688).  A module of elementary bf16 operations rounds g, u, act(g) and h.
 template <int ACT, bool BWD>
 __device__ __forceinline__ void glu_block(const PairArgs &a, uint32_t t, uint32_t td, int c, int which, uint8_t *buf, int row,
                                           int col, int lane) {
@@ -835,6 +840,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         const int64_t tg = i0 < b.M ? a.target[i0] : -1;
         const bool live = tg >= 0 && tg < a.V;
         const float z = live ? a.lse[i0] * kLog2e : 0.f, d = live ? a.dloss[i0] : 0.f;
+        // G is rounded to bf16 as h, dg, du are (glu_block): dh and dw 0.0024 off in the 2-norm, 0.0017 with G in fp32
+        // (4,000 x 100, 16,700 nodes)
         const uint32_t mask = live ? 0xFFFFFFFFu : 0u;            // a held-out row is zeros whatever its logits are
         const int64_t tc = live ? tg - a.v0 : -1;                 // the target's column of this piece
 #pragma unroll 1

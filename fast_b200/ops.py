@@ -727,7 +727,13 @@ def gated_ffn_fwd(x, w_gate, w_up, w_down, act="silu"):
     """y = (act(x w_gate^T) * (x w_up^T)) w_down^T for rows x [n, D] and
     weights w_gate, w_up [F, D], w_down [D, F], all fp32 or all bf16 (any row
     pitch).  act: "silu", "gelu" (erf form) or "relu".  Products accumulate
-    in fp32; the backward needs nothing but the inputs."""
+    in fp32; the backward needs nothing but the inputs.
+
+    fp32 calls round nothing in between.  bf16 calls round the hidden row
+    act(..) * (..) to bf16 before w_down, and the backward its two gradients,
+    each once, as operands of bf16 products: results are 0.0024 off in the
+    2-norm, 0.0017 of it their own rounding.  (Single rows, which run without
+    tensor cores against large weights, keep them in fp32.)"""
     return _head_call(head_ops.gated_ffn_fwd,
                       lambda: (x.element_size() * (2 * x.numel() + 3 * w_gate.numel()), 6 * x.numel() * w_gate.shape[0]), x,
                       w_gate, w_up, w_down, _act(act))
@@ -763,7 +769,9 @@ def softmax_xent_fwd(h, w, target):
 def softmax_xent_bwd(h, w, target, lse, dloss, dw=None, grad_dtype=None):
     """Gradients of softmax_xent_fwd for dloss [n] (fp32): (dh, dw), of the
     inputs' type (dw, a sum in fp32, as it is with grad_dtype=torch.float32);
-    an fp32 buffer given as dw is accumulated into instead."""
+    an fp32 buffer given as dw is accumulated into instead.  bf16 calls round
+    dloss * (softmax - onehot) to bf16 as an operand of both products (but for
+    one or two rows against large tables), fp32 calls do not."""
     return _head_call(head_ops.softmax_xent_bwd,
                       lambda: (2 * h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 6 * h.numel() * w.shape[0]),
                       h, w, target, lse, dloss, dw, _grad_f32("softmax_xent_bwd", grad_dtype, h))

@@ -616,7 +616,9 @@ int fb_layer_norm_bwd(int type, const void *dy, int64_t lddy, const void *x, int
                       size_t ws_bytes, cudaStream_t stream);
 /* Gated feed-forward block  y = (act(x Wg^T) * (x Wu^T)) Wd^T  over rows x
  * [n, D]; w_gate, w_up [F, D], w_down [D, F] (torch.nn.Linear layout), all of
- * one type; products accumulate in fp32.  The backward takes dy and x alone (it
+ * one type; products accumulate in fp32.  bf16: act(..) * (..), and in the
+ * backward its two gradients, are rounded to bf16 as operands of the next
+ * products (few rows keep them in fp32).  The backward takes dy and x alone (it
  * recomputes what the activation saw) and writes dx (rows' type) and the weight
  * gradients (grad_type: fp32 or the rows' type; += when accumulate, fp32 only);
  * any of the four may be NULL.  GELU is the erf form.  Deterministic.
@@ -641,13 +643,16 @@ size_t fb_gated_ffn_ws_bytes(const fb_gated_ffn *args, int backward);
 int fb_gated_ffn_fwd(const fb_gated_ffn *args, void *ws, size_t ws_bytes, cudaStream_t stream);
 int fb_gated_ffn_bwd(const fb_gated_ffn *args, void *ws, size_t ws_bytes, cudaStream_t stream);
 /* Softmax cross entropy of rows h [n, D] over the V rows of a table w [V, D]
- * (logits h w^T, never kept), one type, fp32 accumulation:
+ * (logits h w^T, not kept; calls of few rows or few tiles hold theirs in the
+ * workspace), one type, fp32 accumulation:
  *   lse[i] = log sum_v exp(l_iv),  loss[i] = lse[i] - l_i,target[i]
  * A negative target holds its row out: loss 0 and no gradient, whatever the
- * row holds.  A target >= V gives a NaN loss and no gradient.  Backward, from lse and dloss [n] (fp32):
+ * row holds.  A target >= V gives a NaN loss and no gradient.
+ * Backward, from lse and dloss [n] (fp32):
  *   G_iv = dloss[i] (exp(l_iv - lse[i]) - [v == target[i]])
  *   dh = G w (rows' type),  dw = G^T h (grad_type; += when accumulate, fp32 only)
- * dh or dw may be NULL.  Deterministic.
+ * dh or dw may be NULL.  bf16: G is rounded to bf16 as an operand of both
+ * products (few rows keep it in fp32).  Deterministic.
  * ws: fb_softmax_xent_ws_bytes(args, backward) bytes, 16-byte aligned. */
 typedef struct fb_softmax_xent {
   int type, grad_type, accumulate, D;

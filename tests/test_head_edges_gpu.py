@@ -7,7 +7,7 @@ import threading
 import pytest
 import torch
 
-from test_head_gpu import _c, _check, _gen, _mat
+from test_head_gpu import _c, _check, _gen, _mat, test_gated_ffn as gated_ffn, test_softmax_xent as softmax_xent
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -272,3 +272,43 @@ def test_launches_are_counted(cuda, n, d, f, dtype):
         err, nodes, _ = runtime.cudaGraphGetNodes(raw, count)
         kinds = [runtime.cudaGraphNodeGetType(nd)[1] for nd in nodes[:count]]
         assert counted == kinds.count(runtime.cudaGraphNodeType.cudaGraphNodeTypeKernel), (counted, kinds)
+
+
+# ---- the smallest sizes ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,d,f,pad", [(1, 1, 1, 0), (2, 1, 3, 0), (9, 1, 1, 0), (9, 2, 1, 1), (12, 3, 5, 0), (130, 7, 2, 5),
+                                       (300, 1, 9, 0), (257, 8, 1, 0)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_widths_below_sixteen(cuda, n, d, f, pad, dtype):
+    gated_ffn(cuda, n, d, f, pad, dtype, "silu")
+    softmax_xent(cuda, n, d, f, pad, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_in_a_wider_buffer_leave_the_rest_of_it_alone(cuda, dtype):
+    """Not-a-numbers around every operand are not read into a result; buffers written with a pitch keep what lies between
+    their rows."""
+    from fast_b200 import ops
+    g = _gen(cuda, 11, 3)
+
+    def framed(rows, cols, off):
+        buf = torch.full((rows + 2, cols + 7), math.nan, device=cuda, dtype=dtype)
+        view = buf[1:-1, off:off + cols]
+        view.copy_(torch.randn(rows, cols, device=cuda, generator=g))
+        return view
+    for n in (2, 70):
+        for d, f, off in ((40, 72, 0), (33, 65, 3), (64, 128, 7)):
+            x, dy, wg, wu, wd = (framed(*s, off) for s in ((n, d), (n, d), (f, d), (f, d), (d, f)))
+            t = torch.randint(0, f, (n,), device=cuda, generator=g)
+            lse = ops.softmax_xent_fwd(x, wg, t)[1]
+            one = torch.ones(n, device=cuda)
+            outs = [*ops.layer_norm_fwd(x, torch.ones(d, device=cuda)), ops.gated_ffn_fwd(x, wg, wu, wd), lse,
+                    *ops.gated_ffn_bwd(dy, x, wg, wu, wd), *ops.softmax_xent_bwd(x, wg, t, lse, one),
+                    *ops.layer_norm_bwd(dy, x, torch.ones(d, device=cuda), one, one)]
+            assert all(bool(o.isfinite().all()) for o in outs)
+            bufs = [torch.full((r, c + 5), 7.0, device=cuda) for r, c in ((f, d), (f, d), (d, f), (f, d))]
+            views = [b[:, off % 4:off % 4 + c] for b, c in zip(bufs, (d, d, f, d))]
+            ops.gated_ffn_bwd(dy, x, wg, wu, wd, grads=views[:3])
+            ops.softmax_xent_bwd(x, wg, t, lse, one, dw=views[3])
+            for b, c in zip(bufs, (d, d, f, d)):
+                assert bool((b[:, :off % 4] == 7).all()) and bool((b[:, off % 4 + c:] == 7).all())
+                assert bool(b.isfinite().all())
