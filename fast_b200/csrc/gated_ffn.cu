@@ -112,21 +112,28 @@ int forward_f32(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &wg, con
 // g and u (and dh) of every tile, the activation in the epilogue: h [N, Fp],
 // and for the backward dgu [N, 2 Fp] = [dg | du].  Fp = F rounded up to 64;
 // the padding columns are zeros (weight rows past F read as zeros).
+//
+// ReLU's backward turns with the sign of g, and the tensor cores' accumulation truncates: it sums g and u in slabs of
+// kGluSlab stages (kGluBwdLong) where D is longer than one.  The other activations' derivatives are smooth, and an error
+// of g of some 2^-18 is lost in the rounding to bf16.  us of the whole backward, with slabs / without: 8,192 x 2,048 x
+// 8,192 1,624 / 1,594; 1,500 x 1,024 x 2,000 64 / 64; 12,000 x 300 x 1,200 115 / 120.
 template <int EPI>
 int glu(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, const Mat &wg, const Mat &wu, const Mat &wd,
         __nv_bfloat16 *h, __nv_bfloat16 *dgu, int64_t Fp) {
   using namespace fbpair;
+  constexpr bool bwd = EPI == kGluBwd || EPI == kGluBwdLong;
+  constexpr int dh = EPI == kGluBwd ? 0 : 1;   // the term of dh
   if (c.dry) return FB_OK;
   PairArgs p;
-  one_product(p, a.n, Fp, 128, tiles_of(a.D, BK), EPI == kGluBwd ? 2 : 1);
+  one_product(p, a.n, Fp, 128, tiles_of(a.D, BK), bwd ? 2 : 1);
   p.act = a.act;
   PairProb &b = p.p[0];
-  FBH_TRY(make_map(&b.ta[EPI == kGluBwd ? 1 : 0], x.p, a.n, a.D, x.ld, kHalfM));
+  FBH_TRY(make_map(&b.ta[1 - dh], x.p, a.n, a.D, x.ld, kHalfM));
   FBH_TRY(make_map(&b.tb[0], wg.p, a.F, a.D, wg.ld, 128));
   FBH_TRY(make_map(&b.tb[1], wu.p, a.F, a.D, wu.ld, 128));
   FBH_TRY(make_map(&b.tc, h, a.n, Fp, Fp, 32));
-  if (EPI == kGluBwd) {
-    FBH_TRY(make_map(&b.ta[0], dy.p, a.n, a.D, dy.ld, kHalfM));   // dh comes first
+  if (bwd) {
+    FBH_TRY(make_map(&b.ta[dh], dy.p, a.n, a.D, dy.ld, kHalfM));
     FBH_TRY(make_map(&p.tw, wd.p, a.D, a.F, wd.ld, BK));
     FBH_TRY(make_map(&p.tc2[0], dgu, a.n, Fp, 2 * Fp, 32));
     FBH_TRY(make_map(&p.tc2[1], dgu + Fp, a.n, Fp, 2 * Fp, 32));
@@ -179,7 +186,9 @@ int backward_bf16(Call &c, const fb_gated_ffn &a, const Mat &x, const Mat &dy, c
   const int64_t Fp = round_up(a.F, 64);
   FBH_TAKE(h, c, __nv_bfloat16, a.n * Fp);
   FBH_TAKE(dgu, c, __nv_bfloat16, a.n * 2 * Fp);
-  FBH_TRY(glu<fbpair::kGluBwd>(c, a, x, dy, wg, wu, wd, h, dgu, Fp));
+  const bool slabs = a.act == FB_ACT_RELU && a.D > fbpair::kGluSlab * fbpair::BK;
+  FBH_TRY(slabs ? glu<fbpair::kGluBwdLong>(c, a, x, dy, wg, wu, wd, h, dgu, Fp)
+                : glu<fbpair::kGluBwd>(c, a, x, dy, wg, wu, wd, h, dgu, Fp));
   return gradients(c, a, x, dy, wg, wu, Mat{h, Fp}, Mat{dgu, 2 * Fp}, Fp);
 }
 

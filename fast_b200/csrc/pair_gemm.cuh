@@ -36,6 +36,7 @@
 // (the epilogue drains one while the other fills).  kGluBwd's tile takes 384:
 // g | u has one place and dh two, dh comes first, and the g | u stages wait for
 // the epilogue of the tile before, which has had dh's time to drain them.
+// kGluBwdLong gives each slab of g | u one of the two places, and then dh.
 //
 // No load uses cluster multicast.  Every wait is bounded: past the limit a
 // CTA records an error, stops, gives its copies time to land and leaves.
@@ -53,7 +54,7 @@ namespace fbpair {
 
 using namespace fbtc;
 
-enum : int { kStore = 0, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6, kLsePlanes = 7, kProbPlanes = 8 };
+enum : int { kStore = 0, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6, kLsePlanes = 7, kProbPlanes = 8, kGluBwdLong = 9 };
 using fbact::kGelu;
 using fbact::kRelu;
 using fbact::kSilu;
@@ -73,23 +74,28 @@ template <int EPI> __host__ __device__ constexpr int threads_of() { return (kWar
 constexpr int kTmemCols = 512;
 constexpr int kStageOut = 4096;               // one staged output block: 32 rows of 128 bytes
 constexpr int kLseSlab = 16;                  // kLseLong: stages summed in tensor memory at a time
+constexpr int kGluSlab = 4;                   // kGluBwdLong: the same for g and u
+// Stages after which an accumulator of the first term goes to registers; 0: at the end.
+template <int EPI> __host__ __device__ constexpr int slab_of() {
+  return EPI == kLseLong ? kLseSlab : (EPI == kGluBwdLong ? kGluSlab : 0);
+}
 template <int EPI> __host__ __device__ constexpr int out_bytes() {
-  return EPI == kGluBwd ? 3 * kStageOut : (EPI == kLse || EPI == kLseLong ? 0 : kStageOut);
+  return EPI == kGluBwd || EPI == kGluBwdLong ? 3 * kStageOut : (EPI == kLse || EPI == kLseLong ? 0 : kStageOut);
 }
 template <int EPI, int P> __host__ __device__ constexpr int stages() {
-  return P == 3 ? 8 : (EPI == kGluBwd ? 4 : (EPI == kProb ? 5 : 6));
+  return P == 3 ? 8 : (EPI == kGluBwd || EPI == kGluBwdLong ? 4 : (EPI == kProb ? 5 : 6));
 }
 template <int EPI, int P> __host__ __device__ constexpr int smem_bytes() {
   return 1024 + stages<EPI, P>() * stage_bytes<P>() + epi_warps<EPI>() * out_bytes<EPI>() + 256;
 }
-static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 232448 &&
+static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kGluBwdLong, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 232448 &&
                   smem_bytes<kStore, 1>() <= 232448 &&
                   smem_bytes<kStore, 3>() <= 232448 && smem_bytes<kProbPlanes, 3>() <= 232448, "shared memory exceeds 227 KB");
 
 constexpr int kMaxProbs = 4;
 
 // One product.  Two terms may feed a tile: kGluBwd's first one fills the dh
-// columns, its second g | u; elsewhere the second continues the same sum (dx = dg Wg + du Wu) and its
+// columns, its second g | u (kGluBwdLong: the other way round); elsewhere the second continues the same sum (dx = dg Wg + du Wu) and its
 // stages follow the first's.
 struct PairProb {
   CUtensorMap ta[2], tb[2];                   // by term; kGlu*: tb[0] = Wg, tb[1] = Wu
@@ -464,7 +470,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
   constexpr int kStages = stages<EPI, P>(), kStageBytes = stage_bytes<P>(), kBBytes = b_bytes<P>();
   constexpr int kBufs = EPI == kGluBwd ? 1 : 2, kEpiWarps = epi_warps<EPI>();
   constexpr bool kAlt = EPI == kLse || EPI == kProb;            // two sets of epilogue warps, alternate tiles
-  constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd;      // B: 128 rows of Wg in one CTA, of Wu in the other
+  constexpr bool kDual = EPI == kGluFwd || EPI == kGluBwd || EPI == kGluBwdLong;   // B: 128 rows of Wg in one CTA, of Wu in the other
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
   auto sA = [&](int s) { return smem + s * kStageBytes; };
@@ -498,7 +504,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
     prefetch_map(&b.tb[0]);
     if (b.kb[1]) prefetch_map(&b.ta[1]);
     if (b.kb[1] || kDual) prefetch_map(&b.tb[1]);
-    if (EPI == kGluBwd) prefetch_map(&a.tw);
+    if (EPI == kGluBwd || EPI == kGluBwdLong) prefetch_map(&a.tw);
   }
   tc_fence_before();
   __syncthreads();
@@ -524,7 +530,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
       const int bn_ = P == 3 ? 128 : (EPI == kStore ? b.bn : 256);
       for (int j = q.k0; j < q.k1; ++j) {
         const int p = j >= kb0 ? 1 : 0, jj = j - (p ? kb0 : 0);
-        const bool dh = EPI == kGluBwd && p == 0;
+        const bool dh = (EPI == kGluBwd && p == 0) || (EPI == kGluBwdLong && p == 1);
         const int bn = dh ? 128 : bn_;
         const bool bmn = dh || bmn_;
         const CUtensorMap *ma = &b.ta[p], *mb = dh ? &a.tw : &b.tb[kDual ? rank : p];
@@ -581,13 +587,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         const int bn = P == 3 ? 128 : (EPI == kStore ? b.bn : 256), kb0 = b.kb[0];
         const uint64_t ad0 = sdesc(smem_u32(smem), amn), adv_a = amn ? (2048 >> 4) : 2;
         for (int j = q.k0; j < q.k1; ++j) {
-          const bool dh = EPI == kGluBwd && j < kb0, bmn = dh || bmn_;
+          const bool dh = (EPI == kGluBwd && j < kb0) || (EPI == kGluBwdLong && j >= kb0), bmn = dh || bmn_;
           const uint32_t idesc = dh ? idesc2(128, false, true) : idesc2(bn, amn, bmn);
           const uint64_t bd0 = sdesc(smem_u32(smem + kABytes), bmn), adv_b = bmn ? (2048 >> 4) : 2;
-          // a new accumulator at the tile's start (kGluBwd: where g | u start), or for every slab
-          const bool next = P == 3 || (EPI == kGluBwd ? j == kb0 : j == q.k0) ||
-                            (EPI == kLseLong && (j & (kLseSlab - 1)) == 0);
-          const bool fresh = next || (dh && j == q.k0);
+          // a new accumulator at the tile's start (kGluBwd: where g | u start), or for every slab (kGluBwdLong: and dh)
+          constexpr int kSlab = slab_of<EPI>();
+          const bool next = P == 3 || (EPI == kGluBwd ? j == kb0 : j == q.k0) || (EPI == kGluBwdLong && j == kb0) ||
+                            (kSlab && !dh && (j & (kSlab - 1)) == 0);
+          const bool fresh = next || (EPI == kGluBwd && j == q.k0);
           const uint32_t buf = it % kBufs, use = it / kBufs;
           if (next && use >= 1 && !wait(acce + buf, (use - 1) & 1, abort_flag, err)) {
             stop = true;
@@ -597,8 +604,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
             stop = true;
             break;
           }
-          const bool last = P == 3 || j + 1 == q.k1 || (EPI == kLseLong && ((j + 1) & (kLseSlab - 1)) == 0);
-          const uint32_t d = tmem + (dh ? 256u + (it & 1) * 128u : buf * 256u);
+          const bool last = P == 3 || j + 1 == q.k1 || (EPI == kGluBwdLong && j + 1 == kb0) ||
+                            (kSlab && !dh && ((j + 1) & (kSlab - 1)) == 0);
+          const uint32_t d = tmem + (EPI == kGluBwd && dh ? 256u + (it & 1) * 128u : buf * 256u);
           // one product of 64 k: A of stage sa, B of stage sb
           auto issue = [&](int sa, int sb, bool first) {
             const uint64_t ad = ad0 + (uint64_t)(sa * (kStageBytes >> 4)), bd = bd0 + (uint64_t)(sb * (kStageBytes >> 4));
@@ -751,6 +759,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
         --it;                                 // the loop header counts one
         if (!ok) break;
         if (row + lane < b.M) a.part[(int64_t)(row + lane) * (4 * b.nt) + 4 * q.n + half] = max_sum(v, left);
+        continue;
+      }
+      if constexpr (EPI == kGluBwdLong) {
+        // g and u of 64 columns, slab by slab, then dh: relu'(g) turns with the sign of g, so g is summed like fp32.
+        // (Tensor memory alone, whose additions truncate, turned ten signs of 6,330 x 6,112 at width 2,306, fp32 two.)
+        float g[64], u[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) g[i] = u[i] = 0.f;
+        bool ok = true;
+        auto take = [&]() {
+          const int at = it % kBufs;
+          ok = __all_sync(0xffffffffu, wait(accf + at, (it / kBufs) & 1, abort_flag, err) ? 1 : 0);
+          if (ok) tc_fence_after();
+          return tmem + tlane + (uint32_t)(at * 256 + half * 64);
+        };
+        auto give = [&]() {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(leader_addr(acce + it % kBufs));
+          ++it;
+        };
+        for (int j = 0; j < b.kb[0]; j += kGluSlab) {
+          const uint32_t at = take();
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < 128; c += 16) {
+            uint32_t r[16];
+            tmem_ld16_nowait(at + (c < 64 ? c : 64 + c), r);
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float &s = c < 64 ? g[(c + i) & 63] : u[(c + i) & 63];
+              s += __uint_as_float(r[i]);
+            }
+          }
+          give();
+        }
+        if (!ok) break;
+        const uint32_t at = take();
+        if (!ok) break;
+        const int row = q.m * 256 + (int)rank * kHalfM + qd * 32, col = q.n * 128 + half * 64;
+        if (lane == 0) store_wait<0>();       // the tile before has left the buffers
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t d[16];
+          tmem_ld16_nowait(at + c, d);
+          tmem_wait();
+#pragma unroll
+          for (int k = 0; k < 16; k += 8) {   // 8 columns: one 16-byte piece of the row (stage_row)
+            uint32_t w[3][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float h[2], dg[2], du[2];
+#pragma unroll
+              for (int o = 0; o < 2; ++o) {
+                const float dv = __uint_as_float(d[k + 2 * i + o]), uv = u[c + k + 2 * i + o];
+                const float2 f = fbact::act_fast<kRelu>(g[c + k + 2 * i + o]);
+                h[o] = f.x * uv;
+                dg[o] = dv * uv * f.y;
+                du[o] = dv * f.x;
+              }
+              w[0][i] = pack(h[0], h[1]);
+              w[1][i] = pack(dg[0], dg[1]);
+              w[2][i] = pack(du[0], du[1]);
+            }
+#pragma unroll
+            for (int o = 0; o < 3; ++o)
+              *reinterpret_cast<uint4 *>(obuf + o * kStageOut + lane * 128 + ((((c + k) / 8) ^ (lane & 7)) << 4)) =
+                  make_uint4(w[o][0], w[o][1], w[o][2], w[o][3]);
+          }
+        }
+        give();
+        --it;                                 // the loop header counts one
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (row < b.M && col < b.N)
+#pragma unroll
+            for (int o = 0; o < 3; ++o) store_tile(o ? &a.tc2[o - 1] : &b.tc, obuf + o * kStageOut, col, row);
+          store_commit();
+        }
         continue;
       }
       const int buf = it % kBufs;

@@ -160,3 +160,47 @@ def test_products_of_the_gated_block_keep_all_planes(cuda, n, d, f):
                                    ("dw_down", out[4], DY.t() @ U, 2)):
         off = float((got.double() - want).norm() / want.norm())
         assert off <= chain * 2.0 ** -19.5, (name, math.log2(off))
+
+
+# ---- long sums in front of a discontinuity ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n,d,f", [(300, 1100, 700), (1500, 4096, 2000), (2000, 2306, 3000)])
+def test_relu_gradients_of_wide_bf16_rows(cuda, n, d, f):
+    """relu'(g) turns with the sign of g, so an error of g next to zero is one of the gradients: the products of g must
+    be as good as fp32 sums.  A bf16 rounding is off by 2^-8 / sqrt(3) in the 2-norm at most, and the gradients carry two;
+    fp32 sums turn few enough signs to add nothing that shows."""
+    from fast_b200 import ops
+    g = _gen(cuda, n, d, f)
+    x, dy = _mat(cuda, g, n, d, BF), _mat(cuda, g, n, d, BF)
+    wg, wu, wd = _mat(cuda, g, f, d, BF, d ** -0.5), _mat(cuda, g, f, d, BF, d ** -0.5), _mat(cuda, g, d, f, BF, f ** -0.5)
+    X, DY, WG, WU, WD = (p.double() for p in (x, dy, wg, wu, wd))
+    G, U, DH = X @ WG.t(), X @ WU.t(), DY @ WD
+    A = G.clamp(min=0)
+    DG, DU, H = DH * U * (G > 0), DH * A, A * U
+    out = ops.gated_ffn_bwd(dy, x, wg, wu, wd, act="relu")
+    for name, got, want in (("dx", out[0], DG @ WG + DU @ WU), ("dw_gate", out[1], DG.t() @ X), ("dw_up", out[2], DU.t() @ X),
+                            ("dw_down", out[3], DY.t() @ H)):
+        off = float((got.double() - want).norm() / want.norm())
+        assert off <= 2 ** 0.5 * 2.0 ** -8 / 3 ** 0.5, (name, off)
+
+
+@pytest.mark.parametrize("n,d,f", [(4, 2048, 1000), (300, 700, 900), (300, 2048, 500), (260, 4096, 3000)])
+def test_relu_turns_where_an_fp32_sum_of_bf16_rows_would(cuda, n, d, f):
+    """g = 1024 + (small terms) - 1024, in this order along the row: truncating every 16 terms beside the 1024 loses
+    2^-14 each time, a hundred times and more; summing 256 terms at a time and these sums in fp32 is off by less than
+    16 * 2^-14 + 2^-13 < 2^-9.  u = dh = 1, so dg = relu'(g), which columns of the unit matrix show in dw_gate."""
+    from fast_b200 import ops
+    g = _gen(cuda, n, d, f)
+    x, wg = torch.zeros(n, d, device=cuda, dtype=BF), torch.zeros(f, d, device=cuda, dtype=BF)
+    wu, wd, dy = torch.zeros_like(wg), torch.zeros(d, f, device=cuda, dtype=BF), torch.zeros_like(x)
+    x[:, 0], wu[:, 0], wd[0], dy[:, 0] = 1, 1, 1, 1
+    x[:, 1], wg[:, 1], x[:, d - 1], wg[:, d - 1] = 32, 32, 32, -32
+    small = slice(256, d - 1 - n) if d > 1000 else slice(64, d - 1 - n)
+    x[:, small] = _mat(cuda, g, n, small.stop - small.start, BF)
+    wg[:, small] = _mat(cuda, g, f, small.stop - small.start, BF, 0.02 * (small.stop - small.start) ** -0.5)
+    unit = slice(small.stop, small.stop + n)
+    x[:, unit] = torch.eye(n, device=cuda, dtype=BF)
+    dg = ops.gated_ffn_bwd(dy, x, wg, wu, wd, act="relu")[1][:, unit].t()
+    G = x.double() @ wg.double().t()
+    sure = G.abs() > 2.0 ** -9
+    assert 0.5 < float(sure.double().mean()) < 1
+    assert bool((dg[sure].double() == (G[sure] > 0).double()).all())
