@@ -11,7 +11,7 @@ struct Job {
   void *dst;
   int ldd, cols, wide;                       // wide: 16-byte (8-byte) loads of the source's groups of 4
   const int64_t *target;                     // Operand's
-  int64_t V;
+  int64_t V, again;                          // elements to the second copy (0: none)
   uint32_t groups, per_row;                  // groups of 4 columns, in all and a row
   unsigned first;                            // first CTA of the job
 };
@@ -56,6 +56,7 @@ template <bool PLANES> __global__ void __launch_bounds__(256) k_operands(const _
         if (c + 3 < j.cols) v.w = s[3];
       }
       *reinterpret_cast<ushort4 *>(d) = v;
+      if (j.again) *reinterpret_cast<ushort4 *>(d + j.again) = v;
     }
   }
 }
@@ -72,10 +73,10 @@ int operands(Call &c, int type, const Operand *ops, int n) {
   for (int i = 0; i < n; ++i) {
     const Operand &o = ops[i];
     *o.out = Mat{o.src.p, o.src.ld};
-    if (!planes && !o.target && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * 2)) & 15u) == 0) continue;
+    if (!planes && !o.target && !o.twice && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * 2)) & 15u) == 0) continue;
     // rows on 128-byte boundaries: a 128-byte box row that crosses one costs the copy engine two requests
     const int64_t ld = round_up(o.cols, 64), plane = o.rows * ld;
-    void *p = c.take((size_t)(plane * (planes ? 6 : 2)));
+    void *p = c.take((size_t)(plane * (planes ? 6 : (o.twice ? 4 : 2))));
     if (!p) return fb::set_error(FB_ERR_ARG, "workspace too small");
     *o.out = Mat{p, ld, planes ? plane : 0};
     if (o.rows == 0) continue;
@@ -84,7 +85,7 @@ int operands(Call &c, int type, const Operand *ops, int n) {
     if (groups > UINT32_MAX / 2) return fb::set_error(FB_ERR_UNSUPPORTED, "operand of more than 2^33 elements");
     const int es = elem(type);
     const bool wide = o.cols % 4 == 0 && ((reinterpret_cast<uintptr_t>(o.src.p) | (uintptr_t)(o.src.ld * es)) & (4 * es - 1)) == 0;
-    jobs.j[jobs.n++] = Job{o.src.p, o.src.ld, plane, p, (int)ld, o.cols, wide, o.target, o.V, (uint32_t)groups, per_row, ctas};
+    jobs.j[jobs.n++] = Job{o.src.p, o.src.ld, plane, p, (int)ld, o.cols, wide, o.target, o.V, o.twice ? plane : 0, (uint32_t)groups, per_row, ctas};
     ctas += (unsigned)((groups + 256 * kGroups - 1) / (256 * kGroups));
   }
   if (c.dry || jobs.n == 0) return FB_OK;

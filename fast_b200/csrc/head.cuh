@@ -59,6 +59,7 @@ struct Operand {
   Mat *out;
   const int64_t *target = nullptr;           // given: rows whose target is not one of V are laid out as zeros
   int64_t V = 0;
+  bool twice = false;                        // laid out a second time below itself (2 rows in all); bf16
 };
 int operands(Call &c, int type, const Operand *ops, int n);
 
@@ -88,6 +89,7 @@ struct Product {
   int64_t M;
   int N, b_n;
   Out out;
+  bool fold = false;                         // the result is the M / 2 sums of rows m and m + M / 2
 };
 inline Product rows_product(const Mat &A, int64_t M, int K, const Mat &B, bool b_mn, int N, const Out &out) {
   return Product{false, b_mn, A, K, M, {{B, 0, K}, {}}, 1, M, N, N, out};

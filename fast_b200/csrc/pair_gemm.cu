@@ -7,11 +7,12 @@ namespace {
 using namespace fbpair;
 using namespace fbh;
 
-// out (+)= sum over splits of P[s], in split order; P rows have pitch ldp.
+// out (+)= sum over splits of P[s], in split order; P rows have pitch ldp.  fold > 0: and of the values `fold`
+// elements further on, a sum of its own.
 struct SumJob {
   const float *P;
   void *out;
-  int64_t ldo, ldp, split_stride, rows;
+  int64_t ldo, ldp, split_stride, rows, fold;
   int splits, cols, accumulate, bf16;
   unsigned first;                              // first CTA of the job
 };
@@ -31,22 +32,27 @@ __global__ void __launch_bounds__(kSumPerCta) k_sum_splits(const __grid_constant
   const int64_t r = i < ((int64_t)1 << 31) ? (int64_t)((uint32_t)i / (uint32_t)j.cols) : i / j.cols;
   const int c = (int)(i - r * j.cols);
   const float *p = j.P + r * j.ldp + c;
-  float s = 0.f;
-  int z = 0;
-  for (; z + 8 <= j.splits; z += 8) {
-    float v[8];
+  auto total = [&](const float *p) {
+    float s = 0.f;
+    int z = 0;
+    for (; z + 8 <= j.splits; z += 8) {
+      float v[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = p[(z + u) * stride];
+      for (int u = 0; u < 8; ++u) v[u] = p[(z + u) * stride];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s += v[u];
-  }
-  if (z < j.splits) {                          // the last few at once too
-    float v[7];
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+    if (z < j.splits) {                        // the last few at once too
+      float v[7];
 #pragma unroll
-    for (int u = 0; u < 7; ++u) v[u] = z + u < j.splits ? p[(z + u) * stride] : 0.f;
+      for (int u = 0; u < 7; ++u) v[u] = z + u < j.splits ? p[(z + u) * stride] : 0.f;
 #pragma unroll
-    for (int u = 0; u < 7; ++u) s += v[u];
-  }
+      for (int u = 0; u < 7; ++u) s += v[u];
+    }
+    return s;
+  };
+  float s = total(p);
+  if (j.fold) s += total(p + j.fold);
   if (j.bf16) {
     static_cast<__nv_bfloat16 *>(j.out)[r * j.ldo + c] = __float2bfloat16_rn(s);
   } else {
@@ -173,13 +179,14 @@ int products(Call &c, const Product *all, int n_all) {
     PairProb &b = a.p[i];
     const int64_t prow = (int64_t)b.mt * 256, pld = round_up(p.N, 4);
     b.split_rows = (int)prow;
-    b.f32 = b.splits > 1 || p.out.type == FB_F32;
-    if (b.splits > 1) {
+    b.f32 = b.splits > 1 || p.fold || p.out.type == FB_F32;
+    if (b.splits > 1 || p.fold) {
+      const int64_t rows = p.fold ? p.M / 2 : p.M;
       float *P = static_cast<float *>(c.take((size_t)(b.splits * prow * pld) * 4));
       if (!P) return fb::set_error(FB_ERR_ARG, "workspace too small");
-      sums.j[sums.n++] = SumJob{P, p.out.p, p.out.ld, pld, prow * pld, p.M, b.splits, p.N, p.out.accumulate,
-                                p.out.type == FB_BF16, ctas};
-      ctas += (unsigned)((p.M * p.N + kSumPerCta - 1) / kSumPerCta);
+      sums.j[sums.n++] = SumJob{P, p.out.p, p.out.ld, pld, prow * pld, rows, p.fold ? rows * pld : 0, b.splits, p.N,
+                                p.out.accumulate, p.out.type == FB_BF16, ctas};
+      ctas += (unsigned)((rows * p.N + kSumPerCta - 1) / kSumPerCta);
       b.has_tc = 1;
       if (!c.dry) FBH_TRY(make_map(&b.tc, P, b.splits * prow, p.N, pld, 32, true));
     } else if (!c.dry) {

@@ -54,7 +54,8 @@ namespace fbpair {
 
 using namespace fbtc;
 
-enum : int { kStore = 0, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6, kLsePlanes = 7, kProbPlanes = 8, kGluBwdLong = 9 };
+enum : int { kStore = 0, kGluFwd = 2, kGluBwd = 3, kLse = 4, kProb = 5, kLseLong = 6, kLsePlanes = 7, kProbPlanes = 8, kGluBwdLong = 9,
+              kProbTwo = 10 };
 using fbact::kGelu;
 using fbact::kRelu;
 using fbact::kSilu;
@@ -80,15 +81,15 @@ template <int EPI> __host__ __device__ constexpr int slab_of() {
   return EPI == kLseLong ? kLseSlab : (EPI == kGluBwdLong ? kGluSlab : 0);
 }
 template <int EPI> __host__ __device__ constexpr int out_bytes() {
-  return EPI == kGluBwd || EPI == kGluBwdLong ? 3 * kStageOut : (EPI == kLse || EPI == kLseLong ? 0 : kStageOut);
+  return EPI == kGluBwd || EPI == kGluBwdLong ? 3 * kStageOut : EPI == kProbTwo ? 2 * kStageOut : (EPI == kLse || EPI == kLseLong ? 0 : kStageOut);
 }
 template <int EPI, int P> __host__ __device__ constexpr int stages() {
-  return P == 3 ? 8 : (EPI == kGluBwd || EPI == kGluBwdLong ? 4 : (EPI == kProb ? 5 : 6));
+  return P == 3 ? 8 : (EPI == kGluBwd || EPI == kGluBwdLong ? 4 : (EPI == kProb || EPI == kProbTwo ? 5 : 6));
 }
 template <int EPI, int P> __host__ __device__ constexpr int smem_bytes() {
   return 1024 + stages<EPI, P>() * stage_bytes<P>() + epi_warps<EPI>() * out_bytes<EPI>() + 256;
 }
-static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kGluBwdLong, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 232448 &&
+static_assert(smem_bytes<kGluBwd, 1>() <= 232448 && smem_bytes<kGluBwdLong, 1>() <= 232448 && smem_bytes<kProbTwo, 1>() <= 232448 && smem_bytes<kProb, 1>() <= 232448 &&
                   smem_bytes<kStore, 1>() <= 232448 &&
                   smem_bytes<kStore, 3>() <= 232448 && smem_bytes<kProbPlanes, 3>() <= 232448, "shared memory exceeds 227 KB");
 
@@ -114,7 +115,7 @@ struct PairArgs {
   PairProb p[kMaxProbs];
   int n, tile0[kMaxProbs + 1];                // products; tiles before each
   int32_t *err;
-  CUtensorMap tw, tc2[2];                     // kGluBwd: Wd; outputs dg, du (kProbPlanes: G's planes 1, 2)
+  CUtensorMap tw, tc2[2];                     // kGluBwd: Wd; outputs dg, du (kProbPlanes: G's planes 1, 2; kProbTwo: its second part)
   int act;
   float2 *part;                               // kLse*: [M][2 nt] (kLseLong: [M][4 nt]) (max, sum of exp2) partials
   const int64_t *target;                      // kProb*
@@ -924,14 +925,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
           m = nm;
         }
         if (row + lane < b.M) a.part[(int64_t)(row + lane) * (2 * b.nt) + 2 * q.n + half] = make_float2(m, s);
-      } else if constexpr (EPI == kProb) {
+      } else if constexpr (EPI == kProb || EPI == kProbTwo) {
         constexpr float kLog2e = 1.44269504088896340736f;
         const int i0 = row + lane;
         const int64_t tg = i0 < b.M ? a.target[i0] : -1;
         const bool live = tg >= 0 && tg < a.V;
         const float z = live ? a.lse[i0] * kLog2e : 0.f, d = live ? a.dloss[i0] : 0.f;
         // G is rounded to bf16 as h, dg, du are (glu_block): dh and dw 0.0024 off in the 2-norm, 0.0017 with G in fp32
-        // (4,000 x 100, 16,700 nodes)
+        // (4,000 x 100, 16,700 nodes); kProbTwo keeps what the rounding leaves as a second bf16 part
         const uint32_t mask = live ? 0xFFFFFFFFu : 0u;            // a held-out row is zeros whatever its logits are
         const int64_t tc = live ? tg - a.v0 : -1;                 // the target's column of this piece
 #pragma unroll 1
@@ -951,15 +952,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of<EPI>(), 1
                 if (hit == i) r[i] = __float_as_uint(__uint_as_float(r[i]) - 1.f);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              w[i] = pack(__uint_as_float(r[2 * i]) * d, __uint_as_float(r[2 * i + 1]) * d) & mask;
+            for (int i = 0; i < 16; ++i) {
+              const float v0 = __uint_as_float(r[2 * i]) * d, v1 = __uint_as_float(r[2 * i + 1]) * d;
+              w[i] = pack(v0, v1) & mask;
+              if (EPI == kProbTwo)            // what the rounding left
+                r[i] = pack(v0 - __uint_as_float(w[i] << 16), v1 - __uint_as_float(w[i] & 0xFFFF0000u)) & mask;
+            }
             if (c == 0) {
               if (lane == 0) store_wait<0>(); // the block before has left the buffer
               __syncwarp();
             }
             stage_half(obuf, lane, c / 32, w);
+            if constexpr (EPI == kProbTwo) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = r[i];
+              stage_half(obuf + kStageOut, lane, c / 32, w);
+            }
           }
           send<false>(b, &b.tc, obuf, 0, row, q.n * 256 + c64, lane);
+          if (EPI == kProbTwo) send<false>(b, &a.tc2[0], obuf + kStageOut, 0, row, q.n * 256 + c64, lane);
         }
       }
       tc_fence_before();

@@ -182,6 +182,13 @@ bool few_tiles(const fb_softmax_xent &a) {
   return a.type == FB_F32 && a.D > 8 * fbpair::BK &&
          ((a.n + 255) / 256) * ((a.V + 127) / 128) * 4 <= fbtc::num_sms() / 2;
 }
+// bf16 gradients of few rows hang on few elements of G (the targets', near -1), whose rounding to bf16 would not average
+// out: 3 rows against 895 nodes of width 257 were 0.0033 off in the 2-norm, 0.0017 of it the gradients' own rounding.
+// While twice the rows still make one 256-row tile, G is kept as two bf16 parts, the second below the first, against h
+// laid out twice (dw) and with the halves of dh added at the end.
+// us, forward and backward, two parts / one, 16 rows: 100 x 10,000 32.9 / 30.4, 1,024 x 50,000 107 / 105; 128 rows:
+// 35.6 / 32.5, 122 / 112.  For more rows the products would cost twice, and the rounding of their more elements averages.
+bool two_parts(const fb_softmax_xent &a) { return a.type == FB_BF16 && a.n <= fbpair::kHalfM; }
 int stored_logits(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w, float *l, int64_t ldl) {
   const Product p = rows_product(h, a.n, a.D, w, false, (int)a.V, Out{l, ldl, FB_F32, 0});
   return products(c, &p, 1);
@@ -246,8 +253,9 @@ int forward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
 
 int backward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
   using namespace fbpair;
-  const bool f32 = a.type == FB_F32;
-  const int np = f32 ? 3 : 1;                 // planes of G
+  const bool f32 = a.type == FB_F32, two = two_parts(a);
+  const int np = f32 ? 3 : (two ? 2 : 1);     // planes of G; two: its parts one below the other
+  const int64_t gn = two ? 2 * a.n : a.n;     // rows of G (and of h) to the products
   const int64_t pr = piece_rows(a.n, a.V, 2 * np);
   const bool sum = !f32 && a.dh && pr < a.V;  // bf16 dh adds up over the pieces in fp32
   FBH_TAKE(G, c, uint16_t, np * a.n * pr);
@@ -282,13 +290,15 @@ int backward(Call &c, const fb_softmax_xent &a, const Mat &h, const Mat &w) {
       p.V = a.V;
       p.v0 = v0;
       for (int k = 0; k < np; ++k)
-        FBH_TRY(make_map(k == 0 ? &p.p[0].tc : &p.tc2[k - 1], G + k * Gm.plane, a.n, cols, pr, 32));
-      FBH_TRY(f32 ? (launch_pair<kProbPlanes, 3>(p, c.stream)) : (launch_pair<kProb>(p, c.stream)));
+        FBH_TRY(make_map(k == 0 ? &p.p[0].tc : &p.tc2[k - 1], G + k * a.n * pr, a.n, cols, pr, 32));
+      FBH_TRY(f32 ? (launch_pair<kProbPlanes, 3>(p, c.stream))
+                  : (two ? launch_pair<kProbTwo>(p, c.stream) : launch_pair<kProb>(p, c.stream)));
     }
     void *dw = a.dw ? static_cast<uint8_t *>(a.dw) + v0 * a.lddw * elem(a.grad_type) : nullptr;
     const Out dh = sum ? Out{acc, lds, FB_F32, v0 > 0} : Out{a.dh, a.lddh, a.type, f32 && v0 > 0};
-    const Product p[2] = {rows_product(Gm, a.n, cols, wp, true, a.D, dh),
-                          columns_product(Gm, a.n, cols, h, a.D, Out{dw, a.lddw, a.grad_type, a.accumulate})};
+    Product p[2] = {rows_product(Gm, gn, cols, wp, true, a.D, dh),
+                    columns_product(Gm, gn, cols, h, a.D, Out{dw, a.lddw, a.grad_type, a.accumulate})};
+    p[0].fold = two;
     FBH_TRY(products(c, p, 2));
     // dry: every piece takes the first one's workspace but the last, shorter one, which may split its sums differently
     if (c.dry && v0 == 0) v0 = std::max<int64_t>(0, (a.V - 1) / pr * pr - pr);
@@ -310,7 +320,7 @@ int run(Call &c, const fb_softmax_xent &a, bool bwd) {
   // that: 4,000 x 100 against 16,700 nodes, training, 141 us before that copy and 139 with it; 8,192 x 1,024 against
   // 50,000, 2.73 and 2.71 ms)
   Operand ops[2] = {{Mat{a.h, a.ldh}, a.n, a.D, &h}, {Mat{a.w, a.ldw}, a.V, a.D, &w}};
-  if (bwd && a.dw) ops[0].target = a.target, ops[0].V = a.V;
+  if (bwd && a.dw) ops[0].target = a.target, ops[0].V = a.V, ops[0].twice = two_parts(a);
   FBH_TRY(operands(c, a.type, ops, 2));
   return bwd ? backward(c, a, h, w) : forward(c, a, h, w);
 }

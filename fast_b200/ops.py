@@ -770,8 +770,8 @@ def softmax_xent_bwd(h, w, target, lse, dloss, dw=None, grad_dtype=None):
     """Gradients of softmax_xent_fwd for dloss [n] (fp32): (dh, dw), of the
     inputs' type (dw, a sum in fp32, as it is with grad_dtype=torch.float32);
     an fp32 buffer given as dw is accumulated into instead.  bf16 calls round
-    dloss * (softmax - onehot) to bf16 as an operand of both products (but for
-    one or two rows against large tables), fp32 calls do not."""
+    dloss * (softmax - onehot) to bf16 as an operand of both products (in calls
+    of more than 128 rows; fewer keep 16 bits of it), fp32 calls do not."""
     return _head_call(head_ops.softmax_xent_bwd,
                       lambda: (2 * h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 6 * h.numel() * w.shape[0]),
                       h, w, target, lse, dloss, dw, _grad_f32("softmax_xent_bwd", grad_dtype, h))

@@ -652,7 +652,7 @@ int fb_gated_ffn_bwd(const fb_gated_ffn *args, void *ws, size_t ws_bytes, cudaSt
  *   G_iv = dloss[i] (exp(l_iv - lse[i]) - [v == target[i]])
  *   dh = G w (rows' type),  dw = G^T h (grad_type; += when accumulate, fp32 only)
  * dh or dw may be NULL.  bf16: G is rounded to bf16 as an operand of both
- * products (few rows keep it in fp32).  Deterministic.
+ * products (calls of up to 128 rows keep 16 bits of it).  Deterministic.
  * ws: fb_softmax_xent_ws_bytes(args, backward) bytes, 16-byte aligned. */
 typedef struct fb_softmax_xent {
   int type, grad_type, accumulate, D;

@@ -204,3 +204,34 @@ def test_relu_turns_where_an_fp32_sum_of_bf16_rows_would(cuda, n, d, f):
     sure = G.abs() > 2.0 ** -9
     assert 0.5 < float(sure.double().mean()) < 1
     assert bool((dg[sure].double() == (G[sure] > 0).double()).all())
+
+
+# ---- few rows in bf16 ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,d,v,pad", [(2, 100, 600, 0), (3, 257, 895, 1), (7, 1670, 2207, 0), (17, 43, 58432, 3), (31, 64, 3000, 0),
+                                       (70, 378, 3259, 0), (127, 100, 1001, 4), (128, 1127, 1664, 0)])
+def test_few_bf16_rows_give_gradients_of_one_rounding(cuda, n, d, v, pad):
+    """With few rows the gradients hang on few elements of G (the targets'), whose rounding would not average out.  dh and
+    dw are then off by their own rounding alone: in the 2-norm 2^-8 / sqrt(3) at most, and 2^-12 for the rest."""
+    from fast_b200 import ops
+    for seed in range(4):
+        g = torch.Generator(device=cuda).manual_seed(1000 * seed + n)
+        h, w = _mat(cuda, g, n, d, BF, 1.0, pad), _mat(cuda, g, v, d, BF, 2 * d ** -0.5, pad)
+        t = torch.randint(0, v, (n,), device=cuda, generator=g)
+        if n > 2:
+            t[1] = -1
+            h[1] = math.nan
+        dl = torch.rand(n, device=cuda, generator=g) + 0.5
+        _, lse = ops.softmax_xent_fwd(h, w, t)
+        dh, dw = ops.softmax_xent_bwd(h, w, t, lse, dl)
+        H, W, keep = h.double().nan_to_num(0), w.double(), (t >= 0)
+        G = torch.softmax(H @ W.t(), 1)
+        G.scatter_add_(1, t.clamp(min=0)[:, None], torch.full((n, 1), -1.0, device=cuda, dtype=torch.float64))
+        G = G * (dl.double() * keep)[:, None]
+        for name, got, want in (("dh", dh, G @ W), ("dw", dw, G.t() @ H)):
+            off = float((got.double() - want).norm() / want.norm())
+            assert off <= 2.0 ** -8 / 3 ** 0.5 + 2.0 ** -12, (name, seed, off)
+        buf = torch.zeros(v, d, device=cuda)
+        dh2, _ = ops.softmax_xent_bwd(h, w, t, lse, dl, dw=buf)
+        assert torch.equal(dh, dh2)
+        off = float((buf.double() - G.t() @ H).norm() / (G.t() @ H).norm())
+        assert off <= 2.0 ** -12, (seed, off)                   # fp32 sums of h and G's two parts
