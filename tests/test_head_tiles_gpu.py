@@ -235,3 +235,8 @@ def test_few_bf16_rows_give_gradients_of_one_rounding(cuda, n, d, v, pad):
         assert torch.equal(dh, dh2)
         off = float((buf.double() - G.t() @ H).norm() / (G.t() @ H).norm())
         assert off <= 2.0 ** -12, (seed, off)                   # fp32 sums of h and G's two parts
+
+
+def test_few_bf16_rows_over_several_pieces_of_the_table(cuda):
+    softmax_xent(cuda, 128, 16, 1_200_000, 0, BF)               # 1,048,576 nodes a piece
+    torch.cuda.empty_cache()
