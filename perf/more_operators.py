@@ -436,7 +436,7 @@ def _own(s):
     if s["op"] == "scan":
         kw = dict(D=s["D"], z=s["z"], delta_bias=s["delta_bias"], starts=s["starts"], init=s["init"])
         args = s["u"], s["delta"], s["A"], s["B"], s["C"]
-        y, carry, final = ops.selective_scan_fwd(*args, final=s["init"] is not None, **kw)
+        y, carry, final = ops.selective_scan_fwd(*args, final=s["init"] is not None, keep=s["train"], **kw)
         out = {"y": y}
         if final is not None:
             out["final"] = final
