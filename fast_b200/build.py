@@ -4,6 +4,7 @@
   fast_b200/_ext/fastAgg.so       drop-in fastAgg module     (g++ + libtorch)
   fast_b200/_ext/sampler_core.so  drop-in sampler_core       (g++ + libtorch)
   fast_b200/_ext/head_ops.so      node-ranking head wrappers (g++ + libtorch)
+  fast_b200/_ext/history_ops.so   event-history wrappers     (g++ + libtorch)
 
 Every target is rebuilt only when one of its sources is newer.  nvcc
 cross-compiles for sm_100a, so this runs on machines without a GPU.
@@ -85,7 +86,7 @@ def _torch_flags():
 def build_shim(name, src, verbose=False):
     os.makedirs(EXT, exist_ok=True)
     out = os.path.join(EXT, name + ".so")
-    deps = [src, os.path.join(INC, "fast_b200.h"), LIB]
+    deps = [src, os.path.join(INC, "fast_b200.h"), LIB] + glob.glob(os.path.join(SHIM, "*.h"))
     if not _newer(out, deps):
         return out
     if verbose:
@@ -102,6 +103,7 @@ def build_all(verbose=False):
     build_shim("fastAgg", os.path.join(SHIM, "fastagg.cpp"), verbose)
     build_shim("sampler_core", os.path.join(SHIM, "sampler_core.cpp"), verbose)
     build_shim("head_ops", os.path.join(SHIM, "head_ops.cpp"), verbose)
+    build_shim("history_ops", os.path.join(SHIM, "history_ops.cpp"), verbose)
 
 
 if __name__ == "__main__":

@@ -199,6 +199,36 @@ for _n, _s in (("gated_ffn", GatedFfn), ("softmax_xent", SoftmaxXent)):
     _SIGS["fb_%s_ws_bytes" % _n] = (_SZ, [ctypes.POINTER(_s), _I])
     _SIGS["fb_%s_fwd" % _n] = _SIGS["fb_%s_bwd" % _n] = (_I, [ctypes.POINTER(_s), _P, _SZ, _P])
 
+
+class ShortConv(ctypes.Structure):
+    """fb_short_conv (include/fast_b200.h)."""
+    _fields_ = _fields("type:i act:i starts_type:i D:i K:i rows:q seqs:q starts", "x ldx:q w bias init final y ldy:q",
+                       "dy lddy:q dfinal dx lddx:q dw dbias dinit")
+
+
+class SelectiveScan(ctypes.Structure):
+    """fb_selective_scan (include/fast_b200.h)."""
+    _fields_ = _fields("type:i starts_type:i softplus:i D:i N:i G:i rows:q seqs:q starts",
+                       "u ldu:q delta ld_delta:q B ldb:q ldb_group:q C ldc:q ldc_group:q z ldz:q",
+                       "A skip delta_bias init keep final y ldy:q", "dy lddy:q dfinal du ddelta dz dB dC",
+                       "dA dD ddelta_bias dinit")
+
+
+class SelectiveScanEvent(ctypes.Structure):
+    """fb_selective_scan_event (include/fast_b200.h)."""
+    _fields_ = _fields("type:i softplus:i D:i N:i G:i n:q states:q index",
+                       "u ldu:q delta ld_delta:q B ldb:q ldb_group:q C ldc:q ldc_group:q z ldz:q",
+                       "A skip delta_bias state y ldy:q")
+
+
+for _n, _s in (("short_conv", ShortConv), ("selective_scan", SelectiveScan)):
+    _SIGS["fb_%s_ws_bytes" % _n] = (_SZ, [ctypes.POINTER(_s), _I])
+    _SIGS["fb_%s_fwd" % _n] = _SIGS["fb_%s_bwd" % _n] = (_I, [ctypes.POINTER(_s), _P, _SZ, _P])
+_SIGS["fb_event_step_ws_bytes"] = (_SZ, [_I64])
+_SIGS["fb_short_conv_step"] = (_I, [_I, _I, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I, _I, _P, _SZ, _P])
+_SIGS["fb_selective_scan_step"] = (_I, [ctypes.POINTER(SelectiveScanEvent), _P, _SZ, _P])
+_SIGS["fb_dropout"] = (_I, [_I, _P, _I64, _P, _I64, _P, _I64, _I64, _I, _F, _U64, _U64, _P, _P])
+
 for _name, (_res, _args) in _SIGS.items():
     _fn = getattr(lib, _name)
     _fn.restype = _res

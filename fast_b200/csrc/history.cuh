@@ -1,0 +1,179 @@
+// Packed histories: rows of several sequences one after the other.  Sequence s
+// takes rows starts[s] .. starts[s + 1] - 1; it may be empty.  Rows in front
+// of starts[0] and from starts[S] on belong to none.
+//
+// What the device holds in `starts` is not checked on the host.  Every index
+// made from it is clamped to the rows and sequences of the call, so values out
+// of order give wrong sums and no access out of range.
+#pragma once
+#include <cuda_bf16.h>
+#include "common.cuh"
+
+namespace fbq {
+
+using bf16 = __nv_bfloat16;
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<bf16>(bf16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16_rn(v); }
+
+// V elements of T as one aligned memory access.
+template <typename T, int V> struct alignas(sizeof(T) * V) Vec {
+  T e[V];
+};
+
+struct Starts {
+  const void *p;             // null: one sequence over all rows
+  int wide;                  // 64-bit entries
+  int64_t seqs, rows;
+  __device__ __forceinline__ int64_t operator[](int64_t s) const {
+    if (!p) return s > 0 ? rows : 0;
+    const int64_t v = wide ? static_cast<const int64_t *>(p)[s] : static_cast<const int32_t *>(p)[s];
+    return v < 0 ? 0 : (v > rows ? rows : v);
+  }
+};
+
+// Sequence of a row: the last s in [0, seqs] with starts[s] <= row; -1 in front
+// of them all, seqs behind them all.  The whole warp takes part; 32 probes a
+// round, so 1,024 sequences take two dependent loads.
+__device__ __forceinline__ int64_t owner(const Starts &st, int64_t row) {
+  if (!st.p) return row < 0 ? -1 : (row < st.rows ? 0 : 1);
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = st.seqs + 1;                    // starts[lo - 1] <= row < starts[hi]
+  while (hi > lo) {
+    const int64_t step = (hi - lo + 31) >> 5, i = lo + lane * step;
+    const int c = __popc(__ballot_sync(0xffffffffu, i < hi && st[i] <= row));
+    if (c == 0) break;
+    const int64_t next = lo + c * step;
+    lo = next - step + 1;
+    hi = next < hi ? next : hi;
+  }
+  return lo - 1;
+}
+
+// Walks the rows' boundaries upwards, kTile rows at a time.
+constexpr int kTile = 8;
+struct Walk {
+  Starts st;
+  int64_t next;              // first entry of starts that may lie behind the current tile's first row
+  int64_t first, last;       // rows of all sequences: [first, last)
+  __device__ __forceinline__ void begin(const Starts &s, int64_t row) {
+    st = s;
+    first = st[0], last = st[st.seqs];
+    next = owner(st, row - 1) + 1;
+  }
+  // Bit i: row r0 + i begins a sequence (or is the first behind the last one).
+  __device__ __forceinline__ unsigned tile(int64_t r0) {
+    unsigned bits = 0;
+    const int lane = threadIdx.x & 31;
+    if (!st.p) return (r0 == 0 ? 1u : 0u) | (st.rows >= r0 && st.rows < r0 + kTile ? 1u << (st.rows - r0) : 0u);
+    for (;;) {
+      const int64_t i = next + lane;
+      const int64_t b = i <= st.seqs ? st[i] : INT64_MAX;
+      const bool in = b < r0 + kTile;
+      bits |= __reduce_or_sync(0xffffffffu, in && b >= r0 ? 1u << (int)(b - r0) : 0u);
+      const int c = __popc(__ballot_sync(0xffffffffu, in));
+      next += c;
+      if (c < 32) return bits;
+    }
+  }
+};
+
+// The same, downwards: the first tile asked for holds row `top`, the next ones
+// lie 8 rows lower each.
+struct WalkDown {
+  Starts st;
+  int64_t next;              // last entry of starts that may lie in the next tile
+  __device__ __forceinline__ void begin(const Starts &s, int64_t top) {
+    st = s;
+    next = owner(st, top);
+  }
+  __device__ __forceinline__ unsigned tile(int64_t r0) {
+    if (!st.p) return r0 == 0 ? 1u : 0u;
+    unsigned bits = 0;
+    const int lane = threadIdx.x & 31;
+    for (;;) {
+      const int64_t i = next - lane;
+      const int64_t b = i >= 0 ? st[i] : -1;
+      const bool in = b >= r0;
+      bits |= __reduce_or_sync(0xffffffffu, in && b < r0 + kTile ? 1u << (int)(b - r0) : 0u);
+      const int c = __popc(__ballot_sync(0xffffffffu, in));
+      next -= c;
+      if (c < 32) return bits;
+    }
+  }
+};
+
+// ---- pairs of fp32 values, one instruction for both ------------------------------------------------
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 pack(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// ---- functions of one value ------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ F2 ex2_2(F2 x) {
+  const float2 f = unpack(x);
+  return pack(ex2(f.x), ex2(f.y));
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// log(1 + e^x) and its derivative, relative accuracy a few 2^-24 also where
+// they are small.  With e = e^-|x|: log(1 + e) = 2 artanh(s), s = e / (2 + e) <=
+// 1/3, and artanh(s) / s is a polynomial in s^2 (interpolated at Chebyshev
+// nodes of [0, 1/9], off by 4e-9).  The product |x| log2(e) is carried to two
+// words: its rounding alone would cost e 2^-24 |x|.
+__device__ __forceinline__ float softplus(float x, float &slope) {
+  const float m = fabsf(x), t = m * kLog2e;
+  const float lost = fmaf(m, kLog2e, -t) + m * 1.925963033500011e-8f;      // the rest of m log2(e)
+  float e = ex2(-t);
+  if (m < 88.f) e = fmaf(-0.6931472f * lost, e, e);
+  const float s = e * rcp(2.f + e), w = s * s;
+  float p = fmaf(w, 0.14078889787197113f, 0.13982579112052917f);
+  p = fmaf(w, p, 0.20012298226356506f);
+  p = fmaf(w, p, 0.3333316147327423f);
+  const float l = 2.f * fmaf(w * p, s, s), r = rcp(1.f + e);
+  slope = x >= 0.f ? r : e * r;
+  return x > 0.f ? x + l : (x <= 0.f ? l : x);                             // NaN stays NaN
+}
+
+// 1 / (1 + e^-x)
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
+
+}  // namespace fbq

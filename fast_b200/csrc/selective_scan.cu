@@ -1,0 +1,987 @@
+// Selective state space scan over packed histories, forward and backward.
+//
+//   dt = softplus(delta + delta_bias)   (or delta + delta_bias as it is)
+//   h[t] = exp(dt A) h[t-1] + dt u B[t]      per channel d and state n
+//   v = sum_n C[t] h[t] + D u,   y = v silu(z)
+//
+//   gv = dy silu(z),  dz = dy v silu'(z)
+//   g[t] = C gv + r[t],  r[t-1] = exp(dt A) g[t]      (r = dfinal behind a sequence)
+//   dC = sum_d gv h,  dB = sum_d g dt u,  du = dt <g, B> + D gv
+//   q = g exp(dt A) h[t-1] = r[t-1] h[t-1]
+//   ddelta = (<q, A> + u <g, B>) softplus',  dA = sum_t q dt,  dD = sum_t gv u
+//
+// What bounds it: one exponential for each (row, channel, state).  At 16 states
+// the special function units, 16 a clock and SM, need one clock for a (row,
+// channel) and pass; its bytes (8 in bf16, gate included) need 0.36 of a clock's
+// share of the memory.  So the layout serves the arithmetic:
+//
+// - A warp owns a tile of channels and walks down the rows.  A thread holds 4
+//   channels x 4 states (2 x 4 in the backward): what is read from shared memory
+//   per row (dt, dt u of its channels, B, C of its states) is used 4 times, and
+//   the sums over states (y) and over channels (dB, dC) take a few shuffles in
+//   which every lane ends up with a value of its own.  Channels sit in pairs,
+//   which the packed fp32 instructions take two at a time.
+// - Rows come in tiles of 8.  Their softplus, dt u and the gate are computed
+//   once for each (row, channel) with the lanes along the channels; the next
+//   tile's loads are in flight meanwhile.  Any pitch and alignment is the same.
+// - The packed rows are cut into chunks of a fixed number of rows wherever the
+//   sequences begin, so the grid needs nothing from the device.  A first pass
+//   reduces each chunk to its last state, from the last beginning of a sequence
+//   on (decay over the chunk: exp(A sum dt)), a second joins the chunks in
+//   order, the third computes the rows.  Sequences begin by assignment, never by
+//   a factor of 0: an infinity stays in its own sequence.  One chunk needs one
+//   launch.
+// - For a backward pass the forward keeps the state in front of every 8th row,
+//   2 N bytes a (row, channel): written beside arithmetic that leaves the memory
+//   idle, and cheaper than another pass of exponentials.  The backward
+//   recomputes 8 rows of states and decays into registers and walks them back.
+// - Sums over rows and channels end in per-CTA partials that one more launch
+//   adds in a fixed order: results repeat bit for bit.
+//
+// Everything between the loads and the stores is fp32.
+#include <algorithm>
+#include <cstring>
+#include "head.cuh"
+#include "history.cuh"
+
+namespace {
+using namespace fbq;
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kMaxStates = 64;
+
+struct ScanArgs {
+  int D, N, G, per, tiles, softplus;      // per: channels of a group; tiles: a group's tiles of channels
+  const void *u, *delta, *B, *C, *z, *dy;
+  int64_t ldu, ldd, ldb, gsb, ldc, gsc, ldz, lddy;
+  const float *A, *Ds, *bias, *init, *dfin;
+  float *fin, *dinit;
+  void *y, *du, *ddelta, *dz, *dB, *dC;
+  int64_t ldy;
+  float *keep;                            // [ceil(rows / 8), D, N] states in front of every 8th row
+  float *edge;                            // [nc - 1, D, N] what crosses the chunks' borders
+  float *sumdt;                           // [nc - 1, D]
+  int *cut;                               // [nc - 1] nothing passes through the chunk
+  float *pA, *pD, *pBC;                   // partial sums: [nc, D, N], [nc, 2, D], [G ctas, rows, 2 NP]
+  float *dA, *dD, *dbias;
+  Starts st;
+  int64_t chunk;                          // rows, a multiple of kTile
+  int nc, ctas;                           // chunks; CTAs side by side on a group (backward)
+  int vec;                                // states move four at a time
+};
+
+template <typename T> __device__ __forceinline__ T ld_el(const void *p, int64_t i) { return static_cast<const T *>(p)[i]; }
+
+// Four states from n0 on of one channel.
+__device__ __forceinline__ void load4(const float *p, int n0, int N, int vec, float (&v)[4]) {
+  if (vec) {
+    const float4 f = *reinterpret_cast<const float4 *>(p + n0);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = n0 + k < N ? p[n0 + k] : 0.f;
+}
+__device__ __forceinline__ void store4(float *p, int n0, int N, int vec, const float (&v)[4]) {
+  if (vec) {
+    *reinterpret_cast<float4 *>(p + n0) = make_float4(v[0], v[1], v[2], v[3]);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (n0 + k < N) p[n0 + k] = v[k];
+}
+
+// The states of a thread: P pairs of channels x 4 states.
+template <int P> struct States {
+  F2 v[P][4];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[p][k] = pack(0.f, 0.f);
+  }
+  // From / to [D, N] rows at `base`; c: channel (in the tensor) of the thread's first, `has` of them exist.
+  __device__ __forceinline__ void load(const float *base, int64_t c, int has, int n0, const ScanArgs &a) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      float x[2][4] = {};
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (2 * p + j < has && n0 < a.N) load4(base + (c + 2 * p + j) * a.N, n0, a.N, a.vec, x[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[p][k] = pack(x[0][k], x[1][k]);
+    }
+  }
+  __device__ __forceinline__ void store(float *base, int64_t c, int has, int n0, const ScanArgs &a) const {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      float x[2][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack(v[p][k]);
+        x[0][k] = f.x, x[1][k] = f.y;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (2 * p + j < has && n0 < a.N) store4(base + (c + 2 * p + j) * a.N, n0, a.N, a.vec, x[j]);
+    }
+  }
+};
+
+// Sums V values over L lanes that are STRIDE apart, each lane keeping max(1, V / L)
+// of the sums: v[0 ..], the first of them value number `at`.
+template <int V, int L, int STRIDE> __device__ __forceinline__ int spread_sum(float *v) {
+  if constexpr (L > 1) {
+    constexpr int kBit = STRIDE * L / 2;
+    if constexpr (V > 1) {
+      const bool up = (threadIdx.x & kBit) != 0;
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) {
+        const float send = up ? v[k] : v[k + V / 2], stay = up ? v[k + V / 2] : v[k];
+        v[k] = stay + __shfl_xor_sync(0xffffffffu, send, kBit);
+      }
+      return (up ? V / 2 : 0) + spread_sum<V / 2, L / 2, STRIDE>(v);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], kBit);
+      return spread_sum<1, L / 2, STRIDE>(v);
+    }
+  }
+  return 0;
+}
+
+// A thread's place: NP states (padded to 8, 16, 32 or 64) of P pairs of channels a thread.
+template <int NP, int P> struct Lay {
+  static constexpr int NL = NP / 4, CL = 32 / NL, CH = 2 * P * CL;       // lanes along states, channels; channels a warp
+  static constexpr int E = kTile * CH / 32, EB = kTile * NP / 32;        // a tile's elements a lane: rows x channels, rows x states
+  static constexpr int W = CH > 32 ? CH / 32 : 1;                        // channels a lane stages
+  static __device__ __forceinline__ int ch(int i) { return ((threadIdx.x & 31) + 32 * i) % CH; }
+  static __device__ __forceinline__ int row(int i) { return ((threadIdx.x & 31) + 32 * i) / CH; }
+};
+
+template <typename T, int NP> struct FwdSmem {
+  using L = Lay<NP, 2>;
+  float dt[kTile][L::CH], dtu[kTile][L::CH], y[kTile][L::CH];
+  float2 B[kTile][NP], C[kTile][NP];                                     // each value twice: a pair's factor
+};
+
+// The loads of one tile of rows for a warp, as they come: u, delta (or dy and the
+// gate), B and C.
+template <typename T, int E, int EB> struct Raw {
+  T x[E], d[E], b[EB], c[EB];
+};
+
+// Forward.  LOCAL: the chunk's last state alone, from the last beginning of a
+// sequence on, for all chunks but the last.
+template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThreads, 4) k_scan_fwd(ScanArgs a) {
+  using L = Lay<NP, 2>;
+  fb::pdl_enter();
+  __shared__ __align__(16) FwdSmem<T, NP> smem[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  FwdSmem<T, NP> &sm = smem[warp];
+  const int nct = a.G * a.tiles;
+  const int64_t wid = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t chunk = wid / nct;
+  const int ct = (int)(wid % nct);
+  if (chunk >= a.nc - (LOCAL ? 1 : 0)) return;
+  const int grp = ct / a.tiles, ch0 = (ct % a.tiles) * L::CH, left = a.per - ch0;   // channels the tile has
+  const int64_t cb = (int64_t)grp * a.per + ch0;
+  const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
+  const int64_t mine = cb + cl * 4;
+  const int has = left - cl * 4;
+  const int64_t rows = a.st.rows, c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, rows);
+
+  States<2> A2, h;
+  A2.load(a.A, mine, has, n0, a);
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], pack(kLog2e, kLog2e));
+  h.zero();
+
+  int64_t from = c0, lo = 0, hi = rows;           // first row; rows of sequences
+  Walk walk;
+  if constexpr (LOCAL) {
+    const int64_t s = owner(a.st, c1 - 1);
+    const bool in = s >= 0 && s < a.st.seqs;
+    const int64_t b = in ? a.st[s] : 0;
+    const bool ends = !in || a.st[s + 1] <= c1;   // nothing goes on into the next chunk
+    const bool cut = ends || b >= c0;
+    if (ct == 0 && lane == 0) a.cut[chunk] = cut;
+    if (ends) from = c1;
+    else if (b >= c0) {
+      from = b;
+      if (a.init) h.load(a.init + s * (int64_t)a.D * a.N, mine, has, n0, a);
+    }
+    lo = from, hi = c1;
+  } else {
+    walk.begin(a.st, c0);
+    lo = walk.first, hi = walk.last;
+    if (chunk > 0) h.load(a.edge + (chunk - 1) * (int64_t)a.D * a.N, mine, has, n0, a);
+  }
+
+  float bias[L::W], skip[L::W];
+#pragma unroll
+  for (int w = 0; w < L::W; ++w) {
+    const int c = L::ch(w);
+    bias[w] = a.bias && c < left ? a.bias[cb + c] : 0.f;
+    skip[w] = !LOCAL && a.Ds && c < left ? a.Ds[cb + c] : 0.f;
+  }
+  Raw<T, L::E, L::EB> raw;
+  const T none = from_f<T>(0.f);
+  const auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int i = 0; i < L::E; ++i) {
+      const int64_t r = r0 + L::row(i);
+      const int c = L::ch(i);
+      const bool in = c < left && r >= lo && r < hi && r < c1;
+      raw.x[i] = in ? ld_el<T>(a.u, r * a.ldu + cb + c) : none;
+      raw.d[i] = in ? ld_el<T>(a.delta, r * a.ldd + cb + c) : none;
+    }
+#pragma unroll
+    for (int i = 0; i < L::EB; ++i) {
+      const int n = (lane + 32 * i) % NP;
+      const int64_t r = r0 + (lane + 32 * i) / NP;
+      const bool in = n < a.N && r >= lo && r < hi && r < c1;
+      raw.b[i] = in ? ld_el<T>(a.B, r * a.ldb + grp * a.gsb + n) : none;
+      if (!LOCAL) raw.c[i] = in ? ld_el<T>(a.C, r * a.ldc + grp * a.gsc + n) : none;
+    }
+  };
+  // A sequence begins at `row`: the one before it leaves its last state.
+  const auto begin_at = [&](int64_t row) {
+    if (a.fin && row > c0) {
+      const int64_t s = owner(a.st, row - 1);
+      if (s >= 0 && s < a.st.seqs) h.store(a.fin + s * (int64_t)a.D * a.N, mine, has, n0, a);
+    }
+    h.zero();
+    if (a.init) {
+      const int64_t s = owner(a.st, row);
+      if (s >= 0 && s < a.st.seqs) h.load(a.init + s * (int64_t)a.D * a.N, mine, has, n0, a);
+    }
+  };
+
+  F2 total[2] = {pack(0.f, 0.f), pack(0.f, 0.f)};
+  int64_t r0 = c0 + (from - c0) / kTile * kTile;
+  if (r0 < c1) fetch(r0);
+  for (; r0 < c1; r0 += kTile) {
+    T ku[L::E], kz[L::E];
+    unsigned begins = 0;
+    if constexpr (!LOCAL) {
+      begins = walk.tile(r0);
+      if (c1 - r0 < kTile) begins &= (1u << (int)(c1 - r0)) - 1u;
+    }
+#pragma unroll
+    for (int i = 0; i < L::E; ++i) {
+      const int64_t r = r0 + L::row(i);
+      const int c = L::ch(i);
+      const bool in = r >= lo && r < hi && r < c1;
+      float slope;
+      float dt = to_f(raw.d[i]) + bias[i % L::W];
+      if (a.softplus) dt = softplus(dt, slope);
+      if (!in) dt = 0.f;
+      sm.dt[L::row(i)][c] = dt;
+      sm.dtu[L::row(i)][c] = dt * to_f(raw.x[i]);
+      if constexpr (!LOCAL) {
+        ku[i] = raw.x[i];
+        kz[i] = a.z && in && c < left ? ld_el<T>(a.z, r * a.ldz + cb + c) : none;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < L::EB; ++i) {
+      const int at = lane + 32 * i;
+      const float b = to_f(raw.b[i]);
+      sm.B[at / NP][at % NP] = make_float2(b, b);
+      if constexpr (!LOCAL) {
+        const float c = to_f(raw.c[i]);
+        sm.C[at / NP][at % NP] = make_float2(c, c);
+      }
+    }
+    if (r0 + kTile < c1) fetch(r0 + kTile);
+    __syncwarp();
+    if (!LOCAL && a.keep) h.store(a.keep + r0 / kTile * (int64_t)a.D * a.N, mine, has, n0, a);
+#pragma unroll
+    for (int i = 0; i < kTile; ++i) {
+      if (!LOCAL && (begins >> i & 1u)) begin_at(r0 + i);
+      F2 dt[2], dtu[2], B[4], C[4], y[2];
+      {
+        const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(&sm.dt[i][cl * 4]);
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&sm.dtu[i][cl * 4]);
+        const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
+        dt[0].v = t.x, dt[1].v = t.y, dtu[0].v = x.x, dtu[1].v = x.y;
+        B[0].v = b[0].x, B[1].v = b[0].y, B[2].v = b[1].x, B[3].v = b[1].y;
+        if constexpr (!LOCAL) {
+          const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(&sm.C[i][n0]);
+          C[0].v = c[0].x, C[1].v = c[0].y, C[2].v = c[1].x, C[3].v = c[1].y;
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const F2 decay = ex2_2(mul2(dt[p], A2.v[p][k]));
+          h.v[p][k] = fma2(decay, h.v[p][k], mul2(dtu[p], B[k]));
+          if constexpr (!LOCAL) y[p] = k == 0 ? mul2(C[k], h.v[p][k]) : fma2(C[k], h.v[p][k], y[p]);
+        }
+        if constexpr (LOCAL) total[p] = add2(total[p], dt[p]);
+      }
+      if constexpr (!LOCAL) {
+        const float2 ya = unpack(y[0]), yb = unpack(y[1]);
+        float v[4] = {ya.x, ya.y, yb.x, yb.y};
+        const int at = spread_sum<4, L::NL, 1>(v);
+        constexpr int kOwn = L::NL >= 4 ? 1 : 4 / L::NL;
+        if (L::NL <= 4 || nl % (L::NL / 4 > 0 ? L::NL / 4 : 1) == 0) {
+#pragma unroll
+          for (int k = 0; k < kOwn; ++k) sm.y[i][cl * 4 + at + k] = v[k];
+        }
+      }
+    }
+    __syncwarp();
+    if constexpr (!LOCAL) {
+#pragma unroll
+      for (int i = 0; i < L::E; ++i) {
+        const int64_t r = r0 + L::row(i);
+        const int c = L::ch(i);
+        if (r < c1 && c < left) {
+          float v = fmaf(skip[i % L::W], to_f(ku[i]), sm.y[L::row(i)][c]);
+          if (a.z) {
+            const float z = to_f(kz[i]);
+            v *= z * sigmoid(z);
+          }
+          static_cast<T *>(a.y)[r * a.ldy + cb + c] = from_f<T>(r >= lo && r < hi ? v : 0.f);
+        }
+      }
+    }
+  }
+  if constexpr (LOCAL) {
+    __syncwarp();
+    h.store(a.edge + chunk * (int64_t)a.D * a.N, mine, has, n0, a);
+    if (nl == 0) {
+      const float2 x = unpack(total[0]), y = unpack(total[1]);
+      const float t[4] = {x.x, x.y, y.x, y.y};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < has) a.sumdt[chunk * a.D + mine + j] = t[j];
+    }
+  } else if (a.fin) {
+    const int64_t s = owner(a.st, c1 - 1);
+    if (s >= 0 && s < a.st.seqs && a.st[s + 1] <= c1) h.store(a.fin + s * (int64_t)a.D * a.N, mine, has, n0, a);
+    for (int64_t q = chunk; q < a.st.seqs; q += 32 * (int64_t)a.nc) {          // empty sequences end as they began
+      const int64_t e = q + lane * (int64_t)a.nc;
+      unsigned m = __ballot_sync(0xffffffffu, e < a.st.seqs && a.st[e] >= a.st[e + 1]);
+      for (; m; m &= m - 1) {
+        const int64_t s0 = q + (__ffs(m) - 1) * (int64_t)a.nc;
+        States<2> x;
+        x.zero();
+        if (a.init) x.load(a.init + s0 * (int64_t)a.D * a.N, mine, has, n0, a);
+        x.store(a.fin + s0 * (int64_t)a.D * a.N, mine, has, n0, a);
+      }
+    }
+  }
+}
+
+// Joins the chunks: edge[c], what chunk c alone leaves, becomes what arrives
+// behind it (REV: in front of chunk c + 1, from the rows behind).
+template <bool REV> __global__ void __launch_bounds__(256) k_scan_join(ScanArgs a) {
+  fb::pdl_enter();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, size = (int64_t)a.D * a.N;
+  if (i >= size) return;
+  const int c = (int)(i / a.N);
+  const float A2 = a.A[i] * kLog2e;
+  constexpr int kAhead = 8;
+  const int n = a.nc - 1;
+  float x = 0.f;
+  for (int at = 0; at < n; at += kAhead) {
+    float local[kAhead], sum[kAhead];
+    int cut[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int j = at + k < n ? (REV ? n - 1 - (at + k) : at + k) : 0;
+      local[k] = a.edge[j * size + i], sum[k] = a.sumdt[(int64_t)j * a.D + c], cut[k] = a.cut[j];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (at + k < n) {
+        x = cut[k] ? local[k] : fmaf(ex2(A2 * sum[k]), x, local[k]);
+        a.edge[(REV ? n - 1 - (at + k) : at + k) * size + i] = x;
+      }
+  }
+}
+
+// ---- backward ------------------------------------------------------------------------------------
+template <typename T, int NP> struct RevSmem {
+  using L = Lay<NP, 2>;
+  float dt[kTile][L::CH], gv[kTile][L::CH];
+  float2 C[kTile][NP];
+};
+
+// What chunk c (all but the first) sends up to the chunk in front of it: r in
+// front of its first row, from the rows of the sequence that comes in.
+template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_scan_rev(ScanArgs a) {
+  using L = Lay<NP, 2>;
+  fb::pdl_enter();
+  __shared__ __align__(16) RevSmem<T, NP> smem[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  RevSmem<T, NP> &sm = smem[warp];
+  const int nct = a.G * a.tiles;
+  const int64_t wid = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t chunk = wid / nct + 1;
+  const int ct = (int)(wid % nct);
+  if (chunk >= a.nc) return;
+  const int grp = ct / a.tiles, ch0 = (ct % a.tiles) * L::CH, left = a.per - ch0;
+  const int64_t cb = (int64_t)grp * a.per + ch0;
+  const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
+  const int64_t mine = cb + cl * 4;
+  const int has = left - cl * 4;
+  const int64_t rows = a.st.rows, c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, rows);
+
+  States<2> A2, r;
+  A2.load(a.A, mine, has, n0, a);
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], pack(kLog2e, kLog2e));
+  r.zero();
+  const int64_t s = owner(a.st, c0);
+  const bool in = s >= 0 && s < a.st.seqs && a.st[s] < c0;      // a sequence comes in
+  const int64_t end = in ? a.st[s + 1] : c0, e = min(end, c1);
+  if (ct == 0 && lane == 0) a.cut[chunk - 1] = !in || end <= c1;
+  if (in && end <= c1 && a.dfin) r.load(a.dfin + s * (int64_t)a.D * a.N, mine, has, n0, a);
+
+  float bias[L::W];
+#pragma unroll
+  for (int w = 0; w < L::W; ++w) bias[w] = a.bias && L::ch(w) < left ? a.bias[cb + L::ch(w)] : 0.f;
+  const T none = from_f<T>(0.f);
+  T xd[L::E], xy[L::E], xz[L::E], xc[L::EB];
+  const auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int i = 0; i < L::E; ++i) {
+      const int64_t q = r0 + L::row(i);
+      const int c = L::ch(i);
+      const bool ok = c < left && q < e;
+      xd[i] = ok ? ld_el<T>(a.delta, q * a.ldd + cb + c) : none;
+      xy[i] = ok ? ld_el<T>(a.dy, q * a.lddy + cb + c) : none;
+      xz[i] = ok && a.z ? ld_el<T>(a.z, q * a.ldz + cb + c) : none;
+    }
+#pragma unroll
+    for (int i = 0; i < L::EB; ++i) {
+      const int n = (lane + 32 * i) % NP;
+      const int64_t q = r0 + (lane + 32 * i) / NP;
+      xc[i] = n < a.N && q < e ? ld_el<T>(a.C, q * a.ldc + grp * a.gsc + n) : none;
+    }
+  };
+  F2 total[2] = {pack(0.f, 0.f), pack(0.f, 0.f)};
+  int64_t r0 = e > c0 ? c0 + (e - 1 - c0) / kTile * kTile : c0 - kTile;
+  if (r0 >= c0) fetch(r0);
+  for (; r0 >= c0; r0 -= kTile) {
+#pragma unroll
+    for (int i = 0; i < L::E; ++i) {
+      const bool ok = r0 + L::row(i) < e;
+      float slope, dt = to_f(xd[i]) + bias[i % L::W], gv = to_f(xy[i]);
+      if (a.softplus) dt = softplus(dt, slope);
+      if (a.z) {
+        const float z = to_f(xz[i]);
+        gv *= z * sigmoid(z);
+      }
+      sm.dt[L::row(i)][L::ch(i)] = ok ? dt : 0.f;
+      sm.gv[L::row(i)][L::ch(i)] = ok ? gv : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < L::EB; ++i) {
+      const int at = lane + 32 * i;
+      const float c = to_f(xc[i]);
+      sm.C[at / NP][at % NP] = make_float2(c, c);
+    }
+    if (r0 - kTile >= c0) fetch(r0 - kTile);
+    __syncwarp();
+#pragma unroll
+    for (int i = kTile - 1; i >= 0; --i) {
+      const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(&sm.dt[i][cl * 4]);
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&sm.gv[i][cl * 4]);
+      const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(&sm.C[i][n0]);
+      const F2 dt[2] = {{t.x}, {t.y}}, gv[2] = {{x.x}, {x.y}}, C[4] = {{c[0].x}, {c[0].y}, {c[1].x}, {c[1].y}};
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          r.v[p][k] = mul2(ex2_2(mul2(dt[p], A2.v[p][k])), fma2(C[k], gv[p], r.v[p][k]));
+        total[p] = add2(total[p], dt[p]);
+      }
+    }
+    __syncwarp();
+  }
+  r.store(a.edge + (chunk - 1) * (int64_t)a.D * a.N, mine, has, n0, a);
+  if (nl == 0) {
+    const float2 x = unpack(total[0]), y = unpack(total[1]);
+    const float t[4] = {x.x, x.y, y.x, y.y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < has) a.sumdt[(chunk - 1) * a.D + mine + j] = t[j];
+  }
+}
+
+template <typename T, int NP> struct BwdSmem {
+  using L = Lay<NP, 1>;
+  float dt[kWarps][kTile][L::CH], dtu[kWarps][kTile][L::CH], gv[kWarps][kTile][L::CH];
+  float out[kWarps][3][kTile][L::CH];                            // <g, B>, <q, A log2 e>, <C, h>
+  float2 B[kTile][NP], C[kTile][NP];
+  float sum[kWarps][kTile][2 * NP];                              // the warps' sums over channels: dB, dC
+};
+
+// All gradients of a chunk's rows.  The warps of a CTA stand side by side on a
+// group's channels and add up their parts of dB and dC tile by tile.
+template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_scan_bwd(ScanArgs a) {
+  using L = Lay<NP, 1>;
+  fb::pdl_enter();
+  extern __shared__ __align__(16) unsigned char dyn[];
+  BwdSmem<T, NP> &sm = *reinterpret_cast<BwdSmem<T, NP> *>(dyn);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int grp = blockIdx.x / a.ctas, cta = blockIdx.x % a.ctas;
+  const int64_t chunk = blockIdx.y;
+  const int ch0 = (cta * kWarps + warp) * L::CH, left = a.per - ch0;        // may be <= 0: a warp without channels
+  const int64_t cb = (int64_t)grp * a.per + ch0;
+  const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
+  const int64_t mine = cb + cl * 2;
+  const int has = left - cl * 2;
+  const int64_t rows = a.st.rows, c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, rows);
+  const int64_t first = a.st[0], last = a.st[a.st.seqs], size = (int64_t)a.D * a.N;
+
+  States<1> A2, r, dA;
+  A2.load(a.A, mine, has, n0, a);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) A2.v[0][k] = mul2(A2.v[0][k], pack(kLog2e, kLog2e));
+  dA.zero();
+  // r behind `row`, the last of its sequence
+  const auto behind = [&](int64_t row) {
+    r.zero();
+    if (a.dfin) {
+      const int64_t s = owner(a.st, row);
+      if (s >= 0 && s < a.st.seqs) r.load(a.dfin + s * size, mine, has, n0, a);
+    }
+  };
+  {
+    const int64_t s = owner(a.st, c1 - 1);
+    if (c1 >= rows || s < 0 || s >= a.st.seqs || a.st[s + 1] <= c1) behind(c1 - 1);
+    else r.load(a.edge + chunk * size, mine, has, n0, a);
+  }
+
+  float bias[L::W], skip[L::W], sumD[L::W] = {}, sumb[L::W] = {};
+#pragma unroll
+  for (int w = 0; w < L::W; ++w) {
+    const int c = L::ch(w);
+    bias[w] = a.bias && c < left ? a.bias[cb + c] : 0.f;
+    skip[w] = a.Ds && c < left ? a.Ds[cb + c] : 0.f;
+  }
+  const T none = from_f<T>(0.f);
+  constexpr int EC = kTile * NP / kThreads > 0 ? kTile * NP / kThreads : 1;  // B (and C) elements a thread of the CTA
+  T xu[L::E], xd[L::E], xy[L::E], xz[L::E], xb[EC], xc[EC];
+  const auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int i = 0; i < L::E; ++i) {
+      const int64_t q = r0 + L::row(i);
+      const int c = L::ch(i);
+      const bool ok = c < left && q >= first && q < last && q < c1;
+      xu[i] = ok ? ld_el<T>(a.u, q * a.ldu + cb + c) : none;
+      xd[i] = ok ? ld_el<T>(a.delta, q * a.ldd + cb + c) : none;
+      xy[i] = ok ? ld_el<T>(a.dy, q * a.lddy + cb + c) : none;
+      xz[i] = ok && a.z ? ld_el<T>(a.z, q * a.ldz + cb + c) : none;
+    }
+#pragma unroll
+    for (int i = 0; i < EC; ++i) {
+      const int at = threadIdx.x + kThreads * i, n = at % NP;
+      const int64_t q = r0 + at / NP;
+      const bool ok = at < kTile * NP && n < a.N && q >= first && q < last && q < c1;
+      xb[i] = ok ? ld_el<T>(a.B, q * a.ldb + grp * a.gsb + n) : none;
+      xc[i] = ok ? ld_el<T>(a.C, q * a.ldc + grp * a.gsc + n) : none;
+    }
+  };
+
+  int64_t r0 = c0 + (c1 - 1 - c0) / kTile * kTile;
+  WalkDown walk;
+  walk.begin(a.st, c1 - 1);
+  fetch(r0);
+  for (; r0 >= c0; r0 -= kTile) {
+    // ---- the tile's rows, once for each (row, channel)
+    float ku[L::E], ky[L::E], kz[L::E], kdt[L::E], ksl[L::E];
+#pragma unroll
+    for (int i = 0; i < L::E; ++i) {
+      const int64_t q = r0 + L::row(i);
+      const bool ok = q >= first && q < last && q < c1;
+      float slope = 1.f, dt = to_f(xd[i]) + bias[i % L::W], gv = to_f(xy[i]);
+      if (a.softplus) dt = softplus(dt, slope);
+      ku[i] = to_f(xu[i]), ky[i] = gv, kz[i] = to_f(xz[i]), ksl[i] = slope;
+      if (a.z) gv *= kz[i] * sigmoid(kz[i]);
+      if (!ok) dt = 0.f;
+      kdt[i] = dt;
+      sm.dt[warp][L::row(i)][L::ch(i)] = dt;
+      sm.dtu[warp][L::row(i)][L::ch(i)] = dt * ku[i];
+      sm.gv[warp][L::row(i)][L::ch(i)] = gv;
+    }
+#pragma unroll
+    for (int i = 0; i < EC; ++i) {
+      const int at = threadIdx.x + kThreads * i;
+      if (at < kTile * NP) {
+        const float b = to_f(xb[i]), c = to_f(xc[i]);
+        sm.B[at / NP][at % NP] = make_float2(b, b);
+        sm.C[at / NP][at % NP] = make_float2(c, c);
+      }
+    }
+    const unsigned begins = walk.tile(r0);
+    States<1> h0, h;
+    h0.load(a.keep + r0 / kTile * size, mine, has, n0, a);
+    if (r0 - kTile >= c0) fetch(r0 - kTile);
+    __syncthreads();
+
+    // ---- states and decays of the 8 rows
+    F2 hs[kTile][4], as[kTile][4];
+    // What a sequence that begins at `row` finds.
+    const auto found = [&](States<1> &x, int64_t row) {
+      x.zero();
+      if (a.init) {
+        const int64_t s = owner(a.st, row);
+        if (s >= 0 && s < a.st.seqs) x.load(a.init + s * size, mine, has, n0, a);
+      }
+    };
+    h = h0;
+#pragma unroll
+    for (int i = 0; i < kTile; ++i) {
+      if (begins >> i & 1u) found(h, r0 + i);
+      const F2 dt = {*reinterpret_cast<const unsigned long long *>(&sm.dt[warp][i][cl * 2])};
+      const F2 dtu = {*reinterpret_cast<const unsigned long long *>(&sm.dtu[warp][i][cl * 2])};
+      const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
+      const F2 B[4] = {{b[0].x}, {b[0].y}, {b[1].x}, {b[1].y}};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        as[i][k] = ex2_2(mul2(dt, A2.v[0][k]));
+        h.v[0][k] = fma2(as[i][k], h.v[0][k], mul2(dtu, B[k]));
+        hs[i][k] = h.v[0][k];
+      }
+    }
+    // ---- back up the rows
+#pragma unroll
+    for (int i = kTile - 1; i >= 0; --i) {
+      const F2 dt = {*reinterpret_cast<const unsigned long long *>(&sm.dt[warp][i][cl * 2])};
+      const F2 dtu = {*reinterpret_cast<const unsigned long long *>(&sm.dtu[warp][i][cl * 2])};
+      const F2 gv = {*reinterpret_cast<const unsigned long long *>(&sm.gv[warp][i][cl * 2])};
+      const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
+      const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(&sm.C[i][n0]);
+      const F2 B[4] = {{b[0].x}, {b[0].y}, {b[1].x}, {b[1].y}}, C[4] = {{c[0].x}, {c[0].y}, {c[1].x}, {c[1].y}};
+      States<1> before;
+      if (begins >> i & 1u) {
+        found(before, r0 + i);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) before.v[0][k] = i ? hs[i - 1][k] : h0.v[0][k];
+      }
+      F2 gB, qA, cy;
+      float bc[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const F2 g = fma2(C[k], gv, r.v[0][k]);
+        r.v[0][k] = mul2(as[i][k], g);
+        const F2 q = mul2(r.v[0][k], before.v[0][k]);
+        gB = k == 0 ? mul2(g, B[k]) : fma2(g, B[k], gB);
+        qA = k == 0 ? mul2(q, A2.v[0][k]) : fma2(q, A2.v[0][k], qA);
+        cy = k == 0 ? mul2(C[k], hs[i][k]) : fma2(C[k], hs[i][k], cy);
+        dA.v[0][k] = fma2(q, dt, dA.v[0][k]);
+        const float2 vb = unpack(mul2(g, dtu)), vc = unpack(mul2(gv, hs[i][k]));
+        bc[k] = vb.x + vb.y, bc[4 + k] = vc.x + vc.y;
+      }
+      const float2 vg = unpack(gB), vq = unpack(qA), vy = unpack(cy);
+      float s4[4] = {vg.x, vg.y, vq.x, vq.y}, s2[2] = {vy.x, vy.y};
+      const int at4 = spread_sum<4, L::NL, 1>(s4), at2 = spread_sum<2, L::NL, 1>(s2);
+      constexpr int kOwn4 = L::NL >= 4 ? 1 : 4 / L::NL, kOwn2 = L::NL >= 2 ? 1 : 2;
+#pragma unroll
+      for (int k = 0; k < kOwn4; ++k) sm.out[warp][(at4 + k) >> 1][i][cl * 2 + ((at4 + k) & 1)] = s4[k];
+#pragma unroll
+      for (int k = 0; k < kOwn2; ++k) sm.out[warp][2][i][cl * 2 + at2 + k] = s2[k];
+      const int atc = spread_sum<8, L::CL, L::NL>(bc);
+      constexpr int kOwnC = L::CL >= 8 ? 1 : 8 / L::CL;
+#pragma unroll
+      for (int k = 0; k < kOwnC; ++k) sm.sum[warp][i][((atc + k) >> 2) * NP + n0 + ((atc + k) & 3)] = bc[k];
+      if (begins >> i & 1u) {
+        if (a.dinit) {
+          const int64_t s = owner(a.st, r0 + i);
+          if (s >= 0 && s < a.st.seqs) r.store(a.dinit + s * size, mine, has, n0, a);
+        }
+        behind(r0 + i - 1);
+      }
+    }
+    __syncthreads();
+
+    // ---- results of the tile
+#pragma unroll
+    for (int i = 0; i < L::E; ++i) {
+      const int row = L::row(i), c = L::ch(i), w = i % L::W;
+      const int64_t q = r0 + row;
+      if (q >= c1 || c >= left) continue;
+      const bool ok = q >= first && q < last;
+      const float gB = sm.out[warp][0][row][c], qA = sm.out[warp][1][row][c] * 0.6931471805599453f;
+      float gv = ky[i];
+      if (a.z) {
+        const float sg = sigmoid(kz[i]), v = fmaf(skip[w], ku[i], sm.out[warp][2][row][c]);
+        gv *= kz[i] * sg;
+        const float dz = ky[i] * v * sg * fmaf(kz[i], 1.f - sg, 1.f);
+        static_cast<T *>(a.dz)[q * a.D + cb + c] = from_f<T>(ok ? dz : 0.f);
+      }
+      const float dd = fmaf(ku[i], gB, qA) * ksl[i];
+      static_cast<T *>(a.du)[q * a.D + cb + c] = from_f<T>(ok ? fmaf(kdt[i], gB, skip[w] * gv) : 0.f);
+      static_cast<T *>(a.ddelta)[q * a.D + cb + c] = from_f<T>(ok ? dd : 0.f);
+      if (ok) sumD[w] = fmaf(gv, ku[i], sumD[w]), sumb[w] += dd;
+    }
+    for (int at = threadIdx.x; at < kTile * 2 * NP; at += kThreads) {
+      const int row = at / (2 * NP), col = at % (2 * NP);
+      const int64_t q = r0 + row;
+      if (q >= c1) break;
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) v += sm.sum[w][row][col];
+      if (a.ctas > 1) {
+        a.pBC[(blockIdx.x * rows + q) * (2 * NP) + col] = v;
+      } else if (col % NP < a.N) {
+        static_cast<T *>(col < NP ? a.dB : a.dC)[(q * a.G + grp) * a.N + col % NP] = from_f<T>(v);
+      }
+    }
+  }
+
+  dA.store((a.nc > 1 ? a.pA + chunk * size : a.dA), mine, has, n0, a);
+#pragma unroll
+  for (int w = 0; w < L::W; ++w) {
+    if (L::CH < 32) {
+#pragma unroll
+      for (int o = L::CH; o < 32; o <<= 1) {
+        sumD[w] += __shfl_xor_sync(0xffffffffu, sumD[w], o);
+        sumb[w] += __shfl_xor_sync(0xffffffffu, sumb[w], o);
+      }
+    }
+    const int c = L::ch(w);
+    if (c < left && lane < L::CH) {
+      if (a.nc > 1) a.pD[(chunk * 2) * a.D + cb + c] = sumD[w], a.pD[(chunk * 2 + 1) * a.D + cb + c] = sumb[w];
+      else a.dD[cb + c] = sumD[w], a.dbias[cb + c] = sumb[w];
+    }
+  }
+  if (a.dinit) {
+    for (int64_t q = chunk; q < a.st.seqs; q += 32 * (int64_t)a.nc) {          // empty sequences: dfinal passes through
+      const int64_t e = q + lane * (int64_t)a.nc;
+      unsigned m = __ballot_sync(0xffffffffu, e < a.st.seqs && a.st[e] >= a.st[e + 1]);
+      for (; m; m &= m - 1) {
+        const int64_t s0 = q + (__ffs(m) - 1) * (int64_t)a.nc;
+        States<1> x;
+        x.zero();
+        if (a.dfin) x.load(a.dfin + s0 * size, mine, has, n0, a);
+        x.store(a.dinit + s0 * size, mine, has, n0, a);
+      }
+    }
+  }
+}
+
+// Adds the partials in order: first the CTAs side by side (dB, dC; blocks below
+// bc_blocks), then the chunks (dA, dD, ddelta_bias).
+template <typename T> __global__ void __launch_bounds__(256) k_scan_sums(ScanArgs a, int NP, int64_t bc_blocks) {
+  fb::pdl_enter();
+  const int64_t rows = a.st.rows;
+  if (blockIdx.x < bc_blocks) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;               // [G, rows, 2 NP]
+    const int64_t width = rows * 2 * NP;
+    if (i >= width * a.G) return;
+    const int grp = (int)(i / width), col = (int)(i % (2 * NP));
+    const int64_t q = i % width / (2 * NP);
+    const float *p = a.pBC + grp * a.ctas * width + i % width;
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < a.ctas; ++k) v += p[k * width];
+    if (col % NP < a.N) static_cast<T *>(col < NP ? a.dB : a.dC)[(q * a.G + grp) * a.N + col % NP] = from_f<T>(v);
+    return;
+  }
+  const int64_t i = (blockIdx.x - bc_blocks) * 256 + threadIdx.x, size = (int64_t)a.D * a.N;
+  if (i < size) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < a.nc; ++k) v += a.pA[k * size + i];
+    a.dA[i] = v;
+  } else if (i < size + 2 * (int64_t)a.D) {
+    const int64_t j = i - size;
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < a.nc; ++k) v += a.pD[k * 2 * (int64_t)a.D + j];
+    if (j < a.D) a.dD[j] = v;
+    else a.dbias[j - a.D] = v;
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+int padded(int N) { return N <= 8 ? 8 : (N <= 16 ? 16 : (N <= 32 ? 32 : 64)); }
+
+// Rows of a chunk: enough warps to fill the SMs (kBusy of them), but no chunk
+// below kShort rows.
+int64_t chunk_rows(int64_t rows, int64_t tiles, int64_t busy, int64_t shortest) {
+  const int64_t want = std::max<int64_t>(1, busy / std::max<int64_t>(1, tiles));
+  int64_t c = (rows + want - 1) / want;
+  c = std::max(c, shortest);
+  return (c + kTile - 1) / kTile * kTile;
+}
+
+int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
+  const char *const who = "selective_scan";
+  if (!s) return fb::set_error(FB_ERR_ARG, "selective_scan: no arguments");
+  const auto bad = [&](const char *what) { return fb::set_error(FB_ERR_ARG, std::string(who) + ": " + what); };
+  if (s->type != FB_F32 && s->type != FB_BF16) return bad("unknown element type");
+  if (s->rows < 0 || s->D < 1 || s->N < 1 || s->G < 1 || s->D % s->G || s->seqs < 0) return bad("bad sizes");
+  if (!s->starts && s->seqs != 1) return bad("without starts there is one sequence");
+  if (s->starts_type != FB_I32 && s->starts_type != FB_I64) return bad("unknown type of starts");
+  if (s->N > kMaxStates) return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan: at most 64 states");
+  if (s->D > (1 << 20) || s->rows > (int64_t)1 << 40 || s->seqs > (int64_t)1 << 40)
+    return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan: sizes beyond what the kernels index");
+  if (s->rows && (!s->u || !s->delta || !s->B || !s->C)) return bad("missing operand");
+  if (!s->A) return bad("missing operand");
+  if (s->rows > 1 && (s->ldu < s->D || s->ld_delta < s->D || (s->z && s->ldz < s->D))) return bad("leading dimension below the width");
+  if (s->rows && !backward && (!s->y || (s->rows > 1 && s->ldy < s->D))) return bad("missing or overlapping output");
+  if (backward) {
+    if (s->rows && (!s->dy || (s->rows > 1 && s->lddy < s->D) || !s->keep)) return bad("missing operand of the backward pass");
+    if (s->rows && (!s->du || !s->ddelta || !s->dB || !s->dC || (s->z && !s->dz))) return bad("missing gradient");
+    if (!s->dA || !s->dD || !s->ddelta_bias) return bad("missing gradient");
+  }
+  a = ScanArgs{};
+  a.D = s->D, a.N = s->N, a.G = s->G, a.per = s->D / s->G, a.softplus = s->softplus;
+  a.u = s->u, a.ldu = s->ldu, a.delta = s->delta, a.ldd = s->ld_delta;
+  a.B = s->B, a.ldb = s->ldb, a.gsb = s->ldb_group, a.C = s->C, a.ldc = s->ldc, a.gsc = s->ldc_group;
+  a.z = s->z, a.ldz = s->ldz, a.A = s->A, a.Ds = s->skip, a.bias = s->delta_bias, a.init = s->init, a.fin = s->final;
+  a.y = s->y, a.ldy = s->ldy, a.keep = s->keep;
+  a.dy = s->dy, a.lddy = s->lddy, a.du = s->du, a.ddelta = s->ddelta, a.dz = s->dz, a.dB = s->dB, a.dC = s->dC;
+  a.dA = s->dA, a.dD = s->dD, a.dbias = s->ddelta_bias, a.dfin = s->dfinal, a.dinit = s->dinit;
+  a.st = Starts{s->starts, s->starts_type == FB_I64, s->seqs, s->rows};
+  const uintptr_t at = (uintptr_t)s->A | (uintptr_t)s->init | (uintptr_t)s->final | (uintptr_t)s->keep | (uintptr_t)s->dfinal |
+                       (uintptr_t)s->dinit | (uintptr_t)s->dA;
+  a.vec = s->N % 4 == 0 && at % 16 == 0;
+  return FB_OK;
+}
+
+constexpr int64_t kSms = 148;
+
+// The forward's split, and its pieces of the workspace.
+int plan_fwd(ScanArgs &a, int np, fbh::Call &c) {
+  const int ch = 2 * 2 * 32 / (np / 4);
+  a.tiles = (a.per + ch - 1) / ch;
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * 12, 64);
+  a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
+  if (a.nc > 1) {
+    FBH_TAKE(edge, c, float, (a.nc - 1) * (int64_t)a.D * a.N);
+    FBH_TAKE(sum, c, float, (a.nc - 1) * (int64_t)a.D);
+    FBH_TAKE(cut, c, int, a.nc - 1);
+    a.edge = edge, a.sumdt = sum, a.cut = cut;
+  }
+  return FB_OK;
+}
+
+int plan_bwd(ScanArgs &a, int np, fbh::Call &c) {
+  const int ch = 2 * 32 / (np / 4);                       // channels of a warp
+  const int tiles = (a.per + ch - 1) / ch;
+  a.ctas = (tiles + kWarps - 1) / kWarps;
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.ctas, kSms * 3, 64);
+  a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
+  a.tiles = (a.per + 2 * ch - 1) / (2 * ch);              // k_scan_rev's
+  const int64_t size = (int64_t)a.D * a.N;
+  if (a.nc > 1) {
+    FBH_TAKE(edge, c, float, (a.nc - 1) * size);
+    FBH_TAKE(sum, c, float, (a.nc - 1) * (int64_t)a.D);
+    FBH_TAKE(cut, c, int, a.nc - 1);
+    FBH_TAKE(pA, c, float, a.nc * size);
+    FBH_TAKE(pD, c, float, a.nc * 2 * (int64_t)a.D);
+    a.edge = edge, a.sumdt = sum, a.cut = cut, a.pA = pA, a.pD = pD;
+  }
+  if (a.ctas > 1) {
+    FBH_TAKE(pBC, c, float, (int64_t)a.G * a.ctas * a.st.rows * 2 * np);
+    a.pBC = pBC;
+  }
+  return FB_OK;
+}
+
+unsigned blocks(int64_t n, int64_t each) { return (unsigned)((n + each - 1) / each); }
+
+template <typename T, int NP> int run_fwd(const ScanArgs &a, cudaStream_t stream) {
+  const int64_t nct = (int64_t)a.G * a.tiles;
+  if (a.nc > 1) {
+    FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, true>, blocks(nct * (a.nc - 1), kWarps), kThreads, 0, stream, a));
+    FB_TRY_CUDA(fb::launch(k_scan_join<false>, blocks((int64_t)a.D * a.N, 256), 256, 0, stream, a));
+  }
+  FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, false>, blocks(nct * a.nc, kWarps), kThreads, 0, stream, a));
+  return FB_OK;
+}
+
+template <typename T, int NP> int run_bwd(const ScanArgs &a, cudaStream_t stream) {
+  constexpr size_t smem = sizeof(BwdSmem<T, NP>);
+  if (smem > 48 * 1024)
+    FB_TRY_CUDA(cudaFuncSetAttribute(k_scan_bwd<T, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (a.nc > 1) {
+    const int64_t nct = (int64_t)a.G * a.tiles;
+    FB_TRY_CUDA(fb::launch(k_scan_rev<T, NP>, blocks(nct * (a.nc - 1), kWarps), kThreads, 0, stream, a));
+    FB_TRY_CUDA(fb::launch(k_scan_join<true>, blocks((int64_t)a.D * a.N, 256), 256, 0, stream, a));
+  }
+  FB_TRY_CUDA(fb::launch(k_scan_bwd<T, NP>, dim3((unsigned)(a.G * a.ctas), (unsigned)a.nc), kThreads, smem, stream, a));
+  const int64_t bc = a.ctas > 1 ? blocks((int64_t)a.G * a.st.rows * 2 * NP, 256) : 0;
+  const int64_t rest = a.nc > 1 ? blocks((int64_t)a.D * (a.N + 2), 256) : 0;
+  if (bc + rest) FB_TRY_CUDA(fb::launch(k_scan_sums<T>, dim3((unsigned)(bc + rest)), 256, 0, stream, a, (int)NP, bc));
+  return FB_OK;
+}
+
+template <bool BWD, typename T> int run_states(const ScanArgs &a, int np, cudaStream_t st) {
+  switch (np) {
+    case 8: return BWD ? run_bwd<T, 8>(a, st) : run_fwd<T, 8>(a, st);
+    case 16: return BWD ? run_bwd<T, 16>(a, st) : run_fwd<T, 16>(a, st);
+    case 32: return BWD ? run_bwd<T, 32>(a, st) : run_fwd<T, 32>(a, st);
+    default: return BWD ? run_bwd<T, 64>(a, st) : run_fwd<T, 64>(a, st);
+  }
+}
+
+template <bool BWD> int run(const fb_selective_scan *s, void *ws, size_t ws_bytes, cudaStream_t stream) {
+  ScanArgs a;
+  FBH_TRY(fill(s, a, BWD));
+  const size_t state = (size_t)s->seqs * s->D * s->N * sizeof(float);
+  if (!s->rows) {                                          // nothing but empty sequences
+    if (!BWD && s->final && state) {
+      if (s->init) FB_TRY_CUDA(cudaMemcpyAsync(s->final, s->init, state, cudaMemcpyDeviceToDevice, stream));
+      else FB_TRY_CUDA(cudaMemsetAsync(s->final, 0, state, stream));
+    }
+    if (BWD) {
+      if (s->dinit && state) {
+        if (s->dfinal) FB_TRY_CUDA(cudaMemcpyAsync(s->dinit, s->dfinal, state, cudaMemcpyDeviceToDevice, stream));
+        else FB_TRY_CUDA(cudaMemsetAsync(s->dinit, 0, state, stream));
+      }
+      FB_TRY_CUDA(cudaMemsetAsync(s->dA, 0, (size_t)s->D * s->N * sizeof(float), stream));
+      FB_TRY_CUDA(cudaMemsetAsync(s->dD, 0, (size_t)s->D * sizeof(float), stream));
+      FB_TRY_CUDA(cudaMemsetAsync(s->ddelta_bias, 0, (size_t)s->D * sizeof(float), stream));
+    }
+    return FB_OK;
+  }
+  const int np = padded(s->N);
+  fbh::Call need;
+  {
+    ScanArgs b = a;
+    FBH_TRY(BWD ? plan_bwd(b, np, need) : plan_fwd(b, np, need));
+  }
+  if (need.peak) {
+    FBH_TRY(fbh::check_ws(ws, "selective_scan"));
+    if (ws_bytes < need.peak) return fb::set_error(FB_ERR_ARG, "selective_scan: workspace too small");
+  }
+  fbh::Call c(ws, ws_bytes, stream);
+  FBH_TRY(BWD ? plan_bwd(a, np, c) : plan_fwd(a, np, c));
+  return s->type == FB_F32 ? run_states<BWD, float>(a, np, stream) : run_states<BWD, bf16>(a, np, stream);
+}
+
+}  // namespace
+
+extern "C" size_t fb_selective_scan_ws_bytes(const fb_selective_scan *s, int backward) {
+  if (!s || s->rows <= 0 || s->D < 1 || s->N < 1 || s->N > kMaxStates || s->G < 1 || s->D % s->G) return 0;
+  ScanArgs a{};
+  a.D = s->D, a.N = s->N, a.G = s->G, a.per = s->D / s->G, a.st.rows = s->rows;
+  fbh::Call c;
+  if (backward ? plan_bwd(a, padded(s->N), c) : plan_fwd(a, padded(s->N), c)) return 0;
+  return c.peak;
+}
+
+extern "C" int fb_selective_scan_fwd(const fb_selective_scan *s, void *ws, size_t ws_bytes, cudaStream_t stream) {
+  return run<false>(s, ws, ws_bytes, stream);
+}
+
+extern "C" int fb_selective_scan_bwd(const fb_selective_scan *s, void *ws, size_t ws_bytes, cudaStream_t stream) {
+  return run<true>(s, ws, ws_bytes, stream);
+}

@@ -1,5 +1,6 @@
 """Imports the in-tree drop-in modules ``fastAgg`` and ``sampler_core``, and
-``head_ops``, the torch-level calls of the node-ranking head (``ops`` wraps it).
+``head_ops`` and ``history_ops``, the torch-level calls of the node-ranking head
+and of the event histories (``ops`` wraps them).
 
 They are built into ``fast_b200/_ext`` (``python -m fast_b200.build``).
 ``install_dropin()`` puts that directory on ``sys.path`` so unmodified
@@ -36,3 +37,4 @@ def _load(name):
 fastAgg = _load("fastAgg")
 sampler_core = _load("sampler_core")
 head_ops = _load("head_ops")
+history_ops = _load("history_ops")

@@ -12,7 +12,7 @@ import os
 import torch
 
 from .capi import ACTS, call, ptr, stream_ptr, lib
-from .ext import head_ops
+from .ext import head_ops, history_ops
 from .first_order import first_order
 
 
@@ -52,6 +52,7 @@ TIMER = None            # set to a KernelTimer to time every kernel wrapper
 USE_TC = False          # route eligible gemm_nt calls to the tcgen05 kernel
 LAUNCHES = [0]          # kernels launched through these wrappers
 head_ops.count_into(LAUNCHES)
+history_ops.count_into(LAUNCHES)
 # FB_NVTX=1: each wrapper's launches inside an NVTX range named like its timer
 # entry (eager steps), so a profiler can select one group by name
 NVTX = os.environ.get("FB_NVTX", "0") == "1"
@@ -775,6 +776,114 @@ def softmax_xent_bwd(h, w, target, lse, dloss, dw=None, grad_dtype=None):
     return _head_call(head_ops.softmax_xent_bwd,
                       lambda: (2 * h.element_size() * (h.numel() + w.numel()) + 16 * h.shape[0], 6 * h.numel() * w.shape[0]),
                       h, w, target, lse, dloss, dw, _grad_f32("softmax_xent_bwd", grad_dtype, h))
+
+
+# ---- event histories: short causal convolution, selective state space scan, dropout ----
+# Packed rows: the rows of several sequences one after the other, sequence s in
+# rows starts[s] .. starts[s + 1] - 1 (starts [seqs + 1], int64 or int32, on the
+# device; None: one sequence).  Sequences may be empty.  Rows in front of
+# starts[0] and from starts[-1] on belong to none: their results are zeros, and
+# they reach no gradient, whatever they hold.  starts must ascend; it is not
+# read on the host.  The calls go through the history_ops module, as the head's
+# through head_ops: operands of the wrong type, shape, layout or device raise
+# ValueError.
+def _conv_act(act):
+    try:
+        return {None: -1, "silu": ACTS["silu"]}[act]
+    except (KeyError, TypeError):
+        raise ValueError('short_conv: act must be "silu" or None') from None
+
+
+def short_conv_fwd(x, w, bias=None, starts=None, init=None, act="silu", final=False):
+    """Causal convolution of each column of packed rows x [rows, D] (fp32 or
+    bf16, any row pitch) with its taps w [D, K], K <= 8, oldest input first:
+    y[t] = act(bias + sum_k w[:, k] x[t - K + 1 + k]).  In front of its first row
+    a sequence finds init [seqs, K - 1, D] (its last K - 1 inputs, oldest first,
+    in x's type) or zeros.  Returns y, or with `final` (y, what init would be for
+    the rows to come).  w and bias are fp32; act: "silu" or None."""
+    k = w.shape[-1] if w.dim() else 0
+    return _head_call(history_ops.short_conv_fwd, lambda: (2 * x.element_size() * x.numel(), 2 * k * x.numel()), x, w, bias,
+                      starts, init, _conv_act(act), final)
+
+
+def short_conv_bwd(dy, x, w, bias=None, starts=None, init=None, act="silu", dfinal=None):
+    """Gradients of short_conv_fwd: (dx, dw, dbias, dinit), dw and dbias fp32,
+    None in the place of what was not given.  dfinal: the gradient of `final`."""
+    k = w.shape[-1] if w.dim() else 0
+    return _head_call(history_ops.short_conv_bwd, lambda: (3 * x.element_size() * x.numel(), 6 * k * x.numel()), dy, x, w,
+                      bias, starts, init, _conv_act(act), dfinal)
+
+
+def short_conv_step(x, state, w, bias=None, index=None, act="silu"):
+    """One event a row: x [n, D] continues the inputs of node index[r] (int64;
+    None: row r is node r), whose last K - 1 are state [nodes, K - 1, D] (x's
+    type, updated in place).  Returns y [n, D].  Rows of one node take their
+    turns in the rows' order.  A negative index holds its row out (y 0, no state
+    touched); one >= nodes gives a row of NaN and touches no state."""
+    return _head_call(history_ops.short_conv_step,
+                      lambda: (x.element_size() * x.numel() * 2 * w.shape[1], 2 * w.numel() * x.shape[0]), x, state, w, bias,
+                      index, _conv_act(act))
+
+
+def selective_scan_fwd(u, delta, A, B, C, D=None, z=None, delta_bias=None, starts=None, init=None, softplus=True, final=False,
+                       keep=True):
+    """Selective state space scan of packed rows u, delta (and z) [rows, D], fp32
+    or bf16, any row pitch:
+
+        dt = softplus(delta + delta_bias)      (softplus=False: delta + delta_bias)
+        h[t] = exp(dt A) h[t - 1] + dt u B[t]
+        y[t] = (<C[t], h[t]> + D u) silu(z)    (z None: no gate)
+
+    with A [D, N] (N <= 64), D, delta_bias [D] in fp32 and B, C [rows, N], or
+    [rows, groups, N] for groups of neighbouring channels, in u's type.  Sequences
+    begin with init [seqs, D, N] (fp32) or zeros.  All arithmetic is fp32.
+    Returns (y, carry, final): carry (None without `keep`) is what the backward
+    takes, fp32 states in front of every 8th row, rows D N / 2 bytes; final (None
+    unless asked for) the states [seqs, D, N] behind each sequence."""
+    return _head_call(history_ops.selective_scan_fwd,
+                      lambda: (u.element_size() * ((3 + (z is not None)) * u.numel() + B.numel() + C.numel()), 7 * u.shape[0] * A.numel()),
+                      u, delta, A, B, C, D, z, delta_bias, starts, init, softplus, final, keep)
+
+
+def selective_scan_bwd(dy, u, delta, A, B, C, carry, D=None, z=None, delta_bias=None, starts=None, init=None, softplus=True,
+                       dfinal=None):
+    """Gradients of selective_scan_fwd: (du, ddelta, dA, dB, dC, dD, dz,
+    ddelta_bias, dinit), None in the place of what was not given; those of fp32
+    operands are fp32.  carry is the forward's; dfinal the gradient of `final`."""
+    return _head_call(history_ops.selective_scan_bwd,
+                      lambda: (u.element_size() * ((5 + 2 * (z is not None)) * u.numel() + 2 * (B.numel() + C.numel()))
+                               + 4 * carry.numel(), 21 * u.shape[0] * A.numel()),
+                      dy, u, delta, A, B, C, carry, D, z, delta_bias, starts, init, softplus, dfinal)
+
+
+def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=None, index=None, softplus=True):
+    """One event a row: the scan's next row for node index[r] (int64; None: row r
+    is node r), whose state [nodes, D, N] (fp32) is updated in place.  Returns
+    y [n, D].  Order and held-out rows as in short_conv_step."""
+    return _head_call(history_ops.selective_scan_step,
+                      lambda: (8 * u.shape[0] * A.numel() + u.element_size() * (3 + (z is not None)) * u.numel(),
+                               7 * u.shape[0] * A.numel()), u, delta, A, B, C, state, D, z, delta_bias, index, softplus)
+
+
+def _counter(name, v):
+    if not isinstance(v, int) or isinstance(v, bool) or not 0 <= v < 1 << 64:
+        raise ValueError("dropout: %s must be a whole number of 64 bits" % name)
+    return v
+
+
+def dropout_fwd(x, p, seed, offset=0, res=None, offset_dev=None):
+    """y = res + keep x / (1 - p) for rows x (and res) [rows, D], fp32 or bf16, any
+    row pitch.  keep is drawn from a counter and never stored: word c % 4 of
+    Philox4x32-10 with counter (c / 4, r, offset) and key seed, its upper 24 bits
+    taken as a fraction, is not below p.  offset_dev: a device int64 [1] added to
+    the offset, for graphs whose replays draw anew."""
+    return _head_call(history_ops.dropout, lambda: (x.element_size() * x.numel() * (2 if res is None else 3), 16 * x.numel()),
+                      x, float(p), _counter("seed", seed), _counter("offset", offset), res, offset_dev)
+
+
+def dropout_bwd(dy, p, seed, offset=0, offset_dev=None):
+    """Gradient of x in dropout_fwd (that of res is dy itself)."""
+    return dropout_fwd(dy, p, seed, offset, None, offset_dev)
 
 
 class AttentionCore(torch.autograd.Function):

@@ -669,6 +669,118 @@ size_t fb_softmax_xent_ws_bytes(const fb_softmax_xent *args, int backward);
 int fb_softmax_xent_fwd(const fb_softmax_xent *args, void *ws, size_t ws_bytes, cudaStream_t stream);
 int fb_softmax_xent_bwd(const fb_softmax_xent *args, void *ws, size_t ws_bytes, cudaStream_t stream);
 
+/* ------------------------------------------------------------------------- */
+/* Event histories: a state space encoder over packed sequences of rows, and  */
+/* its steps for single events against per-node state tables.  No counterpart */
+/* in the reference, whose node memory is a GRU over the last mail            */
+/* (memorys.py:270-304) or attention over a mailbox (memorys.py:342-386).     */
+/* ------------------------------------------------------------------------- */
+/* Integer types of device arrays. */
+enum { FB_I32 = 0, FB_I64 = 1 };
+/* Packed sequences: `rows` rows; sequence s < seqs takes rows starts[s] ..
+ * starts[s + 1] - 1 (starts: seqs + 1 ascending device integers of starts_type;
+ * NULL: one sequence over all rows).  Sequences may be empty.  Rows in front of
+ * starts[0] or from starts[seqs] on belong to none: their results are zeros,
+ * and they reach nothing, whatever they hold.  Entries out of order give wrong
+ * results and no access outside the arrays.
+ *
+ * Short causal convolution per column, K <= 8 taps:
+ *   p[t, d] = bias[d] + sum_k w[d, k] x[t - K + 1 + k, d],  y = p or silu(p)
+ * In front of its first row a sequence finds init[s] (its last K - 1 inputs,
+ * oldest first, [seqs, K - 1, D] of the rows' type) or zeros; final, the same
+ * for what comes after it, is written when given.  act: FB_ACT_SILU, or
+ * FB_ACT_NONE.  w [D, K], bias [D] (may be NULL): fp32.
+ * Backward from dy and x (p is recomputed; dfinal, the gradient of final, may be
+ * NULL): dx, dinit in the rows' type (dinit may be NULL), dw, dbias in fp32.
+ * Sums are fp32.  Deterministic.  ws: fb_short_conv_ws_bytes(args, backward). */
+enum { FB_ACT_NONE = -1 };
+typedef struct fb_short_conv {
+  int type, act, starts_type, D, K;
+  int64_t rows, seqs;
+  const void *starts;
+  const void *x; int64_t ldx;
+  const float *w, *bias;
+  const void *init;
+  void *final;                             /* forward */
+  void *y; int64_t ldy;
+  const void *dy; int64_t lddy;            /* backward */
+  const void *dfinal;
+  void *dx; int64_t lddx;
+  float *dw, *dbias;
+  void *dinit;
+} fb_short_conv;
+size_t fb_short_conv_ws_bytes(const fb_short_conv *args, int backward);
+int fb_short_conv_fwd(const fb_short_conv *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+int fb_short_conv_bwd(const fb_short_conv *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+/* Selective scan over packed sequences, N <= 64 states a channel:
+ *   dt = softplus(delta + delta_bias)     (softplus 0: delta + delta_bias)
+ *   h[t, d, n] = exp(dt A[d, n]) h[t - 1, d, n] + dt u[t, d] B[t, g(d), n]
+ *   y[t, d] = (sum_n C[t, g(d), n] h[t, d, n] + skip[d] u[t, d]) silu(z[t, d])
+ * Channels come in G groups of D / G with a B and C each (ldb_group, ldc_group:
+ * elements between groups).  A [D, N], skip, delta_bias [D] (the last two may be
+ * NULL), init and final [seqs, D, N] (may be NULL: sequences begin at zero) are
+ * fp32, u, delta, B, C, z (may be NULL: no gate) and y of `type`.  keep (may be
+ * NULL), fp32 [ceil(rows / 8), D, N], receives the states in front of every 8th
+ * row, which the backward takes.  Backward from dy (and dfinal, may be NULL):
+ * du, ddelta, dz [rows, D], dB, dC [rows, G, N] in `type`; dA, dD, ddelta_bias,
+ * dinit (may be NULL) in fp32; contiguous.  All arithmetic is fp32.
+ * Deterministic.  ws: fb_selective_scan_ws_bytes(args, backward) bytes,
+ * 16-byte aligned. */
+typedef struct fb_selective_scan {
+  int type, starts_type, softplus, D, N, G;
+  int64_t rows, seqs;
+  const void *starts;
+  const void *u; int64_t ldu;
+  const void *delta; int64_t ld_delta;
+  const void *B; int64_t ldb, ldb_group;
+  const void *C; int64_t ldc, ldc_group;
+  const void *z; int64_t ldz;
+  const float *A, *skip, *delta_bias, *init;
+  float *keep;                             /* forward: written; backward: read */
+  float *final;                            /* forward */
+  void *y; int64_t ldy;
+  const void *dy; int64_t lddy;            /* backward */
+  const float *dfinal;
+  void *du, *ddelta, *dz, *dB, *dC;
+  float *dA, *dD, *ddelta_bias, *dinit;
+} fb_selective_scan;
+size_t fb_selective_scan_ws_bytes(const fb_selective_scan *args, int backward);
+int fb_selective_scan_fwd(const fb_selective_scan *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+int fb_selective_scan_bwd(const fb_selective_scan *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+/* Single events against per-node tables, in place: row r works on state
+ * index[r] (index NULL: state r; n <= states).  Rows of one node take their
+ * turns in the rows' order.  A negative index holds its row out: y 0, no state
+ * touched; one >= states gives a row of NaN and touches none.
+ * Convolution: state [states, K - 1, D] of the rows' type holds a node's last
+ * K - 1 inputs, oldest first.  ws: fb_event_step_ws_bytes(n) bytes, 16-byte
+ * aligned (both entries). */
+size_t fb_event_step_ws_bytes(int64_t n);
+int fb_short_conv_step(int type, int act, const void *x, int64_t ldx, const float *w, const float *bias, void *state,
+                       int64_t states, const int64_t *index, void *y, int64_t ldy, int64_t n, int D, int K, void *ws,
+                       size_t ws_bytes, cudaStream_t stream);
+/* Scan: state fp32 [states, D, N]; the other fields as fb_selective_scan's. */
+typedef struct fb_selective_scan_event {
+  int type, softplus, D, N, G;
+  int64_t n, states;
+  const int64_t *index;
+  const void *u; int64_t ldu;
+  const void *delta; int64_t ld_delta;
+  const void *B; int64_t ldb, ldb_group;
+  const void *C; int64_t ldc, ldc_group;
+  const void *z; int64_t ldz;
+  const float *A, *skip, *delta_bias;
+  float *state;
+  void *y; int64_t ldy;
+} fb_selective_scan_event;
+int fb_selective_scan_step(const fb_selective_scan_event *args, void *ws, size_t ws_bytes, cudaStream_t stream);
+/* Dropout from a counter, residual sum included (res may be NULL):
+ *   y = res + keep x / (1 - p),  keep[r, c]: word c % 4 of Philox4x32-10 with
+ *   counter (c / 4, r, offset + *offset_dev) and key seed, its upper 24 bits as
+ *   a fraction, is not below p.  offset_dev may be NULL.  The backward is the
+ *   same call on dy without res.  y may be x or res. */
+int fb_dropout(int type, const void *x, int64_t ldx, const void *res, int64_t ldr, void *y, int64_t ldy, int64_t rows,
+               int D, float p, uint64_t seed, uint64_t offset, const int64_t *offset_dev, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
