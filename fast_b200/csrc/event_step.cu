@@ -171,8 +171,8 @@ template <typename T, int NP> __global__ void __launch_bounds__(256) k_scan_step
     load(state, h);
     for (;;) {
       const float u = has ? to_f(static_cast<const T *>(a.u)[r * a.ldu + d]) : 0.f;
-      float slope, dt = has ? to_f(static_cast<const T *>(a.delta)[r * a.ldd + d]) + bias : 0.f;
-      if (a.softplus) dt = softplus(dt, slope);
+      float dt = has ? to_f(static_cast<const T *>(a.delta)[r * a.ldd + d]) + bias : 0.f;
+      if (a.softplus) dt = softplus(dt);
       const T *b = static_cast<const T *>(a.B) + r * a.ldb + grp * a.gsb, *c = static_cast<const T *>(a.C) + r * a.ldc + grp * a.gsc;
       float v = 0.f;
 #pragma unroll

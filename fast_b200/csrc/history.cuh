@@ -154,26 +154,48 @@ __device__ __forceinline__ float rcp(float x) {
   return r;
 }
 
-// log(1 + e^x) and its derivative, relative accuracy a few 2^-24 also where
-// they are small.  With e = e^-|x|: log(1 + e) = 2 artanh(s), s = e / (2 + e) <=
-// 1/3, and artanh(s) / s is a polynomial in s^2 (interpolated at Chebyshev
-// nodes of [0, 1/9], off by 4e-9).  The product |x| log2(e) is carried to two
-// words: its rounding alone would cost e 2^-24 |x|.
-__device__ __forceinline__ float softplus(float x, float &slope) {
-  const float m = fabsf(x), t = m * kLog2e;
-  const float lost = fmaf(m, kLog2e, -t) + m * 1.925963033500011e-8f;      // the rest of m log2(e)
-  float e = ex2(-t);
-  if (m < 88.f) e = fmaf(-0.6931472f * lost, e, e);
-  const float s = e * rcp(2.f + e), w = s * s;
-  float p = fmaf(w, 0.14078889787197113f, 0.13982579112052917f);
-  p = fmaf(w, p, 0.20012298226356506f);
-  p = fmaf(w, p, 0.3333316147327423f);
-  const float l = 2.f * fmaf(w * p, s, s), r = rcp(1.f + e);
-  slope = x >= 0.f ? r : e * r;
-  return x > 0.f ? x + l : (x <= 0.f ? l : x);                             // NaN stays NaN
+__device__ __forceinline__ F2 both(float a) { return pack(a, a); }
+__device__ __forceinline__ F2 rcp_2(F2 x) {
+  const float2 f = unpack(x);
+  return pack(rcp(f.x), rcp(f.y));
+}
+// The larger one, NaN if there is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// log(1 + e^x) of a pair and (SLOPE) its derivative, relative accuracy a few
+// 2^-24 also where they are small.  With e = e^-|x|: log(1 + e) = 2 artanh(s), s =
+// e / (2 + e) <= 1/3, and artanh(s) / s is a polynomial in s^2 (interpolated at
+// Chebyshev nodes of [0, 1/9], off by 4e-9).  The product |x| log2(e) is carried
+// to two words: its rounding alone would cost e 2^-24 |x|.
+template <bool SLOPE> __device__ __forceinline__ F2 softplus2(F2 x, F2 &slope) {
+  const float2 f = unpack(x);
+  const F2 m = pack(fminf(fabsf(f.x), 100.f), fminf(fabsf(f.y), 100.f));
+  const F2 t = mul2(m, both(-kLog2e));
+  const F2 lost = fma2(m, both(1.925963033500011e-8f), fma2(m, both(kLog2e), t));      // the rest of m log2(e)
+  F2 e = ex2_2(t);
+  e = fma2(mul2(lost, both(-0.6931472f)), e, e);
+  const F2 s = mul2(e, rcp_2(add2(e, both(2.f)))), w = mul2(s, s);
+  F2 p = fma2(w, both(0.14078889787197113f), both(0.13982579112052917f));
+  p = fma2(w, p, both(0.20012298226356506f));
+  p = fma2(w, p, both(0.3333316147327423f));
+  const F2 s2 = add2(s, s), l = fma2(mul2(w, p), s2, s2);
+  if constexpr (SLOPE) {
+    const float2 r = unpack(rcp_2(add2(e, both(1.f)))), er = unpack(mul2(e, pack(r.x, r.y)));
+    slope = pack(f.x >= 0.f ? r.x : er.x, f.y >= 0.f ? r.y : er.y);
+  }
+  return add2(l, pack(max_nan(f.x, 0.f), max_nan(f.y, 0.f)));
+}
+__device__ __forceinline__ float softplus(float x) {
+  F2 none;
+  return unpack(softplus2<false>(both(x), none)).x;
 }
 
 // 1 / (1 + e^-x)
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
+__device__ __forceinline__ F2 sigmoid2(F2 x) { return rcp_2(add2(ex2_2(mul2(x, both(-kLog2e))), both(1.f))); }
 
 }  // namespace fbq

@@ -70,8 +70,6 @@ struct ScanArgs {
   int vec;                                // states move four at a time
 };
 
-template <typename T> __device__ __forceinline__ T ld_el(const void *p, int64_t i) { return static_cast<const T *>(p)[i]; }
-
 // Four states from n0 on of one channel.
 __device__ __forceinline__ void load4(const float *p, int n0, int N, int vec, float (&v)[4]) {
   if (vec) {
@@ -150,42 +148,85 @@ template <int V, int L, int STRIDE> __device__ __forceinline__ int spread_sum(fl
   return 0;
 }
 
+// A warp's tile: kTile rows x CH channels, or x NP states.  The lanes lie along the
+// columns; element i of a lane is row(i), col(i).
+template <int COLS> struct Tile {
+  static constexpr int E = kTile * COLS / 32;                            // elements a lane
+  static constexpr int W = COLS > 32 ? COLS / 32 : 1;                    // columns a lane meets
+  static constexpr int RS = COLS > 32 ? 1 : 32 / COLS;                   // rows between a column's elements
+  static __device__ __forceinline__ int col(int i) { return (threadIdx.x & 31) % COLS + 32 * (i % W); }
+  static __device__ __forceinline__ int row(int i) { return COLS > 32 ? i / W : (threadIdx.x & 31) / COLS + RS * i; }
+  // Loads the rows [a, b) of the tile whose first row, first column is at p.
+  template <typename T> static __device__ __forceinline__ void fetch(T (&x)[E], const void *base, int64_t at, int64_t ld, int cols, int a,
+                                                                     int b) {
+    const T *p = static_cast<const T *>(base) + at + row(0) * ld + col(0);
+    const T none = from_f<T>(0.f);
+    const int64_t step = RS * ld;
+    if (a == 0 && b == kTile) {
+#pragma unroll
+      for (int i = 0; i < E; i += W, p += step)
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[i + w] = col(w) < cols ? p[32 * w] : none;
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i += W, p += step)
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[i + w] = col(w) < cols && row(i) >= a && row(i) < b ? p[32 * w] : none;
+    }
+  }
+};
+
 // A thread's place: NP states (padded to 8, 16, 32 or 64) of P pairs of channels a thread.
 template <int NP, int P> struct Lay {
   static constexpr int NL = NP / 4, CL = 32 / NL, CH = 2 * P * CL;       // lanes along states, channels; channels a warp
-  static constexpr int E = kTile * CH / 32, EB = kTile * NP / 32;        // a tile's elements a lane: rows x channels, rows x states
-  static constexpr int W = CH > 32 ? CH / 32 : 1;                        // channels a lane stages
-  static __device__ __forceinline__ int ch(int i) { return ((threadIdx.x & 31) + 32 * i) % CH; }
-  static __device__ __forceinline__ int row(int i) { return ((threadIdx.x & 31) + 32 * i) / CH; }
+  using X = Tile<CH>;
+  using S = Tile<NP>;
 };
 
-template <typename T, int NP> struct FwdSmem {
-  using L = Lay<NP, 2>;
-  float dt[kTile][L::CH], dtu[kTile][L::CH], y[kTile][L::CH];
+// v with the elements of the rows outside [a, b) at zero.
+template <typename X> __device__ __forceinline__ float only(float v, int i, int a, int b) {
+  return X::row(i) >= a && X::row(i) < b ? v : 0.f;
+}
+
+// dt of a lane's elements (pairs of them) and, with SLOPE, the derivative by delta.
+template <bool SLOPE, typename X, typename T> __device__ __forceinline__ void steps(const T (&raw)[X::E], const float (&bias)[X::W], int sp,
+                                                                                   float (&dt)[X::E], float (&slope)[X::E]) {
+#pragma unroll
+  for (int i = 0; i < X::E; i += 2) {
+    const int j = i + 1 < X::E ? i + 1 : i;
+    const F2 x = add2(pack(to_f(raw[i]), to_f(raw[j])), pack(bias[i % X::W], bias[j % X::W]));
+    F2 sl = both(1.f);
+    const float2 v = unpack(sp ? softplus2<SLOPE>(x, sl) : x), k = unpack(sl);
+    dt[i] = v.x, dt[j] = X::E > 1 ? v.y : v.x;
+    if (SLOPE) slope[i] = k.x, slope[j] = X::E > 1 ? k.y : k.x;
+  }
+}
+
+template <int NP> struct FwdSmem {
+  static constexpr int CH = Lay<NP, 2>::CH;
+  float dt[kTile][CH], dtu[kTile][CH], y[kTile][CH];
   float2 B[kTile][NP], C[kTile][NP];                                     // each value twice: a pair's factor
 };
 
-// The loads of one tile of rows for a warp, as they come: u, delta (or dy and the
-// gate), B and C.
-template <typename T, int E, int EB> struct Raw {
-  T x[E], d[E], b[EB], c[EB];
-};
+__device__ __forceinline__ int rows_in(int64_t v) { return (int)max((int64_t)0, min((int64_t)kTile, v)); }
 
 // Forward.  LOCAL: the chunk's last state alone, from the last beginning of a
 // sequence on, for all chunks but the last.
 template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThreads, 4) k_scan_fwd(ScanArgs a) {
   using L = Lay<NP, 2>;
+  using X = typename L::X;
+  using S = typename L::S;
   fb::pdl_enter();
-  __shared__ __align__(16) FwdSmem<T, NP> smem[kWarps];
+  __shared__ __align__(16) FwdSmem<NP> smem[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  FwdSmem<T, NP> &sm = smem[warp];
+  FwdSmem<NP> &sm = smem[warp];
   const int nct = a.G * a.tiles;
   const int64_t wid = (int64_t)blockIdx.x * kWarps + warp;
   const int64_t chunk = wid / nct;
   const int ct = (int)(wid % nct);
   if (chunk >= a.nc - (LOCAL ? 1 : 0)) return;
   const int grp = ct / a.tiles, ch0 = (ct % a.tiles) * L::CH, left = a.per - ch0;   // channels the tile has
-  const int64_t cb = (int64_t)grp * a.per + ch0;
+  const int64_t cb = (int64_t)grp * a.per + ch0, size = (int64_t)a.D * a.N;
   const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
   const int64_t mine = cb + cl * 4;
   const int has = left - cl * 4;
@@ -196,165 +237,146 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], pack(kLog2e, kLog2e));
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], both(kLog2e));
   h.zero();
 
-  int64_t from = c0, lo = 0, hi = rows;           // first row; rows of sequences
+  int64_t lo, hi;                                 // rows that count
   Walk walk;
   if constexpr (LOCAL) {
     const int64_t s = owner(a.st, c1 - 1);
     const bool in = s >= 0 && s < a.st.seqs;
     const int64_t b = in ? a.st[s] : 0;
     const bool ends = !in || a.st[s + 1] <= c1;   // nothing goes on into the next chunk
-    const bool cut = ends || b >= c0;
-    if (ct == 0 && lane == 0) a.cut[chunk] = cut;
-    if (ends) from = c1;
-    else if (b >= c0) {
-      from = b;
-      if (a.init) h.load(a.init + s * (int64_t)a.D * a.N, mine, has, n0, a);
-    }
-    lo = from, hi = c1;
+    if (ct == 0 && lane == 0) a.cut[chunk] = ends || b >= c0;
+    lo = ends ? c1 : max(b, c0), hi = c1;
+    if (!ends && b >= c0 && a.init) h.load(a.init + s * size, mine, has, n0, a);
   } else {
     walk.begin(a.st, c0);
-    lo = walk.first, hi = walk.last;
-    if (chunk > 0) h.load(a.edge + (chunk - 1) * (int64_t)a.D * a.N, mine, has, n0, a);
+    lo = walk.first, hi = min(walk.last, c1);
+    if (chunk > 0) h.load(a.edge + (chunk - 1) * size, mine, has, n0, a);
   }
 
-  float bias[L::W], skip[L::W];
+  float bias[X::W], skip[X::W];
 #pragma unroll
-  for (int w = 0; w < L::W; ++w) {
-    const int c = L::ch(w);
+  for (int w = 0; w < X::W; ++w) {
+    const int c = X::col(w);
     bias[w] = a.bias && c < left ? a.bias[cb + c] : 0.f;
     skip[w] = !LOCAL && a.Ds && c < left ? a.Ds[cb + c] : 0.f;
   }
-  Raw<T, L::E, L::EB> raw;
-  const T none = from_f<T>(0.f);
+  T xu[X::E], xd[X::E], xb[S::E], xc[LOCAL ? 1 : S::E];
   const auto fetch = [&](int64_t r0) {
-#pragma unroll
-    for (int i = 0; i < L::E; ++i) {
-      const int64_t r = r0 + L::row(i);
-      const int c = L::ch(i);
-      const bool in = c < left && r >= lo && r < hi && r < c1;
-      raw.x[i] = in ? ld_el<T>(a.u, r * a.ldu + cb + c) : none;
-      raw.d[i] = in ? ld_el<T>(a.delta, r * a.ldd + cb + c) : none;
-    }
-#pragma unroll
-    for (int i = 0; i < L::EB; ++i) {
-      const int n = (lane + 32 * i) % NP;
-      const int64_t r = r0 + (lane + 32 * i) / NP;
-      const bool in = n < a.N && r >= lo && r < hi && r < c1;
-      raw.b[i] = in ? ld_el<T>(a.B, r * a.ldb + grp * a.gsb + n) : none;
-      if (!LOCAL) raw.c[i] = in ? ld_el<T>(a.C, r * a.ldc + grp * a.gsc + n) : none;
-    }
+    const int ra = rows_in(lo - r0), rb = rows_in(hi - r0);
+    X::fetch(xu, a.u, r0 * a.ldu + cb, a.ldu, left, ra, rb);
+    X::fetch(xd, a.delta, r0 * a.ldd + cb, a.ldd, left, ra, rb);
+    S::fetch(xb, a.B, r0 * a.ldb + grp * a.gsb, a.ldb, a.N, ra, rb);
+    if constexpr (!LOCAL) S::fetch(xc, a.C, r0 * a.ldc + grp * a.gsc, a.ldc, a.N, ra, rb);
   };
-  // A sequence begins at `row`: the one before it leaves its last state.
-  const auto begin_at = [&](int64_t row) {
-    if (a.fin && row > c0) {
-      const int64_t s = owner(a.st, row - 1);
-      if (s >= 0 && s < a.st.seqs) h.store(a.fin + s * (int64_t)a.D * a.N, mine, has, n0, a);
+
+  F2 total[2] = {both(0.f), both(0.f)};
+  const auto row = [&](int i) {
+    F2 dt[2], dtu[2], B[4], C[4], y[2];
+    const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(&sm.dt[i][cl * 4]);
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&sm.dtu[i][cl * 4]);
+    const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
+    dt[0].v = t.x, dt[1].v = t.y, dtu[0].v = x.x, dtu[1].v = x.y;
+    B[0].v = b[0].x, B[1].v = b[0].y, B[2].v = b[1].x, B[3].v = b[1].y;
+    if constexpr (!LOCAL) {
+      const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(&sm.C[i][n0]);
+      C[0].v = c[0].x, C[1].v = c[0].y, C[2].v = c[1].x, C[3].v = c[1].y;
     }
-    h.zero();
-    if (a.init) {
-      const int64_t s = owner(a.st, row);
-      if (s >= 0 && s < a.st.seqs) h.load(a.init + s * (int64_t)a.D * a.N, mine, has, n0, a);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const F2 decay = ex2_2(mul2(dt[p], A2.v[p][k]));
+        h.v[p][k] = fma2(decay, h.v[p][k], mul2(dtu[p], B[k]));
+        if constexpr (!LOCAL) y[p] = k == 0 ? mul2(C[k], h.v[p][k]) : fma2(C[k], h.v[p][k], y[p]);
+      }
+      if constexpr (LOCAL) total[p] = add2(total[p], dt[p]);
+    }
+    if constexpr (!LOCAL) {
+      const float2 ya = unpack(y[0]), yb = unpack(y[1]);
+      float v[4] = {ya.x, ya.y, yb.x, yb.y};
+      const int at = spread_sum<4, L::NL, 1>(v);
+      constexpr int kOwn = L::NL >= 4 ? 1 : 4 / L::NL;
+      if (L::NL <= 4 || nl % (L::NL / 4 > 0 ? L::NL / 4 : 1) == 0) {
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) sm.y[i][cl * 4 + at + k] = v[k];
+      }
     }
   };
 
-  F2 total[2] = {pack(0.f, 0.f), pack(0.f, 0.f)};
-  int64_t r0 = c0 + (from - c0) / kTile * kTile;
+  int64_t r0 = LOCAL ? c0 + (lo - c0) / kTile * kTile : c0;
   if (r0 < c1) fetch(r0);
   for (; r0 < c1; r0 += kTile) {
-    T ku[L::E], kz[L::E];
+    const int ra = rows_in(lo - r0), rb = rows_in(hi - r0);
+    float dt[X::E], slope[X::E];
+    T ku[X::E], kz[X::E];
+    steps<false, X>(xd, bias, a.softplus, dt, slope);
+#pragma unroll
+    for (int i = 0; i < X::E; ++i) {
+      const float v = only<X>(dt[i], i, ra, rb);
+      sm.dt[X::row(i)][X::col(i)] = v;
+      sm.dtu[X::row(i)][X::col(i)] = v * to_f(xu[i]);
+      ku[i] = xu[i];
+    }
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) {
+      const float b = to_f(xb[i]);
+      sm.B[S::row(i)][S::col(i)] = make_float2(b, b);
+      if constexpr (!LOCAL) {
+        const float c = to_f(xc[i]);
+        sm.C[S::row(i)][S::col(i)] = make_float2(c, c);
+      }
+    }
     unsigned begins = 0;
     if constexpr (!LOCAL) {
       begins = walk.tile(r0);
       if (c1 - r0 < kTile) begins &= (1u << (int)(c1 - r0)) - 1u;
-    }
-#pragma unroll
-    for (int i = 0; i < L::E; ++i) {
-      const int64_t r = r0 + L::row(i);
-      const int c = L::ch(i);
-      const bool in = r >= lo && r < hi && r < c1;
-      float slope;
-      float dt = to_f(raw.d[i]) + bias[i % L::W];
-      if (a.softplus) dt = softplus(dt, slope);
-      if (!in) dt = 0.f;
-      sm.dt[L::row(i)][c] = dt;
-      sm.dtu[L::row(i)][c] = dt * to_f(raw.x[i]);
-      if constexpr (!LOCAL) {
-        ku[i] = raw.x[i];
-        kz[i] = a.z && in && c < left ? ld_el<T>(a.z, r * a.ldz + cb + c) : none;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < L::EB; ++i) {
-      const int at = lane + 32 * i;
-      const float b = to_f(raw.b[i]);
-      sm.B[at / NP][at % NP] = make_float2(b, b);
-      if constexpr (!LOCAL) {
-        const float c = to_f(raw.c[i]);
-        sm.C[at / NP][at % NP] = make_float2(c, c);
-      }
+      if (a.z) X::fetch(kz, a.z, r0 * a.ldz + cb, a.ldz, left, ra, rb);
     }
     if (r0 + kTile < c1) fetch(r0 + kTile);
     __syncwarp();
-    if (!LOCAL && a.keep) h.store(a.keep + r0 / kTile * (int64_t)a.D * a.N, mine, has, n0, a);
+    if (!LOCAL && a.keep) h.store(a.keep + r0 / kTile * size, mine, has, n0, a);
+    if (LOCAL || begins == 0) {
 #pragma unroll
-    for (int i = 0; i < kTile; ++i) {
-      if (!LOCAL && (begins >> i & 1u)) begin_at(r0 + i);
-      F2 dt[2], dtu[2], B[4], C[4], y[2];
-      {
-        const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(&sm.dt[i][cl * 4]);
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&sm.dtu[i][cl * 4]);
-        const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
-        dt[0].v = t.x, dt[1].v = t.y, dtu[0].v = x.x, dtu[1].v = x.y;
-        B[0].v = b[0].x, B[1].v = b[0].y, B[2].v = b[1].x, B[3].v = b[1].y;
-        if constexpr (!LOCAL) {
-          const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(&sm.C[i][n0]);
-          C[0].v = c[0].x, C[1].v = c[0].y, C[2].v = c[1].x, C[3].v = c[1].y;
+      for (int i = 0; i < kTile; ++i) row(i);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kTile; ++i) {
+        if (begins >> i & 1u) {
+          const int64_t at = r0 + i;
+          if (a.fin && at > c0) {                 // the sequence in front leaves its last state
+            const int64_t s = owner(a.st, at - 1);
+            if (s >= 0 && s < a.st.seqs) h.store(a.fin + s * size, mine, has, n0, a);
+          }
+          h.zero();
+          if (a.init) {
+            const int64_t s = owner(a.st, at);
+            if (s >= 0 && s < a.st.seqs) h.load(a.init + s * size, mine, has, n0, a);
+          }
         }
-      }
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const F2 decay = ex2_2(mul2(dt[p], A2.v[p][k]));
-          h.v[p][k] = fma2(decay, h.v[p][k], mul2(dtu[p], B[k]));
-          if constexpr (!LOCAL) y[p] = k == 0 ? mul2(C[k], h.v[p][k]) : fma2(C[k], h.v[p][k], y[p]);
-        }
-        if constexpr (LOCAL) total[p] = add2(total[p], dt[p]);
-      }
-      if constexpr (!LOCAL) {
-        const float2 ya = unpack(y[0]), yb = unpack(y[1]);
-        float v[4] = {ya.x, ya.y, yb.x, yb.y};
-        const int at = spread_sum<4, L::NL, 1>(v);
-        constexpr int kOwn = L::NL >= 4 ? 1 : 4 / L::NL;
-        if (L::NL <= 4 || nl % (L::NL / 4 > 0 ? L::NL / 4 : 1) == 0) {
-#pragma unroll
-          for (int k = 0; k < kOwn; ++k) sm.y[i][cl * 4 + at + k] = v[k];
-        }
+        row(i);
       }
     }
     __syncwarp();
     if constexpr (!LOCAL) {
+      T *py = static_cast<T *>(a.y) + (r0 + X::row(0)) * a.ldy + cb + X::col(0);
+      const int end = rows_in(c1 - r0);
 #pragma unroll
-      for (int i = 0; i < L::E; ++i) {
-        const int64_t r = r0 + L::row(i);
-        const int c = L::ch(i);
-        if (r < c1 && c < left) {
-          float v = fmaf(skip[i % L::W], to_f(ku[i]), sm.y[L::row(i)][c]);
-          if (a.z) {
-            const float z = to_f(kz[i]);
-            v *= z * sigmoid(z);
-          }
-          static_cast<T *>(a.y)[r * a.ldy + cb + c] = from_f<T>(r >= lo && r < hi ? v : 0.f);
+      for (int i = 0; i < X::E; ++i) {
+        float v = fmaf(skip[i % X::W], to_f(ku[i]), sm.y[X::row(i)][X::col(i)]);
+        if (a.z) {
+          const float z = to_f(kz[i]);
+          v *= z * sigmoid(z);
         }
+        if (X::row(i) < end && X::col(i) < left) py[i / X::W * X::RS * a.ldy + 32 * (i % X::W)] = from_f<T>(only<X>(v, i, ra, rb));
       }
     }
   }
   if constexpr (LOCAL) {
     __syncwarp();
-    h.store(a.edge + chunk * (int64_t)a.D * a.N, mine, has, n0, a);
+    h.store(a.edge + chunk * size, mine, has, n0, a);
     if (nl == 0) {
       const float2 x = unpack(total[0]), y = unpack(total[1]);
       const float t[4] = {x.x, x.y, y.x, y.y};
@@ -364,7 +386,7 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
     }
   } else if (a.fin) {
     const int64_t s = owner(a.st, c1 - 1);
-    if (s >= 0 && s < a.st.seqs && a.st[s + 1] <= c1) h.store(a.fin + s * (int64_t)a.D * a.N, mine, has, n0, a);
+    if (s >= 0 && s < a.st.seqs && a.st[s + 1] <= c1) h.store(a.fin + s * size, mine, has, n0, a);
     for (int64_t q = chunk; q < a.st.seqs; q += 32 * (int64_t)a.nc) {          // empty sequences end as they began
       const int64_t e = q + lane * (int64_t)a.nc;
       unsigned m = __ballot_sync(0xffffffffu, e < a.st.seqs && a.st[e] >= a.st[e + 1]);
@@ -372,8 +394,8 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
         const int64_t s0 = q + (__ffs(m) - 1) * (int64_t)a.nc;
         States<2> x;
         x.zero();
-        if (a.init) x.load(a.init + s0 * (int64_t)a.D * a.N, mine, has, n0, a);
-        x.store(a.fin + s0 * (int64_t)a.D * a.N, mine, has, n0, a);
+        if (a.init) x.load(a.init + s0 * size, mine, has, n0, a);
+        x.store(a.fin + s0 * size, mine, has, n0, a);
       }
     }
   }
@@ -408,9 +430,9 @@ template <bool REV> __global__ void __launch_bounds__(256) k_scan_join(ScanArgs 
 }
 
 // ---- backward ------------------------------------------------------------------------------------
-template <typename T, int NP> struct RevSmem {
-  using L = Lay<NP, 2>;
-  float dt[kTile][L::CH], gv[kTile][L::CH];
+template <int NP> struct RevSmem {
+  static constexpr int CH = Lay<NP, 2>::CH;
+  float dt[kTile][CH], gv[kTile][CH];
   float2 C[kTile][NP];
 };
 
@@ -418,17 +440,19 @@ template <typename T, int NP> struct RevSmem {
 // front of its first row, from the rows of the sequence that comes in.
 template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_scan_rev(ScanArgs a) {
   using L = Lay<NP, 2>;
+  using X = typename L::X;
+  using S = typename L::S;
   fb::pdl_enter();
-  __shared__ __align__(16) RevSmem<T, NP> smem[kWarps];
+  __shared__ __align__(16) RevSmem<NP> smem[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  RevSmem<T, NP> &sm = smem[warp];
+  RevSmem<NP> &sm = smem[warp];
   const int nct = a.G * a.tiles;
   const int64_t wid = (int64_t)blockIdx.x * kWarps + warp;
   const int64_t chunk = wid / nct + 1;
   const int ct = (int)(wid % nct);
   if (chunk >= a.nc) return;
   const int grp = ct / a.tiles, ch0 = (ct % a.tiles) * L::CH, left = a.per - ch0;
-  const int64_t cb = (int64_t)grp * a.per + ch0;
+  const int64_t cb = (int64_t)grp * a.per + ch0, size = (int64_t)a.D * a.N;
   const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
   const int64_t mine = cb + cl * 4;
   const int has = left - cl * 4;
@@ -439,57 +463,46 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], pack(kLog2e, kLog2e));
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], both(kLog2e));
   r.zero();
   const int64_t s = owner(a.st, c0);
   const bool in = s >= 0 && s < a.st.seqs && a.st[s] < c0;      // a sequence comes in
   const int64_t end = in ? a.st[s + 1] : c0, e = min(end, c1);
   if (ct == 0 && lane == 0) a.cut[chunk - 1] = !in || end <= c1;
-  if (in && end <= c1 && a.dfin) r.load(a.dfin + s * (int64_t)a.D * a.N, mine, has, n0, a);
+  if (in && end <= c1 && a.dfin) r.load(a.dfin + s * size, mine, has, n0, a);
 
-  float bias[L::W];
+  float bias[X::W];
 #pragma unroll
-  for (int w = 0; w < L::W; ++w) bias[w] = a.bias && L::ch(w) < left ? a.bias[cb + L::ch(w)] : 0.f;
-  const T none = from_f<T>(0.f);
-  T xd[L::E], xy[L::E], xz[L::E], xc[L::EB];
+  for (int w = 0; w < X::W; ++w) bias[w] = a.bias && X::col(w) < left ? a.bias[cb + X::col(w)] : 0.f;
+  T xd[X::E], xy[X::E], xz[X::E], xc[S::E];
   const auto fetch = [&](int64_t r0) {
-#pragma unroll
-    for (int i = 0; i < L::E; ++i) {
-      const int64_t q = r0 + L::row(i);
-      const int c = L::ch(i);
-      const bool ok = c < left && q < e;
-      xd[i] = ok ? ld_el<T>(a.delta, q * a.ldd + cb + c) : none;
-      xy[i] = ok ? ld_el<T>(a.dy, q * a.lddy + cb + c) : none;
-      xz[i] = ok && a.z ? ld_el<T>(a.z, q * a.ldz + cb + c) : none;
-    }
-#pragma unroll
-    for (int i = 0; i < L::EB; ++i) {
-      const int n = (lane + 32 * i) % NP;
-      const int64_t q = r0 + (lane + 32 * i) / NP;
-      xc[i] = n < a.N && q < e ? ld_el<T>(a.C, q * a.ldc + grp * a.gsc + n) : none;
-    }
+    const int rb = rows_in(e - r0);
+    X::fetch(xd, a.delta, r0 * a.ldd + cb, a.ldd, left, 0, rb);
+    X::fetch(xy, a.dy, r0 * a.lddy + cb, a.lddy, left, 0, rb);
+    if (a.z) X::fetch(xz, a.z, r0 * a.ldz + cb, a.ldz, left, 0, rb);
+    S::fetch(xc, a.C, r0 * a.ldc + grp * a.gsc, a.ldc, a.N, 0, rb);
   };
-  F2 total[2] = {pack(0.f, 0.f), pack(0.f, 0.f)};
+  F2 total[2] = {both(0.f), both(0.f)};
   int64_t r0 = e > c0 ? c0 + (e - 1 - c0) / kTile * kTile : c0 - kTile;
   if (r0 >= c0) fetch(r0);
   for (; r0 >= c0; r0 -= kTile) {
+    const int rb = rows_in(e - r0);
+    float dt[X::E], slope[X::E];
+    steps<false, X>(xd, bias, a.softplus, dt, slope);
 #pragma unroll
-    for (int i = 0; i < L::E; ++i) {
-      const bool ok = r0 + L::row(i) < e;
-      float slope, dt = to_f(xd[i]) + bias[i % L::W], gv = to_f(xy[i]);
-      if (a.softplus) dt = softplus(dt, slope);
+    for (int i = 0; i < X::E; ++i) {
+      float gv = to_f(xy[i]);
       if (a.z) {
         const float z = to_f(xz[i]);
         gv *= z * sigmoid(z);
       }
-      sm.dt[L::row(i)][L::ch(i)] = ok ? dt : 0.f;
-      sm.gv[L::row(i)][L::ch(i)] = ok ? gv : 0.f;
+      sm.dt[X::row(i)][X::col(i)] = only<X>(dt[i], i, 0, rb);
+      sm.gv[X::row(i)][X::col(i)] = only<X>(gv, i, 0, rb);
     }
 #pragma unroll
-    for (int i = 0; i < L::EB; ++i) {
-      const int at = lane + 32 * i;
+    for (int i = 0; i < S::E; ++i) {
       const float c = to_f(xc[i]);
-      sm.C[at / NP][at % NP] = make_float2(c, c);
+      sm.C[S::row(i)][S::col(i)] = make_float2(c, c);
     }
     if (r0 - kTile >= c0) fetch(r0 - kTile);
     __syncwarp();
@@ -498,18 +511,18 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
       const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(&sm.dt[i][cl * 4]);
       const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&sm.gv[i][cl * 4]);
       const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(&sm.C[i][n0]);
-      const F2 dt[2] = {{t.x}, {t.y}}, gv[2] = {{x.x}, {x.y}}, C[4] = {{c[0].x}, {c[0].y}, {c[1].x}, {c[1].y}};
+      const F2 dt2[2] = {{t.x}, {t.y}}, gv[2] = {{x.x}, {x.y}}, C[4] = {{c[0].x}, {c[0].y}, {c[1].x}, {c[1].y}};
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          r.v[p][k] = mul2(ex2_2(mul2(dt[p], A2.v[p][k])), fma2(C[k], gv[p], r.v[p][k]));
-        total[p] = add2(total[p], dt[p]);
+          r.v[p][k] = mul2(ex2_2(mul2(dt2[p], A2.v[p][k])), fma2(C[k], gv[p], r.v[p][k]));
+        total[p] = add2(total[p], dt2[p]);
       }
     }
     __syncwarp();
   }
-  r.store(a.edge + (chunk - 1) * (int64_t)a.D * a.N, mine, has, n0, a);
+  r.store(a.edge + (chunk - 1) * size, mine, has, n0, a);
   if (nl == 0) {
     const float2 x = unpack(total[0]), y = unpack(total[1]);
     const float t[4] = {x.x, x.y, y.x, y.y};
@@ -519,79 +532,72 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
   }
 }
 
-template <typename T, int NP> struct BwdSmem {
-  using L = Lay<NP, 1>;
-  float dt[kWarps][kTile][L::CH], dtu[kWarps][kTile][L::CH], gv[kWarps][kTile][L::CH];
-  float out[kWarps][3][kTile][L::CH];                            // <g, B>, <q, A log2 e>, <C, h>
+template <int NP> struct BwdSmem {
+  static constexpr int CH = Lay<NP, 1>::CH;
+  float dt[kWarps][kTile][CH], dtu[kWarps][kTile][CH], gv[kWarps][kTile][CH];
+  float out[kWarps][3][kTile][CH];                               // <g, B>, <q, A log2 e>, <C, h>
   float2 B[kTile][NP], C[kTile][NP];
   float sum[kWarps][kTile][2 * NP];                              // the warps' sums over channels: dB, dC
+  int64_t seq[kWarps][kTile + 1];                                // of the rows in front of and at beginnings
 };
 
 // All gradients of a chunk's rows.  The warps of a CTA stand side by side on a
 // group's channels and add up their parts of dB and dC tile by tile.
 template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_scan_bwd(ScanArgs a) {
   using L = Lay<NP, 1>;
+  using X = typename L::X;
   fb::pdl_enter();
   extern __shared__ __align__(16) unsigned char dyn[];
-  BwdSmem<T, NP> &sm = *reinterpret_cast<BwdSmem<T, NP> *>(dyn);
+  BwdSmem<NP> &sm = *reinterpret_cast<BwdSmem<NP> *>(dyn);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int grp = blockIdx.x / a.ctas, cta = blockIdx.x % a.ctas;
   const int64_t chunk = blockIdx.y;
   const int ch0 = (cta * kWarps + warp) * L::CH, left = a.per - ch0;        // may be <= 0: a warp without channels
-  const int64_t cb = (int64_t)grp * a.per + ch0;
+  const int64_t cb = (int64_t)grp * a.per + ch0, size = (int64_t)a.D * a.N;
   const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
   const int64_t mine = cb + cl * 2;
   const int has = left - cl * 2;
   const int64_t rows = a.st.rows, c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, rows);
-  const int64_t first = a.st[0], last = a.st[a.st.seqs], size = (int64_t)a.D * a.N;
+  const int64_t lo = a.st[0], hi = min(a.st[a.st.seqs], c1);
 
   States<1> A2, r, dA;
   A2.load(a.A, mine, has, n0, a);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) A2.v[0][k] = mul2(A2.v[0][k], pack(kLog2e, kLog2e));
+  for (int k = 0; k < 4; ++k) A2.v[0][k] = mul2(A2.v[0][k], both(kLog2e));
   dA.zero();
-  // r behind `row`, the last of its sequence
-  const auto behind = [&](int64_t row) {
-    r.zero();
-    if (a.dfin) {
-      const int64_t s = owner(a.st, row);
-      if (s >= 0 && s < a.st.seqs) r.load(a.dfin + s * size, mine, has, n0, a);
-    }
-  };
+  r.zero();
   {
     const int64_t s = owner(a.st, c1 - 1);
-    if (c1 >= rows || s < 0 || s >= a.st.seqs || a.st[s + 1] <= c1) behind(c1 - 1);
-    else r.load(a.edge + chunk * size, mine, has, n0, a);
+    const bool in = s >= 0 && s < a.st.seqs;
+    if (c1 >= rows || !in || a.st[s + 1] <= c1) {
+      if (in && a.dfin) r.load(a.dfin + s * size, mine, has, n0, a);
+    } else {
+      r.load(a.edge + chunk * size, mine, has, n0, a);
+    }
   }
 
-  float bias[L::W], skip[L::W], sumD[L::W] = {}, sumb[L::W] = {};
+  float bias[X::W], skip[X::W], sumD[X::W] = {}, sumb[X::W] = {};
 #pragma unroll
-  for (int w = 0; w < L::W; ++w) {
-    const int c = L::ch(w);
+  for (int w = 0; w < X::W; ++w) {
+    const int c = X::col(w);
     bias[w] = a.bias && c < left ? a.bias[cb + c] : 0.f;
     skip[w] = a.Ds && c < left ? a.Ds[cb + c] : 0.f;
   }
   const T none = from_f<T>(0.f);
   constexpr int EC = kTile * NP / kThreads > 0 ? kTile * NP / kThreads : 1;  // B (and C) elements a thread of the CTA
-  T xu[L::E], xd[L::E], xy[L::E], xz[L::E], xb[EC], xc[EC];
+  T xu[X::E], xd[X::E], xy[X::E], xz[X::E], xb[EC], xc[EC];
   const auto fetch = [&](int64_t r0) {
-#pragma unroll
-    for (int i = 0; i < L::E; ++i) {
-      const int64_t q = r0 + L::row(i);
-      const int c = L::ch(i);
-      const bool ok = c < left && q >= first && q < last && q < c1;
-      xu[i] = ok ? ld_el<T>(a.u, q * a.ldu + cb + c) : none;
-      xd[i] = ok ? ld_el<T>(a.delta, q * a.ldd + cb + c) : none;
-      xy[i] = ok ? ld_el<T>(a.dy, q * a.lddy + cb + c) : none;
-      xz[i] = ok && a.z ? ld_el<T>(a.z, q * a.ldz + cb + c) : none;
-    }
+    const int ra = rows_in(lo - r0), rb = rows_in(hi - r0);
+    X::fetch(xu, a.u, r0 * a.ldu + cb, a.ldu, left, ra, rb);
+    X::fetch(xd, a.delta, r0 * a.ldd + cb, a.ldd, left, ra, rb);
+    X::fetch(xy, a.dy, r0 * a.lddy + cb, a.lddy, left, ra, rb);
+    if (a.z) X::fetch(xz, a.z, r0 * a.ldz + cb, a.ldz, left, ra, rb);
 #pragma unroll
     for (int i = 0; i < EC; ++i) {
-      const int at = threadIdx.x + kThreads * i, n = at % NP;
-      const int64_t q = r0 + at / NP;
-      const bool ok = at < kTile * NP && n < a.N && q >= first && q < last && q < c1;
-      xb[i] = ok ? ld_el<T>(a.B, q * a.ldb + grp * a.gsb + n) : none;
-      xc[i] = ok ? ld_el<T>(a.C, q * a.ldc + grp * a.gsc + n) : none;
+      const int at = threadIdx.x + kThreads * i, n = at % NP, row = at / NP;
+      const bool ok = at < kTile * NP && n < a.N && row >= ra && row < rb;
+      xb[i] = ok ? static_cast<const T *>(a.B)[(r0 + row) * a.ldb + grp * a.gsb + n] : none;
+      xc[i] = ok ? static_cast<const T *>(a.C)[(r0 + row) * a.ldc + grp * a.gsc + n] : none;
     }
   };
 
@@ -601,20 +607,22 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
   fetch(r0);
   for (; r0 >= c0; r0 -= kTile) {
     // ---- the tile's rows, once for each (row, channel)
-    float ku[L::E], ky[L::E], kz[L::E], kdt[L::E], ksl[L::E];
+    const int ra = rows_in(lo - r0), rb = rows_in(hi - r0);
+    float ku[X::E], ky[X::E], kz[X::E], kdt[X::E], ksl[X::E];
+    steps<true, X>(xd, bias, a.softplus, kdt, ksl);
 #pragma unroll
-    for (int i = 0; i < L::E; ++i) {
-      const int64_t q = r0 + L::row(i);
-      const bool ok = q >= first && q < last && q < c1;
-      float slope = 1.f, dt = to_f(xd[i]) + bias[i % L::W], gv = to_f(xy[i]);
-      if (a.softplus) dt = softplus(dt, slope);
-      ku[i] = to_f(xu[i]), ky[i] = gv, kz[i] = to_f(xz[i]), ksl[i] = slope;
-      if (a.z) gv *= kz[i] * sigmoid(kz[i]);
-      if (!ok) dt = 0.f;
-      kdt[i] = dt;
-      sm.dt[warp][L::row(i)][L::ch(i)] = dt;
-      sm.dtu[warp][L::row(i)][L::ch(i)] = dt * ku[i];
-      sm.gv[warp][L::row(i)][L::ch(i)] = gv;
+    for (int i = 0; i < X::E; ++i) {
+      ku[i] = to_f(xu[i]), ky[i] = to_f(xy[i]), kz[i] = 0.f;
+      float gv = ky[i];
+      if (a.z) {
+        kz[i] = to_f(xz[i]);
+        gv *= kz[i] * sigmoid(kz[i]);
+      }
+      kdt[i] = only<X>(kdt[i], i, ra, rb);
+      const int row = X::row(i), c = X::col(i);
+      sm.dt[warp][row][c] = kdt[i];
+      sm.dtu[warp][row][c] = kdt[i] * ku[i];
+      sm.gv[warp][row][c] = gv;
     }
 #pragma unroll
     for (int i = 0; i < EC; ++i) {
@@ -626,6 +634,13 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
       }
     }
     const unsigned begins = walk.tile(r0);
+    if (begins && (a.init || a.dfin || a.dinit)) {
+#pragma unroll 1
+      for (int i = 0; i <= kTile; ++i) {
+        const int64_t s = owner(a.st, r0 + i - 1);
+        if (lane == 0) sm.seq[warp][i] = s >= 0 && s < a.st.seqs ? s : -1;
+      }
+    }
     States<1> h0, h;
     h0.load(a.keep + r0 / kTile * size, mine, has, n0, a);
     if (r0 - kTile >= c0) fetch(r0 - kTile);
@@ -633,18 +648,18 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
 
     // ---- states and decays of the 8 rows
     F2 hs[kTile][4], as[kTile][4];
-    // What a sequence that begins at `row` finds.
-    const auto found = [&](States<1> &x, int64_t row) {
+    // What a sequence finds that begins at row i of the tile.
+    const auto found = [&](States<1> &x, int i) {
       x.zero();
       if (a.init) {
-        const int64_t s = owner(a.st, row);
-        if (s >= 0 && s < a.st.seqs) x.load(a.init + s * size, mine, has, n0, a);
+        const int64_t s = sm.seq[warp][i + 1];
+        if (s >= 0) x.load(a.init + s * size, mine, has, n0, a);
       }
     };
     h = h0;
 #pragma unroll
     for (int i = 0; i < kTile; ++i) {
-      if (begins >> i & 1u) found(h, r0 + i);
+      if (begins >> i & 1u) found(h, i);
       const F2 dt = {*reinterpret_cast<const unsigned long long *>(&sm.dt[warp][i][cl * 2])};
       const F2 dtu = {*reinterpret_cast<const unsigned long long *>(&sm.dtu[warp][i][cl * 2])};
       const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
@@ -657,6 +672,8 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
       }
     }
     // ---- back up the rows
+    States<1> tA;                                                // the tile's part of dA: short sums round less
+    tA.zero();
 #pragma unroll
     for (int i = kTile - 1; i >= 0; --i) {
       const F2 dt = {*reinterpret_cast<const unsigned long long *>(&sm.dt[warp][i][cl * 2])};
@@ -667,7 +684,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
       const F2 B[4] = {{b[0].x}, {b[0].y}, {b[1].x}, {b[1].y}}, C[4] = {{c[0].x}, {c[0].y}, {c[1].x}, {c[1].y}};
       States<1> before;
       if (begins >> i & 1u) {
-        found(before, r0 + i);
+        found(before, i);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) before.v[0][k] = i ? hs[i - 1][k] : h0.v[0][k];
@@ -682,7 +699,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
         gB = k == 0 ? mul2(g, B[k]) : fma2(g, B[k], gB);
         qA = k == 0 ? mul2(q, A2.v[0][k]) : fma2(q, A2.v[0][k], qA);
         cy = k == 0 ? mul2(C[k], hs[i][k]) : fma2(C[k], hs[i][k], cy);
-        dA.v[0][k] = fma2(q, dt, dA.v[0][k]);
+        tA.v[0][k] = fma2(q, dt, tA.v[0][k]);
         const float2 vb = unpack(mul2(g, dtu)), vc = unpack(mul2(gv, hs[i][k]));
         bc[k] = vb.x + vb.y, bc[4 + k] = vc.x + vc.y;
       }
@@ -699,34 +716,35 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
 #pragma unroll
       for (int k = 0; k < kOwnC; ++k) sm.sum[warp][i][((atc + k) >> 2) * NP + n0 + ((atc + k) & 3)] = bc[k];
       if (begins >> i & 1u) {
-        if (a.dinit) {
-          const int64_t s = owner(a.st, r0 + i);
-          if (s >= 0 && s < a.st.seqs) r.store(a.dinit + s * size, mine, has, n0, a);
-        }
-        behind(r0 + i - 1);
+        if (a.dinit && sm.seq[warp][i + 1] >= 0) r.store(a.dinit + sm.seq[warp][i + 1] * size, mine, has, n0, a);
+        r.zero();
+        if (a.dfin && sm.seq[warp][i] >= 0) r.load(a.dfin + sm.seq[warp][i] * size, mine, has, n0, a);
       }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dA.v[0][k] = add2(dA.v[0][k], tA.v[0][k]);
     __syncthreads();
 
     // ---- results of the tile
+    const int end = rows_in(c1 - r0);
+    const int64_t to = (r0 + X::row(0)) * a.D + cb + X::col(0);
 #pragma unroll
-    for (int i = 0; i < L::E; ++i) {
-      const int row = L::row(i), c = L::ch(i), w = i % L::W;
-      const int64_t q = r0 + row;
-      if (q >= c1 || c >= left) continue;
-      const bool ok = q >= first && q < last;
+    for (int i = 0; i < X::E; ++i) {
+      const int row = X::row(i), c = X::col(i), w = i % X::W;
+      if (row >= end || c >= left) continue;
+      const int64_t q = to + i / X::W * X::RS * (int64_t)a.D + 32 * w;
       const float gB = sm.out[warp][0][row][c], qA = sm.out[warp][1][row][c] * 0.6931471805599453f;
       float gv = ky[i];
       if (a.z) {
         const float sg = sigmoid(kz[i]), v = fmaf(skip[w], ku[i], sm.out[warp][2][row][c]);
         gv *= kz[i] * sg;
         const float dz = ky[i] * v * sg * fmaf(kz[i], 1.f - sg, 1.f);
-        static_cast<T *>(a.dz)[q * a.D + cb + c] = from_f<T>(ok ? dz : 0.f);
+        static_cast<T *>(a.dz)[q] = from_f<T>(only<X>(dz, i, ra, rb));
       }
-      const float dd = fmaf(ku[i], gB, qA) * ksl[i];
-      static_cast<T *>(a.du)[q * a.D + cb + c] = from_f<T>(ok ? fmaf(kdt[i], gB, skip[w] * gv) : 0.f);
-      static_cast<T *>(a.ddelta)[q * a.D + cb + c] = from_f<T>(ok ? dd : 0.f);
-      if (ok) sumD[w] = fmaf(gv, ku[i], sumD[w]), sumb[w] += dd;
+      const float dd = only<X>(fmaf(ku[i], gB, qA) * ksl[i], i, ra, rb);
+      static_cast<T *>(a.du)[q] = from_f<T>(only<X>(fmaf(kdt[i], gB, skip[w] * gv), i, ra, rb));
+      static_cast<T *>(a.ddelta)[q] = from_f<T>(dd);
+      sumD[w] = fmaf(gv, ku[i], sumD[w]), sumb[w] += dd;
     }
     for (int at = threadIdx.x; at < kTile * 2 * NP; at += kThreads) {
       const int row = at / (2 * NP), col = at % (2 * NP);
@@ -745,7 +763,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
 
   dA.store((a.nc > 1 ? a.pA + chunk * size : a.dA), mine, has, n0, a);
 #pragma unroll
-  for (int w = 0; w < L::W; ++w) {
+  for (int w = 0; w < X::W; ++w) {
     if (L::CH < 32) {
 #pragma unroll
       for (int o = L::CH; o < 32; o <<= 1) {
@@ -753,7 +771,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
         sumb[w] += __shfl_xor_sync(0xffffffffu, sumb[w], o);
       }
     }
-    const int c = L::ch(w);
+    const int c = X::col(w);
     if (c < left && lane < L::CH) {
       if (a.nc > 1) a.pD[(chunk * 2) * a.D + cb + c] = sumD[w], a.pD[(chunk * 2 + 1) * a.D + cb + c] = sumb[w];
       else a.dD[cb + c] = sumD[w], a.dbias[cb + c] = sumb[w];
@@ -856,12 +874,13 @@ int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
 }
 
 constexpr int64_t kSms = 148;
+int64_t knob(const char *n, int64_t d) { const char *e = getenv(n); return e ? atoll(e) : d; }
 
 // The forward's split, and its pieces of the workspace.
 int plan_fwd(ScanArgs &a, int np, fbh::Call &c) {
   const int ch = 2 * 2 * 32 / (np / 4);
   a.tiles = (a.per + ch - 1) / ch;
-  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * 12, 64);
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * knob("FB_FW", 24), knob("FB_FL", 64));
   a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
   if (a.nc > 1) {
     FBH_TAKE(edge, c, float, (a.nc - 1) * (int64_t)a.D * a.N);
@@ -876,7 +895,7 @@ int plan_bwd(ScanArgs &a, int np, fbh::Call &c) {
   const int ch = 2 * 32 / (np / 4);                       // channels of a warp
   const int tiles = (a.per + ch - 1) / ch;
   a.ctas = (tiles + kWarps - 1) / kWarps;
-  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.ctas, kSms * 3, 64);
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.ctas, kSms * knob("FB_BW", 4), knob("FB_BL", 64));
   a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
   a.tiles = (a.per + 2 * ch - 1) / (2 * ch);              // k_scan_rev's
   const int64_t size = (int64_t)a.D * a.N;
@@ -908,7 +927,7 @@ template <typename T, int NP> int run_fwd(const ScanArgs &a, cudaStream_t stream
 }
 
 template <typename T, int NP> int run_bwd(const ScanArgs &a, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(BwdSmem<T, NP>);
+  constexpr size_t smem = sizeof(BwdSmem<NP>);
   if (smem > 48 * 1024)
     FB_TRY_CUDA(cudaFuncSetAttribute(k_scan_bwd<T, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   if (a.nc > 1) {
