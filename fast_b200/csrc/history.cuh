@@ -28,8 +28,9 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Vec {
 struct Starts {
   const void *p;             // null: one sequence over all rows
   int wide;                  // 64-bit entries
-  int64_t seqs, rows;
-  __device__ __forceinline__ int64_t operator[](int64_t s) const {
+  int seqs;
+  int64_t rows;
+  __device__ __forceinline__ int64_t operator[](int s) const {
     if (!p) return s > 0 ? rows : 0;
     const int64_t v = wide ? static_cast<const int64_t *>(p)[s] : static_cast<const int32_t *>(p)[s];
     return v < 0 ? 0 : (v > rows ? rows : v);
@@ -39,15 +40,15 @@ struct Starts {
 // Sequence of a row: the last s in [0, seqs] with starts[s] <= row; -1 in front
 // of them all, seqs behind them all.  The whole warp takes part; 32 probes a
 // round, so 1,024 sequences take two dependent loads.
-__device__ __forceinline__ int64_t owner(const Starts &st, int64_t row) {
+__device__ __forceinline__ int owner(const Starts &st, int64_t row) {
   if (!st.p) return row < 0 ? -1 : (row < st.rows ? 0 : 1);
   const int lane = threadIdx.x & 31;
-  int64_t lo = 0, hi = st.seqs + 1;                    // starts[lo - 1] <= row < starts[hi]
+  int lo = 0, hi = st.seqs + 1;                        // starts[lo - 1] <= row < starts[hi]
   while (hi > lo) {
-    const int64_t step = (hi - lo + 31) >> 5, i = lo + lane * step;
+    const int step = (hi - lo + 31) >> 5, i = lo + lane * step;
     const int c = __popc(__ballot_sync(0xffffffffu, i < hi && st[i] <= row));
     if (c == 0) break;
-    const int64_t next = lo + c * step;
+    const int next = lo + c * step;
     lo = next - step + 1;
     hi = next < hi ? next : hi;
   }
@@ -57,21 +58,15 @@ __device__ __forceinline__ int64_t owner(const Starts &st, int64_t row) {
 // Walks the rows' boundaries upwards, kTile rows at a time.
 constexpr int kTile = 8;
 struct Walk {
-  Starts st;
-  int64_t next;              // first entry of starts that may lie behind the current tile's first row
-  int64_t first, last;       // rows of all sequences: [first, last)
-  __device__ __forceinline__ void begin(const Starts &s, int64_t row) {
-    st = s;
-    first = st[0], last = st[st.seqs];
-    next = owner(st, row - 1) + 1;
-  }
+  int next;                  // first entry of starts that may lie behind the current tile's first row
+  __device__ __forceinline__ void begin(const Starts &st, int64_t row) { next = owner(st, row - 1) + 1; }
   // Bit i: row r0 + i begins a sequence (or is the first behind the last one).
-  __device__ __forceinline__ unsigned tile(int64_t r0) {
+  __device__ __forceinline__ unsigned tile(const Starts &st, int64_t r0) {
     unsigned bits = 0;
     const int lane = threadIdx.x & 31;
     if (!st.p) return (r0 == 0 ? 1u : 0u) | (st.rows >= r0 && st.rows < r0 + kTile ? 1u << (st.rows - r0) : 0u);
     for (;;) {
-      const int64_t i = next + lane;
+      const int i = next + lane;
       const int64_t b = i <= st.seqs ? st[i] : INT64_MAX;
       const bool in = b < r0 + kTile;
       bits |= __reduce_or_sync(0xffffffffu, in && b >= r0 ? 1u << (int)(b - r0) : 0u);
@@ -85,18 +80,14 @@ struct Walk {
 // The same, downwards: the first tile asked for holds row `top`, the next ones
 // lie 8 rows lower each.
 struct WalkDown {
-  Starts st;
-  int64_t next;              // last entry of starts that may lie in the next tile
-  __device__ __forceinline__ void begin(const Starts &s, int64_t top) {
-    st = s;
-    next = owner(st, top);
-  }
-  __device__ __forceinline__ unsigned tile(int64_t r0) {
+  int next;                  // last entry of starts that may lie in the next tile
+  __device__ __forceinline__ void begin(const Starts &st, int64_t top) { next = owner(st, top); }
+  __device__ __forceinline__ unsigned tile(const Starts &st, int64_t r0) {
     if (!st.p) return r0 == 0 ? 1u : 0u;
     unsigned bits = 0;
     const int lane = threadIdx.x & 31;
     for (;;) {
-      const int64_t i = next - lane;
+      const int i = next - lane;
       const int64_t b = i >= 0 ? st[i] : -1;
       const bool in = b >= r0;
       bits |= __reduce_or_sync(0xffffffffu, in && b < r0 + kTile ? 1u << (int)(b - r0) : 0u);

@@ -40,7 +40,7 @@
 //
 // Everything between the loads and the stores is fp32.
 #include <algorithm>
-#include <cstring>
+#include <type_traits>
 #include "head.cuh"
 #include "history.cuh"
 
@@ -49,6 +49,15 @@ using namespace fbq;
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxStates = 64;
+constexpr int kHalf = kTile / 2;          // rows whose states the backward holds at once
+constexpr int kBwdCtas = 3;               // CTAs an SM its registers allow
+constexpr int kKept = 1;                  // pairs of a thread whose decays it holds, too
+
+// exp(dt A) of a pair, A2 = A log2(e).  The exponential unit's results are low by
+// 0.6 to 2.4e-8 on average where decays are slow (measured for exponents of -1e-4
+// to -1), which a state that remembers a thousand steps adds up a thousand
+// times; the summand centres them.
+__device__ __forceinline__ F2 decays(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, both(2e-8f))); }
 
 struct ScanArgs {
   int D, N, G, per, tiles, softplus;      // per: channels of a group; tiles: a group's tiles of channels
@@ -100,7 +109,7 @@ template <int P> struct States {
       for (int k = 0; k < 4; ++k) v[p][k] = pack(0.f, 0.f);
   }
   // From / to [D, N] rows at `base`; c: channel (in the tensor) of the thread's first, `has` of them exist.
-  __device__ __forceinline__ void load(const float *base, int64_t c, int has, int n0, const ScanArgs &a) {
+  __device__ __forceinline__ void load(const float *base, int c, int has, int n0, const ScanArgs &a) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       float x[2][4] = {};
@@ -111,7 +120,7 @@ template <int P> struct States {
       for (int k = 0; k < 4; ++k) v[p][k] = pack(x[0][k], x[1][k]);
     }
   }
-  __device__ __forceinline__ void store(float *base, int64_t c, int has, int n0, const ScanArgs &a) const {
+  __device__ __forceinline__ void store(float *base, int c, int has, int n0, const ScanArgs &a) const {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       float x[2][4];
@@ -127,25 +136,20 @@ template <int P> struct States {
   }
 };
 
-// Sums V values over L lanes that are STRIDE apart, each lane keeping max(1, V / L)
-// of the sums: v[0 ..], the first of them value number `at`.
-template <int V, int L, int STRIDE> __device__ __forceinline__ int spread_sum(float *v) {
-  if constexpr (L > 1) {
-    constexpr int kBit = STRIDE * L / 2;
-    if constexpr (V > 1) {
-      const bool up = (threadIdx.x & kBit) != 0;
+// The sum of the values that L neighbouring lanes left at p.
+template <int L> __device__ __forceinline__ float lanes_sum(const float *p) {
+  float v = 0.f;
+  if constexpr (L == 2) {
+    const float2 f = *reinterpret_cast<const float2 *>(p);
+    v = f.x + f.y;
+  } else {
 #pragma unroll
-      for (int k = 0; k < V / 2; ++k) {
-        const float send = up ? v[k] : v[k + V / 2], stay = up ? v[k + V / 2] : v[k];
-        v[k] = stay + __shfl_xor_sync(0xffffffffu, send, kBit);
-      }
-      return (up ? V / 2 : 0) + spread_sum<V / 2, L / 2, STRIDE>(v);
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], kBit);
-      return spread_sum<1, L / 2, STRIDE>(v);
+    for (int i = 0; i < L; i += 4) {
+      const float4 f = *reinterpret_cast<const float4 *>(p + i);
+      v += (f.x + f.y) + (f.z + f.w);
     }
   }
-  return 0;
+  return v;
 }
 
 // A warp's tile: kTile rows x CH channels, or x NP states.  The lanes lie along the
@@ -181,6 +185,9 @@ template <int NP, int P> struct Lay {
   static constexpr int NL = NP / 4, CL = 32 / NL, CH = 2 * P * CL;       // lanes along states, channels; channels a warp
   using X = Tile<CH>;
   using S = Tile<NP>;
+  // Where a channel's lanes lie in their row of parts: moved by whole groups, so that the groups of neighbouring
+  // channels, read together, meet different banks.
+  static __device__ __forceinline__ int turn(int by) { return by & ~(NL - 1); }
 };
 
 // v with the elements of the rows outside [a, b) at zero.
@@ -204,7 +211,8 @@ template <bool SLOPE, typename X, typename T> __device__ __forceinline__ void st
 
 template <int NP> struct FwdSmem {
   static constexpr int CH = Lay<NP, 2>::CH;
-  float dt[kTile][CH], dtu[kTile][CH], y[kTile][CH];
+  float dt[kTile][CH], dtu[kTile][CH];
+  float y[kTile][4][32];                                                 // each lane's part of its 4 channels' y
   float2 B[kTile][NP], C[kTile][NP];                                     // each value twice: a pair's factor
 };
 
@@ -217,18 +225,18 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
   using X = typename L::X;
   using S = typename L::S;
   fb::pdl_enter();
-  __shared__ __align__(16) FwdSmem<NP> smem[kWarps];
+  extern __shared__ __align__(16) unsigned char dyn[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  FwdSmem<NP> &sm = smem[warp];
+  FwdSmem<NP> &sm = reinterpret_cast<FwdSmem<NP> *>(dyn)[warp];
   const int nct = a.G * a.tiles;
   const int64_t wid = (int64_t)blockIdx.x * kWarps + warp;
   const int64_t chunk = wid / nct;
   const int ct = (int)(wid % nct);
   if (chunk >= a.nc - (LOCAL ? 1 : 0)) return;
   const int grp = ct / a.tiles, ch0 = (ct % a.tiles) * L::CH, left = a.per - ch0;   // channels the tile has
-  const int64_t cb = (int64_t)grp * a.per + ch0, size = (int64_t)a.D * a.N;
+  const int cb = grp * a.per + ch0, size = a.D * a.N;
   const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
-  const int64_t mine = cb + cl * 4;
+  const int mine = cb + cl * 4;
   const int has = left - cl * 4;
   const int64_t rows = a.st.rows, c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, rows);
 
@@ -243,17 +251,17 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
   int64_t lo, hi;                                 // rows that count
   Walk walk;
   if constexpr (LOCAL) {
-    const int64_t s = owner(a.st, c1 - 1);
+    const int s = owner(a.st, c1 - 1);
     const bool in = s >= 0 && s < a.st.seqs;
     const int64_t b = in ? a.st[s] : 0;
     const bool ends = !in || a.st[s + 1] <= c1;   // nothing goes on into the next chunk
     if (ct == 0 && lane == 0) a.cut[chunk] = ends || b >= c0;
     lo = ends ? c1 : max(b, c0), hi = c1;
-    if (!ends && b >= c0 && a.init) h.load(a.init + s * size, mine, has, n0, a);
+    if (!ends && b >= c0 && a.init) h.load(a.init + (int64_t)s * size, mine, has, n0, a);
   } else {
     walk.begin(a.st, c0);
-    lo = walk.first, hi = min(walk.last, c1);
-    if (chunk > 0) h.load(a.edge + (chunk - 1) * size, mine, has, n0, a);
+    lo = a.st[0], hi = min(a.st[a.st.seqs], c1);
+    if (chunk > 0) h.load(a.edge + (chunk - 1) * (int64_t)size, mine, has, n0, a);
   }
 
   float bias[X::W], skip[X::W];
@@ -288,7 +296,7 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
     for (int p = 0; p < 2; ++p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const F2 decay = ex2_2(mul2(dt[p], A2.v[p][k]));
+        const F2 decay = decays(dt[p], A2.v[p][k]);
         h.v[p][k] = fma2(decay, h.v[p][k], mul2(dtu[p], B[k]));
         if constexpr (!LOCAL) y[p] = k == 0 ? mul2(C[k], h.v[p][k]) : fma2(C[k], h.v[p][k], y[p]);
       }
@@ -296,13 +304,9 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
     }
     if constexpr (!LOCAL) {
       const float2 ya = unpack(y[0]), yb = unpack(y[1]);
-      float v[4] = {ya.x, ya.y, yb.x, yb.y};
-      const int at = spread_sum<4, L::NL, 1>(v);
-      constexpr int kOwn = L::NL >= 4 ? 1 : 4 / L::NL;
-      if (L::NL <= 4 || nl % (L::NL / 4 > 0 ? L::NL / 4 : 1) == 0) {
+      const float v[4] = {ya.x, ya.y, yb.x, yb.y};
 #pragma unroll
-        for (int k = 0; k < kOwn; ++k) sm.y[i][cl * 4 + at + k] = v[k];
-      }
+      for (int j = 0; j < 4; ++j) sm.y[i][j][lane ^ L::turn(j * 8)] = v[j];
     }
   };
 
@@ -331,7 +335,7 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
     }
     unsigned begins = 0;
     if constexpr (!LOCAL) {
-      begins = walk.tile(r0);
+      begins = walk.tile(a.st, r0);
       if (c1 - r0 < kTile) begins &= (1u << (int)(c1 - r0)) - 1u;
       if (a.z) X::fetch(kz, a.z, r0 * a.ldz + cb, a.ldz, left, ra, rb);
     }
@@ -347,13 +351,13 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
         if (begins >> i & 1u) {
           const int64_t at = r0 + i;
           if (a.fin && at > c0) {                 // the sequence in front leaves its last state
-            const int64_t s = owner(a.st, at - 1);
-            if (s >= 0 && s < a.st.seqs) h.store(a.fin + s * size, mine, has, n0, a);
+            const int s = owner(a.st, at - 1);
+            if (s >= 0 && s < a.st.seqs) h.store(a.fin + (int64_t)s * size, mine, has, n0, a);
           }
           h.zero();
           if (a.init) {
-            const int64_t s = owner(a.st, at);
-            if (s >= 0 && s < a.st.seqs) h.load(a.init + s * size, mine, has, n0, a);
+            const int s = owner(a.st, at);
+            if (s >= 0 && s < a.st.seqs) h.load(a.init + (int64_t)s * size, mine, has, n0, a);
           }
         }
         row(i);
@@ -365,7 +369,8 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
       const int end = rows_in(c1 - r0);
 #pragma unroll
       for (int i = 0; i < X::E; ++i) {
-        float v = fmaf(skip[i % X::W], to_f(ku[i]), sm.y[X::row(i)][X::col(i)]);
+        const int c = X::col(i);
+        float v = fmaf(skip[i % X::W], to_f(ku[i]), lanes_sum<L::NL>(&sm.y[X::row(i)][c & 3][((c >> 2) * L::NL) ^ L::turn((c & 3) * 8)]));
         if (a.z) {
           const float z = to_f(kz[i]);
           v *= z * sigmoid(z);
@@ -376,7 +381,7 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
   }
   if constexpr (LOCAL) {
     __syncwarp();
-    h.store(a.edge + chunk * size, mine, has, n0, a);
+    h.store(a.edge + chunk * (int64_t)size, mine, has, n0, a);
     if (nl == 0) {
       const float2 x = unpack(total[0]), y = unpack(total[1]);
       const float t[4] = {x.x, x.y, y.x, y.y};
@@ -385,13 +390,13 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
         if (j < has) a.sumdt[chunk * a.D + mine + j] = t[j];
     }
   } else if (a.fin) {
-    const int64_t s = owner(a.st, c1 - 1);
-    if (s >= 0 && s < a.st.seqs && a.st[s + 1] <= c1) h.store(a.fin + s * size, mine, has, n0, a);
-    for (int64_t q = chunk; q < a.st.seqs; q += 32 * (int64_t)a.nc) {          // empty sequences end as they began
-      const int64_t e = q + lane * (int64_t)a.nc;
+    const int s = owner(a.st, c1 - 1);
+    if (s >= 0 && s < a.st.seqs && a.st[s + 1] <= c1) h.store(a.fin + (int64_t)s * size, mine, has, n0, a);
+    for (int q = (int)chunk; q < a.st.seqs; q += 32 * a.nc) {          // empty sequences end as they began
+      const int e = q + lane * a.nc;
       unsigned m = __ballot_sync(0xffffffffu, e < a.st.seqs && a.st[e] >= a.st[e + 1]);
       for (; m; m &= m - 1) {
-        const int64_t s0 = q + (__ffs(m) - 1) * (int64_t)a.nc;
+        const int64_t s0 = q + (__ffs(m) - 1) * a.nc;
         States<2> x;
         x.zero();
         if (a.init) x.load(a.init + s0 * size, mine, has, n0, a);
@@ -452,9 +457,9 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
   const int ct = (int)(wid % nct);
   if (chunk >= a.nc) return;
   const int grp = ct / a.tiles, ch0 = (ct % a.tiles) * L::CH, left = a.per - ch0;
-  const int64_t cb = (int64_t)grp * a.per + ch0, size = (int64_t)a.D * a.N;
+  const int cb = grp * a.per + ch0, size = a.D * a.N;
   const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
-  const int64_t mine = cb + cl * 4;
+  const int mine = cb + cl * 4;
   const int has = left - cl * 4;
   const int64_t rows = a.st.rows, c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, rows);
 
@@ -465,11 +470,11 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
 #pragma unroll
     for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], both(kLog2e));
   r.zero();
-  const int64_t s = owner(a.st, c0);
+  const int s = owner(a.st, c0);
   const bool in = s >= 0 && s < a.st.seqs && a.st[s] < c0;      // a sequence comes in
   const int64_t end = in ? a.st[s + 1] : c0, e = min(end, c1);
   if (ct == 0 && lane == 0) a.cut[chunk - 1] = !in || end <= c1;
-  if (in && end <= c1 && a.dfin) r.load(a.dfin + s * size, mine, has, n0, a);
+  if (in && end <= c1 && a.dfin) r.load(a.dfin + (int64_t)s * size, mine, has, n0, a);
 
   float bias[X::W];
 #pragma unroll
@@ -516,13 +521,13 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
       for (int p = 0; p < 2; ++p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          r.v[p][k] = mul2(ex2_2(mul2(dt2[p], A2.v[p][k])), fma2(C[k], gv[p], r.v[p][k]));
+          r.v[p][k] = mul2(decays(dt2[p], A2.v[p][k]), fma2(C[k], gv[p], r.v[p][k]));
         total[p] = add2(total[p], dt2[p]);
       }
     }
     __syncwarp();
   }
-  r.store(a.edge + (chunk - 1) * size, mine, has, n0, a);
+  r.store(a.edge + (chunk - 1) * (int64_t)size, mine, has, n0, a);
   if (nl == 0) {
     const float2 x = unpack(total[0]), y = unpack(total[1]);
     const float t[4] = {x.x, x.y, y.x, y.y};
@@ -532,47 +537,57 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
   }
 }
 
+// Pairs of channels a thread of the backward holds: one, but for the widest
+// states, whose warps would have fewer elements than lanes.
+template <int NP> constexpr int kBwdPairs = NP > 32 ? 2 : 1;
+
 template <int NP> struct BwdSmem {
-  static constexpr int CH = Lay<NP, 1>::CH;
+  static constexpr int P = kBwdPairs<NP>, CH = Lay<NP, P>::CH;
   float dt[kWarps][kTile][CH], dtu[kWarps][kTile][CH], gv[kWarps][kTile][CH];
-  float out[kWarps][3][kTile][CH];                               // <g, B>, <q, A log2 e>, <C, h>
+  float out[kWarps][3][kHalf][2 * P][32];                            // each lane's part of <g, B>, <q, A log2 e>, <C, h>
   float2 B[kTile][NP], C[kTile][NP];
-  float sum[kWarps][kTile][2 * NP];                              // the warps' sums over channels: dB, dC
-  int64_t seq[kWarps][kTile + 1];                                // of the rows in front of and at beginnings
+  float4 sum[kWarps][kHalf][2][32];                              // each lane's part of dB, dC of its states
+  float4 own[kWarps][Lay<NP, P>::X::E][32];                      // u, dy silu'(z), softplus', dt of each lane's elements
+  int seq[kWarps][kTile + 1];                                    // of the rows in front of and at beginnings
 };
 
 // All gradients of a chunk's rows.  The warps of a CTA stand side by side on a
-// group's channels and add up their parts of dB and dC tile by tile.
-template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_scan_bwd(ScanArgs a) {
-  using L = Lay<NP, 1>;
+// group's channels and add up their parts of dB and dC.
+template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 32 ? 2 : kBwdCtas) k_scan_bwd(ScanArgs a) {
+  constexpr int P = kBwdPairs<NP>;
+  using L = Lay<NP, P>;
   using X = typename L::X;
   fb::pdl_enter();
   extern __shared__ __align__(16) unsigned char dyn[];
   BwdSmem<NP> &sm = *reinterpret_cast<BwdSmem<NP> *>(dyn);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int grp = blockIdx.x / a.ctas, cta = blockIdx.x % a.ctas;
-  const int64_t chunk = blockIdx.y;
+  const int chunk = blockIdx.y;
   const int ch0 = (cta * kWarps + warp) * L::CH, left = a.per - ch0;        // may be <= 0: a warp without channels
-  const int64_t cb = (int64_t)grp * a.per + ch0, size = (int64_t)a.D * a.N;
+  const int cb = grp * a.per + ch0, size = a.D * a.N;
   const int nl = lane % L::NL, cl = lane / L::NL, n0 = nl * 4;
-  const int64_t mine = cb + cl * 2;
-  const int has = left - cl * 2;
+  const int mine = cb + cl * (2 * P);
+  const int has = left - cl * (2 * P);
   const int64_t rows = a.st.rows, c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, rows);
-  const int64_t lo = a.st[0], hi = min(a.st[a.st.seqs], c1);
+  // from here on rows are counted from c0
+  const int len = (int)(c1 - c0), lo = (int)max((int64_t)0, min(a.st[0] - c0, (int64_t)len)),
+            hi = (int)max((int64_t)0, min(a.st[a.st.seqs] - c0, (int64_t)len));
 
-  States<1> A2, r, dA;
+  States<P> A2, r, dA;
   A2.load(a.A, mine, has, n0, a);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) A2.v[0][k] = mul2(A2.v[0][k], both(kLog2e));
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], both(kLog2e));
   dA.zero();
   r.zero();
   {
-    const int64_t s = owner(a.st, c1 - 1);
+    const int s = owner(a.st, c1 - 1);
     const bool in = s >= 0 && s < a.st.seqs;
     if (c1 >= rows || !in || a.st[s + 1] <= c1) {
-      if (in && a.dfin) r.load(a.dfin + s * size, mine, has, n0, a);
+      if (in && a.dfin) r.load(a.dfin + (int64_t)s * size, mine, has, n0, a);
     } else {
-      r.load(a.edge + chunk * size, mine, has, n0, a);
+      r.load(a.edge + chunk * (int64_t)size, mine, has, n0, a);
     }
   }
 
@@ -586,8 +601,9 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
   const T none = from_f<T>(0.f);
   constexpr int EC = kTile * NP / kThreads > 0 ? kTile * NP / kThreads : 1;  // B (and C) elements a thread of the CTA
   T xu[X::E], xd[X::E], xy[X::E], xz[X::E], xb[EC], xc[EC];
-  const auto fetch = [&](int64_t r0) {
-    const int ra = rows_in(lo - r0), rb = rows_in(hi - r0);
+  const auto fetch = [&](int t0) {
+    const int ra = min(max(lo - t0, 0), kTile), rb = t0 >= 0 ? min(max(hi - t0, 0), kTile) : 0;
+    const int64_t r0 = c0 + t0;
     X::fetch(xu, a.u, r0 * a.ldu + cb, a.ldu, left, ra, rb);
     X::fetch(xd, a.delta, r0 * a.ldd + cb, a.ldd, left, ra, rb);
     X::fetch(xy, a.dy, r0 * a.lddy + cb, a.lddy, left, ra, rb);
@@ -601,28 +617,36 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
     }
   };
 
-  int64_t r0 = c0 + (c1 - 1 - c0) / kTile * kTile;
   WalkDown walk;
   walk.begin(a.st, c1 - 1);
-  fetch(r0);
-  for (; r0 >= c0; r0 -= kTile) {
-    // ---- the tile's rows, once for each (row, channel)
-    const int ra = rows_in(lo - r0), rb = rows_in(hi - r0);
-    float ku[X::E], ky[X::E], kz[X::E], kdt[X::E], ksl[X::E];
-    steps<true, X>(xd, bias, a.softplus, kdt, ksl);
+  int t0 = (len - 1) / kTile * kTile;
+  fetch(t0);
+  for (; t0 >= 0; t0 -= kTile) {
+    // ---- the tile's rows, once for each (row, channel); rows of no sequence were fetched as zeros
+    {
+      const int ra = lo - t0, rb = hi - t0;
+      float dt[X::E], slope[X::E];
+      steps<true, X>(xd, bias, a.softplus, dt, slope);
 #pragma unroll
-    for (int i = 0; i < X::E; ++i) {
-      ku[i] = to_f(xu[i]), ky[i] = to_f(xy[i]), kz[i] = 0.f;
-      float gv = ky[i];
-      if (a.z) {
-        kz[i] = to_f(xz[i]);
-        gv *= kz[i] * sigmoid(kz[i]);
+      for (int i = 0; i < X::E; i += 2) {
+        const F2 u = pack(to_f(xu[i]), to_f(xu[i + 1])), dy = pack(to_f(xy[i]), to_f(xy[i + 1]));
+        F2 gv = dy, dg = both(0.f);
+        if (a.z) {
+          const F2 z = pack(to_f(xz[i]), to_f(xz[i + 1])), sg = sigmoid2(z), zs = mul2(z, sg);
+          gv = mul2(dy, zs);
+          dg = mul2(dy, fma2(mul2(zs, sg), both(-1.f), add2(sg, zs)));     // sg (1 + z (1 - sg))
+        }
+        const F2 v = pack(only<X>(dt[i], i, ra, rb), only<X>(dt[i + 1], i + 1, ra, rb));
+        const float2 fu = unpack(u), fg = unpack(gv), fd = unpack(dg), fv = unpack(v), fp = unpack(mul2(v, u));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = X::row(i + j), c = X::col(i + j);
+          sm.dt[warp][row][c] = j ? fv.y : fv.x;
+          sm.dtu[warp][row][c] = j ? fp.y : fp.x;
+          sm.gv[warp][row][c] = j ? fg.y : fg.x;
+          sm.own[warp][i + j][lane] = j ? make_float4(fu.y, fd.y, slope[i + 1], fv.y) : make_float4(fu.x, fd.x, slope[i], fv.x);
+        }
       }
-      kdt[i] = only<X>(kdt[i], i, ra, rb);
-      const int row = X::row(i), c = X::col(i);
-      sm.dt[warp][row][c] = kdt[i];
-      sm.dtu[warp][row][c] = kdt[i] * ku[i];
-      sm.gv[warp][row][c] = gv;
     }
 #pragma unroll
     for (int i = 0; i < EC; ++i) {
@@ -633,135 +657,185 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
         sm.C[at / NP][at % NP] = make_float2(c, c);
       }
     }
-    const unsigned begins = walk.tile(r0);
+    const unsigned begins = walk.tile(a.st, c0 + t0);
     if (begins && (a.init || a.dfin || a.dinit)) {
 #pragma unroll 1
       for (int i = 0; i <= kTile; ++i) {
-        const int64_t s = owner(a.st, r0 + i - 1);
+        const int s = owner(a.st, c0 + t0 + i - 1);
         if (lane == 0) sm.seq[warp][i] = s >= 0 && s < a.st.seqs ? s : -1;
       }
     }
-    States<1> h0, h;
-    h0.load(a.keep + r0 / kTile * size, mine, has, n0, a);
-    if (r0 - kTile >= c0) fetch(r0 - kTile);
+    States<P> from;                                              // the state in front of the rows in work
+    from.load(a.keep + (c0 + t0) / kTile * size, mine, has, n0, a);
     __syncthreads();
 
-    // ---- states and decays of the 8 rows
-    F2 hs[kTile][4], as[kTile][4];
     // What a sequence finds that begins at row i of the tile.
-    const auto found = [&](States<1> &x, int i) {
+    const auto found = [&](States<P> &x, int i) {
       x.zero();
       if (a.init) {
-        const int64_t s = sm.seq[warp][i + 1];
-        if (s >= 0) x.load(a.init + s * size, mine, has, n0, a);
+        const int s = sm.seq[warp][i + 1];
+        if (s >= 0) x.load(a.init + (int64_t)s * size, mine, has, n0, a);
       }
     };
-    h = h0;
-#pragma unroll
-    for (int i = 0; i < kTile; ++i) {
-      if (begins >> i & 1u) found(h, i);
-      const F2 dt = {*reinterpret_cast<const unsigned long long *>(&sm.dt[warp][i][cl * 2])};
-      const F2 dtu = {*reinterpret_cast<const unsigned long long *>(&sm.dtu[warp][i][cl * 2])};
-      const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
-      const F2 B[4] = {{b[0].x}, {b[0].y}, {b[1].x}, {b[1].y}};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        as[i][k] = ex2_2(mul2(dt, A2.v[0][k]));
-        h.v[0][k] = fma2(as[i][k], h.v[0][k], mul2(dtu, B[k]));
-        hs[i][k] = h.v[0][k];
-      }
-    }
-    // ---- back up the rows
-    States<1> tA;                                                // the tile's part of dA: short sums round less
-    tA.zero();
-#pragma unroll
-    for (int i = kTile - 1; i >= 0; --i) {
-      const F2 dt = {*reinterpret_cast<const unsigned long long *>(&sm.dt[warp][i][cl * 2])};
-      const F2 dtu = {*reinterpret_cast<const unsigned long long *>(&sm.dtu[warp][i][cl * 2])};
-      const F2 gv = {*reinterpret_cast<const unsigned long long *>(&sm.gv[warp][i][cl * 2])};
-      const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(&sm.B[i][n0]);
-      const ulonglong2 *c = reinterpret_cast<const ulonglong2 *>(&sm.C[i][n0]);
-      const F2 B[4] = {{b[0].x}, {b[0].y}, {b[1].x}, {b[1].y}}, C[4] = {{c[0].x}, {c[0].y}, {c[1].x}, {c[1].y}};
-      States<1> before;
-      if (begins >> i & 1u) {
-        found(before, i);
+    // The pairs' dt, dt u or gv of a row; B or C of the states, twice each.
+    const auto pairs = [&](const float (&p)[kTile][L::CH], int i, F2 (&v)[P]) {
+      if constexpr (P == 1) {
+        v[0].v = *reinterpret_cast<const unsigned long long *>(&p[i][cl * 2]);
       } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) before.v[0][k] = i ? hs[i - 1][k] : h0.v[0][k];
+        const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(&p[i][cl * 4]);
+        v[0].v = t.x, v[1].v = t.y;
       }
-      F2 gB, qA, cy;
-      float bc[8];
+    };
+    const auto twice = [&](const float2 (&p)[kTile][NP], int i, F2 (&v)[4]) {
+      const ulonglong2 *t = reinterpret_cast<const ulonglong2 *>(&p[i][n0]);
+      v[0].v = t[0].x, v[1].v = t[0].y, v[2].v = t[1].x, v[3].v = t[1].y;
+    };
+    // h behind row i; the decays of the first pair are kept
+    const auto ahead = [&](int i, States<P> &h, F2 (&kept)[4]) {
+      F2 dt[P], dtu[P], B[4];
+      pairs(sm.dt[warp], i, dt), pairs(sm.dtu[warp], i, dtu), twice(sm.B, i, B);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const F2 g = fma2(C[k], gv, r.v[0][k]);
-        r.v[0][k] = mul2(as[i][k], g);
-        const F2 q = mul2(r.v[0][k], before.v[0][k]);
-        gB = k == 0 ? mul2(g, B[k]) : fma2(g, B[k], gB);
-        qA = k == 0 ? mul2(q, A2.v[0][k]) : fma2(q, A2.v[0][k], qA);
-        cy = k == 0 ? mul2(C[k], hs[i][k]) : fma2(C[k], hs[i][k], cy);
-        tA.v[0][k] = fma2(q, dt, tA.v[0][k]);
-        const float2 vb = unpack(mul2(g, dtu)), vc = unpack(mul2(gv, hs[i][k]));
-        bc[k] = vb.x + vb.y, bc[4 + k] = vc.x + vc.y;
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const F2 d = decays(dt[p], A2.v[p][k]);
+          if (p < kKept) kept[k] = d;
+          h.v[p][k] = fma2(d, h.v[p][k], mul2(dtu[p], B[k]));
+        }
+    };
+    // BEGINS: some row of the tile begins a sequence.
+    const auto half = [&](auto some, auto from_row) {
+      constexpr bool BEGINS = decltype(some)::value;
+      constexpr int at = decltype(from_row)::value;
+      F2 as[kHalf][4];
+      if constexpr (at > 0) {
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i) {
+          if (BEGINS && (begins >> i & 1u)) found(from, i);
+          ahead(i, from, as[0]);
+        }
+      } else {
+        from.load(a.keep + (c0 + t0) / kTile * size, mine, has, n0, a);
       }
-      const float2 vg = unpack(gB), vq = unpack(qA), vy = unpack(cy);
-      float s4[4] = {vg.x, vg.y, vq.x, vq.y}, s2[2] = {vy.x, vy.y};
-      const int at4 = spread_sum<4, L::NL, 1>(s4), at2 = spread_sum<2, L::NL, 1>(s2);
-      constexpr int kOwn4 = L::NL >= 4 ? 1 : 4 / L::NL, kOwn2 = L::NL >= 2 ? 1 : 2;
+      // ---- states of half the rows
+      States<P> hs[kHalf];
 #pragma unroll
-      for (int k = 0; k < kOwn4; ++k) sm.out[warp][(at4 + k) >> 1][i][cl * 2 + ((at4 + k) & 1)] = s4[k];
-#pragma unroll
-      for (int k = 0; k < kOwn2; ++k) sm.out[warp][2][i][cl * 2 + at2 + k] = s2[k];
-      const int atc = spread_sum<8, L::CL, L::NL>(bc);
-      constexpr int kOwnC = L::CL >= 8 ? 1 : 8 / L::CL;
-#pragma unroll
-      for (int k = 0; k < kOwnC; ++k) sm.sum[warp][i][((atc + k) >> 2) * NP + n0 + ((atc + k) & 3)] = bc[k];
-      if (begins >> i & 1u) {
-        if (a.dinit && sm.seq[warp][i + 1] >= 0) r.store(a.dinit + sm.seq[warp][i + 1] * size, mine, has, n0, a);
-        r.zero();
-        if (a.dfin && sm.seq[warp][i] >= 0) r.load(a.dfin + sm.seq[warp][i] * size, mine, has, n0, a);
+      for (int j = 0; j < kHalf; ++j) {
+        hs[j] = j ? hs[j - 1] : from;
+        if (BEGINS && (begins >> (at + j) & 1u)) found(hs[j], at + j);
+        ahead(at + j, hs[j], as[j]);
       }
-    }
+      // ---- back up the rows
 #pragma unroll
-    for (int k = 0; k < 4; ++k) dA.v[0][k] = add2(dA.v[0][k], tA.v[0][k]);
-    __syncthreads();
+      for (int j = kHalf - 1; j >= 0; --j) {
+        const int i = at + j;
+        F2 dt[P], dtu[P], gv[P], B[4], C[4];
+        pairs(sm.dt[warp], i, dt), pairs(sm.dtu[warp], i, dtu), pairs(sm.gv[warp], i, gv);
+        twice(sm.B, i, B), twice(sm.C, i, C);
+        States<P> before = j ? hs[j - 1] : from;
+        if (BEGINS && (begins >> i & 1u)) found(before, i);
+        F2 gB[P], qA[P], cy[P];
+        float vb[4], vc[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          F2 sb, sc;
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            const F2 g = fma2(C[k], gv[p], r.v[p][k]), h = hs[j].v[p][k];
+            r.v[p][k] = mul2(p < kKept ? as[j][k] : decays(dt[p], A2.v[p][k]), g);
+            const F2 q = mul2(r.v[p][k], before.v[p][k]);
+            gB[p] = k == 0 ? mul2(g, B[k]) : fma2(g, B[k], gB[p]);
+            qA[p] = k == 0 ? mul2(q, A2.v[p][k]) : fma2(q, A2.v[p][k], qA[p]);
+            cy[p] = k == 0 ? mul2(C[k], h) : fma2(C[k], h, cy[p]);
+            dA.v[p][k] = fma2(q, dt[p], dA.v[p][k]);
+            sb = p == 0 ? mul2(g, dtu[p]) : fma2(g, dtu[p], sb);
+            sc = p == 0 ? mul2(gv[p], h) : fma2(gv[p], h, sc);
+          }
+          const float2 x = unpack(sb), y = unpack(sc);
+          vb[k] = x.x + x.y, vc[k] = y.x + y.y;
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const float2 v[3] = {unpack(gB[p]), unpack(qA[p]), unpack(cy[p])};
+#pragma unroll
+          for (int m = 0; m < 3; ++m) {
+            sm.out[warp][m][j][2 * p][lane ^ L::turn(16 / P * (2 * p))] = v[m].x;
+            sm.out[warp][m][j][2 * p + 1][lane ^ L::turn(16 / P * (2 * p + 1))] = v[m].y;
+          }
+        }
+        sm.sum[warp][j][0][lane] = make_float4(vb[0], vb[1], vb[2], vb[3]);
+        sm.sum[warp][j][1][lane] = make_float4(vc[0], vc[1], vc[2], vc[3]);
+        if (BEGINS && (begins >> i & 1u)) {
+          if (a.dinit && sm.seq[warp][i + 1] >= 0) r.store(a.dinit + (int64_t)sm.seq[warp][i + 1] * size, mine, has, n0, a);
+          r.zero();
+          if (a.dfin && sm.seq[warp][i] >= 0) r.load(a.dfin + (int64_t)sm.seq[warp][i] * size, mine, has, n0, a);
+        }
+      }
+    };
+    const auto both_ways = [&](auto from_row) {
+      constexpr int at = decltype(from_row)::value;
+      if (begins) half(std::true_type{}, from_row);
+      else half(std::false_type{}, from_row);
+      if constexpr (at == 0) fetch(t0 - kTile);                  // nothing in front of the chunk
+      __syncthreads();
 
-    // ---- results of the tile
-    const int end = rows_in(c1 - r0);
-    const int64_t to = (r0 + X::row(0)) * a.D + cb + X::col(0);
+      // ---- results of the half
+      const int end = len - t0;
+      const int64_t to = (c0 + t0 + X::row(0)) * a.D + cb + X::col(0);
+      const int skipped = at ? X::E / 2 : 0;                     // the lane's elements of the other half
 #pragma unroll
-    for (int i = 0; i < X::E; ++i) {
-      const int row = X::row(i), c = X::col(i), w = i % X::W;
-      if (row >= end || c >= left) continue;
-      const int64_t q = to + i / X::W * X::RS * (int64_t)a.D + 32 * w;
-      const float gB = sm.out[warp][0][row][c], qA = sm.out[warp][1][row][c] * 0.6931471805599453f;
-      float gv = ky[i];
-      if (a.z) {
-        const float sg = sigmoid(kz[i]), v = fmaf(skip[w], ku[i], sm.out[warp][2][row][c]);
-        gv *= kz[i] * sg;
-        const float dz = ky[i] * v * sg * fmaf(kz[i], 1.f - sg, 1.f);
-        static_cast<T *>(a.dz)[q] = from_f<T>(only<X>(dz, i, ra, rb));
+      for (int e = 0; e < X::E / 2; ++e) {
+        const int i = e + skipped, row = X::row(0) + X::RS * (i / X::W), w = e % X::W, c = X::col(w);
+        const float4 own = sm.own[warp][i][lane];
+        const auto total = [&](int m) {
+          return lanes_sum<L::NL>(&sm.out[warp][m][row - at][c % (2 * P)][(c / (2 * P) * L::NL) ^ L::turn(16 / P * (c % (2 * P)))]);
+        };
+        const float gB = total(0), qA = total(1) * 0.6931471805599453f, gv = sm.gv[warp][row][c];
+        const float dd = fmaf(own.x, gB, qA) * own.z;
+        if (row >= end || c >= left) continue;
+        sumD[w] = fmaf(gv, own.x, sumD[w]), sumb[w] += dd;
+        const int64_t q = to + i / X::W * X::RS * (int64_t)a.D + 32 * w;
+        if (a.z) static_cast<T *>(a.dz)[q] = from_f<T>(fmaf(skip[w], own.x, total(2)) * own.y);
+        static_cast<T *>(a.du)[q] = from_f<T>(fmaf(own.w, gB, skip[w] * gv));
+        static_cast<T *>(a.ddelta)[q] = from_f<T>(dd);
       }
-      const float dd = only<X>(fmaf(ku[i], gB, qA) * ksl[i], i, ra, rb);
-      static_cast<T *>(a.du)[q] = from_f<T>(only<X>(fmaf(kdt[i], gB, skip[w] * gv), i, ra, rb));
-      static_cast<T *>(a.ddelta)[q] = from_f<T>(dd);
-      sumD[w] = fmaf(gv, ku[i], sumD[w]), sumb[w] += dd;
-    }
-    for (int at = threadIdx.x; at < kTile * 2 * NP; at += kThreads) {
-      const int row = at / (2 * NP), col = at % (2 * NP);
-      const int64_t q = r0 + row;
-      if (q >= c1) break;
-      float v = 0.f;
+      // dB and dC of 4 states of a row: kParts threads share the lanes' parts
+      constexpr int kSums = kHalf * 2 * L::NL, kParts = kSums < kThreads ? kThreads / kSums : 1;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += sm.sum[w][row][col];
-      if (a.ctas > 1) {
-        a.pBC[(blockIdx.x * rows + q) * (2 * NP) + col] = v;
-      } else if (col % NP < a.N) {
-        static_cast<T *>(col < NP ? a.dB : a.dC)[(q * a.G + grp) * a.N + col % NP] = from_f<T>(v);
+      for (int t = threadIdx.x; t < kSums * kParts; t += kThreads) {
+        const int l = t % L::NL, part = t / L::NL % kParts, which = t / (L::NL * kParts) % 2, row = t / (L::NL * kParts * 2);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+          for (int m = part; m < L::CL; m += kParts) {
+            const float4 f = sm.sum[w][row][which][m * L::NL + l];
+            v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+          }
+#pragma unroll
+        for (int o = L::NL; o < L::NL * kParts; o *= 2) {
+          v.x += __shfl_xor_sync(0xffffffffu, v.x, o), v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+          v.z += __shfl_xor_sync(0xffffffffu, v.z, o), v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
+        }
+        if (at + row >= end || part) continue;
+        const int64_t q = c0 + t0 + at + row;
+        if (a.ctas > 1) {
+          *reinterpret_cast<float4 *>(&a.pBC[(blockIdx.x * rows + q) * (2 * NP) + which * NP + l * 4]) = v;
+        } else {
+          T *const p = static_cast<T *>(which ? a.dC : a.dB) + (q * a.G + grp) * a.N + l * 4;
+          const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (l * 4 + k < a.N) p[k] = from_f<T>(f[k]);
+        }
       }
-    }
+      if (at) __syncthreads();
+    };
+    both_ways(std::integral_constant<int, kHalf>{});
+    both_ways(std::integral_constant<int, 0>{});
   }
 
-  dA.store((a.nc > 1 ? a.pA + chunk * size : a.dA), mine, has, n0, a);
+  dA.store((a.nc > 1 ? a.pA + chunk * (int64_t)size : a.dA), mine, has, n0, a);
 #pragma unroll
   for (int w = 0; w < X::W; ++w) {
     if (L::CH < 32) {
@@ -773,17 +847,17 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 2) k_s
     }
     const int c = X::col(w);
     if (c < left && lane < L::CH) {
-      if (a.nc > 1) a.pD[(chunk * 2) * a.D + cb + c] = sumD[w], a.pD[(chunk * 2 + 1) * a.D + cb + c] = sumb[w];
+      if (a.nc > 1) a.pD[chunk * 2 * (int64_t)a.D + cb + c] = sumD[w], a.pD[(chunk * 2 + 1) * (int64_t)a.D + cb + c] = sumb[w];
       else a.dD[cb + c] = sumD[w], a.dbias[cb + c] = sumb[w];
     }
   }
   if (a.dinit) {
-    for (int64_t q = chunk; q < a.st.seqs; q += 32 * (int64_t)a.nc) {          // empty sequences: dfinal passes through
-      const int64_t e = q + lane * (int64_t)a.nc;
+    for (int q = (int)chunk; q < a.st.seqs; q += 32 * a.nc) {          // empty sequences: dfinal passes through
+      const int e = q + lane * a.nc;
       unsigned m = __ballot_sync(0xffffffffu, e < a.st.seqs && a.st[e] >= a.st[e + 1]);
       for (; m; m &= m - 1) {
-        const int64_t s0 = q + (__ffs(m) - 1) * (int64_t)a.nc;
-        States<1> x;
+        const int64_t s0 = q + (__ffs(m) - 1) * a.nc;
+        States<P> x;
         x.zero();
         if (a.dfin) x.load(a.dfin + s0 * size, mine, has, n0, a);
         x.store(a.dinit + s0 * size, mine, has, n0, a);
@@ -829,13 +903,22 @@ template <typename T> __global__ void __launch_bounds__(256) k_scan_sums(ScanArg
 // ---- host ------------------------------------------------------------------------------------------
 int padded(int N) { return N <= 8 ? 8 : (N <= 16 ? 16 : (N <= 32 ? 32 : 64)); }
 
-// Rows of a chunk: enough warps to fill the SMs (kBusy of them), but no chunk
-// below kShort rows.
-int64_t chunk_rows(int64_t rows, int64_t tiles, int64_t busy, int64_t shortest) {
-  const int64_t want = std::max<int64_t>(1, busy / std::max<int64_t>(1, tiles));
-  int64_t c = (rows + want - 1) / want;
-  c = std::max(c, shortest);
-  return (c + kTile - 1) / kTile * kTile;
+// Rows of a chunk, for `tiles` units of work side by side of which the GPU holds
+// `resident`: whole waves of units, three if the chunks stay at kShort rows, for
+// then early ends of some chunks even out (16,384 x 1,024 backward: 922 us with
+// one wave, 881 with two, 866 with three), else two or one.
+constexpr int64_t kShort = 64;
+int64_t chunk_rows(int64_t rows, int64_t tiles, int64_t resident) {
+  int64_t c = kShort;
+  for (int64_t waves = 3; waves; --waves) {
+    const int64_t want = std::max<int64_t>(1, resident * waves / tiles);
+    const int64_t even = ((rows + want - 1) / want + kTile - 1) / kTile * kTile;
+    if (even >= kShort) {
+      c = even;
+      break;
+    }
+  }
+  return c;
 }
 
 int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
@@ -847,7 +930,7 @@ int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
   if (!s->starts && s->seqs != 1) return bad("without starts there is one sequence");
   if (s->starts_type != FB_I32 && s->starts_type != FB_I64) return bad("unknown type of starts");
   if (s->N > kMaxStates) return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan: at most 64 states");
-  if (s->D > (1 << 20) || s->rows > (int64_t)1 << 40 || s->seqs > (int64_t)1 << 40)
+  if (s->D > (1 << 20) || s->rows > (int64_t)1 << 40 || s->seqs > (1 << 30))
     return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan: sizes beyond what the kernels index");
   if (s->rows && (!s->u || !s->delta || !s->B || !s->C)) return bad("missing operand");
   if (!s->A) return bad("missing operand");
@@ -866,7 +949,7 @@ int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
   a.y = s->y, a.ldy = s->ldy, a.keep = s->keep;
   a.dy = s->dy, a.lddy = s->lddy, a.du = s->du, a.ddelta = s->ddelta, a.dz = s->dz, a.dB = s->dB, a.dC = s->dC;
   a.dA = s->dA, a.dD = s->dD, a.dbias = s->ddelta_bias, a.dfin = s->dfinal, a.dinit = s->dinit;
-  a.st = Starts{s->starts, s->starts_type == FB_I64, s->seqs, s->rows};
+  a.st = Starts{s->starts, s->starts_type == FB_I64, (int)s->seqs, s->rows};
   const uintptr_t at = (uintptr_t)s->A | (uintptr_t)s->init | (uintptr_t)s->final | (uintptr_t)s->keep | (uintptr_t)s->dfinal |
                        (uintptr_t)s->dinit | (uintptr_t)s->dA;
   a.vec = s->N % 4 == 0 && at % 16 == 0;
@@ -874,13 +957,12 @@ int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
 }
 
 constexpr int64_t kSms = 148;
-int64_t knob(const char *n, int64_t d) { const char *e = getenv(n); return e ? atoll(e) : d; }
 
 // The forward's split, and its pieces of the workspace.
 int plan_fwd(ScanArgs &a, int np, fbh::Call &c) {
   const int ch = 2 * 2 * 32 / (np / 4);
   a.tiles = (a.per + ch - 1) / ch;
-  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * knob("FB_FW", 24), knob("FB_FL", 64));
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * 16);
   a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
   if (a.nc > 1) {
     FBH_TAKE(edge, c, float, (a.nc - 1) * (int64_t)a.D * a.N);
@@ -892,12 +974,12 @@ int plan_fwd(ScanArgs &a, int np, fbh::Call &c) {
 }
 
 int plan_bwd(ScanArgs &a, int np, fbh::Call &c) {
-  const int ch = 2 * 32 / (np / 4);                       // channels of a warp
+  const int ch = 2 * (np > 32 ? 2 : 1) * 32 / (np / 4);   // channels of a warp
   const int tiles = (a.per + ch - 1) / ch;
   a.ctas = (tiles + kWarps - 1) / kWarps;
-  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.ctas, kSms * knob("FB_BW", 4), knob("FB_BL", 64));
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.ctas, kSms * (np > 32 ? 2 : kBwdCtas));
   a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
-  a.tiles = (a.per + 2 * ch - 1) / (2 * ch);              // k_scan_rev's
+  a.tiles = (a.per + 4 * 32 / (np / 4) - 1) / (4 * 32 / (np / 4));          // k_scan_rev's
   const int64_t size = (int64_t)a.D * a.N;
   if (a.nc > 1) {
     FBH_TAKE(edge, c, float, (a.nc - 1) * size);
@@ -916,20 +998,28 @@ int plan_bwd(ScanArgs &a, int np, fbh::Call &c) {
 
 unsigned blocks(int64_t n, int64_t each) { return (unsigned)((n + each - 1) / each); }
 
+// Shared memory above what a launch has without asking.
+template <typename K> int allow(K *kernel, size_t bytes) {
+  if (bytes > 48 * 1024) FB_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return FB_OK;
+}
+
 template <typename T, int NP> int run_fwd(const ScanArgs &a, cudaStream_t stream) {
   const int64_t nct = (int64_t)a.G * a.tiles;
+  constexpr size_t smem = sizeof(FwdSmem<NP>) * kWarps;
+  FBH_TRY((allow(k_scan_fwd<T, NP, true>, smem)));
+  FBH_TRY((allow(k_scan_fwd<T, NP, false>, smem)));
   if (a.nc > 1) {
-    FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, true>, blocks(nct * (a.nc - 1), kWarps), kThreads, 0, stream, a));
+    FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, true>, blocks(nct * (a.nc - 1), kWarps), kThreads, smem, stream, a));
     FB_TRY_CUDA(fb::launch(k_scan_join<false>, blocks((int64_t)a.D * a.N, 256), 256, 0, stream, a));
   }
-  FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, false>, blocks(nct * a.nc, kWarps), kThreads, 0, stream, a));
+  FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, false>, blocks(nct * a.nc, kWarps), kThreads, smem, stream, a));
   return FB_OK;
 }
 
 template <typename T, int NP> int run_bwd(const ScanArgs &a, cudaStream_t stream) {
   constexpr size_t smem = sizeof(BwdSmem<NP>);
-  if (smem > 48 * 1024)
-    FB_TRY_CUDA(cudaFuncSetAttribute(k_scan_bwd<T, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  FBH_TRY((allow(k_scan_bwd<T, NP>, smem)));
   if (a.nc > 1) {
     const int64_t nct = (int64_t)a.G * a.tiles;
     FB_TRY_CUDA(fb::launch(k_scan_rev<T, NP>, blocks(nct * (a.nc - 1), kWarps), kThreads, 0, stream, a));

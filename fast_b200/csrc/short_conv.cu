@@ -39,11 +39,11 @@ struct ConvArgs {
 };
 
 // Sequence of a row, for one thread (few threads ask).
-__device__ __forceinline__ int64_t owner1(const Starts &st, int64_t row) {
+__device__ __forceinline__ int owner1(const Starts &st, int64_t row) {
   if (!st.p) return row < 0 ? -1 : (row < st.rows ? 0 : 1);
-  int64_t lo = 0, hi = st.seqs + 1;
+  int lo = 0, hi = st.seqs + 1;
   while (lo < hi) {
-    const int64_t m = (lo + hi) >> 1;
+    const int m = lo + ((hi - lo) >> 1);
     if (st[m] <= row) lo = m + 1;
     else hi = m;
   }
@@ -72,7 +72,7 @@ __device__ __forceinline__ void fill_begins(const Starts &st, int64_t from, int 
   walk.begin(st, from + 8 * (int64_t)a);
   for (int i = a; i < b; ++i) {
     const int64_t r0 = from + 8 * (int64_t)i;
-    const unsigned m = r0 < 0 ? 0u : walk.tile(r0);
+    const unsigned m = r0 < 0 ? 0u : walk.tile(st, r0);
     if ((threadIdx.x & 31) == 0) bits[i] = (uint8_t)m;
   }
 }
@@ -300,10 +300,10 @@ __global__ void __launch_bounds__(256) k_conv_sums(ConvArgs a) {
 // final[s, m]: input number len - (K - 1) + m of sequence s; one thread an element.
 template <typename T> __global__ void __launch_bounds__(256) k_conv_final(ConvArgs a) {
   fb::pdl_enter();
-  const int64_t n = a.st.seqs * (a.K - 1) * (int64_t)a.D;
+  const int64_t n = (int64_t)a.st.seqs * (a.K - 1) * a.D;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t d = i % a.D, m = i / a.D % (a.K - 1), s = i / a.D / (a.K - 1);
-    const int64_t b = a.st[s], e = max(a.st[s + 1], b), p = e - b - (a.K - 1) + m;
+    const int64_t b = a.st[(int)s], e = max(a.st[(int)s + 1], b), p = e - b - (a.K - 1) + m;
     T v = from_f<T>(0.f);
     if (p >= 0) v = static_cast<const T *>(a.x)[(b + p) * a.ldx + d];
     else if (a.init) v = static_cast<const T *>(a.init)[(s * (a.K - 1) + a.K - 1 + p) * a.D + d];
@@ -314,9 +314,9 @@ template <typename T> __global__ void __launch_bounds__(256) k_conv_final(ConvAr
 // dinit[s, m] = sum_{i <= m, i < len} w[m - i] dp[i] (+ dfinal[s, m - len]); one thread for a (sequence, column).
 template <typename T> __global__ void __launch_bounds__(256) k_conv_dinit(ConvArgs a) {
   fb::pdl_enter();
-  const int64_t n = a.st.seqs * (int64_t)a.D;
+  const int64_t n = (int64_t)a.st.seqs * a.D;
   for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < n; j += (int64_t)gridDim.x * 256) {
-    const int64_t d = j % a.D, s = j / a.D, b = a.st[s], len = max(a.st[s + 1] - b, (int64_t)0);
+    const int64_t d = j % a.D, s = j / a.D, b = a.st[(int)s], len = max(a.st[(int)s + 1] - b, (int64_t)0);
     const int K = a.K;
     const T *init = static_cast<const T *>(a.init) + s * (K - 1) * a.D + d;
     float w[kMaxTaps], x[2 * kMaxTaps], g[kMaxTaps];
@@ -349,7 +349,7 @@ int fill(const fb_short_conv *s, ConvArgs &a, bool backward) {
   if (!s->starts && s->seqs != 1) return bad("without starts there is one sequence");
   if (s->starts_type != FB_I32 && s->starts_type != FB_I64) return bad("unknown type of starts");
   if (s->K > kMaxTaps) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv: at most 8 taps");
-  if (s->D > (1 << 20) || s->rows > (int64_t)1 << 40 || s->seqs > (int64_t)1 << 40)
+  if (s->D > (1 << 20) || s->rows > (int64_t)1 << 40 || s->seqs > (1 << 30))
     return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv: sizes beyond what the kernels index");
   if (!s->w || (s->rows && !s->x)) return bad("missing operand");
   if (s->rows > 1 && s->ldx < s->D) return bad("leading dimension below the width");
@@ -363,7 +363,7 @@ int fill(const fb_short_conv *s, ConvArgs &a, bool backward) {
   a.x = s->x, a.ldx = s->ldx, a.dy = s->dy, a.lddy = s->lddy, a.init = s->K > 1 ? s->init : nullptr;
   a.dfin = s->K > 1 ? s->dfinal : nullptr, a.fin = s->K > 1 ? s->final : nullptr, a.dinit = s->K > 1 ? s->dinit : nullptr;
   a.y = s->y, a.ldy = s->ldy, a.dx = s->dx, a.lddx = s->lddx, a.w = s->w, a.bias = s->bias, a.dw = s->dw, a.dbias = s->dbias;
-  a.st = Starts{s->starts, s->starts_type == FB_I64, s->seqs, s->rows};
+  a.st = Starts{s->starts, s->starts_type == FB_I64, (int)s->seqs, s->rows};
   return FB_OK;
 }
 
@@ -418,7 +418,7 @@ template <typename T, bool BWD> int launch_v(const ConvArgs &a, int V, cudaStrea
 unsigned some_blocks(int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, kSms * 8); }
 
 template <typename T> int run_conv(const fb_short_conv *s, ConvArgs &a, bool backward, void *ws, size_t ws_bytes, cudaStream_t st) {
-  const int64_t state = a.st.seqs * (a.K - 1) * (int64_t)a.D;
+  const int64_t state = (int64_t)a.st.seqs * (a.K - 1) * a.D;
   if (s->rows) {
     const int V = vector_of(s, backward);
     if (!V) return fb::set_error(FB_ERR_ARG, "short_conv: rows that are not aligned to their elements");
