@@ -6,22 +6,28 @@
 //   dw[k] = sum_t dp[t] x[t - K + 1 + k],  dbias = sum_t dp[t]
 //
 // Bound by memory: x read and y written, dy and x read and dx written.  A thread
-// owns V columns and walks down a run of rows, 8 at a time, with the last K - 1
-// inputs (and, backward, the last K - 1 dp) in registers, so every row is loaded
-// once but for the K - 1 at a run's ends; the 8 loads of a step are in flight
-// together.  Where sequences begin comes as one bit a row, which a CTA works out
-// for its rows before it starts; a beginning replaces the window by assignment.
+// owns up to 4 columns and walks down a run of rows with the last K - 1 inputs
+// (and, backward, the last K - 1 dp) in registers, so every row is loaded once
+// but for the K - 1 at a run's ends.  Loads are asynchronous copies into places
+// of the thread's own, two batches of four rows ahead: held in registers instead
+// they cost the warps that hide the latency (32,768 x 2,048 bf16 forward and
+// backward: loads where they are used 646 + 118 us, two batches of registers
+// 208 + 88, copies 117 + 63; the bytes take 61 + 41).  The arithmetic runs on
+// pairs of columns.  Where sequences begin comes as one bit a row, which a CTA
+// gathers for its rows before it starts; batches inside one sequence run without
+// a branch, others replace the window by assignment where a sequence begins.
 // p is computed again in the backward from x, which is there anyway.  dw and
 // dbias are summed over a thread's run in registers, over a CTA in shared
 // memory, and over the CTAs by a second launch in a fixed order.
 #include <algorithm>
+#include <type_traits>
 #include "head.cuh"
 #include "history.cuh"
 
 namespace {
 using namespace fbq;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxTaps = 8;
 constexpr int64_t kSms = 148;
 
@@ -29,253 +35,325 @@ struct ConvArgs {
   int D, K, silu;
   const void *x, *dy, *init, *dfin;
   void *y, *dx, *fin, *dinit;
-  int64_t ldx, ldy, lddy, lddx;
+  int ldx, ldy, lddy, lddx;
   const float *w, *bias;
   float *part, *dw, *dbias;                // part [blocks, K + 1, D]
   Starts st;
   int cx, ry;                              // threads of a CTA along the columns, runs of rows
   int run;                                 // rows of a run, a multiple of 8
   int64_t blocks;                          // CTAs along the rows
+  int ring;                                // where the rows on their way begin in shared memory
 };
 
-// Sequence of a row, for one thread (few threads ask).
+// Sequence of a row, -1: none, for one thread (few threads ask).
 __device__ __forceinline__ int owner1(const Starts &st, int64_t row) {
-  if (!st.p) return row < 0 ? -1 : (row < st.rows ? 0 : 1);
+  if (!st.p) return row >= 0 && row < st.rows ? 0 : -1;
   int lo = 0, hi = st.seqs + 1;
   while (lo < hi) {
     const int m = lo + ((hi - lo) >> 1);
     if (st[m] <= row) lo = m + 1;
     else hi = m;
   }
-  return lo - 1;
+  return lo - 1 < st.seqs ? lo - 1 : -1;
 }
 
-template <typename T, int V> __device__ __forceinline__ void load(const void *p, int64_t at, float (&v)[V]) {
-  const Vec<T, V> e = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(p) + at);
+// V elements as pairs (one element: with a zero).
+template <typename T, int V> struct Pairs {
+  static constexpr int P = (V + 1) / 2;
+  static __device__ __forceinline__ void widen(const Vec<T, V> &e, F2 (&v)[P]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = to_f(e.e[i]);
-}
-template <typename T, int V> __device__ __forceinline__ void store(void *p, int64_t at, const float (&v)[V]) {
-  Vec<T, V> e;
-#pragma unroll
-  for (int i = 0; i < V; ++i) e.e[i] = from_f<T>(v[i]);
-  *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(p) + at) = e;
-}
-
-// The beginnings of the rows from `from` (a multiple of 8) on, 8 to a byte.
-__device__ __forceinline__ void fill_begins(const Starts &st, int64_t from, int tiles, uint8_t *bits) {
-  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int each = (tiles + warps - 1) / warps;
-  Walk walk;
-  const int a = warp * each, b = min(a + each, tiles);
-  if (a >= b) return;
-  walk.begin(st, from + 8 * (int64_t)a);
-  for (int i = a; i < b; ++i) {
-    const int64_t r0 = from + 8 * (int64_t)i;
-    const unsigned m = r0 < 0 ? 0u : walk.tile(st, r0);
-    if ((threadIdx.x & 31) == 0) bits[i] = (uint8_t)m;
+    for (int i = 0; i < P; ++i) v[i] = pack(to_f(e.e[2 * i]), 2 * i + 1 < V ? to_f(e.e[2 * i + 1 < V ? 2 * i + 1 : 0]) : 0.f);
   }
-}
-
-// What a thread works on.  KT: taps the registers hold; the first `skip` of them
-// do not exist (they are left out, not multiplied by zero).
-template <typename T, int V, int KT> struct Window {
-  float x[KT - 1 + 8][V];                  // the last KT - 1 inputs, then 8 new ones
-  // Inputs in front of the first row of sequence s, newest last.
-  __device__ __forceinline__ void begin(const ConvArgs &a, int at, int64_t row, int64_t col, int skip) {
-    int64_t s = -1;
-    if (a.init) {
-      s = owner1(a.st, row);
-      if (s >= a.st.seqs) s = -1;
+  static __device__ __forceinline__ Vec<T, V> narrow(const F2 (&v)[P]) {
+    Vec<T, V> e;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 f = unpack(v[i]);
+      e.e[2 * i] = from_f<T>(f.x);
+      if (2 * i + 1 < V) e.e[2 * i + 1 < V ? 2 * i + 1 : 0] = from_f<T>(f.y);
     }
-#pragma unroll
-    for (int m = 0; m < KT - 1; ++m)
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        x[at + m][i] = s >= 0 && m >= skip
-                           ? to_f(static_cast<const T *>(a.init)[(s * (a.K - 1) + m - skip) * (int64_t)a.D + col + i]) : 0.f;
+    return e;
   }
 };
 
-template <typename T, int V, int KT, bool BWD> __global__ void __launch_bounds__(kThreads) k_conv(ConvArgs a) {
+// The beginnings of the rows from `from` on, a bit each, 32 * words of them.
+__device__ __forceinline__ void fill_begins(const Starts &st, int64_t from, int words, uint32_t *bits) {
+  for (int i = threadIdx.x; i < words; i += blockDim.x) bits[i] = 0;
+  __syncthreads();
+  const auto mark = [&](int64_t b) {
+    if (b >= from && b < from + 32 * words) atomicOr(&bits[(b - from) >> 5], 1u << ((b - from) & 31));
+  };
+  if (!st.p) {
+    if (threadIdx.x == 0) mark(0), mark(st.rows);
+    __syncthreads();
+    return;
+  }
+  for (int i = owner(st, from - 1) + 1 + threadIdx.x;; i += blockDim.x) {
+    const int64_t b = i <= st.seqs ? st[i] : INT64_MAX;
+    if (b < INT64_MAX) mark(b);
+    if (!__syncthreads_and(b < from + 32 * words)) break;
+  }
+}
+
+template <typename E> __device__ __forceinline__ void copy_async(E *to, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(sizeof(E))
+               : "memory");
+}
+
+// Rows of a batch: 8 single bf16 elements, which no asynchronous copy moves and
+// only their number keeps memory busy with; else 4.
+template <typename T, int V> constexpr int kRows = sizeof(T) * V < 4 ? 8 : 4;
+
+// KT taps in registers; KT 2, 3, 4: exactly K, KT 8: the first 8 - K of them do
+// not exist and are left out, not multiplied by zero.
+template <typename T, int V, int KT, bool BWD> __global__ void __launch_bounds__(kThreads, BWD ? 4 : 6) k_conv(ConvArgs a) {
+  using PV = Pairs<T, V>;
+  using E = Vec<T, V>;
+  constexpr int P = PV::P, H = KT - 1;                                     // pairs of columns; rows of history
+  constexpr bool ASYNC = sizeof(E) >= 4;                                   // what an asynchronous copy moves
+  constexpr int R = kRows<T, V>;                                           // rows at a time
   fb::pdl_enter();
   extern __shared__ __align__(16) unsigned char dyn[];
   const int64_t rows = a.st.rows;
-  const int64_t block0 = (int64_t)blockIdx.y * a.ry * a.run;              // the CTA's first row
-  uint8_t *const bits = dyn;                                              // rows block0 - 8 .. block0 + ry run + 15
-  fill_begins(a.st, block0 - 8, a.ry * a.run / 8 + 3, bits);
-  float *const sums = reinterpret_cast<float *>(dyn + (a.ry * a.run / 8 + 3 + 15) / 16 * 16);
-  __syncthreads();
+  const int64_t block0 = (int64_t)blockIdx.y * a.ry * a.run;               // the CTA's first row
+  const int words = (a.ry * a.run + 24 + 31) / 32;
+  uint32_t *const bits = reinterpret_cast<uint32_t *>(dyn);                // rows from block0 - 8 on
+  float *const sums = reinterpret_cast<float *>(dyn + (words * 4 + 15) / 16 * 16);
+  fill_begins(a.st, block0 - 8, words, bits);
 
   const int c = threadIdx.x % a.cx, q = threadIdx.x / a.cx;
-  const int64_t col = ((int64_t)blockIdx.x * a.cx + c) * V;
-  const int64_t q0 = block0 + (int64_t)q * a.run, q1 = min(q0 + a.run, rows);
-  const bool active = q < a.ry && col < a.D && q0 < q1;
-  const int skip = KT - a.K;
-  float dw[KT][V] = {}, db[V] = {};
+  const int col = (blockIdx.x * a.cx + c) * V;
+  const int K = KT == 8 ? a.K : KT, skip = KT - K;
+  const int64_t q0 = block0 + (int64_t)q * a.run;
+  const int len = (int)max((int64_t)0, min((int64_t)a.run, rows - q0));    // rows of the run
+  const bool active = q < a.ry && col < a.D && len > 0;
+  F2 dw[BWD ? KT : 1][P], db[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    db[p] = both(0.f);
+    if constexpr (BWD)
+#pragma unroll
+      for (int k = 0; k < KT; ++k) dw[k][p] = both(0.f);
+  }
   if (active) {
-    const int64_t first = a.st[0], last = a.st[a.st.seqs];
-    float w[KT][V], bias[V];
+    // rows counted from q0: those of sequences, and those of the tensor
+    const int first = (int)max((int64_t)-64, min(a.st[0] - q0, (int64_t)a.run + 64));
+    const int last = (int)max((int64_t)-64, min(a.st[a.st.seqs] - q0, (int64_t)a.run + 64));
+    const int all = (int)min(rows - q0, (int64_t)a.run + 64);
+    F2 w[KT][P], bias[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      bias[i] = a.bias ? a.bias[col + i] : 0.f;
+    for (int p = 0; p < P; ++p) {
+      const int c0 = col + 2 * p, c1 = 2 * p + 1 < V ? c0 + 1 : c0;
+      bias[p] = a.bias ? pack(a.bias[c0], a.bias[c1]) : both(0.f);
 #pragma unroll
-      for (int k = 0; k < KT; ++k) w[k][i] = k >= skip ? a.w[(col + i) * a.K + k - skip] : 0.f;
+      for (int k = 0; k < KT; ++k)
+        w[k][p] = k >= skip ? pack(a.w[(int64_t)c0 * K + k - skip], a.w[(int64_t)c1 * K + k - skip]) : both(0.f);
     }
-    const auto begins = [&](int64_t row) { return (bits[(row - block0 + 8) >> 3] >> (row & 7)) & 1u; };
+    const T *const px = static_cast<const T *>(a.x) + q0 * a.ldx + col;
+    const T *const pdy = BWD ? static_cast<const T *>(a.dy) + q0 * a.lddy + col : nullptr;
+    T *const py = static_cast<T *>(BWD ? a.dx : a.y) + q0 * (BWD ? a.lddx : a.ldy) + col;
+    const int ldo = BWD ? a.lddx : a.ldy;
+    // 16 beginnings, of the rows t - 8 .. t + 7
+    const auto around = [&](int t) {
+      const int o = q * a.run + t;                                         // bit of row t - 8
+      return (bits[o >> 5] >> (o & 31) | ((o & 31) > 16 ? bits[(o >> 5) + 1] << (32 - (o & 31)) : 0u)) & 0xffffu;
+    };
+    // The m-th oldest of the K - 1 inputs in front of sequence s.
+    const auto older = [&](int s, int m, F2 (&v)[P]) {
+      E e;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        e.e[i] = s >= 0 && m >= 0 ? static_cast<const T *>(a.init)[((int64_t)s * (K - 1) + m) * a.D + col + i] : from_f<T>(0.f);
+      PV::widen(e, v);
+    };
 
-    Window<T, V, KT> win;
+    F2 win[H + R][P];                                                      // the last H inputs, then R new ones
     {
-      // the inputs in front of the run: its own sequence's, as far as they go, older ones from init
-      int64_t b = q0 - (KT - 1);                                           // first row of the sequence, if it is that near
+      // in front of the run: its own sequence's inputs as far as they go, then those of init
+      const unsigned m = around(0);
+      int b = -H;
       bool cut = false;
 #pragma unroll
-      for (int j = KT - 2; j >= 1; --j)
-        if (q0 - j >= 0 && begins(q0 - j)) b = q0 - j, cut = true;
-      if (q0 - (KT - 1) < 0 && !cut) b = 0, cut = true;
-      int64_t s = -1;
-      if (cut && a.init) {
-        s = owner1(a.st, b);
-        if (s >= a.st.seqs) s = -1;
-      }
+      for (int j = H; j >= 1; --j)
+        if (m >> (8 - j) & 1u) b = -j, cut = true;
+      if (!cut && q0 < H) b = (int)-q0, cut = true;
+      const int s = cut && a.init ? owner1(a.st, q0 + b) : -1;
 #pragma unroll
-      for (int m = 0; m < KT - 1; ++m) {
-        const int64_t r = q0 - (KT - 1) + m;
-        const int64_t at = a.K - 1 + (r - b);                              // place in init, where r < b
-        if (r >= b && r >= 0) load<T, V>(a.x, r * a.ldx + col, win.x[m]);
-        else
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            win.x[m][i] = s >= 0 && at >= 0 ? to_f(static_cast<const T *>(a.init)[(s * (a.K - 1) + at) * (int64_t)a.D + col + i]) : 0.f;
+      for (int i = 0; i < H; ++i) {
+        const int t = i - H;
+        if (t >= b) {
+          E e = *reinterpret_cast<const E *>(px + (int64_t)t * a.ldx);
+          PV::widen(e, win[i]);
+        } else {
+          older(s, K - 1 + t - b, win[i]);
+        }
       }
     }
-    float dp[BWD ? KT - 1 + 8 : 1][V];
+    F2 dp[BWD ? H + R : 1][P];
     if constexpr (BWD) {
 #pragma unroll
-      for (int m = 0; m < KT - 1; ++m)
+      for (int i = 0; i < H; ++i)
 #pragma unroll
-        for (int i = 0; i < V; ++i) dp[m][i] = 0.f;
+        for (int p = 0; p < P; ++p) dp[i][p] = both(0.f);
     }
     // Backward, a dx row is complete K - 1 rows later: the walk goes on behind the run.
-    const int64_t end = BWD ? q1 + KT - 1 : q1;
-    for (int64_t t0 = q0; t0 < end; t0 += 8) {
-      float dy[BWD ? 8 : 1][V];
+    const int end = BWD ? len + H : len, have = min(end, all);
+    // Two batches of R rows are on their way while one is in work, each thread's into places of its own.
+    E *const ring = reinterpret_cast<E *>(dyn + a.ring) + threadIdx.x;     // [3 batches, R rows, x and dy][thread]
+    const auto fetch = [&](int t0, int b) {
+      if constexpr (ASYNC) {
+        const T *x = px + (int64_t)t0 * a.ldx, *y = BWD ? pdy + (int64_t)t0 * a.lddy : nullptr;
+        E *to = ring + b * (R * (BWD ? 2 : 1) * kThreads);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = t0 + i < rows && t0 + i < end;
-        if (in) load<T, V>(a.x, (t0 + i) * a.ldx + col, win.x[KT - 1 + i]);
-        else
-#pragma unroll
-          for (int v = 0; v < V; ++v) win.x[KT - 1 + i][v] = 0.f;
-        if constexpr (BWD) {
-          if (in) load<T, V>(a.dy, (t0 + i) * a.lddy + col, dy[i]);
-        }
+        for (int i = 0; i < R; ++i)
+          if (t0 + i < have) {
+            copy_async(to + i * kThreads, x + (int64_t)i * a.ldx);
+            if constexpr (BWD) copy_async(to + (R + i) * kThreads, y + (int64_t)i * a.lddy);
+          }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       }
-      const unsigned now = bits[(t0 - block0 + 8) >> 3];
+    };
+    fetch(0, 0);
+    fetch(R, 1);
+    int batch = 0;
+    for (int t0 = 0; t0 < end; t0 += R) {
+      const unsigned m = around(t0);
+      unsigned live = (1u << R) - 1u;
+      if (t0 < first || t0 + R > last || t0 + R > have) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t t = t0 + i;
-        if (now >> i & 1u) win.begin(a, i, t, col, skip);
-        const bool live = t >= first && t < last && t < end;
-        float p[V];
+        for (int i = 0; i < R; ++i)
+          if (t0 + i < first || t0 + i >= last || t0 + i >= have) live &= ~(1u << i);
+      }
+      fetch(t0 + 2 * R, batch == 0 ? 2 : batch - 1);
+      if constexpr (ASYNC) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      const E *const here = ring + batch * (R * (BWD ? 2 : 1) * kThreads);
+      batch = batch == 2 ? 0 : batch + 1;
+      E rx[ASYNC ? 1 : R], ry[BWD && !ASYNC ? R : 1];
+      if constexpr (!ASYNC) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) p[v] = bias[v];
+        for (int i = 0; i < R; ++i)
+          if (t0 + i < have) {
+            rx[i] = *reinterpret_cast<const E *>(px + (int64_t)(t0 + i) * a.ldx);
+            if constexpr (BWD) ry[i] = *reinterpret_cast<const E *>(pdy + (int64_t)(t0 + i) * a.lddy);
+          }
+      }
+      // PLAIN: rows of one sequence, inside the run
+      const auto work = [&](auto plain) {
+        constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
-          if (KT == 4 ? (k > 2 || k >= skip) : k >= skip)
+      for (int i = 0; i < R; ++i) {
+        const int t = t0 + i;
+        PV::widen(ASYNC ? here[i * kThreads] : rx[ASYNC ? 0 : i], win[H + i]);
+        F2 g[P];
+        if constexpr (BWD) PV::widen(ASYNC ? here[(R + i) * kThreads] : ry[ASYNC ? 0 : i], g);
+        if (!PLAIN && (m >> (8 + i) & 1u)) {                                          // a sequence begins: what was before it
+          const int s = a.init ? owner1(a.st, q0 + t) : -1;
 #pragma unroll
-            for (int v = 0; v < V; ++v) p[v] = fmaf(w[k][v], win.x[i + k][v], p[v]);
+          for (int k = 0; k < H; ++k) older(s, k - skip, win[i + k]);
+        }
+        F2 z[P], sg[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          z[p] = bias[p];
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+            if (k >= skip) z[p] = fma2(w[k][p], win[i + k][p], z[p]);
+          if (a.silu) sg[p] = sigmoid2(z[p]);
+        }
         if constexpr (!BWD) {
-          if (t < q1) {
-            float y[V];
+          if (PLAIN || t < len) {
+            if (a.silu)
 #pragma unroll
-            for (int v = 0; v < V; ++v) y[v] = live ? (a.silu ? p[v] * sigmoid(p[v]) : p[v]) : 0.f;
-            store<T, V>(a.y, t * a.ldy + col, y);
+              for (int p = 0; p < P; ++p) z[p] = mul2(z[p], sg[p]);
+            if (!PLAIN && !(live >> i & 1u))
+#pragma unroll
+              for (int p = 0; p < P; ++p) z[p] = both(0.f);
+            *reinterpret_cast<E *>(py + (int64_t)t * ldo) = PV::narrow(z);
           }
         } else {
-          float(&d)[V] = dp[KT - 1 + i];
+          if (PLAIN || (live >> i & 1u)) {
+            if (a.silu)
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            d[v] = live ? dy[i][v] : 0.f;
-            if (a.silu && live) {
-              const float sg = sigmoid(p[v]);
-              d[v] *= sg * fmaf(p[v], 1.f - sg, 1.f);
+              for (int p = 0; p < P; ++p) {
+                const F2 zs = mul2(z[p], sg[p]);
+                g[p] = mul2(g[p], fma2(mul2(zs, sg[p]), both(-1.f), add2(sg[p], zs)));
+              }
+            if (PLAIN || t < len)
+#pragma unroll
+              for (int p = 0; p < P; ++p) {
+                db[p] = add2(db[p], g[p]);
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+                  if (k >= skip) dw[k][p] = fma2(g[p], win[i + k][p], dw[k][p]);
+              }
+          } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p) g[p] = both(0.f);
+          }
+#pragma unroll
+          for (int p = 0; p < P; ++p) dp[H + i][p] = g[p];
+          // the row whose last dp this was
+          const int r = t - H;
+          if (PLAIN || (r >= 0 && r < len)) {
+            const unsigned ends = PLAIN ? 0u : m >> (8 + i - H + 1);       // bit j - 1: row r + j begins another sequence
+            F2 o[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) o[p] = mul2(w[KT - 1][p], dp[i][p]);
+#pragma unroll
+            for (int j = 1; j < KT; ++j)
+              if (KT - 1 - j >= skip && (PLAIN || !(ends & ((1u << j) - 1u))))
+#pragma unroll
+                for (int p = 0; p < P; ++p) o[p] = fma2(w[KT - 1 - j][p], dp[i + j][p], o[p]);
+            if (!PLAIN && a.dfin && (ends & ((1u << (K - 1)) - 1u))) {               // one of the last K - 1 inputs
+              const int s = owner1(a.st, q0 + r), gap = __ffs(ends);
+              if (s >= 0) {
+                E e;
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                  e.e[v] = static_cast<const T *>(a.dfin)[((int64_t)s * (K - 1) + K - 1 - gap) * a.D + col + v];
+                F2 f[P];
+                PV::widen(e, f);
+#pragma unroll
+                for (int p = 0; p < P; ++p) o[p] = add2(o[p], f[p]);
+              }
             }
-          }
-          if (live && t < q1) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) db[v] += d[v];
-#pragma unroll
-            for (int k = 0; k < KT; ++k)
-              if (k >= skip)
-#pragma unroll
-                for (int v = 0; v < V; ++v) dw[k][v] = fmaf(d[v], win.x[i + k][v], dw[k][v]);
+            *reinterpret_cast<E *>(py + (int64_t)r * ldo) = PV::narrow(o);
           }
         }
       }
-      if constexpr (BWD) {
-        // dx of the rows whose last dp has come
+      };
+      if (live == (1u << R) - 1u && !(m >> (8 - H + 1) & ((1u << (R + H - 1)) - 1u)) && t0 >= (BWD ? H : 0) && t0 + R <= len) work(std::true_type{});
+      else work(std::false_type{});
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int64_t r = t0 + i - (KT - 1);
-          if (r < q0 || r >= q1) continue;
-          float g[V];
+      for (int i = 0; i < H; ++i)
 #pragma unroll
-          for (int v = 0; v < V; ++v) g[v] = w[KT - 1][v] * dp[i][v];
-          bool same = true;
-          int gap = KT;                                                    // rows to the sequence's end
-#pragma unroll
-          for (int j = 1; j < KT; ++j) {
-            if (same && begins(r + j)) same = false, gap = j;
-            if (same && KT - 1 - j >= skip)
-#pragma unroll
-              for (int v = 0; v < V; ++v) g[v] = fmaf(w[KT - 1 - j][v], dp[i + j][v], g[v]);
-          }
-          const bool live = r >= first && r < last;
-          if (a.dfin && live && gap < a.K) {
-            const int64_t s = owner1(a.st, r);
-            if (s >= 0 && s < a.st.seqs)
-#pragma unroll
-              for (int v = 0; v < V; ++v)
-                g[v] += to_f(static_cast<const T *>(a.dfin)[(s * (a.K - 1) + a.K - 1 - gap) * (int64_t)a.D + col + v]);
-          }
-          if (!live)
-#pragma unroll
-            for (int v = 0; v < V; ++v) g[v] = 0.f;
-          store<T, V>(a.dx, r * a.lddx + col, g);
+        for (int p = 0; p < P; ++p) {
+          win[i][p] = win[i + R][p];
+          if constexpr (BWD) dp[i][p] = dp[i + R][p];
         }
-#pragma unroll
-        for (int m = 0; m < KT - 1; ++m)
-#pragma unroll
-          for (int v = 0; v < V; ++v) dp[m][v] = dp[m + 8][v];
-      }
-#pragma unroll
-      for (int m = 0; m < KT - 1; ++m)
-#pragma unroll
-        for (int v = 0; v < V; ++v) win.x[m][v] = win.x[m + 8][v];
     }
   }
   if constexpr (BWD) {
     // the CTA's sums: the runs add up in order
     const int width = a.cx * V;
-    for (int k = 0; k <= a.K; ++k) {
+#pragma unroll
+    for (int k = 0; k <= KT; ++k) {
+      if (k < skip) continue;
       if (q < a.ry && col < a.D)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float x = db[v];
-#pragma unroll
-          for (int m = 0; m < KT; ++m)
-            if (m == k + skip) x = dw[m][v];
-          sums[q * width + c * V + v] = k < a.K ? x : db[v];
+        for (int p = 0; p < P; ++p) {
+          const float2 f = unpack(k < KT ? dw[k < KT ? k : 0][p] : db[p]);
+          sums[q * width + c * V + 2 * p] = f.x;
+          if (2 * p + 1 < V) sums[q * width + c * V + 2 * p + 1] = f.y;
         }
       __syncthreads();
       for (int i = threadIdx.x; i < width; i += kThreads) {
-        const int64_t d = (int64_t)blockIdx.x * width + i;
+        const int d = blockIdx.x * width + i;
         if (d < a.D) {
           float x = 0.f;
           for (int j = 0; j < a.ry; ++j) x += sums[j * width + i];
-          if (a.blocks > 1) a.part[((int64_t)blockIdx.y * (a.K + 1) + k) * a.D + d] = x;
-          else if (k < a.K) a.dw[d * a.K + k] = x;
+          if (a.blocks > 1) a.part[((int64_t)blockIdx.y * (K + 1) + k - skip) * a.D + d] = x;
+          else if (k < KT) a.dw[(int64_t)d * K + k - skip] = x;
           else a.dbias[d] = x;
         }
       }
@@ -284,13 +362,24 @@ template <typename T, int V, int KT, bool BWD> __global__ void __launch_bounds__
   }
 }
 
+// Adds the CTAs' sums in a fixed order: 8 columns a CTA, 32 threads a column.
 __global__ void __launch_bounds__(256) k_conv_sums(ConvArgs a) {
   fb::pdl_enter();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)(a.K + 1) * a.D;
-  if (i >= n) return;
+  __shared__ float part[8][8];
+  const int64_t n = (int64_t)(a.K + 1) * a.D, i = (int64_t)blockIdx.x * 8 + threadIdx.x % 8;
   float v = 0.f;
+  if (i < n) {
 #pragma unroll 8
-  for (int64_t b = 0; b < a.blocks; ++b) v += a.part[b * n + i];
+    for (int64_t b = threadIdx.x / 8; b < a.blocks; b += 32) v += a.part[b * n + i];
+  }
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  v += __shfl_xor_sync(0xffffffffu, v, 16);
+  if (threadIdx.x % 32 < 8) part[threadIdx.x / 32][threadIdx.x % 8] = v;
+  __syncthreads();
+  if (threadIdx.x >= 8 || i >= n) return;
+  v = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v += part[j][threadIdx.x];
   const int k = (int)(i / a.D);
   const int64_t d = i % a.D;
   if (k < a.K) a.dw[d * a.K + k] = v;
@@ -305,7 +394,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_conv_final(ConvAr
     const int64_t d = i % a.D, m = i / a.D % (a.K - 1), s = i / a.D / (a.K - 1);
     const int64_t b = a.st[(int)s], e = max(a.st[(int)s + 1], b), p = e - b - (a.K - 1) + m;
     T v = from_f<T>(0.f);
-    if (p >= 0) v = static_cast<const T *>(a.x)[(b + p) * a.ldx + d];
+    if (p >= 0) v = static_cast<const T *>(a.x)[(b + p) * (int64_t)a.ldx + d];
     else if (a.init) v = static_cast<const T *>(a.init)[(s * (a.K - 1) + a.K - 1 + p) * a.D + d];
     static_cast<T *>(a.fin)[i] = v;
   }
@@ -326,8 +415,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_conv_dinit(ConvAr
       g[m] = m < K - 1 && a.dfin && m >= len ? to_f(static_cast<const T *>(a.dfin)[(s * (K - 1) + m - len) * a.D + d]) : 0.f;
     }
     for (int i = 0; i < K - 1 && i < len; ++i) {
-      x[K - 1 + i] = to_f(static_cast<const T *>(a.x)[(b + i) * a.ldx + d]);
-      float p = a.bias ? a.bias[d] : 0.f, dp = to_f(static_cast<const T *>(a.dy)[(b + i) * a.lddy + d]);
+      x[K - 1 + i] = to_f(static_cast<const T *>(a.x)[(b + i) * (int64_t)a.ldx + d]);
+      float p = a.bias ? a.bias[d] : 0.f, dp = to_f(static_cast<const T *>(a.dy)[(b + i) * (int64_t)a.lddy + d]);
       for (int k = 0; k < K; ++k) p = fmaf(w[k], x[i + k], p);
       if (a.silu) {
         const float sg = sigmoid(p);
@@ -351,6 +440,8 @@ int fill(const fb_short_conv *s, ConvArgs &a, bool backward) {
   if (s->K > kMaxTaps) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv: at most 8 taps");
   if (s->D > (1 << 20) || s->rows > (int64_t)1 << 40 || s->seqs > (1 << 30))
     return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv: sizes beyond what the kernels index");
+  if (std::max(std::max(s->ldx, s->ldy), std::max(s->lddy, s->lddx)) > (1 << 28))
+    return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv: leading dimension beyond what the kernels index");
   if (!s->w || (s->rows && !s->x)) return bad("missing operand");
   if (s->rows > 1 && s->ldx < s->D) return bad("leading dimension below the width");
   if (!backward && s->rows && (!s->y || (s->rows > 1 && s->ldy < s->D))) return bad("missing or overlapping output");
@@ -360,14 +451,19 @@ int fill(const fb_short_conv *s, ConvArgs &a, bool backward) {
   if (backward && s->dinit && !s->init) return bad("dinit without init");
   a = ConvArgs{};
   a.D = s->D, a.K = s->K, a.silu = s->act == FB_ACT_SILU;
-  a.x = s->x, a.ldx = s->ldx, a.dy = s->dy, a.lddy = s->lddy, a.init = s->K > 1 ? s->init : nullptr;
+  a.x = s->x, a.ldx = (int)s->ldx, a.dy = s->dy, a.lddy = (int)s->lddy, a.init = s->K > 1 ? s->init : nullptr;
   a.dfin = s->K > 1 ? s->dfinal : nullptr, a.fin = s->K > 1 ? s->final : nullptr, a.dinit = s->K > 1 ? s->dinit : nullptr;
-  a.y = s->y, a.ldy = s->ldy, a.dx = s->dx, a.lddx = s->lddx, a.w = s->w, a.bias = s->bias, a.dw = s->dw, a.dbias = s->dbias;
+  a.y = s->y, a.ldy = (int)s->ldy, a.dx = s->dx, a.lddx = (int)s->lddx, a.w = s->w, a.bias = s->bias, a.dw = s->dw, a.dbias = s->dbias;
   a.st = Starts{s->starts, s->starts_type == FB_I64, (int)s->seqs, s->rows};
   return FB_OK;
 }
 
-// Columns a thread moves at once: as many (up to 4) as bases, pitches and the width allow.
+// Columns a thread moves at once: as many as bases, pitches and the width allow,
+// up to 4 where that leaves 8 warps an SM (runs of 32 rows), else 2: a lone warp
+// issues an instruction every four cycles (12,000 x 200 fp32, both passes: 2
+// columns 35 us, 4 columns 43, one 40).  8 columns of bf16 take more registers
+// than the wider accesses give back (forward of 32,768 x 2,048: 75 us, with 4
+// columns 63).
 int vector_of(const fb_short_conv *s, bool backward) {
   const int es = s->type == FB_F32 ? 4 : 2;
   const void *p[2] = {backward ? s->dy : s->y, backward ? s->dx : nullptr};
@@ -381,19 +477,20 @@ int vector_of(const fb_short_conv *s, bool backward) {
       bits |= (uint64_t)(uintptr_t)p[i] / es;
       if (s->rows > 1) bits |= (uint64_t)ld[i];
     }
-  return bits % 4 == 0 ? 4 : (bits % 2 == 0 ? 2 : 1);
+  const bool many = s->rows / 32 * (s->D / 128) >= kSms * 8;
+  return bits % 4 == 0 && many ? 4 : (bits % 2 == 0 ? 2 : 1);
 }
 
 // Columns of a CTA, runs side by side, rows of a run: long runs load few rows
-// twice, but the SMs want two CTAs and more each.
+// twice, but the SMs want their CTAs each.
 void plan(ConvArgs &a, int V, bool backward) {
   const int groups = (a.D + V - 1) / V;
   a.cx = std::min(groups, kThreads);
   a.ry = kThreads / a.cx;
   const int64_t across = (groups + a.cx - 1) / a.cx;
-  const int64_t want = std::max<int64_t>(1, kSms * (backward ? 4 : 8) / across);
+  const int64_t want = std::max<int64_t>(1, kSms * (backward ? 4 : 6) / across);
   int64_t run = (a.st.rows + want * a.ry - 1) / (want * a.ry);
-  run = std::min<int64_t>(std::max<int64_t>((run + 7) / 8 * 8, backward ? 32 : 16), 256);
+  run = std::min<int64_t>(std::max<int64_t>((run + 7) / 8 * 8, 16), 256);
   while (run * a.ry > 8192 && run > 8) run -= 8;
   a.run = (int)run;
   a.blocks = (a.st.rows + a.run * (int64_t)a.ry - 1) / (a.run * (int64_t)a.ry);
@@ -401,18 +498,30 @@ void plan(ConvArgs &a, int V, bool backward) {
   while (a.blocks > 65535) a.run *= 2, a.blocks = (a.st.rows + a.run * (int64_t)a.ry - 1) / (a.run * (int64_t)a.ry);
 }
 
-template <typename T, int V, int KT, bool BWD> int launch_main(const ConvArgs &a, cudaStream_t st) {
+template <typename T, int V, int KT, bool BWD> int launch_main(ConvArgs &a, cudaStream_t st) {
   const int width = a.cx * V;
-  const size_t smem = (size_t)(a.ry * a.run / 8 + 3 + 15) / 16 * 16 + (BWD ? (size_t)a.ry * width * 4 : 0);
-  if (smem > 48 * 1024) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv: too many rows");
+  a.ring = ((a.ry * a.run + 24 + 31) / 32 * 4 + 15) / 16 * 16 + (BWD ? (a.ry * width * 4 + 15) / 16 * 16 : 0);
+  const size_t ring = sizeof(T) * V < 4 ? 0 : (size_t)3 * kRows<T, V> * (BWD ? 2 : 1) * kThreads * V * sizeof(T);
+  const size_t smem = a.ring + ring;
+  if (smem > 96 * 1024) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv: too many rows");
+  if (smem > 48 * 1024)
+    FB_TRY_CUDA(cudaFuncSetAttribute(k_conv<T, V, KT, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const dim3 grid((unsigned)((a.D + width - 1) / width), (unsigned)a.blocks);
   FB_TRY_CUDA(fb::launch(k_conv<T, V, KT, BWD>, grid, kThreads, smem, st, a));
   return FB_OK;
 }
 
-template <typename T, bool BWD> int launch_v(const ConvArgs &a, int V, cudaStream_t st) {
-  if (a.K <= 4) return V == 4 ? launch_main<T, 4, 4, BWD>(a, st) : V == 2 ? launch_main<T, 2, 4, BWD>(a, st) : launch_main<T, 1, 4, BWD>(a, st);
-  return V == 4 ? launch_main<T, 4, 8, BWD>(a, st) : V == 2 ? launch_main<T, 2, 8, BWD>(a, st) : launch_main<T, 1, 8, BWD>(a, st);
+template <typename T, int V, bool BWD> int launch_k(ConvArgs &a, cudaStream_t st) {
+  switch (a.K) {
+    case 2: return launch_main<T, V, 2, BWD>(a, st);
+    case 3: return launch_main<T, V, 3, BWD>(a, st);
+    case 4: return launch_main<T, V, 4, BWD>(a, st);
+    default: return launch_main<T, V, 8, BWD>(a, st);
+  }
+}
+
+template <typename T, bool BWD> int launch_v(ConvArgs &a, int V, cudaStream_t st) {
+  return V == 4 ? launch_k<T, 4, BWD>(a, st) : V == 2 ? launch_k<T, 2, BWD>(a, st) : launch_k<T, 1, BWD>(a, st);
 }
 
 unsigned some_blocks(int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, kSms * 8); }
@@ -430,7 +539,7 @@ template <typename T> int run_conv(const fb_short_conv *s, ConvArgs &a, bool bac
       a.part = static_cast<float *>(ws);
     }
     FBH_TRY((backward ? launch_v<T, true>(a, V, st) : launch_v<T, false>(a, V, st)));
-    if (backward && a.blocks > 1) FB_TRY_CUDA(fb::launch(k_conv_sums, dim3((unsigned)(((a.K + 1) * (int64_t)a.D + 255) / 256)), 256, 0, st, a));
+    if (backward && a.blocks > 1) FB_TRY_CUDA(fb::launch(k_conv_sums, dim3((unsigned)(((a.K + 1) * (int64_t)a.D + 7) / 8)), 256, 0, st, a));
   } else if (backward) {
     FB_TRY_CUDA(cudaMemsetAsync(a.dw, 0, (size_t)a.D * a.K * sizeof(float), st));
     FB_TRY_CUDA(cudaMemsetAsync(a.dbias, 0, (size_t)a.D * sizeof(float), st));
