@@ -4,10 +4,14 @@
 //
 // decided on the word's upper 24 bits, as everywhere in the framework.  Nothing
 // is stored: the backward, keep dy / (1 - p), draws the same numbers again.
-// Bound by memory (x, res, y) and, in bf16, nearly as much by the generator's
-// ten rounds for four columns, which is why a thread holds several groups of
-// four at once and loads them before it draws.
+// Bound by memory (x, res, y) once the generator is lean: a thread keeps its
+// group of four columns and goes down the rows, so nothing is divided; the ten
+// rounds' keys come with the launch; the comparison is one of whole numbers
+// (16,384 x 4,096 bf16 with a residual: 107 us with an index divided for each
+// group and the words converted to fractions).  Two rows are loaded before the
+// first is drawn, and 40 warps an SM hide the rest.
 #include <algorithm>
+#include <cmath>
 #include "history.cuh"
 #include "runtime.cuh"
 
@@ -19,63 +23,93 @@ struct DropArgs {
   void *y;
   int64_t ldx, ldr, ldy, rows;
   int D, quads;                            // groups of four columns
-  float p, scale;
-  uint64_t seed, offset;
+  int cx, ry;                              // groups, rows side by side in a CTA
+  uint32_t from;                           // words from here on keep
+  float scale;
+  uint32_t key[10][2];                     // the rounds' keys
+  uint64_t offset;
   const int64_t *offset_dev;
 };
 
+// Philox4x32-10 (fb::philox4x32_10) with the keys of the rounds at hand.
+__device__ __forceinline__ fb::Philox4 draw(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, const uint32_t (&key)[10][2]) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ key[r][0];
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ key[r][1];
+    c1 = (uint32_t)p1, c3 = (uint32_t)p0;
+  }
+  return fb::Philox4{{c0, c1, c2, c3}};
+}
+
+constexpr int kThreads = 256, kAhead = 2;
+
 // VEC: whole groups are moved at once (D is a multiple of 4, rows aligned).
-template <typename T, bool VEC, bool RES> __global__ void __launch_bounds__(256) k_dropout(DropArgs a) {
+template <typename T, bool VEC, bool RES> __global__ void __launch_bounds__(kThreads, 5) k_dropout(const __grid_constant__ DropArgs a) {
   fb::pdl_enter();
+  using E = Vec<T, 4>;
   const uint64_t off = a.offset + (a.offset_dev ? (uint64_t)*a.offset_dev : 0);
-  const int64_t n = a.rows * a.quads, stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-    const int64_t r = i / a.quads;
-    const int q = (int)(i - r * a.quads), c = q * 4, left = VEC ? 4 : a.D - c;
-    Vec<T, 4> x, res;
-    const T *px = static_cast<const T *>(a.x) + r * a.ldx + c;
-    const T *pr = RES ? static_cast<const T *>(a.res) + r * a.ldr + c : nullptr;
+  const int tr = threadIdx.x / a.cx, q = blockIdx.x * a.cx + threadIdx.x % a.cx;
+  if (tr >= a.ry || q >= a.quads) return;
+  const int c = q * 4, left = VEC ? 4 : a.D - c;
+  const int64_t step = (int64_t)gridDim.y * a.ry;
+  const T *const px = static_cast<const T *>(a.x) + c, *const pr = RES ? static_cast<const T *>(a.res) + c : nullptr;
+  T *const py = static_cast<T *>(a.y) + c;
+  const auto load = [&](const T *p, E &e) {
     if (VEC) {
-      x = *reinterpret_cast<const Vec<T, 4> *>(px);
-      if (RES) res = *reinterpret_cast<const Vec<T, 4> *>(pr);
+      e = *reinterpret_cast<const E *>(p);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k < left) {
-          x.e[k] = px[k];
-          if (RES) res.e[k] = pr[k];
-        }
+        if (k < left) e.e[k] = p[k];
     }
-    const fb::Philox4 w = fb::philox4x32_10((uint32_t)q, (uint32_t)r, (uint32_t)off, (uint32_t)(off >> 32), (uint32_t)a.seed,
-                                            (uint32_t)(a.seed >> 32));
-    Vec<T, 4> y;
+  };
+  for (int64_t r0 = (int64_t)blockIdx.y * a.ry + tr; r0 < a.rows; r0 += step * kAhead) {
+    E x[kAhead], res[kAhead];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bool keep = (float)(w.v[k] >> 8) * (1.0f / 16777216.0f) >= a.p;
-      float v = keep ? to_f(x.e[k]) * a.scale : 0.f;
-      if (RES) v += to_f(res.e[k]);
-      y.e[k] = from_f<T>(v);
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t r = r0 + i * step;
+      if (r < a.rows) {
+        load(px + r * a.ldx, x[i]);
+        if (RES) load(pr + r * a.ldr, res[i]);
+      }
     }
-    T *py = static_cast<T *>(a.y) + r * a.ldy + c;
-    if (VEC) {
-      *reinterpret_cast<Vec<T, 4> *>(py) = y;
-    } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k < left) py[k] = y.e[k];
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t r = r0 + i * step;
+      if (r >= a.rows) break;
+      const fb::Philox4 w = draw((uint32_t)q, (uint32_t)r, (uint32_t)off, (uint32_t)(off >> 32), a.key);
+      E y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float v = RES ? to_f(res[i].e[k]) : 0.f;
+        if (w.v[k] >= a.from) v = RES ? fmaf(to_f(x[i].e[k]), a.scale, v) : to_f(x[i].e[k]) * a.scale;
+        y.e[k] = from_f<T>(v);
+      }
+      if (VEC) {
+        *reinterpret_cast<E *>(py + r * a.ldy) = y;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < left) py[r * a.ldy + k] = y.e[k];
+      }
     }
   }
 }
 
-template <typename T> int run(const DropArgs &a, bool vec, cudaStream_t st) {
-  const int64_t n = a.rows * a.quads;
-  const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 148 * 32));
+template <typename T> int run(DropArgs &a, bool vec, cudaStream_t st) {
+  a.cx = std::min(a.quads, kThreads);
+  a.ry = kThreads / a.cx;
+  const int64_t across = (a.quads + a.cx - 1) / a.cx, down = (a.rows + a.ry - 1) / a.ry;
+  // two waves of CTAs (8 an SM) that go down the rows, or a CTA for each few rows
+  const dim3 grid((unsigned)across, (unsigned)std::min<int64_t>(std::max<int64_t>(1, std::min(down, 148 * 16 / across)), 65535));
   if (vec) {
-    if (a.res) FB_TRY_CUDA(fb::launch(k_dropout<T, true, true>, grid, 256, 0, st, a));
-    else FB_TRY_CUDA(fb::launch(k_dropout<T, true, false>, grid, 256, 0, st, a));
+    if (a.res) FB_TRY_CUDA(fb::launch(k_dropout<T, true, true>, grid, kThreads, 0, st, a));
+    else FB_TRY_CUDA(fb::launch(k_dropout<T, true, false>, grid, kThreads, 0, st, a));
   } else {
-    if (a.res) FB_TRY_CUDA(fb::launch(k_dropout<T, false, true>, grid, 256, 0, st, a));
-    else FB_TRY_CUDA(fb::launch(k_dropout<T, false, false>, grid, 256, 0, st, a));
+    if (a.res) FB_TRY_CUDA(fb::launch(k_dropout<T, false, true>, grid, kThreads, 0, st, a));
+    else FB_TRY_CUDA(fb::launch(k_dropout<T, false, false>, grid, kThreads, 0, st, a));
   }
   return FB_OK;
 }
@@ -97,6 +131,13 @@ extern "C" int fb_dropout(int type, const void *x, int64_t ldx, const void *res,
   if (at % es) return bad("rows that are not aligned to their elements");
   uint64_t bits = at / es | (uint64_t)D;
   if (rows > 1) bits |= (uint64_t)ldx | (uint64_t)ldy | (res ? (uint64_t)ldr : 0);
-  const DropArgs a{x, res, y, ldx, ldr, ldy, rows, D, (D + 3) / 4, p, 1.f / (1.f - p), seed, offset, offset_dev};
+  DropArgs a{};
+  a.x = x, a.ldx = ldx, a.res = res, a.ldr = ldr, a.y = y, a.ldy = ldy, a.rows = rows, a.D = D, a.quads = (D + 3) / 4;
+  // a word's upper 24 bits as a fraction are not below p: the word is not below ceil(p 2^24) 2^8 (p has 24 bits, the product is exact)
+  a.from = (uint32_t)std::ceil(p * 16777216.f) << 8;
+  a.scale = 1.f / (1.f - p);
+  for (int r = 0; r < 10; ++r)
+    a.key[r][0] = (uint32_t)seed + (uint32_t)r * 0x9E3779B9u, a.key[r][1] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
+  a.offset = offset, a.offset_dev = offset_dev;
   return type == FB_F32 ? run<float>(a, bits % 4 == 0, stream) : run<bf16>(a, bits % 4 == 0, stream);
 }

@@ -6,9 +6,13 @@
 //
 // Bound by the state's bytes, read once and written once.  Row r works on state
 // index[r].  Events of one node take their turns in the rows' order, as a
-// chronological batch means them: k_links finds each row's successor of the
-// same node, the first row of a node walks the chain with the state in
-// registers, the others do nothing.
+// chronological batch means them: the first row of a node walks its rows with the
+// state in registers, the others do nothing.  Which row is first and which comes
+// next is looked up by comparing indices: by the warps themselves in calls of few
+// rows, in calls of many by k_links before (a lane a row, the other indices from
+// shared memory).
+// Warps stay on their columns and take rows one after the other, so that weights
+// stay in registers, and load some before they work on the first.
 #include <algorithm>
 #include "head.cuh"
 #include "history.cuh"
@@ -18,39 +22,100 @@ using namespace fbq;
 
 constexpr int64_t kSms = 148;
 constexpr int kMaxTaps = 8, kMaxStates = 64;
-constexpr int kFollows = -2;               // link of a row that another row of its node comes before
-constexpr int kLast = -1;                  // end of a chain
+constexpr int kAlone = 64;                 // rows up to which the warps compare indices themselves
+constexpr int kMaxRows = 1 << 16;          // comparing grows with the square of the rows
+constexpr int kLast = -1;                  // end of a node's rows
 
 struct Rows {
   const int64_t *index;                    // null: row r is state r
   int64_t states;
   int rows;
-  const int2 *link;                        // x: the next row of the node, or kLast; y: kFollows where it is not the first
+  const int2 *link;                        // x: the next row of the node, or kLast; y: 1 where another row comes before
   // The state of a row, -1: none.
-  __device__ __forceinline__ int64_t at(int r) const {
+  __device__ __forceinline__ int at(int r) const {
     if (!index) return r;
     const int64_t i = index[r];
-    return i >= 0 && i < states ? i : -1;
+    return i >= 0 && i < states ? (int)i : -1;
+  }
+  // What a row that has no state receives.
+  __device__ __forceinline__ float held(int r) const { return index[r] < 0 ? 0.f : __int_as_float(0x7fffffff); }
+  // Whether a row of the same node comes before r; each lane for a row of its own.
+  __device__ __forceinline__ bool follows(int r) const {
+    if (!index || rows == 1 || r >= rows) return false;
+    if (link) return link[r].y != 0;
+    const int64_t me = index[r];
+    bool yes = false;
+    for (int j = 0; j < rows; ++j) yes |= j < r && index[j] == me;
+    return yes;
+  }
+  // The next row of the node, kLast: none.
+  __device__ __forceinline__ int next(int r) const {
+    if (!index || rows == 1) return kLast;
+    if (link) return link[r].x;
+    const int64_t me = index[r];
+    for (int j = r + 1; j < rows; ++j)
+      if (index[j] == me) return j;
+    return kLast;
   }
 };
 
-// One warp a row: all other rows of the same node, 32 a step.
-__global__ void __launch_bounds__(256) k_links(const int64_t *index, int rows, int2 *link) {
+// A lane a row, the 32 warps of a CTA a 32nd of the other rows each.
+constexpr int kPart = 4096;
+__global__ void __launch_bounds__(1024) k_links(const int64_t *index, int rows, int64_t states, int2 *link) {
   fb::pdl_enter();
-  const int r = (int)((blockIdx.x * 256 + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-  if (r >= rows) return;
-  const int64_t me = index[r];
-  int next = INT32_MAX;
-  bool before = false;
+  __shared__ __align__(16) int some[kPart];
+  __shared__ int2 found[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * 32 + lane;
+  const auto id = [&](int j) {             // rows without a state are of no node
+    const int64_t i = j < rows ? index[j] : -1;
+    return i >= 0 && i < states ? (int)i : -1;
+  };
+  const int me = r < rows ? id(r) : -1;
+  int next = INT32_MAX, before = 0;
+  for (int base = 0; base < rows; base += kPart) {
+    if (base) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPart / 1024; ++i) some[i * 1024 + threadIdx.x] = id(base + i * 1024 + threadIdx.x);
+    __syncthreads();
+    const int from = warp * (kPart / 32), end = min(from + kPart / 32, rows - base);
 #pragma unroll 4
-  for (int j = lane; j < rows; j += 32) {
-    const bool same = index[j] == me;
-    before |= same && j < r;
-    if (same && j > r) next = min(next, j);
+    for (int i = from; i < end; i += 4) {
+      const int4 v = *reinterpret_cast<const int4 *>(&some[i]);
+      const int o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (o[k] == me) {
+          const int j = base + i + k;
+          if (j < r) before = 1;
+          else if (j > r) next = min(next, j);
+        }
+    }
   }
-  next = __reduce_min_sync(0xffffffffu, next);
-  before = __any_sync(0xffffffffu, before);
-  if (lane == 0) link[r] = make_int2(next == INT32_MAX ? kLast : next, before ? kFollows : 0);
+  found[lane][warp] = make_int2(next, before);
+  __syncthreads();
+  const int2 f = found[warp][lane];        // warp w: row w of the 32
+  next = __reduce_min_sync(0xffffffffu, f.x), before = __reduce_or_sync(0xffffffffu, (unsigned)f.y);
+  const int out = blockIdx.x * 32 + warp;
+  if (lane == 0 && out < rows) link[out] = make_int2(next == INT32_MAX ? kLast : next, before);
+}
+
+// The V K taps of V columns, in one go where they are aligned.
+template <int V, int KT> __device__ __forceinline__ void taps(const float *w, int K, bool wide, float (&out)[KT][V]) {
+  constexpr int N = V * KT, A = N % 4 == 0 ? 4 : (N % 2 == 0 ? 2 : 1);
+  if (KT < 8 && wide) {
+    float flat[N];
+#pragma unroll
+    for (int i = 0; i < N; i += A) *reinterpret_cast<Vec<float, A> *>(&flat[i]) = *reinterpret_cast<const Vec<float, A> *>(w + i);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < KT; ++k) out[k][v] = flat[v * KT + k];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < KT; ++k) out[k][v] = k >= KT - K ? w[v * K + k - (KT - K)] : 0.f;
+  }
 }
 
 // ---- convolution -----------------------------------------------------------------------------------
@@ -61,58 +126,86 @@ struct ConvStep {
   void *state;                             // [states, K - 1, D]
   const float *w, *bias;
   Rows r;
+  int across, each;                        // warps along the columns; rows of a warp, at most 32
+  bool wide;                               // w is 16-byte aligned
 };
 
+// KT taps in registers; KT 2, 3, 4: exactly K, KT 8: the first 8 - K of them do not exist.
 template <typename T, int V, int KT> __global__ void __launch_bounds__(256) k_conv_step(ConvStep a) {
   fb::pdl_enter();
-  const int groups = a.D / V;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)groups * a.r.rows) return;
-  int r = (int)(i / groups);
-  const int col = (int)(i % groups) * V;
-  const int64_t at = a.r.at(r);
-  const int skip = KT - a.K;
-  if (at < 0) {                            // held out: nothing is touched
-    Vec<T, V> y;
-#pragma unroll
-    for (int v = 0; v < V; ++v) y.e[v] = from_f<T>(a.r.index[r] < 0 ? 0.f : __int_as_float(0x7fffffff));
-    *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.y) + r * a.ldy + col) = y;
-    return;
-  }
-  if (a.r.link && a.r.link[r].y == kFollows) return;
-  T *const state = static_cast<T *>(a.state) + at * (a.K - 1) * a.D + col;
-  Vec<T, V> win[KT];
-#pragma unroll
-  for (int k = 0; k < KT - 1; ++k)
-    if (k >= skip) win[k] = *reinterpret_cast<const Vec<T, V> *>(state + (int64_t)(k - skip) * a.D);
+  using E = Vec<T, V>;
+  const int lane = threadIdx.x & 31, skip = KT < 8 ? 0 : KT - a.K;
+  const int wid = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5);
+  const int col = (wid % a.across * 32 + lane) * V, base = wid / a.across * a.each;
+  if (base >= a.r.rows) return;
+  const bool has = col < a.D;
+  const int count = min(a.each, a.r.rows - base);
+  // what the lanes know of the warp's rows
+  const int at_ = lane < count ? a.r.at(base + lane) : -1;
+  const bool follows = lane < count && a.r.follows(base + lane);
   float w[KT][V], bias[V];
+  taps<V, KT>(a.w + (int64_t)(has ? col : 0) * a.K, a.K, a.wide, w);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    bias[v] = a.bias ? a.bias[col + v] : 0.f;
+  for (int v = 0; v < V; ++v) bias[v] = has && a.bias ? a.bias[col + v] : 0.f;
+  const auto state_of = [&](int at) { return static_cast<T *>(a.state) + (int64_t)at * (a.K - 1) * a.D + col; };
+  const auto input = [&](int r) { return *reinterpret_cast<const E *>(static_cast<const T *>(a.x) + r * a.ldx + col); };
+  const auto put = [&](int r, const E &y) { *reinterpret_cast<E *>(static_cast<T *>(a.y) + r * a.ldy + col) = y; };
+  const auto window = [&](int at, E (&win)[KT]) {
 #pragma unroll
-    for (int k = 0; k < KT; ++k) w[k][v] = k >= skip ? a.w[(int64_t)(col + v) * a.K + k - skip] : 0.f;
+    for (int k = 0; k < KT - 1; ++k)
+      if (k >= skip) win[k] = *reinterpret_cast<const E *>(state_of(at) + (int64_t)(k - skip) * a.D);
+  };
+  unsigned held = __ballot_sync(0xffffffffu, lane < count && at_ < 0);
+  unsigned heads = __ballot_sync(0xffffffffu, lane < count && at_ >= 0 && !follows);
+  for (; held; held &= held - 1) {
+    const int r = base + __ffs(held) - 1;
+    E y;
+#pragma unroll
+    for (int v = 0; v < V; ++v) y.e[v] = from_f<T>(a.r.held(r));
+    if (has) put(r, y);
   }
-  for (;;) {
-    win[KT - 1] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(a.x) + r * a.ldx + col);
-    Vec<T, V> y;
+  if (!heads) return;
+  // kBatch nodes' windows are loaded together, then worked on one by one
+  constexpr int kBatch = 2;
+  while (heads) {
+    E win[kBatch][KT];
+    int row[kBatch], at[kBatch];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float p = bias[v];
-#pragma unroll
-      for (int k = 0; k < KT; ++k)
-        if (k >= skip) p = fmaf(w[k][v], to_f(win[k].e[v]), p);
-      y.e[v] = from_f<T>(a.silu ? p * sigmoid(p) : p);
+    for (int i = 0; i < kBatch; ++i) {
+      row[i] = heads ? base + __ffs(heads) - 1 : -1;
+      at[i] = __shfl_sync(0xffffffffu, at_, max(row[i] - base, 0));
+      heads &= heads - 1;
+      if (row[i] >= 0 && has) window(at[i], win[i]), win[i][KT - 1] = input(row[i]);
     }
-    *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.y) + r * a.ldy + col) = y;
 #pragma unroll
-    for (int k = 0; k < KT - 1; ++k) win[k] = win[k + 1];
-    const int next = a.r.link ? a.r.link[r].x : kLast;
-    if (next < 0) break;
-    r = next;
+    for (int i = 0; i < kBatch; ++i) {
+      int r = row[i];
+      if (r < 0) break;
+      int next = a.r.next(r);
+      for (;;) {
+        E y;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float p = bias[v];
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+            if (k >= skip) p = fmaf(w[k][v], to_f(win[i][k].e[v]), p);
+          y.e[v] = from_f<T>(a.silu ? p * sigmoid(p) : p);
+        }
+        if (has) put(r, y);
+#pragma unroll
+        for (int k = 0; k < KT - 1; ++k) win[i][k] = win[i][k + 1];
+        if (next < 0) break;
+        r = next;
+        if (has) win[i][KT - 1] = input(r);
+        next = a.r.next(r);
+      }
+      if (has)
+#pragma unroll
+        for (int k = 0; k < KT - 1; ++k)
+          if (k >= skip) *reinterpret_cast<E *>(state_of(at[i]) + (int64_t)(k - skip) * a.D) = win[i][k];
+    }
   }
-#pragma unroll
-  for (int k = 0; k < KT - 1; ++k)
-    if (k >= skip) *reinterpret_cast<Vec<T, V> *>(state + (int64_t)(k - skip) * a.D) = win[k];
 }
 
 // ---- scan ------------------------------------------------------------------------------------------
@@ -124,19 +217,21 @@ struct ScanStep {
   const float *A, *Ds, *bias;
   float *state;                            // [states, D, N]
   Rows r;
-  int across;                              // warps along the channels
+  int across, each;                        // warps along the channels; rows of a warp, at most 32
 };
 
-// A warp holds 32 / NL channels, NL = NP / 4 lanes a channel with 4 states each,
-// and takes every (warps / across)-th row, so A stays in registers.
+// A warp holds 32 / NL channels, NL = NP / 4 lanes a channel with 4 states each.
 template <typename T, int NP> __global__ void __launch_bounds__(256) k_scan_step(ScanStep a) {
   fb::pdl_enter();
   constexpr int NL = NP / 4, CL = 32 / NL;
   const int lane = threadIdx.x & 31, nl = lane % NL, n0 = nl * 4;
-  const int64_t wid = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5, warps = (int64_t)gridDim.x * 8;
-  const int d = (int)(wid % a.across) * CL + lane / NL;
+  const int wid = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5);
+  const int d = wid % a.across * CL + lane / NL, base = wid / a.across * a.each;
+  if (base >= a.r.rows) return;
   const bool has = d < a.D;
-  const int grp = has ? d / a.per : 0;
+  const int grp = has ? d / a.per : 0, count = min(a.each, a.r.rows - base);
+  const int at_ = lane < count ? a.r.at(base + lane) : -1;
+  const bool follows = lane < count && a.r.follows(base + lane);
   const auto load = [&](const float *p, float (&v)[4]) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = 0.f;
@@ -155,54 +250,84 @@ template <typename T, int NP> __global__ void __launch_bounds__(256) k_scan_step
 #pragma unroll
   for (int k = 0; k < 4; ++k) A2[k] *= kLog2e;
   const float bias = has && a.bias ? a.bias[d] : 0.f, skip = has && a.Ds ? a.Ds[d] : 0.f;
-  const int64_t step = warps / a.across;
-  if (wid / a.across >= step) return;
-  for (int64_t head = wid / a.across; head < a.r.rows; head += step) {
-    int r = (int)head;
-    const int64_t at = a.r.at(r);
-    if (at < 0) {
-      if (has && nl == 0)
-        static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(a.r.index[r] < 0 ? 0.f : __int_as_float(0x7fffffff));
-      continue;
+
+  struct Event {
+    T u, delta, z, b[4], c[4];
+  };
+  const auto event = [&](int r, Event &e) {
+    const T none = from_f<T>(0.f);
+    e.u = has ? static_cast<const T *>(a.u)[r * a.ldu + d] : none;
+    e.delta = has ? static_cast<const T *>(a.delta)[r * a.ldd + d] : none;
+    e.z = has && a.z ? static_cast<const T *>(a.z)[r * a.ldz + d] : none;
+    const T *b = static_cast<const T *>(a.B) + r * a.ldb + grp * a.gsb, *c = static_cast<const T *>(a.C) + r * a.ldc + grp * a.gsc;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      e.b[k] = n0 + k < a.N ? b[n0 + k] : none;
+      e.c[k] = n0 + k < a.N ? c[n0 + k] : none;
     }
-    if (a.r.link && a.r.link[r].y == kFollows) continue;
-    float *const state = a.state + (at * a.D + (has ? d : 0)) * a.N;
-    float h[4];
-    load(state, h);
-    for (;;) {
-      const float u = has ? to_f(static_cast<const T *>(a.u)[r * a.ldu + d]) : 0.f;
-      float dt = has ? to_f(static_cast<const T *>(a.delta)[r * a.ldd + d]) + bias : 0.f;
-      if (a.softplus) dt = softplus(dt);
-      const T *b = static_cast<const T *>(a.B) + r * a.ldb + grp * a.gsb, *c = static_cast<const T *>(a.C) + r * a.ldc + grp * a.gsc;
-      float v = 0.f;
+  };
+  const auto state_of = [&](int at) { return a.state + ((int64_t)at * a.D + (has ? d : 0)) * a.N; };
+  unsigned held = __ballot_sync(0xffffffffu, lane < count && at_ < 0);
+  unsigned heads = __ballot_sync(0xffffffffu, lane < count && at_ >= 0 && !follows);
+  for (; held; held &= held - 1) {
+    const int r = base + __ffs(held) - 1;
+    if (has && nl == 0) static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(a.r.held(r));
+  }
+  if (!heads) return;
+  // kBatch nodes' states and events are loaded together, then worked on one by one
+  constexpr int kBatch = 4;
+  while (heads) {
+    Event now[kBatch];
+    float h[kBatch][4];
+    int row[kBatch], at[kBatch];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool in = n0 + k < a.N;
-        const float Bn = in ? to_f(b[n0 + k]) : 0.f, Cn = in ? to_f(c[n0 + k]) : 0.f;
-        h[k] = fmaf(ex2(dt * A2[k]), h[k], dt * u * Bn);
-        v = fmaf(Cn, h[k], v);
-      }
+    for (int i = 0; i < kBatch; ++i) {
+      row[i] = heads ? base + __ffs(heads) - 1 : -1;
+      at[i] = __shfl_sync(0xffffffffu, at_, max(row[i] - base, 0));
+      heads &= heads - 1;
+      if (row[i] >= 0) load(state_of(at[i]), h[i]), event(row[i], now[i]);
+    }
 #pragma unroll
-      for (int o = NL / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (has && nl == 0) {
-        v = fmaf(skip, u, v);
-        if (a.z) {
-          const float z = to_f(static_cast<const T *>(a.z)[r * a.ldz + d]);
-          v *= z * sigmoid(z);
+    for (int i = 0; i < kBatch; ++i) {
+      int r = row[i];
+      if (r < 0) break;
+      int next = a.r.next(r);
+      for (;;) {
+        const Event &e = now[i];
+        const float u = to_f(e.u);
+        float dt = to_f(e.delta) + bias;
+        if (a.softplus) dt = softplus(dt);
+        const float dtu = dt * u;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          h[i][k] = fmaf(ex2(dt * A2[k]), h[i][k], dtu * to_f(e.b[k]));
+          v = fmaf(to_f(e.c[k]), h[i][k], v);
         }
-        static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(v);
-      }
-      const int next = a.r.link ? a.r.link[r].x : kLast;
-      if (next < 0) break;
-      r = next;
-    }
-    if (has && n0 < a.N) {
-      if (a.vec) {
-        *reinterpret_cast<float4 *>(state + n0) = make_float4(h[0], h[1], h[2], h[3]);
-      } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (n0 + k < a.N) state[n0 + k] = h[k];
+        for (int o = NL / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (has && nl == 0) {
+          v = fmaf(skip, u, v);
+          if (a.z) {
+            const float z = to_f(e.z);
+            v *= z * sigmoid(z);
+          }
+          static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(v);
+        }
+        if (next < 0) break;
+        r = next;
+        event(r, now[i]);
+        next = a.r.next(r);
+      }
+      if (has && n0 < a.N) {
+        float *const state = state_of(at[i]);
+        if (a.vec) {
+          *reinterpret_cast<float4 *>(state + n0) = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n0 + k < a.N) state[n0 + k] = h[i][k];
+        }
       }
     }
   }
@@ -211,30 +336,41 @@ template <typename T, int NP> __global__ void __launch_bounds__(256) k_scan_step
 // ---- host ------------------------------------------------------------------------------------------
 int rows_of(const char *who, int64_t n, int64_t states, const int64_t *index, void *ws, size_t ws_bytes, cudaStream_t st, Rows &r) {
   if (!index && n > states) return fb::set_error(FB_ERR_ARG, std::string(who) + ": more rows than states");
+  if (states > INT32_MAX) return fb::set_error(FB_ERR_UNSUPPORTED, std::string(who) + ": too many states");
   r = Rows{index, states, (int)n, nullptr};
-  if (!index || n < 2) return FB_OK;
+  if (!index || n <= kAlone) return FB_OK;
   FBH_TRY(fbh::check_ws(ws, who));
   if (ws_bytes < (size_t)n * sizeof(int2)) return fb::set_error(FB_ERR_ARG, std::string(who) + ": workspace too small");
-  FB_TRY_CUDA(fb::launch(k_links, dim3((unsigned)((n + 7) / 8)), 256, 0, st, index, (int)n, static_cast<int2 *>(ws)));
+  FB_TRY_CUDA(fb::launch(k_links, dim3((unsigned)((n + 31) / 32)), 1024, 0, st, index, (int)n, states, static_cast<int2 *>(ws)));
   r.link = static_cast<const int2 *>(ws);
   return FB_OK;
 }
 
-template <typename T, int V> int conv_step(const ConvStep &a, cudaStream_t st) {
-  const int64_t threads = (int64_t)(a.D / V) * a.r.rows;
-  const dim3 grid((unsigned)((threads + 255) / 256));
-  if (a.K <= 4) FB_TRY_CUDA(fb::launch(k_conv_step<T, V, 4>, grid, 256, 0, st, a));
-  else FB_TRY_CUDA(fb::launch(k_conv_step<T, V, 8>, grid, 256, 0, st, a));
+// Rows of a warp: as few as leave `resident` warps on the GPU, at most 32.
+int rows_each(int64_t rows, int64_t across, int64_t resident) {
+  return (int)std::min<int64_t>(32, std::max<int64_t>(1, (rows * across + resident - 1) / resident));
+}
+dim3 warps_grid(int64_t rows, int each, int64_t across) { return dim3((unsigned)(((rows + each - 1) / each * across + 7) / 8)); }
+
+template <typename T, int V> int conv_step(ConvStep &a, cudaStream_t st) {
+  a.across = (a.D + 32 * V - 1) / (32 * V);
+  a.wide = (uintptr_t)a.w % 16 == 0;
+  a.each = rows_each(a.r.rows, a.across, kSms * 32);
+  const dim3 grid = warps_grid(a.r.rows, a.each, a.across);
+  switch (a.K) {
+    case 2: FB_TRY_CUDA(fb::launch(k_conv_step<T, V, 2>, grid, 256, 0, st, a)); break;
+    case 3: FB_TRY_CUDA(fb::launch(k_conv_step<T, V, 3>, grid, 256, 0, st, a)); break;
+    case 4: FB_TRY_CUDA(fb::launch(k_conv_step<T, V, 4>, grid, 256, 0, st, a)); break;
+    default: FB_TRY_CUDA(fb::launch(k_conv_step<T, V, 8>, grid, 256, 0, st, a));
+  }
   return FB_OK;
 }
 
 template <typename T> int scan_step(ScanStep &a, cudaStream_t st) {
   const int np = a.N <= 8 ? 8 : (a.N <= 16 ? 16 : (a.N <= 32 ? 32 : 64)), cl = 32 / (np / 4);
   a.across = (a.D + cl - 1) / cl;
-  // one resident wave of warps (8 CTAs of 8 an SM), each with as many rows as it takes; at least a warp for each channel
-  const int64_t wave = kSms * 64, need = (int64_t)a.across * a.r.rows;
-  int64_t warps = std::max<int64_t>(std::min(need, wave) / a.across * a.across, a.across);
-  const dim3 grid((unsigned)((warps + 7) / 8));
+  a.each = rows_each(a.r.rows, a.across, kSms * 32);
+  const dim3 grid = warps_grid(a.r.rows, a.each, a.across);
   switch (np) {
     case 8: FB_TRY_CUDA(fb::launch(k_scan_step<T, 8>, grid, 256, 0, st, a)); break;
     case 16: FB_TRY_CUDA(fb::launch(k_scan_step<T, 16>, grid, 256, 0, st, a)); break;
@@ -246,7 +382,7 @@ template <typename T> int scan_step(ScanStep &a, cudaStream_t st) {
 
 }  // namespace
 
-extern "C" size_t fb_event_step_ws_bytes(int64_t n) { return n > 1 ? (size_t)n * sizeof(int2) : 0; }
+extern "C" size_t fb_event_step_ws_bytes(int64_t n) { return n > kAlone ? (size_t)n * sizeof(int2) : 0; }
 
 extern "C" int fb_short_conv_step(int type, int act, const void *x, int64_t ldx, const float *w, const float *bias, void *state,
                                   int64_t states, const int64_t *index, void *y, int64_t ldy, int64_t n, int D, int K,
@@ -256,7 +392,7 @@ extern "C" int fb_short_conv_step(int type, int act, const void *x, int64_t ldx,
   if (act != FB_ACT_NONE && act != FB_ACT_SILU) return bad("unknown activation");
   if (n < 0 || states < 0 || D < 1 || K < 1) return bad("bad sizes");
   if (K > kMaxTaps) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv_step: at most 8 taps");
-  if (n > (1 << 24) || D > (1 << 20)) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv_step: too many rows or columns");
+  if (n > kMaxRows || D > (1 << 20)) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv_step: too many rows or columns");
   if (!w || (n && (!x || !y || (K > 1 && !state)))) return bad("missing operand");
   if (n > 1 && (ldx < D || ldy < D)) return bad("leading dimension below the width");
   if (!n) return FB_OK;
@@ -278,7 +414,7 @@ extern "C" int fb_selective_scan_step(const fb_selective_scan_event *s, void *ws
   if (s->type != FB_F32 && s->type != FB_BF16) return bad("unknown element type");
   if (s->n < 0 || s->states < 0 || s->D < 1 || s->N < 1 || s->G < 1 || s->D % s->G) return bad("bad sizes");
   if (s->N > kMaxStates) return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan_step: at most 64 states");
-  if (s->n > (1 << 24) || s->D > (1 << 20)) return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan_step: too many rows or columns");
+  if (s->n > kMaxRows || s->D > (1 << 20)) return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan_step: too many rows or columns");
   if (!s->A || (s->n && (!s->u || !s->delta || !s->B || !s->C || !s->state || !s->y))) return bad("missing operand");
   if (s->n > 1 && (s->ldu < s->D || s->ld_delta < s->D || s->ldy < s->D || (s->z && s->ldz < s->D)))
     return bad("leading dimension below the width");
