@@ -8,8 +8,9 @@
 // group of four columns and goes down the rows, so nothing is divided; the ten
 // rounds' keys come with the launch; the comparison is one of whole numbers
 // (16,384 x 4,096 bf16 with a residual: 107 us with an index divided for each
-// group and the words converted to fractions).  Two rows are loaded before the
-// first is drawn, and 40 warps an SM hide the rest.
+// group and the words converted to fractions).  One row at a time and
+// many warps: with four rows loaded ahead the registers leave too few (95 us
+// against 89).
 #include <algorithm>
 #include <cmath>
 #include "history.cuh"
@@ -43,74 +44,63 @@ __device__ __forceinline__ fb::Philox4 draw(uint32_t c0, uint32_t c1, uint32_t c
   return fb::Philox4{{c0, c1, c2, c3}};
 }
 
-constexpr int kThreads = 256, kAhead = 2;
+constexpr int kThreads = 256;
 
-// VEC: whole groups are moved at once (D is a multiple of 4, rows aligned).
-template <typename T, bool VEC, bool RES> __global__ void __launch_bounds__(kThreads, 5) k_dropout(const __grid_constant__ DropArgs a) {
+// Q groups of four columns a thread.  VEC: they are moved at once (D is a multiple
+// of 4 Q, rows aligned to them).
+template <typename T, int Q, bool VEC, bool RES>
+__global__ void __launch_bounds__(kThreads, Q > 1 ? 6 : 8) k_dropout(const __grid_constant__ DropArgs a) {
   fb::pdl_enter();
-  using E = Vec<T, 4>;
+  using E = Vec<T, 4 * Q>;
   const uint64_t off = a.offset + (a.offset_dev ? (uint64_t)*a.offset_dev : 0);
-  const int tr = threadIdx.x / a.cx, q = blockIdx.x * a.cx + threadIdx.x % a.cx;
+  const int tr = threadIdx.x / a.cx, q = (blockIdx.x * a.cx + threadIdx.x % a.cx) * Q;
   if (tr >= a.ry || q >= a.quads) return;
-  const int c = q * 4, left = VEC ? 4 : a.D - c;
+  const int c = q * 4, left = VEC ? 4 * Q : a.D - c;
   const int64_t step = (int64_t)gridDim.y * a.ry;
-  const T *const px = static_cast<const T *>(a.x) + c, *const pr = RES ? static_cast<const T *>(a.res) + c : nullptr;
-  T *const py = static_cast<T *>(a.y) + c;
   const auto load = [&](const T *p, E &e) {
     if (VEC) {
       e = *reinterpret_cast<const E *>(p);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4 * Q; ++k)
         if (k < left) e.e[k] = p[k];
     }
   };
-  for (int64_t r0 = (int64_t)blockIdx.y * a.ry + tr; r0 < a.rows; r0 += step * kAhead) {
-    E x[kAhead], res[kAhead];
+  for (int64_t r = (int64_t)blockIdx.y * a.ry + tr; r < a.rows; r += step) {
+    E x, res, y;
+    load(static_cast<const T *>(a.x) + r * a.ldx + c, x);
+    if (RES) load(static_cast<const T *>(a.res) + r * a.ldr + c, res);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int64_t r = r0 + i * step;
-      if (r < a.rows) {
-        load(px + r * a.ldx, x[i]);
-        if (RES) load(pr + r * a.ldr, res[i]);
-      }
-    }
+    for (int j = 0; j < Q; ++j) {
+      const fb::Philox4 w = draw((uint32_t)(q + j), (uint32_t)r, (uint32_t)off, (uint32_t)(off >> 32), a.key);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int64_t r = r0 + i * step;
-      if (r >= a.rows) break;
-      const fb::Philox4 w = draw((uint32_t)q, (uint32_t)r, (uint32_t)off, (uint32_t)(off >> 32), a.key);
-      E y;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v = RES ? to_f(res[i].e[k]) : 0.f;
-        if (w.v[k] >= a.from) v = RES ? fmaf(to_f(x[i].e[k]), a.scale, v) : to_f(x[i].e[k]) * a.scale;
+      for (int i = 0; i < 4; ++i) {
+        const int k = 4 * j + i;
+        float v = RES ? to_f(res.e[k]) : 0.f;
+        if (w.v[i] >= a.from) v = RES ? fmaf(to_f(x.e[k]), a.scale, v) : to_f(x.e[k]) * a.scale;
         y.e[k] = from_f<T>(v);
       }
-      if (VEC) {
-        *reinterpret_cast<E *>(py + r * a.ldy) = y;
-      } else {
+    }
+    T *const p = static_cast<T *>(a.y) + r * a.ldy + c;
+    if (VEC) {
+      *reinterpret_cast<E *>(p) = y;
+    } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < left) py[r * a.ldy + k] = y.e[k];
-      }
+      for (int k = 0; k < 4 * Q; ++k)
+        if (k < left) p[k] = y.e[k];
     }
   }
 }
 
-template <typename T> int run(DropArgs &a, bool vec, cudaStream_t st) {
-  a.cx = std::min(a.quads, kThreads);
+template <typename T, int Q, bool VEC> int run(DropArgs &a, cudaStream_t st) {
+  const int groups = (a.quads + Q - 1) / Q;
+  a.cx = std::min(groups, kThreads);
   a.ry = kThreads / a.cx;
-  const int64_t across = (a.quads + a.cx - 1) / a.cx, down = (a.rows + a.ry - 1) / a.ry;
+  const int64_t across = (groups + a.cx - 1) / a.cx, down = (a.rows + a.ry - 1) / a.ry;
   // two waves of CTAs (8 an SM) that go down the rows, or a CTA for each few rows
   const dim3 grid((unsigned)across, (unsigned)std::min<int64_t>(std::max<int64_t>(1, std::min(down, 148 * 16 / across)), 65535));
-  if (vec) {
-    if (a.res) FB_TRY_CUDA(fb::launch(k_dropout<T, true, true>, grid, kThreads, 0, st, a));
-    else FB_TRY_CUDA(fb::launch(k_dropout<T, true, false>, grid, kThreads, 0, st, a));
-  } else {
-    if (a.res) FB_TRY_CUDA(fb::launch(k_dropout<T, false, true>, grid, kThreads, 0, st, a));
-    else FB_TRY_CUDA(fb::launch(k_dropout<T, false, false>, grid, kThreads, 0, st, a));
-  }
+  if (a.res) FB_TRY_CUDA(fb::launch(k_dropout<T, Q, VEC, true>, grid, kThreads, 0, st, a));
+  else FB_TRY_CUDA(fb::launch(k_dropout<T, Q, VEC, false>, grid, kThreads, 0, st, a));
   return FB_OK;
 }
 
@@ -139,5 +129,6 @@ extern "C" int fb_dropout(int type, const void *x, int64_t ldx, const void *res,
   for (int r = 0; r < 10; ++r)
     a.key[r][0] = (uint32_t)seed + (uint32_t)r * 0x9E3779B9u, a.key[r][1] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
   a.offset = offset, a.offset_dev = offset_dev;
-  return type == FB_F32 ? run<float>(a, bits % 4 == 0, stream) : run<bf16>(a, bits % 4 == 0, stream);
+  if (type == FB_F32) return bits % 4 == 0 ? run<float, 1, true>(a, stream) : run<float, 1, false>(a, stream);
+  return bits % 8 == 0 ? run<bf16, 2, true>(a, stream) : bits % 4 == 0 ? run<bf16, 1, true>(a, stream) : run<bf16, 1, false>(a, stream);
 }

@@ -210,7 +210,7 @@ template <typename T, int V, int KT> __global__ void __launch_bounds__(256) k_co
 
 // ---- scan ------------------------------------------------------------------------------------------
 struct ScanStep {
-  int D, N, per, softplus, vec;
+  int D, N, per, tiles, softplus, vec, vec_bc;   // per: channels of a group; tiles: warps across a group
   const void *u, *delta, *B, *C, *z;
   int64_t ldu, ldd, ldb, gsb, ldc, gsc, ldz, ldy;
   void *y;
@@ -220,65 +220,87 @@ struct ScanStep {
   int across, each;                        // warps along the channels; rows of a warp, at most 32
 };
 
-// A warp holds 32 / NL channels, NL = NP / 4 lanes a channel with 4 states each.
+// A warp holds 64 / NL channels, two a thread, NL = NP / 4 lanes along the states
+// with 4 of them each.
 template <typename T, int NP> __global__ void __launch_bounds__(256) k_scan_step(ScanStep a) {
   fb::pdl_enter();
-  constexpr int NL = NP / 4, CL = 32 / NL;
+  constexpr int NL = NP / 4, CH = 64 / NL;
   const int lane = threadIdx.x & 31, nl = lane % NL, n0 = nl * 4;
   const int wid = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5);
-  const int d = wid % a.across * CL + lane / NL, base = wid / a.across * a.each;
+  const int tile = wid % a.across, grp = tile / a.tiles, in = tile % a.tiles * CH + lane / NL * 2;
+  const int base = wid / a.across * a.each;
   if (base >= a.r.rows) return;
-  const bool has = d < a.D;
-  const int grp = has ? d / a.per : 0, count = min(a.each, a.r.rows - base);
+  const int has = min(2, max(0, a.per - in));                    // channels of the thread
+  const int d = grp * a.per + (has ? in : 0), count = min(a.each, a.r.rows - base);
   const int at_ = lane < count ? a.r.at(base + lane) : -1;
   const bool follows = lane < count && a.r.follows(base + lane);
-  const auto load = [&](const float *p, float (&v)[4]) {
+  // states n0 .. n0 + 3 of the two channels at p
+  const auto load = [&](const float *p, F2 (&v)[4]) {
+    float x[2][4] = {};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = 0.f;
-    if (!has || n0 >= a.N) return;
-    if (a.vec) {
-      const float4 f = *reinterpret_cast<const float4 *>(p + n0);
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-    } else {
+    for (int j = 0; j < 2; ++j)
+      if (j < has && n0 < a.N) {
+        const float *q = p + j * a.N + n0;
+        if (a.vec) {
+          const float4 f = *reinterpret_cast<const float4 *>(q);
+          x[j][0] = f.x, x[j][1] = f.y, x[j][2] = f.z, x[j][3] = f.w;
+        } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n0 + k < a.N) v[k] = p[n0 + k];
-    }
+          for (int k = 0; k < 4; ++k)
+            if (n0 + k < a.N) x[j][k] = q[k];
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = pack(x[0][k], x[1][k]);
   };
-  float A2[4];
-  load(a.A + (int64_t)(has ? d : 0) * a.N, A2);
+  F2 A2[4];
+  load(a.A + (int64_t)d * a.N, A2);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) A2[k] *= kLog2e;
-  const float bias = has && a.bias ? a.bias[d] : 0.f, skip = has && a.Ds ? a.Ds[d] : 0.f;
+  for (int k = 0; k < 4; ++k) A2[k] = mul2(A2[k], both(kLog2e));
+  const auto param = [&](const float *p) { return pack(p && has ? p[d] : 0.f, p && has > 1 ? p[d + 1] : 0.f); };
+  const F2 bias = param(a.bias), skip = param(a.Ds);
 
   struct Event {
-    T u, delta, z, b[4], c[4];
+    T u[2], delta[2], z[2];
+    Vec<T, 4> b, c;
   };
-  const auto event = [&](int r, Event &e) {
-    const T none = from_f<T>(0.f);
-    e.u = has ? static_cast<const T *>(a.u)[r * a.ldu + d] : none;
-    e.delta = has ? static_cast<const T *>(a.delta)[r * a.ldd + d] : none;
-    e.z = has && a.z ? static_cast<const T *>(a.z)[r * a.ldz + d] : none;
-    const T *b = static_cast<const T *>(a.B) + r * a.ldb + grp * a.gsb, *c = static_cast<const T *>(a.C) + r * a.ldc + grp * a.gsc;
+  const T none = from_f<T>(0.f);
+  const auto two = [&](const void *p, int64_t at, T (&v)[2]) {
+    const T *q = static_cast<const T *>(p) + at + d;
+    v[0] = has ? q[0] : none, v[1] = has > 1 ? q[1] : none;
+  };
+  const auto four = [&](const void *p, int64_t at, Vec<T, 4> &v) {
+    const T *q = static_cast<const T *>(p) + at + n0;
+    if (a.vec_bc) {
+      if (n0 < a.N) v = *reinterpret_cast<const Vec<T, 4> *>(q);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      e.b[k] = n0 + k < a.N ? b[n0 + k] : none;
-      e.c[k] = n0 + k < a.N ? c[n0 + k] : none;
+      for (int k = 0; k < 4; ++k) v.e[k] = n0 + k < a.N ? q[k] : none;
     }
   };
-  const auto state_of = [&](int at) { return a.state + ((int64_t)at * a.D + (has ? d : 0)) * a.N; };
+  const auto event = [&](int r, Event &e) {
+    two(a.u, r * a.ldu, e.u), two(a.delta, r * a.ldd, e.delta);
+    if (a.z) two(a.z, r * a.ldz, e.z);
+    four(a.B, r * a.ldb + grp * a.gsb, e.b), four(a.C, r * a.ldc + grp * a.gsc, e.c);
+  };
+  const auto state_of = [&](int at) { return a.state + ((int64_t)at * a.D + d) * a.N; };
+  const auto put = [&](int r, float2 v) {
+    T *const y = static_cast<T *>(a.y) + r * a.ldy + d;
+    if (nl == 0 && has) y[0] = from_f<T>(v.x);
+    if (nl == 0 && has > 1) y[1] = from_f<T>(v.y);
+  };
   unsigned held = __ballot_sync(0xffffffffu, lane < count && at_ < 0);
   unsigned heads = __ballot_sync(0xffffffffu, lane < count && at_ >= 0 && !follows);
   for (; held; held &= held - 1) {
     const int r = base + __ffs(held) - 1;
-    if (has && nl == 0) static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(a.r.held(r));
+    const float v = a.r.held(r);
+    put(r, make_float2(v, v));
   }
-  if (!heads) return;
   // kBatch nodes' states and events are loaded together, then worked on one by one
-  constexpr int kBatch = 4;
+  constexpr int kBatch = 2;
   while (heads) {
     Event now[kBatch];
-    float h[kBatch][4];
+    F2 h[kBatch][4];
     int row[kBatch], at[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -294,41 +316,48 @@ template <typename T, int NP> __global__ void __launch_bounds__(256) k_scan_step
       int next = a.r.next(r);
       for (;;) {
         const Event &e = now[i];
-        const float u = to_f(e.u);
-        float dt = to_f(e.delta) + bias;
-        if (a.softplus) dt = softplus(dt);
-        const float dtu = dt * u;
-        float v = 0.f;
+        const F2 u = pack(to_f(e.u[0]), to_f(e.u[1]));
+        F2 none2, dt = add2(pack(to_f(e.delta[0]), to_f(e.delta[1])), bias);
+        if (a.softplus) dt = softplus2<false>(dt, none2);
+        const F2 dtu = mul2(dt, u);
+        F2 v = both(0.f);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          h[i][k] = fmaf(ex2(dt * A2[k]), h[i][k], dtu * to_f(e.b[k]));
-          v = fmaf(to_f(e.c[k]), h[i][k], v);
-        }
-#pragma unroll
-        for (int o = NL / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (has && nl == 0) {
-          v = fmaf(skip, u, v);
-          if (a.z) {
-            const float z = to_f(e.z);
-            v *= z * sigmoid(z);
+          if (n0 + k < a.N || !a.vec_bc) {
+            h[i][k] = fma2(ex2_2(mul2(dt, A2[k])), h[i][k], mul2(dtu, both(to_f(e.b.e[k]))));
+            v = fma2(both(to_f(e.c.e[k])), h[i][k], v);
           }
-          static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(v);
         }
+        float2 y = unpack(v);
+#pragma unroll
+        for (int o = NL / 2; o > 0; o >>= 1) y.x += __shfl_xor_sync(0xffffffffu, y.x, o), y.y += __shfl_xor_sync(0xffffffffu, y.y, o);
+        v = fma2(skip, u, pack(y.x, y.y));
+        if (a.z) {
+          const F2 z = pack(to_f(e.z[0]), to_f(e.z[1]));
+          v = mul2(v, mul2(z, sigmoid2(z)));
+        }
+        put(r, unpack(v));
         if (next < 0) break;
         r = next;
         event(r, now[i]);
         next = a.r.next(r);
       }
-      if (has && n0 < a.N) {
-        float *const state = state_of(at[i]);
-        if (a.vec) {
-          *reinterpret_cast<float4 *>(state + n0) = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
-        } else {
+      float *const state = state_of(at[i]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n0 + k < a.N) state[n0 + k] = h[i][k];
+      for (int j = 0; j < 2; ++j)
+        if (j < has && n0 < a.N) {
+          float x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = j ? unpack(h[i][k]).y : unpack(h[i][k]).x;
+          float *const q = state + j * a.N + n0;
+          if (a.vec) {
+            *reinterpret_cast<float4 *>(q) = make_float4(x[0], x[1], x[2], x[3]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (n0 + k < a.N) q[k] = x[k];
+          }
         }
-      }
     }
   }
 }
@@ -367,8 +396,8 @@ template <typename T, int V> int conv_step(ConvStep &a, cudaStream_t st) {
 }
 
 template <typename T> int scan_step(ScanStep &a, cudaStream_t st) {
-  const int np = a.N <= 8 ? 8 : (a.N <= 16 ? 16 : (a.N <= 32 ? 32 : 64)), cl = 32 / (np / 4);
-  a.across = (a.D + cl - 1) / cl;
+  const int np = a.N <= 8 ? 8 : (a.N <= 16 ? 16 : (a.N <= 32 ? 32 : 64)), ch = 64 / (np / 4);
+  a.tiles = (a.per + ch - 1) / ch, a.across = a.D / a.per * a.tiles;
   a.each = rows_each(a.r.rows, a.across, kSms * 32);
   const dim3 grid = warps_grid(a.r.rows, a.each, a.across);
   switch (np) {
@@ -425,6 +454,9 @@ extern "C" int fb_selective_scan_step(const fb_selective_scan_event *s, void *ws
   a.u = s->u, a.ldu = s->ldu, a.delta = s->delta, a.ldd = s->ld_delta, a.B = s->B, a.ldb = s->ldb, a.gsb = s->ldb_group;
   a.C = s->C, a.ldc = s->ldc, a.gsc = s->ldc_group, a.z = s->z, a.ldz = s->ldz, a.y = s->y, a.ldy = s->ldy;
   a.A = s->A, a.Ds = s->skip, a.bias = s->delta_bias, a.state = s->state;
+  const uintptr_t es = s->type == FB_F32 ? 4 : 2;
+  const uint64_t bc = (uint64_t)s->ldb | (uint64_t)s->ldb_group | (uint64_t)s->ldc | (uint64_t)s->ldc_group;
+  a.vec_bc = s->N % 4 == 0 && bc % 4 == 0 && ((uintptr_t)s->B | (uintptr_t)s->C) % (4 * es) == 0;
   FBH_TRY(rows_of("selective_scan_step", s->n, s->states, s->index, ws, ws_bytes, stream, a.r));
   return s->type == FB_F32 ? scan_step<float>(a, stream) : scan_step<bf16>(a, stream);
 }
