@@ -220,145 +220,159 @@ struct ScanStep {
   int across, each;                        // warps along the channels; rows of a warp, at most 32
 };
 
-// A warp holds 64 / NL channels, two a thread, NL = NP / 4 lanes along the states
-// with 4 of them each.
-template <typename T, int NP> __global__ void __launch_bounds__(256) k_scan_step(ScanStep a) {
+// Sums V values over V lanes, each lane keeping the sum of its own number.
+template <int V> __device__ __forceinline__ float spread_sum(float *v) {
+  if constexpr (V == 1) {
+    return v[0];
+  } else {
+    constexpr int H = V / 2;
+    const bool up = (threadIdx.x & H) != 0;
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      const float send = up ? v[k] : v[k + H], stay = up ? v[k + H] : v[k];
+      v[k] = stay + __shfl_xor_sync(0xffffffffu, send, H);
+    }
+    return spread_sum<H>(v);
+  }
+}
+
+// A warp holds 32 channels.  NL = NP / 4 lanes side by side share NL of them and
+// hold 4 of their states each; what a channel has once (dt, the gate, y) is one
+// lane's, so it is loaded and computed once, 32 channels in a row.
+template <typename T, int NP> __global__ void __launch_bounds__(256, NP <= 16 ? 3 : 1) k_scan_step(ScanStep a) {
   fb::pdl_enter();
-  constexpr int NL = NP / 4, CH = 64 / NL;
+  constexpr int NL = NP / 4, P = NL / 2;
   const int lane = threadIdx.x & 31, nl = lane % NL, n0 = nl * 4;
   const int wid = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5);
-  const int tile = wid % a.across, grp = tile / a.tiles, in = tile % a.tiles * CH + lane / NL * 2;
+  const int tile = wid % a.across, grp = tile / a.tiles, in = tile % a.tiles * 32;
   const int base = wid / a.across * a.each;
   if (base >= a.r.rows) return;
-  const int has = min(2, max(0, a.per - in));                    // channels of the thread
-  const int d = grp * a.per + (has ? in : 0), count = min(a.each, a.r.rows - base);
+  const bool own = in + lane < a.per;
+  const int d = grp * a.per + in + lane;                         // the lane's own channel
+  const int shared = grp * a.per + in + lane - nl;               // the first of those it shares
+  const int has = n0 < a.N ? a.per - (in + lane - nl) : 0;       // how many of them exist (for its states)
+  const int count = min(a.each, a.r.rows - base);
   const int at_ = lane < count ? a.r.at(base + lane) : -1;
   const bool follows = lane < count && a.r.follows(base + lane);
-  // states n0 .. n0 + 3 of the two channels at p
-  const auto load = [&](const float *p, F2 (&v)[4]) {
-    float x[2][4] = {};
+  const auto load = [&](const float *p, F2 (&v)[P][4]) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (j < has && n0 < a.N) {
-        const float *q = p + j * a.N + n0;
-        if (a.vec) {
-          const float4 f = *reinterpret_cast<const float4 *>(q);
-          x[j][0] = f.x, x[j][1] = f.y, x[j][2] = f.z, x[j][3] = f.w;
-        } else {
+    for (int q = 0; q < P; ++q) {
+      float x[2][4] = {};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n0 + k < a.N) x[j][k] = q[k];
+      for (int j = 0; j < 2; ++j)
+        if (2 * q + j < has) {
+          const float *s = p + (2 * q + j) * a.N + n0;
+          if (a.vec) {
+            const float4 f = *reinterpret_cast<const float4 *>(s);
+            x[j][0] = f.x, x[j][1] = f.y, x[j][2] = f.z, x[j][3] = f.w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (n0 + k < a.N) x[j][k] = s[k];
+          }
         }
-      }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = pack(x[0][k], x[1][k]);
+      for (int k = 0; k < 4; ++k) v[q][k] = pack(x[0][k], x[1][k]);
+    }
   };
-  F2 A2[4];
-  load(a.A + (int64_t)d * a.N, A2);
+  F2 A2[P][4];
+  load(a.A + (int64_t)shared * a.N, A2);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) A2[k] = mul2(A2[k], both(kLog2e));
-  const auto param = [&](const float *p) { return pack(p && has ? p[d] : 0.f, p && has > 1 ? p[d + 1] : 0.f); };
-  const F2 bias = param(a.bias), skip = param(a.Ds);
+  for (int q = 0; q < P; ++q)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) A2[q][k] = mul2(A2[q][k], both(kLog2e));
+  const float bias = own && a.bias ? a.bias[d] : 0.f, skip = own && a.Ds ? a.Ds[d] : 0.f;
 
   struct Event {
-    T u[2], delta[2], z[2];
+    T u, delta, z;
     Vec<T, 4> b, c;
   };
   const T none = from_f<T>(0.f);
-  const auto two = [&](const void *p, int64_t at, T (&v)[2]) {
-    const T *q = static_cast<const T *>(p) + at + d;
-    v[0] = has ? q[0] : none, v[1] = has > 1 ? q[1] : none;
-  };
   const auto four = [&](const void *p, int64_t at, Vec<T, 4> &v) {
     const T *q = static_cast<const T *>(p) + at + n0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v.e[k] = none;
     if (a.vec_bc) {
       if (n0 < a.N) v = *reinterpret_cast<const Vec<T, 4> *>(q);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v.e[k] = n0 + k < a.N ? q[k] : none;
+      for (int k = 0; k < 4; ++k)
+        if (n0 + k < a.N) v.e[k] = q[k];
     }
   };
   const auto event = [&](int r, Event &e) {
-    two(a.u, r * a.ldu, e.u), two(a.delta, r * a.ldd, e.delta);
-    if (a.z) two(a.z, r * a.ldz, e.z);
+    e.u = own ? static_cast<const T *>(a.u)[r * a.ldu + d] : none;
+    e.delta = own ? static_cast<const T *>(a.delta)[r * a.ldd + d] : none;
+    e.z = own && a.z ? static_cast<const T *>(a.z)[r * a.ldz + d] : none;
     four(a.B, r * a.ldb + grp * a.gsb, e.b), four(a.C, r * a.ldc + grp * a.gsc, e.c);
-  };
-  const auto state_of = [&](int at) { return a.state + ((int64_t)at * a.D + d) * a.N; };
-  const auto put = [&](int r, float2 v) {
-    T *const y = static_cast<T *>(a.y) + r * a.ldy + d;
-    if (nl == 0 && has) y[0] = from_f<T>(v.x);
-    if (nl == 0 && has > 1) y[1] = from_f<T>(v.y);
   };
   unsigned held = __ballot_sync(0xffffffffu, lane < count && at_ < 0);
   unsigned heads = __ballot_sync(0xffffffffu, lane < count && at_ >= 0 && !follows);
   for (; held; held &= held - 1) {
     const int r = base + __ffs(held) - 1;
-    const float v = a.r.held(r);
-    put(r, make_float2(v, v));
+    if (own) static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(a.r.held(r));
   }
-  // kBatch nodes' states and events are loaded together, then worked on one by one
-  constexpr int kBatch = 2;
-  while (heads) {
-    Event now[kBatch];
-    F2 h[kBatch][4];
-    int row[kBatch], at[kBatch];
+  for (; heads; heads &= heads - 1) {
+    const int first = __ffs(heads) - 1;
+    int r = base + first;
+    float *const state = a.state + ((int64_t)__shfl_sync(0xffffffffu, at_, first) * a.D + shared) * a.N;
+    Event e;
+    F2 h[P][4];
+    load(state, h);
+    event(r, e);
+    int next = a.r.next(r);
+    for (;;) {
+      const float u = to_f(e.u);
+      float dt = to_f(e.delta) + bias;
+      if (a.softplus) dt = softplus(dt);
+      const float dtu = dt * u;
+      F2 B[4], C[4];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      row[i] = heads ? base + __ffs(heads) - 1 : -1;
-      at[i] = __shfl_sync(0xffffffffu, at_, max(row[i] - base, 0));
-      heads &= heads - 1;
-      if (row[i] >= 0) load(state_of(at[i]), h[i]), event(row[i], now[i]);
-    }
+      for (int k = 0; k < 4; ++k) B[k] = both(to_f(e.b.e[k])), C[k] = both(to_f(e.c.e[k]));
+      float y[NL];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      int r = row[i];
-      if (r < 0) break;
-      int next = a.r.next(r);
-      for (;;) {
-        const Event &e = now[i];
-        const F2 u = pack(to_f(e.u[0]), to_f(e.u[1]));
-        F2 none2, dt = add2(pack(to_f(e.delta[0]), to_f(e.delta[1])), bias);
-        if (a.softplus) dt = softplus2<false>(dt, none2);
-        const F2 dtu = mul2(dt, u);
-        F2 v = both(0.f);
+      for (int q = 0; q < P; ++q) {
+        const auto of = [&](float v) {
+          return pack(__shfl_sync(0xffffffffu, v, lane - nl + 2 * q), __shfl_sync(0xffffffffu, v, lane - nl + 2 * q + 1));
+        };
+        const F2 dt2 = of(dt), dtu2 = of(dtu);
+        F2 v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (n0 + k < a.N || !a.vec_bc) {
-            h[i][k] = fma2(ex2_2(mul2(dt, A2[k])), h[i][k], mul2(dtu, both(to_f(e.b.e[k]))));
-            v = fma2(both(to_f(e.c.e[k])), h[i][k], v);
-          }
+          h[q][k] = fma2(ex2_2(mul2(dt2, A2[q][k])), h[q][k], mul2(dtu2, B[k]));
+          v = k == 0 ? mul2(C[k], h[q][k]) : fma2(C[k], h[q][k], v);
         }
-        float2 y = unpack(v);
-#pragma unroll
-        for (int o = NL / 2; o > 0; o >>= 1) y.x += __shfl_xor_sync(0xffffffffu, y.x, o), y.y += __shfl_xor_sync(0xffffffffu, y.y, o);
-        v = fma2(skip, u, pack(y.x, y.y));
-        if (a.z) {
-          const F2 z = pack(to_f(e.z[0]), to_f(e.z[1]));
-          v = mul2(v, mul2(z, sigmoid2(z)));
-        }
-        put(r, unpack(v));
-        if (next < 0) break;
-        r = next;
-        event(r, now[i]);
-        next = a.r.next(r);
+        const float2 f = unpack(v);
+        y[2 * q] = f.x, y[2 * q + 1] = f.y;
       }
-      float *const state = state_of(at[i]);
+      float v = fmaf(skip, u, spread_sum<NL>(y));
+      if (a.z) {
+        const float z = to_f(e.z);
+        v *= z * sigmoid(z);
+      }
+      if (own) static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(v);
+      if (next < 0) break;
+      r = next;
+      event(r, e);
+      next = a.r.next(r);
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        if (j < has && n0 < a.N) {
+        if (2 * q + j < has) {
           float x[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = j ? unpack(h[i][k]).y : unpack(h[i][k]).x;
-          float *const q = state + j * a.N + n0;
+          for (int k = 0; k < 4; ++k) x[k] = j ? unpack(h[q][k]).y : unpack(h[q][k]).x;
+          float *const s = state + (2 * q + j) * a.N + n0;
           if (a.vec) {
-            *reinterpret_cast<float4 *>(q) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4 *>(s) = make_float4(x[0], x[1], x[2], x[3]);
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (n0 + k < a.N) q[k] = x[k];
+              if (n0 + k < a.N) s[k] = x[k];
           }
         }
-    }
   }
 }
 
@@ -396,7 +410,7 @@ template <typename T, int V> int conv_step(ConvStep &a, cudaStream_t st) {
 }
 
 template <typename T> int scan_step(ScanStep &a, cudaStream_t st) {
-  const int np = a.N <= 8 ? 8 : (a.N <= 16 ? 16 : (a.N <= 32 ? 32 : 64)), ch = 64 / (np / 4);
+  const int np = a.N <= 8 ? 8 : (a.N <= 16 ? 16 : (a.N <= 32 ? 32 : 64)), ch = 32;
   a.tiles = (a.per + ch - 1) / ch, a.across = a.D / a.per * a.tiles;
   a.each = rows_each(a.r.rows, a.across, kSms * 32);
   const dim3 grid = warps_grid(a.r.rows, a.each, a.across);
