@@ -15,7 +15,8 @@ and statistics.  bf16 from fp32 parameters converts them at every call; a head
 that only answers queries saves that as a bf16 module throughout
 (NodeRankingHead(..., dtype=torch.bfloat16).to(torch.bfloat16)).
 
-    python -m fast_b200.ranking          # trains it on a synthetic temporal graph (one GPU)
+    python -m fast_b200.ranking            # trains it on a synthetic temporal graph (one GPU)
+    python -m fast_b200.ranking --history  # the same, roots encoded from their own past events (history.py)
 """
 import argparse
 import math
@@ -203,13 +204,57 @@ def train_synthetic(steps=60, nodes=400, edges=20000, batch=200, dim=64, dtype=t
     return losses
 
 
+def train_histories(steps=60, nodes=400, edges=20000, batch=200, dim=64, longest=50, dropout=0.1, dtype=torch.bfloat16, lr=3e-3,
+                    seed=0, log=None):
+    """Trains a state space encoder of each root's own past events (up to
+    `longest`; some roots have none) and the head on a synthetic graph in which
+    the next node follows from the last one; returns the losses."""
+    import numpy as np
+
+    from .history import HistoryEncoder
+    rng = np.random.default_rng(seed)
+    dev = torch.device("cuda")
+    src = rng.integers(0, nodes, edges)
+    jump, last, past = rng.random(edges) < 0.1, rng.integers(0, nodes, nodes), [[] for _ in range(nodes)]
+    dst, seen = np.empty(edges, np.int64), []
+    for e, s in enumerate(src):
+        dst[e] = rng.integers(0, nodes) if jump[e] else (last[s] * 7 + 3) % nodes
+        seen.append(len(past[s]))
+        last[s] = dst[e]
+        past[s].append(dst[e])
+    torch.manual_seed(seed)
+    embedding = torch.nn.Embedding(nodes, dim).to(dev)
+    encoder, head = HistoryEncoder(dim, 2, dropout=dropout, dtype=dtype).to(dev), NodeRankingHead(dim, nodes, dtype=dtype).to(dev)
+    opt = torch.optim.Adam([*embedding.parameters(), *encoder.parameters(), *head.parameters()], lr=lr)
+    losses, at = [], edges // 4
+    for step in range(steps):
+        if at + batch > edges:
+            at = edges // 4
+        rows, starts = [], [0]
+        for e in range(at, at + batch):
+            rows += past[src[e]][max(0, seen[e] - longest):seen[e]]
+            starts.append(len(rows))
+        starts = torch.tensor(starts, device=dev)
+        x = encoder(embedding(torch.tensor(np.array(rows, dtype=np.int64), device=dev)), starts, seed=seed, offset=step)
+        loss, _ = head(encoder.last(x, starts), torch.from_numpy(dst[at:at + batch]).to(dev))
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+        losses.append(float(loss.detach()))
+        if log and step % 10 == 0:
+            log("step %d: loss %.4f (uniform over %d nodes: %.4f)" % (step, losses[-1], nodes, math.log(nodes)))
+        at += batch
+    return losses
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description="Train the node-ranking head on a synthetic temporal graph (one GPU).")
     ap.add_argument("--steps", type=int, default=100)
     ap.add_argument("--nodes", type=int, default=400)
     ap.add_argument("--dtype", choices=("bf16", "fp32"), default="bf16")
+    ap.add_argument("--history", action="store_true", help="encode roots from their own past events, not sampled neighbours")
     a = ap.parse_args(argv)
-    losses = train_synthetic(a.steps, a.nodes, dtype=torch.bfloat16 if a.dtype == "bf16" else torch.float32, log=print)
+    losses = (train_histories if a.history else train_synthetic)(a.steps, a.nodes, dtype=torch.bfloat16 if a.dtype == "bf16" else torch.float32, log=print)
     print("first ten steps %.4f, last ten %.4f" % (sum(losses[:10]) / len(losses[:10]), sum(losses[-10:]) / len(losses[-10:])))
 
 
