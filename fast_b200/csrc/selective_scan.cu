@@ -408,13 +408,15 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
 
 // Joins the chunks: edge[c], what chunk c alone leaves, becomes what arrives
 // behind it (REV: in front of chunk c + 1, from the rows behind).
-template <bool REV> __global__ void __launch_bounds__(256) k_scan_join(ScanArgs a) {
+// Bound by the latency of its loads, so 32 chunks' are in flight (188 chunks of
+// width 200: 20 us with 8).
+template <bool REV> __global__ void __launch_bounds__(128) k_scan_join(ScanArgs a) {
   fb::pdl_enter();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, size = (int64_t)a.D * a.N;
+  const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x, size = (int64_t)a.D * a.N;
   if (i >= size) return;
   const int c = (int)(i / a.N);
   const float A2 = a.A[i] * kLog2e;
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 32;
   const int n = a.nc - 1;
   float x = 0.f;
   for (int at = 0; at < n; at += kAhead) {
@@ -804,14 +806,16 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
 #pragma unroll
       for (int t = threadIdx.x; t < kSums * kParts; t += kThreads) {
         const int l = t % L::NL, part = t / L::NL % kParts, which = t / (L::NL * kParts) % 2, row = t / (L::NL * kParts * 2);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        F2 v01 = both(0.f), v23 = both(0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w)
 #pragma unroll
           for (int m = part; m < L::CL; m += kParts) {
-            const float4 f = sm.sum[w][row][which][m * L::NL + l];
-            v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(&sm.sum[w][row][which][m * L::NL + l]);
+            v01 = add2(v01, F2{f.x}), v23 = add2(v23, F2{f.y});
           }
+        const float2 v0 = unpack(v01), v2 = unpack(v23);
+        float4 v = make_float4(v0.x, v0.y, v2.x, v2.y);
 #pragma unroll
         for (int o = L::NL; o < L::NL * kParts; o *= 2) {
           v.x += __shfl_xor_sync(0xffffffffu, v.x, o), v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
@@ -884,20 +888,24 @@ template <typename T> __global__ void __launch_bounds__(256) k_scan_sums(ScanArg
     if (col % NP < a.N) static_cast<T *>(col < NP ? a.dB : a.dC)[(q * a.G + grp) * a.N + col % NP] = from_f<T>(v);
     return;
   }
-  const int64_t i = (blockIdx.x - bc_blocks) * 256 + threadIdx.x, size = (int64_t)a.D * a.N;
-  if (i < size) {
-    float v = 0.f;
+  // 32 sums a CTA, 8 threads each
+  __shared__ float part[8][32];
+  const int64_t i = (blockIdx.x - bc_blocks) * 32 + threadIdx.x % 32, size = (int64_t)a.D * a.N, all = size + 2 * (int64_t)a.D;
+  const float *p = i < size ? a.pA + i : a.pD + (i - size);
+  const int64_t step = i < size ? size : 2 * (int64_t)a.D;
+  float v = 0.f;
+  if (i < all) {
 #pragma unroll 8
-    for (int k = 0; k < a.nc; ++k) v += a.pA[k * size + i];
-    a.dA[i] = v;
-  } else if (i < size + 2 * (int64_t)a.D) {
-    const int64_t j = i - size;
-    float v = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < a.nc; ++k) v += a.pD[k * 2 * (int64_t)a.D + j];
-    if (j < a.D) a.dD[j] = v;
-    else a.dbias[j - a.D] = v;
+    for (int k = threadIdx.x / 32; k < a.nc; k += 8) v += p[k * step];
   }
+  part[threadIdx.x / 32][threadIdx.x % 32] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32 || i >= all) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) v += part[k][threadIdx.x];
+  if (i < size) a.dA[i] = v;
+  else if (i < size + a.D) a.dD[i - size] = v;
+  else a.dbias[i - size - a.D] = v;
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -1011,7 +1019,7 @@ template <typename T, int NP> int run_fwd(const ScanArgs &a, cudaStream_t stream
   FBH_TRY((allow(k_scan_fwd<T, NP, false>, smem)));
   if (a.nc > 1) {
     FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, true>, blocks(nct * (a.nc - 1), kWarps), kThreads, smem, stream, a));
-    FB_TRY_CUDA(fb::launch(k_scan_join<false>, blocks((int64_t)a.D * a.N, 256), 256, 0, stream, a));
+    FB_TRY_CUDA(fb::launch(k_scan_join<false>, blocks((int64_t)a.D * a.N, 128), 128, 0, stream, a));
   }
   FB_TRY_CUDA(fb::launch(k_scan_fwd<T, NP, false>, blocks(nct * a.nc, kWarps), kThreads, smem, stream, a));
   return FB_OK;
@@ -1023,11 +1031,11 @@ template <typename T, int NP> int run_bwd(const ScanArgs &a, cudaStream_t stream
   if (a.nc > 1) {
     const int64_t nct = (int64_t)a.G * a.tiles;
     FB_TRY_CUDA(fb::launch(k_scan_rev<T, NP>, blocks(nct * (a.nc - 1), kWarps), kThreads, 0, stream, a));
-    FB_TRY_CUDA(fb::launch(k_scan_join<true>, blocks((int64_t)a.D * a.N, 256), 256, 0, stream, a));
+    FB_TRY_CUDA(fb::launch(k_scan_join<true>, blocks((int64_t)a.D * a.N, 128), 128, 0, stream, a));
   }
   FB_TRY_CUDA(fb::launch(k_scan_bwd<T, NP>, dim3((unsigned)(a.G * a.ctas), (unsigned)a.nc), kThreads, smem, stream, a));
   const int64_t bc = a.ctas > 1 ? blocks((int64_t)a.G * a.st.rows * 2 * NP, 256) : 0;
-  const int64_t rest = a.nc > 1 ? blocks((int64_t)a.D * (a.N + 2), 256) : 0;
+  const int64_t rest = a.nc > 1 ? blocks((int64_t)a.D * (a.N + 2), 32) : 0;
   if (bc + rest) FB_TRY_CUDA(fb::launch(k_scan_sums<T>, dim3((unsigned)(bc + rest)), 256, 0, stream, a, (int)NP, bc));
   return FB_OK;
 }
