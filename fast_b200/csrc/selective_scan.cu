@@ -547,7 +547,7 @@ template <int NP> struct BwdSmem {
   static constexpr int P = kBwdPairs<NP>, CH = Lay<NP, P>::CH;
   float dt[kWarps][kTile][CH], dtu[kWarps][kTile][CH], gv[kWarps][kTile][CH];
   float out[kWarps][3][kHalf][2 * P][32];                            // each lane's part of <g, B>, <q, A log2 e>, <C, h>
-  float2 B[kTile][NP], C[kTile][NP];
+  float B[kTile][NP], C[kTile][NP];                             // once: here the accesses cost more than doubling them
   float4 sum[kWarps][kHalf][2][32];                              // each lane's part of dB, dC of its states
   float4 own[kWarps][Lay<NP, P>::X::E][32];                      // u, dy silu'(z), softplus', dt of each lane's elements
   int seq[kWarps][kTile + 1];                                    // of the rows in front of and at beginnings
@@ -655,8 +655,8 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
       const int at = threadIdx.x + kThreads * i;
       if (at < kTile * NP) {
         const float b = to_f(xb[i]), c = to_f(xc[i]);
-        sm.B[at / NP][at % NP] = make_float2(b, b);
-        sm.C[at / NP][at % NP] = make_float2(c, c);
+        sm.B[at / NP][at % NP] = b;
+        sm.C[at / NP][at % NP] = c;
       }
     }
     const unsigned begins = walk.tile(a.st, c0 + t0);
@@ -688,9 +688,9 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
         v[0].v = t.x, v[1].v = t.y;
       }
     };
-    const auto twice = [&](const float2 (&p)[kTile][NP], int i, F2 (&v)[4]) {
-      const ulonglong2 *t = reinterpret_cast<const ulonglong2 *>(&p[i][n0]);
-      v[0].v = t[0].x, v[1].v = t[0].y, v[2].v = t[1].x, v[3].v = t[1].y;
+    const auto twice = [&](const float (&p)[kTile][NP], int i, F2 (&v)[4]) {
+      const float4 f = *reinterpret_cast<const float4 *>(&p[i][n0]);
+      v[0] = both(f.x), v[1] = both(f.y), v[2] = both(f.z), v[3] = both(f.w);
     };
     // h behind row i; the decays of the first pair are kept
     const auto ahead = [&](int i, States<P> &h, F2 (&kept)[4]) {
@@ -912,16 +912,20 @@ template <typename T> __global__ void __launch_bounds__(256) k_scan_sums(ScanArg
 int padded(int N) { return N <= 8 ? 8 : (N <= 16 ? 16 : (N <= 32 ? 32 : 64)); }
 
 // Rows of a chunk, for `tiles` units of work side by side of which the GPU holds
-// `resident`: whole waves of units, three if the chunks stay at kShort rows, for
-// then early ends of some chunks even out (16,384 x 1,024 backward: 922 us with
-// one wave, 881 with two, 866 with three), else two or one.
-constexpr int64_t kShort = 64;
-int64_t chunk_rows(int64_t rows, int64_t tiles, int64_t resident) {
-  int64_t c = kShort;
-  for (int64_t waves = 3; waves; --waves) {
+// `resident`: whole waves of units as long as the chunks keep `shortest` rows, for
+// then early ends of some chunks even out.  16,384 x 1,024 bf16, both passes:
+// backward in one wave 922 us, two 881, three 866; forward in three 845, two
+// 834.  Shorter chunks lose more to the passes between them than they gain:
+// forward of 2,048 x 2,048 with chunks of at least 32, 48, 64, 96 rows 76, 73,
+// 78, 111 us; both passes of 5,003 x 413 171, 178, 188, 201, of 12,000 x 200 fp32
+// 243, 243, 239, 242; backward of the latter two with 32, 64, 96 rows 260, 243,
+// 246 and 170, 171, 190.
+int64_t chunk_rows(int64_t rows, int64_t tiles, int64_t resident, int64_t waves, int64_t shortest) {
+  int64_t c = shortest;
+  for (; waves; --waves) {
     const int64_t want = std::max<int64_t>(1, resident * waves / tiles);
     const int64_t even = ((rows + want - 1) / want + kTile - 1) / kTile * kTile;
-    if (even >= kShort) {
+    if (even >= shortest) {
       c = even;
       break;
     }
@@ -970,7 +974,7 @@ constexpr int64_t kSms = 148;
 int plan_fwd(ScanArgs &a, int np, fbh::Call &c) {
   const int ch = 2 * 2 * 32 / (np / 4);
   a.tiles = (a.per + ch - 1) / ch;
-  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * 16);
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * 16, 2, 48);
   a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
   if (a.nc > 1) {
     FBH_TAKE(edge, c, float, (a.nc - 1) * (int64_t)a.D * a.N);
@@ -985,7 +989,7 @@ int plan_bwd(ScanArgs &a, int np, fbh::Call &c) {
   const int ch = 2 * (np > 32 ? 2 : 1) * 32 / (np / 4);   // channels of a warp
   const int tiles = (a.per + ch - 1) / ch;
   a.ctas = (tiles + kWarps - 1) / kWarps;
-  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.ctas, kSms * (np > 32 ? 2 : kBwdCtas));
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.ctas, kSms * (np > 32 ? 2 : kBwdCtas), 3, 64);
   a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
   a.tiles = (a.per + 4 * 32 / (np / 4) - 1) / (4 * 32 / (np / 4));          // k_scan_rev's
   const int64_t size = (int64_t)a.D * a.N;
