@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(kThreads, Q > 1 ? 6 : 8) k_dropout(const __gri
     if (RES) load(static_cast<const T *>(a.res) + r * a.ldr + c, res);
 #pragma unroll
     for (int j = 0; j < Q; ++j) {
-      const fb::Philox4 w = draw((uint32_t)(q + j), (uint32_t)r, (uint32_t)off, (uint32_t)(off >> 32), a.key);
+      fb::Philox4 w = {};
+      if (a.from) w = draw((uint32_t)(q + j), (uint32_t)r, (uint32_t)off, (uint32_t)(off >> 32), a.key);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = 4 * j + i;

@@ -10,20 +10,24 @@
 //   q = g exp(dt A) h[t-1] = r[t-1] h[t-1]
 //   ddelta = (<q, A> + u <g, B>) softplus',  dA = sum_t q dt,  dD = sum_t gv u
 //
-// What bounds it: one exponential for each (row, channel, state).  At 16 states
-// the special function units, 16 a clock and SM, need one clock for a (row,
-// channel) and pass; its bytes (8 in bf16, gate included) need 0.36 of a clock's
-// share of the memory.  So the layout serves the arithmetic:
+// What bounds it: instructions.  The special function units give 16 exponentials
+// a clock and SM, so at 16 states one clock for each (row, channel) and pass; the
+// bytes (8 a (row, channel) in bf16, gate included) take 0.36 of that, and the
+// packed fp32 arithmetic about as much as the exponentials.  So the layout saves
+// what surrounds them:
 //
 // - A warp owns a tile of channels and walks down the rows.  A thread holds 4
 //   channels x 4 states (2 x 4 in the backward): what is read from shared memory
-//   per row (dt, dt u of its channels, B, C of its states) is used 4 times, and
-//   the sums over states (y) and over channels (dB, dC) take a few shuffles in
-//   which every lane ends up with a value of its own.  Channels sit in pairs,
-//   which the packed fp32 instructions take two at a time.
+//   per row (dt, dt u of its channels, B, C of its states) serves several of
+//   them.  Channels sit in pairs, which the packed instructions take two at a
+//   time.  Sums over states and over channels go through shared memory: each lane
+//   stores its parts, whoever needs a sum adds them (with shuffles, in which
+//   every lane ended up with one sum, the backward took 485 us instead of 444 at
+//   16,384 x 1,024, 16 states, bf16).
 // - Rows come in tiles of 8.  Their softplus, dt u and the gate are computed
 //   once for each (row, channel) with the lanes along the channels; the next
 //   tile's loads are in flight meanwhile.  Any pitch and alignment is the same.
+//   Tiles in which no sequence begins run without a branch.
 // - The packed rows are cut into chunks of a fixed number of rows wherever the
 //   sequences begin, so the grid needs nothing from the device.  A first pass
 //   reduces each chunk to its last state, from the last beginning of a sequence
@@ -32,11 +36,17 @@
 //   a factor of 0: an infinity stays in its own sequence.  One chunk needs one
 //   launch.
 // - For a backward pass the forward keeps the state in front of every 8th row,
-//   2 N bytes a (row, channel): written beside arithmetic that leaves the memory
-//   idle, and cheaper than another pass of exponentials.  The backward
-//   recomputes 8 rows of states and decays into registers and walks them back.
+//   N / 2 bytes a (row, channel): written beside arithmetic that leaves the memory
+//   idle, and cheaper than another pass of exponentials.  The backward recomputes
+//   4 rows of states and decays into registers and walks them back: 8 rows at
+//   once take the registers of the third CTA an SM (906 us against 866, both
+//   passes).
 // - Sums over rows and channels end in per-CTA partials that one more launch
 //   adds in a fixed order: results repeat bit for bit.
+//
+// 16,384 x 1,024, 64 ragged sequences, bf16, 16 states: forward 88 (last states) +
+// 15 + 160 us, backward 92 (first gradients) + 8 + 444 + 17; at 148 SMs and 1.9 GHz
+// the exponentials alone take 60 us a pass.
 //
 // Everything between the loads and the stores is fp32.
 #include <algorithm>
@@ -57,6 +67,10 @@ constexpr int kKept = 1;                  // pairs of a thread whose decays it h
 // 0.6 to 2.4e-8 on average where decays are slow (measured for exponents of -1e-4
 // to -1), which a state that remembers a thousand steps adds up a thousand
 // times; the summand centres them.
+// A log2(e), kept finite so that a row of no sequence (dt 0) leaves the state as it
+// is even where A is -infinity.
+__device__ __forceinline__ float scaled(float A) { return max_nan(A * kLog2e, -3e38f); }
+
 __device__ __forceinline__ F2 decays(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, both(2e-8f))); }
 
 struct ScanArgs {
@@ -245,7 +259,7 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], both(kLog2e));
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = pack(scaled(unpack(A2.v[p][k]).x), scaled(unpack(A2.v[p][k]).y));
   h.zero();
 
   int64_t lo, hi;                                 // rows that count
@@ -415,7 +429,7 @@ template <bool REV> __global__ void __launch_bounds__(128) k_scan_join(ScanArgs 
   const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x, size = (int64_t)a.D * a.N;
   if (i >= size) return;
   const int c = (int)(i / a.N);
-  const float A2 = a.A[i] * kLog2e;
+  const float A2 = scaled(a.A[i]);
   constexpr int kAhead = 32;
   const int n = a.nc - 1;
   float x = 0.f;
@@ -470,7 +484,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_s
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], both(kLog2e));
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = pack(scaled(unpack(A2.v[p][k]).x), scaled(unpack(A2.v[p][k]).y));
   r.zero();
   const int s = owner(a.st, c0);
   const bool in = s >= 0 && s < a.st.seqs && a.st[s] < c0;      // a sequence comes in
@@ -580,7 +594,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
 #pragma unroll
   for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) A2.v[p][k] = mul2(A2.v[p][k], both(kLog2e));
+    for (int k = 0; k < 4; ++k) A2.v[p][k] = pack(scaled(unpack(A2.v[p][k]).x), scaled(unpack(A2.v[p][k]).y));
   dA.zero();
   r.zero();
   {

@@ -819,7 +819,8 @@ def short_conv_step(x, state, w, bias=None, index=None, act="silu"):
     None: row r is node r), whose last K - 1 are state [nodes, K - 1, D] (x's
     type, updated in place).  Returns y [n, D].  Rows of one node take their
     turns in the rows' order.  A negative index holds its row out (y 0, no state
-    touched); one >= nodes gives a row of NaN and touches no state."""
+    touched); one >= nodes gives a row of NaN and touches no state.  At most
+    65,536 rows with an index."""
     return _head_call(history_ops.short_conv_step,
                       lambda: (x.element_size() * x.numel() * 2 * w.shape[1], 2 * w.numel() * x.shape[0]), x, state, w, bias,
                       index, _conv_act(act))

@@ -750,7 +750,8 @@ int fb_selective_scan_bwd(const fb_selective_scan *args, void *ws, size_t ws_byt
 /* Single events against per-node tables, in place: row r works on state
  * index[r] (index NULL: state r; n <= states).  Rows of one node take their
  * turns in the rows' order.  A negative index holds its row out: y 0, no state
- * touched; one >= states gives a row of NaN and touches none.
+ * touched; one >= states gives a row of NaN and touches none.  n <= 65,536 with
+ * an index.
  * Convolution: state [states, K - 1, D] of the rows' type holds a node's last
  * K - 1 inputs, oldest first.  ws: fb_event_step_ws_bytes(n) bytes, 16-byte
  * aligned (both entries). */

