@@ -10,12 +10,13 @@
 // state in registers, the others do nothing.  Which row is first and which comes
 // next is looked up by comparing indices: by the warps themselves in calls of few
 // rows, in calls of many by k_links before (a lane a row, the other indices from
-// shared memory).
+// shared memory, four a branch: 4.5 us for 4,000 rows, 7.4 with one a branch).
 // Warps stay on their columns and take rows one after the other, so that weights
 // stay in registers; the convolution loads two nodes' windows at once.  (States
 // copied two nodes ahead by asynchronous copies, or two or four nodes' loaded at
-// once, were no faster: 4,000 events of width 200, 46 to 55 us against 45, the
-// state's 115 MB from memory.)
+// once, were no faster: 4,000 events of width 200, 46 to 55 us against 45 with
+// the indices' comparison of then, 40 with today's; the states are 102 MB from and
+// to memory.)
 #include <algorithm>
 #include "head.cuh"
 #include "history.cuh"
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(1024) k_links(const int64_t *index, int rows, 
     const int64_t i = j < rows ? index[j] : -1;
     return i >= 0 && i < states ? (int)i : -1;
   };
-  const int me = r < rows ? id(r) : -1;
+  const int mine = r < rows ? id(r) : -1, me = mine < 0 ? -2 : mine;       // -2: meets nothing
   int next = INT32_MAX, before = 0;
   for (int base = 0; base < rows; base += kPart) {
     if (base) __syncthreads();
@@ -85,14 +86,15 @@ __global__ void __launch_bounds__(1024) k_links(const int64_t *index, int rows, 
 #pragma unroll 4
     for (int i = from; i < end; i += 4) {
       const int4 v = *reinterpret_cast<const int4 *>(&some[i]);
-      const int o[4] = {v.x, v.y, v.z, v.w};
+      if (v.x == me || v.y == me || v.z == me || v.w == me) {     // seldom
+        const int o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (o[k] == me) {
+        for (int k = 0; k < 4; ++k) {
           const int j = base + i + k;
-          if (j < r) before = 1;
-          else if (j > r) next = min(next, j);
+          if (o[k] == me && j < r) before = 1;
+          if (o[k] == me && j > r) next = min(next, j);
         }
+      }
     }
   }
   found[lane][warp] = make_int2(next, before);
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(1024) k_links(const int64_t *index, int rows, 
 template <int V, int KT> __device__ __forceinline__ void taps(const float *w, int K, bool wide, float (&out)[KT][V]) {
   constexpr int N = V * KT, A = N % 4 == 0 ? 4 : (N % 2 == 0 ? 2 : 1);
   if (KT < 8 && wide) {
-    float flat[N];
+    alignas(16) float flat[N];
 #pragma unroll
     for (int i = 0; i < N; i += A) *reinterpret_cast<Vec<float, A> *>(&flat[i]) = *reinterpret_cast<const Vec<float, A> *>(w + i);
 #pragma unroll
