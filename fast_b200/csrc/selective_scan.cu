@@ -60,7 +60,11 @@ using namespace fbq;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kMaxStates = 64;
 constexpr int kHalf = kTile / 2;          // rows whose states the backward holds at once
-constexpr int kBwdCtas = 3;               // CTAs an SM its registers allow
+// CTAs an SM that the registers are shared among.  A fourth in the forward takes
+// what keeps a row's instructions apart: both passes of 12,000 x 200 fp32 224 us,
+// 242 with four, of 5,003 x 413 162 and 177, of 16,384 x 1,024 bf16 825 and 821; five
+// and six spill (957, 1,094).
+constexpr int kFwdCtas = 3, kBwdCtas = 3;
 constexpr int kKept = 1;                  // pairs of a thread whose decays it holds, too
 
 // exp(dt A) of a pair, A2 = A log2(e).  The exponential unit's results are low by
@@ -234,7 +238,7 @@ __device__ __forceinline__ int rows_in(int64_t v) { return (int)max((int64_t)0, 
 
 // Forward.  LOCAL: the chunk's last state alone, from the last beginning of a
 // sequence on, for all chunks but the last.
-template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThreads, 4) k_scan_fwd(ScanArgs a) {
+template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThreads, kFwdCtas) k_scan_fwd(ScanArgs a) {
   using L = Lay<NP, 2>;
   using X = typename L::X;
   using S = typename L::S;
@@ -459,7 +463,7 @@ template <int NP> struct RevSmem {
 
 // What chunk c (all but the first) sends up to the chunk in front of it: r in
 // front of its first row, from the rows of the sequence that comes in.
-template <typename T, int NP> __global__ void __launch_bounds__(kThreads, 4) k_scan_rev(ScanArgs a) {
+template <typename T, int NP> __global__ void __launch_bounds__(kThreads, kFwdCtas) k_scan_rev(ScanArgs a) {
   using L = Lay<NP, 2>;
   using X = typename L::X;
   using S = typename L::S;
@@ -988,7 +992,7 @@ constexpr int64_t kSms = 148;
 int plan_fwd(ScanArgs &a, int np, fbh::Call &c) {
   const int ch = 2 * 2 * 32 / (np / 4);
   a.tiles = (a.per + ch - 1) / ch;
-  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * 16, 2, 48);
+  a.chunk = chunk_rows(a.st.rows, (int64_t)a.G * a.tiles, kSms * kFwdCtas * kWarps, 2, 48);
   a.nc = (int)std::max<int64_t>(1, (a.st.rows + a.chunk - 1) / a.chunk);
   if (a.nc > 1) {
     FBH_TAKE(edge, c, float, (a.nc - 1) * (int64_t)a.D * a.N);
