@@ -59,15 +59,19 @@ __device__ __forceinline__ int owner(const Starts &st, int64_t row) {
 constexpr int kTile = 8;
 struct Walk {
   int next;                  // first entry of starts that may lie behind the current tile's first row
+  int base;                  // the lanes' entries of the last tile: starts[base + lane]
+  int64_t entry;
+  bool all;                  // they are all of the tile's
   __device__ __forceinline__ void begin(const Starts &st, int64_t row) { next = owner(st, row - 1) + 1; }
   // Bit i: row r0 + i begins a sequence (or is the first behind the last one).
   __device__ __forceinline__ unsigned tile(const Starts &st, int64_t r0) {
     unsigned bits = 0;
     const int lane = threadIdx.x & 31;
     if (!st.p) return (r0 == 0 ? 1u : 0u) | (st.rows >= r0 && st.rows < r0 + kTile ? 1u << (st.rows - r0) : 0u);
-    for (;;) {
+    for (all = true;; all = false) {
+      base = next;
       const int i = next + lane;
-      const int64_t b = i <= st.seqs ? st[i] : INT64_MAX;
+      const int64_t b = entry = i <= st.seqs ? st[i] : INT64_MAX;
       const bool in = b < r0 + kTile;
       bits |= __reduce_or_sync(0xffffffffu, in && b >= r0 ? 1u << (int)(b - r0) : 0u);
       const int c = __popc(__ballot_sync(0xffffffffu, in));
@@ -75,26 +79,39 @@ struct Walk {
       if (c < 32) return bits;
     }
   }
+  // owner() of a row of the tile or of the one in front of it, without a load where the lanes hold the tile's entries.
+  __device__ __forceinline__ int sequence(const Starts &st, int64_t row) const {
+    if (!st.p || !all) return owner(st, row);
+    return base + __popc(__ballot_sync(0xffffffffu, entry <= row)) - 1;
+  }
 };
 
 // The same, downwards: the first tile asked for holds row `top`, the next ones
 // lie 8 rows lower each.
 struct WalkDown {
   int next;                  // last entry of starts that may lie in the next tile
+  int base;                  // the lanes' entries of the last tile: starts[base - lane]
+  int64_t entry;
+  bool all;                  // they are all of the tile's
   __device__ __forceinline__ void begin(const Starts &st, int64_t top) { next = owner(st, top); }
   __device__ __forceinline__ unsigned tile(const Starts &st, int64_t r0) {
     if (!st.p) return r0 == 0 ? 1u : 0u;
     unsigned bits = 0;
     const int lane = threadIdx.x & 31;
-    for (;;) {
+    for (all = true;; all = false) {
+      base = next;
       const int i = next - lane;
-      const int64_t b = i >= 0 ? st[i] : -1;
+      const int64_t b = entry = i >= 0 ? st[i] : -1;
       const bool in = b >= r0;
       bits |= __reduce_or_sync(0xffffffffu, in && b < r0 + kTile ? 1u << (int)(b - r0) : 0u);
       const int c = __popc(__ballot_sync(0xffffffffu, in));
       next -= c;
       if (c < 32) return bits;
     }
+  }
+  __device__ __forceinline__ int sequence(const Starts &st, int64_t row) const {
+    if (!st.p || !all) return owner(st, row);
+    return base - __popc(__ballot_sync(0xffffffffu, entry > row));
   }
 };
 

@@ -369,12 +369,12 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
         if (begins >> i & 1u) {
           const int64_t at = r0 + i;
           if (a.fin && at > c0) {                 // the sequence in front leaves its last state
-            const int s = owner(a.st, at - 1);
+            const int s = walk.sequence(a.st, at - 1);
             if (s >= 0 && s < a.st.seqs) h.store(a.fin + (int64_t)s * size, mine, has, n0, a);
           }
           h.zero();
           if (a.init) {
-            const int s = owner(a.st, at);
+            const int s = walk.sequence(a.st, at);
             if (s >= 0 && s < a.st.seqs) h.load(a.init + (int64_t)s * size, mine, has, n0, a);
           }
         }
@@ -681,7 +681,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
     if (begins && (a.init || a.dfin || a.dinit)) {
 #pragma unroll 1
       for (int i = 0; i <= kTile; ++i) {
-        const int s = owner(a.st, c0 + t0 + i - 1);
+        const int s = walk.sequence(a.st, c0 + t0 + i - 1);
         if (lane == 0) sm.seq[warp][i] = s >= 0 && s < a.st.seqs ? s : -1;
       }
     }
