@@ -938,17 +938,16 @@ int padded(int N) { return N <= 8 ? 8 : (N <= 16 ? 16 : (N <= 32 ? 32 : 64)); }
 // 78, 111 us; both passes of 5,003 x 413 171, 178, 188, 201, of 12,000 x 200 fp32
 // 243, 243, 239, 242; backward of the latter two with 32, 64, 96 rows 260, 243,
 // 246 and 170, 171, 190.
+// Where one wave is not filled, a row's latency counts, not the instructions:
+// chunks of down to kLeast rows.
+constexpr int64_t kLeast = 24;
 int64_t chunk_rows(int64_t rows, int64_t tiles, int64_t resident, int64_t waves, int64_t shortest) {
-  int64_t c = shortest;
-  for (; waves; --waves) {
+  for (;; --waves) {
     const int64_t want = std::max<int64_t>(1, resident * waves / tiles);
     const int64_t even = ((rows + want - 1) / want + kTile - 1) / kTile * kTile;
-    if (even >= shortest) {
-      c = even;
-      break;
-    }
+    if (even >= shortest) return even;
+    if (waves == 1) return std::max(even, kLeast);
   }
-  return c;
 }
 
 int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
