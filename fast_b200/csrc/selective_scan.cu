@@ -935,12 +935,12 @@ int padded(int N) { return N <= 8 ? 8 : (N <= 16 ? 16 : (N <= 32 ? 32 : 64)); }
 // backward in one wave 922 us, two 881, three 866; forward in three 845, two
 // 834.  Shorter chunks lose more to the passes between them than they gain:
 // forward of 2,048 x 2,048 with chunks of at least 32, 48, 64, 96 rows 76, 73,
-// 78, 111 us; both passes of 5,003 x 413 171, 178, 188, 201, of 12,000 x 200 fp32
-// 243, 243, 239, 242; backward of the latter two with 32, 64, 96 rows 260, 243,
-// 246 and 170, 171, 190.
+// 78, 111 us; both passes of 12,000 x 200 fp32 243, 243, 239, 242, with 32, 64, 96
+// rows in the backward 260, 243, 246.
 // Where one wave is not filled, a row's latency counts, not the instructions:
-// chunks of down to kLeast rows.
-constexpr int64_t kLeast = 24;
+// chunks of down to kLeast rows (35 scans of sizes drawn from the whole range:
+// 50.7 us in the geometric mean with 32, 47.8 with 24, 44.9 with 16).
+constexpr int64_t kLeast = 16;
 int64_t chunk_rows(int64_t rows, int64_t tiles, int64_t resident, int64_t waves, int64_t shortest) {
   for (;; --waves) {
     const int64_t want = std::max<int64_t>(1, resident * waves / tiles);
