@@ -157,11 +157,13 @@ class StateSpaceBlock(torch.nn.Module):
         behind the block and what each history leaves, which a call for the rows
         to come takes as `conv` and `scan`.  In training, dropout draws from
         (seed, offset)."""
+        return self._run(x, starts, conv, scan, self.dropout if self.training else 0.0, seed, offset)
+
+    def _run(self, x, starts, conv, scan, p, seed=0, offset=0):
         v, z = self._inner(x)
         u, conv = ShortConvFunction.apply(v, self.w_conv.float(), self.b_conv.float(), starts, conv, "silu")
         delta, A, b, c = self._scan_inputs(u)
         s, scan = SelectiveScanFunction.apply(u, delta, A, b, c, self.skip.float(), z, self.b_dt.float(), starts, scan, True)
-        p = self.dropout if self.training else 0.0
         return DropoutFunction.apply(self._product(s, self.w_out), x, p, seed, offset), conv, scan
 
     @torch.no_grad()
@@ -204,10 +206,12 @@ class HistoryEncoder(torch.nn.Module):
     @torch.no_grad()
     def follow(self, x, starts, tables, index):
         """Encodes packed histories that continue those of nodes index [seqs]
-        (each node once; int64), whose states in `tables` are read and replaced."""
+        (each node once; int64, 0 .. nodes - 1), whose states in `tables` are read
+        and replaced.  As in step nothing drops out, in training mode either: the
+        tables outlive the call."""
         x = x.to(self.dtype)
         for b, conv, scan in zip(self.blocks, tables.conv, tables.scan):
-            x, c, s = b(x, starts, conv[index], scan[index])
+            x, c, s = b._run(x, starts, conv[index], scan[index], 0.0)
             conv[index], scan[index] = c, s
         return x
 

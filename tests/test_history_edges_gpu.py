@@ -1,0 +1,35 @@
+"""GPU: event histories at the edges of what the calls document -- dropout and
+training mode, what is kept, gates and decays of extreme values, tables of no
+node, and the kernels that only large calls reach."""
+import pytest
+import torch
+from test_history_gpu import BF, F32
+
+pytestmark = pytest.mark.gpu
+
+
+def _encoder(dim=32, blocks=2, dropout=0.5, dtype=F32):
+    from fast_b200.history import HistoryEncoder
+    torch.manual_seed(0)
+    return HistoryEncoder(dim, blocks, dropout=dropout, dtype=dtype).cuda()
+
+
+def _histories(dim=32, seed=1):
+    x = torch.randn(48, dim, generator=torch.Generator().manual_seed(seed)).cuda()
+    return x, torch.tensor([0, 12, 12, 17, 48], device="cuda"), torch.tensor([6, 2, 0, 3], device="cuda")
+
+
+# ---- modules -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_following_the_stream_drops_nothing_out(cuda, dtype):
+    """follow writes tables that step goes on from: in training mode, too, it computes what it computes in eval mode."""
+    from fast_b200.history import NodeStates
+    enc = _encoder(dtype=dtype)
+    x, starts, nodes = _histories()
+    tables = [NodeStates(enc, 8, cuda) for _ in range(2)]
+    want = enc.eval().follow(x, starts, tables[0], nodes)
+    got = enc.train().follow(x, starts, tables[1], nodes)
+    assert torch.equal(got, want)
+    for a, b in zip(tables[0].conv + tables[0].scan, tables[1].conv + tables[1].scan):
+        assert torch.equal(a, b)
+    assert torch.equal(enc.step(x[:4], tables[0], nodes), enc.step(x[:4], tables[1], nodes))
