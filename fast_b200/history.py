@@ -201,7 +201,7 @@ class HistoryEncoder(torch.nn.Module):
         if not rows.shape[0]:
             return rows.new_zeros(starts.shape[0] - 1, rows.shape[1])
         some = starts[1:] > starts[:-1]
-        return rows[(starts[1:] - 1).clamp(min=0)] * some.unsqueeze(1).to(rows.dtype)
+        return torch.where(some.unsqueeze(1), rows[(starts[1:] - 1).clamp(min=0)], rows.new_zeros(()))
 
     @torch.no_grad()
     def follow(self, x, starts, tables, index):
