@@ -200,6 +200,7 @@ class HistoryEncoder(torch.nn.Module):
         """The last row of each history [seqs, dim]; zeros for an empty one."""
         if not rows.shape[0]:
             return rows.new_zeros(starts.shape[0] - 1, rows.shape[1])
+        starts = starts.clamp(0, rows.shape[0])                      # as the operators do
         some = starts[1:] > starts[:-1]
         return torch.where(some.unsqueeze(1), rows[(starts[1:] - 1).clamp(min=0)], rows.new_zeros(()))
 

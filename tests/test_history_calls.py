@@ -13,3 +13,11 @@ def test_last_row_of_an_empty_history_is_zero_whatever_its_neighbours_hold():
     # an empty history hands no gradient to the row in front of it
     grad, = torch.autograd.grad(out[[0, 2, 4]].sum() + out[3].sum(), rows)
     assert torch.equal(grad, torch.tensor([[0.0, 0.0], [0.0, 0.0], [0.0, 0.0], [1.0, 1.0]]))
+
+
+def test_last_rows_stay_inside_the_rows():
+    """starts beyond the rows are clamped to them, as the operators do, and not left to an index out of range."""
+    from fast_b200.history import HistoryEncoder
+    rows = torch.arange(8.0).view(4, 2)
+    assert torch.equal(HistoryEncoder.last(rows, torch.tensor([0, 2, 9, 9, 12])), torch.stack([rows[1], rows[3], *torch.zeros(2, 2)]))
+    assert torch.equal(HistoryEncoder.last(rows, torch.tensor([-3, -1, 4])), torch.stack([torch.zeros(2), rows[3]]))
