@@ -57,16 +57,18 @@ class ShortConvFunction(torch.autograd.Function):
 
 
 class SelectiveScanFunction(torch.autograd.Function):
-    """(y, final) of packed rows u, delta, z [rows, D]; A [D, N], D, delta_bias [D], init [seqs, D, N] in fp32."""
+    """(y, final) of packed rows u, delta, z [rows, D]; A [D, N], D, delta_bias [D], init [seqs, D, N] in fp32.
+    `graph`: whether the caller records one (torch.is_grad_enabled(), which a
+    function's forward cannot see); without, nothing is kept for a backward."""
 
     @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, starts, init, softplus):
+    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, starts, init, softplus, graph=True):
         u, delta = _rows(u), _rows(delta)
         B, C = (t if t.stride(-1) == 1 else t.contiguous() for t in (B, C))
         z = None if z is None else _rows(z)
         A, D, delta_bias, init = (None if t is None else t.contiguous() for t in (A, D, delta_bias, init))
         y, carry, final = ops.selective_scan_fwd(u, delta, A, B, C, D, z, delta_bias, starts, init, softplus, final=True,
-                                                 keep=any(ctx.needs_input_grad))
+                                                 keep=graph and any(ctx.needs_input_grad))
         ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, starts, init, carry)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
@@ -77,12 +79,12 @@ class SelectiveScanFunction(torch.autograd.Function):
     def backward(ctx, dy, dfinal):
         u, delta, A, B, C, D, z, delta_bias, starts, init, carry = ctx.saved_tensors
         if dy is None and dfinal is None:
-            return (None,) * 11
+            return (None,) * 12
         dy = torch.zeros_like(u) if dy is None else _rows(dy)
         du, dd, dA, dB, dC, dD, dz, db, dinit = ops.selective_scan_bwd(
             dy, u, delta, A, B, C, carry, D, z, delta_bias, starts, init, ctx.softplus,
             None if dfinal is None else dfinal.contiguous())
-        return du, dd, dA, dB, dC, dD, dz, db, None, dinit, None
+        return du, dd, dA, dB, dC, dD, dz, db, None, dinit, None, None
 
 
 class DropoutFunction(torch.autograd.Function):
@@ -163,7 +165,8 @@ class StateSpaceBlock(torch.nn.Module):
         v, z = self._inner(x)
         u, conv = ShortConvFunction.apply(v, self.w_conv.float(), self.b_conv.float(), starts, conv, "silu")
         delta, A, b, c = self._scan_inputs(u)
-        s, scan = SelectiveScanFunction.apply(u, delta, A, b, c, self.skip.float(), z, self.b_dt.float(), starts, scan, True)
+        s, scan = SelectiveScanFunction.apply(u, delta, A, b, c, self.skip.float(), z, self.b_dt.float(), starts, scan, True,
+                                              torch.is_grad_enabled())
         return DropoutFunction.apply(self._product(s, self.w_out), x, p, seed, offset), conv, scan
 
     @torch.no_grad()

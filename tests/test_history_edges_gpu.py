@@ -33,3 +33,36 @@ def test_following_the_stream_drops_nothing_out(cuda, dtype):
     for a, b in zip(tables[0].conv + tables[0].scan, tables[1].conv + tables[1].scan):
         assert torch.equal(a, b)
     assert torch.equal(enc.step(x[:4], tables[0], nodes), enc.step(x[:4], tables[1], nodes))
+
+
+def _recorded(monkeypatch, name, argument):
+    """Values of an argument of ops.`name` from here on."""
+    import inspect
+    from fast_b200 import ops
+    call, seen = getattr(ops, name), []
+    signature = inspect.signature(call)
+
+    def run(*args, **kw):
+        bound = signature.bind(*args, **kw)
+        bound.apply_defaults()
+        seen.append(bound.arguments[argument])
+        return call(*args, **kw)
+    monkeypatch.setattr(ops, name, run)
+    return seen
+
+
+def test_states_are_kept_for_a_backward_pass_only(cuda, monkeypatch):
+    """Parameters require gradients under no_grad, too; the states in front of every 8th row are written only where
+    there is a graph."""
+    from fast_b200.history import NodeStates
+    enc, (x, starts, nodes) = _encoder(), _histories()
+    kept = _recorded(monkeypatch, "selective_scan_fwd", "keep")
+    with torch.no_grad():
+        enc(x, starts)
+    enc.follow(x, starts, NodeStates(enc, 8, cuda), nodes)
+    with torch.inference_mode():
+        enc(x, starts)
+    assert kept == [False] * 6
+    del kept[:]
+    enc(x, starts)
+    assert kept == [True] * 2
