@@ -33,58 +33,61 @@ from .ranking import LayerNormFunction, _rows
 
 
 class ShortConvFunction(torch.autograd.Function):
-    """(y, final) of packed rows x [rows, D]; w [D, K] and bias [D] in fp32."""
+    """(y, final) of packed rows x [rows, D]; w [D, K] and bias [D] in fp32.
+    Without `final` only y is computed, None comes in the states' place."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, starts, init, act):
+    def forward(ctx, x, w, bias, starts, init, act, final=True):
         x, w = _rows(x), w.contiguous()
         bias, init = (None if t is None else t.contiguous() for t in (bias, init))
         ctx.save_for_backward(x, w, bias, starts, init)
         ctx.act = act
         ctx.set_materialize_grads(False)
-        return ops.short_conv_fwd(x, w, bias, starts, init, act, final=True)
+        out = ops.short_conv_fwd(x, w, bias, starts, init, act, final=final)
+        return out if final else (out, None)
 
     @staticmethod
     @first_order
     def backward(ctx, dy, dfinal):
         x, w, bias, starts, init = ctx.saved_tensors
         if dy is None and dfinal is None:
-            return (None,) * 6
+            return (None,) * 7
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
         dx, dw, dbias, dinit = ops.short_conv_bwd(dy, x, w, bias, starts, init, ctx.act,
                                                   None if dfinal is None else dfinal.contiguous())
-        return dx, dw, dbias, None, dinit, None
+        return dx, dw, dbias, None, dinit, None, None
 
 
 class SelectiveScanFunction(torch.autograd.Function):
     """(y, final) of packed rows u, delta, z [rows, D]; A [D, N], D, delta_bias [D], init [seqs, D, N] in fp32.
     `graph`: whether the caller records one (torch.is_grad_enabled(), which a
-    function's forward cannot see); without, nothing is kept for a backward."""
+    function's forward cannot see); without, nothing is kept for a backward.
+    `final` as in ShortConvFunction."""
 
     @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, starts, init, softplus, graph=True):
+    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, starts, init, softplus, graph=True, final=True):
         u, delta = _rows(u), _rows(delta)
         B, C = (t if t.stride(-1) == 1 else t.contiguous() for t in (B, C))
         z = None if z is None else _rows(z)
         A, D, delta_bias, init = (None if t is None else t.contiguous() for t in (A, D, delta_bias, init))
-        y, carry, final = ops.selective_scan_fwd(u, delta, A, B, C, D, z, delta_bias, starts, init, softplus, final=True,
-                                                 keep=graph and any(ctx.needs_input_grad))
+        y, carry, behind = ops.selective_scan_fwd(u, delta, A, B, C, D, z, delta_bias, starts, init, softplus, final=final,
+                                                  keep=graph and any(ctx.needs_input_grad))
         ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, starts, init, carry)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
-        return y, final
+        return y, behind
 
     @staticmethod
     @first_order
     def backward(ctx, dy, dfinal):
         u, delta, A, B, C, D, z, delta_bias, starts, init, carry = ctx.saved_tensors
         if dy is None and dfinal is None:
-            return (None,) * 12
+            return (None,) * 13
         dy = torch.zeros_like(u) if dy is None else _rows(dy)
         du, dd, dA, dB, dC, dD, dz, db, dinit = ops.selective_scan_bwd(
             dy, u, delta, A, B, C, carry, D, z, delta_bias, starts, init, ctx.softplus,
             None if dfinal is None else dfinal.contiguous())
-        return du, dd, dA, dB, dC, dD, dz, db, None, dinit, None, None
+        return du, dd, dA, dB, dC, dD, dz, db, None, dinit, None, None, None
 
 
 class DropoutFunction(torch.autograd.Function):
@@ -154,19 +157,19 @@ class StateSpaceBlock(torch.nn.Module):
         d, b, c = self._product(u, self.w_x).split([self.rank, self.states, self.states], dim=1)
         return self._product(d, self.w_dt), -torch.exp(self.log_decay.float()), b, c
 
-    def forward(self, x, starts=None, conv=None, scan=None, seed=0, offset=0):
+    def forward(self, x, starts=None, conv=None, scan=None, seed=0, offset=0, states=True):
         """Rows x [rows, dim] of packed histories -> (x', conv, scan): the rows
         behind the block and what each history leaves, which a call for the rows
-        to come takes as `conv` and `scan`.  In training, dropout draws from
-        (seed, offset)."""
-        return self._run(x, starts, conv, scan, self.dropout if self.training else 0.0, seed, offset)
+        to come takes as `conv` and `scan` (None without `states`).  In training,
+        dropout draws from (seed, offset)."""
+        return self._run(x, starts, conv, scan, self.dropout if self.training else 0.0, seed, offset, states)
 
-    def _run(self, x, starts, conv, scan, p, seed=0, offset=0):
+    def _run(self, x, starts, conv, scan, p, seed=0, offset=0, states=True):
         v, z = self._inner(x)
-        u, conv = ShortConvFunction.apply(v, self.w_conv.float(), self.b_conv.float(), starts, conv, "silu")
+        u, conv = ShortConvFunction.apply(v, self.w_conv.float(), self.b_conv.float(), starts, conv, "silu", states)
         delta, A, b, c = self._scan_inputs(u)
         s, scan = SelectiveScanFunction.apply(u, delta, A, b, c, self.skip.float(), z, self.b_dt.float(), starts, scan, True,
-                                              torch.is_grad_enabled())
+                                              torch.is_grad_enabled(), states)
         return DropoutFunction.apply(self._product(s, self.w_out), x, p, seed, offset), conv, scan
 
     @torch.no_grad()
@@ -195,7 +198,7 @@ class HistoryEncoder(torch.nn.Module):
         went in.  Block i draws its dropout from (seed + i, offset)."""
         x = x.to(self.dtype)
         for i, b in enumerate(self.blocks):
-            x = b(x, starts, seed=seed + i, offset=offset)[0]
+            x = b(x, starts, seed=seed + i, offset=offset, states=False)[0]
         return x
 
     @staticmethod

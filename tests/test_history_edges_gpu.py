@@ -66,3 +66,21 @@ def test_states_are_kept_for_a_backward_pass_only(cuda, monkeypatch):
     del kept[:]
     enc(x, starts)
     assert kept == [True] * 2
+
+
+def test_states_behind_histories_are_computed_where_they_are_asked_for(cuda, monkeypatch):
+    from fast_b200.history import NodeStates
+    enc, (x, starts, nodes) = _encoder(), _histories()
+    asked = [_recorded(monkeypatch, n, "final") for n in ("short_conv_fwd", "selective_scan_fwd")]
+    enc(x, starts)
+    assert asked == [[False] * 2] * 2
+    enc.follow(x, starts, NodeStates(enc, 8, cuda), nodes)
+    assert asked == [[False] * 2 + [True] * 2] * 2
+    y, conv, scan = enc.blocks[0](x, starts, states=False)
+    assert conv is None and scan is None
+    again, conv, scan = enc.blocks[0](x, starts)
+    assert torch.equal(y, again) and conv.shape == (4, 3, 64) and scan.shape == (4, 64, 16)
+    # the gradients are those of a call that asks for the states
+    a = torch.autograd.grad(y.square().sum(), list(enc.blocks[0].parameters()))
+    b = torch.autograd.grad(again.square().sum(), list(enc.blocks[0].parameters()))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
