@@ -92,18 +92,22 @@ class SelectiveScanFunction(torch.autograd.Function):
 
 class DropoutFunction(torch.autograd.Function):
     """res + dropout(x) (res None: dropout(x)) of rows, from (seed, offset); the
-    mask is drawn again in the backward."""
+    mask is drawn again in the backward.  offset_dev: a device int64 [1] added to
+    the offset, which must keep its value until the backward (autograd refuses one
+    that was changed)."""
 
     @staticmethod
-    def forward(ctx, x, res, p, seed, offset):
+    def forward(ctx, x, res, p, seed, offset, offset_dev=None):
         ctx.how = p, seed, offset
         ctx.has_res = res is not None
-        return ops.dropout_fwd(_rows(x), p, seed, offset, None if res is None else _rows(res))
+        ctx.save_for_backward(offset_dev)
+        return ops.dropout_fwd(_rows(x), p, seed, offset, None if res is None else _rows(res), offset_dev)
 
     @staticmethod
     @first_order
     def backward(ctx, dy):
-        return ops.dropout_bwd(_rows(dy), *ctx.how), dy if ctx.has_res else None, None, None, None
+        offset_dev, = ctx.saved_tensors
+        return ops.dropout_bwd(_rows(dy), *ctx.how, offset_dev), dy if ctx.has_res else None, None, None, None, None
 
 
 class NodeStates:
@@ -157,20 +161,21 @@ class StateSpaceBlock(torch.nn.Module):
         d, b, c = self._product(u, self.w_x).split([self.rank, self.states, self.states], dim=1)
         return self._product(d, self.w_dt), -torch.exp(self.log_decay.float()), b, c
 
-    def forward(self, x, starts=None, conv=None, scan=None, seed=0, offset=0, states=True):
+    def forward(self, x, starts=None, conv=None, scan=None, seed=0, offset=0, states=True, offset_dev=None):
         """Rows x [rows, dim] of packed histories -> (x', conv, scan): the rows
         behind the block and what each history leaves, which a call for the rows
         to come takes as `conv` and `scan` (None without `states`).  In training,
-        dropout draws from (seed, offset)."""
-        return self._run(x, starts, conv, scan, self.dropout if self.training else 0.0, seed, offset, states)
+        dropout draws from (seed, offset + offset_dev), the latter a device int64
+        [1] for graphs whose replays draw anew."""
+        return self._run(x, starts, conv, scan, self.dropout if self.training else 0.0, seed, offset, states, offset_dev)
 
-    def _run(self, x, starts, conv, scan, p, seed=0, offset=0, states=True):
+    def _run(self, x, starts, conv, scan, p, seed=0, offset=0, states=True, offset_dev=None):
         v, z = self._inner(x)
         u, conv = ShortConvFunction.apply(v, self.w_conv.float(), self.b_conv.float(), starts, conv, "silu", states)
         delta, A, b, c = self._scan_inputs(u)
         s, scan = SelectiveScanFunction.apply(u, delta, A, b, c, self.skip.float(), z, self.b_dt.float(), starts, scan, True,
                                               torch.is_grad_enabled(), states)
-        return DropoutFunction.apply(self._product(s, self.w_out), x, p, seed, offset), conv, scan
+        return DropoutFunction.apply(self._product(s, self.w_out), x, p, seed, offset, offset_dev), conv, scan
 
     @torch.no_grad()
     def step(self, x, conv, scan, index=None):
@@ -193,12 +198,14 @@ class HistoryEncoder(torch.nn.Module):
         self.dtype = dtype
         self.blocks = torch.nn.ModuleList(StateSpaceBlock(dim, inner, states, taps, None, dropout, dtype) for _ in range(blocks))
 
-    def forward(self, x, starts=None, seed=0, offset=0):
+    def forward(self, x, starts=None, seed=0, offset=0, offset_dev=None):
         """Rows [rows, dim] -> encoded rows.  Rows of no history come out as they
-        went in.  Block i draws its dropout from (seed + i, offset)."""
+        went in.  Block i draws its dropout from (seed + i, offset + offset_dev);
+        a captured training step advances the counter offset_dev (device int64
+        [1]) behind its backward, so that every replay draws anew."""
         x = x.to(self.dtype)
         for i, b in enumerate(self.blocks):
-            x = b(x, starts, seed=seed + i, offset=offset, states=False)[0]
+            x = b(x, starts, seed=seed + i, offset=offset, states=False, offset_dev=offset_dev)[0]
         return x
 
     @staticmethod

@@ -84,3 +84,43 @@ def test_states_behind_histories_are_computed_where_they_are_asked_for(cuda, mon
     a = torch.autograd.grad(y.square().sum(), list(enc.blocks[0].parameters()))
     b = torch.autograd.grad(again.square().sum(), list(enc.blocks[0].parameters()))
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_captured_training_draws_anew(cuda):
+    """A device counter added to the dropout's offset: a graph of a training step replays with the masks of its value, forward
+    and backward."""
+    enc = _encoder(dropout=0.4).train()
+    x, starts, _ = _histories()
+    params = list(enc.parameters())
+    count = torch.zeros(1, dtype=torch.int64, device=cuda)
+
+    def step(offset, counter):
+        y = enc(x, starts, seed=5, offset=offset, offset_dev=counter)
+        return [y, *torch.autograd.grad(y.square().sum(), params)]
+    want = [[t.detach().clone() for t in step(k, None)] for k in range(3)]
+    assert not torch.equal(want[0][0], want[1][0])
+    count.fill_(2)
+    assert all(torch.equal(a, b) for a, b in zip(step(0, count), want[2]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(0, count)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(0, count)
+    for k in (1, 0, 2):
+        count.fill_(k)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
+
+
+def test_a_counter_that_moves_before_the_backward_is_refused(cuda):
+    """The backward draws the forward's words again: a counter advanced in between would give it others."""
+    from fast_b200.history import DropoutFunction
+    x, count = torch.ones(9, 8, device=cuda, requires_grad=True), torch.zeros(1, dtype=torch.int64, device=cuda)
+    y = DropoutFunction.apply(x, None, 0.5, 1, 0, count)
+    count += 1
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
