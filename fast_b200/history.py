@@ -107,7 +107,8 @@ class DropoutFunction(torch.autograd.Function):
     @first_order
     def backward(ctx, dy):
         offset_dev, = ctx.saved_tensors
-        return ops.dropout_bwd(_rows(dy), *ctx.how, offset_dev), dy if ctx.has_res else None, None, None, None, None
+        dx = ops.dropout_bwd(_rows(dy), *ctx.how, offset_dev) if ctx.how[0] else dy      # p = 0 keeps all, unscaled
+        return dx, dy if ctx.has_res else None, None, None, None, None
 
 
 class NodeStates:

@@ -124,3 +124,15 @@ def test_a_counter_that_moves_before_the_backward_is_refused(cuda):
     count += 1
     with pytest.raises(RuntimeError):
         y.sum().backward()
+
+
+def test_no_dropout_hands_the_gradient_on(cuda):
+    from fast_b200 import ops
+    from fast_b200.history import DropoutFunction
+    x, res = (torch.randn(9, 8, device=cuda, requires_grad=True) for _ in range(2))
+    y = DropoutFunction.apply(x, res, 0.0, 1, 0)
+    dy = torch.randn(9, 8, device=cuda)
+    before = ops.LAUNCHES[0]
+    gx, gr = torch.autograd.grad(y, (x, res), dy)
+    assert ops.LAUNCHES[0] == before
+    assert torch.equal(gx, dy) and torch.equal(gr, dy)
