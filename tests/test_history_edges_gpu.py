@@ -136,3 +136,13 @@ def test_no_dropout_hands_the_gradient_on(cuda):
     gx, gr = torch.autograd.grad(y, (x, res), dy)
     assert ops.LAUNCHES[0] == before
     assert torch.equal(gx, dy) and torch.equal(gr, dy)
+
+
+def test_seeds_up_to_64_bits(cuda):
+    """Block i draws from seed + i, counted in 64 bits."""
+    enc = _encoder().train()
+    x, starts, _ = _histories()
+    with torch.no_grad():
+        y = enc.blocks[0](x, starts, seed=(1 << 64) - 1, offset=3)[0]
+        want = enc.blocks[1](y, starts, seed=0, offset=3)[0]
+        assert torch.equal(enc(x, starts, seed=(1 << 64) - 1, offset=3), want)
