@@ -202,11 +202,12 @@ class HistoryEncoder(torch.nn.Module):
     def forward(self, x, starts=None, seed=0, offset=0, offset_dev=None):
         """Rows [rows, dim] -> encoded rows.  Rows of no history come out as they
         went in.  Block i draws its dropout from (seed + i, offset + offset_dev),
-        counted in 64 bits; a captured training step advances the counter offset_dev (device int64
-        [1]) behind its backward, so that every replay draws anew."""
+        counted in 64 bits; a captured training step advances the counter
+        offset_dev (device int64 [1]) behind its backward, so that every replay
+        draws anew."""
         x = x.to(self.dtype)
         for i, b in enumerate(self.blocks):
-            x = b(x, starts, seed=seed + i & 0xFFFFFFFFFFFFFFFF, offset=offset, states=False, offset_dev=offset_dev)[0]
+            x = b(x, starts, seed=(seed + i) % (1 << 64) if i else seed, offset=offset, states=False, offset_dev=offset_dev)[0]
         return x
 
     @staticmethod

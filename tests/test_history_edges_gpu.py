@@ -146,3 +146,12 @@ def test_seeds_up_to_64_bits(cuda):
         y = enc.blocks[0](x, starts, seed=(1 << 64) - 1, offset=3)[0]
         want = enc.blocks[1](y, starts, seed=0, offset=3)[0]
         assert torch.equal(enc(x, starts, seed=(1 << 64) - 1, offset=3), want)
+
+
+def test_seeds_beyond_64_bits_are_refused(cuda):
+    """The encoder's count past 2^64 does not make a bad seed a good one."""
+    enc = _encoder().train()
+    x, starts, _ = _histories()
+    for seed in (-1, 1 << 64, 1.0, True):
+        with pytest.raises(ValueError, match="seed"):
+            enc(x, starts, seed=seed)
