@@ -120,6 +120,7 @@ extern "C" int fb_dropout(int type, const void *x, int64_t ldx, const void *res,
   const int es = type == FB_F32 ? 4 : 2;
   const uint64_t at = (uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)y | (uint64_t)(uintptr_t)res;
   if (at % es) return bad("rows that are not aligned to their elements");
+  if (!aligned(8, offset_dev)) return bad("an offset that is not aligned to its element");
   uint64_t bits = at / es | (uint64_t)D;
   if (rows > 1) bits |= (uint64_t)ldx | (uint64_t)ldy | (res ? (uint64_t)ldr : 0);
   DropArgs a{};

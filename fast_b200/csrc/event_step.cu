@@ -450,6 +450,7 @@ extern "C" int fb_short_conv_step(int type, int act, const void *x, int64_t ldx,
   const int es = type == FB_F32 ? 4 : 2;
   const uint64_t at = (uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)y | (K > 1 ? (uint64_t)(uintptr_t)state : 0);
   if (at % es) return bad("rows that are not aligned to their elements");
+  if (!aligned(4, w, bias) || !aligned(8, index)) return bad("parameters or indices that are not aligned to their elements");
   FBH_TRY(rows_of("short_conv_step", n, states, index, ws, ws_bytes, stream, a.r));
   uint64_t bits = at / es | (uint64_t)D;
   if (n > 1) bits |= (uint64_t)ldx | (uint64_t)ldy;
@@ -468,14 +469,18 @@ extern "C" int fb_selective_scan_step(const fb_selective_scan_event *s, void *ws
   if (!s->A || (s->n && (!s->u || !s->delta || !s->B || !s->C || !s->state || !s->y))) return bad("missing operand");
   if (s->n > 1 && (s->ldu < s->D || s->ld_delta < s->D || s->ldy < s->D || (s->z && s->ldz < s->D)))
     return bad("leading dimension below the width");
+  if (s->ldb < 0 || s->ldb_group < 0 || s->ldc < 0 || s->ldc_group < 0) return bad("negative pitch");
   if (!s->n) return FB_OK;
+  const uintptr_t es = s->type == FB_F32 ? 4 : 2;
+  if (!aligned(es, s->u, s->delta, s->B, s->C, s->z, s->y)) return bad("rows that are not aligned to their elements");
+  if (!aligned(4, s->A, s->skip, s->delta_bias, s->state) || !aligned(8, s->index))
+    return bad("parameters, states or indices that are not aligned to their elements");
   ScanStep a{};
   a.D = s->D, a.N = s->N, a.per = s->D / s->G, a.softplus = s->softplus;
   a.vec = s->N % 4 == 0 && ((uintptr_t)s->state | (uintptr_t)s->A) % 16 == 0;
   a.u = s->u, a.ldu = s->ldu, a.delta = s->delta, a.ldd = s->ld_delta, a.B = s->B, a.ldb = s->ldb, a.gsb = s->ldb_group;
   a.C = s->C, a.ldc = s->ldc, a.gsc = s->ldc_group, a.z = s->z, a.ldz = s->ldz, a.y = s->y, a.ldy = s->ldy;
   a.A = s->A, a.Ds = s->skip, a.bias = s->delta_bias, a.state = s->state;
-  const uintptr_t es = s->type == FB_F32 ? 4 : 2;
   const uint64_t bc = (uint64_t)s->ldb | (uint64_t)s->ldb_group | (uint64_t)s->ldc | (uint64_t)s->ldc_group;
   a.vec_bc = s->N % 4 == 0 && bc % 4 == 0 && ((uintptr_t)s->B | (uintptr_t)s->C) % (4 * es) == 0;
   FBH_TRY(rows_of("selective_scan_step", s->n, s->states, s->index, ws, ws_bytes, stream, a.r));

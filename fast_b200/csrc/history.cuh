@@ -25,6 +25,9 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Vec {
   T e[V];
 };
 
+// Whether every pointer given (null: none) lies at a multiple of `bytes`, a power of two.
+template <typename... P> bool aligned(uintptr_t bytes, P... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0; }
+
 struct Starts {
   const void *p;             // null: one sequence over all rows
   int wide;                  // 64-bit entries

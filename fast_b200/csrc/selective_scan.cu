@@ -970,6 +970,15 @@ int fill(const fb_selective_scan *s, ScanArgs &a, bool backward) {
     if (s->rows && (!s->du || !s->ddelta || !s->dB || !s->dC || (s->z && !s->dz))) return bad("missing gradient");
     if (!s->dA || !s->dD || !s->ddelta_bias) return bad("missing gradient");
   }
+  if (s->ldb < 0 || s->ldb_group < 0 || s->ldc < 0 || s->ldc_group < 0) return bad("negative pitch");
+  const uintptr_t es = s->type == FB_F32 ? 4 : 2;
+  if (!aligned(es, s->u, s->delta, s->B, s->C, s->z) ||
+      !(backward ? aligned(es, s->dy, s->du, s->ddelta, s->dz, s->dB, s->dC) : aligned(es, s->y)))
+    return bad("rows that are not aligned to their elements");
+  if (!aligned(4, s->A, s->skip, s->delta_bias, s->init, s->keep) ||
+      !(backward ? aligned(4, s->dfinal, s->dA, s->dD, s->ddelta_bias, s->dinit) : aligned(4, s->final)) ||
+      !aligned(s->starts_type == FB_I64 ? 8 : 4, s->starts))
+    return bad("parameters, states or starts that are not aligned to their elements");
   a = ScanArgs{};
   a.D = s->D, a.N = s->N, a.G = s->G, a.per = s->D / s->G, a.softplus = s->softplus;
   a.u = s->u, a.ldu = s->ldu, a.delta = s->delta, a.ldd = s->ld_delta;

@@ -449,6 +449,11 @@ int fill(const fb_short_conv *s, ConvArgs &a, bool backward) {
     return bad("missing or overlapping operand of the backward pass");
   if (backward && (!s->dw || !s->dbias)) return bad("missing gradient");
   if (backward && s->dinit && !s->init) return bad("dinit without init");
+  const uintptr_t es = s->type == FB_F32 ? 4 : 2;
+  if (!aligned(es, s->x, s->init) || !(backward ? aligned(es, s->dy, s->dfinal, s->dx, s->dinit) : aligned(es, s->y, s->final)))
+    return bad("rows that are not aligned to their elements");
+  if (!aligned(4, s->w, s->bias) || (backward && !aligned(4, s->dw, s->dbias)) || !aligned(s->starts_type == FB_I64 ? 8 : 4, s->starts))
+    return bad("parameters or starts that are not aligned to their elements");
   a = ConvArgs{};
   a.D = s->D, a.K = s->K, a.silu = s->act == FB_ACT_SILU;
   a.x = s->x, a.ldx = (int)s->ldx, a.dy = s->dy, a.lddy = (int)s->lddy, a.init = s->K > 1 ? s->init : nullptr;
@@ -469,11 +474,9 @@ int vector_of(const fb_short_conv *s, bool backward) {
   const void *p[2] = {backward ? s->dy : s->y, backward ? s->dx : nullptr};
   const int64_t ld[2] = {backward ? s->lddy : s->ldy, backward ? s->lddx : 0};
   uint64_t bits = (uint64_t)(uintptr_t)s->x / es | (uint64_t)s->D;
-  if ((uintptr_t)s->x % es) return 0;
   if (s->rows > 1) bits |= (uint64_t)s->ldx;
   for (int i = 0; i < 2; ++i)
     if (p[i]) {
-      if ((uintptr_t)p[i] % es) return 0;
       bits |= (uint64_t)(uintptr_t)p[i] / es;
       if (s->rows > 1) bits |= (uint64_t)ld[i];
     }
@@ -530,7 +533,6 @@ template <typename T> int run_conv(const fb_short_conv *s, ConvArgs &a, bool bac
   const int64_t state = (int64_t)a.st.seqs * (a.K - 1) * a.D;
   if (s->rows) {
     const int V = vector_of(s, backward);
-    if (!V) return fb::set_error(FB_ERR_ARG, "short_conv: rows that are not aligned to their elements");
     plan(a, V, backward);
     if (backward && a.blocks > 1) {
       const size_t need = (size_t)a.blocks * (a.K + 1) * a.D * sizeof(float);
