@@ -114,6 +114,7 @@ extern "C" int fb_dropout(int type, const void *x, int64_t ldx, const void *res,
   if (!(p >= 0.f && p < 1.f)) return bad("p must be in [0, 1)");
   if (rows < 0 || D < 1) return bad("bad sizes");
   if (rows >= (int64_t)1 << 32) return fb::set_error(FB_ERR_UNSUPPORTED, "dropout: rows are counted in 32 bits");
+  if (D > (1 << 20)) return fb::set_error(FB_ERR_UNSUPPORTED, "dropout: too many columns");
   if (rows && (!x || !y)) return bad("missing operand");
   if (rows > 1 && (ldx < D || ldy < D || (res && ldr < D))) return bad("leading dimension below the width");
   if (!rows) return FB_OK;

@@ -77,3 +77,12 @@ def test_entries_refuse_operands_off_their_elements():
         for name, values in dict(x=odd, res=odd, y=odd, offset_dev=(p + 4,)).items():
             for v in values:
                 assert lib.fb_dropout(*dict(drop, **{name: v}).values()) == 1, (name, v)
+
+
+def test_dropout_refuses_widths_its_columns_do_not_count():
+    """FB_ERR_UNSUPPORTED above the width the other event-history entries take, too."""
+    from fast_b200.capi import lib
+    buf = ctypes.create_string_buffer(80)
+    p = (ctypes.addressof(buf) + 15) & ~15
+    for width in ((1 << 20) + 1, (1 << 31) - 1):
+        assert lib.fb_dropout(1, p, width, None, 0, p, width, 2, width, 0.5, 1, 0, None, None) == 3
