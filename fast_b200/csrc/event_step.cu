@@ -443,7 +443,7 @@ extern "C" int fb_short_conv_step(int type, int act, const void *x, int64_t ldx,
   if (n < 0 || states < 0 || D < 1 || K < 1) return bad("bad sizes");
   if (K > kMaxTaps) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv_step: at most 8 taps");
   if (n > kMaxRows || D > (1 << 20)) return fb::set_error(FB_ERR_UNSUPPORTED, "short_conv_step: too many rows or columns");
-  if (!w || (n && (!x || !y || (K > 1 && !state)))) return bad("missing operand");
+  if (!w || (n && (!x || !y || (K > 1 && states && !state)))) return bad("missing operand");
   if (n > 1 && (ldx < D || ldy < D)) return bad("leading dimension below the width");
   if (!n) return FB_OK;
   ConvStep a{D, K, act == FB_ACT_SILU, x, ldx, y, ldy, state, w, bias, {}};
@@ -466,7 +466,7 @@ extern "C" int fb_selective_scan_step(const fb_selective_scan_event *s, void *ws
   if (s->n < 0 || s->states < 0 || s->D < 1 || s->N < 1 || s->G < 1 || s->D % s->G) return bad("bad sizes");
   if (s->N > kMaxStates) return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan_step: at most 64 states");
   if (s->n > kMaxRows || s->D > (1 << 20)) return fb::set_error(FB_ERR_UNSUPPORTED, "selective_scan_step: too many rows or columns");
-  if (!s->A || (s->n && (!s->u || !s->delta || !s->B || !s->C || !s->state || !s->y))) return bad("missing operand");
+  if (!s->A || (s->n && (!s->u || !s->delta || !s->B || !s->C || (s->states && !s->state) || !s->y))) return bad("missing operand");
   if (s->n > 1 && (s->ldu < s->D || s->ld_delta < s->D || s->ldy < s->D || (s->z && s->ldz < s->D)))
     return bad("leading dimension below the width");
   if (s->ldb < 0 || s->ldb_group < 0 || s->ldc < 0 || s->ldc_group < 0) return bad("negative pitch");

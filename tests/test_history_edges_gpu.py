@@ -155,3 +155,14 @@ def test_seeds_beyond_64_bits_are_refused(cuda):
     for seed in (-1, 1 << 64, 1.0, True):
         with pytest.raises(ValueError, match="seed"):
             enc(x, starts, seed=seed)
+
+
+# ---- tables ------------------------------------------------------------------------------------------
+def test_tables_of_no_node(cuda):
+    """Every index is beyond the table, or held out."""
+    from fast_b200 import ops
+    x, index = torch.randn(3, 8, device=cuda), torch.tensor([0, -1, 5], device=cuda)
+    w, A, B = torch.randn(8, 4, device=cuda), -torch.rand(8, 16, device=cuda), torch.randn(3, 16, device=cuda)
+    for y in (ops.short_conv_step(x, torch.zeros(0, 3, 8, device=cuda), w, index=index),
+              ops.selective_scan_step(x, x, A, B, B, torch.zeros(0, 8, 16, device=cuda), index=index)):
+        assert bool(torch.isnan(y[[0, 2]]).all()) and not bool(y[1].any())
