@@ -4,6 +4,9 @@
 //   conv: window = [state[i] | x],  y = act(bias + sum_k w[k] window[k]),  state[i] = the window without its oldest
 //   scan: dt = softplus(delta + bias),  h = exp(dt A) state[i] + dt u B,  y = (<C, h> + D u) silu(z),  state[i] = h
 //
+// with the operations of the packed histories (history.cuh), so that events decay as
+// histories do.
+//
 // Bound by the state's bytes, read once and written once.  Row r works on state
 // index[r].  Events of one node take their turns in the rows' order, as a
 // chronological batch means them: the first row of a node walks its rows with the
@@ -286,7 +289,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(256, NP <= 16 ? 
 #pragma unroll
   for (int q = 0; q < P; ++q)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) A2[q][k] = mul2(A2[q][k], both(kLog2e));
+    for (int k = 0; k < 4; ++k) A2[q][k] = pack(scaled(unpack(A2[q][k]).x), scaled(unpack(A2[q][k]).y));
   const float bias = own && a.bias ? a.bias[d] : 0.f, skip = own && a.Ds ? a.Ds[d] : 0.f;
 
   struct Event {
@@ -345,7 +348,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(256, NP <= 16 ? 
         F2 v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          h[q][k] = fma2(ex2_2(mul2(dt2, A2[q][k])), h[q][k], mul2(dtu2, B[k]));
+          h[q][k] = fma2(decays(dt2, A2[q][k]), h[q][k], mul2(dtu2, B[k]));
           v = k == 0 ? mul2(C[k], h[q][k]) : fma2(C[k], h[q][k], v);
         }
         const float2 f = unpack(v);

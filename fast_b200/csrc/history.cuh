@@ -177,6 +177,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// A log2(e), kept finite so that a row of no sequence (dt 0) leaves the state as it
+// is even where A is -infinity.
+__device__ __forceinline__ float scaled(float A) { return max_nan(A * kLog2e, -3e38f); }
+// exp(dt A) of a pair, A2 = scaled(A).  The exponential unit's results are low by
+// 0.6 to 2.4e-8 on average where decays are slow (measured for exponents of -1e-4
+// to -1), which a state that remembers a thousand steps adds up a thousand
+// times; the summand centres them.
+__device__ __forceinline__ F2 decays(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, both(2e-8f))); }
+
 // log(1 + e^x) of a pair and (SLOPE) its derivative, relative accuracy a few
 // 2^-24 also where they are small.  With e = e^-|x|: log(1 + e) = 2 artanh(s), s =
 // e / (2 + e) <= 1/3, and artanh(s) / s is a polynomial in s^2 (interpolated at

@@ -67,16 +67,6 @@ constexpr int kHalf = kTile / 2;          // rows whose states the backward hold
 constexpr int kFwdCtas = 3, kBwdCtas = 3;
 constexpr int kKept = 1;                  // pairs of a thread whose decays it holds, too
 
-// exp(dt A) of a pair, A2 = A log2(e).  The exponential unit's results are low by
-// 0.6 to 2.4e-8 on average where decays are slow (measured for exponents of -1e-4
-// to -1), which a state that remembers a thousand steps adds up a thousand
-// times; the summand centres them.
-// A log2(e), kept finite so that a row of no sequence (dt 0) leaves the state as it
-// is even where A is -infinity.
-__device__ __forceinline__ float scaled(float A) { return max_nan(A * kLog2e, -3e38f); }
-
-__device__ __forceinline__ F2 decays(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, both(2e-8f))); }
-
 struct ScanArgs {
   int D, N, G, per, tiles, softplus;      // per: channels of a group; tiles: a group's tiles of channels
   const void *u, *delta, *B, *C, *z, *dy;

@@ -1,9 +1,10 @@
 """GPU: event histories at the edges of what the calls document -- dropout and
 training mode, what is kept, gates and decays of extreme values, tables of no
 node, and the kernels that only large calls reach."""
+import history_math as hm
 import pytest
 import torch
-from test_history_gpu import BF, F32
+from test_history_gpu import BF, F32, close, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -155,6 +156,59 @@ def test_seeds_beyond_64_bits_are_refused(cuda):
     for seed in (-1, 1 << 64, 1.0, True):
         with pytest.raises(ValueError, match="seed"):
             enc(x, starts, seed=seed)
+
+
+# ---- decays ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("softplus", [False, True])
+@pytest.mark.parametrize("n", [5, 16, 64])
+def test_events_decay_as_histories_do(cuda, softplus, n):
+    """Rows of one chunk, at once and event by event: the same operations in the same order, so the same states."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(n)
+    rows, d = 13, 40
+    u, B, C = rows_of(g, rows, d, F32), rows_of(g, rows, n, F32), rows_of(g, rows, n, F32)
+    delta = (torch.rand(rows, d, generator=g) * 0.01).cuda() - (4.0 if softplus else 0.0)
+    A = -(torch.rand(d, n, generator=g) * 4 + 0.5).cuda()
+    final = ops.selective_scan_fwd(u, delta, A, B, C, softplus=softplus, final=True)[2][0]
+    state = torch.zeros(3, d, n, device="cuda")
+    for r in range(rows):
+        ops.selective_scan_step(u[r:r + 1], delta[r:r + 1], A, B[r:r + 1], C[r:r + 1], state, softplus=softplus,
+                                index=torch.tensor([1], device="cuda"))
+    assert torch.equal(state[1], final) and not bool(state[[0, 2]].any())
+
+
+def test_events_with_decays_of_minus_infinity(cuda):
+    """A state with A = -infinity keeps nothing of the event before, and a step of 0 leaves every state as it is, as in the scan."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(2)
+    d, n = 24, 16
+    u, B, C = rows_of(g, 6, d, F32), rows_of(g, 6, n, F32), rows_of(g, 6, n, F32)
+    delta = rows_of(g, 6, d, F32, 0.5)
+    delta[3] = -200.0                                               # softplus gives 0
+    A = -(torch.rand(d, n, generator=g) + 0.5).cuda()
+    A[:, 3] = float("-inf")
+    y, _, final = ops.selective_scan_fwd(u, delta, A, B, C, final=True)
+    state = torch.zeros(1, d, n, device="cuda")
+    for r in range(6):
+        close(ops.selective_scan_step(u[r:r + 1], delta[r:r + 1], A, B[r:r + 1], C[r:r + 1], state), y[r:r + 1], "row %d" % r)
+    assert torch.equal(state, final)
+
+
+def test_slow_decays_over_a_long_stream(cuda):
+    """4,000 events of one node.  As for a history (a decay's mean error at most 1.3e-8 of itself, a thousand steps remembered):
+    2^-16 of the state."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(8)
+    rows, d, n = 4000, 32, 16
+    u, B, C = rows_of(g, rows, d, F32).abs(), rows_of(g, rows, n, F32).abs(), rows_of(g, rows, n, F32)
+    delta = (torch.rand(rows, d, generator=g) * 0.001 + 0.0005).cuda()
+    A = -torch.arange(1, n + 1, dtype=torch.float32, device="cuda").repeat(d, 1)
+    state = torch.zeros(2, d, n, device="cuda")
+    y = ops.selective_scan_step(u, delta, A, B, C, state, index=torch.ones(rows, dtype=torch.int64, device="cuda"), softplus=False)
+    wide = [t.double() for t in (u, delta, A, B.unsqueeze(1), C.unsqueeze(1))]
+    wy, wf = hm.selective_scan(*wide, None, None, None, None, None, False)
+    for got, ref in ((y, wy), (state[1], wf[0])):
+        assert float((got.double() - ref).norm() / ref.norm()) <= 2.0 ** -16
 
 
 # ---- tables ------------------------------------------------------------------------------------------
