@@ -218,4 +218,10 @@ __device__ __forceinline__ float softplus(float x) {
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
 __device__ __forceinline__ F2 sigmoid2(F2 x) { return rcp_2(add2(ex2_2(mul2(x, both(-kLog2e))), both(1.f))); }
 
+// The derivative of x sigmoid(x), sg = sigmoid(x): sg (1 + x (1 - sg)).  Written out,
+// sg + x sg - x sg^2, it would cancel for large x.
+__device__ __forceinline__ F2 silu_slope2(F2 x, F2 sg) {
+  return mul2(sg, fma2(x, fma2(sg, both(-1.f), both(1.f)), both(1.f)));
+}
+
 }  // namespace fbq

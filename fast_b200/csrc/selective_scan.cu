@@ -642,9 +642,9 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
         const F2 u = pack(to_f(xu[i]), to_f(xu[i + 1])), dy = pack(to_f(xy[i]), to_f(xy[i + 1]));
         F2 gv = dy, dg = both(0.f);
         if (a.z) {
-          const F2 z = pack(to_f(xz[i]), to_f(xz[i + 1])), sg = sigmoid2(z), zs = mul2(z, sg);
-          gv = mul2(dy, zs);
-          dg = mul2(dy, fma2(mul2(zs, sg), both(-1.f), add2(sg, zs)));     // sg (1 + z (1 - sg))
+          const F2 z = pack(to_f(xz[i]), to_f(xz[i + 1])), sg = sigmoid2(z);
+          gv = mul2(dy, mul2(z, sg));
+          dg = mul2(dy, silu_slope2(z, sg));
         }
         const F2 v = pack(only<X>(dt[i], i, ra, rb), only<X>(dt[i + 1], i + 1, ra, rb));
         const float2 fu = unpack(u), fg = unpack(gv), fd = unpack(dg), fv = unpack(v), fp = unpack(mul2(v, u));

@@ -274,10 +274,7 @@ template <typename T, int V, int KT, bool BWD> __global__ void __launch_bounds__
           if (PLAIN || (live >> i & 1u)) {
             if (a.silu)
 #pragma unroll
-              for (int p = 0; p < P; ++p) {
-                const F2 zs = mul2(z[p], sg[p]);
-                g[p] = mul2(g[p], fma2(mul2(zs, sg[p]), both(-1.f), add2(sg[p], zs)));
-              }
+              for (int p = 0; p < P; ++p) g[p] = mul2(g[p], silu_slope2(z[p], sg[p]));
             if (PLAIN || t < len)
 #pragma unroll
               for (int p = 0; p < P; ++p) {

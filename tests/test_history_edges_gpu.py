@@ -158,6 +158,58 @@ def test_seeds_beyond_64_bits_are_refused(cuda):
             enc(x, starts, seed=seed)
 
 
+# ---- gates -------------------------------------------------------------------------------------------
+def _gate_calls(z, dtype=F32):
+    """silu(z) and silu'(z) as every kernel that gates computes them: (name, values, slopes or None) with the factor 1."""
+    from fast_b200 import ops
+    n = z.numel()
+    rows, one = z.to(dtype).reshape(-1, 8), torch.ones(n // 8, 8, device="cuda", dtype=dtype)
+    w, r = torch.ones(8, 1, device="cuda"), n // 8
+    yield "convolution", ops.short_conv_fwd(rows, w), ops.short_conv_bwd(one, rows, w)[0]
+    # the gradient of the inputs in front of a sequence: w = (1, 0), one row a sequence
+    two = torch.tensor([[1.0, 0.0]], device="cuda").repeat(8, 1)
+    starts = torch.arange(r + 1, device="cuda")
+    yield ("convolution, states in", ops.short_conv_fwd(one, two, starts=starts, init=rows.unsqueeze(1)),
+           ops.short_conv_bwd(one, one, two, starts=starts, init=rows.unsqueeze(1))[3].squeeze(1))
+    yield "convolution, event", ops.short_conv_step(rows, torch.zeros(r, 0, 8, device="cuda", dtype=dtype), w), None
+    A, B, D = -torch.ones(8, 4, device="cuda"), torch.zeros(r, 4, device="cuda", dtype=dtype), torch.ones(8, device="cuda")
+    y, carry, _ = ops.selective_scan_fwd(one, one, A, B, B, D, rows)
+    yield "scan", y, ops.selective_scan_bwd(one, one, one, A, B, B, carry, D, rows)[6]
+    yield "scan, event", ops.selective_scan_step(one, one, A, B, B, torch.zeros(r, 8, 4, device="cuda"), D, rows), None
+
+
+def test_gates_of_large_positive_values(cuda):
+    """silu'(z) is 1 + z (1 - sigmoid(z)) times sigmoid(z), which tends to 1.  The sigmoid is off by 2^-23 (its reciprocal)
+    + 2^-24; 1 - sigmoid is that much off where it does not vanish (z <= 17): 17 * 1.5 * 2^-23 < 2^-18 of the result."""
+    z = torch.cat([torch.linspace(1, 40, 400), torch.logspace(1.6, 30, 400)]).cuda()
+    w = z.double().requires_grad_(True)
+    y = torch.nn.functional.silu(w)
+    slope, = torch.autograd.grad(y.sum(), w)
+    w, y = w.detach(), y.detach()
+    for name, got, dgot in _gate_calls(z):
+        assert float(((got.reshape(-1).double() - y) / y).abs().amax()) <= 2.0 ** -18, name
+        if dgot is not None:
+            assert float(((dgot.reshape(-1).double() - slope) / slope).abs().amax()) <= 2.0 ** -18, name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_gates_of_the_largest_values(cuda, dtype):
+    """Neither end of the type overflows on the way: silu tends to 0 and z, its slope to 0 and 1; NaN stays."""
+    top = torch.finfo(dtype).max
+    z = torch.tensor([-top, -1e30, -200.0, -90.0, 0.0, 90.0, 1e30, top], device=cuda)
+    for name, got, dgot in _gate_calls(z, dtype):
+        want = torch.nn.functional.silu(z.to(dtype).double())
+        assert float((got.reshape(-1).double() - want).abs()[:5].amax()) <= 1e-30, name
+        assert torch.equal(got.reshape(-1)[5:], z.to(dtype)[5:]), name
+        if dgot is not None:
+            assert float(dgot.reshape(-1)[:4].abs().amax()) <= 1e-30, name
+            assert torch.equal(dgot.reshape(-1)[4:].float(), torch.tensor([0.5, 1, 1, 1], device=cuda)), name
+    for name, got, dgot in _gate_calls(torch.full((8,), float("nan"), device=cuda), dtype):
+        assert bool(torch.isnan(got).all()) and (dgot is None or bool(torch.isnan(dgot).all())), name
+    for name, got, _ in _gate_calls(torch.full((8,), float("inf"), device=cuda), dtype):
+        assert bool((got == float("inf")).all()), name
+
+
 # ---- decays ------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("softplus", [False, True])
 @pytest.mark.parametrize("n", [5, 16, 64])
