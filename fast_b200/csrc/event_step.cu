@@ -199,7 +199,7 @@ template <typename T, int V, int KT> __global__ void __launch_bounds__(256) k_co
 #pragma unroll
           for (int k = 0; k < KT; ++k)
             if (k >= skip) p = fmaf(w[k][v], to_f(win[i][k].e[v]), p);
-          y.e[v] = from_f<T>(a.silu ? p * sigmoid(p) : p);
+          y.e[v] = from_f<T>(a.silu ? p * sigmoid<T>(p) : p);
         }
         if (has) put(r, y);
 #pragma unroll
@@ -357,7 +357,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(256, NP <= 16 ? 
       float v = fmaf(skip, u, spread_sum<NL>(y));
       if (a.z) {
         const float z = to_f(e.z);
-        v *= z * sigmoid(z);
+        v *= z * sigmoid<T>(z);
       }
       if (own) static_cast<T *>(a.y)[r * a.ldy + d] = from_f<T>(v);
       if (next < 0) break;

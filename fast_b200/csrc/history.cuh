@@ -170,7 +170,12 @@ __device__ __forceinline__ F2 rcp_2(F2 x) {
   const float2 f = unpack(x);
   return pack(rcp(f.x), rcp(f.y));
 }
-// The larger one, NaN if there is one.
+// The smaller and the larger one, NaN if there is one.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -186,18 +191,23 @@ __device__ __forceinline__ float scaled(float A) { return max_nan(A * kLog2e, -3
 // times; the summand centres them.
 __device__ __forceinline__ F2 decays(F2 dt, F2 A2) { return ex2_2(fma2(dt, A2, both(2e-8f))); }
 
+// What t = -m log2(e), rounded, lacks: m log2(e) + t.
+__device__ __forceinline__ F2 exponent_rest2(F2 m, F2 t) {
+  return fma2(m, both(1.925963033500011e-8f), fma2(m, both(kLog2e), t));
+}
+
 // log(1 + e^x) of a pair and (SLOPE) its derivative, relative accuracy a few
 // 2^-24 also where they are small.  With e = e^-|x|: log(1 + e) = 2 artanh(s), s =
 // e / (2 + e) <= 1/3, and artanh(s) / s is a polynomial in s^2 (interpolated at
 // Chebyshev nodes of [0, 1/9], off by 4e-9).  The product |x| log2(e) is carried
-// to two words: its rounding alone would cost e 2^-24 |x|.
+// to two words: its rounding alone would cost e 2^-24 |x|.  Below x = -87.3 e is
+// flushed to 0.
 template <bool SLOPE> __device__ __forceinline__ F2 softplus2(F2 x, F2 &slope) {
   const float2 f = unpack(x);
   const F2 m = pack(fminf(fabsf(f.x), 100.f), fminf(fabsf(f.y), 100.f));
   const F2 t = mul2(m, both(-kLog2e));
-  const F2 lost = fma2(m, both(1.925963033500011e-8f), fma2(m, both(kLog2e), t));      // the rest of m log2(e)
   F2 e = ex2_2(t);
-  e = fma2(mul2(lost, both(-0.6931472f)), e, e);
+  e = fma2(mul2(exponent_rest2(m, t), both(-0.6931472f)), e, e);
   const F2 s = mul2(e, rcp_2(add2(e, both(2.f)))), w = mul2(s, s);
   F2 p = fma2(w, both(0.14078889787197113f), both(0.13982579112052917f));
   p = fma2(w, p, both(0.20012298226356506f));
@@ -214,14 +224,48 @@ __device__ __forceinline__ float softplus(float x) {
   return unpack(softplus2<false>(both(x), none)).x;
 }
 
-// 1 / (1 + e^-x)
-__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
-__device__ __forceinline__ F2 sigmoid2(F2 x) { return rcp_2(add2(ex2_2(mul2(x, both(-kLog2e))), both(1.f))); }
-
-// The derivative of x sigmoid(x), sg = sigmoid(x): sg (1 + x (1 - sg)).  Written out,
-// sg + x sg - x sg^2, it would cancel for large x.
-__device__ __forceinline__ F2 silu_slope2(F2 x, F2 sg) {
-  return mul2(sg, fma2(x, fma2(sg, both(-1.f), both(1.f)), both(1.f)));
+// 1 / (1 + e^-x) of a pair in rows of type T, and what it leaves to 1.  For fp32
+// rows both keep their relative accuracy, a few 2^-24, where they are small: the
+// product x log2(e) is carried to two words, as in softplus2, and the rest is e^-x
+// times the first.  x is held to where no step overflows; below -87.3 the sigmoid
+// is flushed to 0.  For bf16 rows, whose results are rounded to 2^-9, one word and
+// the difference from 1 do (|x| 2^-24 off).
+template <typename T> __device__ __forceinline__ F2 sigmoid2(F2 x, F2 &rest) {
+  if constexpr (sizeof(T) == 4) {
+    const float2 f = unpack(x);
+    const F2 m = pack(min_nan(max_nan(f.x, -88.f), 100.f), min_nan(max_nan(f.y, -88.f), 100.f)), t = mul2(m, both(-kLog2e));
+    F2 e = ex2_2(t);
+    e = fma2(mul2(exponent_rest2(m, t), both(-0.6931472f)), e, e);
+    const F2 sg = rcp_2(add2(e, both(1.f)));
+    rest = mul2(e, sg);
+    return sg;
+  } else {
+    const F2 sg = rcp_2(add2(ex2_2(mul2(x, both(-kLog2e))), both(1.f)));
+    rest = fma2(sg, both(-1.f), both(1.f));
+    return sg;
+  }
 }
+template <typename T> __device__ __forceinline__ float sigmoid(float x, float &rest) {
+  if constexpr (sizeof(T) == 4) {
+    const float m = min_nan(max_nan(x, -88.f), 100.f), t = __fmul_rn(m, -kLog2e);
+    float e = ex2(t);
+    e = fmaf(fmaf(m, 1.925963033500011e-8f, fmaf(m, kLog2e, t)) * -0.6931472f, e, e);
+    const float sg = rcp(1.f + e);
+    rest = e * sg;
+    return sg;
+  } else {
+    const float sg = rcp(1.f + ex2(-kLog2e * x));
+    rest = 1.f - sg;
+    return sg;
+  }
+}
+template <typename T> __device__ __forceinline__ float sigmoid(float x) {
+  float rest;
+  return sigmoid<T>(x, rest);
+}
+
+// The derivative of x sigmoid(x) from the sigmoid and its rest: sg (1 + x (1 - sg)).
+// Written out, sg + x sg - x sg^2, it would cancel for large x.
+__device__ __forceinline__ F2 silu_slope2(F2 x, F2 sg, F2 rest) { return mul2(sg, fma2(x, rest, both(1.f))); }
 
 }  // namespace fbq

@@ -381,7 +381,7 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
         float v = fmaf(skip[i % X::W], to_f(ku[i]), lanes_sum<L::NL>(&sm.y[X::row(i)][c & 3][((c >> 2) * L::NL) ^ L::turn((c & 3) * 8)]));
         if (a.z) {
           const float z = to_f(kz[i]);
-          v *= z * sigmoid(z);
+          v *= z * sigmoid<T>(z);
         }
         if (X::row(i) < end && X::col(i) < left) py[i / X::W * X::RS * a.ldy + 32 * (i % X::W)] = from_f<T>(only<X>(v, i, ra, rb));
       }
@@ -509,7 +509,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, kFwdCt
       float gv = to_f(xy[i]);
       if (a.z) {
         const float z = to_f(xz[i]);
-        gv *= z * sigmoid(z);
+        gv *= z * sigmoid<T>(z);
       }
       sm.dt[X::row(i)][X::col(i)] = only<X>(dt[i], i, 0, rb);
       sm.gv[X::row(i)][X::col(i)] = only<X>(gv, i, 0, rb);
@@ -642,9 +642,11 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
         const F2 u = pack(to_f(xu[i]), to_f(xu[i + 1])), dy = pack(to_f(xy[i]), to_f(xy[i + 1]));
         F2 gv = dy, dg = both(0.f);
         if (a.z) {
-          const F2 z = pack(to_f(xz[i]), to_f(xz[i + 1])), sg = sigmoid2(z);
+          const F2 z = pack(to_f(xz[i]), to_f(xz[i + 1]));
+          F2 rest;
+          const F2 sg = sigmoid2<T>(z, rest);
           gv = mul2(dy, mul2(z, sg));
-          dg = mul2(dy, silu_slope2(z, sg));
+          dg = mul2(dy, silu_slope2(z, sg, rest));
         }
         const F2 v = pack(only<X>(dt[i], i, ra, rb), only<X>(dt[i + 1], i + 1, ra, rb));
         const float2 fu = unpack(u), fg = unpack(gv), fd = unpack(dg), fv = unpack(v), fp = unpack(mul2(v, u));

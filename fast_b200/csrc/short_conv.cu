@@ -251,14 +251,14 @@ template <typename T, int V, int KT, bool BWD> __global__ void __launch_bounds__
 #pragma unroll
           for (int k = 0; k < H; ++k) older(s, k - skip, win[i + k]);
         }
-        F2 z[P], sg[P];
+        F2 z[P], sg[P], rest[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
           z[p] = bias[p];
 #pragma unroll
           for (int k = 0; k < KT; ++k)
             if (k >= skip) z[p] = fma2(w[k][p], win[i + k][p], z[p]);
-          if (a.silu) sg[p] = sigmoid2(z[p]);
+          if (a.silu) sg[p] = sigmoid2<T>(z[p], rest[p]);
         }
         if constexpr (!BWD) {
           if (PLAIN || t < len) {
@@ -274,7 +274,7 @@ template <typename T, int V, int KT, bool BWD> __global__ void __launch_bounds__
           if (PLAIN || (live >> i & 1u)) {
             if (a.silu)
 #pragma unroll
-              for (int p = 0; p < P; ++p) g[p] = mul2(g[p], silu_slope2(z[p], sg[p]));
+              for (int p = 0; p < P; ++p) g[p] = mul2(g[p], silu_slope2(z[p], sg[p], rest[p]));
             if (PLAIN || t < len)
 #pragma unroll
               for (int p = 0; p < P; ++p) {
@@ -416,8 +416,9 @@ template <typename T> __global__ void __launch_bounds__(256) k_conv_dinit(ConvAr
       float p = a.bias ? a.bias[d] : 0.f, dp = to_f(static_cast<const T *>(a.dy)[(b + i) * (int64_t)a.lddy + d]);
       for (int k = 0; k < K; ++k) p = fmaf(w[k], x[i + k], p);
       if (a.silu) {
-        const float sg = sigmoid(p);
-        dp *= sg * fmaf(p, 1.f - sg, 1.f);
+        float rest;
+        const float sg = sigmoid<T>(p, rest);
+        dp *= sg * fmaf(p, rest, 1.f);
       }
       for (int m = i; m < K - 1; ++m) g[m] = fmaf(w[m - i], dp, g[m]);
     }

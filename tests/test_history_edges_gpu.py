@@ -192,6 +192,21 @@ def test_gates_of_large_positive_values(cuda):
             assert float(((dgot.reshape(-1).double() - slope) / slope).abs().amax()) <= 2.0 ** -18, name
 
 
+def test_gates_keep_their_relative_accuracy(cuda):
+    """fp32.  e^-z: 2^-22 of the exponential unit and 2^-23 of its correction; 1 + e^-z, the reciprocal (2^-23) and the product
+    with z: 2^-22 more.  The slope, away from its zero at -1.28, has the sigmoid's error and 1 + z (1 - sigmoid)'s: twice that."""
+    z = torch.cat([torch.linspace(-86, -20, 400), torch.linspace(-20, 20, 800)]).cuda()
+    w = z.double().requires_grad_(True)
+    y = torch.nn.functional.silu(w)
+    slope, = torch.autograd.grad(y.sum(), w)
+    w, y = w.detach(), y.detach()
+    far = (z < -2.5) | (z > 0)                                      # 1 + z (1 - sigmoid) does not cancel there
+    for name, got, dgot in _gate_calls(z):
+        assert float(((got.reshape(-1).double() - y) / y).abs().amax()) <= 2.5 * 2.0 ** -22, name
+        if dgot is not None:
+            assert float(((dgot.reshape(-1).double() - slope) / slope).abs()[far].amax()) <= 5 * 2.0 ** -22, name
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_gates_of_the_largest_values(cuda, dtype):
     """Neither end of the type overflows on the way: silu tends to 0 and z, its slope to 0 and 1; NaN stays."""
