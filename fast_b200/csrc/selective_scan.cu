@@ -416,6 +416,8 @@ template <typename T, int NP, bool LOCAL> __global__ void __launch_bounds__(kThr
 
 // Joins the chunks: edge[c], what chunk c alone leaves, becomes what arrives
 // behind it (REV: in front of chunk c + 1, from the rows behind).
+// A chunk's factor is applied as its root, twice: where states grow (A > 0) it can
+// lie beyond fp32 and what it makes of a small state inside; of a 0 it makes 0.
 // Bound by the latency of its loads, so 32 chunks' are in flight (188 chunks of
 // width 200: 20 us with 8).
 template <bool REV> __global__ void __launch_bounds__(128) k_scan_join(ScanArgs a) {
@@ -438,7 +440,8 @@ template <bool REV> __global__ void __launch_bounds__(128) k_scan_join(ScanArgs 
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       if (at + k < n) {
-        x = cut[k] ? local[k] : fmaf(ex2(A2 * sum[k]), x, local[k]);
+        const float root = ex2(A2 * sum[k] * 0.5f);
+        x = cut[k] || x == 0.f ? local[k] : fmaf(root, root * x, local[k]);
         a.edge[(REV ? n - 1 - (at + k) : at + k) * size + i] = x;
       }
   }

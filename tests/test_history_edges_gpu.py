@@ -2,6 +2,7 @@
 training mode, what is kept, gates and decays of extreme values, tables of no
 node, and the kernels that only large calls reach."""
 import history_math as hm
+import numpy as np
 import pytest
 import torch
 from test_history_gpu import BF, F32, close, rows_of
@@ -276,6 +277,42 @@ def test_slow_decays_over_a_long_stream(cuda):
     wy, wf = hm.selective_scan(*wide, None, None, None, None, None, False)
     for got, ref in ((y, wy), (state[1], wf[0])):
         assert float((got.double() - ref).norm() / ref.norm()) <= 2.0 ** -16
+
+
+def test_growth_over_chunks(cuda):
+    """States that grow (A > 0): a chunk's factor beyond fp32 carries a 0 as 0 and a small state as the product it is, in both
+    directions."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(4)
+    rows, d, n = 64, 8, 8
+    u, B, C, dy = (rows_of(g, rows, c, F32) for c in (d, n, n, d))
+    u[:40], dy[24:] = 0, 0                                          # nothing until row 40; nothing wanted from row 24 on
+    delta = torch.ones(rows, d, device="cuda")
+    for rate in (1.0, 4.0, 7.0, 20.0):
+        A = torch.full((d, n), rate, device="cuda") * torch.linspace(0.25, 1, n, device="cuda")
+        v = u.clone()
+        v[40:] = 0
+        v[60:] = u[60:]
+        y, carry, final = ops.selective_scan_fwd(v, delta, A, B, C, softplus=False, final=True)
+        wide = [t.double().requires_grad_(True) for t in (v, delta, A, B, C)]
+        wy, wf = hm.selective_scan(*wide[:3], wide[3].unsqueeze(1), wide[4].unsqueeze(1), None, None, None, None, None, False)
+        assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(final).all()), rate
+        assert float((final.double() - wf).norm() / wf.norm()) <= 2.0 ** -14, rate
+        e = dy.clone()
+        e[4:] = 0
+        du = ops.selective_scan_bwd(e, v, delta, A, B, C, carry, softplus=False)[0]
+        want, = torch.autograd.grad(wy, wide[0], e.double())
+        assert bool(torch.isfinite(du).all()), rate
+        assert float((du.double() - want).norm() / want.norm()) <= 2.0 ** -14, rate
+    # a state of 2^-100 that a chunk of 16 rows lifts by e^112 = 2^161.6
+    u = torch.zeros(rows, d, device="cuda")
+    u[15], A = 2.0 ** -100, torch.full((d, n), 7.0, device="cuda")
+    delta[32:] = 0
+    B = torch.ones(rows, n, device="cuda")
+    final = ops.selective_scan_fwd(u, delta, A, B, B, softplus=False, final=True)[2]
+    want = 2.0 ** -100 * float(np.exp(112.0))
+    # 161.6 = 16 * 7 * log2 e, off by 2^-17.3 where the steps' exponents or the chunk's are rounded, each way twice at most
+    assert float((final.double() / want - 1).abs().amax()) <= 2.0 ** -15
 
 
 # ---- tables ------------------------------------------------------------------------------------------
