@@ -5,7 +5,7 @@ import history_math as hm
 import numpy as np
 import pytest
 import torch
-from test_history_gpu import BF, F32, close, rows_of
+from test_history_gpu import BF, F32, close, poison, rows_of, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -324,3 +324,70 @@ def test_tables_of_no_node(cuda):
     for y in (ops.short_conv_step(x, torch.zeros(0, 3, 8, device=cuda), w, index=index),
               ops.selective_scan_step(x, x, A, B, B, torch.zeros(0, 8, 16, device=cuda), index=index)):
         assert bool(torch.isnan(y[[0, 2]]).all()) and not bool(y[1].any())
+
+
+# ---- kernels of large calls --------------------------------------------------------------------------
+def conv_at_once(x, w, bias, starts, init, act):
+    """(y, final) of hm.short_conv for many rows, by gathering."""
+    rows, (d, k) = x.shape[0], w.shape
+    seqs, t = starts.shape[0] - 1, torch.arange(rows, device=x.device)
+    s = torch.searchsorted(starts, t, right=True) - 1
+    some = (s >= 0) & (s < seqs)
+    s = s.clamp(0, seqs - 1)
+    pos = t - starts[s]
+
+    def before(at, seq):                                            # input number `at` of a sequence, from -(k - 1) on
+        v = x[(starts[seq] + at).clamp(0, rows - 1)]
+        past = x.new_zeros(1, d) if init is None or k == 1 else init[seq, (at + k - 1).clamp(0, k - 2)]
+        return torch.where((at >= 0).unsqueeze(1), v, past)
+    p = sum(w[:, i] * before(pos - (k - 1 - i), s) for i in range(k))
+    p = p if bias is None else p + bias
+    y = torch.where(some.unsqueeze(1), p * torch.sigmoid(p) if act == "silu" else p, x.new_zeros(1))
+    every = torch.arange(seqs, device=x.device)
+    n = starts[1:] - starts[:-1]
+    final = [before(n - (k - 1) + m, every) for m in range(k - 1)]
+    return y, torch.stack(final, 1) if final else x.new_zeros(seqs, 0, d)
+
+
+def test_convolution_at_once_is_the_restatement(cuda):
+    g = torch.Generator().manual_seed(0)
+    starts = starts_of([5, 0, 1, 9, 0, 2], 3)
+    for k in (1, 2, 4, 7):
+        x, w, b = (torch.randn(*s, generator=g, dtype=torch.float64).cuda() for s in ((25, 6), (6, k), (6,)))
+        i = torch.randn(6, k - 1, 6, generator=g, dtype=torch.float64).cuda()
+        for a, c in zip(conv_at_once(x, w, b, starts, i, "silu"), hm.short_conv(x, w, b, starts, i, "silu")):
+            assert torch.allclose(a, c, rtol=1e-13, atol=1e-13)
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 5, 8])
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("whole", [True, False])
+def test_conv_of_four_columns_a_thread(cuda, k, dtype, whole):
+    """From 9,472 rows of width 512 on a thread has four columns (rows / 32 * (width / 128) >= 148 * 8)."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(k)
+    lengths, d = [4000, 0, 1, 2, 3, 0, 2500, 64, 17] + [5] * 300 + [0, 1400, 7], 512
+    starts = starts_of(lengths, 3)
+    n = int(starts[-1]) + 70
+    x, dy = rows_of(g, n, d, dtype, 1, 8), rows_of(g, n, d, dtype, 1, 4)
+    w = (torch.randn(d, k, generator=g) * k ** -0.5).cuda()
+    b, act = (torch.randn(d, generator=g).cuda() * 0.2, "silu") if whole else (None, None)
+    i, df = ((torch.randn(len(lengths), k - 1, d, generator=g).to(dtype).cuda() if whole else None) for _ in range(2))
+    poison(n, starts, x, dy)
+    wide = [None if t is None else t.double().nan_to_num(0, 0, 0).requires_grad_(True) for t in (x, w, b, i)]
+    y, final = conv_at_once(*wide[:3], starts, wide[3], act)
+    got_y, got_final = ops.short_conv_fwd(x, w, b, starts, i, act, final=True)
+    close(got_y, y, "y")
+    assert torch.equal(got_final.double(), final.double())
+    names = [m for m, t in zip(("dx", "dw", "dbias", "dinit"), wide) if t is not None]
+    have = [t for t in wide if t is not None]
+    outs, grads = [y], [dy.double().nan_to_num(0, 0, 0)]
+    if whole:
+        outs, grads = outs + [final + 0 * wide[0].sum()], grads + [df.double()]
+    want = dict(zip(names, torch.autograd.grad(outs, have, grads, allow_unused=True)))
+    got = dict(zip(("dx", "dw", "dbias", "dinit"), ops.short_conv_bwd(dy, x, w, b, starts, i, act, dfinal=df)))
+    for m, v in got.items():
+        if m in want:
+            close(v, torch.zeros_like(v) if want[m] is None else want[m], m)
+        else:
+            assert v is None
