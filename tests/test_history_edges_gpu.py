@@ -5,7 +5,7 @@ import history_math as hm
 import numpy as np
 import pytest
 import torch
-from test_history_gpu import BF, F32, close, poison, rows_of, starts_of
+from test_history_gpu import BF, F32, close, poison, rows_of, scan_case, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -391,3 +391,21 @@ def test_conv_of_four_columns_a_thread(cuda, k, dtype, whole):
             close(v, torch.zeros_like(v) if want[m] is None else want[m], m)
         else:
             assert v is None
+
+
+# With so wide rows a chunk has as many rows as make two waves of warps forward (three of CTAs backward), if those are 48
+# (64) or more, else those that make one less.
+LONG = [400, 0, 1, 7, 64, 0, 0, 300, 3, 500]
+
+
+@pytest.mark.parametrize("n,d,dtype,lengths", [
+    (5, 8192, BF, LONG), (16, 4096, F32, LONG), (16, 4096, BF, LONG), (13, 4096, BF, LONG), (32, 2048, BF, LONG),   # 56 and 72 rows
+    (16, 2048, F32, [700, 0, 1, 1100, 9, 111]),                                                                     # 80 and 80
+    (64, 2048, F32, [310, 2, 0, 300, 9])])                                                                          # 56 and 80
+def test_scan_of_long_chunks(cuda, n, d, dtype, lengths):
+    """Chunks of many tiles of eight rows, sequences that begin inside them, several waves of chunks."""
+    scan_case(lengths, d, n, dtype, init=True, front=30, tail=45)
+
+
+def test_scan_of_long_chunks_in_groups(cuda):
+    scan_case(LONG, 4096, 16, BF, groups=4, gate=False, skip=False, pad=3, front=5, tail=70)
