@@ -409,3 +409,47 @@ def test_scan_of_long_chunks(cuda, n, d, dtype, lengths):
 
 def test_scan_of_long_chunks_in_groups(cuda):
     scan_case(LONG, 4096, 16, BF, groups=4, gate=False, skip=False, pad=3, front=5, tail=70)
+
+
+def _event_case(g, n, nodes):
+    """Indices of n events: nodes that come once or several times, anywhere; the last rows hold one that is held out and one
+    beyond the table."""
+    index = torch.randint(0, nodes, (n,), generator=g)
+    index[-2], index[-5 if n > 5 else 0] = -1, nodes
+    index[-1] = index[0]
+    return index
+
+
+@pytest.mark.parametrize("n", [64, 65, 4095, 4096, 4097, 8193, 9000])
+@pytest.mark.parametrize("often", [1, 3, 700])
+def test_events_that_meet_their_nodes_again(cuda, n, often):
+    """Up to 64 rows the warps compare indices themselves; beyond, a kernel does, 4,096 rows at a time."""
+    from fast_b200 import ops
+    g = torch.Generator().manual_seed(n + often)
+    nodes, d, k, s = max(2, n // often), 4, 3, 4
+    index = _event_case(g, n, nodes)
+    x, delta = torch.randn(n, d, generator=g), torch.randn(n, d, generator=g) * 0.5
+    B, C = torch.randn(n, 1, s, generator=g), torch.randn(n, 1, s, generator=g)
+    w, A = torch.randn(d, k, generator=g), -(0.5 + torch.rand(d, s, generator=g) * s)
+    conv, scan = torch.randn(nodes, k - 1, d, generator=g), torch.randn(nodes, d, s, generator=g)
+    at = index.cuda()
+    c, h = conv.cuda(), scan.cuda()
+    yc = ops.short_conv_step(x.cuda(), c, w.cuda(), None, at)
+    ys = ops.selective_scan_step(x.cuda(), delta.cuda(), A.cuda(), B.cuda(), C.cuda(), h, index=at)
+    dt = np.logaddexp(delta.double().numpy(), 0.0)
+    x, B, C, w, A, conv, scan = (t.double().numpy() for t in (x, B, C, w, A, conv, scan))
+    wc, wsc = np.zeros((n, d)), np.zeros((n, d))
+    for r, i in enumerate(index.tolist()):
+        if 0 <= i < nodes:
+            win = np.concatenate([conv[i], x[r:r + 1]])
+            p = (win * w.T).sum(0)
+            wc[r], conv[i] = p / (1 + np.exp(-p)), win[1:]
+            scan[i] = np.exp(dt[r][:, None] * A) * scan[i] + (dt[r] * x[r])[:, None] * B[r]
+            wsc[r] = (C[r] * scan[i]).sum(1)
+    beyond, held = index >= nodes, index < 0
+    for got, want in ((yc, wc), (ys, wsc)):
+        assert bool(torch.isnan(got[beyond.cuda()]).all()) and not bool(got[held.cuda()].any())
+        got[beyond.cuda()] = 0
+        close(got, torch.from_numpy(want).cuda(), "y")
+    assert torch.equal(c.double().cpu(), torch.from_numpy(conv))
+    close(h, torch.from_numpy(scan).cuda(), "state")
