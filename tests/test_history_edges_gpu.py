@@ -453,3 +453,36 @@ def test_events_that_meet_their_nodes_again(cuda, n, often):
         close(got, torch.from_numpy(want).cuda(), "y")
     assert torch.equal(c.double().cpu(), torch.from_numpy(conv))
     close(h, torch.from_numpy(scan).cuda(), "state")
+
+
+def philox_at_once(rows, cols, seed, offset):
+    """hm.philox for many rows."""
+    m = np.uint64(0xFFFFFFFF)
+    c = [np.broadcast_to(np.arange((cols + 3) // 4, dtype=np.uint64), (rows, (cols + 3) // 4)),
+         np.broadcast_to(np.arange(rows, dtype=np.uint64)[:, None], (rows, (cols + 3) // 4)),
+         np.uint64(offset & 0xFFFFFFFF), np.uint64(offset >> 32)]
+    for r in range(10):
+        k = [np.uint64((seed + r * 0x9E3779B9) & 0xFFFFFFFF), np.uint64(((seed >> 32) + r * 0xBB67AE85) & 0xFFFFFFFF)]
+        p0, p1 = np.uint64(0xD2511F53) * c[0], np.uint64(0xCD9E8D57) * c[2]
+        c = [(p1 >> np.uint64(32)) ^ c[1] ^ k[0], p1 & m, (p0 >> np.uint64(32)) ^ c[3] ^ k[1], p0 & m]
+        c = [np.broadcast_to(v, (rows, (cols + 3) // 4)) for v in c]
+    return torch.from_numpy(np.stack(c, 2).reshape(rows, -1)[:, :cols].astype(np.int64))
+
+
+@pytest.mark.parametrize("d,pad", [(1028, 0), (1026, 0), (2056, 8), (2056, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_dropout_down_the_rows(cuda, d, pad, dtype):
+    """Wide rows, more than CTAs down the grid: a thread draws for several rows."""
+    from fast_b200 import ops
+    assert torch.equal(philox_at_once(5, 11, 0x123456789ABCDEF0, (7 << 32) + 5), hm.philox(5, 11, 0x123456789ABCDEF0, (7 << 32) + 5))
+    g = torch.Generator().manual_seed(1)
+    n, p, seed, offset = 2900, 0.3, 0xFFFFFFFF00000001, (3 << 40) + 9
+    x, res = (rows_of(g, n, d, dtype, pad=pad) for _ in range(2))
+    kept = (philox_at_once(n, d, seed, offset).cuda() >> 8).double() * 2.0 ** -24 >= float(torch.tensor(p))
+    scale = kept.double() / (1 - p)
+    half = torch.finfo(dtype).eps / 2
+    for got, want in ((ops.dropout_fwd(x, p, seed, offset), x.double() * scale),
+                      (ops.dropout_fwd(x, p, seed, offset, res), res.double() + x.double() * scale)):
+        # the scale, its product and the sum are rounded in fp32, the result once more
+        room = half * want.abs() + 3 * 2.0 ** -24 * (x.double().abs().amax() / (1 - p) + res.double().abs())
+        assert bool(((got.double() - want).abs() <= room).all())
