@@ -649,7 +649,7 @@ template <typename T, int NP> __global__ void __launch_bounds__(kThreads, NP > 3
           F2 rest;
           const F2 sg = sigmoid2<T>(z, rest);
           gv = mul2(dy, mul2(z, sg));
-          dg = mul2(dy, silu_slope2(z, sg, rest));
+          dg = mul2(dy, silu_slope2<T>(z, sg, rest));
         }
         const F2 v = pack(only<X>(dt[i], i, ra, rb), only<X>(dt[i + 1], i + 1, ra, rb));
         const float2 fu = unpack(u), fg = unpack(gv), fd = unpack(dg), fv = unpack(v), fp = unpack(mul2(v, u));

@@ -274,7 +274,7 @@ template <typename T, int V, int KT, bool BWD> __global__ void __launch_bounds__
           if (PLAIN || (live >> i & 1u)) {
             if (a.silu)
 #pragma unroll
-              for (int p = 0; p < P; ++p) g[p] = mul2(g[p], silu_slope2(z[p], sg[p], rest[p]));
+              for (int p = 0; p < P; ++p) g[p] = mul2(g[p], silu_slope2<T>(z[p], sg[p], rest[p]));
             if (PLAIN || t < len)
 #pragma unroll
               for (int p = 0; p < P; ++p) {

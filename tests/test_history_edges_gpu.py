@@ -193,6 +193,22 @@ def test_gates_of_large_positive_values(cuda):
             assert float(((dgot.reshape(-1).double() - slope) / slope).abs().amax()) <= 2.0 ** -18, name
 
 
+def test_gates_of_bf16_rows(cuda):
+    """One rounding to bf16 (8 bits of significand: half a step is up to 2^-8 of the value); in front of it at most |z| 2^-23
+    (|z| <= 64 where it counts) = 2^-17."""
+    z = torch.cat([torch.linspace(-60, 60, 800), torch.logspace(1.7, 38, 400)]).cuda().to(BF)
+    w = z.double().requires_grad_(True)
+    y = torch.nn.functional.silu(w)
+    slope, = torch.autograd.grad(y.sum(), w)
+    w, y = w.detach(), y.detach()
+    near = (z < -2.5) | (z > 0)                                     # away from the slope's zero at -1.28
+    for name, got, dgot in _gate_calls(z, BF):
+        assert bool(((got.reshape(-1).double() - y).abs() <= (2.0 ** -8 + 2.0 ** -16) * y.abs()).all()), name
+        if dgot is not None:
+            off = (dgot.reshape(-1).double() - slope).abs()
+            assert bool((off <= (2.0 ** -8 + 2.0 ** -16) * slope.abs())[near].all()), name
+
+
 def test_gates_keep_their_relative_accuracy(cuda):
     """fp32.  e^-z: 2^-22 of the exponential unit and 2^-23 of its correction; 1 + e^-z, the reciprocal (2^-23) and the product
     with z: 2^-22 more.  The slope, away from its zero at -1.28, has the sigmoid's error and 1 + z (1 - sigmoid)'s: twice that."""
