@@ -13,7 +13,8 @@
 // state in registers, the others do nothing.  Which row is first and which comes
 // next is looked up by comparing indices: by the warps themselves in calls of few
 // rows, in calls of many by k_links before (a lane a row, the other indices from
-// shared memory, four a branch: 4.5 us for 4,000 rows, 7.4 with one a branch).
+// shared memory, four a branch: 4.5 us for 4,000 rows, 7.4 with one a branch; it
+// grows with the square of the rows, about 35 us for 16,384 and 425 for 65,536).
 // Warps stay on their columns and take rows one after the other, so that weights
 // stay in registers; the convolution loads two nodes' windows at once.  (States
 // copied two nodes ahead by asynchronous copies, or two or four nodes' loaded at

@@ -44,9 +44,10 @@
 // - Sums over rows and channels end in per-CTA partials that one more launch
 //   adds in a fixed order: results repeat bit for bit.
 //
-// 16,384 x 1,024, 64 ragged sequences, bf16, 16 states: forward 88 (last states) +
-// 15 + 160 us, backward 92 (first gradients) + 8 + 444 + 17; at 148 SMs and 1.9 GHz
-// the exponentials alone take 60 us a pass.
+// 16,384 x 1,024, 64 ragged sequences, bf16, 16 states: both passes 832 us; under a
+// profiler, with cold caches, forward 89 (last states) + 14 + 170, backward 95 (first
+// gradients) + 12 + 464 + 18; at 148 SMs and 1.9 GHz the exponentials alone take 60 us
+// a pass.
 //
 // Everything between the loads and the stores is fp32.
 #include <algorithm>

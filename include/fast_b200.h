@@ -674,6 +674,8 @@ int fb_softmax_xent_bwd(const fb_softmax_xent *args, void *ws, size_t ws_bytes, 
 /* its steps for single events against per-node state tables.  No counterpart */
 /* in the reference, whose node memory is a GRU over the last mail            */
 /* (memorys.py:270-304) or attention over a mailbox (memorys.py:342-386).     */
+/* Rows are at most 1,048,576 wide; operands that are not aligned to their     */
+/* elements are refused.                                                       */
 /* ------------------------------------------------------------------------- */
 /* Integer types of device arrays. */
 enum { FB_I32 = 0, FB_I64 = 1 };
@@ -723,7 +725,9 @@ int fb_short_conv_bwd(const fb_short_conv *args, void *ws, size_t ws_bytes, cuda
  * NULL), fp32 [ceil(rows / 8), D, N], receives the states in front of every 8th
  * row, which the backward takes.  Backward from dy (and dfinal, may be NULL):
  * du, ddelta, dz [rows, D], dB, dC [rows, G, N] in `type`; dA, dD, ddelta_bias,
- * dinit (may be NULL) in fp32; contiguous.  All arithmetic is fp32.
+ * dinit (may be NULL) in fp32; contiguous.  All arithmetic is fp32.  A state
+ * with A = -infinity keeps nothing of the row before, but where dt is 0, which
+ * leaves every state as it is.
  * Deterministic.  ws: fb_selective_scan_ws_bytes(args, backward) bytes,
  * 16-byte aligned. */
 typedef struct fb_selective_scan {
