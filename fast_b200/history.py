@@ -100,7 +100,7 @@ class DropoutFunction(torch.autograd.Function):
     def forward(ctx, x, res, p, seed, offset, offset_dev=None):
         ctx.how = p, seed, offset
         ctx.has_res = res is not None
-        ctx.save_for_backward(offset_dev)
+        ctx.save_for_backward(offset_dev if p else None)                # p = 0 draws nothing again
         return ops.dropout_fwd(_rows(x), p, seed, offset, None if res is None else _rows(res), offset_dev)
 
     @staticmethod

@@ -128,6 +128,15 @@ def test_a_counter_that_moves_before_the_backward_is_refused(cuda):
         y.sum().backward()
 
 
+def test_a_counter_may_move_where_nothing_drops_out(cuda):
+    from fast_b200.history import DropoutFunction
+    x, count = torch.ones(9, 8, device=cuda, requires_grad=True), torch.zeros(1, dtype=torch.int64, device=cuda)
+    y = DropoutFunction.apply(x, None, 0.0, 1, 0, count)
+    count += 1
+    grad, = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(grad, torch.ones_like(grad))
+
+
 def test_no_dropout_hands_the_gradient_on(cuda):
     from fast_b200 import ops
     from fast_b200.history import DropoutFunction
