@@ -14,14 +14,15 @@
 // backward: loads where they are used 646 + 118 us, two batches of registers
 // 208 + 88, copies 121 + 61; the bytes take 61 + 41).  What holds them now is neither
 // memory nor issue slots (53% and 57% used): 14 and 19 warps an SM wait for the
-// results of their own instructions.  Above four taps one form of eight serves all,
-// which spills at four columns (16,384 x 2,048 bf16: five taps 258 + 79 us, eight
-// 272 + 92).  The arithmetic runs on pairs of columns.  Where sequences begin comes as one bit a row, which a CTA
-// gathers for its rows before it starts; batches inside one sequence run without
-// a branch, others replace the window by assignment where a sequence begins.
-// p is computed again in the backward from x, which is there anyway.  dw and
-// dbias are summed over a thread's run in registers, over a CTA in shared
-// memory, and over the CTAs by a second launch in a fixed order.
+// results of their own instructions.  Above four taps one form of eight serves
+// all, which spills at four columns (16,384 x 2,048 bf16: five taps 258 + 79 us,
+// eight 272 + 92).  The arithmetic runs on pairs of columns.  Where sequences
+// begin comes as one bit a row, which a CTA gathers for its rows before it starts;
+// batches inside one sequence run without a branch, others replace the window by
+// assignment where a sequence begins. p is computed again in the backward from x,
+// which is there anyway.  dw and dbias are summed over a thread's run in
+// registers, over a CTA in shared memory, and over the CTAs by a second launch in
+// a fixed order.
 #include <algorithm>
 #include <type_traits>
 #include "head.cuh"
